@@ -334,6 +334,59 @@ int pesq_iir_set_spin_limit(pesq_iir* filter, uint32_t polls);
  * (a bounded wait that ran out; its rows are then wrong). */
 int pesq_iir_check(pesq_iir* filter, void* stream, uint32_t* failed);
 
+/* ---------------------------------------------------------------------------
+ * Operators of the networks trained on the loss.  They keep no object: a call
+ * works on the current device, on `stream`, in the workspace it is given, and
+ * can be captured in a CUDA graph.  Descriptors are only read during the call.
+ * ------------------------------------------------------------------------- */
+
+/* element types of the streams */
+#define PESQ_F32 0
+#define PESQ_BF16 1
+#define PESQ_F16 2
+
+/* A [batch, step, channel] stream: element strides of batch and step (any,
+ * negative or zero too); channels are adjacent. */
+typedef struct pesq_stream {
+  const void* data;
+  int64_t batch_stride;
+  int64_t step_stride;
+} pesq_stream;
+
+/* Gated linear recurrence along the steps of every row and channel,
+ *   r = sigmoid(decay_gate), i = sigmoid(input_gate),
+ *   log a = -rate softplus(decay) r,
+ *   h = a h + sqrt(1 - a^2) i x,  y = h
+ * (csrc/gated_scan.cuh).  The reference has fixed-coefficient recurrences only
+ * (torch_pesq/triton_ops/iir.py). */
+typedef struct pesq_gated_scan_desc {
+  int64_t batch, steps, width;
+  int32_t dtype;      /* PESQ_F32, PESQ_BF16 or PESQ_F16: x, the gates, y and their gradients */
+  int32_t reverse;    /* scan from the last step to the first */
+  float rate;         /* > 0 */
+  uint32_t spin_limit;/* polls of a look-back wait before it gives up; 0: 2^21 (about 0.1 s) */
+  pesq_stream x, input_gate, decay_gate;
+  const float* decay; /* [width] */
+  const float* state; /* [batch, width], the state before the first step; NULL: zeros */
+  const uint8_t* reset;   /* nonzero: the step forgets the state (a = 0); NULL: none */
+  int64_t reset_batch_stride, reset_step_stride;
+  const int64_t* lengths; /* [batch]: steps at or past it keep the state and give 0; NULL: all steps */
+  uint32_t* error;    /* device word, set to nonzero when a wait gave up; never cleared here */
+} pesq_gated_scan_desc;
+
+/* Bytes of workspace of a forward (`backward` 0) or backward call (1), 16-byte aligned. */
+int pesq_gated_scan_workspace(const pesq_gated_scan_desc* desc, int backward, size_t* bytes);
+/* y: [batch, steps, width] dense; last: [batch, width], the state after the
+ * last step.  The workspace of a forward call is what its backward call reads
+ * as `saved` (the states at the tiles' starts). */
+int pesq_gated_scan_forward(const pesq_gated_scan_desc* desc, void* stream, void* y, float* last, void* workspace,
+                            size_t workspace_bytes);
+/* dy.data and dlast may be NULL (zeros); dstate may be NULL (not wanted).
+ * dx, dinput_gate, ddecay_gate: dense; ddecay: [width]. */
+int pesq_gated_scan_backward(const pesq_gated_scan_desc* desc, void* stream, const void* saved, size_t saved_bytes,
+                             pesq_stream dy, const float* dlast, void* dx, void* dinput_gate, void* ddecay_gate,
+                             float* ddecay, float* dstate, void* workspace, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,52 @@
+"""Definitions of the training operators in 64 bits (torch on the CPU, one
+step or row at a time; gradients by autograd), and how far an output may be
+from them."""
+
+import torch
+
+#: unit roundoff of an output's type: one rounding at the end, relative
+ROUND = {t: torch.finfo(t).eps / 2 for t in (torch.float32, torch.bfloat16, torch.float16)}
+
+
+def close(got, want, tol, what=""):
+    """|got - want| is at most one rounding to got's type, with a quarter to
+    spare, plus ``tol`` of the largest value: what the 32-bit arithmetic before
+    that rounding may be off by.  Non-finite values have to agree."""
+
+    assert tuple(got.shape) == tuple(want.shape), f"{what}: {tuple(got.shape)} against {tuple(want.shape)}"
+    g, w = got.detach().cpu().double(), want.detach().cpu().double()
+    finite = torch.isfinite(w)
+    assert torch.equal(finite, torch.isfinite(g)), f"{what}: non-finite values differ"
+    g, w = g[finite], w[finite]
+    if g.numel() == 0:
+        return
+    tiny = 2.0**-24 if got.dtype == torch.float16 else 0.0  # spacing of float16 below its normal range
+    allowed = 1.25 * ROUND[got.dtype] * w.abs() + tol * w.abs().max() + tiny
+    worst = float(((g - w).abs() - allowed).max())
+    assert worst <= 0, f"{what}: over the bound by {worst:.3e}, peak {float(w.abs().max()):.3e}"
+
+
+def gated_scan(x, ig, rg, decay, state=None, reset=None, lengths=None, reverse=False, rate=8.0):
+    """h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(ig) x, step by step."""
+
+    batch, steps, width = x.shape
+    h = torch.zeros(batch, width, dtype=torch.float64) if state is None else state
+    soft = torch.nn.functional.softplus(decay, threshold=1e4)
+    ys = [None] * steps
+    for t in range(steps - 1, -1, -1) if reverse else range(steps):
+        la = -rate * soft * torch.sigmoid(rg[:, t])
+        a, beta = torch.exp(la), torch.sqrt(-torch.expm1(2 * la))
+        if reset is not None:
+            cut = reset[:, t, None]
+            a, beta = torch.where(cut, 0.0, a), torch.where(cut, 1.0, beta)
+            new = a * torch.where(cut, 0.0, h)
+        else:
+            new = a * h
+        new = new + beta * torch.sigmoid(ig[:, t]) * x[:, t]
+        if lengths is not None:
+            live = (t < lengths)[:, None]
+            ys[t] = torch.where(live, new, 0.0)
+            h = torch.where(live, new, h)
+        else:
+            ys[t] = h = new
+    return (torch.stack(ys, dim=1) if steps else x.clone()), h

@@ -6,10 +6,14 @@ through the C ABI of ``libpesq_cuda.so`` (``include/pesq_cuda.h``);
 ``ResampleCuda`` is the reference's ``TritonResample`` (its polyphase sinc
 resampler as a standalone op) and ``IIRCuda`` its ``TritonIIR`` (the causal
 IIR filter as a standalone op) on the same library.
+
+Beside them, the operators of the networks that are trained on the loss:
+``gated_scan`` / ``GatedScanCuda`` (a gated linear recurrence).
 """
 
+from .gated_scan import GatedScanCuda, gated_scan, gated_scan_errors
 from .iir import IIRCuda
 from .loss import PesqLossCuda
 from .resample import ResampleCuda
 
-__all__ = ["PesqLossCuda", "ResampleCuda", "IIRCuda"]
+__all__ = ["PesqLossCuda", "ResampleCuda", "IIRCuda", "GatedScanCuda", "gated_scan", "gated_scan_errors"]

@@ -121,6 +121,40 @@ IIR_RERUN = 2
 IIR_CHAINED = 4
 
 
+#: element types of the training operators' streams
+F32, BF16, F16 = 0, 1, 2
+
+
+class Stream(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("batch_stride", ctypes.c_int64),
+        ("step_stride", ctypes.c_int64),
+    ]
+
+
+class GatedScanDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int64),
+        ("steps", ctypes.c_int64),
+        ("width", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("reverse", ctypes.c_int32),
+        ("rate", ctypes.c_float),
+        ("spin_limit", ctypes.c_uint32),
+        ("x", Stream),
+        ("input_gate", Stream),
+        ("decay_gate", Stream),
+        ("decay", ctypes.c_void_p),
+        ("state", ctypes.c_void_p),
+        ("reset", ctypes.c_void_p),
+        ("reset_batch_stride", ctypes.c_int64),
+        ("reset_step_stride", ctypes.c_int64),
+        ("lengths", ctypes.c_void_p),
+        ("error", ctypes.c_void_p),
+    ]
+
+
 class Shape(ctypes.Structure):
     _fields_ = [("n16", ctypes.c_int64), ("frames", ctypes.c_int32), ("windows", ctypes.c_int32)]
 
@@ -208,6 +242,20 @@ SIGNATURES = {
         ctypes.c_int,
         [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
          ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p],
+    ),
+    "pesq_gated_scan_workspace": (
+        ctypes.c_int, [ctypes.POINTER(GatedScanDesc), ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)],
+    ),
+    "pesq_gated_scan_forward": (
+        ctypes.c_int,
+        [ctypes.POINTER(GatedScanDesc), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+         ctypes.c_size_t],
+    ),
+    "pesq_gated_scan_backward": (
+        ctypes.c_int,
+        [ctypes.POINTER(GatedScanDesc), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, Stream, ctypes.c_void_p,
+         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+         ctypes.c_size_t],
     ),
 }
 
@@ -299,6 +347,27 @@ def _register_fakes() -> None:
     @torch.library.register_fake("pesq_cuda::iir")
     def _iir(filt, signal, flags):
         return signal.new_empty(signal.shape)
+
+    def scan_workspace(x, backward):
+        desc = GatedScanDesc(batch=x.shape[0], steps=x.shape[1], width=x.shape[2], rate=1.0)
+        if x.numel() == 0:
+            return 0
+        nbytes = ctypes.c_size_t()
+        check(library().pesq_gated_scan_workspace(ctypes.byref(desc), backward, ctypes.byref(nbytes)),
+              "pesq_gated_scan_workspace")
+        return nbytes.value
+
+    @torch.library.register_fake("pesq_cuda::gated_scan_forward")
+    def _gated_scan(x, input_gate, decay_gate, decay, state, reset, lengths, reverse, rate, error, spin_limit):
+        return (x.new_empty(x.shape), x.new_empty((x.shape[0], x.shape[2]), dtype=torch.float32),
+                x.new_empty((scan_workspace(x, 0),), dtype=torch.uint8))
+
+    @torch.library.register_fake("pesq_cuda::gated_scan_backward")
+    def _gated_scan_backward(x, input_gate, decay_gate, decay, state, reset, lengths, reverse, rate, error, spin_limit,
+                             saved, dy, dlast):
+        return (x.new_empty(x.shape), x.new_empty(x.shape), x.new_empty(x.shape),
+                x.new_empty((x.shape[2],), dtype=torch.float32),
+                x.new_empty((x.shape[0], x.shape[2]), dtype=torch.float32))
 
 
 def plan_check(handle: int, stream: int = 0) -> int:

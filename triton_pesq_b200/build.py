@@ -28,7 +28,7 @@ OPS = os.path.join(HERE, "_pesq_torch_ops.so")
 
 CUDA_SOURCES = ["front.cu", "align.cu", "back.cu", "spectrum.cu", "chain.cu", "resample.cu", "pesq_abi.cu", "noalloc.cu",
                 "resample_abi.cu", "iir_abi.cu", "iir_ka.cu", "iir_kb.cu", "iir_kc.cu", "iir_kd.cu", "iir_ke.cu",
-                "iir_kf.cu"]
+                "iir_kf.cu", "gated_scan_f32.cu", "gated_scan_bf16.cu", "gated_scan_f16.cu", "gated_scan_abi.cu"]
 NVCC_FLAGS = [
     "-std=c++17",
     "-O3",
@@ -113,7 +113,7 @@ def build_torch_ops(force: bool = False, verbose: bool = False) -> str:
     ctypes.CDLL(LIB, mode=ctypes.RTLD_GLOBAL)
     cpp_extension.load(
         name="pesq_torch_ops",
-        sources=[os.path.join(CSRC, "torch_ops.cpp")],
+        sources=[os.path.join(CSRC, "torch_ops.cpp"), os.path.join(CSRC, "torch_train_ops.cpp")],
         extra_cflags=["-O2", "-std=c++17"],
         extra_ldflags=[f"-L{HERE}", "-lpesq_cuda", "-Wl,-rpath,\\$$ORIGIN"],
         build_directory=bdir,

@@ -1,0 +1,297 @@
+// torch custom ops of the training operators over the C ABI of
+// libpesq_cuda.so, with their autograd nodes.
+//
+// Every operator is three ops: the one a caller uses (composite: it records an
+// autograd node when a gradient is wanted), and the forward and backward it is
+// made of, which allocate with torch's caching allocator, take the current
+// stream and call the C ABI.  Shapes, types and devices are checked in the
+// forward; the backward gets what the forward has checked.
+#include <algorithm>
+#include <limits>
+
+#include <ATen/ATen.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/library.h>
+
+#include "../../include/pesq_cuda.h"
+
+namespace {
+
+using OptTensor = std::optional<at::Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::Variable;
+using torch::autograd::variable_list;
+
+void check_status(int status, const char* what) {
+  if (status == PESQ_OK) return;
+  const char* msg = pesq_last_error();
+  if (status == PESQ_ERR_INVALID_ARGUMENT) TORCH_CHECK_VALUE(false, what, ": ", msg);
+  TORCH_CHECK(false, what, " failed (status ", status, "): ", msg);
+}
+
+int dtype_code(const at::Tensor& t, const char* op, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kFloat:
+      return PESQ_F32;
+    case at::kBFloat16:
+      return PESQ_BF16;
+    case at::kHalf:
+      return PESQ_F16;
+    default:
+      TORCH_CHECK(false, "The CUDA ", op, " supports float32, bfloat16 and float16, `", name, "` is ", t.scalar_type(),
+                  ".");
+  }
+}
+
+void check_cuda(const at::Tensor& t, const at::Tensor& first, const char* op, const char* name) {
+  TORCH_CHECK(t.is_cuda(), "The CUDA ", op, " needs `", name, "` to live on a GPU.");
+  TORCH_CHECK(t.device() == first.device(), "The CUDA ", op, " needs all tensors on one device, `", name, "` is on ",
+              t.device(), ", not ", first.device(), ".");
+}
+
+void check_shape(const at::Tensor& t, at::IntArrayRef want, const char* op, const char* name) {
+  TORCH_CHECK_VALUE(t.sizes() == want, "The CUDA ", op, " needs `", name, "` of shape ", want, ", got ", t.sizes(), ".");
+}
+
+void check_float(const at::Tensor& t, const char* op, const char* name) {
+  TORCH_CHECK(t.scalar_type() == at::kFloat, "The CUDA ", op, " needs `", name, "` in float32, it is ", t.scalar_type(),
+              ".");
+}
+
+// channels adjacent
+at::Tensor rows(const at::Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+
+pesq_stream stream_of(const at::Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1)}; }
+
+const float* floats(const OptTensor& t) { return t.has_value() && t->defined() ? t->data_ptr<float>() : nullptr; }
+
+OptTensor optional_of(const Variable& v) { return v.defined() ? OptTensor(v) : std::nullopt; }
+
+void no_second_derivative(const char* op) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), "The CUDA ", op, " has no second derivative (create_graph=True).");
+}
+
+bool wants_grad(const at::Tensor& t) { return t.requires_grad(); }
+bool wants_grad(const OptTensor& t) { return t.has_value() && t->defined() && t->requires_grad(); }
+
+// ------------------------------------------------------------------ gated scan
+
+constexpr const char* kScan = "gated scan";
+
+struct ScanCall {
+  at::Tensor x, ig, rg, decay, state, reset, lengths;
+  pesq_gated_scan_desc d{};
+
+  ScanCall(const at::Tensor& x_, const at::Tensor& ig_, const at::Tensor& rg_, const at::Tensor& decay_,
+           const OptTensor& state_, const OptTensor& reset_, const OptTensor& lengths_, bool reverse, double rate,
+           const at::Tensor& error) {
+    check_cuda(x_, x_, kScan, "x");
+    d.dtype = dtype_code(x_, kScan, "x");
+    TORCH_CHECK(x_.dim() == 3, "The CUDA gated scan needs `x` [batch, step, channel], got ", x_.sizes(), ".");
+    check_cuda(ig_, x_, kScan, "input_gate");
+    check_cuda(rg_, x_, kScan, "decay_gate");
+    check_cuda(decay_, x_, kScan, "decay");
+    check_shape(ig_, x_.sizes(), kScan, "input_gate");
+    check_shape(rg_, x_.sizes(), kScan, "decay_gate");
+    check_shape(decay_, {x_.size(2)}, kScan, "decay");
+    check_float(decay_, kScan, "decay");
+    TORCH_CHECK(ig_.scalar_type() == x_.scalar_type() && rg_.scalar_type() == x_.scalar_type(),
+                "The CUDA gated scan needs `x` and the gates in one type, got ", x_.scalar_type(), ", ",
+                ig_.scalar_type(), " and ", rg_.scalar_type(), ".");
+    TORCH_CHECK_VALUE(rate > 0.0 && rate <= 1e6, "The CUDA gated scan needs a positive `rate`, got ", rate, ".");
+    TORCH_CHECK(error.is_cuda() && error.device() == x_.device() && error.scalar_type() == at::kInt &&
+                    error.numel() >= 1,
+                "The CUDA gated scan needs its error word on the inputs' device.");
+    x = rows(x_);
+    ig = rows(ig_);
+    rg = rows(rg_);
+    decay = decay_.contiguous();
+    d.batch = x.size(0);
+    d.steps = x.size(1);
+    d.width = x.size(2);
+    if (state_.has_value() && state_->defined()) {
+      check_cuda(*state_, x_, kScan, "state");
+      check_float(*state_, kScan, "state");
+      check_shape(*state_, {d.batch, d.width}, kScan, "state");
+      state = state_->contiguous();
+      d.state = state.data_ptr<float>();
+    }
+    if (reset_.has_value() && reset_->defined()) {
+      check_cuda(*reset_, x_, kScan, "reset");
+      check_shape(*reset_, {d.batch, d.steps}, kScan, "reset");
+      TORCH_CHECK(reset_->scalar_type() == at::kBool, "The CUDA gated scan needs `reset` in bool, it is ",
+                  reset_->scalar_type(), ".");
+      reset = *reset_;
+      d.reset = static_cast<const uint8_t*>(reset.data_ptr());
+      d.reset_batch_stride = reset.stride(0);
+      d.reset_step_stride = reset.stride(1);
+    }
+    if (lengths_.has_value() && lengths_->defined()) {
+      check_cuda(*lengths_, x_, kScan, "lengths");
+      check_shape(*lengths_, {d.batch}, kScan, "lengths");
+      TORCH_CHECK(lengths_->scalar_type() == at::kLong || lengths_->scalar_type() == at::kInt,
+                  "The CUDA gated scan needs `lengths` in int64 or int32, it is ", lengths_->scalar_type(), ".");
+      lengths = lengths_->to(at::kLong).contiguous();
+      d.lengths = lengths.data_ptr<int64_t>();
+    }
+    d.reverse = reverse;
+    d.rate = static_cast<float>(rate);
+    d.x = stream_of(x);
+    d.input_gate = stream_of(ig);
+    d.decay_gate = stream_of(rg);
+    d.decay = decay.data_ptr<float>();
+    d.error = reinterpret_cast<uint32_t*>(error.data_ptr<int>());
+  }
+
+  bool empty() const { return d.batch == 0 || d.steps == 0 || d.width == 0; }
+};
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_scan_forward(const at::Tensor& x, const at::Tensor& ig,
+                                                                  const at::Tensor& rg, const at::Tensor& decay,
+                                                                  const OptTensor& state, const OptTensor& reset,
+                                                                  const OptTensor& lengths, bool reverse, double rate,
+                                                                  const at::Tensor& error, int64_t spin_limit) {
+  ScanCall c(x, ig, rg, decay, state, reset, lengths, reverse, rate, error);
+  c.d.spin_limit = static_cast<uint32_t>(spin_limit);
+  c10::cuda::CUDAGuard guard(x.device());
+  const auto f32 = x.options().dtype(at::kFloat);
+  at::Tensor y = at::empty(x.sizes(), x.options());
+  at::Tensor last = at::empty({c.d.batch, c.d.width}, f32);
+  if (c.empty()) {
+    if (c.d.state) {
+      last.copy_(c.state);
+    } else {
+      last.zero_();
+    }
+    return {y, last, at::empty({0}, f32.dtype(at::kByte))};
+  }
+  size_t bytes = 0;
+  check_status(pesq_gated_scan_workspace(&c.d, 0, &bytes), "pesq_gated_scan_workspace");
+  at::Tensor ws = at::empty({static_cast<int64_t>(bytes)}, f32.dtype(at::kByte));
+  check_status(pesq_gated_scan_forward(&c.d, at::cuda::getCurrentCUDAStream(), y.data_ptr(), last.data_ptr<float>(),
+                                       ws.data_ptr(), bytes),
+               "pesq_gated_scan_forward");
+  return {y, last, ws};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> gated_scan_backward(
+    const at::Tensor& x, const at::Tensor& ig, const at::Tensor& rg, const at::Tensor& decay, const OptTensor& state,
+    const OptTensor& reset, const OptTensor& lengths, bool reverse, double rate, const at::Tensor& error,
+    int64_t spin_limit, const at::Tensor& saved, const OptTensor& dy_, const OptTensor& dlast_) {
+  ScanCall c(x, ig, rg, decay, state, reset, lengths, reverse, rate, error);
+  c.d.spin_limit = static_cast<uint32_t>(spin_limit);
+  c10::cuda::CUDAGuard guard(x.device());
+  const auto f32 = x.options().dtype(at::kFloat);
+  at::Tensor dx = at::empty(x.sizes(), x.options()), dig = at::empty(x.sizes(), x.options()),
+             drg = at::empty(x.sizes(), x.options());
+  at::Tensor ddecay = at::empty({c.d.width}, f32), dstate = at::empty({c.d.batch, c.d.width}, f32);
+  at::Tensor dlast;
+  if (dlast_.has_value() && dlast_->defined()) dlast = dlast_->contiguous();
+  if (c.empty()) {
+    ddecay.zero_();
+    if (dlast.defined()) {
+      dstate.copy_(dlast);
+    } else {
+      dstate.zero_();
+    }
+    return {dx, dig, drg, ddecay, dstate};
+  }
+  at::Tensor dy;
+  pesq_stream dys{nullptr, 0, 0};
+  if (dy_.has_value() && dy_->defined()) {
+    dy = rows(dy_->to(x.scalar_type()));
+    dys = stream_of(dy);
+  }
+  size_t bytes = 0;
+  check_status(pesq_gated_scan_workspace(&c.d, 1, &bytes), "pesq_gated_scan_workspace");
+  at::Tensor ws = at::empty({static_cast<int64_t>(bytes)}, f32.dtype(at::kByte));
+  check_status(pesq_gated_scan_backward(&c.d, at::cuda::getCurrentCUDAStream(), saved.data_ptr(), saved.numel(), dys,
+                                        dlast.defined() ? dlast.data_ptr<float>() : nullptr, dx.data_ptr(),
+                                        dig.data_ptr(), drg.data_ptr(), ddecay.data_ptr<float>(),
+                                        dstate.data_ptr<float>(), ws.data_ptr(), bytes),
+               "pesq_gated_scan_backward");
+  return {dx, dig, drg, ddecay, dstate};
+}
+
+const auto& scan_forward_op() {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("pesq_cuda::gated_scan_forward", "")
+                       .typed<decltype(gated_scan_forward)>();
+  return op;
+}
+const auto& scan_backward_op() {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("pesq_cuda::gated_scan_backward", "")
+                       .typed<decltype(gated_scan_backward)>();
+  return op;
+}
+
+struct GatedScan : public torch::autograd::Function<GatedScan> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& ig, const at::Tensor& rg,
+                               const at::Tensor& decay, const OptTensor& state, const OptTensor& reset,
+                               const OptTensor& lengths, bool reverse, double rate, const at::Tensor& error,
+                               int64_t spin_limit) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [y, last, ws] = scan_forward_op().call(x, ig, rg, decay, state, reset, lengths, reverse, rate, error, spin_limit);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, ig, rg, decay, state.value_or(at::Tensor()), reset.value_or(at::Tensor()),
+                            lengths.value_or(at::Tensor()), ws, error});
+    ctx->saved_data["reverse"] = reverse;
+    ctx->saved_data["rate"] = rate;
+    ctx->saved_data["spin"] = spin_limit;
+    return {y, last};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    no_second_derivative(kScan);
+    const auto s = ctx->get_saved_variables();
+    variable_list out(11);
+    if (!g[0].defined() && !g[1].defined()) return out;
+    auto [dx, dig, drg, ddecay, dstate] = scan_backward_op().call(
+        s[0], s[1], s[2], s[3], optional_of(s[4]), optional_of(s[5]), optional_of(s[6]),
+        ctx->saved_data["reverse"].toBool(), ctx->saved_data["rate"].toDouble(), s[8], ctx->saved_data["spin"].toInt(),
+        s[7], optional_of(g[0]), optional_of(g[1]));
+    out[0] = dx;
+    out[1] = dig;
+    out[2] = drg;
+    out[3] = ddecay;
+    if (s[4].defined()) out[4] = dstate;
+    return out;
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> gated_scan(const at::Tensor& x, const at::Tensor& ig, const at::Tensor& rg,
+                                              const at::Tensor& decay, const OptTensor& state, const OptTensor& reset,
+                                              const OptTensor& lengths, bool reverse, double rate,
+                                              const at::Tensor& error, int64_t spin_limit) {
+  check_cuda(x, x, kScan, "x");
+  if (at::GradMode::is_enabled() &&
+      (wants_grad(x) || wants_grad(ig) || wants_grad(rg) || wants_grad(decay) || wants_grad(state))) {
+    auto out = GatedScan::apply(x, ig, rg, decay, state, reset, lengths, reverse, rate, error, spin_limit);
+    return {out[0], out[1]};
+  }
+  auto [y, last, ws] = scan_forward_op().call(x, ig, rg, decay, state, reset, lengths, reverse, rate, error, spin_limit);
+  return {y, last};
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(pesq_cuda, m) {
+  const char* scan_in =
+      "(Tensor x, Tensor input_gate, Tensor decay_gate, Tensor decay, Tensor? state, Tensor? reset, Tensor? lengths, "
+      "bool reverse, float rate, Tensor error, int spin_limit";
+  m.def((std::string("gated_scan") + scan_in + ") -> (Tensor, Tensor)").c_str());
+  m.def((std::string("gated_scan_forward") + scan_in + ") -> (Tensor, Tensor, Tensor)").c_str());
+  m.def((std::string("gated_scan_backward") + scan_in +
+         ", Tensor saved, Tensor? dy, Tensor? dlast) -> (Tensor, Tensor, Tensor, Tensor, Tensor)")
+            .c_str());
+}
+
+TORCH_LIBRARY_IMPL(pesq_cuda, CompositeImplicitAutograd, m) { m.impl("gated_scan", &gated_scan); }
+
+TORCH_LIBRARY_IMPL(pesq_cuda, CUDA, m) {
+  m.impl("gated_scan_forward", &gated_scan_forward);
+  m.impl("gated_scan_backward", &gated_scan_backward);
+}
