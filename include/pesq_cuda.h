@@ -364,26 +364,26 @@ typedef struct pesq_gated_scan_desc {
   int32_t dtype;      /* PESQ_F32, PESQ_BF16 or PESQ_F16: x, the gates, y and their gradients */
   int32_t reverse;    /* scan from the last step to the first */
   float rate;         /* > 0 */
-  uint32_t spin_limit;/* polls of a look-back wait before it gives up; 0: 2^21 (about 0.1 s) */
+  int32_t reserved0;
   pesq_stream x, input_gate, decay_gate;
   const float* decay; /* [width] */
   const float* state; /* [batch, width], the state before the first step; NULL: zeros */
   const uint8_t* reset;   /* nonzero: the step forgets the state (a = 0); NULL: none */
   int64_t reset_batch_stride, reset_step_stride;
   const int64_t* lengths; /* [batch]: steps at or past it keep the state and give 0; NULL: all steps */
-  uint32_t* error;    /* device word, set to nonzero when a wait gave up; never cleared here */
 } pesq_gated_scan_desc;
 
-/* Bytes of workspace of a forward (`backward` 0) or backward call (1), 16-byte aligned. */
-int pesq_gated_scan_workspace(const pesq_gated_scan_desc* desc, int backward, size_t* bytes);
+/* Bytes (16-byte aligned buffers) of a forward's workspace, of the states it
+ * keeps for a backward call, and of the backward's workspace. */
+int pesq_gated_scan_sizes(const pesq_gated_scan_desc* desc, size_t* forward, size_t* kept, size_t* backward);
 /* y: [batch, steps, width] dense; last: [batch, width], the state after the
- * last step.  The workspace of a forward call is what its backward call reads
- * as `saved` (the states at the tiles' starts). */
-int pesq_gated_scan_forward(const pesq_gated_scan_desc* desc, void* stream, void* y, float* last, void* workspace,
-                            size_t workspace_bytes);
+ * last step; kept: for the backward call, or NULL. */
+int pesq_gated_scan_forward(const pesq_gated_scan_desc* desc, void* stream, void* y, float* last, void* kept,
+                            size_t kept_bytes, void* workspace, size_t workspace_bytes);
 /* dy.data and dlast may be NULL (zeros); dstate may be NULL (not wanted).
- * dx, dinput_gate, ddecay_gate: dense; ddecay: [width]. */
-int pesq_gated_scan_backward(const pesq_gated_scan_desc* desc, void* stream, const void* saved, size_t saved_bytes,
+ * dx, dinput_gate, ddecay_gate: dense; ddecay: [width].  Gradients are at
+ * least as aligned as the inputs. */
+int pesq_gated_scan_backward(const pesq_gated_scan_desc* desc, void* stream, const void* kept, size_t kept_bytes,
                              pesq_stream dy, const float* dlast, void* dx, void* dinput_gate, void* ddecay_gate,
                              float* ddecay, float* dstate, void* workspace, size_t workspace_bytes);
 

@@ -11,9 +11,9 @@ Beside them, the operators of the networks that are trained on the loss:
 ``gated_scan`` / ``GatedScanCuda`` (a gated linear recurrence).
 """
 
-from .gated_scan import GatedScanCuda, gated_scan, gated_scan_errors
+from .gated_scan import GatedScanCuda, gated_scan
 from .iir import IIRCuda
 from .loss import PesqLossCuda
 from .resample import ResampleCuda
 
-__all__ = ["PesqLossCuda", "ResampleCuda", "IIRCuda", "GatedScanCuda", "gated_scan", "gated_scan_errors"]
+__all__ = ["PesqLossCuda", "ResampleCuda", "IIRCuda", "GatedScanCuda", "gated_scan"]

@@ -141,7 +141,7 @@ class GatedScanDesc(ctypes.Structure):
         ("dtype", ctypes.c_int32),
         ("reverse", ctypes.c_int32),
         ("rate", ctypes.c_float),
-        ("spin_limit", ctypes.c_uint32),
+        ("reserved0", ctypes.c_int32),
         ("x", Stream),
         ("input_gate", Stream),
         ("decay_gate", Stream),
@@ -151,7 +151,6 @@ class GatedScanDesc(ctypes.Structure):
         ("reset_batch_stride", ctypes.c_int64),
         ("reset_step_stride", ctypes.c_int64),
         ("lengths", ctypes.c_void_p),
-        ("error", ctypes.c_void_p),
     ]
 
 
@@ -243,13 +242,15 @@ SIGNATURES = {
         [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
          ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p],
     ),
-    "pesq_gated_scan_workspace": (
-        ctypes.c_int, [ctypes.POINTER(GatedScanDesc), ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)],
+    "pesq_gated_scan_sizes": (
+        ctypes.c_int,
+        [ctypes.POINTER(GatedScanDesc), ctypes.POINTER(ctypes.c_size_t), ctypes.POINTER(ctypes.c_size_t),
+         ctypes.POINTER(ctypes.c_size_t)],
     ),
     "pesq_gated_scan_forward": (
         ctypes.c_int,
         [ctypes.POINTER(GatedScanDesc), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
-         ctypes.c_size_t],
+         ctypes.c_size_t, ctypes.c_void_p, ctypes.c_size_t],
     ),
     "pesq_gated_scan_backward": (
         ctypes.c_int,
@@ -348,23 +349,20 @@ def _register_fakes() -> None:
     def _iir(filt, signal, flags):
         return signal.new_empty(signal.shape)
 
-    def scan_workspace(x, backward):
-        desc = GatedScanDesc(batch=x.shape[0], steps=x.shape[1], width=x.shape[2], rate=1.0)
-        if x.numel() == 0:
-            return 0
-        nbytes = ctypes.c_size_t()
-        check(library().pesq_gated_scan_workspace(ctypes.byref(desc), backward, ctypes.byref(nbytes)),
-              "pesq_gated_scan_workspace")
-        return nbytes.value
-
     @torch.library.register_fake("pesq_cuda::gated_scan_forward")
-    def _gated_scan(x, input_gate, decay_gate, decay, state, reset, lengths, reverse, rate, error, spin_limit):
+    def _gated_scan(x, input_gate, decay_gate, decay, state, reset, lengths, reverse, rate, keep):
+        kept = 0
+        if keep and x.numel():
+            desc = GatedScanDesc(batch=x.shape[0], steps=x.shape[1], width=x.shape[2], rate=1.0)
+            sizes = [ctypes.c_size_t() for _ in range(3)]
+            check(library().pesq_gated_scan_sizes(ctypes.byref(desc), *[ctypes.byref(n) for n in sizes]),
+                  "pesq_gated_scan_sizes")
+            kept = sizes[1].value
         return (x.new_empty(x.shape), x.new_empty((x.shape[0], x.shape[2]), dtype=torch.float32),
-                x.new_empty((scan_workspace(x, 0),), dtype=torch.uint8))
+                x.new_empty((kept,), dtype=torch.uint8))
 
     @torch.library.register_fake("pesq_cuda::gated_scan_backward")
-    def _gated_scan_backward(x, input_gate, decay_gate, decay, state, reset, lengths, reverse, rate, error, spin_limit,
-                             saved, dy, dlast):
+    def _gated_scan_backward(x, input_gate, decay_gate, decay, state, reset, lengths, reverse, rate, kept, dy, dlast):
         return (x.new_empty(x.shape), x.new_empty(x.shape), x.new_empty(x.shape),
                 x.new_empty((x.shape[2],), dtype=torch.float32),
                 x.new_empty((x.shape[0], x.shape[2]), dtype=torch.float32))

@@ -8,33 +8,29 @@
 // A `reset` step forgets the state (a = 0, hence beta = 1); a step at or past
 // the row's length keeps it (a = 1, beta = 0) and its output is zero.
 //
-// The recurrence is the composition of maps h -> A h + H, so it splits over
-// time: a tile is kTile = kWarps * L steps by 32 V channels.  Warp w of a CTA
-// owns L consecutive steps of the tile, a lane V neighbouring channels of all
-// of them, so a warp's access is one contiguous piece of a step.  Each
-// thread reads its L x V elements of every stream once, forms (a, b) in
-// registers and folds them to its (A, H); the warps' pairs meet in shared
-// memory; the tiles of a row are chained by a look-back (below); the
-// recursion is then run from the exact start state.  One pass over the data.
+// A warp owns V neighbouring channels per lane and a strip of consecutive steps,
+// and walks the strip in chunks of kChunk steps with the state in registers:
+// everything of a step but one multiply-add is independent of the steps before it,
+// so a chunk's gates are worked out side by side, while the elements of the chunks
+// to come are on their way.  Warps wait for nobody: no barrier, no flag, no
+// atomic, and the order of every operation is fixed.
+//
+// With rows and channels enough to fill the device a strip is the whole row,
+// and the data pass once.  Otherwise rows are cut into strips: the recurrence is
+// the composition of maps h -> A h + H, a first kernel (`maps`) works out every
+// strip's (A, H), and the second starts each strip from the state that the maps
+// before it give.  The strips of a CTA meet in shared memory, so a strip composes
+// the maps of the CTAs before its own and one more.
 //
 // Backward.  With g_t = dL/dh_t: g_t = dy_t + a_{t+1} g_{t+1}, the same kind of
 // scan from the end of the row, carried as e_t = a_t g_t.  Then
 //   dx = g beta i,   dinput_gate = dx x (1 - i),
 //   dlog a = g (a h_{t-1} - (a^2 / beta) i x),   ddecay_gate = dlog a log a (1 - r),
 //   ddecay = -rate sigmoid(decay) sum over rows and steps of dlog a r.
-// h is not read back from the rounded y: each tile recomputes it from its
-// start state, which the forward keeps in 32 bits (one value per channel and
-// tile).  beta -> 0 only together with log a, whose quotient goes to zero: the
-// term is dropped there.
-//
-// Look-back.  A tile publishes its (A, H) as soon as it has it and its end
-// state once it knows its start state.  A tile walks back to the nearest
-// predecessor whose end state is there and applies the pairs in between in
-// time order, h <- A h + H -- the very operations the predecessors perform for
-// their own end states, so the result does not depend, to the last bit, on how
-// far it had to walk.  Tiles are claimed by a ticket, earliest steps first, so
-// a predecessor is always running or done; the wait is bounded all the same
-// (it sets the error word and goes on from zero).
+// h is not read back from the rounded y: the forward keeps the state before every
+// chunk in 32 bits (1 / kChunk of the elements), and the backward recomputes the
+// chunk from it.  beta -> 0 only together with log a, whose quotient goes to
+// zero: the term is dropped there.
 #pragma once
 
 #include "../../include/pesq_cuda.h"
@@ -45,16 +41,13 @@ namespace gscan {
 
 using namespace train;
 
-constexpr int kWarps = 8;
-constexpr int kSteps = 8;                 // steps per thread (L) of a tiled row
-constexpr int kTile = kWarps * kSteps;    // steps per tile
-constexpr int kForwardCtas = 4;           // CTAs an SM holds: the registers a thread may use
-constexpr int kBackwardCtas = 2;
-constexpr uint32_t kSpinLimit = 1u << 21; // polls with a 64 ns pause: about 0.1 s
+constexpr int kChunk = 8;   // steps of a chunk
+constexpr int kStrips = 8;  // strips (warps) of a CTA, where rows are cut
 
 struct Stream {
   const void* p;
-  int64_t sb, st;  // strides of batch and step, in elements
+  int64_t sb;  // strides of batch, in elements,
+  int st;      // and step, in bytes
 };
 
 struct Args {
@@ -65,17 +58,15 @@ struct Args {
   int64_t reset_b, reset_t;
   const int64_t* lengths;
   int64_t batch, steps, width;
-  int tiles;                  // per row
-  int ctiles;                 // channel tiles
+  int ctiles;                 // warps across the channels
+  int strips, strip;          // strips of a row, steps of one (a multiple of the chunk)
   int reverse;
   float rate;
-  // look-back words, [batch][tile][width]
-  unsigned long long* pair;   // (-A, H): the set sign bit is the tag
-  unsigned long long* end;    // (1, end state)
-  const unsigned long long* start;  // backward: the forward's `end` words
-  unsigned* ticket;
-  uint32_t* error;
-  uint32_t spin_limit;
+  // cut rows: (A, H) of the strips before a strip in its CTA, [batch][rank][width],
+  // and of a CTA's strips, [batch][CTA][width]; ranks count in the order of the scan at hand
+  float2* before;
+  float2* total;
+  float* kept;                // state before every chunk, [batch][chunk][width]
   // forward
   void* y;
   float* last;
@@ -83,7 +74,7 @@ struct Args {
   const float* dlast;
   void *dx, *dig, *drg;
   float* dstate;
-  float* dpart;               // [batch * tiles, width] sums of dlog a r
+  float* dpart;               // [batch * strips, width] sums of dlog a r
 };
 
 // softplus(v): log1p(e) = 2 artanh(e / (2 + e)) by its series, e = exp(-|v|)
@@ -102,411 +93,624 @@ __device__ __forceinline__ float softplus(float v) {
   return max_nan(v, 0.0f) + 2.0f * s * p;
 }
 
-struct Gates {
-  float i, r, a, w;  // w = 1 - a^2
-};
-
 // logits are held at kShut so that the product below stays finite
 // (sigmoid(-43) = 2e-19)
 constexpr float kShut = -43.0f;
+// 1 - a^2 is held above this where its root is divided by
+constexpr float kTiny = 1e-36f;
+// rates -log a up to here go by the series alone
+constexpr float kNear = 0.25f;
 
-// k = -rate softplus(decay).  The two sigmoids share one reciprocal.
-__device__ __forceinline__ Gates gates(float ig, float rg, float k) {
-  const float di = 1.0f + exp2_approx(max_nan(ig, kShut) * -kLog2e);
-  const float dr = 1.0f + exp2_approx(max_nan(rg, kShut) * -kLog2e);
-  const float q = rcp_approx(di * dr);
-  Gates o;
+template <int N>
+struct Gates {
+  Vec<N> i, r, a, w;  // w = 1 - a^2
+};
+
+// k = rate softplus(decay) >= 0.  The two sigmoids share one reciprocal.
+// With m = -log a = k r, 1 - a = m (1 - m/2 + m^2/6 - ...) by its Taylor
+// series (m^6 / 5040 < 5e-8 at 1/4): a is then rounded once, without the bias
+// that a long memory would sum up, and 1 - a^2 = (1 - a)(2 - (1 - a)) does not
+// cancel.  kFar: m may be above kNear, where the exponential takes over.
+template <bool kFar, int N>
+__device__ __forceinline__ void decays(Vec<N> r, Vec<N> k, Vec<N>& a, Vec<N>& w) {
+  const Vec<N> m = k * r;
+  Vec<N> p = fma(m, splat<N>(-1.0f / 720), splat<N>(1.0f / 120));
+  p = fma(m, p, splat<N>(-1.0f / 24));
+  p = fma(m, p, splat<N>(1.0f / 6));
+  p = fma(m, p, splat<N>(-0.5f));
+  p = fma(m, p, splat<N>(1.0f));
+  const Vec<N> u = m * p;
+  a = fma(u, splat<N>(-1.0f), splat<N>(1.0f));
+  w = u * fma(u, splat<N>(-1.0f), splat<N>(2.0f));
+  if (kFar) {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (!(m.v[j] < kNear)) {
+        a.v[j] = exp2_approx(m.v[j] * -kLog2e);
+        w.v[j] = fmaf(-a.v[j], a.v[j], 1.0f);
+      }
+  }
+}
+
+template <bool kFar, int N>
+__device__ __forceinline__ Gates<N> gates(Vec<N> ig, Vec<N> rg, Vec<N> k) {
+  Vec<N> di = ig * splat<N>(-kLog2e), dr = rg * splat<N>(-kLog2e), q;
+#pragma unroll
+  for (int j = 0; j < N; ++j) di.v[j] = exp2_approx(di.v[j]), dr.v[j] = exp2_approx(dr.v[j]);
+  di = di + splat<N>(1.0f);
+  dr = dr + splat<N>(1.0f);
+  q = di * dr;
+#pragma unroll
+  for (int j = 0; j < N; ++j) q.v[j] = rcp_approx(q.v[j]);
+  Gates<N> o;
   o.i = q * dr;
   o.r = q * di;
-  const float la = k * o.r;
-  // near zero u = a - 1 by its Taylor series (la^6 / 5040 < 5e-8 at 1/4): then
-  // a = 1 + u is rounded once, without the bias that a long memory would sum
-  // up, and 1 - a^2 = -u (2 + u) does not cancel
-  float p = fmaf(la, 1.0f / 720, 1.0f / 120);
-  p = fmaf(la, p, 1.0f / 24);
-  p = fmaf(la, p, 1.0f / 6);
-  p = fmaf(la, p, 0.5f);
-  p = fmaf(la, p, 1.0f);
-  const float u = la * p;
-  o.a = 1.0f + u;
-  o.w = -u * (2.0f + u);
-  if (!(la > -0.25f)) {
-    o.a = exp2_approx(la * kLog2e);
-    o.w = fmaf(-o.a, o.a, 1.0f);
-  }
+  decays<kFar, N>(o.r, k, o.a, o.w);
   return o;
 }
 
-// A state that a = 0 cuts off is not looked at (it may be infinite or NaN)
-template <bool kMask>
-__device__ __forceinline__ float apply(float a, float h, float b) {
-  if (kMask) h = a == 0.0f ? 0.0f : h;
-  return fmaf(a, h, b);
+// The decay alone
+template <bool kFar, int N>
+__device__ __forceinline__ Vec<N> decay_of(Vec<N> rg, Vec<N> k) {
+  Vec<N> dr = rg * splat<N>(-kLog2e);
+#pragma unroll
+  for (int j = 0; j < N; ++j) dr.v[j] = exp2_approx(dr.v[j]);
+  dr = dr + splat<N>(1.0f);
+#pragma unroll
+  for (int j = 0; j < N; ++j) dr.v[j] = rcp_approx(dr.v[j]);
+  Vec<N> a, w;
+  decays<kFar, N>(dr, k, a, w);
+  return a;
 }
 
-// Start value of tile `tile` (>= 1 predecessors, nearest at `tile - dir`) of
-// one channel: words at `pair`/`end` + k * pitch for the k-th tile back.
-// `count` predecessors exist; the farthest always publishes its end value
-// without waiting.
-template <bool kMask>
-__device__ float look_back(const Args& p, const unsigned long long* pair, const unsigned long long* end, int64_t pitch,
-                           int count) {
-  constexpr int kWin = 8;
-  int done = 0;  // pairs nearer than this are all there
-  unsigned polls = 0;
-  float h = 0.0f;
-  for (;;) {
-    unsigned long long e[kWin], q[kWin];
+// sqrt(w) of w >= 0
+template <int N>
+__device__ __forceinline__ Vec<N> root(Vec<N> w) {
+  Vec<N> s;
 #pragma unroll
-    for (int j = 0; j < kWin; ++j) {
-      const bool in = done + j < count;
-      e[j] = in ? get_word(end + (done + j) * pitch) : 0ull;
-      q[j] = in ? get_word(pair + (done + j) * pitch) : 0ull;
-    }
-    int at = -1;  // nearest end value with every pair before it there
-    bool open = true;
+  for (int j = 0; j < N; ++j) s.v[j] = rsqrt_approx(fmaxf(w.v[j], kTiny));
+  return w * s;
+}
+
+// a h + b.  A state that a = 0 cuts off is not looked at (it may be infinite or NaN).
+template <bool kMask, int N>
+__device__ __forceinline__ Vec<N> apply(Vec<N> a, Vec<N> h, Vec<N> b) {
+  if (kMask) {
 #pragma unroll
-    for (int j = 0; j < kWin; ++j) {
-      if (open && at < 0 && e[j] != 0ull) at = j;
-      if (q[j] == 0ull) open = false;
-    }
-    if (at >= 0) {
-#pragma unroll
-      for (int j = kWin - 1; j >= 0; --j) {
-        if (j == at) h = __uint_as_float((unsigned)e[j]);
-        if (j < at) h = apply<kMask>(-__uint_as_float((unsigned)(q[j] >> 32)), h, __uint_as_float((unsigned)q[j]));
-      }
-      break;
-    }
-    if (open) {
-      done += kWin;
-      continue;
-    }
-    if (++polls > p.spin_limit) {
-      atomicOr(p.error, 1u);
-      break;
-    }
-    __nanosleep(64);
+    for (int j = 0; j < N; ++j) h.v[j] = a.v[j] == 0.0f ? 0.0f : h.v[j];
   }
-  // the windows passed on the way, farthest first
-  for (int k = done; k > 0; k -= kWin) {
-    unsigned long long q[kWin];
-#pragma unroll
-    for (int j = 0; j < kWin; ++j) q[j] = get_word(pair + (k - 1 - j) * pitch);
-#pragma unroll
-    for (int j = 0; j < kWin; ++j)
-      h = apply<kMask>(-__uint_as_float((unsigned)(q[j] >> 32)), h, __uint_as_float((unsigned)q[j]));
-  }
-  return h;
+  return fma(a, h, b);
 }
 
-__device__ __forceinline__ unsigned long long pair_word(float a, float h) {
-  return ((unsigned long long)(__float_as_uint(a) | 0x80000000u) << 32) | __float_as_uint(h);
+// logits at least kShut (a NaN stays)
+__device__ __forceinline__ void hold(Pack<float, 1>& p) { p.v[0] = max_nan(p.v[0], kShut); }
+__device__ __forceinline__ void hold(Pack<__nv_bfloat16, 1>& p) {
+  p.v[0] = __hmax_nan(p.v[0], __float2bfloat16_rn(kShut));
 }
-__device__ __forceinline__ unsigned long long end_word(float h) { return (1ull << 32) | __float_as_uint(h); }
-
-// L steps of V channels of one stream, steps s0, s0 + 1, ... in scan order;
-// those outside `live` (a bit per step) read as `other` and are not touched.
-// A decay gate of kShut makes a step the identity to the last bit: a = 1, and
-// b = 0 for x = 0.
-template <class T, int V, int L>
-__device__ __forceinline__ void load(Pack<T, V> (&out)[L], const Stream& s, int64_t b, int64_t t0, int dir, int64_t c,
-                                     unsigned live, float other = 0.0f) {
-  const T* p = static_cast<const T*>(s.p) + b * s.sb + t0 * s.st + c;
-  const int64_t step = dir * s.st;
+__device__ __forceinline__ void hold(Pack<__half, 1>& p) { p.v[0] = __hmax_nan(p.v[0], __float2half_rn(kShut)); }
+template <int V>
+__device__ __forceinline__ void hold(Pack<float, V>& p) {
 #pragma unroll
-  for (int l = 0; l < L; ++l) {
-    if ((live >> l) & 1u) {
-      out[l] = *reinterpret_cast<const Pack<T, V>*>(p + l * step);
-    } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) out[l].v[v] = narrow<T>(other);
-    }
-  }
+  for (int v = 0; v < V; ++v) p.v[v] = max_nan(p.v[v], kShut);
 }
-
-template <class T, int V, int L>
-__device__ __forceinline__ void store(void* base, const Args& p, int64_t b, int64_t t, int64_t c, const float (&val)[V]) {
-  Pack<T, V> o;
+template <int V>
+__device__ __forceinline__ void hold(Pack<__nv_bfloat16, V>& p) {
+  __nv_bfloat162* q = reinterpret_cast<__nv_bfloat162*>(&p);
 #pragma unroll
-  for (int v = 0; v < V; ++v) o.v[v] = narrow<T>(val[v]);
-  *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(base) + (b * p.steps + t) * p.width + c) = o;
+  for (int v = 0; v < V / 2; ++v) q[v] = __hmax2_nan(q[v], __float2bfloat162_rn(kShut));
+}
+template <int V>
+__device__ __forceinline__ void hold(Pack<__half, V>& p) {
+  __half2* q = reinterpret_cast<__half2*>(&p);
+#pragma unroll
+  for (int v = 0; v < V / 2; ++v) q[v] = __hmax2_nan(q[v], __float2half2_rn(kShut));
 }
 
-// What a thread works on
-struct Place {
+// What a lane works on, and where its strip lies
+struct Lane {
   int64_t b, c;      // row, first channel
-  int tile;          // in scan order
-  int64_t s0;        // first step of the thread, in scan order
-  int64_t t0;        // and in memory
-  int dir;
-  bool on;           // channel in range
-  unsigned inside;   // steps of the row
+  int rank;          // of the strip, in the order of this scan
+  int first, count;  // chunks of the strip, in the order of the steps' scan
+  int whole;         // those of them that have all their steps
+  int dir;           // memory direction of the steps' scan
+  int64_t len;       // the row's length
+  bool on;           // channels in range
+  int64_t from;      // first channel to read
+};
+
+template <int V, int L, bool kMask, bool kBack>
+__device__ __forceinline__ Lane lane_of(const Args& p) {
+  Lane o;
+  o.b = blockIdx.y;
+  const unsigned block = blockIdx.x / p.ctiles;  // CTA along the row
+  o.c = (int64_t)(blockIdx.x - block * p.ctiles) * (32 * V) + threadIdx.x * V;
+  o.on = o.c < p.width;
+  o.from = o.on ? o.c : 0;
+  o.rank = block * blockDim.y + threadIdx.y;
+  const int strip = kBack ? p.strips - 1 - o.rank : o.rank;
+  const int all = (int)((p.steps + L - 1) / L), per = p.strip / L;
+  o.first = strip * per;
+  o.count = strip < 0 || strip >= p.strips ? 0 : min(per, all - o.first);
+  o.whole = min(o.count, max(0, (int)(p.steps / L) - o.first));
+  o.dir = p.reverse ? -1 : 1;
+  o.len = kMask && p.lengths ? p.lengths[o.b] : p.steps;
+  return o;
+}
+
+// Steps of one chunk
+struct Chunk {
+  int64_t t0;        // first step, in memory
+  unsigned inside;   // steps of the row (a bit each)
   unsigned live;     // before the row's length
   unsigned cut;      // reset
 };
-
-template <int V, int L, bool kMask>
-__device__ __forceinline__ Place place(const Args& p, unsigned id, bool from_end) {
-  Place o;
-  const unsigned per = (unsigned)(p.batch * p.ctiles);
-  o.tile = id / per;
-  const unsigned rest = id - o.tile * per;
-  if (from_end) o.tile = p.tiles - 1 - o.tile;
-  o.b = rest / p.ctiles;
-  o.c = (int64_t)(rest - (unsigned)o.b * p.ctiles) * (32 * V) + threadIdx.x * V;
-  o.on = o.c < p.width;
-  o.s0 = (int64_t)o.tile * (blockDim.y * L) + threadIdx.y * L;
-  o.dir = p.reverse ? -1 : 1;
-  o.t0 = p.reverse ? p.steps - 1 - o.s0 : o.s0;
-  const int64_t left = p.steps - o.s0;
-  o.inside = left >= L ? (1u << L) - 1 : left <= 0 ? 0u : (1u << left) - 1;
-  o.live = o.inside;
-  o.cut = 0u;
+template <int L, bool kMask>
+__device__ __forceinline__ Chunk chunk_of(const Args& p, const Lane& o, int k) {
+  Chunk q;
+  const int64_t s0 = (int64_t)k * L, left = p.steps - s0;
+  q.t0 = p.reverse ? p.steps - 1 - s0 : s0;
+  q.inside = left >= L ? (1u << L) - 1 : (1u << left) - 1;
+  q.live = q.inside;
+  q.cut = 0u;
   if (kMask) {
-    if (p.lengths) {
-      const int64_t len = p.lengths[o.b];
 #pragma unroll
-      for (int l = 0; l < L; ++l)
-        if (o.t0 + l * o.dir >= len) o.live &= ~(1u << l);
-    }
-    if (p.reset) {
-#pragma unroll
-      for (int l = 0; l < L; ++l)
-        if ((o.live >> l) & 1u)
-          if (p.reset[o.b * p.reset_b + (o.t0 + l * o.dir) * p.reset_t]) o.cut |= 1u << l;
+    for (int l = 0; l < L; ++l) {
+      const int64_t t = q.t0 + l * o.dir;
+      if (t >= o.len) q.live &= ~(1u << l);
+      if (p.reset && ((q.live >> l) & 1u) && p.reset[o.b * p.reset_b + t * p.reset_t]) q.cut |= 1u << l;
     }
   }
-  return o;
+  return q;
 }
 
-__device__ __forceinline__ unsigned claim(const Args& p) {
-  __shared__ unsigned s_id;
-  if (p.tiles == 1) return blockIdx.x;
-  if (threadIdx.x == 0 && threadIdx.y == 0) s_id = atomicAdd(p.ticket, 1u);
-  __syncthreads();
-  return s_id;
-}
-
-template <class T, int V, int L, bool kMask>
-__global__ void __launch_bounds__(32 * kWarps, kForwardCtas) forward_kernel(const __grid_constant__ Args p) {
-  constexpr int C = 32 * V;
-  __shared__ float sA[kWarps][C], sH[kWarps][C], sS[C];
-  const Place o = place<V, L, kMask>(p, claim(p), false);
-  const int lane = threadIdx.x, warp = threadIdx.y, warps = blockDim.y;
-
-  Pack<T, V> x[L], ig[L], rg[L];
-  const unsigned touch = o.on ? o.live : 0u;
-  load<T, V, L>(rg, p.rg, o.b, o.t0, o.dir, o.c, touch, kShut);
-  load<T, V, L>(ig, p.ig, o.b, o.t0, o.dir, o.c, touch);
-  load<T, V, L>(x, p.x, o.b, o.t0, o.dir, o.c, touch);
-  float kd[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) kd[v] = o.on ? -p.rate * softplus(p.decay[o.c + v]) : 0.0f;
-
-  float a[L][V], b[L][V], A[V], H[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) A[v] = 1.0f, H[v] = 0.0f;
-#pragma unroll
-  for (int l = 0; l < L; ++l) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const Gates g = gates(widen(ig[l].v[v]), widen(rg[l].v[v]), kd[v]);
-      float beta = g.w > 0.0f ? g.w * rsqrt_approx(g.w) : g.w;
-      float ga = g.a;
-      if (kMask && ((o.cut >> l) & 1u)) ga = 0.0f, beta = 1.0f;
-      a[l][v] = ga;
-      b[l][v] = beta * g.i * widen(x[l].v[v]);
-      H[v] = apply<kMask>(ga, H[v], b[l][v]);
-      A[v] *= ga;
-    }
-  }
-#pragma unroll
-  for (int v = 0; v < V; ++v) sA[warp][lane * V + v] = A[v], sH[warp][lane * V + v] = H[v];
-  __syncthreads();
-
-  const int64_t c0 = o.c - lane * V;
-  for (int k = warp * 32 + lane; k < C; k += warps * 32) {
-    const int64_t c = c0 + k;
-    if (c >= p.width) break;
-    float tA = 1.0f, tH = 0.0f;
-    for (int w = 0; w < warps; ++w) {
-      tH = apply<kMask>(sA[w][k], tH, sH[w][k]);
-      tA *= sA[w][k];
-    }
-    const int64_t at = (o.b * p.tiles + o.tile) * p.width + c;
-    float h = o.tile == 0 && p.state ? p.state[o.b * p.width + c] : 0.0f;
-    if (o.tile > 0) {
-      put_word(p.pair + at, pair_word(tA, tH));
-      h = look_back<kMask>(p, p.pair + at - p.width, p.end + at - p.width, -p.width, o.tile);
-    }
-    sS[k] = h;
-    h = apply<kMask>(tA, h, tH);
-    if (p.tiles > 1) put_word(p.end + at, end_word(h));
-    if (o.tile == p.tiles - 1) p.last[o.b * p.width + c] = h;
-  }
-  __syncthreads();
-  if (!o.on || o.inside == 0u) return;
-
-  float h[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) h[v] = sS[lane * V + v];
-  for (int w = 0; w < warp; ++w) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = apply<kMask>(sA[w][lane * V + v], h[v], sH[w][lane * V + v]);
-  }
-#pragma unroll
-  for (int l = 0; l < L; ++l) {
-    float out[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      h[v] = apply<kMask>(a[l][v], h[v], b[l][v]);
-      out[v] = !kMask || ((o.live >> l) & 1u) ? h[v] : 0.0f;
-    }
-    if ((o.inside >> l) & 1u) store<T, V, L>(p.y, p, o.b, o.t0 + l * o.dir, o.c, out);
+// Loads one pack where `take` is nonzero and leaves it as it is otherwise: a
+// predicated load, with no branch whose join would wait for it
+template <class P>
+__device__ __forceinline__ void load_if(P& out, const char* p, unsigned take) {
+  if constexpr (sizeof(P) == 2) {
+    asm("{\n.reg .pred q;\nsetp.ne.u32 q, %2, 0;\n@q ld.global.b16 %0, [%1];\n}"
+        : "+h"(reinterpret_cast<unsigned short&>(out))
+        : "l"(p), "r"(take));
+  } else if constexpr (sizeof(P) == 4) {
+    asm("{\n.reg .pred q;\nsetp.ne.u32 q, %2, 0;\n@q ld.global.b32 %0, [%1];\n}"
+        : "+r"(reinterpret_cast<unsigned&>(out))
+        : "l"(p), "r"(take));
+  } else {
+    asm("{\n.reg .pred q;\nsetp.ne.u32 q, %2, 0;\n@q ld.global.b64 %0, [%1];\n}"
+        : "+l"(reinterpret_cast<unsigned long long&>(out))
+        : "l"(p), "r"(take));
   }
 }
 
-template <class T, int V, int L, bool kMask>
-__global__ void __launch_bounds__(32 * kWarps, kBackwardCtas) backward_kernel(const __grid_constant__ Args p) {
-  constexpr int C = 32 * V;
-  // (A, H): the forward map of each warp's steps; E: what the carry e leaves them with from zero
-  __shared__ float sA[kWarps][C], sH[kWarps][C], sE[kWarps][C], sC[C];
-  const Place o = place<V, L, kMask>(p, claim(p), true);
-  const int lane = threadIdx.x, warp = threadIdx.y, warps = blockDim.y;
-
-  Pack<T, V> x[L], ig[L], rg[L], dy[L];
-  const unsigned touch = o.on ? o.live : 0u;
-  load<T, V, L>(rg, p.rg, o.b, o.t0, o.dir, o.c, touch, kShut);
-  load<T, V, L>(ig, p.ig, o.b, o.t0, o.dir, o.c, touch);
-  load<T, V, L>(x, p.x, o.b, o.t0, o.dir, o.c, touch);
-  load<T, V, L>(dy, p.dy, o.b, o.t0, o.dir, o.c, p.dy.p ? touch : 0u);
-  float kd[V];
+// The steps of a chunk, in scan order; those that are not live read as `other`
+// and are not touched.  A decay gate of kShut makes a step the identity to the
+// last bit: a = 1, and b = 0 for x = 0.  kFull: all steps are live.
+template <class T, int V, int L, bool kFull>
+__device__ __forceinline__ void load(Pack<T, V> (&out)[L], const Stream& s, const Lane& o, const Chunk& q,
+                                     float other = 0.0f) {
+  // (lanes past the width read the row's first channels)
+  const char* p = reinterpret_cast<const char*>(static_cast<const T*>(s.p) + o.b * s.sb + o.from) + q.t0 * s.st;
+  const int step = o.dir * s.st;
+  if (kFull) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) kd[v] = o.on ? -p.rate * softplus(p.decay[o.c + v]) : 0.0f;
-
-  float gi[L][V], gr[L][V], a[L][V], be[L][V], hp[L][V], A[V], H[V], E[V];
+    for (int l = 0; l < L; ++l) out[l] = *reinterpret_cast<const Pack<T, V>*>(p + (int64_t)step * l);
+  } else {
 #pragma unroll
-  for (int v = 0; v < V; ++v) A[v] = 1.0f, H[v] = 0.0f, E[v] = 0.0f;
+    for (int l = 0; l < L; ++l) {
 #pragma unroll
-  for (int l = 0; l < L; ++l) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const Gates g = gates(widen(ig[l].v[v]), widen(rg[l].v[v]), kd[v]);
-      gi[l][v] = g.i, gr[l][v] = g.r, a[l][v] = g.a;
-      be[l][v] = g.w > 0.0f ? g.w * rsqrt_approx(g.w) : g.w;
-      if (kMask && ((o.cut >> l) & 1u)) a[l][v] = 0.0f, be[l][v] = 1.0f;
-      H[v] = apply<kMask>(a[l][v], H[v], be[l][v] * g.i * widen(x[l].v[v]));
-      A[v] *= a[l][v];
+      for (int v = 0; v < V; ++v) out[l].v[v] = narrow<T>(other);
+      load_if(out[l], p + (int64_t)step * l, (q.live >> l) & 1u);
     }
   }
+}
+template <class T, int V, int N>
+__device__ __forceinline__ void store(void* p, const Vec<N> (&val)[V / N]) {
+  Pack<T, V> o;
 #pragma unroll
-  for (int l = L - 1; l >= 0; --l) {
+  for (int v = 0; v < V; ++v) o.v[v] = narrow<T>(val[v / N].v[v % N]);
+  *static_cast<Pack<T, V>*>(p) = o;
+}
+
+// How L x V elements are paired for the two-wide instructions: by channel, or by
+// step where a lane has a single channel.
+template <int V, int L>
+struct Pairing {
+  static constexpr int N = V > 1 ? 2 : 1;                 // channels of a Vec
+  static constexpr int P = V / N;                         // Vecs of a step
+  static constexpr int S = V == 1 && L % 2 == 0 ? 2 : 1;  // steps worked out together
+};
+
+// Calls emit(l, j, gates, beta) for every step and Vec of a chunk, steps in order
+template <class T, int V, int L, bool kMask, bool kFar, class F>
+__device__ __forceinline__ void each_gate(const Chunk& q, const Pack<T, V> (&ig)[L], const Pack<T, V> (&rg)[L],
+                                          const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P], F emit) {
+  using Q = Pairing<V, L>;
+  constexpr int N = Q::N, S = Q::S;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      E[v] += widen(dy[l].v[v]);
-      E[v] = kMask && a[l][v] == 0.0f ? 0.0f : a[l][v] * E[v];
+  for (int l = 0; l < L; l += S) {
+    if constexpr (S == 2) {
+      Pack<T, 2> r2{{rg[l].v[0], rg[l + 1].v[0]}}, i2{{ig[l].v[0], ig[l + 1].v[0]}};
+      hold(r2), hold(i2);
+      const Gates<2> g = gates<kFar, 2>(widen<2>(i2, 0), widen<2>(r2, 0), splat<2>(rate[0].v[0]));
+      const Vec<2> beta = root(g.w);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        Gates<1> one{{{g.i.v[i]}}, {{g.r.v[i]}}, {{g.a.v[i]}}, {{g.w.v[i]}}};
+        Vec<1> b1{{beta.v[i]}};
+        if (kMask && ((q.cut >> (l + i)) & 1u)) one.a = splat<1>(0.0f), b1 = splat<1>(1.0f);
+        emit(l + i, 0, one, b1);
+      }
+    } else {
+      Pack<T, V> r1 = rg[l], i1 = ig[l];
+      hold(r1), hold(i1);
+#pragma unroll
+      for (int j = 0; j < Q::P; ++j) {
+        Gates<N> g = gates<kFar, N>(widen<N>(i1, j), widen<N>(r1, j), rate[j]);
+        Vec<N> beta = root(g.w);
+        if (kMask && ((q.cut >> l) & 1u)) g.a = splat<N>(0.0f), beta = splat<N>(1.0f);
+        emit(l, j, g, beta);
+      }
     }
   }
-#pragma unroll
-  for (int v = 0; v < V; ++v) sA[warp][lane * V + v] = A[v], sH[warp][lane * V + v] = H[v], sE[warp][lane * V + v] = E[v];
-  __syncthreads();
+}
 
-  const int64_t c0 = o.c - lane * V;
-  for (int k = warp * 32 + lane; k < C; k += warps * 32) {
-    const int64_t c = c0 + k;
-    if (c >= p.width) break;
-    float tA = 1.0f, tE = 0.0f;
-    for (int w = warps - 1; w >= 0; --w) {
-      tE = apply<kMask>(sA[w][k], tE, sE[w][k]);
-      tA *= sA[w][k];
-    }
-    const int64_t at = (o.b * p.tiles + o.tile) * p.width + c;
-    const int after = p.tiles - 1 - o.tile;
-    float e = after == 0 && p.dlast ? p.dlast[o.b * p.width + c] : 0.0f;
-    if (after > 0) {
-      put_word(p.pair + at, pair_word(tA, tE));
-      e = look_back<kMask>(p, p.pair + at + p.width, p.end + at + p.width, p.width, after);
-    }
-    sC[k] = e;
-    e = apply<kMask>(tA, e, tE);
-    if (p.tiles > 1) put_word(p.end + at, end_word(e));
-    if (o.tile == 0 && p.dstate) p.dstate[o.b * p.width + c] = e;
-  }
-
-  // the states before each step, from the tile's start state
-  float h[V], e[V], acc[V];
+// The rates of a lane's channels, and whether one of the warp's is above kNear
+template <int V, int N>
+__device__ __forceinline__ bool rates(const Args& p, const Lane& o, Vec<N> (&rate)[V / N]) {
+  bool far = false;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    h[v] = 0.0f, acc[v] = 0.0f;
-    if (o.on) {
-      if (o.tile > 0)
-        h[v] = __uint_as_float((unsigned)p.start[(o.b * p.tiles + o.tile - 1) * p.width + o.c + v]);
-      else if (p.state)
-        h[v] = p.state[o.b * p.width + o.c + v];
-    }
+    const float k = o.on ? p.rate * softplus(p.decay[o.c + v]) : 0.0f;
+    rate[v / N].v[v % N] = k;
+    far = far || !(k < kNear);
   }
-  for (int w = 0; w < warp; ++w) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = apply<kMask>(sA[w][lane * V + v], h[v], sH[w][lane * V + v]);
-  }
-#pragma unroll
-  for (int l = 0; l < L; ++l) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      hp[l][v] = h[v];
-      h[v] = apply<kMask>(a[l][v], h[v], be[l][v] * gi[l][v] * widen(x[l].v[v]));
-    }
-  }
-  __syncthreads();
+  return __any_sync(0xffffffffu, far);
+}
 
+template <int V, int N>
+__device__ __forceinline__ void read_row(const float* p, Vec<N> (&out)[V / N]) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) e[v] = sC[lane * V + v];
-  for (int w = warps - 1; w > warp; --w) {
+  for (int v = 0; v < V; ++v) out[v / N].v[v % N] = p[v];
+}
+
+// Start value of a strip: the row's, through the maps of the CTAs before and of
+// the strips before in the CTA
+template <int V, int N, bool kMask>
+__device__ __forceinline__ void start_of(const Args& p, const Lane& o, Vec<N> (&h)[V / N]) {
+  if (p.strips == 1 || !o.on || o.rank >= p.strips) return;
+  const int ctas = (p.strips + kStrips - 1) / kStrips, cta = o.rank / kStrips;
+  const float2* t = p.total + o.b * ctas * p.width + o.c;
 #pragma unroll
-    for (int v = 0; v < V; ++v) e[v] = apply<kMask>(sA[w][lane * V + v], e[v], sE[w][lane * V + v]);
+  for (int v = 0; v < V; ++v) {
+    Vec<1> s{{h[v / N].v[v % N]}};
+#pragma unroll 8
+    for (int k = 0; k < cta; ++k) {
+      const float2 m = t[k * p.width + v];
+      s = apply<kMask>(Vec<1>{{m.x}}, s, Vec<1>{{m.y}});
+    }
+    const float2 m = p.before[(o.b * p.strips + o.rank) * p.width + o.c + v];
+    h[v / N].v[v % N] = apply<kMask>(Vec<1>{{m.x}}, s, Vec<1>{{m.y}}).v[0];
   }
+}
+
+// The maps of a CTA's strips, warp by warp: leaves in `before` what the strips
+// before each make of a state, and in `total` all of them.
+template <int V, int N, bool kMask>
+__device__ __forceinline__ void join_maps(const Args& p, const Lane& o, const Vec<N> (&A)[V / N], const Vec<N> (&H)[V / N]) {
+  __shared__ float2 s_map[kStrips][32 * V];
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    s_map[threadIdx.y][threadIdx.x * V + v] = make_float2(A[v / N].v[v % N], H[v / N].v[v % N]);
+  __syncthreads();
+  if (!o.on || o.rank >= p.strips) return;
+  const bool end = threadIdx.y == kStrips - 1 || o.rank == p.strips - 1;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    Vec<1> a{{1.0f}}, h{{0.0f}};
+    for (int w = 0; w < (int)threadIdx.y; ++w) {
+      const float2 m = s_map[w][threadIdx.x * V + v];
+      h = apply<kMask>(Vec<1>{{m.x}}, h, Vec<1>{{m.y}});
+      a.v[0] *= m.x;
+    }
+    p.before[(o.b * p.strips + o.rank) * p.width + o.c + v] = make_float2(a.v[0], h.v[0]);
+    if (end) {
+      const float2 m = s_map[threadIdx.y][threadIdx.x * V + v];
+      h = apply<kMask>(Vec<1>{{m.x}}, h, Vec<1>{{m.y}});
+      const int ctas = (p.strips + kStrips - 1) / kStrips;
+      p.total[(o.b * ctas + o.rank / kStrips) * p.width + o.c + v] = make_float2(a.v[0] * m.x, h.v[0]);
+    }
+  }
+}
+
+// ------------------------------------------------------------------- forward
+
+template <class T, int V, int L>
+struct Loaded {
+  Chunk q;
+  Pack<T, V> x[L], ig[L], rg[L];
+};
+
+template <class T, int V, int L, bool kMask, bool kFull>
+__device__ __forceinline__ void read_chunk(const Args& p, const Lane& o, int k, Loaded<T, V, L>& in) {
+  in.q = chunk_of<L, kMask>(p, o, k);
+  load<T, V, L, kFull>(in.rg, p.rg, o, in.q, kShut);
+  load<T, V, L, kFull>(in.ig, p.ig, o, in.q);
+  load<T, V, L, kFull>(in.x, p.x, o, in.q);
+}
+
+template <class T, int V, int L, bool kMask, bool kFar>
+__device__ __forceinline__ void forward_maps(const Args& p, const Lane& o,
+                                             const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P]) {
+  using Q = Pairing<V, L>;
+  constexpr int N = Q::N, P = Q::P;
+  Vec<N> A[P], H[P];
+#pragma unroll
+  for (int j = 0; j < P; ++j) A[j] = splat<N>(1.0f), H[j] = splat<N>(0.0f);
+#pragma unroll 1
+  for (int k = 0; k < o.count; ++k) {
+    Loaded<T, V, L> in;
+    read_chunk<T, V, L, kMask, false>(p, o, o.first + k, in);
+    each_gate<T, V, L, kMask, kFar>(in.q, in.ig, in.rg, rate, [&](int l, int j, const Gates<N>& g, Vec<N> beta) {
+      H[j] = apply<kMask>(g.a, H[j], beta * (g.i * widen<N>(in.x[l], j)));
+      A[j] = A[j] * g.a;
+    });
+  }
+  join_maps<V, N, kMask>(p, o, A, H);
+}
+
+template <class T, int V, int L, bool kMask>
+__global__ void __launch_bounds__(32 * kStrips) forward_maps_kernel(const __grid_constant__ Args p) {
+  using Q = Pairing<V, L>;
+  const Lane o = lane_of<V, L, kMask, false>(p);
+  Vec<Q::N> rate[Q::P];
+  // (the CTA's warps share their channels, so they agree, and meet in join_maps)
+  if (rates<V, Q::N>(p, o, rate))
+    forward_maps<T, V, L, kMask, true>(p, o, rate);
+  else
+    forward_maps<T, V, L, kMask, false>(p, o, rate);
+}
+
+template <class T, int V, int L, bool kMask, bool kFar, bool kFull>
+__device__ __forceinline__ void forward_chunk(const Args& p, const Lane& o, int k, const Loaded<T, V, L>& in,
+                                              const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P],
+                                              Vec<Pairing<V, L>::N> (&h)[Pairing<V, L>::P]) {
+  using Q = Pairing<V, L>;
+  constexpr int N = Q::N, P = Q::P;
+  if (p.kept && o.on) {
+    float* keep = p.kept + (o.b * ((p.steps + L - 1) / L) + k) * p.width + o.c;
+#pragma unroll
+    for (int v = 0; v < V; ++v) keep[v] = h[v / N].v[v % N];
+  }
+  char* y = reinterpret_cast<char*>(static_cast<T*>(p.y) + (o.b * p.steps + in.q.t0) * p.width + o.c);
+  const int step = o.dir * (int)p.width * (int)sizeof(T);
+  Vec<N> out[P];
+  each_gate<T, V, L, kMask, kFar>(in.q, in.ig, in.rg, rate, [&](int l, int j, const Gates<N>& g, Vec<N> beta) {
+    h[j] = apply<kMask>(g.a, h[j], beta * (g.i * widen<N>(in.x[l], j)));
+    out[j] = !kMask || ((in.q.live >> l) & 1u) ? h[j] : splat<N>(0.0f);
+    if (j == P - 1 && o.on && (kFull || ((in.q.inside >> l) & 1u))) store<T, V, N>(y + (int64_t)step * l, out);
+  });
+}
+
+template <class T, int V, int L, bool kMask, bool kFar>
+__device__ __forceinline__ void forward_strip(const Args& p, const Lane& o,
+                                              const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P]) {
+  using Q = Pairing<V, L>;
+  constexpr int N = Q::N, P = Q::P;
+  if (o.count == 0) return;
+  // whole chunks two at a time, each read while the one before it is worked on;
+  // then the row's last steps (with masks every chunk may be partial)
+  constexpr bool kFull = !kMask;
+  const int whole = kMask ? o.count : o.whole;
+  Loaded<T, V, L> one, two;
+  if (whole) read_chunk<T, V, L, kMask, kFull>(p, o, o.first, one);
+  Vec<N> h[P];
+#pragma unroll
+  for (int j = 0; j < P; ++j) h[j] = splat<N>(0.0f);
+  if (p.state) read_row<V, N>(p.state + o.b * p.width + o.from, h);
+  start_of<V, N, kMask>(p, o, h);
+#pragma unroll 1
+  for (int k = 0; k < whole; k += 2) {
+    read_chunk<T, V, L, kMask, kFull>(p, o, o.first + min(k + 1, whole - 1), two);
+    forward_chunk<T, V, L, kMask, kFar, kFull>(p, o, o.first + k, one, rate, h);
+    read_chunk<T, V, L, kMask, kFull>(p, o, o.first + min(k + 2, whole - 1), one);
+    if (k + 1 < whole) forward_chunk<T, V, L, kMask, kFar, kFull>(p, o, o.first + k + 1, two, rate, h);
+  }
+  if (whole < o.count) {
+    read_chunk<T, V, L, kMask, false>(p, o, o.first + whole, one);
+    forward_chunk<T, V, L, kMask, kFar, false>(p, o, o.first + whole, one, rate, h);
+  }
+  if (o.rank == p.strips - 1 && o.on) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) p.last[o.b * p.width + o.c + v] = h[v / N].v[v % N];
+  }
+}
+
+template <class T, int V, int L, bool kMask>
+__global__ void __launch_bounds__(32 * kStrips) forward_kernel(const __grid_constant__ Args p) {
+  using Q = Pairing<V, L>;
+  const Lane o = lane_of<V, L, kMask, false>(p);
+  Vec<Q::N> rate[Q::P];
+  if (rates<V, Q::N>(p, o, rate))
+    forward_strip<T, V, L, kMask, true>(p, o, rate);
+  else
+    forward_strip<T, V, L, kMask, false>(p, o, rate);
+}
+
+// ------------------------------------------------------------------ backward
+
+// e -> A e + E of a strip, from its last step to its first: the decay gate and
+// dy are all it takes
+template <class T, int V, int L, bool kMask, bool kFar>
+__device__ __forceinline__ void backward_maps(const Args& p, const Lane& o,
+                                              const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P]) {
+  using Q = Pairing<V, L>;
+  constexpr int N = Q::N, P = Q::P;
+  Vec<N> A[P], E[P];
+#pragma unroll
+  for (int j = 0; j < P; ++j) A[j] = splat<N>(1.0f), E[j] = splat<N>(0.0f);
+#pragma unroll 1
+  for (int k = o.count - 1; k >= 0; --k) {
+    const Chunk q = chunk_of<L, kMask>(p, o, o.first + k);
+    Pack<T, V> rg[L], dy[L];
+    load<T, V, L, false>(rg, p.rg, o, q, kShut);
+    load<T, V, L, false>(dy, p.dy, o, q);
+#pragma unroll
+    for (int l = L - 1; l >= 0; --l) {
+      hold(rg[l]);
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        Vec<N> a = decay_of<kFar, N>(widen<N>(rg[l], j), rate[j]);
+        if (kMask && ((q.cut >> l) & 1u)) a = splat<N>(0.0f);
+        E[j] = apply<kMask>(a, E[j] + widen<N>(dy[l], j), splat<N>(0.0f));
+        A[j] = A[j] * a;
+      }
+    }
+  }
+  join_maps<V, N, kMask>(p, o, A, E);
+}
+
+template <class T, int V, int L, bool kMask>
+__global__ void __launch_bounds__(32 * kStrips) backward_maps_kernel(const __grid_constant__ Args p) {
+  using Q = Pairing<V, L>;
+  const Lane o = lane_of<V, L, kMask, true>(p);
+  Vec<Q::N> rate[Q::P];
+  if (rates<V, Q::N>(p, o, rate))
+    backward_maps<T, V, L, kMask, true>(p, o, rate);
+  else
+    backward_maps<T, V, L, kMask, false>(p, o, rate);
+}
+
+template <class T, int V, int L>
+struct LoadedBack {
+  Chunk q;
+  Pack<T, V> x[L], ig[L], rg[L], dy[L];
+  Vec<Pairing<V, L>::N> h[Pairing<V, L>::P];  // state before the chunk
+};
+
+template <class T, int V, int L, bool kMask, bool kFull>
+__device__ __forceinline__ void read_back(const Args& p, const Lane& o, int k, LoadedBack<T, V, L>& in) {
+  in.q = chunk_of<L, kMask>(p, o, k);
+  load<T, V, L, kFull>(in.rg, p.rg, o, in.q, kShut);
+  load<T, V, L, kFull>(in.ig, p.ig, o, in.q);
+  load<T, V, L, kFull>(in.x, p.x, o, in.q);
+  load<T, V, L, kFull>(in.dy, p.dy, o, in.q);
+  read_row<V, Pairing<V, L>::N>(p.kept + (o.b * ((p.steps + L - 1) / L) + k) * p.width + o.from, in.h);
+}
+
+// With e = a g (see above) everything but g is known before the carry comes in:
+//   dx = g P1, dinput_gate = dx P2, s = g R1, ddecay_gate = s R2,
+//   P1 = beta i, P2 = x (1 - i), R1 = r (a h_{t-1} - (a^2 / beta) i x), R2 = rate (r - 1),
+// and s sums up to the decay gradient.
+template <class T, int V, int L, bool kMask, bool kFar, bool kFull>
+__device__ __forceinline__ void backward_chunk(const Args& p, const Lane& o, const LoadedBack<T, V, L>& in,
+                                               const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P],
+                                               Vec<Pairing<V, L>::N> (&e)[Pairing<V, L>::P],
+                                               Vec<Pairing<V, L>::N> (&acc)[Pairing<V, L>::P]) {
+  using Q = Pairing<V, L>;
+  constexpr int N = Q::N, P = Q::P;
+  Vec<N> a[L][P], p1[L][P], p2[L][P], r1[L][P], r2[L][P], h[P];
+#pragma unroll
+  for (int j = 0; j < P; ++j) h[j] = in.h[j];
+  each_gate<T, V, L, kMask, kFar>(in.q, in.ig, in.rg, rate, [&](int l, int j, const Gates<N>& g, Vec<N> beta) {
+    const Vec<N> x = widen<N>(in.x[l], j);
+    Vec<N> inverse;  // dropped with beta
+#pragma unroll
+    for (int i = 0; i < N; ++i) inverse.v[i] = beta.v[i] > kTiny ? -rcp_approx(beta.v[i]) : 0.0f;
+    const Vec<N> ah = apply<kMask>(g.a, h[j], splat<N>(0.0f)), ix = g.i * x;
+    Vec<N> d = fma(g.a * (g.a * inverse), ix, ah);
+    if (kMask) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (g.a.v[i] == 0.0f || !((in.q.live >> l) & 1u)) d.v[i] = 0.0f;
+    }
+    a[l][j] = g.a;
+    p1[l][j] = beta * g.i;
+    p2[l][j] = fma(ix, splat<N>(-1.0f), x);
+    r1[l][j] = g.r * d;
+    r2[l][j] = rate[j] * (g.r + splat<N>(-1.0f));
+    h[j] = fma(beta, ix, ah);
+  });
+  const int64_t first = (o.b * p.steps + in.q.t0) * p.width + o.c;
+  const int step = o.dir * (int)p.width * (int)sizeof(T);
+  char *px = reinterpret_cast<char*>(static_cast<T*>(p.dx) + first),
+       *pi = reinterpret_cast<char*>(static_cast<T*>(p.dig) + first),
+       *pr = reinterpret_cast<char*>(static_cast<T*>(p.drg) + first);
 #pragma unroll
   for (int l = L - 1; l >= 0; --l) {
-    float dx[V], di[V], dr[V];
+    Vec<N> dx[P], di[P], dr[P];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float g = e[v] + widen(dy[l].v[v]), av = a[l][v], bv = be[l][v], xv = widen(x[l].v[v]);
-      const bool zero = kMask && av == 0.0f;
-      e[v] = zero ? 0.0f : av * g;
-      const bool dead = kMask && !((o.live >> l) & 1u);
-      dx[v] = dead ? 0.0f : g * bv * gi[l][v];
-      di[v] = dx[v] * xv * (1.0f - gi[l][v]);
-      const float slope = bv > 0.0f ? av * av * rcp_approx(bv) : 0.0f;
-      float dla = fmaf(e[v], hp[l][v], -g * gi[l][v] * xv * slope);
-      if (zero || dead) dla = 0.0f;
-      const float s = dla * gr[l][v];
-      acc[v] += s;
-      dr[v] = s * kd[v] * (1.0f - gr[l][v]);
+    for (int j = 0; j < P; ++j) {
+      const Vec<N> g = e[j] + widen<N>(in.dy[l], j);
+      e[j] = apply<kMask>(a[l][j], g, splat<N>(0.0f));
+      dx[j] = g * p1[l][j];
+      Vec<N> s = g * r1[l][j];
+      if (kMask) {  // (a gradient that is not finite is not spread to where nothing flows)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if (!((in.q.live >> l) & 1u)) dx[j].v[i] = 0.0f;
+          if (r1[l][j].v[i] == 0.0f) s.v[i] = 0.0f;
+        }
+      }
+      di[j] = dx[j] * p2[l][j];
+      acc[j] = acc[j] + s;
+      dr[j] = s * r2[l][j];
     }
-    if (o.on && ((o.inside >> l) & 1u)) {
-      const int64_t t = o.t0 + l * o.dir;
-      store<T, V, L>(p.dx, p, o.b, t, o.c, dx);
-      store<T, V, L>(p.dig, p, o.b, t, o.c, di);
-      store<T, V, L>(p.drg, p, o.b, t, o.c, dr);
+    if (o.on && (kFull || ((in.q.inside >> l) & 1u))) {
+      const int64_t at = (int64_t)step * l;
+      store<T, V, N>(px + at, dx);
+      store<T, V, N>(pi + at, di);
+      store<T, V, N>(pr + at, dr);
     }
   }
-  __syncthreads();
+}
+
+template <class T, int V, int L, bool kMask, bool kFar>
+__device__ __forceinline__ void backward_strip(const Args& p, const Lane& o,
+                                               const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P]) {
+  using Q = Pairing<V, L>;
+  constexpr int N = Q::N, P = Q::P;
+  if (o.count == 0) return;
+  constexpr bool kFull = !kMask;
+  const int whole = kMask ? o.count : o.whole;
+  LoadedBack<T, V, L> one, two;
+  Vec<N> e[P], acc[P];
 #pragma unroll
-  for (int v = 0; v < V; ++v) sE[warp][lane * V + v] = acc[v];
-  __syncthreads();
-  for (int k = warp * 32 + lane; k < C; k += warps * 32) {
-    const int64_t c = c0 + k;
-    if (c >= p.width) break;
-    float s = 0.0f;
-    for (int w = 0; w < warps; ++w) s += sE[w][k];
-    p.dpart[(o.b * p.tiles + o.tile) * p.width + c] = s;
+  for (int j = 0; j < P; ++j) e[j] = acc[j] = splat<N>(0.0f);
+  if (p.dlast) read_row<V, N>(p.dlast + o.b * p.width + o.from, e);
+  start_of<V, N, kMask>(p, o, e);
+  if (whole) read_back<T, V, L, kMask, kFull>(p, o, o.first + whole - 1, one);
+  if (whole < o.count) {
+    read_back<T, V, L, kMask, false>(p, o, o.first + whole, two);
+    backward_chunk<T, V, L, kMask, kFar, false>(p, o, two, rate, e, acc);
   }
+#pragma unroll 1
+  for (int k = whole - 1; k >= 0; k -= 2) {
+    read_back<T, V, L, kMask, kFull>(p, o, o.first + max(k - 1, 0), two);
+    backward_chunk<T, V, L, kMask, kFar, kFull>(p, o, one, rate, e, acc);
+    read_back<T, V, L, kMask, kFull>(p, o, o.first + max(k - 2, 0), one);
+    if (k >= 1) backward_chunk<T, V, L, kMask, kFar, kFull>(p, o, two, rate, e, acc);
+  }
+  if (!o.on) return;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    if (o.rank == p.strips - 1 && p.dstate) p.dstate[o.b * p.width + o.c + v] = e[v / N].v[v % N];
+    p.dpart[(o.b * p.strips + o.rank) * p.width + o.c + v] = acc[v / N].v[v % N];
+  }
+}
+
+template <class T, int V, int L, bool kMask>
+__global__ void __launch_bounds__(32 * kStrips) backward_kernel(const __grid_constant__ Args p) {
+  using Q = Pairing<V, L>;
+  const Lane o = lane_of<V, L, kMask, true>(p);
+  Vec<Q::N> rate[Q::P];
+  if (rates<V, Q::N>(p, o, rate))
+    backward_strip<T, V, L, kMask, true>(p, o, rate);
+  else
+    backward_strip<T, V, L, kMask, false>(p, o, rate);
 }
 
 struct Geometry {
-  int tiles, ctiles, warps, steps_per_thread, vec;
-  int64_t blocks;
+  int vec, chunk, ctiles, strips, strip;
 };
 
 template <class T>

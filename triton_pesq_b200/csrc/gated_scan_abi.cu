@@ -46,63 +46,80 @@ __global__ void __launch_bounds__(32 * kSumRows) decay_sum_kernel(const float* p
 
 size_t element(int dtype) { return dtype == PESQ_F32 ? 4 : 2; }
 
-bool even(const pesq_stream& s, const pesq_gated_scan_desc& d) {
-  return reinterpret_cast<uintptr_t>(s.data) % (2 * element(d.dtype)) == 0 &&
-         (d.batch == 1 || s.batch_stride % 2 == 0) && (d.steps == 1 || s.step_stride % 2 == 0);
-}
-
 int check(const pesq_gated_scan_desc* d) {
   if (!d) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL descriptor");
   if (d->batch < 1 || d->steps < 1 || d->width < 1)
     return set_error(PESQ_ERR_INVALID_ARGUMENT, "batch, steps and width must be at least 1");
   if (d->dtype < PESQ_F32 || d->dtype > PESQ_F16) return set_error(PESQ_ERR_INVALID_ARGUMENT, "unknown element type");
   if (!(d->rate > 0.0f) || d->rate > 1e6f) return set_error(PESQ_ERR_INVALID_ARGUMENT, "rate must be positive");
-  const int64_t most = INT64_C(0x7fffffff);
-  if (d->batch > most || d->width > most || d->steps > (most << 4) ||
-      (double)d->batch * (double)((d->width + 31) / 32) * (double)((d->steps + kTile - 1) / kTile) > (double)most)
-    return set_error(PESQ_ERR_UNSUPPORTED, "too many tiles for one launch");
+  if (d->batch > 65535 || d->width > (1 << 24) || d->steps > INT32_MAX - kChunk)
+    return set_error(PESQ_ERR_UNSUPPORTED, "more than 65535 rows, 2^24 channels or 2^31 steps in one call");
   return PESQ_OK;
 }
 
-// Vector width and tile of a call.  Pairs of channels when everything allows
-// it.  A row of at most kWarps steps gives each its own warp; a longer one
-// goes by tiles of kWarps * kSteps steps.
-Geometry geometry(const pesq_gated_scan_desc& d, int vec) {
+bool fits(const void* p, int vec, const pesq_gated_scan_desc& d) {
+  return reinterpret_cast<uintptr_t>(p) % (vec * element(d.dtype)) == 0;
+}
+bool fits(const pesq_stream& s, int vec, const pesq_gated_scan_desc& d) {
+  return fits(s.data, vec, d) && (d.batch == 1 || s.batch_stride % vec == 0) &&
+         (d.steps == 1 || s.step_stride % vec == 0);
+}
+
+// Warps that fill the device, and the fewest chunks of a strip
+constexpr int64_t kWarpsWanted = 148 * 8;
+constexpr int64_t kWarpsEnough = 148 * 4;
+constexpr int kFewestChunks = 4;
+
+// Pairs of channels where everything allows it (a backward call has its
+// forward's inputs, so takes its forward's).  One strip a row once rows and
+// channels make kWarpsEnough warps; otherwise as many as make kWarpsWanted.
+Geometry geometry(const pesq_gated_scan_desc& d) {
   Geometry g{};
-  g.vec = vec;
-  g.ctiles = (int)((d.width + 32 * vec - 1) / (32 * vec));
-  g.steps_per_thread = d.steps <= kWarps ? 1 : kSteps;
-  const int64_t warps = (d.steps + g.steps_per_thread - 1) / g.steps_per_thread;
-  g.warps = (int)std::min<int64_t>(warps, kWarps);
-  g.tiles = (int)((d.steps + (int64_t)g.warps * g.steps_per_thread - 1) / ((int64_t)g.warps * g.steps_per_thread));
-  g.blocks = d.batch * g.ctiles * g.tiles;
+  g.vec = d.width % 2 == 0 && fits(d.x, 2, d) && fits(d.input_gate, 2, d) && fits(d.decay_gate, 2, d) ? 2 : 1;
+  g.ctiles = (int)((d.width + 32 * g.vec - 1) / (32 * g.vec));
+  g.chunk = d.steps == 1 ? 1 : kChunk;
+  const int64_t chunks = (d.steps + g.chunk - 1) / g.chunk, warps = d.batch * g.ctiles;
+  int64_t strips = 1;
+  if (warps < kWarpsEnough)
+    strips = std::max<int64_t>(1, std::min((kWarpsWanted + warps - 1) / warps, chunks / kFewestChunks));
+  const int64_t per = (chunks + strips - 1) / strips;
+  g.strips = (int)((chunks + per - 1) / per);
+  g.strip = (int)(per * g.chunk);
   return g;
 }
 
-int64_t row_tiles(const pesq_gated_scan_desc& d) { return d.steps <= kTile ? 1 : (d.steps + kTile - 1) / kTile; }
-
-// [ticket, 16 bytes][end words][pair words][backward: partial decay sums]
-size_t words(const pesq_gated_scan_desc& d) {
-  const int64_t t = row_tiles(d);
-  return t == 1 ? 0 : (size_t)(d.batch * t * d.width) * 8;
+size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+// maps of strips and of CTAs of strips
+size_t map_bytes(const pesq_gated_scan_desc& d, const Geometry& g) {
+  return g.strips == 1 ? 0 : round16((size_t)(d.batch * (g.strips + (g.strips + kStrips - 1) / kStrips) * d.width) * 8);
 }
-size_t chain_bytes(const pesq_gated_scan_desc& d) {
-  const size_t w = words(d);
-  return w ? 16 + 2 * w : 0;
+size_t kept_bytes(const pesq_gated_scan_desc& d, const Geometry& g) {
+  return round16((size_t)(d.batch * ((d.steps + g.chunk - 1) / g.chunk) * d.width) * 4);
 }
-size_t need(const pesq_gated_scan_desc& d, bool backward) {
-  return chain_bytes(d) + (backward ? (size_t)(d.batch * row_tiles(d) * d.width) * 4 : 0);
+size_t part_bytes(const pesq_gated_scan_desc& d, const Geometry& g) {
+  return round16((size_t)(d.batch * g.strips * d.width) * 4);
 }
 
-int prepare(const pesq_gated_scan_desc& d, void* ws, size_t ws_bytes, bool backward, cudaStream_t stream, Args& a) {
+// [partial decay sums][maps][a row of zeros]
+size_t back_bytes(const pesq_gated_scan_desc& d, const Geometry& g) {
+  return part_bytes(d, g) + map_bytes(d, g) + round16(d.width * element(d.dtype));
+}
+
+// A step stride as the kernels take it: in bytes, 32 bits
+int narrow_stride(const pesq_stream& s, const pesq_gated_scan_desc& d, Stream& out) {
+  const int64_t bytes = d.steps == 1 ? 0 : s.step_stride * (int64_t)element(d.dtype);
+  if (bytes > INT32_MAX || bytes < -INT32_MAX)
+    return set_error(PESQ_ERR_UNSUPPORTED, "steps lie more than 2 GiB apart");
+  out = {s.data, s.batch_stride, (int)bytes};
+  return PESQ_OK;
+}
+
+int prepare(const pesq_gated_scan_desc& d, const Geometry& g, char* maps, Args& a) {
   if (!d.x.data || !d.input_gate.data || !d.decay_gate.data || !d.decay)
     return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL input");
-  const size_t bytes = need(d, backward);
-  if (bytes && (!ws || ws_bytes < bytes || reinterpret_cast<uintptr_t>(ws) % 16))
-    return set_error(PESQ_ERR_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
-  a.x = {d.x.data, d.x.batch_stride, d.x.step_stride};
-  a.ig = {d.input_gate.data, d.input_gate.batch_stride, d.input_gate.step_stride};
-  a.rg = {d.decay_gate.data, d.decay_gate.batch_stride, d.decay_gate.step_stride};
+  if (const int status = narrow_stride(d.x, d, a.x)) return status;
+  if (const int status = narrow_stride(d.input_gate, d, a.ig)) return status;
+  if (const int status = narrow_stride(d.decay_gate, d, a.rg)) return status;
   a.decay = d.decay;
   a.state = d.state;
   a.reset = d.reset;
@@ -114,23 +131,21 @@ int prepare(const pesq_gated_scan_desc& d, void* ws, size_t ws_bytes, bool backw
   a.width = d.width;
   a.reverse = d.reverse != 0;
   a.rate = d.rate;
-  a.spin_limit = d.spin_limit ? d.spin_limit : kSpinLimit;
-  const size_t w = words(d);
-  if (w) {
-    if (!d.error) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL error word");
-    a.error = d.error;
-    a.ticket = static_cast<unsigned*>(ws);
-    a.end = reinterpret_cast<unsigned long long*>(static_cast<char*>(ws) + 16);
-    a.pair = a.end + w / 8;
-    if (cudaMemsetAsync(ws, 0, 16 + 2 * w, stream) != cudaSuccess)
-      return set_error(PESQ_ERR_CUDA, cudaGetErrorString(cudaGetLastError()));
+  a.ctiles = g.ctiles;
+  a.strips = g.strips;
+  a.strip = g.strip;
+  if (g.strips > 1) {
+    a.before = reinterpret_cast<float2*>(maps);
+    a.total = a.before + d.batch * g.strips * d.width;
   }
   return PESQ_OK;
 }
 
-int run(const pesq_gated_scan_desc& d, Args& a, const Geometry& g, bool backward, cudaStream_t s) {
-  a.tiles = g.tiles;
-  a.ctiles = g.ctiles;
+bool missing(const void* p, size_t have, size_t want) {
+  return want && (!p || have < want || reinterpret_cast<uintptr_t>(p) % 16);
+}
+
+int run(const pesq_gated_scan_desc& d, const Args& a, const Geometry& g, bool backward, cudaStream_t s) {
   const bool mask = d.reset || d.lengths;
   const cudaError_t e = d.dtype == PESQ_F32    ? launch<float>(a, g, backward, mask, s)
                         : d.dtype == PESQ_BF16 ? launch<__nv_bfloat16>(a, g, backward, mask, s)
@@ -138,60 +153,71 @@ int run(const pesq_gated_scan_desc& d, Args& a, const Geometry& g, bool backward
   return e == cudaSuccess ? PESQ_OK : set_error(PESQ_ERR_CUDA, cudaGetErrorString(e));
 }
 
-bool aligned(const void* p, const pesq_gated_scan_desc& d) {
-  return reinterpret_cast<uintptr_t>(p) % (2 * element(d.dtype)) == 0;
-}
-
 }  // namespace
 
 extern "C" {
 
-int pesq_gated_scan_workspace(const pesq_gated_scan_desc* d, int backward, size_t* bytes) {
-  if (!bytes) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL argument");
+int pesq_gated_scan_sizes(const pesq_gated_scan_desc* d, size_t* forward, size_t* kept, size_t* backward) {
+  if (!forward || !kept || !backward) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL argument");
   if (const int status = check(d)) return status;
-  *bytes = need(*d, backward != 0);
+  const Geometry g = geometry(*d);
+  *forward = map_bytes(*d, g);
+  *kept = kept_bytes(*d, g);
+  *backward = back_bytes(*d, g);
   return PESQ_OK;
 }
 
-int pesq_gated_scan_forward(const pesq_gated_scan_desc* d, void* stream, void* y, float* last, void* workspace,
-                            size_t workspace_bytes) {
+int pesq_gated_scan_forward(const pesq_gated_scan_desc* d, void* stream, void* y, float* last, void* kept,
+                            size_t kept_size, void* workspace, size_t workspace_bytes) {
   if (const int status = check(d)) return status;
   if (!y || !last) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL output");
-  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const Geometry g = geometry(*d);
+  if (!fits(y, g.vec, *d)) return set_error(PESQ_ERR_INVALID_ARGUMENT, "y is less aligned than the inputs");
+  if (missing(workspace, workspace_bytes, map_bytes(*d, g)) || (kept && missing(kept, kept_size, kept_bytes(*d, g))))
+    return set_error(PESQ_ERR_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
   Args a{};
-  if (const int status = prepare(*d, workspace, workspace_bytes, false, s, a)) return status;
+  if (const int status = prepare(*d, g, static_cast<char*>(workspace), a)) return status;
   a.y = y;
   a.last = last;
-  const bool pairs = d->width % 2 == 0 && even(d->x, *d) && even(d->input_gate, *d) && even(d->decay_gate, *d) &&
-                     aligned(y, *d);
-  return run(*d, a, geometry(*d, pairs ? 2 : 1), false, s);
+  a.kept = static_cast<float*>(kept);
+  return run(*d, a, g, false, static_cast<cudaStream_t>(stream));
 }
 
-int pesq_gated_scan_backward(const pesq_gated_scan_desc* d, void* stream, const void* saved, size_t saved_bytes,
+int pesq_gated_scan_backward(const pesq_gated_scan_desc* d, void* stream, const void* kept, size_t kept_size,
                              pesq_stream dy, const float* dlast, void* dx, void* dinput_gate, void* ddecay_gate,
                              float* ddecay, float* dstate, void* workspace, size_t workspace_bytes) {
   if (const int status = check(d)) return status;
   if (!dx || !dinput_gate || !ddecay_gate || !ddecay) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL output");
-  if (chain_bytes(*d) && (!saved || saved_bytes < chain_bytes(*d) || reinterpret_cast<uintptr_t>(saved) % 16))
-    return set_error(PESQ_ERR_WORKSPACE, "the forward's workspace is missing or too small");
+  const Geometry g = geometry(*d);
+  if ((dy.data && !fits(dy, g.vec, *d)) || !fits(dx, g.vec, *d) || !fits(dinput_gate, g.vec, *d) ||
+      !fits(ddecay_gate, g.vec, *d))
+    return set_error(PESQ_ERR_INVALID_ARGUMENT, "a gradient is less aligned than the inputs");
+  if (missing(kept, kept_size, kept_bytes(*d, g)))
+    return set_error(PESQ_ERR_WORKSPACE, "the states that the forward kept are missing");
+  if (missing(workspace, workspace_bytes, back_bytes(*d, g)))
+    return set_error(PESQ_ERR_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   Args a{};
-  if (const int status = prepare(*d, workspace, workspace_bytes, true, s, a)) return status;
-  a.dy = {dy.data, dy.batch_stride, dy.step_stride};
+  char* ws = static_cast<char*>(workspace);
+  if (const int status = prepare(*d, g, ws + part_bytes(*d, g), a)) return status;
+  if (dy.data) {
+    if (const int status = narrow_stride(dy, *d, a.dy)) return status;
+  } else {  // one row of zeros for all steps
+    char* zeros = ws + part_bytes(*d, g) + map_bytes(*d, g);
+    if (cudaMemsetAsync(zeros, 0, d->width * element(d->dtype), s) != cudaSuccess)
+      return set_error(PESQ_ERR_CUDA, cudaGetErrorString(cudaGetLastError()));
+    a.dy = {zeros, 0, 0};
+  }
   a.dlast = dlast;
   a.dx = dx;
   a.dig = dinput_gate;
   a.drg = ddecay_gate;
   a.dstate = dstate;
-  a.dpart = reinterpret_cast<float*>(static_cast<char*>(workspace) + chain_bytes(*d));
-  if (words(*d)) a.start = reinterpret_cast<const unsigned long long*>(static_cast<const char*>(saved) + 16);
-  const bool pairs = d->width % 2 == 0 && even(d->x, *d) && even(d->input_gate, *d) && even(d->decay_gate, *d) &&
-                     (!dy.data || even(dy, *d)) && aligned(dx, *d) && aligned(dinput_gate, *d) &&
-                     aligned(ddecay_gate, *d);
-  const Geometry g = geometry(*d, pairs ? 2 : 1);
+  a.dpart = reinterpret_cast<float*>(ws);
+  a.kept = const_cast<float*>(static_cast<const float*>(kept));
   if (const int status = run(*d, a, g, true, s)) return status;
   decay_sum_kernel<<<(unsigned)((d->width + 31) / 32), dim3(32, kSumRows), 0, s>>>(
-      a.dpart, d->batch * g.tiles, d->width, d->decay, d->rate, ddecay);
+      a.dpart, d->batch * g.strips, d->width, d->decay, d->rate, ddecay);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? PESQ_OK : set_error(PESQ_ERR_CUDA, cudaGetErrorString(e));
 }

@@ -60,8 +60,20 @@ void check_float(const at::Tensor& t, const char* op, const char* name) {
               ".");
 }
 
-// channels adjacent
-at::Tensor rows(const at::Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+// channels adjacent, steps less than 2 GiB apart
+at::Tensor rows(const at::Tensor& t) {
+  const int64_t far = INT64_C(0x7fffffff) / t.element_size();
+  const bool near = t.size(1) <= 1 || (t.stride(1) <= far && t.stride(1) >= -far);
+  return near && (t.size(2) <= 1 || t.stride(2) == 1) ? t : t.contiguous();
+}
+
+// as aligned as a dense tensor (the pointer and every stride of more than one
+// element a multiple of 4 elements), or a copy that is
+at::Tensor aligned(const at::Tensor& t) {
+  const bool ok = reinterpret_cast<uintptr_t>(t.data_ptr()) % (4 * t.element_size()) == 0 &&
+                  (t.size(0) <= 1 || t.stride(0) % 4 == 0) && (t.size(1) <= 1 || t.stride(1) % 4 == 0);
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
 
 pesq_stream stream_of(const at::Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1)}; }
 
@@ -85,8 +97,7 @@ struct ScanCall {
   pesq_gated_scan_desc d{};
 
   ScanCall(const at::Tensor& x_, const at::Tensor& ig_, const at::Tensor& rg_, const at::Tensor& decay_,
-           const OptTensor& state_, const OptTensor& reset_, const OptTensor& lengths_, bool reverse, double rate,
-           const at::Tensor& error) {
+           const OptTensor& state_, const OptTensor& reset_, const OptTensor& lengths_, bool reverse, double rate) {
     check_cuda(x_, x_, kScan, "x");
     d.dtype = dtype_code(x_, kScan, "x");
     TORCH_CHECK(x_.dim() == 3, "The CUDA gated scan needs `x` [batch, step, channel], got ", x_.sizes(), ".");
@@ -101,9 +112,6 @@ struct ScanCall {
                 "The CUDA gated scan needs `x` and the gates in one type, got ", x_.scalar_type(), ", ",
                 ig_.scalar_type(), " and ", rg_.scalar_type(), ".");
     TORCH_CHECK_VALUE(rate > 0.0 && rate <= 1e6, "The CUDA gated scan needs a positive `rate`, got ", rate, ".");
-    TORCH_CHECK(error.is_cuda() && error.device() == x_.device() && error.scalar_type() == at::kInt &&
-                    error.numel() >= 1,
-                "The CUDA gated scan needs its error word on the inputs' device.");
     x = rows(x_);
     ig = rows(ig_);
     rg = rows(rg_);
@@ -142,21 +150,20 @@ struct ScanCall {
     d.input_gate = stream_of(ig);
     d.decay_gate = stream_of(rg);
     d.decay = decay.data_ptr<float>();
-    d.error = reinterpret_cast<uint32_t*>(error.data_ptr<int>());
   }
 
   bool empty() const { return d.batch == 0 || d.steps == 0 || d.width == 0; }
 };
 
+// (y, last, the states kept for the backward where `keep`)
 std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_scan_forward(const at::Tensor& x, const at::Tensor& ig,
                                                                   const at::Tensor& rg, const at::Tensor& decay,
                                                                   const OptTensor& state, const OptTensor& reset,
                                                                   const OptTensor& lengths, bool reverse, double rate,
-                                                                  const at::Tensor& error, int64_t spin_limit) {
-  ScanCall c(x, ig, rg, decay, state, reset, lengths, reverse, rate, error);
-  c.d.spin_limit = static_cast<uint32_t>(spin_limit);
+                                                                  bool keep) {
+  ScanCall c(x, ig, rg, decay, state, reset, lengths, reverse, rate);
   c10::cuda::CUDAGuard guard(x.device());
-  const auto f32 = x.options().dtype(at::kFloat);
+  const auto f32 = x.options().dtype(at::kFloat), bytes = x.options().dtype(at::kByte);
   at::Tensor y = at::empty(x.sizes(), x.options());
   at::Tensor last = at::empty({c.d.batch, c.d.width}, f32);
   if (c.empty()) {
@@ -165,23 +172,23 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_scan_forward(const at::Tens
     } else {
       last.zero_();
     }
-    return {y, last, at::empty({0}, f32.dtype(at::kByte))};
+    return {y, last, at::empty({0}, bytes)};
   }
-  size_t bytes = 0;
-  check_status(pesq_gated_scan_workspace(&c.d, 0, &bytes), "pesq_gated_scan_workspace");
-  at::Tensor ws = at::empty({static_cast<int64_t>(bytes)}, f32.dtype(at::kByte));
+  size_t work = 0, kept = 0, back = 0;
+  check_status(pesq_gated_scan_sizes(&c.d, &work, &kept, &back), "pesq_gated_scan_sizes");
+  at::Tensor states = at::empty({keep ? static_cast<int64_t>(kept) : 0}, bytes), ws;
+  if (work) ws = at::empty({static_cast<int64_t>(work)}, bytes);
   check_status(pesq_gated_scan_forward(&c.d, at::cuda::getCurrentCUDAStream(), y.data_ptr(), last.data_ptr<float>(),
-                                       ws.data_ptr(), bytes),
+                                       keep ? states.data_ptr() : nullptr, kept, work ? ws.data_ptr() : nullptr, work),
                "pesq_gated_scan_forward");
-  return {y, last, ws};
+  return {y, last, states};
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> gated_scan_backward(
     const at::Tensor& x, const at::Tensor& ig, const at::Tensor& rg, const at::Tensor& decay, const OptTensor& state,
-    const OptTensor& reset, const OptTensor& lengths, bool reverse, double rate, const at::Tensor& error,
-    int64_t spin_limit, const at::Tensor& saved, const OptTensor& dy_, const OptTensor& dlast_) {
-  ScanCall c(x, ig, rg, decay, state, reset, lengths, reverse, rate, error);
-  c.d.spin_limit = static_cast<uint32_t>(spin_limit);
+    const OptTensor& reset, const OptTensor& lengths, bool reverse, double rate, const at::Tensor& kept,
+    const OptTensor& dy_, const OptTensor& dlast_) {
+  ScanCall c(x, ig, rg, decay, state, reset, lengths, reverse, rate);
   c10::cuda::CUDAGuard guard(x.device());
   const auto f32 = x.options().dtype(at::kFloat);
   at::Tensor dx = at::empty(x.sizes(), x.options()), dig = at::empty(x.sizes(), x.options()),
@@ -202,15 +209,16 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> gated_sca
   pesq_stream dys{nullptr, 0, 0};
   if (dy_.has_value() && dy_->defined()) {
     dy = rows(dy_->to(x.scalar_type()));
+    if (x.size(2) % 2 == 0) dy = aligned(dy);
     dys = stream_of(dy);
   }
-  size_t bytes = 0;
-  check_status(pesq_gated_scan_workspace(&c.d, 1, &bytes), "pesq_gated_scan_workspace");
-  at::Tensor ws = at::empty({static_cast<int64_t>(bytes)}, f32.dtype(at::kByte));
-  check_status(pesq_gated_scan_backward(&c.d, at::cuda::getCurrentCUDAStream(), saved.data_ptr(), saved.numel(), dys,
+  size_t work = 0, states = 0, back = 0;
+  check_status(pesq_gated_scan_sizes(&c.d, &work, &states, &back), "pesq_gated_scan_sizes");
+  at::Tensor ws = at::empty({static_cast<int64_t>(back)}, f32.dtype(at::kByte));
+  check_status(pesq_gated_scan_backward(&c.d, at::cuda::getCurrentCUDAStream(), kept.data_ptr(), kept.numel(), dys,
                                         dlast.defined() ? dlast.data_ptr<float>() : nullptr, dx.data_ptr(),
                                         dig.data_ptr(), drg.data_ptr(), ddecay.data_ptr<float>(),
-                                        dstate.data_ptr<float>(), ws.data_ptr(), bytes),
+                                        dstate.data_ptr<float>(), ws.data_ptr(), back),
                "pesq_gated_scan_backward");
   return {dx, dig, drg, ddecay, dstate};
 }
@@ -231,28 +239,26 @@ const auto& scan_backward_op() {
 struct GatedScan : public torch::autograd::Function<GatedScan> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& ig, const at::Tensor& rg,
                                const at::Tensor& decay, const OptTensor& state, const OptTensor& reset,
-                               const OptTensor& lengths, bool reverse, double rate, const at::Tensor& error,
-                               int64_t spin_limit) {
+                               const OptTensor& lengths, bool reverse, double rate) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [y, last, ws] = scan_forward_op().call(x, ig, rg, decay, state, reset, lengths, reverse, rate, error, spin_limit);
+    auto [y, last, kept] = scan_forward_op().call(x, ig, rg, decay, state, reset, lengths, reverse, rate, true);
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({x, ig, rg, decay, state.value_or(at::Tensor()), reset.value_or(at::Tensor()),
-                            lengths.value_or(at::Tensor()), ws, error});
+                            lengths.value_or(at::Tensor()), kept});
     ctx->saved_data["reverse"] = reverse;
     ctx->saved_data["rate"] = rate;
-    ctx->saved_data["spin"] = spin_limit;
     return {y, last};
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     no_second_derivative(kScan);
     const auto s = ctx->get_saved_variables();
-    variable_list out(11);
+    variable_list out(9);
     if (!g[0].defined() && !g[1].defined()) return out;
     auto [dx, dig, drg, ddecay, dstate] = scan_backward_op().call(
         s[0], s[1], s[2], s[3], optional_of(s[4]), optional_of(s[5]), optional_of(s[6]),
-        ctx->saved_data["reverse"].toBool(), ctx->saved_data["rate"].toDouble(), s[8], ctx->saved_data["spin"].toInt(),
-        s[7], optional_of(g[0]), optional_of(g[1]));
+        ctx->saved_data["reverse"].toBool(), ctx->saved_data["rate"].toDouble(), s[7], optional_of(g[0]),
+        optional_of(g[1]));
     out[0] = dx;
     out[1] = dig;
     out[2] = drg;
@@ -264,15 +270,14 @@ struct GatedScan : public torch::autograd::Function<GatedScan> {
 
 std::tuple<at::Tensor, at::Tensor> gated_scan(const at::Tensor& x, const at::Tensor& ig, const at::Tensor& rg,
                                               const at::Tensor& decay, const OptTensor& state, const OptTensor& reset,
-                                              const OptTensor& lengths, bool reverse, double rate,
-                                              const at::Tensor& error, int64_t spin_limit) {
+                                              const OptTensor& lengths, bool reverse, double rate) {
   check_cuda(x, x, kScan, "x");
   if (at::GradMode::is_enabled() &&
       (wants_grad(x) || wants_grad(ig) || wants_grad(rg) || wants_grad(decay) || wants_grad(state))) {
-    auto out = GatedScan::apply(x, ig, rg, decay, state, reset, lengths, reverse, rate, error, spin_limit);
+    auto out = GatedScan::apply(x, ig, rg, decay, state, reset, lengths, reverse, rate);
     return {out[0], out[1]};
   }
-  auto [y, last, ws] = scan_forward_op().call(x, ig, rg, decay, state, reset, lengths, reverse, rate, error, spin_limit);
+  auto [y, last, kept] = scan_forward_op().call(x, ig, rg, decay, state, reset, lengths, reverse, rate, false);
   return {y, last};
 }
 
@@ -281,11 +286,11 @@ std::tuple<at::Tensor, at::Tensor> gated_scan(const at::Tensor& x, const at::Ten
 TORCH_LIBRARY_FRAGMENT(pesq_cuda, m) {
   const char* scan_in =
       "(Tensor x, Tensor input_gate, Tensor decay_gate, Tensor decay, Tensor? state, Tensor? reset, Tensor? lengths, "
-      "bool reverse, float rate, Tensor error, int spin_limit";
+      "bool reverse, float rate";
   m.def((std::string("gated_scan") + scan_in + ") -> (Tensor, Tensor)").c_str());
-  m.def((std::string("gated_scan_forward") + scan_in + ") -> (Tensor, Tensor, Tensor)").c_str());
+  m.def((std::string("gated_scan_forward") + scan_in + ", bool keep) -> (Tensor, Tensor, Tensor)").c_str());
   m.def((std::string("gated_scan_backward") + scan_in +
-         ", Tensor saved, Tensor? dy, Tensor? dlast) -> (Tensor, Tensor, Tensor, Tensor, Tensor)")
+         ", Tensor kept, Tensor? dy, Tensor? dlast) -> (Tensor, Tensor, Tensor, Tensor, Tensor)")
             .c_str());
 }
 

@@ -58,6 +58,57 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return y;
 }
 
+// N floats worked on together; pairs go through the two-wide float instructions
+// (half the issue slots of the scalar ones)
+template <int N>
+struct Vec {
+  float v[N];
+};
+template <int N>
+__device__ __forceinline__ Vec<N> splat(float x) {
+  Vec<N> r;
+#pragma unroll
+  for (int j = 0; j < N; ++j) r.v[j] = x;
+  return r;
+}
+__device__ __forceinline__ unsigned long long bits(Vec<2> a) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.v[0]), "f"(a.v[1]));
+  return r;
+}
+__device__ __forceinline__ Vec<2> pair(unsigned long long a) {
+  Vec<2> r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.v[0]), "=f"(r.v[1]) : "l"(a));
+  return r;
+}
+__device__ __forceinline__ Vec<2> fma(Vec<2> a, Vec<2> b, Vec<2> c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+  return pair(r);
+}
+__device__ __forceinline__ Vec<2> operator*(Vec<2> a, Vec<2> b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+  return pair(r);
+}
+__device__ __forceinline__ Vec<2> operator+(Vec<2> a, Vec<2> b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+  return pair(r);
+}
+__device__ __forceinline__ Vec<1> fma(Vec<1> a, Vec<1> b, Vec<1> c) { return {{fmaf(a.v[0], b.v[0], c.v[0])}}; }
+__device__ __forceinline__ Vec<1> operator*(Vec<1> a, Vec<1> b) { return {{a.v[0] * b.v[0]}}; }
+__device__ __forceinline__ Vec<1> operator+(Vec<1> a, Vec<1> b) { return {{a.v[0] + b.v[0]}}; }
+
+// elements N j .. N j + N - 1 of a pack, in float
+template <int N, class T, int M>
+__device__ __forceinline__ Vec<N> widen(const Pack<T, M>& p, int j) {
+  Vec<N> r;
+#pragma unroll
+  for (int n = 0; n < N; ++n) r.v[n] = widen(p.v[N * j + n]);
+  return r;
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 

@@ -8,8 +8,9 @@ Per row and channel, in scan order::
     log a = -rate * softplus(decay) * r
     h = a * h + sqrt(1 - a**2) * i * x,   y = h
 
-One pass over the data in each direction (csrc/gated_scan.cuh); the state, the
-gates and every sum are float32 whatever the streams' type.  A call of one step
+Rows and channels side by side, and steps in strips where those are few
+(csrc/gated_scan.cuh); the state, the gates and every sum are float32 whatever
+the streams' type, and a result is the same, to the last bit, every time.  A call of one step
 with ``state`` is the streaming form.  The reference has fixed-coefficient
 recurrences only (torch_pesq/triton_ops/iir.py).
 """
@@ -17,18 +18,13 @@ recurrences only (torch_pesq/triton_ops/iir.py).
 from __future__ import annotations
 
 import math
-from typing import Dict, Optional, Tuple
+from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
 
-__all__ = ["gated_scan", "gated_scan_errors", "GatedScanCuda"]
-
-#: device index -> int32 word that a wait which gave up sets
-_errors: Dict[int, torch.Tensor] = {}
-#: polls a look-back wait makes before it gives up (0: the library's default, about 0.1 s)
-spin_limit = 0
+__all__ = ["gated_scan", "GatedScanCuda"]
 
 _op = None
 
@@ -39,16 +35,6 @@ def _load():
         _lib.load_ops()
         _op = torch.ops.pesq_cuda.gated_scan.default
     return _op
-
-
-def _error_word(device: torch.device) -> torch.Tensor:
-    word = _errors.get(device.index)
-    if word is None:
-        if device.type != "cuda":
-            raise RuntimeError("The CUDA gated scan needs `x` to live on a GPU.")
-        with torch.inference_mode(False):  # (it is saved for backward passes too)
-            word = _errors[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
-    return word
 
 
 def gated_scan(x: torch.Tensor, input_gate: torch.Tensor, decay_gate: torch.Tensor, decay: torch.Tensor,
@@ -88,20 +74,7 @@ def gated_scan(x: torch.Tensor, input_gate: torch.Tensor, decay_gate: torch.Tens
     op = _op or _load()
     if not isinstance(x, torch.Tensor):
         raise TypeError("`x` must be a torch.Tensor")
-    return op(x, input_gate, decay_gate, decay, state, reset, lengths, reverse, rate, _error_word(x.device), spin_limit)
-
-
-def gated_scan_errors(device: Optional[torch.device] = None) -> int:
-    """Synchronise and return (and clear) a device's error word: nonzero if a
-    tile of an earlier call gave up waiting for its predecessor."""
-
-    index = torch.device("cuda" if device is None else device).index
-    word = _errors.get(torch.cuda.current_device() if index is None else index)
-    if word is None:
-        return 0
-    value = int(word.item())
-    word.zero_()
-    return value
+    return op(x, input_gate, decay_gate, decay, state, reset, lengths, reverse, rate)
 
 
 class GatedScanCuda(torch.nn.Module):
@@ -152,11 +125,6 @@ class GatedScanCuda(torch.nn.Module):
 
         y, last = self(x.unsqueeze(1), input_gate.unsqueeze(1), decay_gate.unsqueeze(1), state)
         return y.squeeze(1), last
-
-    def check_errors(self) -> int:
-        """Synchronise and return the error word of the parameter's device."""
-
-        return gated_scan_errors(self.decay.device)
 
     def extra_repr(self) -> str:
         return f"channels={self.channels}, rate={self.rate}, reverse={self.reverse}"
