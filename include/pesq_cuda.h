@@ -387,6 +387,11 @@ int pesq_gated_scan_backward(const pesq_gated_scan_desc* desc, void* stream, con
                              pesq_stream dy, const float* dlast, void* dx, void* dinput_gate, void* ddecay_gate,
                              float* ddecay, float* dstate, void* workspace, size_t workspace_bytes);
 
+/* Synchronises `stream`, then reads and clears the current device's error
+ * word: nonzero when a copy of an earlier call did not come in time (a bounded
+ * wait that ran out; that call's results are then wrong). */
+int pesq_gated_scan_check(void* stream, uint32_t* failed);
+
 #ifdef __cplusplus
 }
 #endif

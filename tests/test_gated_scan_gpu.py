@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import train_reference as R
-from triton_pesq_b200 import GatedScanCuda, gated_scan
+from triton_pesq_b200 import GatedScanCuda, _lib, gated_scan
 
 pytestmark = pytest.mark.gpu
 
@@ -60,6 +60,7 @@ def compare(tensors, dy, dlast, device, reset=None, lengths=None, reverse=False,
     for name, g, w, t in zip([n for n, t in zip(NAMES, tensors) if t is not None], got, want, leaves):
         assert g.dtype == t.dtype
         R.close(g, torch.zeros(g.shape, dtype=torch.float64) if w is None else w, GTOL, "d " + name)
+    assert _lib.gated_scan_check() == 0
 
 
 SHAPES = [(1, 1, 1), (3, 1, 70), (2, 2, 33), (2, 8, 64), (1, 9, 66), (2, 64, 31), (1, 65, 129), (3, 130, 40),
@@ -229,6 +230,7 @@ def test_pieces_and_single_steps_continue_a_sequence(cuda_device):
         for t in range(5):
             y, s = module.step(dev[0][:, t], dev[1][:, t], dev[2][:, t], s)
             R.close(y, want[:, t].double(), TOL, "step")
+    assert module.check_errors() == 0
 
 
 def test_empty_sizes(cuda_device):

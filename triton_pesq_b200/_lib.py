@@ -258,6 +258,7 @@ SIGNATURES = {
          ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
          ctypes.c_size_t],
     ),
+    "pesq_gated_scan_check": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint32)]),
 }
 
 
@@ -563,4 +564,12 @@ def iir_check(handle: int, stream: int = 0) -> int:
     failed = ctypes.c_uint32(0)
     check(library().pesq_iir_check(ctypes.c_void_p(handle), ctypes.c_void_p(stream), ctypes.byref(failed)),
           "pesq_iir_check")
+    return int(failed.value)
+
+
+def gated_scan_check(stream: int = 0) -> int:
+    """Synchronise ``stream`` and return (and clear) the current device's gated scan error word."""
+
+    failed = ctypes.c_uint32(0)
+    check(library().pesq_gated_scan_check(ctypes.c_void_p(stream), ctypes.byref(failed)), "pesq_gated_scan_check")
     return int(failed.value)

@@ -12,8 +12,13 @@
 // and walks the strip in chunks of kChunk steps with the state in registers:
 // everything of a step but one multiply-add is independent of the steps before it,
 // so a chunk's gates are worked out side by side, while the elements of the chunks
-// to come are on their way.  Warps wait for nobody: no barrier, no flag, no
+// to come are on their way.  Warps wait for nobody but their own copies: no flag, no
 // atomic, and the order of every operation is fixed.
+//
+// Elements come in two ways.  Where channels and strides allow (multiples of 16
+// bytes), a warp's chunks are boxes of 64 channels x 8 steps that tensor copies bring to
+// a ring in shared memory: one instruction for a box, no registers held, and two or three
+// chunks in flight.  Otherwise every lane loads its own elements a chunk ahead.
 //
 // With rows and channels enough to fill the device a strip is the whole row,
 // and the data pass once.  Otherwise rows are cut into strips: the recurrence is
@@ -33,7 +38,10 @@
 // zero: the term is dropped there.
 #pragma once
 
+#include <cuda.h>
+
 #include "../../include/pesq_cuda.h"
+#include "common.cuh"
 #include "train.cuh"
 
 namespace pesq {
@@ -43,6 +51,9 @@ using namespace train;
 
 constexpr int kChunk = 8;   // steps of a chunk
 constexpr int kStrips = 8;  // strips (warps) of a CTA, where rows are cut
+// chunks of a warp in shared memory: what 8 warps' chunks of four 32-bit streams leave room for
+template <class T>
+constexpr int kRing = sizeof(T) == 2 ? 4 : 3;
 
 struct Stream {
   const void* p;
@@ -75,6 +86,12 @@ struct Args {
   void *dx, *dig, *drg;
   float* dstate;
   float* dpart;               // [batch * strips, width] sums of dlog a r
+  uint32_t* error;            // set when a copy does not come
+};
+
+// Tensor maps of the streams: [batch][step][channel], boxes of 1 x kChunk x 64
+struct Maps {
+  CUtensorMap rg, ig, x, dy;
 };
 
 // softplus(v): log1p(e) = 2 artanh(e / (2 + e)) by its series, e = exp(-|v|)
@@ -422,6 +439,110 @@ __device__ __forceinline__ void join_maps(const Args& p, const Lane& o, const Ve
   }
 }
 
+// Takes n chunks in turn, each read one before its use: read(k, in) and
+// work(k, in) for k = 0 .. n - 1.  (The last reads are repeated rather than
+// branched around: a join would wait for them.)
+template <class In, class R, class W>
+__device__ __forceinline__ void walk(int n, R read, W work) {
+  if (n <= 0) return;
+  In one, two;
+  read(0, one);
+#pragma unroll 1
+  for (int k = 0; k < n; k += 2) {
+    read(min(k + 1, n - 1), two);
+    work(k, one);
+    read(min(k + 2, n - 1), one);
+    if (k + 1 < n) work(k + 1, two);
+  }
+}
+
+// A warp's ring of chunks in shared memory: kRing stages of S streams' boxes
+// [kChunk][64] and, with kState, the 64 states before the chunk.
+template <class T, int S, bool kState>
+struct Ring {
+  static constexpr int kBox = kChunk * 64 * (int)sizeof(T);
+  static constexpr int kStage = S * kBox + (kState ? 256 : 0);
+  static constexpr int kBytes = kRing<T> * kStage;  // of a warp
+  char* base;
+  uint64_t* bar;
+  const CUtensorMap* map[S];
+
+  __device__ __forceinline__ Ring(char* smem, uint64_t* bars)
+      : base(smem + threadIdx.y * kBytes), bar(bars + threadIdx.y * kRing<T>) {
+    if (threadIdx.x == 0) {
+#pragma unroll
+      for (int i = 0; i < kRing<T>; ++i) mbar_init(bar + i);
+    }
+    __syncwarp();
+  }
+  // one lane
+  __device__ __forceinline__ void send(const Args& p, const Lane& o, int k, int stage) {
+    const int c0 = (int)o.c, t0 = p.reverse ? (int)p.steps - (k + 1) * kChunk : k * kChunk;
+    char* to = base + stage * kStage;
+    uint32_t bytes = S * kBox, state = 0;
+    if (kState) state = (uint32_t)min((int64_t)64, p.width - o.c) * 4, bytes += state;
+    mbar_arrive_expect_tx(bar + stage, bytes);
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+      asm volatile(
+          "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+              smem_u32(to + i * kBox)),
+          "l"(map[i]), "r"(smem_u32(bar + stage)), "r"(c0), "r"(t0), "r"((int)o.b)
+          : "memory");
+    if (kState)
+      bulk_g2s(to + S * kBox, p.kept + (o.b * ((p.steps + kChunk - 1) / kChunk) + k) * p.width + o.c, state, bar + stage);
+  }
+  // one stream of the stage, in scan order
+  __device__ __forceinline__ void get(const Args& p, int stage, int i, Pack<T, 2> (&out)[kChunk]) const {
+    const Pack<T, 2>* s = reinterpret_cast<const Pack<T, 2>*>(base + stage * kStage + i * kBox) + threadIdx.x;
+    const int step = p.reverse ? -32 : 32;
+    s += p.reverse ? 7 * 32 : 0;
+#pragma unroll
+    for (int l = 0; l < kChunk; ++l) out[l] = s[l * step];
+  }
+  __device__ __forceinline__ Pack<float, 2> state(int stage) const {
+    return reinterpret_cast<const Pack<float, 2>*>(base + stage * kStage + S * kBox)[threadIdx.x];
+  }
+  // Chunks first, first + way, ...: read(stage, k, in) takes a chunk out of its stage, work(k, in)
+  // works on it while the stage fills again.  Returns false where a copy does not come.
+  template <class In, class R, class W>
+  __device__ __forceinline__ bool walk(const Args& p, const Lane& o, int first, int n, int way, R read, W work) {
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < kRing<T> && i < n; ++i) send(p, o, first + way * i, i);
+    }
+    int stage = 0, parity = 0;
+    bool ok = true;
+#pragma unroll 1
+    for (int k = 0; k < n; ++k) {
+      if (!__all_sync(0xffffffffu, mbar_wait(bar + stage, parity))) {
+        ok = false;
+        break;
+      }
+      In in;
+      read(stage, first + way * k, in);
+      __syncwarp();
+      if (threadIdx.x == 0 && k + kRing<T> < n) send(p, o, first + way * (k + kRing<T>), stage);
+      work(first + way * k, in);
+      if (++stage == kRing<T>) stage = 0, parity ^= 1;
+    }
+    if (!ok) {  // nothing may be in flight to shared memory that another block gets
+      if (threadIdx.x == 0) atomicOr(p.error, 1u);
+      for (int i = 0; i < kRing<T>; ++i) mbar_wait(bar + i, i < stage ? parity ^ 1 : parity);
+    }
+    return ok;
+  }
+};
+
+// Steps of a ring's chunk that are not live: as load() leaves them
+template <class T, int V, int L>
+__device__ __forceinline__ void blank(Pack<T, V> (&out)[L], const Chunk& q, float other = 0.0f) {
+#pragma unroll
+  for (int l = 0; l < L; ++l)
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (!((q.live >> l) & 1u)) out[l].v[v] = narrow<T>(other);
+}
+
 // ------------------------------------------------------------------- forward
 
 template <class T, int V, int L>
@@ -438,36 +559,67 @@ __device__ __forceinline__ void read_chunk(const Args& p, const Lane& o, int k, 
   load<T, V, L, kFull>(in.x, p.x, o, in.q);
 }
 
-template <class T, int V, int L, bool kMask, bool kFar>
-__device__ __forceinline__ void forward_maps(const Args& p, const Lane& o,
+template <class T, bool kMask>
+__device__ __forceinline__ void ring_chunk(const Args& p, const Lane& o, const Ring<T, 3, false>& ring, int stage, int k,
+                                           int whole, Loaded<T, 2, kChunk>& in) {
+  in.q = chunk_of<kChunk, kMask>(p, o, k);
+  ring.get(p, stage, 0, in.rg);
+  ring.get(p, stage, 1, in.ig);
+  ring.get(p, stage, 2, in.x);
+  if (kMask || k - o.first >= whole) {
+    blank(in.rg, in.q, kShut);
+    blank(in.ig, in.q);
+    blank(in.x, in.q);
+  }
+}
+
+template <class T, int V, int L, bool kMask, bool kFar, bool kBulk>
+__device__ __forceinline__ void forward_maps(const Args& p, const Maps& m, const Lane& o,
                                              const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P]) {
   using Q = Pairing<V, L>;
   constexpr int N = Q::N, P = Q::P;
   Vec<N> A[P], H[P];
 #pragma unroll
   for (int j = 0; j < P; ++j) A[j] = splat<N>(1.0f), H[j] = splat<N>(0.0f);
-#pragma unroll 1
-  for (int k = 0; k < o.count; ++k) {
-    Loaded<T, V, L> in;
-    read_chunk<T, V, L, kMask, false>(p, o, o.first + k, in);
+  const auto work = [&](int, const Loaded<T, V, L>& in) {
     each_gate<T, V, L, kMask, kFar>(in.q, in.ig, in.rg, rate, [&](int l, int j, const Gates<N>& g, Vec<N> beta) {
       H[j] = apply<kMask>(g.a, H[j], beta * (g.i * widen<N>(in.x[l], j)));
       A[j] = A[j] * g.a;
     });
+  };
+  const int whole = kMask ? o.count : o.whole;
+  if constexpr (kBulk) {
+    extern __shared__ __align__(128) char dynamic[];
+    __shared__ uint64_t s_bar[kStrips * kRing<T>];
+    Ring<T, 3, false> ring(dynamic, s_bar);
+    ring.map[0] = &m.rg, ring.map[1] = &m.ig, ring.map[2] = &m.x;
+    ring.template walk<Loaded<T, V, L>>(
+        p, o, o.first, o.count, 1,
+        [&](int stage, int k, Loaded<T, V, L>& in) { ring_chunk<T, kMask>(p, o, ring, stage, k, whole, in); },
+        [&](int k, const Loaded<T, V, L>& in) { work(k, in); });
+  } else {
+    walk<Loaded<T, V, L>>(
+        whole, [&](int k, Loaded<T, V, L>& in) { read_chunk<T, V, L, kMask, !kMask>(p, o, o.first + k, in); }, work);
+    if (whole < o.count) {
+      Loaded<T, V, L> in;
+      read_chunk<T, V, L, kMask, false>(p, o, o.first + whole, in);
+      work(0, in);
+    }
   }
   join_maps<V, N, kMask>(p, o, A, H);
 }
 
-template <class T, int V, int L, bool kMask>
-__global__ void __launch_bounds__(32 * kStrips) forward_maps_kernel(const __grid_constant__ Args p) {
+template <class T, int V, int L, bool kMask, bool kBulk>
+__global__ void __launch_bounds__(32 * kStrips) forward_maps_kernel(const __grid_constant__ Args p,
+                                                              const __grid_constant__ Maps m) {
   using Q = Pairing<V, L>;
   const Lane o = lane_of<V, L, kMask, false>(p);
   Vec<Q::N> rate[Q::P];
   // (the CTA's warps share their channels, so they agree, and meet in join_maps)
   if (rates<V, Q::N>(p, o, rate))
-    forward_maps<T, V, L, kMask, true>(p, o, rate);
+    forward_maps<T, V, L, kMask, true, kBulk>(p, m, o, rate);
   else
-    forward_maps<T, V, L, kMask, false>(p, o, rate);
+    forward_maps<T, V, L, kMask, false, kBulk>(p, m, o, rate);
 }
 
 template <class T, int V, int L, bool kMask, bool kFar, bool kFull>
@@ -491,33 +643,45 @@ __device__ __forceinline__ void forward_chunk(const Args& p, const Lane& o, int 
   });
 }
 
-template <class T, int V, int L, bool kMask, bool kFar>
-__device__ __forceinline__ void forward_strip(const Args& p, const Lane& o,
+template <class T, int V, int L, bool kMask, bool kFar, bool kBulk>
+__device__ __forceinline__ void forward_strip(const Args& p, const Maps& m, const Lane& o,
                                               const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P]) {
   using Q = Pairing<V, L>;
   constexpr int N = Q::N, P = Q::P;
   if (o.count == 0) return;
-  // whole chunks two at a time, each read while the one before it is worked on;
-  // then the row's last steps (with masks every chunk may be partial)
-  constexpr bool kFull = !kMask;
-  const int whole = kMask ? o.count : o.whole;
-  Loaded<T, V, L> one, two;
-  if (whole) read_chunk<T, V, L, kMask, kFull>(p, o, o.first, one);
   Vec<N> h[P];
 #pragma unroll
   for (int j = 0; j < P; ++j) h[j] = splat<N>(0.0f);
   if (p.state) read_row<V, N>(p.state + o.b * p.width + o.from, h);
   start_of<V, N, kMask>(p, o, h);
-#pragma unroll 1
-  for (int k = 0; k < whole; k += 2) {
-    read_chunk<T, V, L, kMask, kFull>(p, o, o.first + min(k + 1, whole - 1), two);
-    forward_chunk<T, V, L, kMask, kFar, kFull>(p, o, o.first + k, one, rate, h);
-    read_chunk<T, V, L, kMask, kFull>(p, o, o.first + min(k + 2, whole - 1), one);
-    if (k + 1 < whole) forward_chunk<T, V, L, kMask, kFar, kFull>(p, o, o.first + k + 1, two, rate, h);
-  }
-  if (whole < o.count) {
-    read_chunk<T, V, L, kMask, false>(p, o, o.first + whole, one);
-    forward_chunk<T, V, L, kMask, kFar, false>(p, o, o.first + whole, one, rate, h);
+  // whole chunks, then the row's last steps (with masks every chunk may be partial)
+  const int whole = kMask ? o.count : o.whole;
+  if constexpr (kBulk) {
+    extern __shared__ __align__(128) char dynamic[];
+    __shared__ uint64_t s_bar[kStrips * kRing<T>];
+    Ring<T, 3, false> ring(dynamic, s_bar);
+    ring.map[0] = &m.rg, ring.map[1] = &m.ig, ring.map[2] = &m.x;
+    if (!ring.template walk<Loaded<T, V, L>>(
+            p, o, o.first, o.count, 1,
+            [&](int stage, int k, Loaded<T, V, L>& in) { ring_chunk<T, kMask>(p, o, ring, stage, k, whole, in); },
+            [&](int k, const Loaded<T, V, L>& in) {
+              if (kMask || k - o.first < whole)
+                forward_chunk<T, V, L, kMask, kFar, !kMask>(p, o, k, in, rate, h);
+              else
+                forward_chunk<T, V, L, kMask, kFar, false>(p, o, k, in, rate, h);
+            }))
+      return;
+  } else {
+    walk<Loaded<T, V, L>>(
+        whole, [&](int k, Loaded<T, V, L>& in) { read_chunk<T, V, L, kMask, !kMask>(p, o, o.first + k, in); },
+        [&](int k, const Loaded<T, V, L>& in) {
+          forward_chunk<T, V, L, kMask, kFar, !kMask>(p, o, o.first + k, in, rate, h);
+        });
+    if (whole < o.count) {
+      Loaded<T, V, L> in;
+      read_chunk<T, V, L, kMask, false>(p, o, o.first + whole, in);
+      forward_chunk<T, V, L, kMask, kFar, false>(p, o, o.first + whole, in, rate, h);
+    }
   }
   if (o.rank == p.strips - 1 && o.on) {
 #pragma unroll
@@ -525,59 +689,95 @@ __device__ __forceinline__ void forward_strip(const Args& p, const Lane& o,
   }
 }
 
-template <class T, int V, int L, bool kMask>
-__global__ void __launch_bounds__(32 * kStrips) forward_kernel(const __grid_constant__ Args p) {
+template <class T, int V, int L, bool kMask, bool kBulk>
+__global__ void __launch_bounds__(32 * kStrips) forward_kernel(const __grid_constant__ Args p,
+                                                              const __grid_constant__ Maps m) {
   using Q = Pairing<V, L>;
   const Lane o = lane_of<V, L, kMask, false>(p);
   Vec<Q::N> rate[Q::P];
   if (rates<V, Q::N>(p, o, rate))
-    forward_strip<T, V, L, kMask, true>(p, o, rate);
+    forward_strip<T, V, L, kMask, true, kBulk>(p, m, o, rate);
   else
-    forward_strip<T, V, L, kMask, false>(p, o, rate);
+    forward_strip<T, V, L, kMask, false, kBulk>(p, m, o, rate);
 }
 
 // ------------------------------------------------------------------ backward
 
+template <class T, int V, int L>
+struct LoadedMap {
+  Chunk q;
+  Pack<T, V> rg[L], dy[L];
+};
+
+template <class T, int V, int L, bool kMask, bool kFull>
+__device__ __forceinline__ void read_map(const Args& p, const Lane& o, int k, LoadedMap<T, V, L>& in) {
+  in.q = chunk_of<L, kMask>(p, o, k);
+  load<T, V, L, kFull>(in.rg, p.rg, o, in.q, kShut);
+  load<T, V, L, kFull>(in.dy, p.dy, o, in.q);
+}
+
 // e -> A e + E of a strip, from its last step to its first: the decay gate and
 // dy are all it takes
-template <class T, int V, int L, bool kMask, bool kFar>
-__device__ __forceinline__ void backward_maps(const Args& p, const Lane& o,
+template <class T, int V, int L, bool kMask, bool kFar, bool kBulk>
+__device__ __forceinline__ void backward_maps(const Args& p, const Maps& m, const Lane& o,
                                               const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P]) {
   using Q = Pairing<V, L>;
   constexpr int N = Q::N, P = Q::P;
   Vec<N> A[P], E[P];
 #pragma unroll
   for (int j = 0; j < P; ++j) A[j] = splat<N>(1.0f), E[j] = splat<N>(0.0f);
-#pragma unroll 1
-  for (int k = o.count - 1; k >= 0; --k) {
-    const Chunk q = chunk_of<L, kMask>(p, o, o.first + k);
-    Pack<T, V> rg[L], dy[L];
-    load<T, V, L, false>(rg, p.rg, o, q, kShut);
-    load<T, V, L, false>(dy, p.dy, o, q);
+  const auto work = [&](int, LoadedMap<T, V, L>& in) {
 #pragma unroll
     for (int l = L - 1; l >= 0; --l) {
-      hold(rg[l]);
+      hold(in.rg[l]);
 #pragma unroll
       for (int j = 0; j < P; ++j) {
-        Vec<N> a = decay_of<kFar, N>(widen<N>(rg[l], j), rate[j]);
-        if (kMask && ((q.cut >> l) & 1u)) a = splat<N>(0.0f);
-        E[j] = apply<kMask>(a, E[j] + widen<N>(dy[l], j), splat<N>(0.0f));
+        Vec<N> a = decay_of<kFar, N>(widen<N>(in.rg[l], j), rate[j]);
+        if (kMask && ((in.q.cut >> l) & 1u)) a = splat<N>(0.0f);
+        E[j] = apply<kMask>(a, E[j] + widen<N>(in.dy[l], j), splat<N>(0.0f));
         A[j] = A[j] * a;
       }
     }
+  };
+  const int whole = kMask ? o.count : o.whole;
+  if constexpr (kBulk) {
+    extern __shared__ __align__(128) char dynamic[];
+    __shared__ uint64_t s_bar[kStrips * kRing<T>];
+    Ring<T, 2, false> ring(dynamic, s_bar);
+    ring.map[0] = &m.rg, ring.map[1] = &m.dy;
+    ring.template walk<LoadedMap<T, V, L>>(
+        p, o, o.first + o.count - 1, o.count, -1,
+        [&](int stage, int k, LoadedMap<T, V, L>& in) {
+          in.q = chunk_of<L, kMask>(p, o, k);
+          ring.get(p, stage, 0, in.rg);
+          ring.get(p, stage, 1, in.dy);
+          if (kMask || k - o.first >= whole) blank(in.rg, in.q, kShut), blank(in.dy, in.q);
+        },
+        work);
+  } else {
+    if (whole < o.count) {
+      LoadedMap<T, V, L> in;
+      read_map<T, V, L, kMask, false>(p, o, o.first + whole, in);
+      work(0, in);
+    }
+    walk<LoadedMap<T, V, L>>(
+        whole,
+        [&](int k, LoadedMap<T, V, L>& in) { read_map<T, V, L, kMask, !kMask>(p, o, o.first + whole - 1 - k, in); },
+        work);
   }
   join_maps<V, N, kMask>(p, o, A, E);
 }
 
-template <class T, int V, int L, bool kMask>
-__global__ void __launch_bounds__(32 * kStrips) backward_maps_kernel(const __grid_constant__ Args p) {
+template <class T, int V, int L, bool kMask, bool kBulk>
+__global__ void __launch_bounds__(32 * kStrips) backward_maps_kernel(const __grid_constant__ Args p,
+                                                              const __grid_constant__ Maps m) {
   using Q = Pairing<V, L>;
   const Lane o = lane_of<V, L, kMask, true>(p);
   Vec<Q::N> rate[Q::P];
   if (rates<V, Q::N>(p, o, rate))
-    backward_maps<T, V, L, kMask, true>(p, o, rate);
+    backward_maps<T, V, L, kMask, true, kBulk>(p, m, o, rate);
   else
-    backward_maps<T, V, L, kMask, false>(p, o, rate);
+    backward_maps<T, V, L, kMask, false, kBulk>(p, m, o, rate);
 }
 
 template <class T, int V, int L>
@@ -664,31 +864,55 @@ __device__ __forceinline__ void backward_chunk(const Args& p, const Lane& o, con
   }
 }
 
-template <class T, int V, int L, bool kMask, bool kFar>
-__device__ __forceinline__ void backward_strip(const Args& p, const Lane& o,
+template <class T, int V, int L, bool kMask, bool kFar, bool kBulk>
+__device__ __forceinline__ void backward_strip(const Args& p, const Maps& m, const Lane& o,
                                                const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P]) {
   using Q = Pairing<V, L>;
   constexpr int N = Q::N, P = Q::P;
   if (o.count == 0) return;
-  constexpr bool kFull = !kMask;
   const int whole = kMask ? o.count : o.whole;
-  LoadedBack<T, V, L> one, two;
   Vec<N> e[P], acc[P];
 #pragma unroll
   for (int j = 0; j < P; ++j) e[j] = acc[j] = splat<N>(0.0f);
   if (p.dlast) read_row<V, N>(p.dlast + o.b * p.width + o.from, e);
   start_of<V, N, kMask>(p, o, e);
-  if (whole) read_back<T, V, L, kMask, kFull>(p, o, o.first + whole - 1, one);
-  if (whole < o.count) {
-    read_back<T, V, L, kMask, false>(p, o, o.first + whole, two);
-    backward_chunk<T, V, L, kMask, kFar, false>(p, o, two, rate, e, acc);
-  }
-#pragma unroll 1
-  for (int k = whole - 1; k >= 0; k -= 2) {
-    read_back<T, V, L, kMask, kFull>(p, o, o.first + max(k - 1, 0), two);
-    backward_chunk<T, V, L, kMask, kFar, kFull>(p, o, one, rate, e, acc);
-    read_back<T, V, L, kMask, kFull>(p, o, o.first + max(k - 2, 0), one);
-    if (k >= 1) backward_chunk<T, V, L, kMask, kFar, kFull>(p, o, two, rate, e, acc);
+  if constexpr (kBulk) {
+    extern __shared__ __align__(128) char dynamic[];
+    __shared__ uint64_t s_bar[kStrips * kRing<T>];
+    Ring<T, 4, true> ring(dynamic, s_bar);
+    ring.map[0] = &m.rg, ring.map[1] = &m.ig, ring.map[2] = &m.x, ring.map[3] = &m.dy;
+    if (!ring.template walk<LoadedBack<T, V, L>>(
+            p, o, o.first + o.count - 1, o.count, -1,
+            [&](int stage, int k, LoadedBack<T, V, L>& in) {
+              in.q = chunk_of<L, kMask>(p, o, k);
+              ring.get(p, stage, 0, in.rg);
+              ring.get(p, stage, 1, in.ig);
+              ring.get(p, stage, 2, in.x);
+              ring.get(p, stage, 3, in.dy);
+              const Pack<float, 2> h = ring.state(stage);
+              in.h[0] = widen<2>(h, 0);
+              if (kMask || k - o.first >= whole)
+                blank(in.rg, in.q, kShut), blank(in.ig, in.q), blank(in.x, in.q), blank(in.dy, in.q);
+            },
+            [&](int k, const LoadedBack<T, V, L>& in) {
+              if (kMask || k - o.first < whole)
+                backward_chunk<T, V, L, kMask, kFar, !kMask>(p, o, in, rate, e, acc);
+              else
+                backward_chunk<T, V, L, kMask, kFar, false>(p, o, in, rate, e, acc);
+            }))
+      return;
+  } else {
+    if (whole < o.count) {
+      LoadedBack<T, V, L> in;
+      read_back<T, V, L, kMask, false>(p, o, o.first + whole, in);
+      backward_chunk<T, V, L, kMask, kFar, false>(p, o, in, rate, e, acc);
+    }
+    walk<LoadedBack<T, V, L>>(
+        whole,
+        [&](int k, LoadedBack<T, V, L>& in) { read_back<T, V, L, kMask, !kMask>(p, o, o.first + whole - 1 - k, in); },
+        [&](int, const LoadedBack<T, V, L>& in) {
+          backward_chunk<T, V, L, kMask, kFar, !kMask>(p, o, in, rate, e, acc);
+        });
   }
   if (!o.on) return;
 #pragma unroll
@@ -698,23 +922,25 @@ __device__ __forceinline__ void backward_strip(const Args& p, const Lane& o,
   }
 }
 
-template <class T, int V, int L, bool kMask>
-__global__ void __launch_bounds__(32 * kStrips) backward_kernel(const __grid_constant__ Args p) {
+template <class T, int V, int L, bool kMask, bool kBulk>
+__global__ void __launch_bounds__(32 * kStrips) backward_kernel(const __grid_constant__ Args p,
+                                                              const __grid_constant__ Maps m) {
   using Q = Pairing<V, L>;
   const Lane o = lane_of<V, L, kMask, true>(p);
   Vec<Q::N> rate[Q::P];
   if (rates<V, Q::N>(p, o, rate))
-    backward_strip<T, V, L, kMask, true>(p, o, rate);
+    backward_strip<T, V, L, kMask, true, kBulk>(p, m, o, rate);
   else
-    backward_strip<T, V, L, kMask, false>(p, o, rate);
+    backward_strip<T, V, L, kMask, false, kBulk>(p, m, o, rate);
 }
 
 struct Geometry {
   int vec, chunk, ctiles, strips, strip;
+  bool bulk;
 };
 
 template <class T>
-cudaError_t launch(const Args& p, const Geometry& g, bool backward, bool mask, cudaStream_t s);
+cudaError_t launch(const Args& p, const Maps& m, const Geometry& g, bool backward, bool mask, cudaStream_t s);
 
 }  // namespace gscan
 }  // namespace pesq

@@ -11,13 +11,16 @@ using pesq::set_error;
 
 namespace pesq {
 namespace gscan {
-extern template cudaError_t launch<float>(const Args&, const Geometry&, bool, bool, cudaStream_t);
-extern template cudaError_t launch<__nv_bfloat16>(const Args&, const Geometry&, bool, bool, cudaStream_t);
-extern template cudaError_t launch<__half>(const Args&, const Geometry&, bool, bool, cudaStream_t);
+extern template cudaError_t launch<float>(const Args&, const Maps&, const Geometry&, bool, bool, cudaStream_t);
+extern template cudaError_t launch<__nv_bfloat16>(const Args&, const Maps&, const Geometry&, bool, bool, cudaStream_t);
+extern template cudaError_t launch<__half>(const Args&, const Maps&, const Geometry&, bool, bool, cudaStream_t);
 }  // namespace gscan
 }  // namespace pesq
 
 namespace {
+
+// Set by a kernel whose copies do not come; one a device
+__device__ uint32_t g_error;
 
 // ddecay[c] = -rate sigmoid(decay[c]) sum over the rows of part, in a fixed
 // order: 32 columns a block, every thread a stride of the rows, then a tree.
@@ -70,8 +73,15 @@ constexpr int64_t kWarpsWanted = 148 * 8;
 constexpr int64_t kWarpsEnough = 148 * 4;
 constexpr int kFewestChunks = 4;
 
-// Pairs of channels where everything allows it (a backward call has its
-// forward's inputs, so takes its forward's).  One strip a row once rows and
+// Whether boxes of 64 channels can be copied: 16-byte addresses and strides, which a tensor map asks for
+bool boxes(const pesq_stream& s, const pesq_gated_scan_desc& d) {
+  const int64_t e = element(d.dtype), most = INT64_C(1) << 39;
+  return reinterpret_cast<uintptr_t>(s.data) % 16 == 0 && s.step_stride > 0 && s.step_stride < most &&
+         s.step_stride * e % 16 == 0 &&
+         (d.batch == 1 || (s.batch_stride > 0 && s.batch_stride < most && s.batch_stride * e % 16 == 0));
+}
+
+// Pairs of channels where everything allows it.  One strip a row once rows and
 // channels make kWarpsEnough warps; otherwise as many as make kWarpsWanted.
 Geometry geometry(const pesq_gated_scan_desc& d) {
   Geometry g{};
@@ -85,7 +95,37 @@ Geometry geometry(const pesq_gated_scan_desc& d) {
   const int64_t per = (chunks + strips - 1) / strips;
   g.strips = (int)((chunks + per - 1) / per);
   g.strip = (int)(per * g.chunk);
+  g.bulk = chunks >= kFewestChunks && d.width * (int64_t)element(d.dtype) % 16 == 0 && boxes(d.x, d) &&
+           boxes(d.input_gate, d) && boxes(d.decay_gate, d);
   return g;
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encoder() {
+  static const EncodeTiled fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeTiled>(f);
+  }();
+  return fn;
+}
+
+bool encode(CUtensorMap& m, const pesq_stream& s, const pesq_gated_scan_desc& d) {
+  const cuuint64_t e = element(d.dtype), step = s.step_stride * e;
+  const cuuint64_t dims[3] = {(cuuint64_t)d.width, (cuuint64_t)d.steps, (cuuint64_t)d.batch};
+  const cuuint64_t strides[2] = {step, d.batch == 1 ? step : s.batch_stride * e};
+  const cuuint32_t box[3] = {64, kChunk, 1}, unit[3] = {1, 1, 1};
+  const CUtensorMapDataType type = d.dtype == PESQ_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : d.dtype == PESQ_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                          : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return encoder()(&m, type, 3, const_cast<void*>(s.data), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
@@ -145,11 +185,33 @@ bool missing(const void* p, size_t have, size_t want) {
   return want && (!p || have < want || reinterpret_cast<uintptr_t>(p) % 16);
 }
 
-int run(const pesq_gated_scan_desc& d, const Args& a, const Geometry& g, bool backward, cudaStream_t s) {
-  const bool mask = d.reset || d.lengths;
-  const cudaError_t e = d.dtype == PESQ_F32    ? launch<float>(a, g, backward, mask, s)
-                        : d.dtype == PESQ_BF16 ? launch<__nv_bfloat16>(a, g, backward, mask, s)
-                                               : launch<__half>(a, g, backward, mask, s);
+// The current device's error word
+uint32_t* error_word() {
+  static uint32_t* words[64] = {nullptr};  // by device; an address that does not change
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+  if (!words[dev]) {
+    void* p = nullptr;
+    if (cudaGetSymbolAddress(&p, g_error) != cudaSuccess) return nullptr;
+    words[dev] = static_cast<uint32_t*>(p);
+  }
+  return words[dev];
+}
+
+int run(const pesq_gated_scan_desc& d, Args& a, Geometry g, const pesq_stream* dy, cudaStream_t s) {
+  const bool backward = dy != nullptr, mask = d.reset || d.lengths;
+  Maps m;
+  g.bulk = g.bulk && (!backward || (dy->data && boxes(*dy, d))) && encoder();
+  if (g.bulk) {
+    a.error = error_word();
+    if (!a.error) return set_error(PESQ_ERR_CUDA, "no error word");
+    if (!encode(m.x, d.x, d) || !encode(m.ig, d.input_gate, d) || !encode(m.rg, d.decay_gate, d) ||
+        (backward && !encode(m.dy, *dy, d)))
+      return set_error(PESQ_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+  }
+  const cudaError_t e = d.dtype == PESQ_F32    ? launch<float>(a, m, g, backward, mask, s)
+                        : d.dtype == PESQ_BF16 ? launch<__nv_bfloat16>(a, m, g, backward, mask, s)
+                                               : launch<__half>(a, m, g, backward, mask, s);
   return e == cudaSuccess ? PESQ_OK : set_error(PESQ_ERR_CUDA, cudaGetErrorString(e));
 }
 
@@ -180,7 +242,7 @@ int pesq_gated_scan_forward(const pesq_gated_scan_desc* d, void* stream, void* y
   a.y = y;
   a.last = last;
   a.kept = static_cast<float*>(kept);
-  return run(*d, a, g, false, static_cast<cudaStream_t>(stream));
+  return run(*d, a, g, nullptr, static_cast<cudaStream_t>(stream));
 }
 
 int pesq_gated_scan_backward(const pesq_gated_scan_desc* d, void* stream, const void* kept, size_t kept_size,
@@ -215,10 +277,21 @@ int pesq_gated_scan_backward(const pesq_gated_scan_desc* d, void* stream, const 
   a.dstate = dstate;
   a.dpart = reinterpret_cast<float*>(ws);
   a.kept = const_cast<float*>(static_cast<const float*>(kept));
-  if (const int status = run(*d, a, g, true, s)) return status;
+  if (const int status = run(*d, a, g, &dy, s)) return status;
   decay_sum_kernel<<<(unsigned)((d->width + 31) / 32), dim3(32, kSumRows), 0, s>>>(
       a.dpart, d->batch * g.strips, d->width, d->decay, d->rate, ddecay);
   const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? PESQ_OK : set_error(PESQ_ERR_CUDA, cudaGetErrorString(e));
+}
+
+int pesq_gated_scan_check(void* stream, uint32_t* failed) {
+  if (!failed) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL argument");
+  uint32_t* word = error_word();
+  if (!word) return set_error(PESQ_ERR_CUDA, "no error word");
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaMemcpyAsync(failed, word, sizeof(uint32_t), cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaMemsetAsync(word, 0, sizeof(uint32_t), s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
   return e == cudaSuccess ? PESQ_OK : set_error(PESQ_ERR_CUDA, cudaGetErrorString(e));
 }
 

@@ -3,6 +3,6 @@
 
 namespace pesq {
 namespace gscan {
-template cudaError_t launch<float>(const Args&, const Geometry&, bool, bool, cudaStream_t);
+template cudaError_t launch<float>(const Args&, const Maps&, const Geometry&, bool, bool, cudaStream_t);
 }  // namespace gscan
 }  // namespace pesq

@@ -126,5 +126,12 @@ class GatedScanCuda(torch.nn.Module):
         y, last = self(x.unsqueeze(1), input_gate.unsqueeze(1), decay_gate.unsqueeze(1), state)
         return y.squeeze(1), last
 
+    def check_errors(self) -> int:
+        """Synchronise and return the error word of the parameter's device (nonzero
+        if an earlier call's copies into shared memory did not come in time)."""
+
+        with torch.cuda.device(self.decay.device):
+            return _lib.gated_scan_check(torch.cuda.current_stream().cuda_stream)
+
     def extra_repr(self) -> str:
         return f"channels={self.channels}, rate={self.rate}, reverse={self.reverse}"
