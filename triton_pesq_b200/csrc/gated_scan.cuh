@@ -9,16 +9,15 @@
 // the row's length keeps it (a = 1, beta = 0) and its output is zero.
 //
 // A warp owns V neighbouring channels per lane and a strip of consecutive steps,
-// and walks the strip in chunks of kChunk steps with the state in registers:
+// and walks the strip in chunks of 8 or 16 steps with the state in registers:
 // everything of a step but one multiply-add is independent of the steps before it,
 // so a chunk's gates are worked out side by side, while the elements of the chunks
 // to come are on their way.  Warps wait for nobody but their own copies: no flag, no
 // atomic, and the order of every operation is fixed.
 //
 // Elements come in two ways.  Where channels and strides allow (multiples of 16
-// bytes), a warp's chunks are boxes of 64 channels x 8 steps that tensor copies bring to
-// a ring in shared memory: one instruction for a box, no registers held, and two or three
-// chunks in flight.  Otherwise every lane loads its own elements a chunk ahead.
+// bytes), a warp's chunks are boxes of 64 channels x 8 steps, or 32 x 16, that tensor copies bring to
+// a ring in shared memory: one instruction for a box, no registers held.  Otherwise every lane loads its own elements a chunk ahead.
 //
 // With rows and channels enough to fill the device a strip is the whole row,
 // and the data pass once.  Otherwise rows are cut into strips: the recurrence is
@@ -33,7 +32,7 @@
 //   dlog a = g (a h_{t-1} - (a^2 / beta) i x),   ddecay_gate = dlog a log a (1 - r),
 //   ddecay = -rate sigmoid(decay) sum over rows and steps of dlog a r.
 // h is not read back from the rounded y: the forward keeps the state before every
-// chunk in 32 bits (1 / kChunk of the elements), and the backward recomputes the
+// chunk in 32 bits (1 / 8 or 1 / 16 of the elements), and the backward recomputes the
 // chunk from it.  beta -> 0 only together with log a, whose quotient goes to
 // zero: the term is dropped there.
 #pragma once
@@ -49,11 +48,13 @@ namespace gscan {
 
 using namespace train;
 
-constexpr int kChunk = 8;   // steps of a chunk
+// steps of a chunk, by the channels of a lane: in shared memory sixteen elements of each
+// stream either way, in registers no more than 8 steps
+constexpr int chunk_steps(int vec, bool bulk) { return bulk ? 16 / vec : 8; }
 constexpr int kStrips = 8;  // strips (warps) of a CTA, where rows are cut
 // chunks of a warp in shared memory: what 8 warps' chunks of four 32-bit streams leave room for
 template <class T>
-constexpr int kRing = sizeof(T) == 2 ? 4 : 3;
+constexpr int kRing = sizeof(T) == 2 ? 3 : 2;
 
 struct Stream {
   const void* p;
@@ -89,7 +90,7 @@ struct Args {
   uint32_t* error;            // set when a copy does not come
 };
 
-// Tensor maps of the streams: [batch][step][channel], boxes of 1 x kChunk x 64
+// Tensor maps of the streams: [batch][step][channel], boxes of a chunk
 struct Maps {
   CUtensorMap rg, ig, x, dy;
 };
@@ -120,73 +121,101 @@ constexpr float kNear = 0.25f;
 
 template <int N>
 struct Gates {
-  Vec<N> i, r, a, w;  // w = 1 - a^2
+  Vec<N> i, r, a;
 };
 
+// The gates of G Vecs side by side: operation by operation rather than Vec by
+// Vec, so that every instruction has G independent ones next to it.
+//
 // k = rate softplus(decay) >= 0.  The two sigmoids share one reciprocal.
 // With m = -log a = k r, 1 - a = m (1 - m/2 + m^2/6 - ...) by its Taylor
 // series (m^6 / 5040 < 5e-8 at 1/4): a is then rounded once, without the bias
 // that a long memory would sum up, and 1 - a^2 = (1 - a)(2 - (1 - a)) does not
 // cancel.  kFar: m may be above kNear, where the exponential takes over.
-template <bool kFar, int N>
-__device__ __forceinline__ void decays(Vec<N> r, Vec<N> k, Vec<N>& a, Vec<N>& w) {
-  const Vec<N> m = k * r;
-  Vec<N> p = fma(m, splat<N>(-1.0f / 720), splat<N>(1.0f / 120));
-  p = fma(m, p, splat<N>(-1.0f / 24));
-  p = fma(m, p, splat<N>(1.0f / 6));
-  p = fma(m, p, splat<N>(-0.5f));
-  p = fma(m, p, splat<N>(1.0f));
-  const Vec<N> u = m * p;
-  a = fma(u, splat<N>(-1.0f), splat<N>(1.0f));
-  w = u * fma(u, splat<N>(-1.0f), splat<N>(2.0f));
+template <bool kFar, int N, int G>
+__device__ __forceinline__ void decays(const Vec<N> (&r)[G], const Vec<N> (&k)[G], Vec<N> (&a)[G], Vec<N> (&w)[G]) {
+  Vec<N> m[G], p[G];
+  constexpr float kSeries[5] = {1.0f / 120, -1.0f / 24, 1.0f / 6, -0.5f, 1.0f};
+#pragma unroll
+  for (int g = 0; g < G; ++g) m[g] = k[g] * r[g];
+#pragma unroll
+  for (int g = 0; g < G; ++g) p[g] = splat<N>(-1.0f / 720);
+#pragma unroll
+  for (int i = 0; i < 5; ++i)
+#pragma unroll
+    for (int g = 0; g < G; ++g) p[g] = fma(m[g], p[g], splat<N>(kSeries[i]));
+#pragma unroll
+  for (int g = 0; g < G; ++g) p[g] = m[g] * p[g];
+#pragma unroll
+  for (int g = 0; g < G; ++g) a[g] = fma(p[g], splat<N>(-1.0f), splat<N>(1.0f));
+#pragma unroll
+  for (int g = 0; g < G; ++g) w[g] = fma(p[g], splat<N>(-1.0f), splat<N>(2.0f));
+#pragma unroll
+  for (int g = 0; g < G; ++g) w[g] = p[g] * w[g];
   if (kFar) {
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (!(m.v[j] < kNear)) {
-        a.v[j] = exp2_approx(m.v[j] * -kLog2e);
-        w.v[j] = fmaf(-a.v[j], a.v[j], 1.0f);
-      }
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (!(m[g].v[j] < kNear)) {
+          a[g].v[j] = exp2_approx(m[g].v[j] * -kLog2e);
+          w[g].v[j] = fmaf(-a[g].v[j], a[g].v[j], 1.0f);
+        }
   }
 }
 
-template <bool kFar, int N>
-__device__ __forceinline__ Gates<N> gates(Vec<N> ig, Vec<N> rg, Vec<N> k) {
-  Vec<N> di = ig * splat<N>(-kLog2e), dr = rg * splat<N>(-kLog2e), q;
+template <bool kFar, int N, int G>
+__device__ __forceinline__ void gates(const Vec<N> (&ig)[G], const Vec<N> (&rg)[G], const Vec<N> (&k)[G],
+                                      Gates<N> (&out)[G], Vec<N> (&beta)[G]) {
+  Vec<N> di[G], dr[G], q[G], r[G], a[G], w[G];
 #pragma unroll
-  for (int j = 0; j < N; ++j) di.v[j] = exp2_approx(di.v[j]), dr.v[j] = exp2_approx(dr.v[j]);
-  di = di + splat<N>(1.0f);
-  dr = dr + splat<N>(1.0f);
-  q = di * dr;
+  for (int g = 0; g < G; ++g) di[g] = ig[g] * splat<N>(-kLog2e), dr[g] = rg[g] * splat<N>(-kLog2e);
 #pragma unroll
-  for (int j = 0; j < N; ++j) q.v[j] = rcp_approx(q.v[j]);
-  Gates<N> o;
-  o.i = q * dr;
-  o.r = q * di;
-  decays<kFar, N>(o.r, k, o.a, o.w);
-  return o;
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int j = 0; j < N; ++j) di[g].v[j] = exp2_approx(di[g].v[j]), dr[g].v[j] = exp2_approx(dr[g].v[j]);
+#pragma unroll
+  for (int g = 0; g < G; ++g) di[g] = di[g] + splat<N>(1.0f), dr[g] = dr[g] + splat<N>(1.0f);
+#pragma unroll
+  for (int g = 0; g < G; ++g) q[g] = di[g] * dr[g];
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int j = 0; j < N; ++j) q[g].v[j] = rcp_approx(q[g].v[j]);
+#pragma unroll
+  for (int g = 0; g < G; ++g) r[g] = q[g] * di[g];
+#pragma unroll
+  for (int g = 0; g < G; ++g) di[g] = q[g] * dr[g];
+  decays<kFar>(r, k, a, w);
+  Vec<N> s[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int j = 0; j < N; ++j) s[g].v[j] = rsqrt_approx(fmaxf(w[g].v[j], kTiny));
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    beta[g] = w[g] * s[g];
+    out[g].i = di[g], out[g].r = r[g], out[g].a = a[g];
+  }
 }
 
-// The decay alone
-template <bool kFar, int N>
-__device__ __forceinline__ Vec<N> decay_of(Vec<N> rg, Vec<N> k) {
-  Vec<N> dr = rg * splat<N>(-kLog2e);
+// The decays alone
+template <bool kFar, int N, int G>
+__device__ __forceinline__ void decays_of(const Vec<N> (&rg)[G], const Vec<N> (&k)[G], Vec<N> (&a)[G]) {
+  Vec<N> r[G], w[G];
 #pragma unroll
-  for (int j = 0; j < N; ++j) dr.v[j] = exp2_approx(dr.v[j]);
-  dr = dr + splat<N>(1.0f);
+  for (int g = 0; g < G; ++g) r[g] = rg[g] * splat<N>(-kLog2e);
 #pragma unroll
-  for (int j = 0; j < N; ++j) dr.v[j] = rcp_approx(dr.v[j]);
-  Vec<N> a, w;
-  decays<kFar, N>(dr, k, a, w);
-  return a;
-}
-
-// sqrt(w) of w >= 0
-template <int N>
-__device__ __forceinline__ Vec<N> root(Vec<N> w) {
-  Vec<N> s;
+  for (int g = 0; g < G; ++g)
 #pragma unroll
-  for (int j = 0; j < N; ++j) s.v[j] = rsqrt_approx(fmaxf(w.v[j], kTiny));
-  return w * s;
+    for (int j = 0; j < N; ++j) r[g].v[j] = exp2_approx(r[g].v[j]);
+#pragma unroll
+  for (int g = 0; g < G; ++g) r[g] = r[g] + splat<N>(1.0f);
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int j = 0; j < N; ++j) r[g].v[j] = rcp_approx(r[g].v[j]);
+  decays<kFar>(r, k, a, w);
 }
 
 // a h + b.  A state that a = 0 cuts off is not looked at (it may be infinite or NaN).
@@ -332,9 +361,9 @@ __device__ __forceinline__ void store(void* p, const Vec<N> (&val)[V / N]) {
 // step where a lane has a single channel.
 template <int V, int L>
 struct Pairing {
-  static constexpr int N = V > 1 ? 2 : 1;                 // channels of a Vec
-  static constexpr int P = V / N;                         // Vecs of a step
-  static constexpr int S = V == 1 && L % 2 == 0 ? 2 : 1;  // steps worked out together
+  static constexpr int N = V > 1 ? 2 : 1;  // channels of a Vec
+  static constexpr int P = V / N;          // Vecs of a step
+  static constexpr bool kBySteps = V == 1 && L % 2 == 0;
 };
 
 // Calls emit(l, j, gates, beta) for every step and Vec of a chunk, steps in order
@@ -342,32 +371,46 @@ template <class T, int V, int L, bool kMask, bool kFar, class F>
 __device__ __forceinline__ void each_gate(const Chunk& q, const Pack<T, V> (&ig)[L], const Pack<T, V> (&rg)[L],
                                           const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P], F emit) {
   using Q = Pairing<V, L>;
-  constexpr int N = Q::N, S = Q::S;
+  constexpr int N = Q::N;
+  if constexpr (Q::kBySteps) {
+    constexpr int G = L / 2;
+    Vec<2> i2[G], r2[G], k2[G], beta[G];
+    Gates<2> out[G];
 #pragma unroll
-  for (int l = 0; l < L; l += S) {
-    if constexpr (S == 2) {
-      Pack<T, 2> r2{{rg[l].v[0], rg[l + 1].v[0]}}, i2{{ig[l].v[0], ig[l + 1].v[0]}};
-      hold(r2), hold(i2);
-      const Gates<2> g = gates<kFar, 2>(widen<2>(i2, 0), widen<2>(r2, 0), splat<2>(rate[0].v[0]));
-      const Vec<2> beta = root(g.w);
+    for (int g = 0; g < G; ++g) {
+      Pack<T, 2> r{{rg[2 * g].v[0], rg[2 * g + 1].v[0]}}, i{{ig[2 * g].v[0], ig[2 * g + 1].v[0]}};
+      hold(r), hold(i);
+      i2[g] = widen<2>(i, 0), r2[g] = widen<2>(r, 0), k2[g] = splat<2>(rate[0].v[0]);
+    }
+    gates<kFar>(i2, r2, k2, out, beta);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        Gates<1> one{{{g.i.v[i]}}, {{g.r.v[i]}}, {{g.a.v[i]}}, {{g.w.v[i]}}};
-        Vec<1> b1{{beta.v[i]}};
-        if (kMask && ((q.cut >> (l + i)) & 1u)) one.a = splat<1>(0.0f), b1 = splat<1>(1.0f);
-        emit(l + i, 0, one, b1);
-      }
-    } else {
-      Pack<T, V> r1 = rg[l], i1 = ig[l];
-      hold(r1), hold(i1);
+    for (int l = 0; l < L; ++l) {
+      Gates<1> one{{{out[l / 2].i.v[l % 2]}}, {{out[l / 2].r.v[l % 2]}}, {{out[l / 2].a.v[l % 2]}}};
+      Vec<1> b1{{beta[l / 2].v[l % 2]}};
+      if (kMask && ((q.cut >> l) & 1u)) one.a = splat<1>(0.0f), b1 = splat<1>(1.0f);
+      emit(l, 0, one, b1);
+    }
+  } else {
+    constexpr int G = L * Q::P;
+    Vec<N> i2[G], r2[G], k2[G], beta[G];
+    Gates<N> out[G];
+#pragma unroll
+    for (int l = 0; l < L; ++l) {
+      Pack<T, V> r = rg[l], i = ig[l];
+      hold(r), hold(i);
+#pragma unroll
+      for (int j = 0; j < Q::P; ++j)
+        i2[l * Q::P + j] = widen<N>(i, j), r2[l * Q::P + j] = widen<N>(r, j), k2[l * Q::P + j] = rate[j];
+    }
+    gates<kFar>(i2, r2, k2, out, beta);
+#pragma unroll
+    for (int l = 0; l < L; ++l)
 #pragma unroll
       for (int j = 0; j < Q::P; ++j) {
-        Gates<N> g = gates<kFar, N>(widen<N>(i1, j), widen<N>(r1, j), rate[j]);
-        Vec<N> beta = root(g.w);
-        if (kMask && ((q.cut >> l) & 1u)) g.a = splat<N>(0.0f), beta = splat<N>(1.0f);
-        emit(l, j, g, beta);
+        Gates<N>& one = out[l * Q::P + j];
+        if (kMask && ((q.cut >> l) & 1u)) one.a = splat<N>(0.0f), beta[l * Q::P + j] = splat<N>(1.0f);
+        emit(l, j, one, beta[l * Q::P + j]);
       }
-    }
   }
 }
 
@@ -457,11 +500,11 @@ __device__ __forceinline__ void walk(int n, R read, W work) {
 }
 
 // A warp's ring of chunks in shared memory: kRing stages of S streams' boxes
-// [kChunk][64] and, with kState, the 64 states before the chunk.
-template <class T, int S, bool kState>
+// [L][32 V] and, with kState, the states before the chunk.
+template <class T, int V, int L, int S, bool kState>
 struct Ring {
-  static constexpr int kBox = kChunk * 64 * (int)sizeof(T);
-  static constexpr int kStage = S * kBox + (kState ? 256 : 0);
+  static constexpr int kBox = L * 32 * V * (int)sizeof(T);
+  static constexpr int kStage = S * kBox + (kState ? 128 * V : 0);
   static constexpr int kBytes = kRing<T> * kStage;  // of a warp
   char* base;
   uint64_t* bar;
@@ -477,10 +520,10 @@ struct Ring {
   }
   // one lane
   __device__ __forceinline__ void send(const Args& p, const Lane& o, int k, int stage) {
-    const int c0 = (int)o.c, t0 = p.reverse ? (int)p.steps - (k + 1) * kChunk : k * kChunk;
+    const int c0 = (int)o.c, t0 = p.reverse ? (int)p.steps - (k + 1) * L : k * L;
     char* to = base + stage * kStage;
     uint32_t bytes = S * kBox, state = 0;
-    if (kState) state = (uint32_t)min((int64_t)64, p.width - o.c) * 4, bytes += state;
+    if (kState) state = (uint32_t)min((int64_t)(32 * V), p.width - o.c) * 4, bytes += state;
     mbar_arrive_expect_tx(bar + stage, bytes);
 #pragma unroll
     for (int i = 0; i < S; ++i)
@@ -490,18 +533,18 @@ struct Ring {
           "l"(map[i]), "r"(smem_u32(bar + stage)), "r"(c0), "r"(t0), "r"((int)o.b)
           : "memory");
     if (kState)
-      bulk_g2s(to + S * kBox, p.kept + (o.b * ((p.steps + kChunk - 1) / kChunk) + k) * p.width + o.c, state, bar + stage);
+      bulk_g2s(to + S * kBox, p.kept + (o.b * ((p.steps + L - 1) / L) + k) * p.width + o.c, state, bar + stage);
   }
   // one stream of the stage, in scan order
-  __device__ __forceinline__ void get(const Args& p, int stage, int i, Pack<T, 2> (&out)[kChunk]) const {
-    const Pack<T, 2>* s = reinterpret_cast<const Pack<T, 2>*>(base + stage * kStage + i * kBox) + threadIdx.x;
+  __device__ __forceinline__ void get(const Args& p, int stage, int i, Pack<T, V> (&out)[L]) const {
+    const Pack<T, V>* s = reinterpret_cast<const Pack<T, V>*>(base + stage * kStage + i * kBox) + threadIdx.x;
     const int step = p.reverse ? -32 : 32;
-    s += p.reverse ? 7 * 32 : 0;
+    s += p.reverse ? (L - 1) * 32 : 0;
 #pragma unroll
-    for (int l = 0; l < kChunk; ++l) out[l] = s[l * step];
+    for (int l = 0; l < L; ++l) out[l] = s[l * step];
   }
-  __device__ __forceinline__ Pack<float, 2> state(int stage) const {
-    return reinterpret_cast<const Pack<float, 2>*>(base + stage * kStage + S * kBox)[threadIdx.x];
+  __device__ __forceinline__ Pack<float, V> state(int stage) const {
+    return reinterpret_cast<const Pack<float, V>*>(base + stage * kStage + S * kBox)[threadIdx.x];
   }
   // Chunks first, first + way, ...: read(stage, k, in) takes a chunk out of its stage, work(k, in)
   // works on it while the stage fills again.  Returns false where a copy does not come.
@@ -559,10 +602,10 @@ __device__ __forceinline__ void read_chunk(const Args& p, const Lane& o, int k, 
   load<T, V, L, kFull>(in.x, p.x, o, in.q);
 }
 
-template <class T, bool kMask>
-__device__ __forceinline__ void ring_chunk(const Args& p, const Lane& o, const Ring<T, 3, false>& ring, int stage, int k,
-                                           int whole, Loaded<T, 2, kChunk>& in) {
-  in.q = chunk_of<kChunk, kMask>(p, o, k);
+template <class T, int V, int L, bool kMask>
+__device__ __forceinline__ void ring_chunk(const Args& p, const Lane& o, const Ring<T, V, L, 3, false>& ring, int stage, int k,
+                                           int whole, Loaded<T, V, L>& in) {
+  in.q = chunk_of<L, kMask>(p, o, k);
   ring.get(p, stage, 0, in.rg);
   ring.get(p, stage, 1, in.ig);
   ring.get(p, stage, 2, in.x);
@@ -591,11 +634,11 @@ __device__ __forceinline__ void forward_maps(const Args& p, const Maps& m, const
   if constexpr (kBulk) {
     extern __shared__ __align__(128) char dynamic[];
     __shared__ uint64_t s_bar[kStrips * kRing<T>];
-    Ring<T, 3, false> ring(dynamic, s_bar);
+    Ring<T, V, L, 3, false> ring(dynamic, s_bar);
     ring.map[0] = &m.rg, ring.map[1] = &m.ig, ring.map[2] = &m.x;
     ring.template walk<Loaded<T, V, L>>(
         p, o, o.first, o.count, 1,
-        [&](int stage, int k, Loaded<T, V, L>& in) { ring_chunk<T, kMask>(p, o, ring, stage, k, whole, in); },
+        [&](int stage, int k, Loaded<T, V, L>& in) { ring_chunk<T, V, L, kMask>(p, o, ring, stage, k, whole, in); },
         [&](int k, const Loaded<T, V, L>& in) { work(k, in); });
   } else {
     walk<Loaded<T, V, L>>(
@@ -659,11 +702,11 @@ __device__ __forceinline__ void forward_strip(const Args& p, const Maps& m, cons
   if constexpr (kBulk) {
     extern __shared__ __align__(128) char dynamic[];
     __shared__ uint64_t s_bar[kStrips * kRing<T>];
-    Ring<T, 3, false> ring(dynamic, s_bar);
+    Ring<T, V, L, 3, false> ring(dynamic, s_bar);
     ring.map[0] = &m.rg, ring.map[1] = &m.ig, ring.map[2] = &m.x;
     if (!ring.template walk<Loaded<T, V, L>>(
             p, o, o.first, o.count, 1,
-            [&](int stage, int k, Loaded<T, V, L>& in) { ring_chunk<T, kMask>(p, o, ring, stage, k, whole, in); },
+            [&](int stage, int k, Loaded<T, V, L>& in) { ring_chunk<T, V, L, kMask>(p, o, ring, stage, k, whole, in); },
             [&](int k, const Loaded<T, V, L>& in) {
               if (kMask || k - o.first < whole)
                 forward_chunk<T, V, L, kMask, kFar, !kMask>(p, o, k, in, rate, h);
@@ -727,15 +770,22 @@ __device__ __forceinline__ void backward_maps(const Args& p, const Maps& m, cons
 #pragma unroll
   for (int j = 0; j < P; ++j) A[j] = splat<N>(1.0f), E[j] = splat<N>(0.0f);
   const auto work = [&](int, LoadedMap<T, V, L>& in) {
+    Vec<N> rg[L * P], k2[L * P], a[L * P];
 #pragma unroll
-    for (int l = L - 1; l >= 0; --l) {
+    for (int l = 0; l < L; ++l) {
       hold(in.rg[l]);
 #pragma unroll
+      for (int j = 0; j < P; ++j) rg[l * P + j] = widen<N>(in.rg[l], j), k2[l * P + j] = rate[j];
+    }
+    decays_of<kFar>(rg, k2, a);
+#pragma unroll
+    for (int l = L - 1; l >= 0; --l) {
+#pragma unroll
       for (int j = 0; j < P; ++j) {
-        Vec<N> a = decay_of<kFar, N>(widen<N>(in.rg[l], j), rate[j]);
-        if (kMask && ((in.q.cut >> l) & 1u)) a = splat<N>(0.0f);
-        E[j] = apply<kMask>(a, E[j] + widen<N>(in.dy[l], j), splat<N>(0.0f));
-        A[j] = A[j] * a;
+        Vec<N> al = a[l * P + j];
+        if (kMask && ((in.q.cut >> l) & 1u)) al = splat<N>(0.0f);
+        E[j] = apply<kMask>(al, E[j] + widen<N>(in.dy[l], j), splat<N>(0.0f));
+        A[j] = A[j] * al;
       }
     }
   };
@@ -743,7 +793,7 @@ __device__ __forceinline__ void backward_maps(const Args& p, const Maps& m, cons
   if constexpr (kBulk) {
     extern __shared__ __align__(128) char dynamic[];
     __shared__ uint64_t s_bar[kStrips * kRing<T>];
-    Ring<T, 2, false> ring(dynamic, s_bar);
+    Ring<T, V, L, 2, false> ring(dynamic, s_bar);
     ring.map[0] = &m.rg, ring.map[1] = &m.dy;
     ring.template walk<LoadedMap<T, V, L>>(
         p, o, o.first + o.count - 1, o.count, -1,
@@ -879,7 +929,7 @@ __device__ __forceinline__ void backward_strip(const Args& p, const Maps& m, con
   if constexpr (kBulk) {
     extern __shared__ __align__(128) char dynamic[];
     __shared__ uint64_t s_bar[kStrips * kRing<T>];
-    Ring<T, 4, true> ring(dynamic, s_bar);
+    Ring<T, V, L, 4, true> ring(dynamic, s_bar);
     ring.map[0] = &m.rg, ring.map[1] = &m.ig, ring.map[2] = &m.x, ring.map[3] = &m.dy;
     if (!ring.template walk<LoadedBack<T, V, L>>(
             p, o, o.first + o.count - 1, o.count, -1,
@@ -889,8 +939,9 @@ __device__ __forceinline__ void backward_strip(const Args& p, const Maps& m, con
               ring.get(p, stage, 1, in.ig);
               ring.get(p, stage, 2, in.x);
               ring.get(p, stage, 3, in.dy);
-              const Pack<float, 2> h = ring.state(stage);
-              in.h[0] = widen<2>(h, 0);
+              const Pack<float, V> h = ring.state(stage);
+#pragma unroll
+              for (int j = 0; j < P; ++j) in.h[j] = widen<N>(h, j);
               if (kMask || k - o.first >= whole)
                 blank(in.rg, in.q, kShut), blank(in.ig, in.q), blank(in.x, in.q), blank(in.dy, in.q);
             },

@@ -55,7 +55,7 @@ int check(const pesq_gated_scan_desc* d) {
     return set_error(PESQ_ERR_INVALID_ARGUMENT, "batch, steps and width must be at least 1");
   if (d->dtype < PESQ_F32 || d->dtype > PESQ_F16) return set_error(PESQ_ERR_INVALID_ARGUMENT, "unknown element type");
   if (!(d->rate > 0.0f) || d->rate > 1e6f) return set_error(PESQ_ERR_INVALID_ARGUMENT, "rate must be positive");
-  if (d->batch > 65535 || d->width > (1 << 24) || d->steps > INT32_MAX - kChunk)
+  if (d->batch > 65535 || d->width > (1 << 24) || d->steps > INT32_MAX - 64)
     return set_error(PESQ_ERR_UNSUPPORTED, "more than 65535 rows, 2^24 channels or 2^31 steps in one call");
   return PESQ_OK;
 }
@@ -68,36 +68,19 @@ bool fits(const pesq_stream& s, int vec, const pesq_gated_scan_desc& d) {
          (d.steps == 1 || s.step_stride % vec == 0);
 }
 
-// Warps that fill the device, and the fewest chunks of a strip
-constexpr int64_t kWarpsWanted = 148 * 8;
+// Warps that fill the device, and the fewest steps of a strip and of a row that is copied in boxes
+constexpr int64_t kWarpsWanted = 148 * 12;
 constexpr int64_t kWarpsEnough = 148 * 4;
-constexpr int kFewestChunks = 4;
+constexpr int kFewestSteps = 32;
+constexpr int64_t kFewestBulk = 32;
+constexpr int64_t kWarpsForPairs = 148 * 12;
 
-// Whether boxes of 64 channels can be copied: 16-byte addresses and strides, which a tensor map asks for
+// Whether boxes can be copied: 16-byte addresses and strides, which a tensor map asks for
 bool boxes(const pesq_stream& s, const pesq_gated_scan_desc& d) {
   const int64_t e = element(d.dtype), most = INT64_C(1) << 39;
   return reinterpret_cast<uintptr_t>(s.data) % 16 == 0 && s.step_stride > 0 && s.step_stride < most &&
          s.step_stride * e % 16 == 0 &&
          (d.batch == 1 || (s.batch_stride > 0 && s.batch_stride < most && s.batch_stride * e % 16 == 0));
-}
-
-// Pairs of channels where everything allows it.  One strip a row once rows and
-// channels make kWarpsEnough warps; otherwise as many as make kWarpsWanted.
-Geometry geometry(const pesq_gated_scan_desc& d) {
-  Geometry g{};
-  g.vec = d.width % 2 == 0 && fits(d.x, 2, d) && fits(d.input_gate, 2, d) && fits(d.decay_gate, 2, d) ? 2 : 1;
-  g.ctiles = (int)((d.width + 32 * g.vec - 1) / (32 * g.vec));
-  g.chunk = d.steps == 1 ? 1 : kChunk;
-  const int64_t chunks = (d.steps + g.chunk - 1) / g.chunk, warps = d.batch * g.ctiles;
-  int64_t strips = 1;
-  if (warps < kWarpsEnough)
-    strips = std::max<int64_t>(1, std::min((kWarpsWanted + warps - 1) / warps, chunks / kFewestChunks));
-  const int64_t per = (chunks + strips - 1) / strips;
-  g.strips = (int)((chunks + per - 1) / per);
-  g.strip = (int)(per * g.chunk);
-  g.bulk = chunks >= kFewestChunks && d.width * (int64_t)element(d.dtype) % 16 == 0 && boxes(d.x, d) &&
-           boxes(d.input_gate, d) && boxes(d.decay_gate, d);
-  return g;
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -115,11 +98,38 @@ EncodeTiled encoder() {
   return fn;
 }
 
-bool encode(CUtensorMap& m, const pesq_stream& s, const pesq_gated_scan_desc& d) {
-  const cuuint64_t e = element(d.dtype), step = s.step_stride * e;
-  const cuuint64_t dims[3] = {(cuuint64_t)d.width, (cuuint64_t)d.steps, (cuuint64_t)d.batch};
-  const cuuint64_t strides[2] = {step, d.batch == 1 ? step : s.batch_stride * e};
-  const cuuint32_t box[3] = {64, kChunk, 1}, unit[3] = {1, 1, 1};
+// From the inputs alone, so that a backward call takes its forward's chunks.
+// Pairs of channels where everything allows it and leaves warps enough.  One strip a
+// row once rows and channels make kWarpsEnough warps; otherwise as many as make
+// kWarpsWanted.
+Geometry geometry(const pesq_gated_scan_desc& d) {
+  Geometry g{};
+  g.bulk = d.steps >= kFewestBulk && d.width * (int64_t)element(d.dtype) % 16 == 0 && boxes(d.x, d) &&
+           boxes(d.input_gate, d) && boxes(d.decay_gate, d);
+  g.vec = d.width % 2 == 0 && d.batch * ((d.width + 63) / 64) >= kWarpsForPairs && fits(d.x, 2, d) &&
+                  fits(d.input_gate, 2, d) && fits(d.decay_gate, 2, d)
+              ? 2
+              : 1;
+  g.ctiles = (int)((d.width + 32 * g.vec - 1) / (32 * g.vec));
+  g.chunk = d.steps == 1 ? 1 : chunk_steps(g.vec, g.bulk);
+  const int64_t chunks = (d.steps + g.chunk - 1) / g.chunk, warps = d.batch * g.ctiles;
+  int64_t strips = 1;
+  if (warps < kWarpsEnough)
+    strips = std::max<int64_t>(
+        1, std::min((kWarpsWanted + warps - 1) / warps, (d.steps + kFewestSteps - 1) / kFewestSteps));
+  const int64_t per = (chunks + strips - 1) / strips;
+  g.strips = (int)((chunks + per - 1) / per);
+  g.strip = (int)(per * g.chunk);
+  return g;
+}
+
+// (a step stride of 0: one row of zeros, and what lies outside a map reads as zero)
+bool encode(CUtensorMap& m, const pesq_stream& s, const pesq_gated_scan_desc& d, const Geometry& g) {
+  const bool one = s.step_stride == 0;
+  const cuuint64_t e = element(d.dtype), step = (one ? d.width : s.step_stride) * e;
+  const cuuint64_t dims[3] = {(cuuint64_t)d.width, one ? 1 : (cuuint64_t)d.steps, one ? 1 : (cuuint64_t)d.batch};
+  const cuuint64_t strides[2] = {step, one || d.batch == 1 ? step : s.batch_stride * e};
+  const cuuint32_t box[3] = {32u * g.vec, (cuuint32_t)g.chunk, 1}, unit[3] = {1, 1, 1};
   const CUtensorMapDataType type = d.dtype == PESQ_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : d.dtype == PESQ_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                           : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -198,15 +208,15 @@ uint32_t* error_word() {
   return words[dev];
 }
 
-int run(const pesq_gated_scan_desc& d, Args& a, Geometry g, const pesq_stream* dy, cudaStream_t s) {
+int run(const pesq_gated_scan_desc& d, Args& a, const Geometry& g, const pesq_stream* dy, cudaStream_t s) {
   const bool backward = dy != nullptr, mask = d.reset || d.lengths;
   Maps m;
-  g.bulk = g.bulk && (!backward || (dy->data && boxes(*dy, d))) && encoder();
   if (g.bulk) {
+    if (!encoder()) return set_error(PESQ_ERR_CUDA, "no cuTensorMapEncodeTiled");
     a.error = error_word();
     if (!a.error) return set_error(PESQ_ERR_CUDA, "no error word");
-    if (!encode(m.x, d.x, d) || !encode(m.ig, d.input_gate, d) || !encode(m.rg, d.decay_gate, d) ||
-        (backward && !encode(m.dy, *dy, d)))
+    if (!encode(m.x, d.x, d, g) || !encode(m.ig, d.input_gate, d, g) || !encode(m.rg, d.decay_gate, d, g) ||
+        (backward && !encode(m.dy, *dy, d, g)))
       return set_error(PESQ_ERR_CUDA, "cuTensorMapEncodeTiled failed");
   }
   const cudaError_t e = d.dtype == PESQ_F32    ? launch<float>(a, m, g, backward, mask, s)
@@ -251,7 +261,7 @@ int pesq_gated_scan_backward(const pesq_gated_scan_desc* d, void* stream, const 
   if (const int status = check(d)) return status;
   if (!dx || !dinput_gate || !ddecay_gate || !ddecay) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL output");
   const Geometry g = geometry(*d);
-  if ((dy.data && !fits(dy, g.vec, *d)) || !fits(dx, g.vec, *d) || !fits(dinput_gate, g.vec, *d) ||
+  if ((dy.data && (g.bulk ? !boxes(dy, *d) : !fits(dy, g.vec, *d))) || !fits(dx, g.vec, *d) || !fits(dinput_gate, g.vec, *d) ||
       !fits(ddecay_gate, g.vec, *d))
     return set_error(PESQ_ERR_INVALID_ARGUMENT, "a gradient is less aligned than the inputs");
   if (missing(kept, kept_size, kept_bytes(*d, g)))
@@ -269,6 +279,7 @@ int pesq_gated_scan_backward(const pesq_gated_scan_desc* d, void* stream, const 
     if (cudaMemsetAsync(zeros, 0, d->width * element(d->dtype), s) != cudaSuccess)
       return set_error(PESQ_ERR_CUDA, cudaGetErrorString(cudaGetLastError()));
     a.dy = {zeros, 0, 0};
+    dy = {zeros, 0, 0};
   }
   a.dlast = dlast;
   a.dx = dx;

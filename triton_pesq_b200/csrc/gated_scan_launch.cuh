@@ -24,31 +24,32 @@ template <class T, int V, int L, bool kMask, bool kBulk>
 cudaError_t launch_vl(const Args& p, const Maps& m, const Geometry& g, bool backward, cudaStream_t s) {
   cudaError_t e = cudaSuccess;
   if (!backward) {
-    const size_t smem = kBulk ? Ring<T, 3, false>::kBytes : 0;
+    const size_t smem = kBulk ? Ring<T, V, L, 3, false>::kBytes : 0;
     if (g.strips > 1) e = start(forward_maps_kernel<T, V, L, kMask, kBulk>, p, m, g, smem, s);
     return e != cudaSuccess ? e : start(forward_kernel<T, V, L, kMask, kBulk>, p, m, g, smem, s);
   }
   if (g.strips > 1)
-    e = start(backward_maps_kernel<T, V, L, kMask, kBulk>, p, m, g, kBulk ? Ring<T, 2, false>::kBytes : 0, s);
+    e = start(backward_maps_kernel<T, V, L, kMask, kBulk>, p, m, g, kBulk ? Ring<T, V, L, 2, false>::kBytes : 0, s);
   return e != cudaSuccess
              ? e
-             : start(backward_kernel<T, V, L, kMask, kBulk>, p, m, g, kBulk ? Ring<T, 4, true>::kBytes : 0, s);
+             : start(backward_kernel<T, V, L, kMask, kBulk>, p, m, g, kBulk ? Ring<T, V, L, 4, true>::kBytes : 0, s);
 }
 
-template <class T, int V, int L, bool kBulk>
-cudaError_t launch_m(const Args& p, const Maps& m, const Geometry& g, bool backward, bool mask, cudaStream_t s) {
-  return mask ? launch_vl<T, V, L, true, kBulk>(p, m, g, backward, s)
-              : launch_vl<T, V, L, false, kBulk>(p, m, g, backward, s);
+template <class T, int V>
+cudaError_t launch_v(const Args& p, const Maps& m, const Geometry& g, bool backward, bool mask, cudaStream_t s) {
+  if (g.chunk == 1)
+    return mask ? launch_vl<T, V, 1, true, false>(p, m, g, backward, s)
+                : launch_vl<T, V, 1, false, false>(p, m, g, backward, s);
+  if (g.bulk)
+    return mask ? launch_vl<T, V, chunk_steps(V, true), true, true>(p, m, g, backward, s)
+                : launch_vl<T, V, chunk_steps(V, true), false, true>(p, m, g, backward, s);
+  return mask ? launch_vl<T, V, chunk_steps(V, false), true, false>(p, m, g, backward, s)
+              : launch_vl<T, V, chunk_steps(V, false), false, false>(p, m, g, backward, s);
 }
 
 template <class T>
 cudaError_t launch(const Args& p, const Maps& m, const Geometry& g, bool backward, bool mask, cudaStream_t s) {
-  if (g.bulk) return launch_m<T, 2, kChunk, true>(p, m, g, backward, mask, s);
-  if (g.chunk == 1)
-    return g.vec == 2 ? launch_m<T, 2, 1, false>(p, m, g, backward, mask, s)
-                      : launch_m<T, 1, 1, false>(p, m, g, backward, mask, s);
-  return g.vec == 2 ? launch_m<T, 2, kChunk, false>(p, m, g, backward, mask, s)
-                    : launch_m<T, 1, kChunk, false>(p, m, g, backward, mask, s);
+  return g.vec == 2 ? launch_v<T, 2>(p, m, g, backward, mask, s) : launch_v<T, 1>(p, m, g, backward, mask, s);
 }
 
 }  // namespace gscan

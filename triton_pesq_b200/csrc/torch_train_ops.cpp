@@ -68,10 +68,14 @@ at::Tensor rows(const at::Tensor& t) {
 }
 
 // as aligned as a dense tensor (the pointer and every stride of more than one
-// element a multiple of 4 elements), or a copy that is
+// element a multiple of 16 bytes, or of what a row is), or a copy that is
 at::Tensor aligned(const at::Tensor& t) {
-  const bool ok = reinterpret_cast<uintptr_t>(t.data_ptr()) % (4 * t.element_size()) == 0 &&
-                  (t.size(0) <= 1 || t.stride(0) % 4 == 0) && (t.size(1) <= 1 || t.stride(1) % 4 == 0);
+  const int64_t size = t.element_size();
+  int64_t unit = 16 / size;
+  while (t.size(2) % unit) unit /= 2;
+  const auto good = [&](int64_t n, int64_t stride) { return n <= 1 || (stride > 0 && stride % unit == 0); };
+  const bool ok = reinterpret_cast<uintptr_t>(t.data_ptr()) % (unit * size) == 0 && good(t.size(0), t.stride(0)) &&
+                  good(t.size(1), t.stride(1));
   return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
@@ -208,8 +212,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> gated_sca
   at::Tensor dy;
   pesq_stream dys{nullptr, 0, 0};
   if (dy_.has_value() && dy_->defined()) {
-    dy = rows(dy_->to(x.scalar_type()));
-    if (x.size(2) % 2 == 0) dy = aligned(dy);
+    dy = aligned(rows(dy_->to(x.scalar_type())));
     dys = stream_of(dy);
   }
   size_t work = 0, states = 0, back = 0;
