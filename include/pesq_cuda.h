@@ -392,6 +392,38 @@ int pesq_gated_scan_backward(const pesq_gated_scan_desc* desc, void* stream, con
  * wait that ran out; that call's results are then wrong). */
 int pesq_gated_scan_check(void* stream, uint32_t* failed);
 
+#define PESQ_SIGMOID 0
+#define PESQ_SILU 1
+
+/* The join of a block's output with the residual stream, and the norm before
+ * the next block:
+ *   stream' = stream + scale act(gate) post block / rms(block)
+ *   normed = pre stream' / rms(stream'),  rms(v) = sqrt(mean(v^2) + eps)
+ * over the channels of every row (csrc/norm_join.cuh).  Without a block (NULL)
+ * stream' = stream and only the norm is left. */
+typedef struct pesq_norm_join_desc {
+  int64_t batch, steps, width; /* width: 1 .. 8192 */
+  int32_t stream_dtype;        /* of stream, stream' and their gradients: PESQ_F32, or `dtype` */
+  int32_t dtype;               /* of block, gate, normed and their gradients */
+  int32_t activation;          /* PESQ_SIGMOID or PESQ_SILU */
+  int32_t gate_shared;         /* one gate row a batch item ([batch, 1, channel]; its step stride is not used) */
+  float eps;
+  int32_t reserved0;
+  pesq_stream stream, block, gate; /* gate.data NULL: act = 1 */
+  const float *post, *pre, *scale; /* [width]; scale NULL: 1 */
+} pesq_norm_join_desc;
+
+/* out_stream, normed: [batch, steps, width] dense; out_stream may be NULL without a block. */
+int pesq_norm_join_forward(const pesq_norm_join_desc* desc, void* stream, void* out_stream, void* normed);
+/* Bytes of a backward's workspace. */
+int pesq_norm_join_workspace(const pesq_norm_join_desc* desc, size_t* bytes);
+/* dstream.data or dnormed.data may be NULL (zeros).  dx, dblock, dgate: dense
+ * (dgate [batch, 1, width] where shared); dpost, dpre, dscale: [width].  What
+ * belongs to an operand that is NULL may be NULL. */
+int pesq_norm_join_backward(const pesq_norm_join_desc* desc, void* stream, pesq_stream dstream, pesq_stream dnormed,
+                            void* dx, void* dblock, void* dgate, float* dpost, float* dpre, float* dscale,
+                            void* workspace, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

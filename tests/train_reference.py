@@ -8,10 +8,12 @@ import torch
 ROUND = {t: torch.finfo(t).eps / 2 for t in (torch.float32, torch.bfloat16, torch.float16)}
 
 
-def close(got, want, tol, what=""):
+def close(got, want, tol, what="", terms=None):
     """|got - want| is at most one rounding to got's type, with a quarter to
     spare, plus ``tol`` of the largest value: what the 32-bit arithmetic before
-    that rounding may be off by.  Non-finite values have to agree."""
+    that rounding may be off by.  Where the value is a difference of larger
+    ``terms``, that arithmetic is off by a share of those.  Non-finite values have to
+    agree."""
 
     assert tuple(got.shape) == tuple(want.shape), f"{what}: {tuple(got.shape)} against {tuple(want.shape)}"
     g, w = got.detach().cpu().double(), want.detach().cpu().double()
@@ -21,7 +23,8 @@ def close(got, want, tol, what=""):
     if g.numel() == 0:
         return
     tiny = 2.0**-24 if got.dtype == torch.float16 else 0.0  # spacing of float16 below its normal range
-    allowed = 1.25 * ROUND[got.dtype] * w.abs() + tol * w.abs().max() + tiny
+    size = w.abs().max() if terms is None else torch.maximum(w.abs().max(), terms.abs().max())
+    allowed = 1.25 * ROUND[got.dtype] * w.abs() + tol * size + tiny
     worst = float(((g - w).abs() - allowed).max())
     assert worst <= 0, f"{what}: over the bound by {worst:.3e}, peak {float(w.abs().max()):.3e}"
 
@@ -50,3 +53,22 @@ def gated_scan(x, ig, rg, decay, state=None, reset=None, lengths=None, reverse=F
         else:
             ys[t] = h = new
     return (torch.stack(ys, dim=1) if steps else x.clone()), h
+
+
+def norm_join(stream, block, post, pre, gate=None, scale=None, eps=1e-6, activation="sigmoid", fixed=False):
+    """The two norms, the gate and the residual, operation by operation.
+    ``fixed``: the norms' statistics count as constants, so that autograd gives
+    the terms that a norm's gradient subtracts its mean from."""
+
+    def rms(v):
+        root = torch.sqrt((v * v).mean(dim=-1, keepdim=True) + eps)
+        return v / (root.detach() if fixed else root)
+
+    if block is not None:
+        branch = rms(block) * post
+        if gate is not None:
+            branch = branch * (torch.nn.functional.silu(gate) if activation == "silu" else torch.sigmoid(gate))
+        if scale is not None:
+            branch = branch * scale
+        stream = stream + branch
+    return stream, rms(stream) * pre

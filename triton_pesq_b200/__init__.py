@@ -8,12 +8,16 @@ resampler as a standalone op) and ``IIRCuda`` its ``TritonIIR`` (the causal
 IIR filter as a standalone op) on the same library.
 
 Beside them, the operators of the networks that are trained on the loss:
-``gated_scan`` / ``GatedScanCuda`` (a gated linear recurrence).
+``gated_scan`` / ``GatedScanCuda`` (a gated linear recurrence) and
+``norm_join`` / ``pre_norm`` / ``NormJoinCuda`` (the norms before and after a
+block with its gate and residual).
 """
 
 from .gated_scan import GatedScanCuda, gated_scan
 from .iir import IIRCuda
 from .loss import PesqLossCuda
+from .norm_join import NormJoinCuda, norm_join, pre_norm
 from .resample import ResampleCuda
 
-__all__ = ["PesqLossCuda", "ResampleCuda", "IIRCuda", "GatedScanCuda", "gated_scan"]
+__all__ = ["PesqLossCuda", "ResampleCuda", "IIRCuda", "GatedScanCuda", "gated_scan", "NormJoinCuda",
+           "norm_join", "pre_norm"]

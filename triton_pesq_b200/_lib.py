@@ -154,6 +154,26 @@ class GatedScanDesc(ctypes.Structure):
     ]
 
 
+class NormJoinDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int64),
+        ("steps", ctypes.c_int64),
+        ("width", ctypes.c_int64),
+        ("stream_dtype", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("activation", ctypes.c_int32),
+        ("gate_shared", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("reserved0", ctypes.c_int32),
+        ("stream", Stream),
+        ("block", Stream),
+        ("gate", Stream),
+        ("post", ctypes.c_void_p),
+        ("pre", ctypes.c_void_p),
+        ("scale", ctypes.c_void_p),
+    ]
+
+
 class Shape(ctypes.Structure):
     _fields_ = [("n16", ctypes.c_int64), ("frames", ctypes.c_int32), ("windows", ctypes.c_int32)]
 
@@ -257,6 +277,15 @@ SIGNATURES = {
         [ctypes.POINTER(GatedScanDesc), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, Stream, ctypes.c_void_p,
          ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
          ctypes.c_size_t],
+    ),
+    "pesq_norm_join_forward": (
+        ctypes.c_int, [ctypes.POINTER(NormJoinDesc), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p],
+    ),
+    "pesq_norm_join_workspace": (ctypes.c_int, [ctypes.POINTER(NormJoinDesc), ctypes.POINTER(ctypes.c_size_t)]),
+    "pesq_norm_join_backward": (
+        ctypes.c_int,
+        [ctypes.POINTER(NormJoinDesc), ctypes.c_void_p, Stream, Stream, ctypes.c_void_p, ctypes.c_void_p,
+         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t],
     ),
     "pesq_gated_scan_check": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint32)]),
 }
@@ -367,6 +396,21 @@ def _register_fakes() -> None:
         return (x.new_empty(x.shape), x.new_empty(x.shape), x.new_empty(x.shape),
                 x.new_empty((x.shape[2],), dtype=torch.float32),
                 x.new_empty((x.shape[0], x.shape[2]), dtype=torch.float32))
+
+
+    dtypes = (torch.float32, torch.bfloat16, torch.float16)
+
+    @torch.library.register_fake("pesq_cuda::norm_join_forward")
+    def _norm_join(stream, block, gate, post, pre, scale, eps, silu, shared, dtype):
+        return (stream.new_empty(stream.shape if block is not None else (0,)),
+                stream.new_empty(stream.shape, dtype=dtypes[dtype]))
+
+    @torch.library.register_fake("pesq_cuda::norm_join_backward")
+    def _norm_join_backward(stream, block, gate, post, pre, scale, eps, silu, shared, dtype, dstream, dnormed):
+        def like(t):
+            return stream.new_empty((0,)) if t is None else t.new_empty(t.shape)
+
+        return like(stream), like(block), like(gate), like(post), like(pre), like(scale)
 
 
 def plan_check(handle: int, stream: int = 0) -> int:

@@ -28,7 +28,9 @@ OPS = os.path.join(HERE, "_pesq_torch_ops.so")
 
 CUDA_SOURCES = ["front.cu", "align.cu", "back.cu", "spectrum.cu", "chain.cu", "resample.cu", "pesq_abi.cu", "noalloc.cu",
                 "resample_abi.cu", "iir_abi.cu", "iir_ka.cu", "iir_kb.cu", "iir_kc.cu", "iir_kd.cu", "iir_ke.cu",
-                "iir_kf.cu", "gated_scan_f32.cu", "gated_scan_bf16.cu", "gated_scan_f16.cu", "gated_scan_abi.cu"]
+                "iir_kf.cu", "gated_scan_f32.cu", "gated_scan_bf16.cu", "gated_scan_f16.cu", "gated_scan_abi.cu",
+                "norm_join_f32.cu", "norm_join_bf16.cu", "norm_join_f16.cu", "norm_join_f32_bf16.cu", "norm_join_f32_f16.cu",
+                "norm_join_abi.cu"]
 NVCC_FLAGS = [
     "-std=c++17",
     "-O3",

@@ -1,0 +1,413 @@
+// The join of a block's output with the residual stream, and the norm before
+// the next block, row by row of [batch, step, channel]:
+//
+//   n = post * block / rms(block),        rms(v) = sqrt(mean(v^2) + eps)
+//   stream' = stream + scale * act(gate) * n
+//   normed = pre * stream' / rms(stream')
+//
+// A team of threads keeps a row in registers, eight channels a thread, so each
+// operand is read once and each result written once: the bound is memory.  The
+// next row's operands are on their way while a row is worked on.  The forward
+// takes two sums over a row, one after the other.  The backward needs, with
+// w = scale act n (so that stream' = stream + w) and h = stream' / rms(stream'),
+//
+//   q = dnormed pre,   dr = dstream' + (q - h mean(q h)) / rms(stream')
+//   dblock = (dr scale act post - (block / rms(block)) mean(dr w)) / rms(block)
+//   dgate = dr scale n act',   dstream = dr
+//
+// and mean(dr w) = mean(dstream' w) + (mean(q w) - mean(q h) mean(h w)) / rms(stream'),
+// so its five sums are taken together: two rounds of sums again instead of four.
+// The vectors' gradients are sums over rows of dnormed h (pre) and of
+// u = dr act block / rms(block): dpost = scale sum u, dscale = post sum u.  They stay in
+// registers over the rows of a CTA; the CTAs' sums are added up in a fixed order by a
+// second kernel.  The gradient of a gate that the steps of a batch item share is summed
+// the same way.
+#pragma once
+
+#include <type_traits>
+
+#include "../../include/pesq_cuda.h"
+#include "train.cuh"
+
+namespace pesq {
+namespace njoin {
+
+using namespace train;
+
+constexpr int kEach = 8;      // channels of a thread
+constexpr int kThreads = 128; // of a CTA, unless a row takes more
+// threads an SM holds, which the registers of one follow from (72 and 128)
+constexpr int kForwardThreads = 896, kBackwardThreads = 512;
+constexpr int ctas(int threads_of_sm, int team) {
+  const int threads = team > kThreads ? team : kThreads;
+  return threads_of_sm / threads > 0 ? threads_of_sm / threads : 1;
+}
+
+struct Rows {
+  const void* p;
+  int64_t sb, st;  // strides of batch and step, in elements
+};
+
+struct Args {
+  Rows stream, block, gate, dstream, dnormed;  // block, gate and either upstream gradient may be null
+  const float *post, *pre, *scale;             // scale may be null (ones)
+  int64_t batch, steps;
+  int width;
+  int units, span;  // CTAs of a batch item, rows of a CTA
+  int silu;
+  float eps;
+  void *out_stream, *out_normed;  // forward, dense; the stream may be null
+  void *dx, *dblock, *dgate;      // backward, dense; dgate null where it is shared
+  float *part_u, *part_pre, *part_gate;  // [batch * units, width]; part_gate null where the gate is not shared
+};
+
+// Sums of K values over a team: by shuffles within a warp, through shared
+// memory across warps (two buffers in turn, so that one barrier a round is enough).
+template <int K, int TEAM>
+__device__ __forceinline__ void team_sum(float (&v)[K], float (*s_sum)[32][8], int& turn) {
+#pragma unroll
+  for (int off = (TEAM < 32 ? TEAM : 32) / 2; off > 0; off >>= 1)
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], off);
+  if (TEAM > 32) {
+    constexpr int W = TEAM / 32;
+    const int warp = threadIdx.x >> 5, first = warp / W * W;
+    float(*s)[8] = s_sum[turn];
+    turn ^= 1;
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) s[warp][k] = v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float t = 0.0f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) t += s[first + w][k];
+      v[k] = t;
+    }
+  }
+}
+
+// A thread's channels: eight in a row as 16-byte accesses (kWide), or one in
+// every TEAM.  Those past the width are zero.  They stay as the words they were
+// read as until they are used.
+template <class T, int TEAM, bool kWide>
+struct Eight {
+  static constexpr int kWords = kWide ? kEach * (int)sizeof(T) / 4 : kEach;
+  unsigned w[kWords];
+
+  static __device__ __forceinline__ int column(int j) {
+    const int t = threadIdx.x % TEAM;
+    return kWide ? t * kEach + j : t + j * TEAM;
+  }
+  __device__ __forceinline__ void load(const void* base, int64_t row, int width, bool take) {
+    const T* r = static_cast<const T*>(base) + row;
+    if (kWide) {
+      take = take && column(0) < width;
+      const uint4* q = reinterpret_cast<const uint4*>(r + column(0));
+#pragma unroll
+      for (int i = 0; i < kWords / 4; ++i) {
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (take) v = q[i];
+        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        w[j] = 0u;
+        if (take && column(j) < width) {
+          if constexpr (sizeof(T) == 4)
+            w[j] = reinterpret_cast<const unsigned*>(r)[column(j)];
+          else
+            w[j] = reinterpret_cast<const unsigned short*>(r)[column(j)];
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ float at(int j) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[j]);
+    } else {
+      const unsigned v = kWide ? w[j / 2] : w[j], half = kWide && j % 2 ? v >> 16 : v & 0xffffu;
+      if constexpr (std::is_same<T, __half>::value) {
+        return __half2float(__ushort_as_half((unsigned short)half));
+      } else {
+        return __uint_as_float(kWide && j % 2 ? v & 0xffff0000u : v << 16);
+      }
+    }
+  }
+  // channels j and j + 1 (j even)
+  __device__ __forceinline__ void set(int j, float a, float b) {
+    if constexpr (sizeof(T) == 4) {
+      w[j] = __float_as_uint(a), w[j + 1] = __float_as_uint(b);
+    } else {
+      unsigned v;
+      if constexpr (std::is_same<T, __half>::value)
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(b), "f"(a));
+      else
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(b), "f"(a));
+      if (kWide)
+        w[j / 2] = v;
+      else
+        w[j] = v & 0xffffu, w[j + 1] = v >> 16;
+    }
+  }
+  __device__ __forceinline__ void store(void* base, int64_t row, int width) const {
+    T* r = static_cast<T*>(base) + row;
+    if (kWide) {
+      uint4* q = reinterpret_cast<uint4*>(r + column(0));
+      if (column(0) < width) {
+#pragma unroll
+        for (int i = 0; i < kWords / 4; ++i) q[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kEach; ++j)
+        if (column(j) < width) {
+          if constexpr (sizeof(T) == 4)
+            reinterpret_cast<unsigned*>(r)[column(j)] = w[j];
+          else
+            reinterpret_cast<unsigned short*>(r)[column(j)] = (unsigned short)w[j];
+        }
+    }
+  }
+};
+
+struct Act {
+  float value, slope;
+};
+__device__ __forceinline__ Act act_of(float g, int silu) {
+  const float s = rcp_approx(1.0f + exp2_approx(-g * kLog2e));
+  return silu ? Act{g * s, s * fmaf(g, 1.0f - s, 1.0f)} : Act{s, s * (1.0f - s)};
+}
+
+// The row that a team works on in its k-th turn, dense and for an operand
+template <int TEAM, int THREADS>
+struct Turn {
+  int64_t b, t;
+  bool on;
+  __device__ __forceinline__ Turn(const Args& p, int k) {
+    b = blockIdx.x / p.units;
+    const int unit = blockIdx.x - (int)b * p.units;
+    const int in = k * (THREADS / TEAM) + threadIdx.x / TEAM;
+    t = (int64_t)unit * p.span + in;
+    on = in < p.span && t < p.steps;
+  }
+  __device__ __forceinline__ int64_t of(const Rows& r) const { return b * r.sb + t * r.st; }
+  __device__ __forceinline__ int64_t dense(const Args& p) const { return (b * p.steps + t) * p.width; }
+};
+
+// ------------------------------------------------------------------- forward
+
+template <class TS, class TB, int TEAM, bool kWide>
+__global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(kForwardThreads, TEAM)) forward_kernel(const __grid_constant__ Args p) {
+  constexpr int THREADS = TEAM > kThreads ? TEAM : kThreads, TEAMS = THREADS / TEAM;
+  using S = Eight<TS, TEAM, kWide>;
+  using B = Eight<TB, TEAM, kWide>;
+  using F = Eight<float, TEAM, kWide>;
+  __shared__ float s_sum[2][32][8];
+  int turn = 0;
+  F post, pre, scale;
+  pre.load(p.pre, 0, p.width, true);
+  post.load(p.post, 0, p.width, p.post != nullptr);
+  scale.load(p.scale, 0, p.width, p.scale != nullptr);
+  if (p.scale) {
+#pragma unroll
+    for (int j = 0; j < kEach; j += 2) post.set(j, post.at(j) * scale.at(j), post.at(j + 1) * scale.at(j + 1));
+  }
+  const int turns = (p.span + TEAMS - 1) / TEAMS;
+  const float inv = 1.0f / (float)p.width;
+  S x;
+  B z, g;
+  Turn<TEAM, THREADS> now(p, 0);
+  x.load(p.stream.p, now.of(p.stream), p.width, now.on);
+  z.load(p.block.p, now.of(p.block), p.width, now.on && p.block.p);
+  g.load(p.gate.p, now.of(p.gate), p.width, now.on && p.gate.p);
+#pragma unroll 1
+  for (int k = 0; k < turns; ++k) {
+    const Turn<TEAM, THREADS> next(p, k + 1);
+    S x1;
+    B z1, g1;
+    x1.load(p.stream.p, next.of(p.stream), p.width, next.on);
+    z1.load(p.block.p, next.of(p.block), p.width, next.on && p.block.p);
+    g1.load(p.gate.p, next.of(p.gate), p.width, next.on && p.gate.p);
+
+    float r[kEach], sum[1] = {0.0f};
+    if (p.block.p) {
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) sum[0] = fmaf(z.at(j), z.at(j), sum[0]);
+      team_sum<1, TEAM>(sum, s_sum, turn);
+      const float rz = rsqrt_approx(fmaf(sum[0], inv, p.eps));
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        float w = z.at(j) * rz * post.at(j);
+        if (p.gate.p) w *= act_of(g.at(j), p.silu).value;
+        r[j] = x.at(j) + w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) r[j] = x.at(j);
+    }
+    sum[0] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) sum[0] = fmaf(r[j], r[j], sum[0]);
+    team_sum<1, TEAM>(sum, s_sum, turn);
+    const float rr = rsqrt_approx(fmaf(sum[0], inv, p.eps));
+    if (now.on) {
+      S out;
+      B y;
+#pragma unroll
+      for (int j = 0; j < kEach; j += 2) {
+        out.set(j, r[j], r[j + 1]);
+        y.set(j, r[j] * rr * pre.at(j), r[j + 1] * rr * pre.at(j + 1));
+      }
+      if (p.out_stream) out.store(p.out_stream, now.dense(p), p.width);
+      y.store(p.out_normed, now.dense(p), p.width);
+    }
+    x = x1, z = z1, g = g1, now = next;
+  }
+}
+
+// ------------------------------------------------------------------ backward
+
+// The CTA's sum of what its teams hold, to a row of `part`
+template <int TEAM, int TEAMS, bool kWide>
+__device__ __forceinline__ void store_part(const float (&v)[kEach], float* part, int width, float* s_part) {
+  using F = Eight<float, TEAM, kWide>;
+  F f;
+#pragma unroll
+  for (int j = 0; j < kEach; j += 2) f.set(j, v[j], v[j + 1]);
+  if (TEAMS == 1) {
+    f.store(part, (int64_t)blockIdx.x * width, width);
+    return;
+  }
+  const int team = threadIdx.x / TEAM;
+  f.store(s_part, (int64_t)team * kEach * TEAM, kEach * TEAM);
+  __syncthreads();
+  for (int c = threadIdx.x; c < width; c += TEAM * TEAMS) {
+    float t = 0.0f;
+#pragma unroll 8
+    for (int w = 0; w < TEAMS; ++w) t += s_part[w * kEach * TEAM + c];
+    part[(int64_t)blockIdx.x * width + c] = t;
+  }
+  __syncthreads();
+}
+
+template <class TS, class TB, int TEAM, bool kWide>
+__global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(kBackwardThreads, TEAM)) backward_kernel(const __grid_constant__ Args p) {
+  constexpr int THREADS = TEAM > kThreads ? TEAM : kThreads, TEAMS = THREADS / TEAM;
+  using S = Eight<TS, TEAM, kWide>;
+  using B = Eight<TB, TEAM, kWide>;
+  using F = Eight<float, TEAM, kWide>;
+  __shared__ float s_sum[2][32][8];
+  __shared__ __align__(16) float s_part[TEAMS > 1 ? THREADS * kEach : 4];
+  int turn = 0;
+  F post, pre;  // post times scale
+  pre.load(p.pre, 0, p.width, true);
+  post.load(p.post, 0, p.width, p.post != nullptr);
+  if (p.scale) {
+    F scale;
+    scale.load(p.scale, 0, p.width, true);
+#pragma unroll
+    for (int j = 0; j < kEach; j += 2) post.set(j, post.at(j) * scale.at(j), post.at(j + 1) * scale.at(j + 1));
+  }
+  float acc_u[kEach], acc_pre[kEach], acc_gate[kEach];
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) acc_u[j] = acc_pre[j] = acc_gate[j] = 0.0f;
+  const int turns = (p.span + TEAMS - 1) / TEAMS;
+  const float inv = 1.0f / (float)p.width;
+  S x, ds;
+  B z, g, dy;
+  const auto load = [&](const Turn<TEAM, THREADS>& at, S& x, S& ds, B& z, B& g, B& dy) {
+    z.load(p.block.p, at.of(p.block), p.width, at.on && p.block.p);
+    g.load(p.gate.p, at.of(p.gate), p.width, at.on && p.gate.p);
+    x.load(p.stream.p, at.of(p.stream), p.width, at.on);
+    dy.load(p.dnormed.p, at.of(p.dnormed), p.width, at.on && p.dnormed.p);
+    ds.load(p.dstream.p, at.of(p.dstream), p.width, at.on && p.dstream.p);
+  };
+  Turn<TEAM, THREADS> now(p, 0);
+  load(now, x, ds, z, g, dy);
+#pragma unroll 1
+  for (int k = 0; k < turns; ++k) {
+    const Turn<TEAM, THREADS> next(p, k + 1);
+    S x1, ds1;
+    B z1, g1, dy1;
+    load(next, x1, ds1, z1, g1, dy1);
+
+    float rz = 0.0f;
+    if (p.block.p) {
+      float one[1] = {0.0f};
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) one[0] = fmaf(z.at(j), z.at(j), one[0]);
+      team_sum<1, TEAM>(one, s_sum, turn);
+      rz = now.on ? rsqrt_approx(fmaf(one[0], inv, p.eps)) : 0.0f;
+    }
+    // sums of r^2, q r, ds w, q w, r w
+    float w[kEach], value[kEach], slope[kEach], sum[5] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      Act a{1.0f, 0.0f};
+      if (p.gate.p) a = act_of(g.at(j), p.silu);
+      value[j] = a.value, slope[j] = a.slope;
+      w[j] = z.at(j) * rz * post.at(j) * a.value;
+      const float r = x.at(j) + w[j], q = dy.at(j) * pre.at(j);
+      sum[0] = fmaf(r, r, sum[0]);
+      sum[1] = fmaf(q, r, sum[1]);
+      sum[2] = fmaf(ds.at(j), w[j], sum[2]);
+      sum[3] = fmaf(q, w[j], sum[3]);
+      sum[4] = fmaf(r, w[j], sum[4]);
+    }
+    team_sum<5, TEAM>(sum, s_sum, turn);
+    // (a row that is off is zeros, and adds zeros for any eps)
+    const float rr = now.on ? rsqrt_approx(fmaf(sum[0], inv, p.eps)) : 0.0f;
+    const float mq = sum[1] * inv * rr * rr;                        // mean(q h) / rms
+    const float mw = (sum[2] + rr * (sum[3] - mq * sum[4])) * inv;  // mean(dr w)
+    float dx[kEach], dz[kEach], dg[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const float r = x.at(j) + w[j], zh = z.at(j) * rz;
+      dx[j] = fmaf(rr, fmaf(dy.at(j), pre.at(j), -r * mq), ds.at(j));
+      const float u = dx[j] * zh;
+      dg[j] = u * post.at(j) * slope[j];
+      dz[j] = rz * fmaf(dx[j] * post.at(j), value[j], -zh * mw);
+      acc_u[j] = fmaf(u, value[j], acc_u[j]);
+      acc_pre[j] = fmaf(dy.at(j), r * rr, acc_pre[j]);
+      acc_gate[j] += dg[j];
+    }
+    if (now.on) {
+      const int64_t at = now.dense(p);
+      S a;
+      B b;
+#pragma unroll
+      for (int j = 0; j < kEach; j += 2) a.set(j, dx[j], dx[j + 1]);
+      a.store(p.dx, at, p.width);
+      if (p.dblock) {
+#pragma unroll
+        for (int j = 0; j < kEach; j += 2) b.set(j, dz[j], dz[j + 1]);
+        b.store(p.dblock, at, p.width);
+      }
+      if (p.dgate) {
+#pragma unroll
+        for (int j = 0; j < kEach; j += 2) b.set(j, dg[j], dg[j + 1]);
+        b.store(p.dgate, at, p.width);
+      }
+    }
+    x = x1, ds = ds1, z = z1, g = g1, dy = dy1, now = next;
+  }
+  if (p.part_u) store_part<TEAM, TEAMS, kWide>(acc_u, p.part_u, p.width, s_part);
+  store_part<TEAM, TEAMS, kWide>(acc_pre, p.part_pre, p.width, s_part);
+  if (p.part_gate) store_part<TEAM, TEAMS, kWide>(acc_gate, p.part_gate, p.width, s_part);
+}
+
+struct Geometry {
+  int team;
+  bool wide;
+  int64_t blocks;
+};
+
+template <class TS, class TB>
+cudaError_t launch(const Args& p, const Geometry& g, bool backward, cudaStream_t s);
+
+}  // namespace njoin
+}  // namespace pesq

@@ -1,0 +1,8 @@
+// The join's kernels for a stream of float and blocks of float.
+#include "norm_join_launch.cuh"
+
+namespace pesq {
+namespace njoin {
+template cudaError_t launch<float, float>(const Args&, const Geometry&, bool, cudaStream_t);
+}  // namespace njoin
+}  // namespace pesq

@@ -1,0 +1,8 @@
+// The join's kernels for a stream of float and blocks of __nv_bfloat16.
+#include "norm_join_launch.cuh"
+
+namespace pesq {
+namespace njoin {
+template cudaError_t launch<float, __nv_bfloat16>(const Args&, const Geometry&, bool, cudaStream_t);
+}  // namespace njoin
+}  // namespace pesq

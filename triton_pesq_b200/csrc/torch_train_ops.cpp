@@ -284,6 +284,195 @@ std::tuple<at::Tensor, at::Tensor> gated_scan(const at::Tensor& x, const at::Ten
   return {y, last};
 }
 
+// ------------------------------------------------------------------- norm join
+
+constexpr const char* kJoin = "norm join";
+
+bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+struct JoinCall {
+  at::Tensor x, z, g, post, pre, scale;
+  pesq_norm_join_desc d{};
+  at::ScalarType out;
+
+  at::Tensor vector(const at::Tensor& t, const char* name) {
+    check_cuda(t, x, kJoin, name);
+    check_float(t, kJoin, name);
+    check_shape(t, {x.size(2)}, kJoin, name);
+    return t.contiguous();
+  }
+
+  JoinCall(const at::Tensor& x_, const OptTensor& z_, const OptTensor& g_, const OptTensor& post_,
+           const at::Tensor& pre_, const OptTensor& scale_, double eps, bool silu, bool shared, int64_t dtype) {
+    check_cuda(x_, x_, kJoin, "stream");
+    TORCH_CHECK(x_.dim() == 3, "The CUDA norm join needs `stream` [batch, step, channel], got ", x_.sizes(), ".");
+    d.stream_dtype = dtype_code(x_, kJoin, "stream");
+    d.dtype = static_cast<int32_t>(dtype);
+    out = dtype == PESQ_F32 ? at::kFloat : dtype == PESQ_BF16 ? at::kBFloat16 : at::kHalf;
+    TORCH_CHECK_VALUE(eps >= 0.0, "The CUDA norm join needs an `eps` that is not negative, got ", eps, ".");
+    TORCH_CHECK(x_.scalar_type() == at::kFloat || x_.scalar_type() == out,
+                "The CUDA norm join needs `stream` in float32 or in the block's type, it is ", x_.scalar_type(), ".");
+    x = rows(x_);
+    d.batch = x.size(0);
+    d.steps = x.size(1);
+    d.width = x.size(2);
+    d.activation = silu ? PESQ_SILU : PESQ_SIGMOID;
+    d.gate_shared = shared;
+    d.eps = static_cast<float>(eps);
+    d.stream = stream_of(x);
+    pre = vector(pre_, "pre_weight");
+    d.pre = pre.data_ptr<float>();
+    if (!given(z_)) {
+      TORCH_CHECK_VALUE(!given(g_), "The CUDA norm join needs a `block` for its `gate`.");
+      return;
+    }
+    check_cuda(*z_, x, kJoin, "block");
+    check_shape(*z_, x.sizes(), kJoin, "block");
+    TORCH_CHECK(z_->scalar_type() == out, "The CUDA norm join needs `block` in ", out, ", it is ", z_->scalar_type(), ".");
+    z = rows(*z_);
+    d.block = stream_of(z);
+    TORCH_CHECK_VALUE(given(post_), "The CUDA norm join needs `post_weight`.");
+    post = vector(*post_, "post_weight");
+    d.post = post.data_ptr<float>();
+    if (given(g_)) {
+      check_cuda(*g_, x, kJoin, "gate");
+      const int64_t want[3] = {d.batch, shared ? 1 : d.steps, d.width};
+      check_shape(*g_, want, kJoin, "gate");
+      TORCH_CHECK(g_->scalar_type() == out, "The CUDA norm join needs `gate` in the block's type ", out, ", it is ",
+                  g_->scalar_type(), ".");
+      g = rows(*g_);
+      d.gate = stream_of(g);
+    }
+    if (given(scale_)) {
+      scale = vector(*scale_, "scale");
+      d.scale = scale.data_ptr<float>();
+    }
+  }
+
+  bool empty() const { return x.numel() == 0; }
+};
+
+// (stream', normed); stream' is empty without a block
+std::tuple<at::Tensor, at::Tensor> norm_join_forward(const at::Tensor& x, const OptTensor& z, const OptTensor& g,
+                                                     const OptTensor& post, const at::Tensor& pre,
+                                                     const OptTensor& scale, double eps, bool silu, bool shared,
+                                                     int64_t dtype) {
+  JoinCall c(x, z, g, post, pre, scale, eps, silu, shared, dtype);
+  c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor out = c.z.defined() ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
+  at::Tensor normed = at::empty(x.sizes(), x.options().dtype(c.out));
+  if (!c.empty())
+    check_status(pesq_norm_join_forward(&c.d, at::cuda::getCurrentCUDAStream(),
+                                        c.z.defined() ? out.data_ptr() : nullptr, normed.data_ptr()),
+                 "pesq_norm_join_forward");
+  return {out, normed};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> norm_join_backward(
+    const at::Tensor& x, const OptTensor& z, const OptTensor& g, const OptTensor& post, const at::Tensor& pre,
+    const OptTensor& scale, double eps, bool silu, bool shared, int64_t dtype, const OptTensor& dstream_,
+    const OptTensor& dnormed_) {
+  JoinCall c(x, z, g, post, pre, scale, eps, silu, shared, dtype);
+  c10::cuda::CUDAGuard guard(x.device());
+  const auto make = [&](const at::Tensor& t) {
+    return t.defined() ? at::empty(t.sizes(), t.options()) : at::empty({0}, x.options());
+  };
+  at::Tensor dx = make(c.x), dz = make(c.z), dg = make(c.g), dpost = make(c.post), dpre = make(c.pre),
+             dscale = make(c.scale);
+  if (c.empty()) {
+    for (at::Tensor* t : {&dpost, &dpre, &dscale, &dg}) t->zero_();
+    return {dx, dz, dg, dpost, dpre, dscale};
+  }
+  at::Tensor ds, dn;
+  pesq_stream s{nullptr, 0, 0}, n{nullptr, 0, 0};
+  if (given(dstream_)) {
+    ds = rows(dstream_->to(x.scalar_type()));
+    s = stream_of(ds);
+  }
+  if (given(dnormed_)) {
+    dn = rows(dnormed_->to(c.out));
+    n = stream_of(dn);
+  }
+  size_t bytes = 0;
+  check_status(pesq_norm_join_workspace(&c.d, &bytes), "pesq_norm_join_workspace");
+  at::Tensor ws = at::empty({static_cast<int64_t>(bytes)}, x.options().dtype(at::kByte));
+  const auto vec = [](const at::Tensor& have, at::Tensor& t) { return have.defined() ? t.data_ptr<float>() : nullptr; };
+  check_status(pesq_norm_join_backward(&c.d, at::cuda::getCurrentCUDAStream(), s, n, dx.data_ptr(),
+                                       c.z.defined() ? dz.data_ptr() : nullptr,
+                                       c.g.defined() ? dg.data_ptr() : nullptr, vec(c.post, dpost), vec(c.pre, dpre),
+                                       vec(c.scale, dscale), ws.data_ptr(), bytes),
+               "pesq_norm_join_backward");
+  return {dx, dz, dg, dpost, dpre, dscale};
+}
+
+const auto& join_forward_op() {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("pesq_cuda::norm_join_forward", "")
+                       .typed<decltype(norm_join_forward)>();
+  return op;
+}
+const auto& join_backward_op() {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("pesq_cuda::norm_join_backward", "")
+                       .typed<decltype(norm_join_backward)>();
+  return op;
+}
+
+struct NormJoin : public torch::autograd::Function<NormJoin> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const OptTensor& z, const OptTensor& g,
+                               const OptTensor& post, const at::Tensor& pre, const OptTensor& scale, double eps,
+                               bool silu, bool shared, int64_t dtype) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [out, normed] = join_forward_op().call(x, z, g, post, pre, scale, eps, silu, shared, dtype);
+    const auto or_none = [](const OptTensor& t) { return t.value_or(at::Tensor()); };
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, or_none(z), or_none(g), or_none(post), pre, or_none(scale)});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["silu"] = silu;
+    ctx->saved_data["shared"] = shared;
+    ctx->saved_data["dtype"] = dtype;
+    return {out, normed};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grad) {
+    no_second_derivative(kJoin);
+    const auto s = ctx->get_saved_variables();
+    variable_list out(10);
+    if (!grad[0].defined() && !grad[1].defined()) return out;
+    const OptTensor dstream = s[1].defined() ? optional_of(grad[0]) : std::nullopt;
+    auto [dx, dz, dg, dpost, dpre, dscale] = join_backward_op().call(
+        s[0], optional_of(s[1]), optional_of(s[2]), optional_of(s[3]), s[4], optional_of(s[5]),
+        ctx->saved_data["eps"].toDouble(), ctx->saved_data["silu"].toBool(), ctx->saved_data["shared"].toBool(),
+        ctx->saved_data["dtype"].toInt(), dstream, optional_of(grad[1]));
+    out[0] = dx;
+    if (s[1].defined()) out[1] = dz, out[3] = dpost;
+    if (s[2].defined()) out[2] = dg;
+    out[4] = dpre;
+    if (s[1].defined() && s[5].defined()) out[5] = dscale;
+    return out;
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> norm_join(const at::Tensor& x, const OptTensor& z, const OptTensor& g_,
+                                             const OptTensor& post, const at::Tensor& pre, const OptTensor& scale,
+                                             double eps, bool silu, int64_t dtype) {
+  check_cuda(x, x, kJoin, "stream");
+  TORCH_CHECK(x.dim() == 3, "The CUDA norm join needs `stream` [batch, step, channel], got ", x.sizes(), ".");
+  // one gate row for all steps of a batch item is summed by the kernels, any other broadcast by torch
+  OptTensor g = g_;
+  bool shared = false;
+  if (given(g) && g->sizes() != x.sizes()) {
+    shared = g->dim() == 3 && g->size(0) == x.size(0) && g->size(1) == 1 && g->size(2) == x.size(2);
+    if (!shared) g = g->expand(x.sizes());
+  }
+  if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(z) || wants_grad(g) || wants_grad(post) ||
+                                     wants_grad(pre) || wants_grad(scale))) {
+    auto out = NormJoin::apply(x, z, g, post, pre, scale, eps, silu, shared, dtype);
+    return {out[0], out[1]};
+  }
+  return join_forward_op().call(x, z, g, post, pre, scale, eps, silu, shared, dtype);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(pesq_cuda, m) {
@@ -295,11 +484,22 @@ TORCH_LIBRARY_FRAGMENT(pesq_cuda, m) {
   m.def((std::string("gated_scan_backward") + scan_in +
          ", Tensor kept, Tensor? dy, Tensor? dlast) -> (Tensor, Tensor, Tensor, Tensor, Tensor)")
             .c_str());
+  const char* join_in = "(Tensor stream, Tensor? block, Tensor? gate, Tensor? post, Tensor pre, Tensor? scale, float eps, bool silu";
+  m.def((std::string("norm_join") + join_in + ", int dtype) -> (Tensor, Tensor)").c_str());
+  m.def((std::string("norm_join_forward") + join_in + ", bool shared, int dtype) -> (Tensor, Tensor)").c_str());
+  m.def((std::string("norm_join_backward") + join_in +
+         ", bool shared, int dtype, Tensor? dstream, Tensor? dnormed) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)")
+            .c_str());
 }
 
-TORCH_LIBRARY_IMPL(pesq_cuda, CompositeImplicitAutograd, m) { m.impl("gated_scan", &gated_scan); }
+TORCH_LIBRARY_IMPL(pesq_cuda, CompositeImplicitAutograd, m) {
+  m.impl("gated_scan", &gated_scan);
+  m.impl("norm_join", &norm_join);
+}
 
 TORCH_LIBRARY_IMPL(pesq_cuda, CUDA, m) {
   m.impl("gated_scan_forward", &gated_scan_forward);
   m.impl("gated_scan_backward", &gated_scan_backward);
+  m.impl("norm_join_forward", &norm_join_forward);
+  m.impl("norm_join_backward", &norm_join_backward);
 }
