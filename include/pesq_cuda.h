@@ -424,6 +424,33 @@ int pesq_norm_join_backward(const pesq_norm_join_desc* desc, void* stream, pesq_
                             void* dx, void* dblock, void* dgate, float* dpost, float* dpre, float* dscale,
                             void* workspace, size_t workspace_bytes);
 
+/* One tensor of an AdamW step.  Its moments are the next ceil(n / 256) units of
+ * 256 values of the moments' buffers. */
+typedef struct pesq_adamw_tensor {
+  float* param;      /* [n] */
+  const void* grad;  /* [n], of grad_dtype; NULL leaves the tensor and its moments as they are */
+  void* copy;        /* [n], the new values in the gradients' 16-bit type; or NULL */
+  int64_t n;
+} pesq_adamw_tensor;
+
+typedef struct pesq_adamw_desc {
+  int32_t grad_dtype; /* PESQ_F32, PESQ_BF16 or PESQ_F16 */
+  int32_t state_bits; /* 32: float moments; 8: float8 (e4m3) moments, the second as its root, in units of scales */
+  int64_t units;      /* units of 256 values that the moments' buffers hold */
+  void *moment1, *moment2;  /* [units * 256] */
+  float *scale1, *scale2;   /* [units], 8 bits */
+  int64_t* step;      /* device [2]: steps taken; 0 between calls (counts a launch's blocks) */
+  const float* grad_scale;  /* device, times every gradient; the step is skipped where it is not finite; NULL: 1 */
+  double beta1, beta2;
+  float lr, eps, weight_decay;
+  uint32_t seed;      /* of the 8-bit second moment's rounding */
+} pesq_adamw_desc;
+
+/* m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2,
+ * p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
+ * over all tensors in one launch (csrc/adamw.cu; one more for every further 800 tensors). */
+int pesq_adamw_step(const pesq_adamw_desc* desc, const pesq_adamw_tensor* tensors, int64_t count, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -72,3 +72,12 @@ def norm_join(stream, block, post, pre, gate=None, scale=None, eps=1e-6, activat
             branch = branch * scale
         stream = stream + branch
     return stream, rms(stream) * pre
+
+
+def adamw(p, g, m, v, t, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, decay=1e-2):
+    """New (p, m, v) of step t (the first is 1)."""
+
+    m = betas[0] * m + (1 - betas[0]) * g
+    v = betas[1] * v + (1 - betas[1]) * g * g
+    p = p - lr * decay * p - lr * (m / (1 - betas[0] ** t)) / (torch.sqrt(v / (1 - betas[1] ** t)) + eps)
+    return p, m, v

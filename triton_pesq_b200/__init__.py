@@ -8,11 +8,13 @@ resampler as a standalone op) and ``IIRCuda`` its ``TritonIIR`` (the causal
 IIR filter as a standalone op) on the same library.
 
 Beside them, the operators of the networks that are trained on the loss:
-``gated_scan`` / ``GatedScanCuda`` (a gated linear recurrence) and
+``gated_scan`` / ``GatedScanCuda`` (a gated linear recurrence),
 ``norm_join`` / ``pre_norm`` / ``NormJoinCuda`` (the norms before and after a
-block with its gate and residual).
+block with its gate and residual) and ``adamw_step`` / ``AdamWCuda`` (the
+optimiser over all parameters at once).
 """
 
+from .adamw import AdamWCuda, adamw_step
 from .gated_scan import GatedScanCuda, gated_scan
 from .iir import IIRCuda
 from .loss import PesqLossCuda
@@ -20,4 +22,4 @@ from .norm_join import NormJoinCuda, norm_join, pre_norm
 from .resample import ResampleCuda
 
 __all__ = ["PesqLossCuda", "ResampleCuda", "IIRCuda", "GatedScanCuda", "gated_scan", "NormJoinCuda",
-           "norm_join", "pre_norm"]
+           "norm_join", "pre_norm", "AdamWCuda", "adamw_step"]

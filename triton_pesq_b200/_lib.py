@@ -174,6 +174,35 @@ class NormJoinDesc(ctypes.Structure):
     ]
 
 
+class AdamwTensor(ctypes.Structure):
+    _fields_ = [
+        ("param", ctypes.c_void_p),
+        ("grad", ctypes.c_void_p),
+        ("copy", ctypes.c_void_p),
+        ("n", ctypes.c_int64),
+    ]
+
+
+class AdamwDesc(ctypes.Structure):
+    _fields_ = [
+        ("grad_dtype", ctypes.c_int32),
+        ("state_bits", ctypes.c_int32),
+        ("units", ctypes.c_int64),
+        ("moment1", ctypes.c_void_p),
+        ("moment2", ctypes.c_void_p),
+        ("scale1", ctypes.c_void_p),
+        ("scale2", ctypes.c_void_p),
+        ("step", ctypes.c_void_p),
+        ("grad_scale", ctypes.c_void_p),
+        ("beta1", ctypes.c_double),
+        ("beta2", ctypes.c_double),
+        ("lr", ctypes.c_float),
+        ("eps", ctypes.c_float),
+        ("weight_decay", ctypes.c_float),
+        ("seed", ctypes.c_uint32),
+    ]
+
+
 class Shape(ctypes.Structure):
     _fields_ = [("n16", ctypes.c_int64), ("frames", ctypes.c_int32), ("windows", ctypes.c_int32)]
 
@@ -286,6 +315,10 @@ SIGNATURES = {
         ctypes.c_int,
         [ctypes.POINTER(NormJoinDesc), ctypes.c_void_p, Stream, Stream, ctypes.c_void_p, ctypes.c_void_p,
          ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t],
+    ),
+    "pesq_adamw_step": (
+        ctypes.c_int,
+        [ctypes.POINTER(AdamwDesc), ctypes.POINTER(AdamwTensor), ctypes.c_int64, ctypes.c_void_p],
     ),
     "pesq_gated_scan_check": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint32)]),
 }
@@ -411,6 +444,12 @@ def _register_fakes() -> None:
             return stream.new_empty((0,)) if t is None else t.new_empty(t.shape)
 
         return like(stream), like(block), like(gate), like(post), like(pre), like(scale)
+
+
+    @torch.library.register_fake("pesq_cuda::adamw_step")
+    def _adamw_step(params, grads, moment1, moment2, step, scales, copies, lr, beta1, beta2, eps, weight_decay,
+                    grad_scale, seed):
+        return None
 
 
 def plan_check(handle: int, stream: int = 0) -> int:

@@ -30,7 +30,7 @@ CUDA_SOURCES = ["front.cu", "align.cu", "back.cu", "spectrum.cu", "chain.cu", "r
                 "resample_abi.cu", "iir_abi.cu", "iir_ka.cu", "iir_kb.cu", "iir_kc.cu", "iir_kd.cu", "iir_ke.cu",
                 "iir_kf.cu", "gated_scan_f32.cu", "gated_scan_bf16.cu", "gated_scan_f16.cu", "gated_scan_abi.cu",
                 "norm_join_f32.cu", "norm_join_bf16.cu", "norm_join_f16.cu", "norm_join_f32_bf16.cu", "norm_join_f32_f16.cu",
-                "norm_join_abi.cu"]
+                "norm_join_abi.cu", "adamw.cu"]
 NVCC_FLAGS = [
     "-std=c++17",
     "-O3",

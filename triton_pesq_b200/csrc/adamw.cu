@@ -1,0 +1,415 @@
+// AdamW over many tensors in one launch, moments in 32 or in 8 bits.
+//
+// With g the gradient (times grad_scale), t the step:
+//   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
+//   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
+//
+// Every value is read and written once: the bound is memory (28 bytes a value
+// with 32-bit moments and gradients, 18 with 8-bit moments, a 16-bit gradient and
+// a 16-bit copy).  All tensors go in one launch: their addresses and sizes travel as
+// kernel parameters, so nothing of them is kept or copied beforehand.  The moments
+// of all tensors lie in one buffer each, a tensor's part beginning at a multiple of
+// 256 values, so that the blocks of 256 of the buffer are the units of work, and one warp
+// takes a unit: eight values a lane.  A warp finds its tensor by bisection.
+//
+// 8 bits.  A block of 256 has a 32-bit scale, its largest magnitude / 448, and its
+// values are float8 (e4m3) in units of it.  The first moment is rounded to nearest:
+// it moves by a tenth of itself a step, more than half the rounding step, so it is not stuck.
+// The second moment is kept as its root, which halves the range that 8 bits have to
+// span (2^-9 .. 448 of the root are 10 decades of the moment), and moves by less
+// than 1 / 2000 of itself a step, where nearest rounding (steps of 1/8) would
+// hold it for good: it is rounded stochastically, with bits that are a hash of
+// position, step and seed, so that its mean is right and a run can be repeated.
+// A root that is not zero is never rounded to zero: the update would divide by
+// the gradient's own share alone and be too large by up to 1 / sqrt(1 - b2).  The hash
+// is the multiply-xorshift finaliser "lowbias32" (C. Wellons, "Prospecting for Hash
+// Functions", 2018).
+//
+// The step count lives on the device, so that a captured step counts on: [0]
+// counts the steps, [1] the launch's blocks that are done; the last one adds to
+// [0] and clears [1].  A grad_scale that is not finite skips the step whole.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstring>
+#include <type_traits>
+
+#include "../../include/pesq_cuda.h"
+#include "train.cuh"
+
+namespace {
+
+using namespace pesq::train;
+using pesq::set_error;
+
+constexpr int kBlock = 256;   // values of a unit, and of a scale
+constexpr int kThreads = 256; // of a CTA
+constexpr float kTop = 448.0f;
+
+struct Entry {
+  float* param;
+  const void* grad;
+  void* copy;
+  int64_t n;      // values
+  int64_t first;  // first unit
+};
+
+// Tensors of a launch.  Kernel parameters hold 32,764 bytes; a launch of few tensors
+// takes the short table.
+template <int N>
+struct Table {
+  Entry e[N];
+};
+constexpr int kShort = 96, kLong = 800;
+
+struct Args {
+  int count;
+  int64_t units, first;  // of this launch, and before it
+  void *moment1, *moment2;
+  float *scale1, *scale2;  // of the units (8 bits)
+  long long* step;
+  const float* grad_scale;
+  double beta1, beta2;
+  float lr, eps, decay;
+  unsigned seed;
+  int last;              // of the call's launches
+};
+
+__device__ __forceinline__ unsigned hash(unsigned h) {
+  h = (h ^ (h >> 16)) * 0x7feb352du;
+  h = (h ^ (h >> 15)) * 0x846ca68bu;
+  return h ^ (h >> 16);
+}
+
+__device__ __forceinline__ void from_e4m3(unsigned w, float* v) {  // four values
+  unsigned lo, hi;
+  asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\ncvt.rn.f16x2.e4m3x2 %0, l;\ncvt.rn.f16x2.e4m3x2 %1, h;\n}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
+  const float2 a = __half22float2(*reinterpret_cast<__half2*>(&lo)), b = __half22float2(*reinterpret_cast<__half2*>(&hi));
+  v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+}
+__device__ __forceinline__ unsigned to_e4m3(const float* v) {  // nearest
+  unsigned w;
+  asm("{\n.reg .b16 l, h;\ncvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\ncvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\nmov.b32 %0, {l, h};\n}"
+      : "=r"(w)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]));
+  return w;
+}
+
+// u >= 0 to one of its two neighbours in e4m3, the upper with the probability of
+// its nearness: 20 random bits are added below the 3 mantissa bits that stay.
+// Below 2^-6, where the steps are 2^-9 throughout, that is done to u + 2^-6.  What is
+// above zero does not become zero.
+__device__ __forceinline__ float dither(float u, unsigned bits) {
+  const float base = u < 0x1p-6f ? 0x1p-6f : 0.0f;
+  const float t = __uint_as_float((__float_as_uint(u + base) + (bits & 0xfffffu)) & ~0xfffffu) - base;
+  return u > 0.0f ? fmaxf(t, 0x1p-9f) : u;
+}
+
+// Eight values of a tensor, as the words they were read as
+template <class T>
+struct Eight {
+  unsigned w[2 * sizeof(T)];
+  // from `at` on of n, as 16-byte accesses where `wide`
+  __device__ __forceinline__ void read(const T* p, int64_t at, int64_t n, bool wide) {
+    if (wide) {
+      const uint4* q = reinterpret_cast<const uint4*>(p + at);
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+        const uint4 v = q[i];
+        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+      }
+    } else {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = at + j < n ? widen(p[at + j]) : 0.0f;
+      set(v);
+    }
+  }
+  __device__ __forceinline__ float at(int j) const {
+    if constexpr (sizeof(T) == 4)
+      return __uint_as_float(w[j]);
+    else if constexpr (std::is_same<T, __half>::value)
+      return __half2float(__ushort_as_half((unsigned short)(j % 2 ? w[j / 2] >> 16 : w[j / 2])));
+    else
+      return __uint_as_float(j % 2 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+  }
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      if constexpr (sizeof(T) == 4)
+        w[j] = __float_as_uint(v[j]), w[j + 1] = __float_as_uint(v[j + 1]);
+      else if constexpr (std::is_same<T, __half>::value)
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[j / 2]) : "f"(v[j + 1]), "f"(v[j]));
+      else
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[j / 2]) : "f"(v[j + 1]), "f"(v[j]));
+    }
+  }
+  __device__ __forceinline__ void write(T* p, int64_t at, int64_t n, bool wide) const {
+    if (wide) {
+      uint4* q = reinterpret_cast<uint4*>(p + at);
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+        q[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (at + j < n) p[at + j] = narrow<T>(this->at(j));
+    }
+  }
+};
+
+__device__ __forceinline__ float root_of(float v) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, off));
+  return v;
+}
+
+// What a lane has read of a unit
+template <class G, bool kEight>
+struct Unit {
+  int tensor;
+  int64_t at;  // in the tensor
+  bool wide, wide_g;
+  Eight<float> p;
+  Eight<G> g;
+  Eight<float> m, v;  // 32 bits
+  uint2 c1, c2;       // 8 bits
+  float s1, s2;
+};
+
+// CTAs an SM holds: the registers of a thread
+template <bool kEight>
+constexpr int kCtas = 3;
+
+// A CTA takes a run of units, its warps one of them each at a time; the next unit's
+// values are on their way while one is worked on.
+template <class G, bool kEight, int N>
+__global__ void __launch_bounds__(kThreads, kCtas<kEight>) adamw_kernel(const __grid_constant__ Args p,
+                                                                        const __grid_constant__ Table<N> t) {
+  __shared__ float s_c[3];  // lr / (1 - b1^t), 1 / sqrt(1 - b2^t), grad scale
+  __shared__ unsigned s_step;
+  const int lane = threadIdx.x & 31;
+  constexpr int kWarps = kThreads / 32;
+  const int64_t run = (p.units + gridDim.x - 1) / gridDim.x, end = min(p.units, (blockIdx.x + 1) * run);
+  int64_t unit = blockIdx.x * run + threadIdx.x / 32;
+
+  int lo = 0, hi = p.count;  // the last tensor that begins at or before the unit
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (t.e[mid].first <= unit) lo = mid;
+    else hi = mid;
+  }
+  const auto read = [&](int64_t unit, Unit<G, kEight>& u) {
+    while (lo + 1 < p.count && t.e[lo + 1].first <= unit) ++lo;
+    const Entry& e = t.e[lo];
+    u.tensor = lo;
+    u.at = (unit - e.first) * kBlock + lane * 8;
+    if (!e.grad) return;
+    const bool whole = u.at + 8 <= e.n;
+    u.wide = whole && reinterpret_cast<uintptr_t>(e.param) % 16 == 0;
+    u.wide_g = whole && reinterpret_cast<uintptr_t>(e.grad) % 16 == 0;
+    u.g.read(static_cast<const G*>(e.grad), u.at, e.n, u.wide_g);
+    u.p.read(e.param, u.at, e.n, u.wide);
+    const int64_t place = (p.first + unit) * kBlock + lane * 8;  // in the moments' buffers
+    if (kEight) {
+      u.c1 = *reinterpret_cast<const uint2*>(static_cast<const unsigned char*>(p.moment1) + place);
+      u.c2 = *reinterpret_cast<const uint2*>(static_cast<const unsigned char*>(p.moment2) + place);
+      u.s1 = p.scale1[p.first + unit], u.s2 = p.scale2[p.first + unit];
+    } else {
+      u.m.read(static_cast<const float*>(p.moment1), place, 0, true);
+      u.v.read(static_cast<const float*>(p.moment2), place, 0, true);
+    }
+  };
+  Unit<G, kEight> now;
+  if (unit < end) read(unit, now);
+
+  if (threadIdx.x < 32) {
+    const long long step = *reinterpret_cast<volatile long long*>(p.step) + 1;
+    if (threadIdx.x == 0) s_c[0] = (float)((double)p.lr / (1.0 - pow(p.beta1, (double)step))), s_step = (unsigned)step;
+    if (threadIdx.x == 1) s_c[1] = (float)(1.0 / sqrt(1.0 - pow(p.beta2, (double)step)));
+    if (threadIdx.x == 2) s_c[2] = p.grad_scale ? *p.grad_scale : 1.0f;
+  }
+  __syncthreads();
+  const float scale = s_c[2];
+  const bool skip = !isfinite(scale);
+  const float rate = s_c[0], root = s_c[1], keep = 1.0f - p.lr * p.decay;
+  const float b1 = (float)p.beta1, b2 = (float)p.beta2, a1 = (float)(1.0 - p.beta1), a2 = (float)(1.0 - p.beta2);
+  const unsigned salt = s_step * 0x9e3779b9u + p.seed * 0x85ebca6bu;
+
+  if (skip) unit = end;
+  for (; unit < end; unit += kWarps) {
+    Unit<G, kEight> next;
+    if (unit + kWarps < end) read(unit + kWarps, next);
+    const Entry& e = t.e[now.tensor];
+    if (e.grad) {
+      const int64_t place = (p.first + unit) * kBlock + lane * 8;
+      float w[8], m[8], v[8];
+      if (kEight) {
+        from_e4m3(now.c1.x, m), from_e4m3(now.c1.y, m + 4), from_e4m3(now.c2.x, v), from_e4m3(now.c2.y, v + 4);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          m[j] *= now.s1;
+          v[j] *= now.s2;
+          v[j] *= v[j];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m[j] = now.m.at(j), v[j] = now.v.at(j);
+      }
+      float r[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float g = now.g.at(j) * scale;
+        m[j] = fmaf(b1, m[j], a1 * g);
+        v[j] = fmaf(b2, v[j], a2 * g * g);
+        r[j] = root_of(v[j]);
+        w[j] = fmaf(now.p.at(j), keep, -rate * __fdividef(m[j], fmaf(r[j], root, p.eps)));
+      }
+      Eight<float> out;
+      out.set(w);
+      out.write(e.param, now.at, e.n, now.wide);
+      if (e.copy) {
+        using C = typename std::conditional<std::is_same<G, __half>::value, __half, __nv_bfloat16>::type;
+        Eight<C> c;
+        c.set(w);
+        c.write(static_cast<C*>(e.copy), now.at, e.n, now.at + 8 <= e.n && reinterpret_cast<uintptr_t>(e.copy) % 16 == 0);
+      }
+      if (kEight) {
+        float top1 = 0.0f, top2 = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top1 = max_nan(top1, fabsf(m[j])), top2 = max_nan(top2, r[j]);
+        const float s1 = warp_max(top1) * (1.0f / kTop), s2 = warp_max(top2) * (1.0f / kTop);
+        const float i1 = s1 > 1e-36f ? rcp_approx(s1) : 0.0f, i2 = s2 > 1e-36f ? rcp_approx(s2) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          m[j] *= i1;
+          r[j] = dither(r[j] * i2, hash((unsigned)(place + j) + salt));
+        }
+        uint2 c1, c2;
+        c1.x = to_e4m3(m), c1.y = to_e4m3(m + 4), c2.x = to_e4m3(r), c2.y = to_e4m3(r + 4);
+        *reinterpret_cast<uint2*>(static_cast<unsigned char*>(p.moment1) + place) = c1;
+        *reinterpret_cast<uint2*>(static_cast<unsigned char*>(p.moment2) + place) = c2;
+        if (lane == 0) p.scale1[p.first + unit] = s1, p.scale2[p.first + unit] = s2;
+      } else {
+        now.m.set(m), now.v.set(v);
+        now.m.write(static_cast<float*>(p.moment1), place, 0, true);
+        now.v.write(static_cast<float*>(p.moment2), place, 0, true);
+      }
+    }
+    now = next;
+  }
+
+  // the call's last block counts the step: every block has read it by then
+  if (p.last) {
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      unsigned long long* done = reinterpret_cast<unsigned long long*>(p.step) + 1;
+      __threadfence();
+      if (atomicAdd(done, 1ull) == gridDim.x - 1) {
+        *done = 0ull;
+        if (!skip) p.step[0] += 1;
+      }
+    }
+  }
+}
+
+int sms() {
+  static int count[64] = {0};  // by device; a property that does not change
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (count[dev] == 0) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    count[dev] = n;
+  }
+  return count[dev];
+}
+
+template <class G, bool kEight, int N>
+cudaError_t start(const Args& a, const Entry* e, cudaStream_t s) {
+  Table<N> t;
+  std::memcpy(t.e, e, sizeof(Entry) * a.count);
+  const int64_t blocks = (a.units + kThreads / 32 - 1) / (kThreads / 32);
+  const unsigned grid = (unsigned)std::min<int64_t>(blocks, (int64_t)sms() * kCtas<kEight>);
+  adamw_kernel<G, kEight, N><<<grid, kThreads, 0, s>>>(a, t);
+  return cudaGetLastError();
+}
+template <class G>
+cudaError_t launch(const Args& a, const Entry* e, bool eight, cudaStream_t s) {
+  if (a.count <= kShort) return eight ? start<G, true, kShort>(a, e, s) : start<G, false, kShort>(a, e, s);
+  return eight ? start<G, true, kLong>(a, e, s) : start<G, false, kLong>(a, e, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+int pesq_adamw_step(const pesq_adamw_desc* d, const pesq_adamw_tensor* tensors, int64_t count, void* stream) {
+  if (!d || (count > 0 && !tensors) || count < 0) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL argument");
+  if (d->grad_dtype < PESQ_F32 || d->grad_dtype > PESQ_F16)
+    return set_error(PESQ_ERR_INVALID_ARGUMENT, "unknown gradient type");
+  if (d->state_bits != 8 && d->state_bits != 32) return set_error(PESQ_ERR_INVALID_ARGUMENT, "states have 8 or 32 bits");
+  if (!d->moment1 || !d->moment2 || !d->step || (d->state_bits == 8 && (!d->scale1 || !d->scale2)))
+    return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL state");
+  if (reinterpret_cast<uintptr_t>(d->moment1) % 16 || reinterpret_cast<uintptr_t>(d->moment2) % 16 ||
+      reinterpret_cast<uintptr_t>(d->step) % 8)
+    return set_error(PESQ_ERR_INVALID_ARGUMENT, "the moments are 16-byte, the step 8-byte aligned");
+  if (!(d->beta1 >= 0.0 && d->beta1 < 1.0 && d->beta2 >= 0.0 && d->beta2 < 1.0))
+    return set_error(PESQ_ERR_INVALID_ARGUMENT, "betas lie in [0, 1)");
+  if (!(d->eps >= 0.0f) || !(d->lr >= 0.0f) || !(d->weight_decay >= 0.0f))
+    return set_error(PESQ_ERR_INVALID_ARGUMENT, "lr, eps and weight decay must not be negative");
+  int64_t units = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    if (tensors[i].n < 0 || (tensors[i].n > 0 && tensors[i].grad && !tensors[i].param))
+      return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL tensor");
+    if (tensors[i].copy && d->grad_dtype == PESQ_F32)
+      return set_error(PESQ_ERR_INVALID_ARGUMENT, "copies are of the gradients' 16-bit type");
+    units += (tensors[i].n + kBlock - 1) / kBlock;
+  }
+  if (units > d->units) return set_error(PESQ_ERR_WORKSPACE, "the moments are shorter than the tensors");
+  Args a{};
+  a.moment1 = d->moment1;
+  a.moment2 = d->moment2;
+  a.scale1 = d->scale1;
+  a.scale2 = d->scale2;
+  a.step = reinterpret_cast<long long*>(d->step);
+  a.grad_scale = d->grad_scale;
+  a.beta1 = d->beta1;
+  a.beta2 = d->beta2;
+  a.lr = d->lr;
+  a.eps = d->eps;
+  a.decay = d->weight_decay;
+  a.seed = d->seed;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  Entry table[kLong];
+  int64_t i = 0, before = 0;
+  do {  // (once at least: a step without values counts)
+    a.count = 0;
+    a.units = 0;
+    a.first = before;
+    for (; i < count && a.count < kLong; ++i) {
+      if (tensors[i].n == 0) continue;
+      table[a.count++] = {tensors[i].param, tensors[i].grad, tensors[i].copy, tensors[i].n, a.units};
+      a.units += (tensors[i].n + kBlock - 1) / kBlock;
+    }
+    before += a.units;
+    a.last = before == units;
+    if (a.units == 0) table[0] = {nullptr, nullptr, nullptr, 0, 0}, a.count = 1;
+    const bool eight = d->state_bits == 8;
+    const cudaError_t e = d->grad_dtype == PESQ_F32    ? launch<float>(a, table, eight, s)
+                          : d->grad_dtype == PESQ_BF16 ? launch<__nv_bfloat16>(a, table, eight, s)
+                                                       : launch<__half>(a, table, eight, s);
+    if (e != cudaSuccess) return set_error(PESQ_ERR_CUDA, cudaGetErrorString(e));
+  } while (!a.last);
+  return PESQ_OK;
+}
+
+}  // extern "C"

@@ -36,11 +36,12 @@ using namespace train;
 
 constexpr int kEach = 8;      // channels of a thread
 constexpr int kThreads = 128; // of a CTA, unless a row takes more
-// threads an SM holds, which the registers of one follow from (72 and 128)
-constexpr int kForwardThreads = 896, kBackwardThreads = 512;
-constexpr int ctas(int threads_of_sm, int team) {
-  const int threads = team > kThreads ? team : kThreads;
-  return threads_of_sm / threads > 0 ? threads_of_sm / threads : 1;
+// CTAs that an SM holds, which the registers of a thread follow from: 72 in the forward (96
+// where every channel is addressed by itself), 168 in the backward, where 16 warps of 128
+// registers spill and take 25 % longer than 12 that do not
+constexpr int ctas(bool backward, bool wide, int team) {
+  const int threads = team > kThreads ? team : kThreads, sm = backward ? 384 : wide ? 896 : 640;
+  return sm / threads > 0 ? sm / threads : 1;
 }
 
 struct Rows {
@@ -138,6 +139,8 @@ struct Eight {
     }
   }
   // channels j and j + 1 (j even)
+  __device__ __forceinline__ Vec<2> two(int j) const { return {{at(j), at(j + 1)}}; }
+  __device__ __forceinline__ void set(int j, Vec<2> v) { set(j, v.v[0], v.v[1]); }
   __device__ __forceinline__ void set(int j, float a, float b) {
     if constexpr (sizeof(T) == 4) {
       w[j] = __float_as_uint(a), w[j + 1] = __float_as_uint(b);
@@ -174,12 +177,33 @@ struct Eight {
   }
 };
 
-struct Act {
-  float value, slope;
-};
-__device__ __forceinline__ Act act_of(float g, int silu) {
-  const float s = rcp_approx(1.0f + exp2_approx(-g * kLog2e));
-  return silu ? Act{g * s, s * fmaf(g, 1.0f - s, 1.0f)} : Act{s, s * (1.0f - s)};
+// The gate's activation of eight channels, and its slope
+template <bool kSlope, class E>
+__device__ __forceinline__ void activate(const E& g, int silu, Vec<2> (&value)[kEach / 2], Vec<2> (&slope)[kEach / 2]) {
+  Vec<2> s[kEach / 2];
+#pragma unroll
+  for (int i = 0; i < kEach / 2; ++i) s[i] = g.two(2 * i) * splat<2>(-kLog2e);
+#pragma unroll
+  for (int i = 0; i < kEach / 2; ++i) s[i] = {{exp2_approx(s[i].v[0]), exp2_approx(s[i].v[1])}};
+#pragma unroll
+  for (int i = 0; i < kEach / 2; ++i) s[i] = s[i] + splat<2>(1.0f);
+#pragma unroll
+  for (int i = 0; i < kEach / 2; ++i) s[i] = {{rcp_approx(s[i].v[0]), rcp_approx(s[i].v[1])}};
+#pragma unroll
+  for (int i = 0; i < kEach / 2; ++i) {
+    value[i] = s[i];
+    if (kSlope) slope[i] = fma(s[i], splat<2>(-1.0f), splat<2>(1.0f));  // 1 - s
+  }
+  if (silu) {  // g s, s (1 + g (1 - s))
+#pragma unroll
+    for (int i = 0; i < kEach / 2; ++i) {
+      value[i] = g.two(2 * i) * s[i];
+      if (kSlope) slope[i] = s[i] * fma(g.two(2 * i), slope[i], splat<2>(1.0f));
+    }
+  } else if (kSlope) {  // s, s (1 - s)
+#pragma unroll
+    for (int i = 0; i < kEach / 2; ++i) slope[i] = s[i] * slope[i];
+  }
 }
 
 // The row that a team works on in its k-th turn, dense and for an operand
@@ -201,7 +225,7 @@ struct Turn {
 // ------------------------------------------------------------------- forward
 
 template <class TS, class TB, int TEAM, bool kWide>
-__global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(kForwardThreads, TEAM)) forward_kernel(const __grid_constant__ Args p) {
+__global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(false, kWide, TEAM)) forward_kernel(const __grid_constant__ Args p) {
   constexpr int THREADS = TEAM > kThreads ? TEAM : kThreads, TEAMS = THREADS / TEAM;
   using S = Eight<TS, TEAM, kWide>;
   using B = Eight<TB, TEAM, kWide>;
@@ -233,35 +257,41 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(kForwa
     z1.load(p.block.p, next.of(p.block), p.width, next.on && p.block.p);
     g1.load(p.gate.p, next.of(p.gate), p.width, next.on && p.gate.p);
 
-    float r[kEach], sum[1] = {0.0f};
+    constexpr int H = kEach / 2;
+    Vec<2> r[H], total = splat<2>(0.0f);
+    float sum[1];
     if (p.block.p) {
 #pragma unroll
-      for (int j = 0; j < kEach; ++j) sum[0] = fmaf(z.at(j), z.at(j), sum[0]);
+      for (int i = 0; i < H; ++i) total = fma(z.two(2 * i), z.two(2 * i), total);
+      sum[0] = total.v[0] + total.v[1];
       team_sum<1, TEAM>(sum, s_sum, turn);
-      const float rz = rsqrt_approx(fmaf(sum[0], inv, p.eps));
+      const Vec<2> rz = splat<2>(rsqrt_approx(fmaf(sum[0], inv, p.eps)));
+      Vec<2> w[H];
 #pragma unroll
-      for (int j = 0; j < kEach; ++j) {
-        float w = z.at(j) * rz * post.at(j);
-        if (p.gate.p) w *= act_of(g.at(j), p.silu).value;
-        r[j] = x.at(j) + w;
+      for (int i = 0; i < H; ++i) w[i] = z.two(2 * i) * (rz * post.two(2 * i));
+      if (p.gate.p) {
+        Vec<2> value[H], slope[H];
+        activate<false>(g, p.silu, value, slope);
+#pragma unroll
+        for (int i = 0; i < H; ++i) w[i] = w[i] * value[i];
       }
+#pragma unroll
+      for (int i = 0; i < H; ++i) r[i] = x.two(2 * i) + w[i];
     } else {
 #pragma unroll
-      for (int j = 0; j < kEach; ++j) r[j] = x.at(j);
+      for (int i = 0; i < H; ++i) r[i] = x.two(2 * i);
     }
-    sum[0] = 0.0f;
+    total = splat<2>(0.0f);
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) sum[0] = fmaf(r[j], r[j], sum[0]);
+    for (int i = 0; i < H; ++i) total = fma(r[i], r[i], total);
+    sum[0] = total.v[0] + total.v[1];
     team_sum<1, TEAM>(sum, s_sum, turn);
-    const float rr = rsqrt_approx(fmaf(sum[0], inv, p.eps));
+    const Vec<2> rr = splat<2>(rsqrt_approx(fmaf(sum[0], inv, p.eps)));
     if (now.on) {
       S out;
       B y;
 #pragma unroll
-      for (int j = 0; j < kEach; j += 2) {
-        out.set(j, r[j], r[j + 1]);
-        y.set(j, r[j] * rr * pre.at(j), r[j + 1] * rr * pre.at(j + 1));
-      }
+      for (int i = 0; i < H; ++i) out.set(2 * i, r[i]), y.set(2 * i, r[i] * (rr * pre.two(2 * i)));
       if (p.out_stream) out.store(p.out_stream, now.dense(p), p.width);
       y.store(p.out_normed, now.dense(p), p.width);
     }
@@ -273,11 +303,11 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(kForwa
 
 // The CTA's sum of what its teams hold, to a row of `part`
 template <int TEAM, int TEAMS, bool kWide>
-__device__ __forceinline__ void store_part(const float (&v)[kEach], float* part, int width, float* s_part) {
+__device__ __forceinline__ void store_part(const Vec<2> (&v)[kEach / 2], float* part, int width, float* s_part) {
   using F = Eight<float, TEAM, kWide>;
   F f;
 #pragma unroll
-  for (int j = 0; j < kEach; j += 2) f.set(j, v[j], v[j + 1]);
+  for (int i = 0; i < kEach / 2; ++i) f.set(2 * i, v[i]);
   if (TEAMS == 1) {
     f.store(part, (int64_t)blockIdx.x * width, width);
     return;
@@ -295,7 +325,7 @@ __device__ __forceinline__ void store_part(const float (&v)[kEach], float* part,
 }
 
 template <class TS, class TB, int TEAM, bool kWide>
-__global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(kBackwardThreads, TEAM)) backward_kernel(const __grid_constant__ Args p) {
+__global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(true, kWide, TEAM)) backward_kernel(const __grid_constant__ Args p) {
   constexpr int THREADS = TEAM > kThreads ? TEAM : kThreads, TEAMS = THREADS / TEAM;
   using S = Eight<TS, TEAM, kWide>;
   using B = Eight<TB, TEAM, kWide>;
@@ -312,9 +342,10 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(kBackw
 #pragma unroll
     for (int j = 0; j < kEach; j += 2) post.set(j, post.at(j) * scale.at(j), post.at(j + 1) * scale.at(j + 1));
   }
-  float acc_u[kEach], acc_pre[kEach], acc_gate[kEach];
+  constexpr int H = kEach / 2;
+  Vec<2> acc_u[H], acc_pre[H], acc_gate[H];
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) acc_u[j] = acc_pre[j] = acc_gate[j] = 0.0f;
+  for (int i = 0; i < H; ++i) acc_u[i] = acc_pre[i] = acc_gate[i] = splat<2>(0.0f);
   const int turns = (p.span + TEAMS - 1) / TEAMS;
   const float inv = 1.0f / (float)p.width;
   S x, ds;
@@ -337,59 +368,69 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(kBackw
 
     float rz = 0.0f;
     if (p.block.p) {
-      float one[1] = {0.0f};
+      Vec<2> total = splat<2>(0.0f);
 #pragma unroll
-      for (int j = 0; j < kEach; ++j) one[0] = fmaf(z.at(j), z.at(j), one[0]);
+      for (int i = 0; i < H; ++i) total = fma(z.two(2 * i), z.two(2 * i), total);
+      float one[1] = {total.v[0] + total.v[1]};
       team_sum<1, TEAM>(one, s_sum, turn);
       rz = now.on ? rsqrt_approx(fmaf(one[0], inv, p.eps)) : 0.0f;
     }
     // sums of r^2, q r, ds w, q w, r w
-    float w[kEach], value[kEach], slope[kEach], sum[5] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    Vec<2> value[H], slope[H], w[H], part[5];
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      Act a{1.0f, 0.0f};
-      if (p.gate.p) a = act_of(g.at(j), p.silu);
-      value[j] = a.value, slope[j] = a.slope;
-      w[j] = z.at(j) * rz * post.at(j) * a.value;
-      const float r = x.at(j) + w[j], q = dy.at(j) * pre.at(j);
-      sum[0] = fmaf(r, r, sum[0]);
-      sum[1] = fmaf(q, r, sum[1]);
-      sum[2] = fmaf(ds.at(j), w[j], sum[2]);
-      sum[3] = fmaf(q, w[j], sum[3]);
-      sum[4] = fmaf(r, w[j], sum[4]);
+    for (int k5 = 0; k5 < 5; ++k5) part[k5] = splat<2>(0.0f);
+    if (p.gate.p) {
+      activate<true>(g, p.silu, value, slope);
+    } else {
+#pragma unroll
+      for (int i = 0; i < H; ++i) value[i] = splat<2>(1.0f), slope[i] = splat<2>(0.0f);
     }
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      w[i] = z.two(2 * i) * (splat<2>(rz) * (post.two(2 * i) * value[i]));
+      const Vec<2> r = x.two(2 * i) + w[i], q = dy.two(2 * i) * pre.two(2 * i);
+      part[0] = fma(r, r, part[0]);
+      part[1] = fma(q, r, part[1]);
+      part[2] = fma(ds.two(2 * i), w[i], part[2]);
+      part[3] = fma(q, w[i], part[3]);
+      part[4] = fma(r, w[i], part[4]);
+    }
+    float sum[5];
+#pragma unroll
+    for (int k5 = 0; k5 < 5; ++k5) sum[k5] = part[k5].v[0] + part[k5].v[1];
     team_sum<5, TEAM>(sum, s_sum, turn);
     // (a row that is off is zeros, and adds zeros for any eps)
     const float rr = now.on ? rsqrt_approx(fmaf(sum[0], inv, p.eps)) : 0.0f;
     const float mq = sum[1] * inv * rr * rr;                        // mean(q h) / rms
     const float mw = (sum[2] + rr * (sum[3] - mq * sum[4])) * inv;  // mean(dr w)
-    float dx[kEach], dz[kEach], dg[kEach];
+    Vec<2> dx[H], dz[H], dg[H];
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      const float r = x.at(j) + w[j], zh = z.at(j) * rz;
-      dx[j] = fmaf(rr, fmaf(dy.at(j), pre.at(j), -r * mq), ds.at(j));
-      const float u = dx[j] * zh;
-      dg[j] = u * post.at(j) * slope[j];
-      dz[j] = rz * fmaf(dx[j] * post.at(j), value[j], -zh * mw);
-      acc_u[j] = fmaf(u, value[j], acc_u[j]);
-      acc_pre[j] = fmaf(dy.at(j), r * rr, acc_pre[j]);
-      acc_gate[j] += dg[j];
+    for (int i = 0; i < H; ++i) {
+      const Vec<2> r = x.two(2 * i) + w[i], zh = z.two(2 * i) * splat<2>(rz), ps = post.two(2 * i);
+      const Vec<2> q = dy.two(2 * i) * pre.two(2 * i);
+      dx[i] = fma(splat<2>(rr), fma(r, splat<2>(-mq), q), ds.two(2 * i));
+      const Vec<2> u = dx[i] * zh;
+      dg[i] = u * (ps * slope[i]);
+      dz[i] = splat<2>(rz) * fma(dx[i], ps * value[i], zh * splat<2>(-mw));
+      acc_u[i] = fma(u, value[i], acc_u[i]);
+      acc_pre[i] = fma(dy.two(2 * i), r * splat<2>(rr), acc_pre[i]);
+      acc_gate[i] = acc_gate[i] + dg[i];
     }
     if (now.on) {
       const int64_t at = now.dense(p);
       S a;
       B b;
 #pragma unroll
-      for (int j = 0; j < kEach; j += 2) a.set(j, dx[j], dx[j + 1]);
+      for (int i = 0; i < H; ++i) a.set(2 * i, dx[i]);
       a.store(p.dx, at, p.width);
       if (p.dblock) {
 #pragma unroll
-        for (int j = 0; j < kEach; j += 2) b.set(j, dz[j], dz[j + 1]);
+        for (int i = 0; i < H; ++i) b.set(2 * i, dz[i]);
         b.store(p.dblock, at, p.width);
       }
       if (p.dgate) {
 #pragma unroll
-        for (int j = 0; j < kEach; j += 2) b.set(j, dg[j], dg[j + 1]);
+        for (int i = 0; i < H; ++i) b.set(2 * i, dg[i]);
         b.store(p.dgate, at, p.width);
       }
     }

@@ -124,7 +124,7 @@ Plan plan(const pesq_norm_join_desc& d, bool backward, const pesq_stream* dstrea
              wide(d.gate, d, d.dtype) && wide(ds, d, d.stream_dtype) && wide(dn, d, d.dtype) && wide(d.post) &&
              wide(d.pre) && wide(d.scale);
   const int threads = std::max(q.g.team, kThreads), teams = threads / q.g.team;
-  const int64_t most = std::max<int64_t>(1, 148 * ctas(backward ? kBackwardThreads : kForwardThreads, q.g.team) / q.batch);
+  const int64_t most = std::max<int64_t>(1, 148 * ctas(backward, q.g.wide, q.g.team) / q.batch);
   const int64_t units = std::min<int64_t>(most, (q.steps + teams - 1) / teams);
   q.span = (int)std::min<int64_t>(INT32_MAX - 1024, (q.steps + units - 1) / units);
   q.units = (int)((q.steps + q.span - 1) / q.span);
@@ -135,7 +135,7 @@ Plan plan(const pesq_norm_join_desc& d, bool backward, const pesq_stream* dstrea
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 size_t part_bytes(const pesq_norm_join_desc& d) {
   // (whatever the gradients' strides, no more CTAs than this)
-  const int64_t rows = std::max<int64_t>(d.batch, 148 * ctas(kBackwardThreads, 1)) + d.batch;
+  const int64_t rows = std::max<int64_t>(d.batch, 148 * ctas(true, true, 1)) + d.batch;
   return round16((size_t)rows * d.width * 4);
 }
 

@@ -473,6 +473,107 @@ std::tuple<at::Tensor, at::Tensor> norm_join(const at::Tensor& x, const OptTenso
   return join_forward_op().call(x, z, g, post, pre, scale, eps, silu, shared, dtype);
 }
 
+// ---------------------------------------------------------------------- AdamW
+
+constexpr const char* kAdam = "AdamW step";
+
+void check_dense(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_contiguous(), "The CUDA AdamW step needs dense `", name, "`.");
+}
+
+void adamw_step(at::TensorList params, at::TensorList grads, const at::Tensor& moment1, const at::Tensor& moment2,
+                const at::Tensor& step, const OptTensor& scales, at::TensorList copies, double lr, double beta1,
+                double beta2, double eps, double decay, const OptTensor& grad_scale, int64_t seed) {
+  TORCH_CHECK_VALUE(params.size() == grads.size(), "The CUDA AdamW step needs a gradient for every parameter, got ",
+                    params.size(), " and ", grads.size(), ".");
+  TORCH_CHECK_VALUE(copies.empty() || copies.size() == params.size(),
+                    "The CUDA AdamW step needs a copy for every parameter or none, got ", copies.size(), ".");
+  check_cuda(moment1, moment1, kAdam, "moment1");
+  check_cuda(moment2, moment1, kAdam, "moment2");
+  check_cuda(step, moment1, kAdam, "step");
+  check_dense(moment1, "moment1");
+  check_dense(moment2, "moment2");
+  check_dense(step, "step");
+  TORCH_CHECK(step.scalar_type() == at::kLong && step.numel() == 2,
+              "The CUDA AdamW step needs `step` as two int64 values.");
+  TORCH_CHECK_VALUE(moment1.numel() == moment2.numel() && moment1.numel() % 256 == 0,
+                    "The CUDA AdamW step needs moments of one size, a multiple of 256, got ", moment1.numel(), " and ",
+                    moment2.numel(), ".");
+  pesq_adamw_desc d{};
+  d.units = moment1.numel() / 256;
+  const bool eight = moment1.scalar_type() == at::kFloat8_e4m3fn;
+  TORCH_CHECK(moment1.scalar_type() == moment2.scalar_type() && (eight || moment1.scalar_type() == at::kFloat),
+              "The CUDA AdamW step needs both moments in float32 or float8_e4m3fn, they are ", moment1.scalar_type(),
+              " and ", moment2.scalar_type(), ".");
+  d.state_bits = eight ? 8 : 32;
+  if (eight) {
+    TORCH_CHECK_VALUE(given(scales), "The CUDA AdamW step needs `scales` for 8-bit moments.");
+    check_cuda(*scales, moment1, kAdam, "scales");
+    check_float(*scales, kAdam, "scales");
+    const int64_t want[2] = {2, d.units};
+    check_shape(*scales, want, kAdam, "scales");
+    check_dense(*scales, "scales");
+    d.scale1 = scales->data_ptr<float>();
+    d.scale2 = d.scale1 + d.units;
+  }
+  if (given(grad_scale)) {
+    check_cuda(*grad_scale, moment1, kAdam, "grad_scale");
+    check_float(*grad_scale, kAdam, "grad_scale");
+    TORCH_CHECK_VALUE(grad_scale->numel() == 1, "The CUDA AdamW step needs one `grad_scale`.");
+    d.grad_scale = grad_scale->data_ptr<float>();
+  }
+  std::vector<pesq_adamw_tensor> table;
+  std::vector<at::Tensor> dense;  // gradients that had to be copied
+  table.reserve(params.size());
+  bool typed = false;
+  at::ScalarType type = at::kFloat;
+  for (size_t i = 0; i < params.size(); ++i) {
+    const at::Tensor& p = params[i];
+    const at::Tensor* g = &grads[i];
+    check_cuda(p, moment1, kAdam, "params");
+    check_float(p, kAdam, "params");
+    check_dense(p, "params");
+    pesq_adamw_tensor e{p.data_ptr<float>(), nullptr, nullptr, p.numel()};
+    if (g->defined() && g->numel() > 0) {
+      check_cuda(*g, moment1, kAdam, "grads");
+      check_shape(*g, p.sizes(), kAdam, "grads");
+      if (!typed) type = g->scalar_type(), d.grad_dtype = dtype_code(*g, kAdam, "grads"), typed = true;
+      TORCH_CHECK(g->scalar_type() == type, "The CUDA AdamW step needs gradients of one type, got ", type, " and ",
+                  g->scalar_type(), ".");
+      if (!g->is_contiguous()) {
+        c10::cuda::CUDAGuard guard(moment1.device());
+        dense.push_back(g->contiguous());
+        g = &dense.back();
+      }
+      e.grad = g->data_ptr();
+      if (!copies.empty()) {
+        const at::Tensor& c = copies[i];
+        check_cuda(c, moment1, kAdam, "copies");
+        check_shape(c, p.sizes(), kAdam, "copies");
+        check_dense(c, "copies");
+        TORCH_CHECK(c.scalar_type() == type && type != at::kFloat,
+                    "The CUDA AdamW step needs copies in the gradients' 16-bit type, they are ", c.scalar_type(), ".");
+        e.copy = c.data_ptr();
+        c.unsafeGetTensorImpl()->bump_version();
+      }
+      p.unsafeGetTensorImpl()->bump_version();
+    }
+    table.push_back(e);
+  }
+  d.moment1 = moment1.data_ptr();
+  d.moment2 = moment2.data_ptr();
+  d.step = step.data_ptr<int64_t>();
+  d.beta1 = beta1;
+  d.beta2 = beta2;
+  d.lr = static_cast<float>(lr);
+  d.eps = static_cast<float>(eps);
+  d.weight_decay = static_cast<float>(decay);
+  d.seed = static_cast<uint32_t>(seed);
+  c10::cuda::CUDAGuard guard(moment1.device());
+  check_status(pesq_adamw_step(&d, table.data(), static_cast<int64_t>(table.size()), at::cuda::getCurrentCUDAStream()),
+               "pesq_adamw_step");
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(pesq_cuda, m) {
@@ -492,6 +593,13 @@ TORCH_LIBRARY_FRAGMENT(pesq_cuda, m) {
             .c_str());
 }
 
+TORCH_LIBRARY_FRAGMENT(pesq_cuda, m) {
+  m.def(
+      "adamw_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!) moment1, Tensor(c!) moment2, Tensor(d!) step, "
+      "Tensor(e!)? scales, Tensor(f!)[] copies, float lr, float beta1, float beta2, float eps, float weight_decay, "
+      "Tensor? grad_scale, int seed) -> ()");
+}
+
 TORCH_LIBRARY_IMPL(pesq_cuda, CompositeImplicitAutograd, m) {
   m.impl("gated_scan", &gated_scan);
   m.impl("norm_join", &norm_join);
@@ -502,4 +610,5 @@ TORCH_LIBRARY_IMPL(pesq_cuda, CUDA, m) {
   m.impl("gated_scan_backward", &gated_scan_backward);
   m.impl("norm_join_forward", &norm_join_forward);
   m.impl("norm_join_backward", &norm_join_backward);
+  m.impl("adamw_step", &adamw_step);
 }
