@@ -31,6 +31,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <type_traits>
 
@@ -69,7 +70,8 @@ struct Args {
   float *scale1, *scale2;  // of the units (8 bits)
   long long* step;
   const float* grad_scale;
-  double beta1, beta2;
+  double log_beta1, log_beta2;
+  float beta1, beta2, rest1, rest2;  // betas, and 1 less them
   float lr, eps, decay;
   unsigned seed;
   int last;              // of the call's launches
@@ -166,10 +168,9 @@ __device__ __forceinline__ float root_of(float v) {
   return r;
 }
 
+// The warp's largest of values >= 0, whose bits order as they do; a NaN is the largest
 __device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, off));
-  return v;
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu));
 }
 
 // What a lane has read of a unit
@@ -185,11 +186,11 @@ struct Unit {
   float s1, s2;
 };
 
-// CTAs an SM holds: the registers of a thread
+// CTAs an SM holds, all of a launch: the registers of a thread, and how many rows of DRAM are open
 template <bool kEight>
-constexpr int kCtas = 3;
+constexpr int kCtas = kEight ? 3 : 2;  // (32 bits, 83M values: 1 takes 190 us, 2 162, 3 178, 4 193)
 
-// A CTA takes a run of units, its warps one of them each at a time; the next unit's
+// The CTAs take eight units at a time in turn, a warp one of them; the next unit's
 // values are on their way while one is worked on.
 template <class G, bool kEight, int N>
 __global__ void __launch_bounds__(kThreads, kCtas<kEight>) adamw_kernel(const __grid_constant__ Args p,
@@ -198,8 +199,8 @@ __global__ void __launch_bounds__(kThreads, kCtas<kEight>) adamw_kernel(const __
   __shared__ unsigned s_step;
   const int lane = threadIdx.x & 31;
   constexpr int kWarps = kThreads / 32;
-  const int64_t run = (p.units + gridDim.x - 1) / gridDim.x, end = min(p.units, (blockIdx.x + 1) * run);
-  int64_t unit = blockIdx.x * run + threadIdx.x / 32;
+  const int64_t end = p.units, turn = (int64_t)gridDim.x * kWarps;
+  int64_t unit = (int64_t)blockIdx.x * kWarps + threadIdx.x / 32;
 
   int lo = 0, hi = p.count;  // the last tensor that begins at or before the unit
   while (hi - lo > 1) {
@@ -233,45 +234,49 @@ __global__ void __launch_bounds__(kThreads, kCtas<kEight>) adamw_kernel(const __
 
   if (threadIdx.x < 32) {
     const long long step = *reinterpret_cast<volatile long long*>(p.step) + 1;
-    if (threadIdx.x == 0) s_c[0] = (float)((double)p.lr / (1.0 - pow(p.beta1, (double)step))), s_step = (unsigned)step;
-    if (threadIdx.x == 1) s_c[1] = (float)(1.0 / sqrt(1.0 - pow(p.beta2, (double)step)));
+    // 1 - b^t = -expm1(t log b): the product in 64 bits, the rest is accurate in 32
+    if (threadIdx.x == 0) s_c[0] = -p.lr / expm1f((float)((double)step * p.log_beta1)), s_step = (unsigned)step;
+    if (threadIdx.x == 1) s_c[1] = 1.0f / sqrtf(-expm1f((float)((double)step * p.log_beta2)));
     if (threadIdx.x == 2) s_c[2] = p.grad_scale ? *p.grad_scale : 1.0f;
   }
   __syncthreads();
   const float scale = s_c[2];
   const bool skip = !isfinite(scale);
   const float rate = s_c[0], root = s_c[1], keep = 1.0f - p.lr * p.decay;
-  const float b1 = (float)p.beta1, b2 = (float)p.beta2, a1 = (float)(1.0 - p.beta1), a2 = (float)(1.0 - p.beta2);
+  const Vec<2> b1 = splat<2>(p.beta1), b2 = splat<2>(p.beta2), a1 = splat<2>(p.rest1 * scale);
+  const Vec<2> a2 = splat<2>(p.rest2), sc = splat<2>(scale);
   const unsigned salt = s_step * 0x9e3779b9u + p.seed * 0x85ebca6bu;
 
   if (skip) unit = end;
-  for (; unit < end; unit += kWarps) {
+  for (; unit < end; unit += turn) {
     Unit<G, kEight> next;
-    if (unit + kWarps < end) read(unit + kWarps, next);
+    if (unit + turn < end) read(unit + turn, next);
     const Entry& e = t.e[now.tensor];
     if (e.grad) {
       const int64_t place = (p.first + unit) * kBlock + lane * 8;
-      float w[8], m[8], v[8];
+      float w[8], m[8], v[8], r[8];
       if (kEight) {
         from_e4m3(now.c1.x, m), from_e4m3(now.c1.y, m + 4), from_e4m3(now.c2.x, v), from_e4m3(now.c2.y, v + 4);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          m[j] *= now.s1;
-          v[j] *= now.s2;
-          v[j] *= v[j];
-        }
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) m[j] = now.m.at(j), v[j] = now.v.at(j);
       }
-      float r[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float g = now.g.at(j) * scale;
-        m[j] = fmaf(b1, m[j], a1 * g);
-        v[j] = fmaf(b2, v[j], a2 * g * g);
-        r[j] = root_of(v[j]);
-        w[j] = fmaf(now.p.at(j), keep, -rate * __fdividef(m[j], fmaf(r[j], root, p.eps)));
+      for (int j = 0; j < 8; j += 2) {
+        const Vec<2> g{{now.g.at(j), now.g.at(j + 1)}}, gs = g * sc;
+        Vec<2> m2{{m[j], m[j + 1]}}, v2{{v[j], v[j + 1]}}, p2{{now.p.at(j), now.p.at(j + 1)}};
+        if (kEight) {
+          m2 = m2 * splat<2>(now.s1);
+          v2 = v2 * splat<2>(now.s2);
+          v2 = v2 * v2;
+        }
+        m2 = fma(b1, m2, a1 * g);
+        v2 = fma(b2, v2, a2 * (gs * gs));
+        const Vec<2> r2{{root_of(v2.v[0]), root_of(v2.v[1])}}, below = fma(r2, splat<2>(root), splat<2>(p.eps));
+        const Vec<2> update = m2 * Vec<2>{{rcp_approx(below.v[0]), rcp_approx(below.v[1])}};
+        p2 = fma(p2, splat<2>(keep), update * splat<2>(-rate));
+        m[j] = m2.v[0], m[j + 1] = m2.v[1], v[j] = v2.v[0], v[j + 1] = v2.v[1];
+        r[j] = r2.v[0], r[j + 1] = r2.v[1], w[j] = p2.v[0], w[j + 1] = p2.v[1];
       }
       Eight<float> out;
       out.set(w);
@@ -382,8 +387,12 @@ int pesq_adamw_step(const pesq_adamw_desc* d, const pesq_adamw_tensor* tensors, 
   a.scale2 = d->scale2;
   a.step = reinterpret_cast<long long*>(d->step);
   a.grad_scale = d->grad_scale;
-  a.beta1 = d->beta1;
-  a.beta2 = d->beta2;
+  a.log_beta1 = std::log(d->beta1);  // (of 0: minus infinity, and 1 - 0^t = 1)
+  a.log_beta2 = std::log(d->beta2);
+  a.beta1 = (float)d->beta1;
+  a.beta2 = (float)d->beta2;
+  a.rest1 = (float)(1.0 - d->beta1);
+  a.rest2 = (float)(1.0 - d->beta2);
   a.lr = d->lr;
   a.eps = d->eps;
   a.decay = d->weight_decay;
