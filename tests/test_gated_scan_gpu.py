@@ -311,6 +311,21 @@ def test_other_streams_and_graphs(cuda_device):
         assert torch.equal(a, b)
 
 
+def test_threads_that_have_not_used_the_device(cuda_device):
+    """The backward of a first pass runs on such a thread of autograd's."""
+
+    import threading
+
+    tensors, _, _ = inputs(2, 100, 64, torch.bfloat16, seed=16)
+    dev = [t.to(cuda_device) for t in tensors]
+    want, got = gated_scan(*dev)[0], []
+    thread = threading.Thread(target=lambda: got.append(gated_scan(*dev)[0]))
+    thread.start()
+    thread.join()
+    torch.cuda.synchronize()
+    assert len(got) == 1 and torch.equal(got[0], want)
+
+
 def test_refusals(cuda_device):
     tensors, _, _ = inputs(2, 4, 6, torch.float32)
     x, ig, rg, decay, state = (t.to(cuda_device) for t in tensors)

@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<kEight>) adamw_kernel(const __
   const float scale = s_c[2];
   const bool skip = !isfinite(scale);
   const float rate = s_c[0], root = s_c[1], keep = 1.0f - p.lr * p.decay;
-  const Vec<2> b1 = splat<2>(p.beta1), b2 = splat<2>(p.beta2), a1 = splat<2>(p.rest1 * scale);
+  const Vec<2> b1 = splat<2>(p.beta1), b2 = splat<2>(p.beta2), a1 = splat<2>(p.rest1);
   const Vec<2> a2 = splat<2>(p.rest2), sc = splat<2>(scale);
   const unsigned salt = s_step * 0x9e3779b9u + p.seed * 0x85ebca6bu;
 
@@ -270,9 +270,22 @@ __global__ void __launch_bounds__(kThreads, kCtas<kEight>) adamw_kernel(const __
           v2 = v2 * splat<2>(now.s2);
           v2 = v2 * v2;
         }
-        m2 = fma(b1, m2, a1 * g);
-        v2 = fma(b2, v2, a2 * (gs * gs));
-        const Vec<2> r2{{root_of(v2.v[0]), root_of(v2.v[1])}}, below = fma(r2, splat<2>(root), splat<2>(p.eps));
+        Vec<2> r2;
+        if (kEight) {
+          // operation by operation: what is rounded to 8 bits has the bits of the definition in 32,
+          // because a value that falls on the other side of a rounding is off by 1/8
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            m2.v[i] = __fadd_rn(__fmul_rn(p.beta1, m2.v[i]), __fmul_rn(p.rest1, gs.v[i]));
+            v2.v[i] = __fadd_rn(__fmul_rn(p.beta2, v2.v[i]), __fmul_rn(__fmul_rn(p.rest2, gs.v[i]), gs.v[i]));
+            r2.v[i] = __fsqrt_rn(v2.v[i]);
+          }
+        } else {
+          m2 = fma(b1, m2, a1 * gs);
+          v2 = fma(b2, v2, a2 * (gs * gs));
+          r2 = {{root_of(v2.v[0]), root_of(v2.v[1])}};
+        }
+        const Vec<2> below = fma(r2, splat<2>(root), splat<2>(p.eps));
         const Vec<2> update = m2 * Vec<2>{{rcp_approx(below.v[0]), rcp_approx(below.v[1])}};
         p2 = fma(p2, splat<2>(keep), update * splat<2>(-rate));
         m[j] = m2.v[0], m[j + 1] = m2.v[1], v[j] = v2.v[0], v[j + 1] = v2.v[1];
@@ -292,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<kEight>) adamw_kernel(const __
 #pragma unroll
         for (int j = 0; j < 8; ++j) top1 = max_nan(top1, fabsf(m[j])), top2 = max_nan(top2, r[j]);
         const float s1 = warp_max(top1) * (1.0f / kTop), s2 = warp_max(top2) * (1.0f / kTop);
-        const float i1 = s1 > 1e-36f ? rcp_approx(s1) : 0.0f, i2 = s2 > 1e-36f ? rcp_approx(s2) : 0.0f;
+        const float i1 = s1 > 1e-36f ? __frcp_rn(s1) : 0.0f, i2 = s2 > 1e-36f ? __frcp_rn(s2) : 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           m[j] *= i1;

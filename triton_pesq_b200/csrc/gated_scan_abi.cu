@@ -213,6 +213,10 @@ int run(const pesq_gated_scan_desc& d, Args& a, const Geometry& g, const pesq_st
   Maps m;
   if (g.bulk) {
     if (!encoder()) return set_error(PESQ_ERR_CUDA, "no cuTensorMapEncodeTiled");
+    // the encoder is the driver's: it wants a context, which a thread that has not called the runtime yet lacks
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess)
+      return set_error(PESQ_ERR_CUDA, cudaGetErrorString(cudaGetLastError()));
     a.error = error_word();
     if (!a.error) return set_error(PESQ_ERR_CUDA, "no error word");
     if (!encode(m.x, d.x, d, g) || !encode(m.ig, d.input_gate, d, g) || !encode(m.rg, d.decay_gate, d, g) ||
