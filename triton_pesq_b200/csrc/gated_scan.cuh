@@ -39,6 +39,8 @@
 
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "../../include/pesq_cuda.h"
 #include "common.cuh"
 #include "train.cuh"
@@ -51,7 +53,7 @@ using namespace train;
 // steps of a chunk, by the channels of a lane: in shared memory sixteen elements of each
 // stream either way, in registers no more than 8 steps
 constexpr int chunk_steps(int vec, bool bulk) { return bulk ? 16 / vec : 8; }
-constexpr int kStrips = 8;  // strips (warps) of a CTA, where rows are cut
+constexpr int kStrips = 8;  // strips (warps) of a CTA at most, where rows are cut
 // chunks of a warp in shared memory: what 8 warps' chunks of four 32-bit streams leave room for
 template <class T>
 constexpr int kRing = sizeof(T) == 2 ? 3 : 2;
@@ -252,14 +254,16 @@ __device__ __forceinline__ void hold(Pack<__half, V>& p) {
   for (int v = 0; v < V / 2; ++v) q[v] = __hmax2_nan(q[v], __float2half2_rn(kShut));
 }
 
-// What a lane works on, and where its strip lies
+// What a lane works on, and where its strip lies.  Chunks are counted in the order of
+// the steps' scan.
 struct Lane {
   int64_t b, c;      // row, first channel
   int rank;          // of the strip, in the order of this scan
-  int first, count;  // chunks of the strip, in the order of the steps' scan
+  int all_first, all_count;  // the strip's chunks
+  int first, count;  // those with a step before the row's length
   int whole;         // those of them that have all their steps
   int dir;           // memory direction of the steps' scan
-  int64_t len;       // the row's length
+  int len;           // the row's length
   bool on;           // channels in range
   int64_t from;      // first channel to read
 };
@@ -273,41 +277,67 @@ __device__ __forceinline__ Lane lane_of(const Args& p) {
   o.on = o.c < p.width;
   o.from = o.on ? o.c : 0;
   o.rank = block * blockDim.y + threadIdx.y;
-  const int strip = kBack ? p.strips - 1 - o.rank : o.rank;
-  const int all = (int)((p.steps + L - 1) / L), per = p.strip / L;
-  o.first = strip * per;
-  o.count = strip < 0 || strip >= p.strips ? 0 : min(per, all - o.first);
-  o.whole = min(o.count, max(0, (int)(p.steps / L) - o.first));
+  const int strip = kBack ? p.strips - 1 - o.rank : o.rank, steps = (int)p.steps;
+  const int all = (steps + L - 1) / L, per = p.strip / L;
+  o.all_first = strip * per;
+  o.all_count = strip < 0 || strip >= p.strips ? 0 : min(per, all - o.all_first);
+  o.first = o.all_first, o.count = o.all_count;
+  o.len = steps;
   o.dir = p.reverse ? -1 : 1;
-  o.len = kMask && p.lengths ? p.lengths[o.b] : p.steps;
+  if (kMask && p.lengths) {
+    o.len = (int)max(INT64_C(0), min(p.lengths[o.b], p.steps));
+    const int lo = p.reverse ? (steps - o.len) / L : 0, hi = o.len == 0 ? lo : p.reverse ? all : (o.len + L - 1) / L;
+    o.first = max(o.all_first, lo);
+    o.count = max(0, min(o.all_first + o.all_count, hi) - o.first);
+  }
+  o.whole = min(o.count, max(0, steps / L - o.first));
   return o;
 }
 
-// Steps of one chunk
+// Steps of one chunk, a bit each
 struct Chunk {
-  int64_t t0;        // first step, in memory
-  unsigned inside;   // steps of the row (a bit each)
-  unsigned live;     // before the row's length
-  unsigned cut;      // reset
+  int64_t t0;       // first step, in memory
+  unsigned inside;  // steps of the row
+  unsigned live;    // before the row's length
+  unsigned flag;    // reset, of the step with the lane's number
 };
 template <int L, bool kMask>
 __device__ __forceinline__ Chunk chunk_of(const Args& p, const Lane& o, int k) {
+  constexpr unsigned kAll = (1u << L) - 1;
   Chunk q;
-  const int64_t s0 = (int64_t)k * L, left = p.steps - s0;
-  q.t0 = p.reverse ? p.steps - 1 - s0 : s0;
-  q.inside = left >= L ? (1u << L) - 1 : (1u << left) - 1;
+  const int s0 = k * L, left = (int)p.steps - s0, t0 = p.reverse ? left - 1 : s0;
+  q.t0 = t0;
+  q.inside = left >= L ? kAll : (1u << left) - 1;
   q.live = q.inside;
-  q.cut = 0u;
   if (kMask) {
-#pragma unroll
-    for (int l = 0; l < L; ++l) {
-      const int64_t t = q.t0 + l * o.dir;
-      if (t >= o.len) q.live &= ~(1u << l);
-      if (p.reset && ((q.live >> l) & 1u) && p.reset[o.b * p.reset_b + t * p.reset_t]) q.cut |= 1u << l;
+    if (p.reverse) {
+      const int dead = t0 - o.len + 1;  // steps at the chunk's start
+      if (dead > 0) q.live &= dead >= L ? 0u : ~0u << dead;
+    } else if (o.len - t0 < L) {
+      q.live &= o.len <= t0 ? 0u : (1u << (o.len - t0)) - 1;
     }
   }
+  q.flag = 0u;
   return q;
 }
+// Starts the load of the chunk's resets, one lane a step; cuts() gathers them
+template <int L, bool kMask>
+__device__ __forceinline__ void flag_chunk(const Args& p, const Lane& o, Chunk& q) {
+  if (!kMask || !p.reset) return;
+  const unsigned mine = threadIdx.x < L ? (q.live >> threadIdx.x) & 1u : 0u;
+  const uint8_t* at = p.reset + o.b * p.reset_b + (q.t0 + (int)threadIdx.x * o.dir) * p.reset_t;
+  asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %2, 0;\n@q ld.global.u8 %0, [%1];\n}" : "+r"(q.flag) : "l"(at), "r"(mine));
+}
+template <bool kMask>
+__device__ __forceinline__ unsigned cuts(const Args& p, const Chunk& q) {
+  return kMask && p.reset ? __ballot_sync(0xffffffffu, q.flag != 0u) : 0u;
+}
+
+// Launches of one call follow one another closely: the next one may start once
+// all blocks of this one have
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// and waits here until this one is done
+__device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Loads one pack where `take` is nonzero and leaves it as it is otherwise: a
 // predicated load, with no branch whose join would wait for it
@@ -368,7 +398,7 @@ struct Pairing {
 
 // Calls emit(l, j, gates, beta) for every step and Vec of a chunk, steps in order
 template <class T, int V, int L, bool kMask, bool kFar, class F>
-__device__ __forceinline__ void each_gate(const Chunk& q, const Pack<T, V> (&ig)[L], const Pack<T, V> (&rg)[L],
+__device__ __forceinline__ void each_gate(unsigned cut, const Pack<T, V> (&ig)[L], const Pack<T, V> (&rg)[L],
                                           const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P], F emit) {
   using Q = Pairing<V, L>;
   constexpr int N = Q::N;
@@ -387,7 +417,7 @@ __device__ __forceinline__ void each_gate(const Chunk& q, const Pack<T, V> (&ig)
     for (int l = 0; l < L; ++l) {
       Gates<1> one{{{out[l / 2].i.v[l % 2]}}, {{out[l / 2].r.v[l % 2]}}, {{out[l / 2].a.v[l % 2]}}};
       Vec<1> b1{{beta[l / 2].v[l % 2]}};
-      if (kMask && ((q.cut >> l) & 1u)) one.a = splat<1>(0.0f), b1 = splat<1>(1.0f);
+      if (kMask && ((cut >> l) & 1u)) one.a = splat<1>(0.0f), b1 = splat<1>(1.0f);
       emit(l, 0, one, b1);
     }
   } else {
@@ -408,7 +438,7 @@ __device__ __forceinline__ void each_gate(const Chunk& q, const Pack<T, V> (&ig)
 #pragma unroll
       for (int j = 0; j < Q::P; ++j) {
         Gates<N>& one = out[l * Q::P + j];
-        if (kMask && ((q.cut >> l) & 1u)) one.a = splat<N>(0.0f), beta[l * Q::P + j] = splat<N>(1.0f);
+        if (kMask && ((cut >> l) & 1u)) one.a = splat<N>(0.0f), beta[l * Q::P + j] = splat<N>(1.0f);
         emit(l, j, one, beta[l * Q::P + j]);
       }
   }
@@ -438,7 +468,7 @@ __device__ __forceinline__ void read_row(const float* p, Vec<N> (&out)[V / N]) {
 template <int V, int N, bool kMask>
 __device__ __forceinline__ void start_of(const Args& p, const Lane& o, Vec<N> (&h)[V / N]) {
   if (p.strips == 1 || !o.on || o.rank >= p.strips) return;
-  const int ctas = (p.strips + kStrips - 1) / kStrips, cta = o.rank / kStrips;
+  const int w = blockDim.y, ctas = (p.strips + w - 1) / w, cta = o.rank / w;
   const float2* t = p.total + o.b * ctas * p.width + o.c;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -463,7 +493,8 @@ __device__ __forceinline__ void join_maps(const Args& p, const Lane& o, const Ve
     s_map[threadIdx.y][threadIdx.x * V + v] = make_float2(A[v / N].v[v % N], H[v / N].v[v % N]);
   __syncthreads();
   if (!o.on || o.rank >= p.strips) return;
-  const bool end = threadIdx.y == kStrips - 1 || o.rank == p.strips - 1;
+  const int strips = blockDim.y;
+  const bool end = threadIdx.y == strips - 1 || o.rank == p.strips - 1;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     Vec<1> a{{1.0f}}, h{{0.0f}};
@@ -476,9 +507,35 @@ __device__ __forceinline__ void join_maps(const Args& p, const Lane& o, const Ve
     if (end) {
       const float2 m = s_map[threadIdx.y][threadIdx.x * V + v];
       h = apply<kMask>(Vec<1>{{m.x}}, h, Vec<1>{{m.y}});
-      const int ctas = (p.strips + kStrips - 1) / kStrips;
-      p.total[(o.b * ctas + o.rank / kStrips) * p.width + o.c + v] = make_float2(a.v[0] * m.x, h.v[0]);
+      const int ctas = (p.strips + strips - 1) / strips;
+      p.total[(o.b * ctas + o.rank / strips) * p.width + o.c + v] = make_float2(a.v[0] * m.x, h.v[0]);
     }
+  }
+}
+
+// What a chunk holds of the steps that are not live: the identity to the last bit
+template <class T, int V, int L>
+__device__ __forceinline__ void blank(Pack<T, V> (&out)[L], const Chunk& q, float other = 0.0f) {
+#pragma unroll
+  for (int l = 0; l < L; ++l)
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (!((q.live >> l) & 1u)) out[l].v[v] = narrow<T>(other);
+}
+
+// Zeros for a strip's chunks that the row's length leaves out
+template <class T, int V, int L>
+__device__ __forceinline__ void zero_rest(const Args& p, const Lane& o, void* out) {
+  if (o.count == o.all_count || !o.on) return;
+  Pack<T, V> z;
+#pragma unroll
+  for (int v = 0; v < V; ++v) z.v[v] = narrow<T>(0.0f);
+  const int end = min((o.all_first + o.all_count) * L, (int)p.steps);
+  for (int s = o.all_first * L; s < end; ++s) {
+    if (o.count && s == o.first * L) s += o.count * L;
+    if (s >= end) break;
+    const int64_t t = p.reverse ? p.steps - 1 - s : s;
+    *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(out) + (o.b * p.steps + t) * p.width + o.c) = z;
   }
 }
 
@@ -546,15 +603,21 @@ struct Ring {
   __device__ __forceinline__ Pack<float, V> state(int stage) const {
     return reinterpret_cast<const Pack<float, V>*>(base + stage * kStage + S * kBox)[threadIdx.x];
   }
-  // Chunks first, first + way, ...: read(stage, k, in) takes a chunk out of its stage, work(k, in)
-  // works on it while the stage fills again.  Returns false where a copy does not come.
-  template <class In, class R, class W>
-  __device__ __forceinline__ bool walk(const Args& p, const Lane& o, int first, int n, int way, R read, W work) {
+  // The first copies of a walk
+  __device__ __forceinline__ void start(const Args& p, const Lane& o, int first, int n, int way) {
     if (threadIdx.x == 0) {
       for (int i = 0; i < kRing<T> && i < n; ++i) send(p, o, first + way * i, i);
     }
+  }
+  // Chunks first, first + way, ..., after start(): read(stage, q, in) takes a chunk out of its
+  // stage, work(k, in) works on it while the stage fills again.  Returns false where a copy
+  // does not come.
+  template <bool kMask, class In, class R, class W>
+  __device__ __forceinline__ bool walk(const Args& p, const Lane& o, int first, int n, int way, R read, W work) {
     int stage = 0, parity = 0;
     bool ok = true;
+    Chunk q = chunk_of<L, kMask>(p, o, first);
+    if (n > 0) flag_chunk<L, kMask>(p, o, q);
 #pragma unroll 1
     for (int k = 0; k < n; ++k) {
       if (!__all_sync(0xffffffffu, mbar_wait(bar + stage, parity))) {
@@ -562,9 +625,12 @@ struct Ring {
         break;
       }
       In in;
-      read(stage, first + way * k, in);
+      in.q = q;
+      read(stage, in);
       __syncwarp();
       if (threadIdx.x == 0 && k + kRing<T> < n) send(p, o, first + way * (k + kRing<T>), stage);
+      q = chunk_of<L, kMask>(p, o, first + way * min(k + 1, n - 1));
+      flag_chunk<L, kMask>(p, o, q);
       work(first + way * k, in);
       if (++stage == kRing<T>) stage = 0, parity ^= 1;
     }
@@ -575,16 +641,8 @@ struct Ring {
     return ok;
   }
 };
-
-// Steps of a ring's chunk that are not live: as load() leaves them
-template <class T, int V, int L>
-__device__ __forceinline__ void blank(Pack<T, V> (&out)[L], const Chunk& q, float other = 0.0f) {
-#pragma unroll
-  for (int l = 0; l < L; ++l)
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (!((q.live >> l) & 1u)) out[l].v[v] = narrow<T>(other);
-}
+// a warp without a ring, where every lane loads its own
+struct NoRing {};
 
 // ------------------------------------------------------------------- forward
 
@@ -592,81 +650,99 @@ template <class T, int V, int L>
 struct Loaded {
   Chunk q;
   Pack<T, V> x[L], ig[L], rg[L];
+  template <class R>
+  __device__ __forceinline__ void get(const Args& p, const R& ring, int stage) {
+    ring.get(p, stage, 0, rg);
+    ring.get(p, stage, 1, ig);
+    ring.get(p, stage, 2, x);
+  }
+  template <bool kMask, bool kFull>
+  __device__ __forceinline__ void read(const Args& p, const Lane& o, int k) {
+    q = chunk_of<L, kMask>(p, o, k);
+    flag_chunk<L, kMask>(p, o, q);
+    load<T, V, L, kFull>(rg, p.rg, o, q, kShut);
+    load<T, V, L, kFull>(ig, p.ig, o, q);
+    load<T, V, L, kFull>(x, p.x, o, q);
+  }
 };
 
-template <class T, int V, int L, bool kMask, bool kFull>
-__device__ __forceinline__ void read_chunk(const Args& p, const Lane& o, int k, Loaded<T, V, L>& in) {
-  in.q = chunk_of<L, kMask>(p, o, k);
-  load<T, V, L, kFull>(in.rg, p.rg, o, in.q, kShut);
-  load<T, V, L, kFull>(in.ig, p.ig, o, in.q);
-  load<T, V, L, kFull>(in.x, p.x, o, in.q);
-}
-
-template <class T, int V, int L, bool kMask>
-__device__ __forceinline__ void ring_chunk(const Args& p, const Lane& o, const Ring<T, V, L, 3, false>& ring, int stage, int k,
-                                           int whole, Loaded<T, V, L>& in) {
-  in.q = chunk_of<L, kMask>(p, o, k);
-  ring.get(p, stage, 0, in.rg);
-  ring.get(p, stage, 1, in.ig);
-  ring.get(p, stage, 2, in.x);
-  if (kMask || k - o.first >= whole) {
-    blank(in.rg, in.q, kShut);
-    blank(in.ig, in.q);
-    blank(in.x, in.q);
+// Takes the strip's chunks in scan order: work(k, in, whole).  The last one of a row may lack steps.
+template <class T, int V, int L, bool kMask, class R, class W>
+__device__ __forceinline__ bool forward_walk(const Args& p, const Lane& o, R& ring, W work) {
+  using In = Loaded<T, V, L>;
+  if constexpr (!std::is_same<R, NoRing>::value) {
+    return ring.template walk<kMask, In>(
+        p, o, o.first, o.count, 1, [&](int stage, In& in) { in.get(p, ring, stage); },
+        [&](int k, In& in) {
+          if (k - o.first < o.whole)
+            work(k, in, std::true_type{});
+          else
+            work(k, in, std::false_type{});
+        });
+  } else {
+    walk<In>(
+        o.whole, [&](int k, In& in) { in.template read<kMask, true>(p, o, o.first + k); },
+        [&](int k, In& in) { work(o.first + k, in, std::true_type{}); });
+    if (o.whole < o.count) {
+      In in;
+      in.template read<kMask, false>(p, o, o.first + o.whole);
+      work(o.first + o.whole, in, std::false_type{});
+    }
+    return true;
   }
 }
 
-template <class T, int V, int L, bool kMask, bool kFar, bool kBulk>
-__device__ __forceinline__ void forward_maps(const Args& p, const Maps& m, const Lane& o,
+template <class T, int V, int L, bool kMask, bool kFar, class R>
+__device__ __forceinline__ void forward_maps(const Args& p, const Lane& o, R& ring,
                                              const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P]) {
   using Q = Pairing<V, L>;
   constexpr int N = Q::N, P = Q::P;
   Vec<N> A[P], H[P];
 #pragma unroll
   for (int j = 0; j < P; ++j) A[j] = splat<N>(1.0f), H[j] = splat<N>(0.0f);
-  const auto work = [&](int, const Loaded<T, V, L>& in) {
-    each_gate<T, V, L, kMask, kFar>(in.q, in.ig, in.rg, rate, [&](int l, int j, const Gates<N>& g, Vec<N> beta) {
-      H[j] = apply<kMask>(g.a, H[j], beta * (g.i * widen<N>(in.x[l], j)));
-      A[j] = A[j] * g.a;
-    });
-  };
-  const int whole = kMask ? o.count : o.whole;
+  forward_walk<T, V, L, kMask>(p, o, ring, [&](int, Loaded<T, V, L>& in, auto) {
+    if (in.q.live != (1u << L) - 1) blank(in.rg, in.q, kShut), blank(in.ig, in.q), blank(in.x, in.q);
+    each_gate<T, V, L, kMask, kFar>(
+        cuts<kMask>(p, in.q), in.ig, in.rg, rate, [&](int l, int j, const Gates<N>& g, Vec<N> beta) {
+          H[j] = apply<kMask>(g.a, H[j], beta * (g.i * widen<N>(in.x[l], j)));
+          A[j] = A[j] * g.a;
+        });
+  });
+  join_maps<V, N, kMask>(p, o, A, H);
+}
+
+// The ring of a forward warp, with its first copies on their way
+template <class T, int V, int L, bool kBulk>
+__device__ __forceinline__ auto forward_ring(const Args& p, const Maps& m, const Lane& o) {
   if constexpr (kBulk) {
     extern __shared__ __align__(128) char dynamic[];
     __shared__ uint64_t s_bar[kStrips * kRing<T>];
     Ring<T, V, L, 3, false> ring(dynamic, s_bar);
     ring.map[0] = &m.rg, ring.map[1] = &m.ig, ring.map[2] = &m.x;
-    ring.template walk<Loaded<T, V, L>>(
-        p, o, o.first, o.count, 1,
-        [&](int stage, int k, Loaded<T, V, L>& in) { ring_chunk<T, V, L, kMask>(p, o, ring, stage, k, whole, in); },
-        [&](int k, const Loaded<T, V, L>& in) { work(k, in); });
+    ring.start(p, o, o.first, o.count, 1);
+    return ring;
   } else {
-    walk<Loaded<T, V, L>>(
-        whole, [&](int k, Loaded<T, V, L>& in) { read_chunk<T, V, L, kMask, !kMask>(p, o, o.first + k, in); }, work);
-    if (whole < o.count) {
-      Loaded<T, V, L> in;
-      read_chunk<T, V, L, kMask, false>(p, o, o.first + whole, in);
-      work(0, in);
-    }
+    return NoRing{};
   }
-  join_maps<V, N, kMask>(p, o, A, H);
 }
 
 template <class T, int V, int L, bool kMask, bool kBulk>
 __global__ void __launch_bounds__(32 * kStrips) forward_maps_kernel(const __grid_constant__ Args p,
-                                                              const __grid_constant__ Maps m) {
+                                                                    const __grid_constant__ Maps m) {
   using Q = Pairing<V, L>;
+  let_next_start();
   const Lane o = lane_of<V, L, kMask, false>(p);
+  auto ring = forward_ring<T, V, L, kBulk>(p, m, o);
   Vec<Q::N> rate[Q::P];
   // (the CTA's warps share their channels, so they agree, and meet in join_maps)
   if (rates<V, Q::N>(p, o, rate))
-    forward_maps<T, V, L, kMask, true, kBulk>(p, m, o, rate);
+    forward_maps<T, V, L, kMask, true>(p, o, ring, rate);
   else
-    forward_maps<T, V, L, kMask, false, kBulk>(p, m, o, rate);
+    forward_maps<T, V, L, kMask, false>(p, o, ring, rate);
 }
 
 template <class T, int V, int L, bool kMask, bool kFar, bool kFull>
-__device__ __forceinline__ void forward_chunk(const Args& p, const Lane& o, int k, const Loaded<T, V, L>& in,
+__device__ __forceinline__ void forward_chunk(const Args& p, const Lane& o, int k, Loaded<T, V, L>& in,
                                               const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P],
                                               Vec<Pairing<V, L>::N> (&h)[Pairing<V, L>::P]) {
   using Q = Pairing<V, L>;
@@ -676,56 +752,35 @@ __device__ __forceinline__ void forward_chunk(const Args& p, const Lane& o, int 
 #pragma unroll
     for (int v = 0; v < V; ++v) keep[v] = h[v / N].v[v % N];
   }
+  if (in.q.live != (1u << L) - 1) blank(in.rg, in.q, kShut), blank(in.ig, in.q), blank(in.x, in.q);
   char* y = reinterpret_cast<char*>(static_cast<T*>(p.y) + (o.b * p.steps + in.q.t0) * p.width + o.c);
   const int step = o.dir * (int)p.width * (int)sizeof(T);
   Vec<N> out[P];
-  each_gate<T, V, L, kMask, kFar>(in.q, in.ig, in.rg, rate, [&](int l, int j, const Gates<N>& g, Vec<N> beta) {
-    h[j] = apply<kMask>(g.a, h[j], beta * (g.i * widen<N>(in.x[l], j)));
-    out[j] = !kMask || ((in.q.live >> l) & 1u) ? h[j] : splat<N>(0.0f);
-    if (j == P - 1 && o.on && (kFull || ((in.q.inside >> l) & 1u))) store<T, V, N>(y + (int64_t)step * l, out);
-  });
+  each_gate<T, V, L, kMask, kFar>(
+      cuts<kMask>(p, in.q), in.ig, in.rg, rate, [&](int l, int j, const Gates<N>& g, Vec<N> beta) {
+        h[j] = apply<kMask>(g.a, h[j], beta * (g.i * widen<N>(in.x[l], j)));
+        out[j] = !kMask || ((in.q.live >> l) & 1u) ? h[j] : splat<N>(0.0f);
+        if (j == P - 1 && o.on && (kFull || ((in.q.inside >> l) & 1u))) store<T, V, N>(y + (int64_t)step * l, out);
+      });
 }
 
-template <class T, int V, int L, bool kMask, bool kFar, bool kBulk>
-__device__ __forceinline__ void forward_strip(const Args& p, const Maps& m, const Lane& o,
+template <class T, int V, int L, bool kMask, bool kFar, class R>
+__device__ __forceinline__ void forward_strip(const Args& p, const Lane& o, R& ring,
                                               const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P]) {
   using Q = Pairing<V, L>;
   constexpr int N = Q::N, P = Q::P;
-  if (o.count == 0) return;
   Vec<N> h[P];
 #pragma unroll
   for (int j = 0; j < P; ++j) h[j] = splat<N>(0.0f);
   if (p.state) read_row<V, N>(p.state + o.b * p.width + o.from, h);
+  if (p.strips > 1) wait_for_last();
+  if (o.all_count == 0) return;
   start_of<V, N, kMask>(p, o, h);
-  // whole chunks, then the row's last steps (with masks every chunk may be partial)
-  const int whole = kMask ? o.count : o.whole;
-  if constexpr (kBulk) {
-    extern __shared__ __align__(128) char dynamic[];
-    __shared__ uint64_t s_bar[kStrips * kRing<T>];
-    Ring<T, V, L, 3, false> ring(dynamic, s_bar);
-    ring.map[0] = &m.rg, ring.map[1] = &m.ig, ring.map[2] = &m.x;
-    if (!ring.template walk<Loaded<T, V, L>>(
-            p, o, o.first, o.count, 1,
-            [&](int stage, int k, Loaded<T, V, L>& in) { ring_chunk<T, V, L, kMask>(p, o, ring, stage, k, whole, in); },
-            [&](int k, const Loaded<T, V, L>& in) {
-              if (kMask || k - o.first < whole)
-                forward_chunk<T, V, L, kMask, kFar, !kMask>(p, o, k, in, rate, h);
-              else
-                forward_chunk<T, V, L, kMask, kFar, false>(p, o, k, in, rate, h);
-            }))
-      return;
-  } else {
-    walk<Loaded<T, V, L>>(
-        whole, [&](int k, Loaded<T, V, L>& in) { read_chunk<T, V, L, kMask, !kMask>(p, o, o.first + k, in); },
-        [&](int k, const Loaded<T, V, L>& in) {
-          forward_chunk<T, V, L, kMask, kFar, !kMask>(p, o, o.first + k, in, rate, h);
-        });
-    if (whole < o.count) {
-      Loaded<T, V, L> in;
-      read_chunk<T, V, L, kMask, false>(p, o, o.first + whole, in);
-      forward_chunk<T, V, L, kMask, kFar, false>(p, o, o.first + whole, in, rate, h);
-    }
-  }
+  if (!forward_walk<T, V, L, kMask>(p, o, ring, [&](int k, Loaded<T, V, L>& in, auto full) {
+        forward_chunk<T, V, L, kMask, kFar, decltype(full)::value>(p, o, k, in, rate, h);
+      }))
+    return;
+  if (kMask) zero_rest<T, V, L>(p, o, p.y);
   if (o.rank == p.strips - 1 && o.on) {
 #pragma unroll
     for (int v = 0; v < V; ++v) p.last[o.b * p.width + o.c + v] = h[v / N].v[v % N];
@@ -734,14 +789,15 @@ __device__ __forceinline__ void forward_strip(const Args& p, const Maps& m, cons
 
 template <class T, int V, int L, bool kMask, bool kBulk>
 __global__ void __launch_bounds__(32 * kStrips) forward_kernel(const __grid_constant__ Args p,
-                                                              const __grid_constant__ Maps m) {
+                                                               const __grid_constant__ Maps m) {
   using Q = Pairing<V, L>;
   const Lane o = lane_of<V, L, kMask, false>(p);
+  auto ring = forward_ring<T, V, L, kBulk>(p, m, o);
   Vec<Q::N> rate[Q::P];
   if (rates<V, Q::N>(p, o, rate))
-    forward_strip<T, V, L, kMask, true, kBulk>(p, m, o, rate);
+    forward_strip<T, V, L, kMask, true>(p, o, ring, rate);
   else
-    forward_strip<T, V, L, kMask, false, kBulk>(p, m, o, rate);
+    forward_strip<T, V, L, kMask, false>(p, o, ring, rate);
 }
 
 // ------------------------------------------------------------------ backward
@@ -750,26 +806,86 @@ template <class T, int V, int L>
 struct LoadedMap {
   Chunk q;
   Pack<T, V> rg[L], dy[L];
+  template <class R>
+  __device__ __forceinline__ void get(const Args& p, const R& ring, int stage) {
+    ring.get(p, stage, 0, rg);
+    ring.get(p, stage, 1, dy);
+  }
+  template <bool kMask, bool kFull>
+  __device__ __forceinline__ void read(const Args& p, const Lane& o, int k) {
+    q = chunk_of<L, kMask>(p, o, k);
+    flag_chunk<L, kMask>(p, o, q);
+    load<T, V, L, kFull>(rg, p.rg, o, q, kShut);
+    load<T, V, L, kFull>(dy, p.dy, o, q);
+  }
 };
 
-template <class T, int V, int L, bool kMask, bool kFull>
-__device__ __forceinline__ void read_map(const Args& p, const Lane& o, int k, LoadedMap<T, V, L>& in) {
-  in.q = chunk_of<L, kMask>(p, o, k);
-  load<T, V, L, kFull>(in.rg, p.rg, o, in.q, kShut);
-  load<T, V, L, kFull>(in.dy, p.dy, o, in.q);
+template <class T, int V, int L>
+struct LoadedBack {
+  Chunk q;
+  Pack<T, V> x[L], ig[L], rg[L], dy[L];
+  Vec<Pairing<V, L>::N> h[Pairing<V, L>::P];  // state before the chunk
+  template <class R>
+  __device__ __forceinline__ void get(const Args& p, const R& ring, int stage) {
+    ring.get(p, stage, 0, rg);
+    ring.get(p, stage, 1, ig);
+    ring.get(p, stage, 2, x);
+    ring.get(p, stage, 3, dy);
+    const Pack<float, V> s = ring.state(stage);
+#pragma unroll
+    for (int j = 0; j < Pairing<V, L>::P; ++j) h[j] = widen<Pairing<V, L>::N>(s, j);
+  }
+  template <bool kMask, bool kFull>
+  __device__ __forceinline__ void read(const Args& p, const Lane& o, int k) {
+    q = chunk_of<L, kMask>(p, o, k);
+    flag_chunk<L, kMask>(p, o, q);
+    load<T, V, L, kFull>(rg, p.rg, o, q, kShut);
+    load<T, V, L, kFull>(ig, p.ig, o, q);
+    load<T, V, L, kFull>(x, p.x, o, q);
+    load<T, V, L, kFull>(dy, p.dy, o, q);
+    read_row<V, Pairing<V, L>::N>(p.kept + (o.b * ((p.steps + L - 1) / L) + k) * p.width + o.from, h);
+  }
+};
+
+// Takes the strip's chunks against scan order
+template <class T, int V, int L, bool kMask, class In, class R, class W>
+__device__ __forceinline__ bool backward_walk(const Args& p, const Lane& o, R& ring, W work) {
+  if constexpr (!std::is_same<R, NoRing>::value) {
+    return ring.template walk<kMask, In>(
+        p, o, o.first + o.count - 1, o.count, -1, [&](int stage, In& in) { in.get(p, ring, stage); },
+        [&](int k, In& in) {
+          if (k - o.first < o.whole)
+            work(in, std::true_type{});
+          else
+            work(in, std::false_type{});
+        });
+  } else {
+    if (o.whole < o.count) {
+      In in;
+      in.template read<kMask, false>(p, o, o.first + o.whole);
+      work(in, std::false_type{});
+    }
+    walk<In>(
+        o.whole, [&](int k, In& in) { in.template read<kMask, true>(p, o, o.first + o.whole - 1 - k); },
+        [&](int, In& in) { work(in, std::true_type{}); });
+    return true;
+  }
 }
 
 // e -> A e + E of a strip, from its last step to its first: the decay gate and
 // dy are all it takes
-template <class T, int V, int L, bool kMask, bool kFar, bool kBulk>
-__device__ __forceinline__ void backward_maps(const Args& p, const Maps& m, const Lane& o,
+template <class T, int V, int L, bool kMask, bool kFar, class R>
+__device__ __forceinline__ void backward_maps(const Args& p, const Lane& o, R& ring,
                                               const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P]) {
   using Q = Pairing<V, L>;
   constexpr int N = Q::N, P = Q::P;
   Vec<N> A[P], E[P];
 #pragma unroll
   for (int j = 0; j < P; ++j) A[j] = splat<N>(1.0f), E[j] = splat<N>(0.0f);
-  const auto work = [&](int, LoadedMap<T, V, L>& in) {
+  using In = LoadedMap<T, V, L>;
+  backward_walk<T, V, L, kMask, In>(p, o, ring, [&](In& in, auto) {
+    if (in.q.live != (1u << L) - 1) blank(in.rg, in.q, kShut), blank(in.dy, in.q);
+    const unsigned cut = cuts<kMask>(p, in.q);
     Vec<N> rg[L * P], k2[L * P], a[L * P];
 #pragma unroll
     for (int l = 0; l < L; ++l) {
@@ -783,68 +899,45 @@ __device__ __forceinline__ void backward_maps(const Args& p, const Maps& m, cons
 #pragma unroll
       for (int j = 0; j < P; ++j) {
         Vec<N> al = a[l * P + j];
-        if (kMask && ((in.q.cut >> l) & 1u)) al = splat<N>(0.0f);
+        if (kMask && ((cut >> l) & 1u)) al = splat<N>(0.0f);
         E[j] = apply<kMask>(al, E[j] + widen<N>(in.dy[l], j), splat<N>(0.0f));
         A[j] = A[j] * al;
       }
     }
-  };
-  const int whole = kMask ? o.count : o.whole;
+  });
+  join_maps<V, N, kMask>(p, o, A, E);
+}
+
+template <class T, int V, int L, bool kBulk, bool kMaps>
+__device__ __forceinline__ auto backward_ring(const Args& p, const Maps& m, const Lane& o) {
   if constexpr (kBulk) {
     extern __shared__ __align__(128) char dynamic[];
     __shared__ uint64_t s_bar[kStrips * kRing<T>];
-    Ring<T, V, L, 2, false> ring(dynamic, s_bar);
-    ring.map[0] = &m.rg, ring.map[1] = &m.dy;
-    ring.template walk<LoadedMap<T, V, L>>(
-        p, o, o.first + o.count - 1, o.count, -1,
-        [&](int stage, int k, LoadedMap<T, V, L>& in) {
-          in.q = chunk_of<L, kMask>(p, o, k);
-          ring.get(p, stage, 0, in.rg);
-          ring.get(p, stage, 1, in.dy);
-          if (kMask || k - o.first >= whole) blank(in.rg, in.q, kShut), blank(in.dy, in.q);
-        },
-        work);
+    Ring<T, V, L, kMaps ? 2 : 4, !kMaps> ring(dynamic, s_bar);
+    ring.map[0] = &m.rg;
+    if constexpr (kMaps)
+      ring.map[1] = &m.dy;
+    else
+      ring.map[1] = &m.ig, ring.map[2] = &m.x, ring.map[3] = &m.dy;
+    ring.start(p, o, o.first + o.count - 1, o.count, -1);
+    return ring;
   } else {
-    if (whole < o.count) {
-      LoadedMap<T, V, L> in;
-      read_map<T, V, L, kMask, false>(p, o, o.first + whole, in);
-      work(0, in);
-    }
-    walk<LoadedMap<T, V, L>>(
-        whole,
-        [&](int k, LoadedMap<T, V, L>& in) { read_map<T, V, L, kMask, !kMask>(p, o, o.first + whole - 1 - k, in); },
-        work);
+    return NoRing{};
   }
-  join_maps<V, N, kMask>(p, o, A, E);
 }
 
 template <class T, int V, int L, bool kMask, bool kBulk>
 __global__ void __launch_bounds__(32 * kStrips) backward_maps_kernel(const __grid_constant__ Args p,
-                                                              const __grid_constant__ Maps m) {
+                                                                     const __grid_constant__ Maps m) {
   using Q = Pairing<V, L>;
+  let_next_start();
   const Lane o = lane_of<V, L, kMask, true>(p);
+  auto ring = backward_ring<T, V, L, kBulk, true>(p, m, o);
   Vec<Q::N> rate[Q::P];
   if (rates<V, Q::N>(p, o, rate))
-    backward_maps<T, V, L, kMask, true, kBulk>(p, m, o, rate);
+    backward_maps<T, V, L, kMask, true>(p, o, ring, rate);
   else
-    backward_maps<T, V, L, kMask, false, kBulk>(p, m, o, rate);
-}
-
-template <class T, int V, int L>
-struct LoadedBack {
-  Chunk q;
-  Pack<T, V> x[L], ig[L], rg[L], dy[L];
-  Vec<Pairing<V, L>::N> h[Pairing<V, L>::P];  // state before the chunk
-};
-
-template <class T, int V, int L, bool kMask, bool kFull>
-__device__ __forceinline__ void read_back(const Args& p, const Lane& o, int k, LoadedBack<T, V, L>& in) {
-  in.q = chunk_of<L, kMask>(p, o, k);
-  load<T, V, L, kFull>(in.rg, p.rg, o, in.q, kShut);
-  load<T, V, L, kFull>(in.ig, p.ig, o, in.q);
-  load<T, V, L, kFull>(in.x, p.x, o, in.q);
-  load<T, V, L, kFull>(in.dy, p.dy, o, in.q);
-  read_row<V, Pairing<V, L>::N>(p.kept + (o.b * ((p.steps + L - 1) / L) + k) * p.width + o.from, in.h);
+    backward_maps<T, V, L, kMask, false>(p, o, ring, rate);
 }
 
 // With e = a g (see above) everything but g is known before the carry comes in:
@@ -852,16 +945,18 @@ __device__ __forceinline__ void read_back(const Args& p, const Lane& o, int k, L
 //   P1 = beta i, P2 = x (1 - i), R1 = r (a h_{t-1} - (a^2 / beta) i x), R2 = rate (r - 1),
 // and s sums up to the decay gradient.
 template <class T, int V, int L, bool kMask, bool kFar, bool kFull>
-__device__ __forceinline__ void backward_chunk(const Args& p, const Lane& o, const LoadedBack<T, V, L>& in,
+__device__ __forceinline__ void backward_chunk(const Args& p, const Lane& o, LoadedBack<T, V, L>& in,
                                                const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P],
                                                Vec<Pairing<V, L>::N> (&e)[Pairing<V, L>::P],
                                                Vec<Pairing<V, L>::N> (&acc)[Pairing<V, L>::P]) {
   using Q = Pairing<V, L>;
   constexpr int N = Q::N, P = Q::P;
+  if (in.q.live != (1u << L) - 1)
+    blank(in.rg, in.q, kShut), blank(in.ig, in.q), blank(in.x, in.q), blank(in.dy, in.q);
   Vec<N> a[L][P], p1[L][P], p2[L][P], r1[L][P], r2[L][P], h[P];
 #pragma unroll
   for (int j = 0; j < P; ++j) h[j] = in.h[j];
-  each_gate<T, V, L, kMask, kFar>(in.q, in.ig, in.rg, rate, [&](int l, int j, const Gates<N>& g, Vec<N> beta) {
+  each_gate<T, V, L, kMask, kFar>(cuts<kMask>(p, in.q), in.ig, in.rg, rate, [&](int l, int j, const Gates<N>& g, Vec<N> beta) {
     const Vec<N> x = widen<N>(in.x[l], j);
     Vec<N> inverse;  // dropped with beta
 #pragma unroll
@@ -914,56 +1009,27 @@ __device__ __forceinline__ void backward_chunk(const Args& p, const Lane& o, con
   }
 }
 
-template <class T, int V, int L, bool kMask, bool kFar, bool kBulk>
-__device__ __forceinline__ void backward_strip(const Args& p, const Maps& m, const Lane& o,
+template <class T, int V, int L, bool kMask, bool kFar, class R>
+__device__ __forceinline__ void backward_strip(const Args& p, const Lane& o, R& ring,
                                                const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P]) {
   using Q = Pairing<V, L>;
   constexpr int N = Q::N, P = Q::P;
-  if (o.count == 0) return;
-  const int whole = kMask ? o.count : o.whole;
   Vec<N> e[P], acc[P];
 #pragma unroll
   for (int j = 0; j < P; ++j) e[j] = acc[j] = splat<N>(0.0f);
   if (p.dlast) read_row<V, N>(p.dlast + o.b * p.width + o.from, e);
+  if (p.strips > 1) wait_for_last();
+  if (o.all_count == 0) return;
   start_of<V, N, kMask>(p, o, e);
-  if constexpr (kBulk) {
-    extern __shared__ __align__(128) char dynamic[];
-    __shared__ uint64_t s_bar[kStrips * kRing<T>];
-    Ring<T, V, L, 4, true> ring(dynamic, s_bar);
-    ring.map[0] = &m.rg, ring.map[1] = &m.ig, ring.map[2] = &m.x, ring.map[3] = &m.dy;
-    if (!ring.template walk<LoadedBack<T, V, L>>(
-            p, o, o.first + o.count - 1, o.count, -1,
-            [&](int stage, int k, LoadedBack<T, V, L>& in) {
-              in.q = chunk_of<L, kMask>(p, o, k);
-              ring.get(p, stage, 0, in.rg);
-              ring.get(p, stage, 1, in.ig);
-              ring.get(p, stage, 2, in.x);
-              ring.get(p, stage, 3, in.dy);
-              const Pack<float, V> h = ring.state(stage);
-#pragma unroll
-              for (int j = 0; j < P; ++j) in.h[j] = widen<N>(h, j);
-              if (kMask || k - o.first >= whole)
-                blank(in.rg, in.q, kShut), blank(in.ig, in.q), blank(in.x, in.q), blank(in.dy, in.q);
-            },
-            [&](int k, const LoadedBack<T, V, L>& in) {
-              if (kMask || k - o.first < whole)
-                backward_chunk<T, V, L, kMask, kFar, !kMask>(p, o, in, rate, e, acc);
-              else
-                backward_chunk<T, V, L, kMask, kFar, false>(p, o, in, rate, e, acc);
-            }))
-      return;
-  } else {
-    if (whole < o.count) {
-      LoadedBack<T, V, L> in;
-      read_back<T, V, L, kMask, false>(p, o, o.first + whole, in);
-      backward_chunk<T, V, L, kMask, kFar, false>(p, o, in, rate, e, acc);
-    }
-    walk<LoadedBack<T, V, L>>(
-        whole,
-        [&](int k, LoadedBack<T, V, L>& in) { read_back<T, V, L, kMask, !kMask>(p, o, o.first + whole - 1 - k, in); },
-        [&](int, const LoadedBack<T, V, L>& in) {
-          backward_chunk<T, V, L, kMask, kFar, !kMask>(p, o, in, rate, e, acc);
-        });
+  using In = LoadedBack<T, V, L>;
+  if (!backward_walk<T, V, L, kMask, In>(p, o, ring, [&](In& in, auto full) {
+        backward_chunk<T, V, L, kMask, kFar, decltype(full)::value>(p, o, in, rate, e, acc);
+      }))
+    return;
+  if (kMask) {
+    zero_rest<T, V, L>(p, o, p.dx);
+    zero_rest<T, V, L>(p, o, p.dig);
+    zero_rest<T, V, L>(p, o, p.drg);
   }
   if (!o.on) return;
 #pragma unroll
@@ -975,18 +1041,20 @@ __device__ __forceinline__ void backward_strip(const Args& p, const Maps& m, con
 
 template <class T, int V, int L, bool kMask, bool kBulk>
 __global__ void __launch_bounds__(32 * kStrips) backward_kernel(const __grid_constant__ Args p,
-                                                              const __grid_constant__ Maps m) {
+                                                                const __grid_constant__ Maps m) {
   using Q = Pairing<V, L>;
+  let_next_start();
   const Lane o = lane_of<V, L, kMask, true>(p);
+  auto ring = backward_ring<T, V, L, kBulk, false>(p, m, o);
   Vec<Q::N> rate[Q::P];
   if (rates<V, Q::N>(p, o, rate))
-    backward_strip<T, V, L, kMask, true, kBulk>(p, m, o, rate);
+    backward_strip<T, V, L, kMask, true>(p, o, ring, rate);
   else
-    backward_strip<T, V, L, kMask, false, kBulk>(p, m, o, rate);
+    backward_strip<T, V, L, kMask, false>(p, o, ring, rate);
 }
 
 struct Geometry {
-  int vec, chunk, ctiles, strips, strip;
+  int vec, chunk, ctiles, strips, strip, warps;
   bool bulk;
 };
 

@@ -24,11 +24,12 @@ __device__ uint32_t g_error;
 
 // ddecay[c] = -rate sigmoid(decay[c]) sum over the rows of part, in a fixed
 // order: 32 columns a block, every thread a stride of the rows, then a tree.
-constexpr int kSumRows = 16;
+constexpr int kSumRows = 32;
 __global__ void __launch_bounds__(32 * kSumRows) decay_sum_kernel(const float* part, int64_t rows, int64_t width,
                                                                   const float* decay, float rate, float* out) {
   __shared__ float s[kSumRows][33];
   const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x;
+  wait_for_last();
   float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   if (c < width) {
     int64_t r = threadIdx.y;
@@ -68,12 +69,24 @@ bool fits(const pesq_stream& s, int vec, const pesq_gated_scan_desc& d) {
          (d.steps == 1 || s.step_stride % vec == 0);
 }
 
-// Warps that fill the device, and the fewest steps of a strip and of a row that is copied in boxes
-constexpr int64_t kWarpsWanted = 148 * 12;
+// Rows and channels that make this many warps are not cut
 constexpr int64_t kWarpsEnough = 148 * 4;
+// and that many take pairs of channels
+constexpr int64_t kWarpsForPairs = 148 * 12;
+// the fewest steps of a strip, and of a row that is copied in boxes
 constexpr int kFewestSteps = 32;
 constexpr int64_t kFewestBulk = 32;
-constexpr int64_t kWarpsForPairs = 148 * 12;
+
+// What an SM holds by registers and shared memory, as CTAs of so many warps: cut rows
+// make one wave of them
+struct Resident {
+  int ctas, warps;
+};
+Resident resident(bool bulk, bool backward, bool mask, int dtype) {
+  if (!backward) return bulk ? Resident{3, 8} : Resident{2, 8};
+  if (!bulk) return Resident{3, 4};
+  return mask ? Resident{2, 4} : dtype == PESQ_F32 ? Resident{3, 4} : Resident{2, 8};
+}
 
 // Whether boxes can be copied: 16-byte addresses and strides, which a tensor map asks for
 bool boxes(const pesq_stream& s, const pesq_gated_scan_desc& d) {
@@ -98,11 +111,9 @@ EncodeTiled encoder() {
   return fn;
 }
 
-// From the inputs alone, so that a backward call takes its forward's chunks.
-// Pairs of channels where everything allows it and leaves warps enough.  One strip a
-// row once rows and channels make kWarpsEnough warps; otherwise as many as make
-// kWarpsWanted.
-Geometry geometry(const pesq_gated_scan_desc& d) {
+// Chunks follow from the inputs alone, so that a backward call takes its forward's.
+// Pairs of channels where everything allows it and leaves warps enough.
+Geometry geometry(const pesq_gated_scan_desc& d, bool backward) {
   Geometry g{};
   g.bulk = d.steps >= kFewestBulk && d.width * (int64_t)element(d.dtype) % 16 == 0 && boxes(d.x, d) &&
            boxes(d.input_gate, d) && boxes(d.decay_gate, d);
@@ -114,12 +125,15 @@ Geometry geometry(const pesq_gated_scan_desc& d) {
   g.chunk = d.steps == 1 ? 1 : chunk_steps(g.vec, g.bulk);
   const int64_t chunks = (d.steps + g.chunk - 1) / g.chunk, warps = d.batch * g.ctiles;
   int64_t strips = 1;
-  if (warps < kWarpsEnough)
-    strips = std::max<int64_t>(
-        1, std::min((kWarpsWanted + warps - 1) / warps, (d.steps + kFewestSteps - 1) / kFewestSteps));
+  const Resident sm = resident(g.bulk, backward, d.reset || d.lengths, d.dtype);
+  if (warps < kWarpsEnough) {
+    strips = std::max<int64_t>(1, 148 * sm.ctas / warps) * sm.warps;
+    strips = std::max<int64_t>(1, std::min(strips, (d.steps + kFewestSteps - 1) / kFewestSteps));
+  }
   const int64_t per = (chunks + strips - 1) / strips;
   g.strips = (int)((chunks + per - 1) / per);
   g.strip = (int)(per * g.chunk);
+  g.warps = std::min(g.strips, sm.warps);
   return g;
 }
 
@@ -141,7 +155,7 @@ bool encode(CUtensorMap& m, const pesq_stream& s, const pesq_gated_scan_desc& d,
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 // maps of strips and of CTAs of strips
 size_t map_bytes(const pesq_gated_scan_desc& d, const Geometry& g) {
-  return g.strips == 1 ? 0 : round16((size_t)(d.batch * (g.strips + (g.strips + kStrips - 1) / kStrips) * d.width) * 8);
+  return g.strips == 1 ? 0 : round16((size_t)(d.batch * (g.strips + (g.strips + g.warps - 1) / g.warps) * d.width) * 8);
 }
 size_t kept_bytes(const pesq_gated_scan_desc& d, const Geometry& g) {
   return round16((size_t)(d.batch * ((d.steps + g.chunk - 1) / g.chunk) * d.width) * 4);
@@ -236,10 +250,10 @@ extern "C" {
 int pesq_gated_scan_sizes(const pesq_gated_scan_desc* d, size_t* forward, size_t* kept, size_t* backward) {
   if (!forward || !kept || !backward) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL argument");
   if (const int status = check(d)) return status;
-  const Geometry g = geometry(*d);
+  const Geometry g = geometry(*d, false);
   *forward = map_bytes(*d, g);
   *kept = kept_bytes(*d, g);
-  *backward = back_bytes(*d, g);
+  *backward = back_bytes(*d, geometry(*d, true));
   return PESQ_OK;
 }
 
@@ -247,7 +261,7 @@ int pesq_gated_scan_forward(const pesq_gated_scan_desc* d, void* stream, void* y
                             size_t kept_size, void* workspace, size_t workspace_bytes) {
   if (const int status = check(d)) return status;
   if (!y || !last) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL output");
-  const Geometry g = geometry(*d);
+  const Geometry g = geometry(*d, false);
   if (!fits(y, g.vec, *d)) return set_error(PESQ_ERR_INVALID_ARGUMENT, "y is less aligned than the inputs");
   if (missing(workspace, workspace_bytes, map_bytes(*d, g)) || (kept && missing(kept, kept_size, kept_bytes(*d, g))))
     return set_error(PESQ_ERR_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
@@ -264,7 +278,7 @@ int pesq_gated_scan_backward(const pesq_gated_scan_desc* d, void* stream, const 
                              float* ddecay, float* dstate, void* workspace, size_t workspace_bytes) {
   if (const int status = check(d)) return status;
   if (!dx || !dinput_gate || !ddecay_gate || !ddecay) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL output");
-  const Geometry g = geometry(*d);
+  const Geometry g = geometry(*d, true);
   if ((dy.data && (g.bulk ? !boxes(dy, *d) : !fits(dy, g.vec, *d))) || !fits(dx, g.vec, *d) || !fits(dinput_gate, g.vec, *d) ||
       !fits(ddecay_gate, g.vec, *d))
     return set_error(PESQ_ERR_INVALID_ARGUMENT, "a gradient is less aligned than the inputs");
@@ -293,9 +307,17 @@ int pesq_gated_scan_backward(const pesq_gated_scan_desc* d, void* stream, const 
   a.dpart = reinterpret_cast<float*>(ws);
   a.kept = const_cast<float*>(static_cast<const float*>(kept));
   if (const int status = run(*d, a, g, &dy, s)) return status;
-  decay_sum_kernel<<<(unsigned)((d->width + 31) / 32), dim3(32, kSumRows), 0, s>>>(
-      a.dpart, d->batch * g.strips, d->width, d->decay, d->rate, ddecay);
-  const cudaError_t e = cudaGetLastError();
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3((unsigned)((d->width + 31) / 32));
+  c.blockDim = dim3(32, kSumRows);
+  c.stream = s;
+  c.attrs = &at;
+  c.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&c, decay_sum_kernel, (const float*)a.dpart, (int64_t)(d->batch * g.strips),
+                                           d->width, d->decay, d->rate, ddecay);
   return e == cudaSuccess ? PESQ_OK : set_error(PESQ_ERR_CUDA, cudaGetErrorString(e));
 }
 

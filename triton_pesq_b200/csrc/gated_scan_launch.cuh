@@ -7,32 +7,43 @@
 namespace pesq {
 namespace gscan {
 
+// `after`: the kernel waits by itself for the one launched before it
 template <class K>
-cudaError_t start(K kernel, const Args& p, const Maps& m, const Geometry& g, size_t warp_smem, cudaStream_t s) {
-  const int warps = g.strips < kStrips ? g.strips : kStrips;
+cudaError_t start(K kernel, const Args& p, const Maps& m, const Geometry& g, size_t warp_smem, bool after,
+                  cudaStream_t s) {
+  const int warps = g.warps;
   const size_t smem = warps * warp_smem;
   if (smem > 40 << 10) {  // beside the static part, more than a kernel gets without asking
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
   }
-  const dim3 grid((unsigned)(g.ctiles * ((g.strips + warps - 1) / warps)), (unsigned)p.batch);
-  kernel<<<grid, dim3(32, warps), smem, s>>>(p, m);
-  return cudaGetLastError();
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3((unsigned)(g.ctiles * ((g.strips + warps - 1) / warps)), (unsigned)p.batch);
+  c.blockDim = dim3(32, warps);
+  c.dynamicSmemBytes = smem;
+  c.stream = s;
+  c.attrs = &at;
+  c.numAttrs = after ? 1 : 0;
+  return cudaLaunchKernelEx(&c, kernel, p, m);
 }
 
 template <class T, int V, int L, bool kMask, bool kBulk>
 cudaError_t launch_vl(const Args& p, const Maps& m, const Geometry& g, bool backward, cudaStream_t s) {
   cudaError_t e = cudaSuccess;
+  const bool cut = g.strips > 1;
   if (!backward) {
     const size_t smem = kBulk ? Ring<T, V, L, 3, false>::kBytes : 0;
-    if (g.strips > 1) e = start(forward_maps_kernel<T, V, L, kMask, kBulk>, p, m, g, smem, s);
-    return e != cudaSuccess ? e : start(forward_kernel<T, V, L, kMask, kBulk>, p, m, g, smem, s);
+    if (cut) e = start(forward_maps_kernel<T, V, L, kMask, kBulk>, p, m, g, smem, false, s);
+    return e != cudaSuccess ? e : start(forward_kernel<T, V, L, kMask, kBulk>, p, m, g, smem, cut, s);
   }
-  if (g.strips > 1)
-    e = start(backward_maps_kernel<T, V, L, kMask, kBulk>, p, m, g, kBulk ? Ring<T, V, L, 2, false>::kBytes : 0, s);
+  if (cut)
+    e = start(backward_maps_kernel<T, V, L, kMask, kBulk>, p, m, g, kBulk ? Ring<T, V, L, 2, false>::kBytes : 0, false, s);
   return e != cudaSuccess
              ? e
-             : start(backward_kernel<T, V, L, kMask, kBulk>, p, m, g, kBulk ? Ring<T, V, L, 4, true>::kBytes : 0, s);
+             : start(backward_kernel<T, V, L, kMask, kBulk>, p, m, g, kBulk ? Ring<T, V, L, 4, true>::kBytes : 0, cut, s);
 }
 
 template <class T, int V>

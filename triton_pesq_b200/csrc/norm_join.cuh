@@ -330,6 +330,7 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(true, 
   using S = Eight<TS, TEAM, kWide>;
   using B = Eight<TB, TEAM, kWide>;
   using F = Eight<float, TEAM, kWide>;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ float s_sum[2][32][8];
   __shared__ __align__(16) float s_part[TEAMS > 1 ? THREADS * kEach : 4];
   int turn = 0;

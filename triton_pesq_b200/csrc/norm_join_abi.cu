@@ -33,13 +33,14 @@ struct SumArgs {
   int64_t rows, per_item;
   int width, dtype;
 };
-constexpr int kSumRows = 16;
+constexpr int kSumRows = 32;
 __global__ void __launch_bounds__(32 * kSumRows) vectors_kernel(const __grid_constant__ SumArgs p) {
   __shared__ float s[kSumRows][33];
   const int c = blockIdx.x * 32 + threadIdx.x, which = blockIdx.y;
   const float* part = which == 0 ? p.pre : which == 1 ? p.u : p.gate + (which - 2) * p.per_item * p.width;
   const int64_t rows = which < 2 ? p.rows : p.per_item;
   if (!part) return;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // for the kernel before, which this one is launched close to
   float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   if (c < p.width) {
     int64_t r = threadIdx.y;
@@ -234,8 +235,16 @@ int pesq_norm_join_backward(const pesq_norm_join_desc* d, void* stream, pesq_str
     t.width = (int)d->width;
     t.dtype = d->dtype;
     const dim3 grid((unsigned)((d->width + 31) / 32), (unsigned)(2 + (a.part_gate ? q.batch : 0)));
-    vectors_kernel<<<grid, dim3(32, kSumRows), 0, s>>>(t);
-    e = cudaGetLastError();
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t c{};
+    c.gridDim = grid;
+    c.blockDim = dim3(32, kSumRows);
+    c.stream = s;
+    c.attrs = &at;
+    c.numAttrs = 1;
+    e = cudaLaunchKernelEx(&c, vectors_kernel, t);
   }
   return e == cudaSuccess ? PESQ_OK : set_error(PESQ_ERR_CUDA, cudaGetErrorString(e));
 }
