@@ -54,6 +54,7 @@ using namespace train;
 // stream either way, in registers no more than 8 steps
 constexpr int chunk_steps(int vec, bool bulk) { return bulk ? 16 / vec : 8; }
 constexpr int kStrips = 8;  // strips (warps) of a CTA at most, where rows are cut
+constexpr int kRowWarps = 16, kHeld = 32;  // a row of up to 512 steps in one CTA
 // chunks of a warp in shared memory: what 8 warps' chunks of four 32-bit streams leave room for
 template <class T>
 constexpr int kRing = sizeof(T) == 2 ? 3 : 2;
@@ -716,7 +717,7 @@ template <class T, int V, int L, bool kBulk>
 __device__ __forceinline__ auto forward_ring(const Args& p, const Maps& m, const Lane& o) {
   if constexpr (kBulk) {
     extern __shared__ __align__(128) char dynamic[];
-    __shared__ uint64_t s_bar[kStrips * kRing<T>];
+    __shared__ uint64_t s_bar[kRowWarps * kRing<T>];
     Ring<T, V, L, 3, false> ring(dynamic, s_bar);
     ring.map[0] = &m.rg, ring.map[1] = &m.ig, ring.map[2] = &m.x;
     ring.start(p, o, o.first, o.count, 1);
@@ -798,6 +799,85 @@ __global__ void __launch_bounds__(32 * kStrips) forward_kernel(const __grid_cons
     forward_strip<T, V, L, kMask, true>(p, o, ring, rate);
   else
     forward_strip<T, V, L, kMask, false>(p, o, ring, rate);
+}
+
+// A short row in one CTA: a warp holds its strip of kHeld steps as (a, b) in registers,
+// the strips' maps meet in shared memory, and the recursion is run from the state that
+// they give.  The data pass once, in one launch.
+template <class T, int L, bool kMask, bool kFar, class R>
+__device__ __forceinline__ void forward_row(const Args& p, const Lane& o, R& ring, const Vec<1> (&rate)[1]) {
+  constexpr int NC = kHeld / L;
+  __shared__ float2 s_map[kRowWarps][32];
+  Vec<1> a[NC][L], b[NC][L], A{{1.0f}}, H{{0.0f}};
+  unsigned live[NC];
+  using In = Loaded<T, 1, L>;
+  In in[2];
+  if constexpr (std::is_same<R, NoRing>::value) {
+    if (o.count > 0) in[0].template read<kMask, false>(p, o, o.first);
+  }
+  bool ok = true;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    live[c] = 0u;
+#pragma unroll
+    for (int l = 0; l < L; ++l) a[c][l] = splat<1>(1.0f), b[c][l] = splat<1>(0.0f);
+    if (c >= o.count) continue;
+    In& now = in[c % 2];
+    if constexpr (std::is_same<R, NoRing>::value) {
+      if (c + 1 < NC && c + 1 < o.count) in[(c + 1) % 2].template read<kMask, false>(p, o, o.first + c + 1);
+    } else {
+      now.q = chunk_of<L, kMask>(p, o, o.first + c);
+      flag_chunk<L, kMask>(p, o, now.q);
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(ring.bar + c, 0));
+      now.get(p, ring, c);
+    }
+    if (now.q.live != (1u << L) - 1) blank(now.rg, now.q, kShut), blank(now.ig, now.q), blank(now.x, now.q);
+    live[c] = now.q.live;
+    each_gate<T, 1, L, kMask, kFar>(
+        cuts<kMask>(p, now.q), now.ig, now.rg, rate, [&](int l, int, const Gates<1>& g, Vec<1> beta) {
+          a[c][l] = g.a;
+          b[c][l] = beta * (g.i * widen<1>(now.x[l], 0));
+          H = apply<kMask>(g.a, H, b[c][l]);
+          A = A * g.a;
+        });
+  }
+  if (!ok && threadIdx.x == 0) atomicOr(p.error, 1u);
+  s_map[threadIdx.y][threadIdx.x] = make_float2(A.v[0], H.v[0]);
+  __syncthreads();
+  Vec<1> h{{p.state ? p.state[o.b * p.width + o.from] : 0.0f}};
+  for (int w = 0; w < (int)threadIdx.y; ++w) {
+    const float2 m = s_map[w][threadIdx.x];
+    h = apply<kMask>(Vec<1>{{m.x}}, h, Vec<1>{{m.y}});
+  }
+  if (!o.on) return;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    if (c >= o.count) continue;
+    const Chunk q = chunk_of<L, kMask>(p, o, o.first + c);
+    if (p.kept) p.kept[(o.b * ((p.steps + L - 1) / L) + o.first + c) * p.width + o.c] = h.v[0];
+    char* y = reinterpret_cast<char*>(static_cast<T*>(p.y) + (o.b * p.steps + q.t0) * p.width + o.c);
+    const int step = o.dir * (int)p.width * (int)sizeof(T);
+#pragma unroll
+    for (int l = 0; l < L; ++l) {
+      h = apply<kMask>(a[c][l], h, b[c][l]);
+      const Vec<1> out[1] = {!kMask || ((live[c] >> l) & 1u) ? h : splat<1>(0.0f)};
+      if ((q.inside >> l) & 1u) store<T, 1, 1>(y + (int64_t)step * l, out);
+    }
+  }
+  if (kMask) zero_rest<T, 1, L>(p, o, p.y);
+  if (o.rank == p.strips - 1) p.last[o.b * p.width + o.c] = h.v[0];
+}
+
+template <class T, int L, bool kMask, bool kBulk>
+__global__ void __launch_bounds__(32 * kRowWarps) forward_row_kernel(const __grid_constant__ Args p,
+                                                                     const __grid_constant__ Maps m) {
+  const Lane o = lane_of<1, L, kMask, false>(p);
+  auto ring = forward_ring<T, 1, L, kBulk>(p, m, o);
+  Vec<1> rate[1];
+  if (rates<1, 1>(p, o, rate))
+    forward_row<T, L, kMask, true>(p, o, ring, rate);
+  else
+    forward_row<T, L, kMask, false>(p, o, ring, rate);
 }
 
 // ------------------------------------------------------------------ backward
@@ -1056,6 +1136,7 @@ __global__ void __launch_bounds__(32 * kStrips) backward_kernel(const __grid_con
 struct Geometry {
   int vec, chunk, ctiles, strips, strip, warps;
   bool bulk;
+  bool row;  // the strips of a row are one CTA's, and are held by it (forward)
 };
 
 template <class T>

@@ -130,10 +130,12 @@ Geometry geometry(const pesq_gated_scan_desc& d, bool backward) {
     strips = std::max<int64_t>(1, 148 * sm.ctas / warps) * sm.warps;
     strips = std::max<int64_t>(1, std::min(strips, (d.steps + kFewestSteps - 1) / kFewestSteps));
   }
-  const int64_t per = (chunks + strips - 1) / strips;
+  g.row = !backward && g.vec == 1 && warps < kWarpsEnough && d.steps > kHeld && d.steps <= kHeld * kRowWarps;
+  if (g.row) strips = (d.steps + kHeld - 1) / kHeld;
+  const int64_t per = g.row ? kHeld / g.chunk : (chunks + strips - 1) / strips;
   g.strips = (int)((chunks + per - 1) / per);
   g.strip = (int)(per * g.chunk);
-  g.warps = std::min(g.strips, sm.warps);
+  g.warps = g.row ? g.strips : std::min(g.strips, sm.warps);
   return g;
 }
 
@@ -155,7 +157,7 @@ bool encode(CUtensorMap& m, const pesq_stream& s, const pesq_gated_scan_desc& d,
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 // maps of strips and of CTAs of strips
 size_t map_bytes(const pesq_gated_scan_desc& d, const Geometry& g) {
-  return g.strips == 1 ? 0 : round16((size_t)(d.batch * (g.strips + (g.strips + g.warps - 1) / g.warps) * d.width) * 8);
+  return g.strips == 1 || g.row ? 0 : round16((size_t)(d.batch * (g.strips + (g.strips + g.warps - 1) / g.warps) * d.width) * 8);
 }
 size_t kept_bytes(const pesq_gated_scan_desc& d, const Geometry& g) {
   return round16((size_t)(d.batch * ((d.steps + g.chunk - 1) / g.chunk) * d.width) * 4);
@@ -198,7 +200,7 @@ int prepare(const pesq_gated_scan_desc& d, const Geometry& g, char* maps, Args& 
   a.ctiles = g.ctiles;
   a.strips = g.strips;
   a.strip = g.strip;
-  if (g.strips > 1) {
+  if (g.strips > 1 && !g.row) {
     a.before = reinterpret_cast<float2*>(maps);
     a.total = a.before + d.batch * g.strips * d.width;
   }

@@ -36,6 +36,9 @@ cudaError_t launch_vl(const Args& p, const Maps& m, const Geometry& g, bool back
   const bool cut = g.strips > 1;
   if (!backward) {
     const size_t smem = kBulk ? Ring<T, V, L, 3, false>::kBytes : 0;
+    if constexpr (V == 1 && L > 1) {
+      if (g.row) return start(forward_row_kernel<T, L, kMask, kBulk>, p, m, g, smem, false, s);
+    }
     if (cut) e = start(forward_maps_kernel<T, V, L, kMask, kBulk>, p, m, g, smem, false, s);
     return e != cudaSuccess ? e : start(forward_kernel<T, V, L, kMask, kBulk>, p, m, g, smem, cut, s);
   }
