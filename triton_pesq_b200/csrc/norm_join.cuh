@@ -62,6 +62,11 @@ struct Args {
   float *part_u, *part_pre, *part_gate;  // [batch * units, width]; part_gate null where the gate is not shared
 };
 
+// Backward rows of so many threads leave a thread too few registers to hold the vectors,
+// the sums and the next row: those come from cache, go to shared memory, and wait
+template <int TEAM>
+constexpr bool kLeanRow = TEAM >= 512;
+
 // Sums of K values over a team: by shuffles within a warp, through shared
 // memory across warps (two buffers in turn, so that one barrier a round is enough).
 template <int K, int TEAM>
@@ -70,7 +75,7 @@ __device__ __forceinline__ void team_sum(float (&v)[K], float (*s_sum)[32][8], i
   for (int off = (TEAM < 32 ? TEAM : 32) / 2; off > 0; off >>= 1)
 #pragma unroll
     for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], off);
-  if (TEAM > 32) {
+  if constexpr (TEAM > 32) {
     constexpr int W = TEAM / 32;
     const int warp = threadIdx.x >> 5, first = warp / W * W;
     float(*s)[8] = s_sum[turn];
@@ -87,6 +92,45 @@ __device__ __forceinline__ void team_sum(float (&v)[K], float (*s_sum)[32][8], i
       for (int w = 0; w < W; ++w) t += s[first + w][k];
       v[k] = t;
     }
+  }
+}
+
+// The same of five values.  Across a team of several warps the first four are added
+// up by halves: half the lanes go on with two of them, a quarter with one, so that it takes 11
+// shuffles instead of 25.
+template <int TEAM>
+__device__ __forceinline__ void team_sum5(float (&v)[5], float (*s_sum)[32][8], int& turn) {
+  if constexpr (TEAM <= 32) {
+    team_sum<5, TEAM>(v, s_sum, turn);
+  } else {
+    constexpr unsigned kAll = 0xffffffffu;
+    constexpr int W = TEAM / 32;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, first = warp / W * W;
+    const bool high = lane & 16, odd = lane & 8;
+    float k0 = high ? v[2] : v[0], k1 = high ? v[3] : v[1];
+    k0 += __shfl_xor_sync(kAll, high ? v[0] : v[2], 16);
+    k1 += __shfl_xor_sync(kAll, high ? v[1] : v[3], 16);
+    float k = odd ? k1 : k0;
+    k += __shfl_xor_sync(kAll, odd ? k0 : k1, 8);
+#pragma unroll
+    for (int off = 4; off > 0; off >>= 1) k += __shfl_xor_sync(kAll, k, off);
+    float last = v[4];
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) last += __shfl_xor_sync(kAll, last, off);
+    float(*s)[8] = s_sum[turn];
+    turn ^= 1;
+    if ((lane & 7) == 0) s[warp][lane >> 3] = k;
+    if (lane == 0) s[warp][4] = last;
+    __syncthreads();
+    float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float t4 = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float4 q = *reinterpret_cast<const float4*>(s[first + w]);
+      t.x += q.x, t.y += q.y, t.z += q.z, t.w += q.w;
+      t4 += s[first + w][4];
+    }
+    v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w, v[4] = t4;
   }
 }
 
@@ -230,7 +274,7 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(false,
   using S = Eight<TS, TEAM, kWide>;
   using B = Eight<TB, TEAM, kWide>;
   using F = Eight<float, TEAM, kWide>;
-  __shared__ float s_sum[2][32][8];
+  __shared__ __align__(16) float s_sum[2][32][8];
   int turn = 0;
   F post, pre, scale;
   pre.load(p.pre, 0, p.width, true);
@@ -327,26 +371,37 @@ __device__ __forceinline__ void store_part(const Vec<2> (&v)[kEach / 2], float* 
 template <class TS, class TB, int TEAM, bool kWide>
 __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(true, kWide, TEAM)) backward_kernel(const __grid_constant__ Args p) {
   constexpr int THREADS = TEAM > kThreads ? TEAM : kThreads, TEAMS = THREADS / TEAM;
+  constexpr bool kLean = kLeanRow<TEAM>;
   using S = Eight<TS, TEAM, kWide>;
   using B = Eight<TB, TEAM, kWide>;
   using F = Eight<float, TEAM, kWide>;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  __shared__ float s_sum[2][32][8];
+  __shared__ __align__(16) float s_sum[2][32][8];
   __shared__ __align__(16) float s_part[TEAMS > 1 ? THREADS * kEach : 4];
   int turn = 0;
   F post, pre;  // post times scale
-  pre.load(p.pre, 0, p.width, true);
-  post.load(p.post, 0, p.width, p.post != nullptr);
-  if (p.scale) {
-    F scale;
-    scale.load(p.scale, 0, p.width, true);
+  const auto vectors = [&] {
+    pre.load(p.pre, 0, p.width, true);
+    post.load(p.post, 0, p.width, p.post != nullptr);
+    if (p.scale) {
+      F scale;
+      scale.load(p.scale, 0, p.width, true);
 #pragma unroll
-    for (int j = 0; j < kEach; j += 2) post.set(j, post.at(j) * scale.at(j), post.at(j + 1) * scale.at(j + 1));
-  }
+      for (int j = 0; j < kEach; j += 2) post.set(j, post.at(j) * scale.at(j), post.at(j + 1) * scale.at(j + 1));
+    }
+  };
+  if (!kLean) vectors();
   constexpr int H = kEach / 2;
   Vec<2> acc_u[H], acc_pre[H], acc_gate[H];
 #pragma unroll
   for (int i = 0; i < H; ++i) acc_u[i] = acc_pre[i] = acc_gate[i] = splat<2>(0.0f);
+  // (rows of 512 and more threads: sums in shared memory, [3][i][thread])
+  extern __shared__ __align__(16) char dynamic[];
+  Vec<2>* own = reinterpret_cast<Vec<2>*>(dynamic) + threadIdx.x;
+  if (kLean) {
+#pragma unroll
+    for (int i = 0; i < 3 * H; ++i) own[i * THREADS] = splat<2>(0.0f);
+  }
   const int turns = (p.span + TEAMS - 1) / TEAMS;
   const float inv = 1.0f / (float)p.width;
   S x, ds;
@@ -359,13 +414,18 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(true, 
     ds.load(p.dstream.p, at.of(p.dstream), p.width, at.on && p.dstream.p);
   };
   Turn<TEAM, THREADS> now(p, 0);
-  load(now, x, ds, z, g, dy);
+  if (!kLean) load(now, x, ds, z, g, dy);
 #pragma unroll 1
   for (int k = 0; k < turns; ++k) {
     const Turn<TEAM, THREADS> next(p, k + 1);
     S x1, ds1;
     B z1, g1, dy1;
-    load(next, x1, ds1, z1, g1, dy1);
+    if (kLean) {
+      load(now, x, ds, z, g, dy);
+      vectors();
+    } else {
+      load(next, x1, ds1, z1, g1, dy1);
+    }
 
     float rz = 0.0f;
     if (p.block.p) {
@@ -399,7 +459,7 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(true, 
     float sum[5];
 #pragma unroll
     for (int k5 = 0; k5 < 5; ++k5) sum[k5] = part[k5].v[0] + part[k5].v[1];
-    team_sum<5, TEAM>(sum, s_sum, turn);
+    team_sum5<TEAM>(sum, s_sum, turn);
     // (a row that is off is zeros, and adds zeros for any eps)
     const float rr = now.on ? rsqrt_approx(fmaf(sum[0], inv, p.eps)) : 0.0f;
     const float mq = sum[1] * inv * rr * rr;                        // mean(q h) / rms
@@ -413,9 +473,15 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(true, 
       const Vec<2> u = dx[i] * zh;
       dg[i] = u * (ps * slope[i]);
       dz[i] = splat<2>(rz) * fma(dx[i], ps * value[i], zh * splat<2>(-mw));
-      acc_u[i] = fma(u, value[i], acc_u[i]);
-      acc_pre[i] = fma(dy.two(2 * i), r * splat<2>(rr), acc_pre[i]);
-      acc_gate[i] = acc_gate[i] + dg[i];
+      if (kLean) {
+        own[i * THREADS] = fma(u, value[i], own[i * THREADS]);
+        own[(H + i) * THREADS] = fma(dy.two(2 * i), r * splat<2>(rr), own[(H + i) * THREADS]);
+        if (p.part_gate) own[(2 * H + i) * THREADS] = own[(2 * H + i) * THREADS] + dg[i];
+      } else {
+        acc_u[i] = fma(u, value[i], acc_u[i]);
+        acc_pre[i] = fma(dy.two(2 * i), r * splat<2>(rr), acc_pre[i]);
+        acc_gate[i] = acc_gate[i] + dg[i];
+      }
     }
     if (now.on) {
       const int64_t at = now.dense(p);
@@ -435,7 +501,13 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(true, 
         b.store(p.dgate, at, p.width);
       }
     }
-    x = x1, ds = ds1, z = z1, g = g1, dy = dy1, now = next;
+    if (!kLean) x = x1, ds = ds1, z = z1, g = g1, dy = dy1;
+    now = next;
+  }
+  if (kLean) {
+#pragma unroll
+    for (int i = 0; i < H; ++i)
+      acc_u[i] = own[i * THREADS], acc_pre[i] = own[(H + i) * THREADS], acc_gate[i] = own[(2 * H + i) * THREADS];
   }
   if (p.part_u) store_part<TEAM, TEAMS, kWide>(acc_u, p.part_u, p.width, s_part);
   store_part<TEAM, TEAMS, kWide>(acc_pre, p.part_pre, p.width, s_part);

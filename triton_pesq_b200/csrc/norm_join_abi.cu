@@ -119,7 +119,7 @@ Plan plan(const pesq_norm_join_desc& d, bool backward, const pesq_stream* dstrea
   q.batch = flat ? 1 : d.batch;
   q.steps = flat ? d.batch * d.steps : d.steps;
   q.g.team = 4;
-  for (int t : {16, 32, 64, 128, 256, 512, 1024})
+  for (int t : {8, 16, 32, 64, 128, 256, 512, 1024})
     if (q.g.team * kEach < d.width) q.g.team = t;
   q.g.wide = d.width % kEach == 0 && wide(d.stream, d, d.stream_dtype) && wide(d.block, d, d.dtype) &&
              wide(d.gate, d, d.dtype) && wide(ds, d, d.stream_dtype) && wide(dn, d, d.dtype) && wide(d.post) &&
