@@ -260,8 +260,8 @@ __device__ __forceinline__ void hold(Pack<__half, V>& p) {
 struct Lane {
   int64_t b, c;      // row, first channel
   int rank;          // of the strip, in the order of this scan
-  int all_first, all_count;  // the strip's chunks
-  int first, count;  // those with a step before the row's length
+  int lo, hi;        // the row's chunks that have a step before its length: the strips share these
+  int first, count;  // the strip's
   int whole;         // those of them that have all their steps
   int dir;           // memory direction of the steps' scan
   int len;           // the row's length
@@ -279,18 +279,19 @@ __device__ __forceinline__ Lane lane_of(const Args& p) {
   o.from = o.on ? o.c : 0;
   o.rank = block * blockDim.y + threadIdx.y;
   const int strip = kBack ? p.strips - 1 - o.rank : o.rank, steps = (int)p.steps;
-  const int all = (steps + L - 1) / L, per = p.strip / L;
-  o.all_first = strip * per;
-  o.all_count = strip < 0 || strip >= p.strips ? 0 : min(per, all - o.all_first);
-  o.first = o.all_first, o.count = o.all_count;
+  const int all = (steps + L - 1) / L;
+  int per = p.strip / L;
+  o.lo = 0, o.hi = all;
   o.len = steps;
   o.dir = p.reverse ? -1 : 1;
   if (kMask && p.lengths) {
     o.len = (int)max(INT64_C(0), min(p.lengths[o.b], p.steps));
-    const int lo = p.reverse ? (steps - o.len) / L : 0, hi = o.len == 0 ? lo : p.reverse ? all : (o.len + L - 1) / L;
-    o.first = max(o.all_first, lo);
-    o.count = max(0, min(o.all_first + o.all_count, hi) - o.first);
+    o.lo = p.reverse ? (steps - o.len) / L : 0;
+    o.hi = o.len == 0 ? o.lo : p.reverse ? all : (o.len + L - 1) / L;
+    per = (o.hi - o.lo + p.strips - 1) / p.strips;
   }
+  o.first = o.lo + strip * per;
+  o.count = strip < 0 || strip >= p.strips ? 0 : max(0, min(per, o.hi - o.first));
   o.whole = min(o.count, max(0, steps / L - o.first));
   return o;
 }
@@ -524,19 +525,25 @@ __device__ __forceinline__ void blank(Pack<T, V> (&out)[L], const Chunk& q, floa
       if (!((q.live >> l) & 1u)) out[l].v[v] = narrow<T>(other);
 }
 
-// Zeros for a strip's chunks that the row's length leaves out
-template <class T, int V, int L>
-__device__ __forceinline__ void zero_rest(const Args& p, const Lane& o, void* out) {
-  if (o.count == o.all_count || !o.on) return;
+// Zeros for the steps of the chunks that the row's length leaves out, the warps of
+// the row sharing them
+template <class T, int V, int L, int K>
+__device__ __forceinline__ void zero_rest(const Args& p, const Lane& o, void* const (&out)[K]) {
+  const int all = ((int)p.steps + L - 1) / L, dead = all - (o.hi - o.lo);
+  if (dead == 0 || !o.on || o.rank >= p.strips) return;
   Pack<T, V> z;
 #pragma unroll
   for (int v = 0; v < V; ++v) z.v[v] = narrow<T>(0.0f);
-  const int end = min((o.all_first + o.all_count) * L, (int)p.steps);
-  for (int s = o.all_first * L; s < end; ++s) {
-    if (o.count && s == o.first * L) s += o.count * L;
-    if (s >= end) break;
-    const int64_t t = p.reverse ? p.steps - 1 - s : s;
-    *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(out) + (o.b * p.steps + t) * p.width + o.c) = z;
+  // (they lie at one end of the row)
+  const int base = o.lo > 0 ? 0 : o.hi, per = (dead + p.strips - 1) / p.strips;
+  const int s0 = (base + o.rank * per) * L, s1 = min((int)p.steps, min(base + dead, base + (o.rank + 1) * per) * L);
+  const int64_t t = p.reverse ? p.steps - 1 - s0 : s0, step = o.dir * p.width;
+  const int64_t at = (o.b * p.steps + t) * p.width + o.c;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    T* to = static_cast<T*>(out[k]) + at;
+#pragma unroll 4
+    for (int s = s0; s < s1; ++s, to += step) *reinterpret_cast<Pack<T, V>*>(to) = z;
   }
 }
 
@@ -775,13 +782,13 @@ __device__ __forceinline__ void forward_strip(const Args& p, const Lane& o, R& r
   for (int j = 0; j < P; ++j) h[j] = splat<N>(0.0f);
   if (p.state) read_row<V, N>(p.state + o.b * p.width + o.from, h);
   if (p.strips > 1) wait_for_last();
-  if (o.all_count == 0) return;
+  if (o.rank >= p.strips) return;
   start_of<V, N, kMask>(p, o, h);
   if (!forward_walk<T, V, L, kMask>(p, o, ring, [&](int k, Loaded<T, V, L>& in, auto full) {
         forward_chunk<T, V, L, kMask, kFar, decltype(full)::value>(p, o, k, in, rate, h);
       }))
     return;
-  if (kMask) zero_rest<T, V, L>(p, o, p.y);
+  if (kMask) zero_rest<T, V, L, 1>(p, o, {p.y});
   if (o.rank == p.strips - 1 && o.on) {
 #pragma unroll
     for (int v = 0; v < V; ++v) p.last[o.b * p.width + o.c + v] = h[v / N].v[v % N];
@@ -864,7 +871,7 @@ __device__ __forceinline__ void forward_row(const Args& p, const Lane& o, R& rin
       if ((q.inside >> l) & 1u) store<T, 1, 1>(y + (int64_t)step * l, out);
     }
   }
-  if (kMask) zero_rest<T, 1, L>(p, o, p.y);
+  if (kMask) zero_rest<T, 1, L, 1>(p, o, {p.y});
   if (o.rank == p.strips - 1) p.last[o.b * p.width + o.c] = h.v[0];
 }
 
@@ -1099,18 +1106,14 @@ __device__ __forceinline__ void backward_strip(const Args& p, const Lane& o, R& 
   for (int j = 0; j < P; ++j) e[j] = acc[j] = splat<N>(0.0f);
   if (p.dlast) read_row<V, N>(p.dlast + o.b * p.width + o.from, e);
   if (p.strips > 1) wait_for_last();
-  if (o.all_count == 0) return;
+  if (o.rank >= p.strips) return;
   start_of<V, N, kMask>(p, o, e);
   using In = LoadedBack<T, V, L>;
   if (!backward_walk<T, V, L, kMask, In>(p, o, ring, [&](In& in, auto full) {
         backward_chunk<T, V, L, kMask, kFar, decltype(full)::value>(p, o, in, rate, e, acc);
       }))
     return;
-  if (kMask) {
-    zero_rest<T, V, L>(p, o, p.dx);
-    zero_rest<T, V, L>(p, o, p.dig);
-    zero_rest<T, V, L>(p, o, p.drg);
-  }
+  if (kMask) zero_rest<T, V, L, 3>(p, o, {p.dx, p.dig, p.drg});
   if (!o.on) return;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
