@@ -54,6 +54,16 @@ using namespace train;
 // stream either way, in registers no more than 8 steps
 constexpr int chunk_steps(int vec, bool bulk) { return bulk ? 16 / vec : 8; }
 constexpr int kStrips = 8;  // strips (warps) of a CTA at most, where rows are cut
+// CTAs of so many strips (4 or 8) that an SM holds by registers and shared memory, of elements of `size` bytes
+constexpr int forward_ctas(int strips, bool bulk, int size) {
+  return bulk && size == 2 ? (strips == 8 ? 3 : 5) : 16 / strips;
+}
+// (backward: 8 strips of 128 registers in the one case, where spills of 36 bytes cost less than the
+// warps that they make room for; 4 of 168 in the others)
+constexpr int backward_strips(bool bulk, bool mask, int size) { return bulk && !mask && size == 2 ? 8 : 4; }
+constexpr int backward_ctas(int strips, bool bulk, bool mask, int size) {
+  return (backward_strips(bulk, mask, size) == 8 ? 16 : 12) / strips;
+}
 constexpr int kRowWarps = 16, kHeld = 32;  // a row of up to 512 steps in one CTA
 // chunks of a warp in shared memory: what 8 warps' chunks of four 32-bit streams leave room for
 template <class T>
@@ -93,9 +103,10 @@ struct Args {
   uint32_t* error;            // set when a copy does not come
 };
 
-// Tensor maps of the streams: [batch][step][channel], boxes of a chunk
+// Tensor maps of the streams: [batch][step][channel], boxes of a chunk.  `out` by the input whose box in
+// shared memory it leaves from: ddecay_gate, dinput_gate, and y or dx.
 struct Maps {
-  CUtensorMap rg, ig, x, dy;
+  CUtensorMap rg, ig, x, dy, out[3];
 };
 
 // softplus(v): log1p(e) = 2 artanh(e / (2 + e)) by its series, e = exp(-|v|)
@@ -114,33 +125,34 @@ __device__ __forceinline__ float softplus(float v) {
   return max_nan(v, 0.0f) + 2.0f * s * p;
 }
 
-// logits are held at kShut so that the product below stays finite
-// (sigmoid(-43) = 2e-19)
-constexpr float kShut = -43.0f;
+// The decay gate that steps past the length and outside the row read as
+constexpr float kShut = -INFINITY;
 // 1 - a^2 is held above this where its root is divided by
 constexpr float kTiny = 1e-36f;
+// rate softplus(decay) is held at this, so that times a shut gate it is zero
+constexpr float kFast = 1e30f;
 // rates -log a up to here go by the series alone
 constexpr float kNear = 0.25f;
 
-template <int N>
+template <int N, int G>
 struct Gates {
-  Vec<N> i, r, a;
+  Vec<N> i[G], r[G], a[G], beta[G];
+  Vec<N> s[G];  // 1 / beta, or 1 / sqrt(kTiny) where beta is zero
 };
 
 // The gates of G Vecs side by side: operation by operation rather than Vec by
 // Vec, so that every instruction has G independent ones next to it.
 //
-// k = rate softplus(decay) >= 0.  The two sigmoids share one reciprocal.
-// With m = -log a = k r, 1 - a = m (1 - m/2 + m^2/6 - ...) by its Taylor
-// series (m^6 / 5040 < 5e-8 at 1/4): a is then rounded once, without the bias
+// k = rate softplus(decay) >= 0.  With m = -log a = k r, 1 - a = m (1 - m/2 + m^2/6 - ...)
+// by its Taylor series (m^6 / 5040 < 5e-8 at 1/4): a is then rounded once, without the bias
 // that a long memory would sum up, and 1 - a^2 = (1 - a)(2 - (1 - a)) does not
 // cancel.  kFar: m may be above kNear, where the exponential takes over.
 template <bool kFar, int N, int G>
-__device__ __forceinline__ void decays(const Vec<N> (&r)[G], const Vec<N> (&k)[G], Vec<N> (&a)[G], Vec<N> (&w)[G]) {
+__device__ __forceinline__ void decays(const Vec<N> (&r)[G], Vec<N> k, Vec<N> (&a)[G], Vec<N> (&w)[G]) {
   Vec<N> m[G], p[G];
   constexpr float kSeries[5] = {1.0f / 120, -1.0f / 24, 1.0f / 6, -0.5f, 1.0f};
 #pragma unroll
-  for (int g = 0; g < G; ++g) m[g] = k[g] * r[g];
+  for (int g = 0; g < G; ++g) m[g] = k * r[g];
 #pragma unroll
   for (int g = 0; g < G; ++g) p[g] = splat<N>(-1.0f / 720);
 #pragma unroll
@@ -167,58 +179,38 @@ __device__ __forceinline__ void decays(const Vec<N> (&r)[G], const Vec<N> (&k)[G
   }
 }
 
-template <bool kFar, int N, int G>
-__device__ __forceinline__ void gates(const Vec<N> (&ig)[G], const Vec<N> (&rg)[G], const Vec<N> (&k)[G],
-                                      Gates<N> (&out)[G], Vec<N> (&beta)[G]) {
-  Vec<N> di[G], dr[G], q[G], r[G], a[G], w[G];
+// 1 / (1 + exp(-v)); a reciprocal for each: one for the product of two would need
+// both exponentials to be held below overflow, which costs more
+template <int N, int G>
+__device__ __forceinline__ void sigmoids(const Vec<N> (&v)[G], Vec<N> (&out)[G]) {
 #pragma unroll
-  for (int g = 0; g < G; ++g) di[g] = ig[g] * splat<N>(-kLog2e), dr[g] = rg[g] * splat<N>(-kLog2e);
-#pragma unroll
-  for (int g = 0; g < G; ++g)
-#pragma unroll
-    for (int j = 0; j < N; ++j) di[g].v[j] = exp2_approx(di[g].v[j]), dr[g].v[j] = exp2_approx(dr[g].v[j]);
-#pragma unroll
-  for (int g = 0; g < G; ++g) di[g] = di[g] + splat<N>(1.0f), dr[g] = dr[g] + splat<N>(1.0f);
-#pragma unroll
-  for (int g = 0; g < G; ++g) q[g] = di[g] * dr[g];
+  for (int g = 0; g < G; ++g) out[g] = v[g] * splat<N>(-kLog2e);
 #pragma unroll
   for (int g = 0; g < G; ++g)
 #pragma unroll
-    for (int j = 0; j < N; ++j) q[g].v[j] = rcp_approx(q[g].v[j]);
+    for (int j = 0; j < N; ++j) out[g].v[j] = exp2_approx(out[g].v[j]);
 #pragma unroll
-  for (int g = 0; g < G; ++g) r[g] = q[g] * di[g];
-#pragma unroll
-  for (int g = 0; g < G; ++g) di[g] = q[g] * dr[g];
-  decays<kFar>(r, k, a, w);
-  Vec<N> s[G];
+  for (int g = 0; g < G; ++g) out[g] = out[g] + splat<N>(1.0f);
 #pragma unroll
   for (int g = 0; g < G; ++g)
 #pragma unroll
-    for (int j = 0; j < N; ++j) s[g].v[j] = rsqrt_approx(fmaxf(w[g].v[j], kTiny));
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    beta[g] = w[g] * s[g];
-    out[g].i = di[g], out[g].r = r[g], out[g].a = a[g];
-  }
+    for (int j = 0; j < N; ++j) out[g].v[j] = rcp_approx(out[g].v[j]);
 }
 
-// The decays alone
 template <bool kFar, int N, int G>
-__device__ __forceinline__ void decays_of(const Vec<N> (&rg)[G], const Vec<N> (&k)[G], Vec<N> (&a)[G]) {
-  Vec<N> r[G], w[G];
+__device__ __forceinline__ void gates(const Vec<N> (&ig)[G], const Vec<N> (&rg)[G], Vec<N> k, Gates<N, G>& o) {
+  Vec<N> w[G];
+  sigmoids(rg, o.r);
+  sigmoids(ig, o.i);
+  decays<kFar>(o.r, k, o.a, w);
 #pragma unroll
-  for (int g = 0; g < G; ++g) r[g] = rg[g] * splat<N>(-kLog2e);
-#pragma unroll
-  for (int g = 0; g < G; ++g)
-#pragma unroll
-    for (int j = 0; j < N; ++j) r[g].v[j] = exp2_approx(r[g].v[j]);
-#pragma unroll
-  for (int g = 0; g < G; ++g) r[g] = r[g] + splat<N>(1.0f);
+  for (int g = 0; g < G; ++g) o.s[g] = w[g] + splat<N>(kTiny);
 #pragma unroll
   for (int g = 0; g < G; ++g)
 #pragma unroll
-    for (int j = 0; j < N; ++j) r[g].v[j] = rcp_approx(r[g].v[j]);
-  decays<kFar>(r, k, a, w);
+    for (int j = 0; j < N; ++j) o.s[g].v[j] = rsqrt_approx(o.s[g].v[j]);
+#pragma unroll
+  for (int g = 0; g < G; ++g) o.beta[g] = w[g] * o.s[g];
 }
 
 // a h + b.  A state that a = 0 cuts off is not looked at (it may be infinite or NaN).
@@ -229,30 +221,6 @@ __device__ __forceinline__ Vec<N> apply(Vec<N> a, Vec<N> h, Vec<N> b) {
     for (int j = 0; j < N; ++j) h.v[j] = a.v[j] == 0.0f ? 0.0f : h.v[j];
   }
   return fma(a, h, b);
-}
-
-// logits at least kShut (a NaN stays)
-__device__ __forceinline__ void hold(Pack<float, 1>& p) { p.v[0] = max_nan(p.v[0], kShut); }
-__device__ __forceinline__ void hold(Pack<__nv_bfloat16, 1>& p) {
-  p.v[0] = __hmax_nan(p.v[0], __float2bfloat16_rn(kShut));
-}
-__device__ __forceinline__ void hold(Pack<__half, 1>& p) { p.v[0] = __hmax_nan(p.v[0], __float2half_rn(kShut)); }
-template <int V>
-__device__ __forceinline__ void hold(Pack<float, V>& p) {
-#pragma unroll
-  for (int v = 0; v < V; ++v) p.v[v] = max_nan(p.v[v], kShut);
-}
-template <int V>
-__device__ __forceinline__ void hold(Pack<__nv_bfloat16, V>& p) {
-  __nv_bfloat162* q = reinterpret_cast<__nv_bfloat162*>(&p);
-#pragma unroll
-  for (int v = 0; v < V / 2; ++v) q[v] = __hmax2_nan(q[v], __float2bfloat162_rn(kShut));
-}
-template <int V>
-__device__ __forceinline__ void hold(Pack<__half, V>& p) {
-  __half2* q = reinterpret_cast<__half2*>(&p);
-#pragma unroll
-  for (int v = 0; v < V / 2; ++v) q[v] = __hmax2_nan(q[v], __float2half2_rn(kShut));
 }
 
 // What a lane works on, and where its strip lies.  Chunks are counted in the order of
@@ -381,137 +349,117 @@ __device__ __forceinline__ void load(Pack<T, V> (&out)[L], const Stream& s, cons
     }
   }
 }
-template <class T, int V, int N>
-__device__ __forceinline__ void store(void* p, const Vec<N> (&val)[V / N]) {
+template <class T, int V>
+__device__ __forceinline__ void store(void* p, Vec<V> val) {
   Pack<T, V> o;
 #pragma unroll
-  for (int v = 0; v < V; ++v) o.v[v] = narrow<T>(val[v / N].v[v % N]);
+  for (int v = 0; v < V; ++v) o.v[v] = narrow<T>(val.v[v]);
   *static_cast<Pack<T, V>*>(p) = o;
 }
 
-// How L x V elements are paired for the two-wide instructions: by channel, or by
-// step where a lane has a single channel.
+// The L x V elements of a chunk as G Vecs for the two-wide instructions: pairs of
+// channels, or of steps where a lane has a single channel.
 template <int V, int L>
-struct Pairing {
-  static constexpr int N = V > 1 ? 2 : 1;  // channels of a Vec
-  static constexpr int P = V / N;          // Vecs of a step
-  static constexpr bool kBySteps = V == 1 && L % 2 == 0;
+struct Cells {
+  static constexpr int N = V == 2 || L % 2 == 0 ? 2 : 1, G = L * V / N;
+  using Array = Vec<N>[G];
+  // those of a step
+  static __device__ __forceinline__ Vec<V> at(const Array& c, int l) {
+    if constexpr (V == N)
+      return c[l];
+    else
+      return {{c[l / N].v[l % N]}};
+  }
+  static __device__ __forceinline__ void put(Array& c, int l, Vec<V> x) {
+    if constexpr (V == N)
+      c[l] = x;
+    else
+      c[l / N].v[l % N] = x.v[0];
+  }
+  template <class T>
+  static __device__ __forceinline__ void widen(const Pack<T, V> (&p)[L], Array& out) {
+#pragma unroll
+    for (int l = 0; l < L; ++l) put(out, l, train::widen<V>(p[l], 0));
+  }
 };
 
-// Calls emit(l, j, gates, beta) for every step and Vec of a chunk, steps in order
-template <class T, int V, int L, bool kMask, bool kFar, class F>
-__device__ __forceinline__ void each_gate(unsigned cut, const Pack<T, V> (&ig)[L], const Pack<T, V> (&rg)[L],
-                                          const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P], F emit) {
-  using Q = Pairing<V, L>;
-  constexpr int N = Q::N;
-  if constexpr (Q::kBySteps) {
-    constexpr int G = L / 2;
-    Vec<2> i2[G], r2[G], k2[G], beta[G];
-    Gates<2> out[G];
+// The gates of a chunk; a step that `cut` has a bit for forgets the state
+template <class T, int V, int L, bool kMask, bool kFar>
+__device__ __forceinline__ void gates_of(unsigned cut, const Pack<T, V> (&ig)[L], const Pack<T, V> (&rg)[L],
+                                         Vec<V> rate, Gates<Cells<V, L>::N, Cells<V, L>::G>& out) {
+  using C = Cells<V, L>;
+  typename C::Array i, r;
+  C::widen(ig, i), C::widen(rg, r);
+  Vec<C::N> k;
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      Pack<T, 2> r{{rg[2 * g].v[0], rg[2 * g + 1].v[0]}}, i{{ig[2 * g].v[0], ig[2 * g + 1].v[0]}};
-      hold(r), hold(i);
-      i2[g] = widen<2>(i, 0), r2[g] = widen<2>(r, 0), k2[g] = splat<2>(rate[0].v[0]);
-    }
-    gates<kFar>(i2, r2, k2, out, beta);
-#pragma unroll
-    for (int l = 0; l < L; ++l) {
-      Gates<1> one{{{out[l / 2].i.v[l % 2]}}, {{out[l / 2].r.v[l % 2]}}, {{out[l / 2].a.v[l % 2]}}};
-      Vec<1> b1{{beta[l / 2].v[l % 2]}};
-      if (kMask && ((cut >> l) & 1u)) one.a = splat<1>(0.0f), b1 = splat<1>(1.0f);
-      emit(l, 0, one, b1);
-    }
-  } else {
-    constexpr int G = L * Q::P;
-    Vec<N> i2[G], r2[G], k2[G], beta[G];
-    Gates<N> out[G];
-#pragma unroll
-    for (int l = 0; l < L; ++l) {
-      Pack<T, V> r = rg[l], i = ig[l];
-      hold(r), hold(i);
-#pragma unroll
-      for (int j = 0; j < Q::P; ++j)
-        i2[l * Q::P + j] = widen<N>(i, j), r2[l * Q::P + j] = widen<N>(r, j), k2[l * Q::P + j] = rate[j];
-    }
-    gates<kFar>(i2, r2, k2, out, beta);
+  for (int j = 0; j < C::N; ++j) k.v[j] = rate.v[j % V];
+  gates<kFar>(i, r, k, out);
+  if (kMask) {
 #pragma unroll
     for (int l = 0; l < L; ++l)
-#pragma unroll
-      for (int j = 0; j < Q::P; ++j) {
-        Gates<N>& one = out[l * Q::P + j];
-        if (kMask && ((cut >> l) & 1u)) one.a = splat<N>(0.0f), beta[l * Q::P + j] = splat<N>(1.0f);
-        emit(l, j, one, beta[l * Q::P + j]);
-      }
+      if ((cut >> l) & 1u) C::put(out.a, l, splat<V>(0.0f)), C::put(out.beta, l, splat<V>(1.0f));
   }
 }
 
 // The rates of a lane's channels, and whether one of the warp's is above kNear
-template <int V, int N>
-__device__ __forceinline__ bool rates(const Args& p, const Lane& o, Vec<N> (&rate)[V / N]) {
+template <int V>
+__device__ __forceinline__ bool rates(const Args& p, const Lane& o, Vec<V>& rate) {
   bool far = false;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const float k = o.on ? p.rate * softplus(p.decay[o.c + v]) : 0.0f;
-    rate[v / N].v[v % N] = k;
+    float k = o.on ? p.rate * softplus(p.decay[o.c + v]) : 0.0f;
+    if (k > kFast) k = kFast;
+    rate.v[v] = k;
     far = far || !(k < kNear);
   }
   return __any_sync(0xffffffffu, far);
 }
 
-template <int V, int N>
-__device__ __forceinline__ void read_row(const float* p, Vec<N> (&out)[V / N]) {
+template <int V>
+__device__ __forceinline__ Vec<V> read_row(const float* p) {
+  Vec<V> out;
 #pragma unroll
-  for (int v = 0; v < V; ++v) out[v / N].v[v % N] = p[v];
+  for (int v = 0; v < V; ++v) out.v[v] = p[v];
+  return out;
 }
 
 // Start value of a strip: the row's, through the maps of the CTAs before and of
 // the strips before in the CTA
-template <int V, int N, bool kMask>
-__device__ __forceinline__ void start_of(const Args& p, const Lane& o, Vec<N> (&h)[V / N]) {
+template <bool kMask>
+__device__ __forceinline__ void start_of(const Args& p, const Lane& o, Vec<1>& h) {
   if (p.strips == 1 || !o.on || o.rank >= p.strips) return;
   const int w = blockDim.y, ctas = (p.strips + w - 1) / w, cta = o.rank / w;
   const float2* t = p.total + o.b * ctas * p.width + o.c;
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    Vec<1> s{{h[v / N].v[v % N]}};
 #pragma unroll 8
-    for (int k = 0; k < cta; ++k) {
-      const float2 m = t[k * p.width + v];
-      s = apply<kMask>(Vec<1>{{m.x}}, s, Vec<1>{{m.y}});
-    }
-    const float2 m = p.before[(o.b * p.strips + o.rank) * p.width + o.c + v];
-    h[v / N].v[v % N] = apply<kMask>(Vec<1>{{m.x}}, s, Vec<1>{{m.y}}).v[0];
+  for (int k = 0; k < cta; ++k) {
+    const float2 m = t[k * p.width];
+    h = apply<kMask>(Vec<1>{{m.x}}, h, Vec<1>{{m.y}});
   }
+  const float2 m = p.before[(o.b * p.strips + o.rank) * p.width + o.c];
+  h = apply<kMask>(Vec<1>{{m.x}}, h, Vec<1>{{m.y}});
 }
 
 // The maps of a CTA's strips, warp by warp: leaves in `before` what the strips
 // before each make of a state, and in `total` all of them.
-template <int V, int N, bool kMask>
-__device__ __forceinline__ void join_maps(const Args& p, const Lane& o, const Vec<N> (&A)[V / N], const Vec<N> (&H)[V / N]) {
-  __shared__ float2 s_map[kStrips][32 * V];
-#pragma unroll
-  for (int v = 0; v < V; ++v)
-    s_map[threadIdx.y][threadIdx.x * V + v] = make_float2(A[v / N].v[v % N], H[v / N].v[v % N]);
+template <bool kMask>
+__device__ __forceinline__ void join_maps(const Args& p, const Lane& o, Vec<1> A, Vec<1> H) {
+  __shared__ float2 s_map[kStrips][32];
+  s_map[threadIdx.y][threadIdx.x] = make_float2(A.v[0], H.v[0]);
   __syncthreads();
   if (!o.on || o.rank >= p.strips) return;
   const int strips = blockDim.y;
-  const bool end = threadIdx.y == strips - 1 || o.rank == p.strips - 1;
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    Vec<1> a{{1.0f}}, h{{0.0f}};
-    for (int w = 0; w < (int)threadIdx.y; ++w) {
-      const float2 m = s_map[w][threadIdx.x * V + v];
-      h = apply<kMask>(Vec<1>{{m.x}}, h, Vec<1>{{m.y}});
-      a.v[0] *= m.x;
-    }
-    p.before[(o.b * p.strips + o.rank) * p.width + o.c + v] = make_float2(a.v[0], h.v[0]);
-    if (end) {
-      const float2 m = s_map[threadIdx.y][threadIdx.x * V + v];
-      h = apply<kMask>(Vec<1>{{m.x}}, h, Vec<1>{{m.y}});
-      const int ctas = (p.strips + strips - 1) / strips;
-      p.total[(o.b * ctas + o.rank / strips) * p.width + o.c + v] = make_float2(a.v[0] * m.x, h.v[0]);
-    }
+  Vec<1> a{{1.0f}}, h{{0.0f}};
+  for (int w = 0; w < (int)threadIdx.y; ++w) {
+    const float2 m = s_map[w][threadIdx.x];
+    h = apply<kMask>(Vec<1>{{m.x}}, h, Vec<1>{{m.y}});
+    a.v[0] *= m.x;
+  }
+  p.before[(o.b * p.strips + o.rank) * p.width + o.c] = make_float2(a.v[0], h.v[0]);
+  if ((int)threadIdx.y == strips - 1 || o.rank == p.strips - 1) {
+    const float2 m = s_map[threadIdx.y][threadIdx.x];
+    h = apply<kMask>(Vec<1>{{m.x}}, h, Vec<1>{{m.y}});
+    const int ctas = (p.strips + strips - 1) / strips;
+    p.total[(o.b * ctas + o.rank / strips) * p.width + o.c] = make_float2(a.v[0] * m.x, h.v[0]);
   }
 }
 
@@ -536,7 +484,7 @@ __device__ __forceinline__ void zero_rest(const Args& p, const Lane& o, void* co
   for (int v = 0; v < V; ++v) z.v[v] = narrow<T>(0.0f);
   // (they lie at one end of the row)
   const int base = o.lo > 0 ? 0 : o.hi, per = (dead + p.strips - 1) / p.strips;
-  const int s0 = (base + o.rank * per) * L, s1 = min((int)p.steps, min(base + dead, base + (o.rank + 1) * per) * L);
+  const int s0 = min((int)p.steps, min(base + dead, base + o.rank * per) * L), s1 = min((int)p.steps, min(base + dead, base + (o.rank + 1) * per) * L);
   const int64_t t = p.reverse ? p.steps - 1 - s0 : s0, step = o.dir * p.width;
   const int64_t at = (o.b * p.steps + t) * p.width + o.c;
 #pragma unroll
@@ -565,15 +513,18 @@ __device__ __forceinline__ void walk(int n, R read, W work) {
 }
 
 // A warp's ring of chunks in shared memory: kRing stages of S streams' boxes
-// [L][32 V] and, with kState, the states before the chunk.
-template <class T, int V, int L, int S, bool kState>
+// [L][32 V] and, with kState, the states before the chunk.  With kOut, 16-bit results take the place
+// of the inputs in their stage and leave by tensor copies as well, which saves a thread their
+// addresses; the stage is filled again a chunk later.
+template <class T, int V, int L, int S, bool kState, bool kOut>
 struct Ring {
+  static constexpr bool kStaged = kOut && sizeof(T) == 2;
   static constexpr int kBox = L * 32 * V * (int)sizeof(T);
   static constexpr int kStage = S * kBox + (kState ? 128 * V : 0);
   static constexpr int kBytes = kRing<T> * kStage;  // of a warp
   char* base;
   uint64_t* bar;
-  const CUtensorMap* map[S];
+  const CUtensorMap *map[S], *out;
 
   __device__ __forceinline__ Ring(char* smem, uint64_t* bars)
       : base(smem + threadIdx.y * kBytes), bar(bars + threadIdx.y * kRing<T>) {
@@ -608,6 +559,27 @@ struct Ring {
 #pragma unroll
     for (int l = 0; l < L; ++l) out[l] = s[l * step];
   }
+  // a result of step l in the place of stream i, and all of the chunk's from stream `from` on to memory
+  __device__ __forceinline__ void put(const Args& p, int stage, int i, int l, Vec<V> val) const {
+    Pack<T, V>* s = reinterpret_cast<Pack<T, V>*>(base + stage * kStage + i * kBox) + threadIdx.x;
+    const int step = p.reverse ? -32 : 32;
+    s += p.reverse ? (L - 1) * 32 : 0;
+    store<T>(s + l * step, val);
+  }
+  template <int kFrom>
+  __device__ __forceinline__ void leave(const Args& p, const Lane& o, int k, int stage) const {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (threadIdx.x == 0) {
+      const int c0 = (int)o.c, t0 = p.reverse ? (int)p.steps - (k + 1) * L : k * L;  // (a whole chunk: not negative)
+#pragma unroll
+      for (int i = kFrom; i < 3; ++i)
+        asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(out + i),
+                     "r"(smem_u32(base + stage * kStage + i * kBox)), "r"(c0), "r"(t0), "r"((int)o.b)
+                     : "memory");
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+  }
   __device__ __forceinline__ Pack<float, V> state(int stage) const {
     return reinterpret_cast<const Pack<float, V>*>(base + stage * kStage + S * kBox)[threadIdx.x];
   }
@@ -634,9 +606,17 @@ struct Ring {
       }
       In in;
       in.q = q;
+      in.stage = stage;
       read(stage, in);
       __syncwarp();
-      if (threadIdx.x == 0 && k + kRing<T> < n) send(p, o, first + way * (k + kRing<T>), stage);
+      if (kStaged) {  // the stage before, once its results have left it
+        if (threadIdx.x == 0 && k > 0 && k - 1 + kRing<T> < n) {
+          asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          send(p, o, first + way * (k - 1 + kRing<T>), stage == 0 ? kRing<T> - 1 : stage - 1);
+        }
+      } else if (threadIdx.x == 0 && k + kRing<T> < n) {
+        send(p, o, first + way * (k + kRing<T>), stage);
+      }
       q = chunk_of<L, kMask>(p, o, first + way * min(k + 1, n - 1));
       flag_chunk<L, kMask>(p, o, q);
       work(first + way * k, in);
@@ -646,17 +626,21 @@ struct Ring {
       if (threadIdx.x == 0) atomicOr(p.error, 1u);
       for (int i = 0; i < kRing<T>; ++i) mbar_wait(bar + i, i < stage ? parity ^ 1 : parity);
     }
+    if (kStaged && threadIdx.x == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     return ok;
   }
 };
 // a warp without a ring, where every lane loads its own
-struct NoRing {};
+struct NoRing {
+  static constexpr bool kStaged = false;
+};
 
 // ------------------------------------------------------------------- forward
 
 template <class T, int V, int L>
 struct Loaded {
   Chunk q;
+  int stage;  // of a ring
   Pack<T, V> x[L], ig[L], rg[L];
   template <class R>
   __device__ __forceinline__ void get(const Args& p, const R& ring, int stage) {
@@ -671,6 +655,16 @@ struct Loaded {
     load<T, V, L, kFull>(rg, p.rg, o, q, kShut);
     load<T, V, L, kFull>(ig, p.ig, o, q);
     load<T, V, L, kFull>(x, p.x, o, q);
+  }
+  // Every step as h -> a h + b
+  template <bool kMask, bool kFar>
+  __device__ __forceinline__ void steps(const Args& p, Vec<V> rate, Gates<Cells<V, L>::N, Cells<V, L>::G>& g,
+                                        typename Cells<V, L>::Array& b) {
+    if (q.live != (1u << L) - 1) blank(rg, q, kShut), blank(ig, q), blank(x, q);
+    gates_of<T, V, L, kMask, kFar>(cuts<kMask>(p, q), ig, rg, rate, g);
+    Cells<V, L>::widen(x, b);
+#pragma unroll
+    for (int i = 0; i < Cells<V, L>::G; ++i) b[i] = g.beta[i] * (g.i[i] * b[i]);
   }
 };
 
@@ -700,33 +694,31 @@ __device__ __forceinline__ bool forward_walk(const Args& p, const Lane& o, R& ri
   }
 }
 
-template <class T, int V, int L, bool kMask, bool kFar, class R>
-__device__ __forceinline__ void forward_maps(const Args& p, const Lane& o, R& ring,
-                                             const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P]) {
-  using Q = Pairing<V, L>;
-  constexpr int N = Q::N, P = Q::P;
-  Vec<N> A[P], H[P];
+template <class T, int L, bool kMask, bool kFar, class R>
+__device__ __forceinline__ void forward_maps(const Args& p, const Lane& o, R& ring, Vec<1> rate) {
+  using C = Cells<1, L>;
+  Vec<1> A = splat<1>(1.0f), H = splat<1>(0.0f);
+  forward_walk<T, 1, L, kMask>(p, o, ring, [&](int, Loaded<T, 1, L>& in, auto) {
+    Gates<C::N, C::G> g;
+    typename C::Array b;
+    in.template steps<kMask, kFar>(p, rate, g, b);
 #pragma unroll
-  for (int j = 0; j < P; ++j) A[j] = splat<N>(1.0f), H[j] = splat<N>(0.0f);
-  forward_walk<T, V, L, kMask>(p, o, ring, [&](int, Loaded<T, V, L>& in, auto) {
-    if (in.q.live != (1u << L) - 1) blank(in.rg, in.q, kShut), blank(in.ig, in.q), blank(in.x, in.q);
-    each_gate<T, V, L, kMask, kFar>(
-        cuts<kMask>(p, in.q), in.ig, in.rg, rate, [&](int l, int j, const Gates<N>& g, Vec<N> beta) {
-          H[j] = apply<kMask>(g.a, H[j], beta * (g.i * widen<N>(in.x[l], j)));
-          A[j] = A[j] * g.a;
-        });
+    for (int l = 0; l < L; ++l) {
+      H = apply<kMask>(C::at(g.a, l), H, C::at(b, l));
+      A = A * C::at(g.a, l);
+    }
   });
-  join_maps<V, N, kMask>(p, o, A, H);
+  join_maps<kMask>(p, o, A, H);
 }
 
 // The ring of a forward warp, with its first copies on their way
-template <class T, int V, int L, bool kBulk>
+template <class T, int V, int L, bool kBulk, bool kOut>
 __device__ __forceinline__ auto forward_ring(const Args& p, const Maps& m, const Lane& o) {
   if constexpr (kBulk) {
     extern __shared__ __align__(128) char dynamic[];
     __shared__ uint64_t s_bar[kRowWarps * kRing<T>];
-    Ring<T, V, L, 3, false> ring(dynamic, s_bar);
-    ring.map[0] = &m.rg, ring.map[1] = &m.ig, ring.map[2] = &m.x;
+    Ring<T, V, L, 3, false, kOut> ring(dynamic, s_bar);
+    ring.map[0] = &m.rg, ring.map[1] = &m.ig, ring.map[2] = &m.x, ring.out = m.out;
     ring.start(p, o, o.first, o.count, 1);
     return ring;
   } else {
@@ -734,75 +726,73 @@ __device__ __forceinline__ auto forward_ring(const Args& p, const Maps& m, const
   }
 }
 
-template <class T, int V, int L, bool kMask, bool kBulk>
-__global__ void __launch_bounds__(32 * kStrips) forward_maps_kernel(const __grid_constant__ Args p,
+template <class T, int L, bool kMask, bool kBulk>
+__global__ void __launch_bounds__(32 * kStrips, forward_ctas(8, kBulk, sizeof(T))) forward_maps_kernel(const __grid_constant__ Args p,
                                                                     const __grid_constant__ Maps m) {
-  using Q = Pairing<V, L>;
   let_next_start();
-  const Lane o = lane_of<V, L, kMask, false>(p);
-  auto ring = forward_ring<T, V, L, kBulk>(p, m, o);
-  Vec<Q::N> rate[Q::P];
+  const Lane o = lane_of<1, L, kMask, false>(p);
+  auto ring = forward_ring<T, 1, L, kBulk, false>(p, m, o);
+  Vec<1> rate;
   // (the CTA's warps share their channels, so they agree, and meet in join_maps)
-  if (rates<V, Q::N>(p, o, rate))
-    forward_maps<T, V, L, kMask, true>(p, o, ring, rate);
+  if (rates<1>(p, o, rate))
+    forward_maps<T, L, kMask, true>(p, o, ring, rate);
   else
-    forward_maps<T, V, L, kMask, false>(p, o, ring, rate);
+    forward_maps<T, L, kMask, false>(p, o, ring, rate);
 }
 
-template <class T, int V, int L, bool kMask, bool kFar, bool kFull>
-__device__ __forceinline__ void forward_chunk(const Args& p, const Lane& o, int k, Loaded<T, V, L>& in,
-                                              const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P],
-                                              Vec<Pairing<V, L>::N> (&h)[Pairing<V, L>::P]) {
-  using Q = Pairing<V, L>;
-  constexpr int N = Q::N, P = Q::P;
+template <class T, int V, int L, bool kMask, bool kFar, bool kFull, class R>
+__device__ __forceinline__ void forward_chunk(const Args& p, const Lane& o, const R& ring, int k, Loaded<T, V, L>& in,
+                                              Vec<V> rate, Vec<V>& h) {
+  using C = Cells<V, L>;
   if (p.kept && o.on) {
     float* keep = p.kept + (o.b * ((p.steps + L - 1) / L) + k) * p.width + o.c;
 #pragma unroll
-    for (int v = 0; v < V; ++v) keep[v] = h[v / N].v[v % N];
+    for (int v = 0; v < V; ++v) keep[v] = h.v[v];
   }
-  if (in.q.live != (1u << L) - 1) blank(in.rg, in.q, kShut), blank(in.ig, in.q), blank(in.x, in.q);
+  Gates<C::N, C::G> g;
+  typename C::Array b;
+  in.template steps<kMask, kFar>(p, rate, g, b);
   char* y = reinterpret_cast<char*>(static_cast<T*>(p.y) + (o.b * p.steps + in.q.t0) * p.width + o.c);
   const int step = o.dir * (int)p.width * (int)sizeof(T);
-  Vec<N> out[P];
-  each_gate<T, V, L, kMask, kFar>(
-      cuts<kMask>(p, in.q), in.ig, in.rg, rate, [&](int l, int j, const Gates<N>& g, Vec<N> beta) {
-        h[j] = apply<kMask>(g.a, h[j], beta * (g.i * widen<N>(in.x[l], j)));
-        out[j] = !kMask || ((in.q.live >> l) & 1u) ? h[j] : splat<N>(0.0f);
-        if (j == P - 1 && o.on && (kFull || ((in.q.inside >> l) & 1u))) store<T, V, N>(y + (int64_t)step * l, out);
-      });
+#pragma unroll
+  for (int l = 0; l < L; ++l) {
+    h = apply<kMask>(C::at(g.a, l), h, C::at(b, l));
+    const Vec<V> out = !kMask || ((in.q.live >> l) & 1u) ? h : splat<V>(0.0f);
+    if constexpr (R::kStaged && kFull)
+      ring.put(p, in.stage, 2, l, out);
+    else if (o.on && (kFull || ((in.q.inside >> l) & 1u)))
+      store<T>(y + (int64_t)step * l, out);
+  }
+  if constexpr (R::kStaged && kFull) ring.template leave<2>(p, o, k, in.stage);
 }
 
 template <class T, int V, int L, bool kMask, bool kFar, class R>
-__device__ __forceinline__ void forward_strip(const Args& p, const Lane& o, R& ring,
-                                              const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P]) {
-  using Q = Pairing<V, L>;
-  constexpr int N = Q::N, P = Q::P;
-  Vec<N> h[P];
-#pragma unroll
-  for (int j = 0; j < P; ++j) h[j] = splat<N>(0.0f);
-  if (p.state) read_row<V, N>(p.state + o.b * p.width + o.from, h);
-  if (p.strips > 1) wait_for_last();
-  if (o.rank >= p.strips) return;
-  start_of<V, N, kMask>(p, o, h);
+__device__ __forceinline__ void forward_strip(const Args& p, const Lane& o, R& ring, Vec<V> rate) {
+  Vec<V> h = splat<V>(0.0f);
+  if (p.state) h = read_row<V>(p.state + o.b * p.width + o.from);
+  if constexpr (V == 1) {
+    if (p.strips > 1) wait_for_last();
+    if (o.rank >= p.strips) return;
+    start_of<kMask>(p, o, h);
+  }
   if (!forward_walk<T, V, L, kMask>(p, o, ring, [&](int k, Loaded<T, V, L>& in, auto full) {
-        forward_chunk<T, V, L, kMask, kFar, decltype(full)::value>(p, o, k, in, rate, h);
+        forward_chunk<T, V, L, kMask, kFar, decltype(full)::value>(p, o, ring, k, in, rate, h);
       }))
     return;
   if (kMask) zero_rest<T, V, L, 1>(p, o, {p.y});
   if (o.rank == p.strips - 1 && o.on) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) p.last[o.b * p.width + o.c + v] = h[v / N].v[v % N];
+    for (int v = 0; v < V; ++v) p.last[o.b * p.width + o.c + v] = h.v[v];
   }
 }
 
 template <class T, int V, int L, bool kMask, bool kBulk>
-__global__ void __launch_bounds__(32 * kStrips) forward_kernel(const __grid_constant__ Args p,
+__global__ void __launch_bounds__(V == 2 ? 32 : 32 * kStrips, V == 2 ? (kBulk ? 16 : 11) : forward_ctas(8, kBulk, sizeof(T))) forward_kernel(const __grid_constant__ Args p,
                                                                const __grid_constant__ Maps m) {
-  using Q = Pairing<V, L>;
   const Lane o = lane_of<V, L, kMask, false>(p);
-  auto ring = forward_ring<T, V, L, kBulk>(p, m, o);
-  Vec<Q::N> rate[Q::P];
-  if (rates<V, Q::N>(p, o, rate))
+  auto ring = forward_ring<T, V, L, kBulk, true>(p, m, o);
+  Vec<V> rate;
+  if (rates<V>(p, o, rate))
     forward_strip<T, V, L, kMask, true>(p, o, ring, rate);
   else
     forward_strip<T, V, L, kMask, false>(p, o, ring, rate);
@@ -812,10 +802,12 @@ __global__ void __launch_bounds__(32 * kStrips) forward_kernel(const __grid_cons
 // the strips' maps meet in shared memory, and the recursion is run from the state that
 // they give.  The data pass once, in one launch.
 template <class T, int L, bool kMask, bool kFar, class R>
-__device__ __forceinline__ void forward_row(const Args& p, const Lane& o, R& ring, const Vec<1> (&rate)[1]) {
+__device__ __forceinline__ void forward_row(const Args& p, const Lane& o, R& ring, Vec<1> rate) {
+  using C = Cells<1, L>;
   constexpr int NC = kHeld / L;
   __shared__ float2 s_map[kRowWarps][32];
-  Vec<1> a[NC][L], b[NC][L], A{{1.0f}}, H{{0.0f}};
+  typename C::Array a[NC], b[NC];
+  Vec<1> A{{1.0f}}, H{{0.0f}};
   unsigned live[NC];
   using In = Loaded<T, 1, L>;
   In in[2];
@@ -827,7 +819,7 @@ __device__ __forceinline__ void forward_row(const Args& p, const Lane& o, R& rin
   for (int c = 0; c < NC; ++c) {
     live[c] = 0u;
 #pragma unroll
-    for (int l = 0; l < L; ++l) a[c][l] = splat<1>(1.0f), b[c][l] = splat<1>(0.0f);
+    for (int g = 0; g < C::G; ++g) a[c][g] = splat<C::N>(1.0f), b[c][g] = splat<C::N>(0.0f);
     if (c >= o.count) continue;
     In& now = in[c % 2];
     if constexpr (std::is_same<R, NoRing>::value) {
@@ -835,20 +827,27 @@ __device__ __forceinline__ void forward_row(const Args& p, const Lane& o, R& rin
     } else {
       now.q = chunk_of<L, kMask>(p, o, o.first + c);
       flag_chunk<L, kMask>(p, o, now.q);
-      ok = ok && __all_sync(0xffffffffu, mbar_wait(ring.bar + c, 0));
+      const bool came = __all_sync(0xffffffffu, mbar_wait(ring.bar + c, 0));
+      ok = ok && came;
       now.get(p, ring, c);
     }
-    if (now.q.live != (1u << L) - 1) blank(now.rg, now.q, kShut), blank(now.ig, now.q), blank(now.x, now.q);
+    Gates<C::N, C::G> g;
+    now.template steps<kMask, kFar>(p, rate, g, b[c]);
     live[c] = now.q.live;
-    each_gate<T, 1, L, kMask, kFar>(
-        cuts<kMask>(p, now.q), now.ig, now.rg, rate, [&](int l, int, const Gates<1>& g, Vec<1> beta) {
-          a[c][l] = g.a;
-          b[c][l] = beta * (g.i * widen<1>(now.x[l], 0));
-          H = apply<kMask>(g.a, H, b[c][l]);
-          A = A * g.a;
-        });
+#pragma unroll
+    for (int i = 0; i < C::G; ++i) a[c][i] = g.a[i];
+#pragma unroll
+    for (int l = 0; l < L; ++l) {
+      H = apply<kMask>(C::at(a[c], l), H, C::at(b[c], l));
+      A = A * C::at(a[c], l);
+    }
   }
-  if (!ok && threadIdx.x == 0) atomicOr(p.error, 1u);
+  if constexpr (!std::is_same<R, NoRing>::value) {
+    if (!ok) {  // as in Ring::walk
+      if (threadIdx.x == 0) atomicOr(p.error, 1u);
+      for (int c = 0; c < o.count; ++c) mbar_wait(ring.bar + c, 0);
+    }
+  }
   s_map[threadIdx.y][threadIdx.x] = make_float2(A.v[0], H.v[0]);
   __syncthreads();
   Vec<1> h{{p.state ? p.state[o.b * p.width + o.from] : 0.0f}};
@@ -866,9 +865,9 @@ __device__ __forceinline__ void forward_row(const Args& p, const Lane& o, R& rin
     const int step = o.dir * (int)p.width * (int)sizeof(T);
 #pragma unroll
     for (int l = 0; l < L; ++l) {
-      h = apply<kMask>(a[c][l], h, b[c][l]);
-      const Vec<1> out[1] = {!kMask || ((live[c] >> l) & 1u) ? h : splat<1>(0.0f)};
-      if ((q.inside >> l) & 1u) store<T, 1, 1>(y + (int64_t)step * l, out);
+      h = apply<kMask>(C::at(a[c], l), h, C::at(b[c], l));
+      const Vec<1> out = !kMask || ((live[c] >> l) & 1u) ? h : splat<1>(0.0f);
+      if ((q.inside >> l) & 1u) store<T>(y + (int64_t)step * l, out);
     }
   }
   if (kMask) zero_rest<T, 1, L, 1>(p, o, {p.y});
@@ -879,9 +878,9 @@ template <class T, int L, bool kMask, bool kBulk>
 __global__ void __launch_bounds__(32 * kRowWarps) forward_row_kernel(const __grid_constant__ Args p,
                                                                      const __grid_constant__ Maps m) {
   const Lane o = lane_of<1, L, kMask, false>(p);
-  auto ring = forward_ring<T, 1, L, kBulk>(p, m, o);
-  Vec<1> rate[1];
-  if (rates<1, 1>(p, o, rate))
+  auto ring = forward_ring<T, 1, L, kBulk, false>(p, m, o);
+  Vec<1> rate;
+  if (rates<1>(p, o, rate))
     forward_row<T, L, kMask, true>(p, o, ring, rate);
   else
     forward_row<T, L, kMask, false>(p, o, ring, rate);
@@ -892,6 +891,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) forward_row_kernel(const __gri
 template <class T, int V, int L>
 struct LoadedMap {
   Chunk q;
+  int stage;  // of a ring
   Pack<T, V> rg[L], dy[L];
   template <class R>
   __device__ __forceinline__ void get(const Args& p, const R& ring, int stage) {
@@ -910,17 +910,16 @@ struct LoadedMap {
 template <class T, int V, int L>
 struct LoadedBack {
   Chunk q;
+  int stage;  // of a ring
   Pack<T, V> x[L], ig[L], rg[L], dy[L];
-  Vec<Pairing<V, L>::N> h[Pairing<V, L>::P];  // state before the chunk
+  Vec<V> h;  // state before the chunk
   template <class R>
   __device__ __forceinline__ void get(const Args& p, const R& ring, int stage) {
     ring.get(p, stage, 0, rg);
     ring.get(p, stage, 1, ig);
     ring.get(p, stage, 2, x);
     ring.get(p, stage, 3, dy);
-    const Pack<float, V> s = ring.state(stage);
-#pragma unroll
-    for (int j = 0; j < Pairing<V, L>::P; ++j) h[j] = widen<Pairing<V, L>::N>(s, j);
+    h = widen<V>(ring.state(stage), 0);
   }
   template <bool kMask, bool kFull>
   __device__ __forceinline__ void read(const Args& p, const Lane& o, int k) {
@@ -930,7 +929,7 @@ struct LoadedBack {
     load<T, V, L, kFull>(ig, p.ig, o, q);
     load<T, V, L, kFull>(x, p.x, o, q);
     load<T, V, L, kFull>(dy, p.dy, o, q);
-    read_row<V, Pairing<V, L>::N>(p.kept + (o.b * ((p.steps + L - 1) / L) + k) * p.width + o.from, h);
+    h = read_row<V>(p.kept + (o.b * ((p.steps + L - 1) / L) + k) * p.width + o.from);
   }
 };
 
@@ -942,57 +941,49 @@ __device__ __forceinline__ bool backward_walk(const Args& p, const Lane& o, R& r
         p, o, o.first + o.count - 1, o.count, -1, [&](int stage, In& in) { in.get(p, ring, stage); },
         [&](int k, In& in) {
           if (k - o.first < o.whole)
-            work(in, std::true_type{});
+            work(k, in, std::true_type{});
           else
-            work(in, std::false_type{});
+            work(k, in, std::false_type{});
         });
   } else {
     if (o.whole < o.count) {
       In in;
       in.template read<kMask, false>(p, o, o.first + o.whole);
-      work(in, std::false_type{});
+      work(o.first + o.whole, in, std::false_type{});
     }
     walk<In>(
         o.whole, [&](int k, In& in) { in.template read<kMask, true>(p, o, o.first + o.whole - 1 - k); },
-        [&](int, In& in) { work(in, std::true_type{}); });
+        [&](int k, In& in) { work(o.first + o.whole - 1 - k, in, std::true_type{}); });
     return true;
   }
 }
 
 // e -> A e + E of a strip, from its last step to its first: the decay gate and
 // dy are all it takes
-template <class T, int V, int L, bool kMask, bool kFar, class R>
-__device__ __forceinline__ void backward_maps(const Args& p, const Lane& o, R& ring,
-                                              const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P]) {
-  using Q = Pairing<V, L>;
-  constexpr int N = Q::N, P = Q::P;
-  Vec<N> A[P], E[P];
-#pragma unroll
-  for (int j = 0; j < P; ++j) A[j] = splat<N>(1.0f), E[j] = splat<N>(0.0f);
-  using In = LoadedMap<T, V, L>;
-  backward_walk<T, V, L, kMask, In>(p, o, ring, [&](In& in, auto) {
+template <class T, int L, bool kMask, bool kFar, class R>
+__device__ __forceinline__ void backward_maps(const Args& p, const Lane& o, R& ring, Vec<1> rate) {
+  using C = Cells<1, L>;
+  Vec<1> A = splat<1>(1.0f), E = splat<1>(0.0f);
+  using In = LoadedMap<T, 1, L>;
+  backward_walk<T, 1, L, kMask, In>(p, o, ring, [&](int, In& in, auto) {
     if (in.q.live != (1u << L) - 1) blank(in.rg, in.q, kShut), blank(in.dy, in.q);
     const unsigned cut = cuts<kMask>(p, in.q);
-    Vec<N> rg[L * P], k2[L * P], a[L * P];
+    typename C::Array r, a, w;
+    C::widen(in.rg, a);
+    sigmoids(a, r);
+    Vec<C::N> k;
 #pragma unroll
-    for (int l = 0; l < L; ++l) {
-      hold(in.rg[l]);
-#pragma unroll
-      for (int j = 0; j < P; ++j) rg[l * P + j] = widen<N>(in.rg[l], j), k2[l * P + j] = rate[j];
-    }
-    decays_of<kFar>(rg, k2, a);
+    for (int j = 0; j < C::N; ++j) k.v[j] = rate.v[0];
+    decays<kFar>(r, k, a, w);
 #pragma unroll
     for (int l = L - 1; l >= 0; --l) {
-#pragma unroll
-      for (int j = 0; j < P; ++j) {
-        Vec<N> al = a[l * P + j];
-        if (kMask && ((cut >> l) & 1u)) al = splat<N>(0.0f);
-        E[j] = apply<kMask>(al, E[j] + widen<N>(in.dy[l], j), splat<N>(0.0f));
-        A[j] = A[j] * al;
-      }
+      Vec<1> al = C::at(a, l);
+      if (kMask && ((cut >> l) & 1u)) al = splat<1>(0.0f);
+      E = apply<kMask>(al, E + widen<1>(in.dy[l], 0), splat<1>(0.0f));
+      A = A * al;
     }
   });
-  join_maps<V, N, kMask>(p, o, A, E);
+  join_maps<kMask>(p, o, A, E);
 }
 
 template <class T, int V, int L, bool kBulk, bool kMaps>
@@ -1000,8 +991,8 @@ __device__ __forceinline__ auto backward_ring(const Args& p, const Maps& m, cons
   if constexpr (kBulk) {
     extern __shared__ __align__(128) char dynamic[];
     __shared__ uint64_t s_bar[kStrips * kRing<T>];
-    Ring<T, V, L, kMaps ? 2 : 4, !kMaps> ring(dynamic, s_bar);
-    ring.map[0] = &m.rg;
+    Ring<T, V, L, kMaps ? 2 : 4, !kMaps, !kMaps> ring(dynamic, s_bar);
+    ring.map[0] = &m.rg, ring.out = m.out;
     if constexpr (kMaps)
       ring.map[1] = &m.dy;
     else
@@ -1013,124 +1004,149 @@ __device__ __forceinline__ auto backward_ring(const Args& p, const Maps& m, cons
   }
 }
 
-template <class T, int V, int L, bool kMask, bool kBulk>
+template <class T, int L, bool kMask, bool kBulk>
 __global__ void __launch_bounds__(32 * kStrips) backward_maps_kernel(const __grid_constant__ Args p,
                                                                      const __grid_constant__ Maps m) {
-  using Q = Pairing<V, L>;
   let_next_start();
-  const Lane o = lane_of<V, L, kMask, true>(p);
-  auto ring = backward_ring<T, V, L, kBulk, true>(p, m, o);
-  Vec<Q::N> rate[Q::P];
-  if (rates<V, Q::N>(p, o, rate))
-    backward_maps<T, V, L, kMask, true>(p, o, ring, rate);
+  const Lane o = lane_of<1, L, kMask, true>(p);
+  auto ring = backward_ring<T, 1, L, kBulk, true>(p, m, o);
+  Vec<1> rate;
+  if (rates<1>(p, o, rate))
+    backward_maps<T, L, kMask, true>(p, o, ring, rate);
   else
-    backward_maps<T, V, L, kMask, false>(p, o, ring, rate);
+    backward_maps<T, L, kMask, false>(p, o, ring, rate);
 }
 
 // With e = a g (see above) everything but g is known before the carry comes in:
 //   dx = g P1, dinput_gate = dx P2, s = g R1, ddecay_gate = s R2,
-//   P1 = beta i, P2 = x (1 - i), R1 = r (a h_{t-1} - (a^2 / beta) i x), R2 = rate (r - 1),
-// and s sums up to the decay gradient.
-template <class T, int V, int L, bool kMask, bool kFar, bool kFull>
-__device__ __forceinline__ void backward_chunk(const Args& p, const Lane& o, LoadedBack<T, V, L>& in,
-                                               const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P],
-                                               Vec<Pairing<V, L>::N> (&e)[Pairing<V, L>::P],
-                                               Vec<Pairing<V, L>::N> (&acc)[Pairing<V, L>::P]) {
-  using Q = Pairing<V, L>;
-  constexpr int N = Q::N, P = Q::P;
+//   P1 = beta i, P2 = x (1 - i), R1 = r (a h_{t-1} - (a / beta)^2 b), R2 = rate (r - 1),
+// with b = beta i x, and s sums up to the decay gradient.
+template <class T, int V, int L, bool kMask, bool kFar, bool kFull, class R>
+__device__ __forceinline__ void backward_chunk(const Args& p, const Lane& o, const R& ring, int k, LoadedBack<T, V, L>& in,
+                                               Vec<V> rate, Vec<V>& e, Vec<Cells<V, L>::N>& acc) {
+  using C = Cells<V, L>;
+  constexpr int N = C::N, G = C::G;
+  const Vec<N> minus = splat<N>(-1.0f);
   if (in.q.live != (1u << L) - 1)
     blank(in.rg, in.q, kShut), blank(in.ig, in.q), blank(in.x, in.q), blank(in.dy, in.q);
-  Vec<N> a[L][P], p1[L][P], p2[L][P], r1[L][P], r2[L][P], h[P];
+  Gates<N, G> q;
+  gates_of<T, V, L, kMask, kFar>(cuts<kMask>(p, in.q), in.ig, in.rg, rate, q);
+  typename C::Array b, p1, p2, r1, r2, ah, g;
+  C::widen(in.x, p2);
+  Vec<N> fast;
 #pragma unroll
-  for (int j = 0; j < P; ++j) h[j] = in.h[j];
-  each_gate<T, V, L, kMask, kFar>(cuts<kMask>(p, in.q), in.ig, in.rg, rate, [&](int l, int j, const Gates<N>& g, Vec<N> beta) {
-    const Vec<N> x = widen<N>(in.x[l], j);
-    Vec<N> inverse;  // dropped with beta
+  for (int j = 0; j < N; ++j) fast.v[j] = rate.v[j % V];
 #pragma unroll
-    for (int i = 0; i < N; ++i) inverse.v[i] = beta.v[i] > kTiny ? -rcp_approx(beta.v[i]) : 0.0f;
-    const Vec<N> ah = apply<kMask>(g.a, h[j], splat<N>(0.0f)), ix = g.i * x;
-    Vec<N> d = fma(g.a * (g.a * inverse), ix, ah);
-    if (kMask) {
+  for (int i = 0; i < G; ++i) {
+    const Vec<N> ix = q.i[i] * p2[i], u = q.a[i] * q.s[i];
+    b[i] = q.beta[i] * ix;
+    p1[i] = q.beta[i] * q.i[i];
+    p2[i] = fma(ix, minus, p2[i]);
+    r1[i] = u * (u * b[i]);  // (where beta is zero, b is: the term is dropped)
+    r2[i] = fast * (q.r[i] + minus);
+  }
+  Vec<V> h = in.h;
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (g.a.v[i] == 0.0f || !((in.q.live >> l) & 1u)) d.v[i] = 0.0f;
+  for (int l = 0; l < L; ++l) {
+    C::put(ah, l, apply<kMask>(C::at(q.a, l), h, splat<V>(0.0f)));
+    h = apply<kMask>(C::at(q.a, l), h, C::at(b, l));
+  }
+#pragma unroll
+  for (int i = 0; i < G; ++i) r1[i] = q.r[i] * fma(r1[i], minus, ah[i]);
+  if (kMask) {
+#pragma unroll
+    for (int l = 0; l < L; ++l) {
+      Vec<V> d = C::at(r1, l);
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (C::at(q.a, l).v[v] == 0.0f || !((in.q.live >> l) & 1u)) d.v[v] = 0.0f;
+      C::put(r1, l, d);
     }
-    a[l][j] = g.a;
-    p1[l][j] = beta * g.i;
-    p2[l][j] = fma(ix, splat<N>(-1.0f), x);
-    r1[l][j] = g.r * d;
-    r2[l][j] = rate[j] * (g.r + splat<N>(-1.0f));
-    h[j] = fma(beta, ix, ah);
-  });
+  }
+#pragma unroll
+  for (int l = L - 1; l >= 0; --l) {
+    const Vec<V> now = e + widen<V>(in.dy[l], 0);
+    e = apply<kMask>(C::at(q.a, l), now, splat<V>(0.0f));
+    C::put(g, l, now);
+  }
+  // dx, dinput_gate, ddecay_gate take the places of p1, p2, r2
+#pragma unroll
+  for (int i = 0; i < G; ++i) {
+    p1[i] = g[i] * p1[i];
+    Vec<N> s = g[i] * r1[i];
+    if (kMask) {  // (a gradient that is not finite is not spread to where nothing flows)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int l = V == N ? i : i * N + j;
+        if (!((in.q.live >> l) & 1u)) p1[i].v[j] = 0.0f;
+        if (r1[i].v[j] == 0.0f) s.v[j] = 0.0f;
+      }
+    }
+    p2[i] = p1[i] * p2[i];
+    acc = acc + s;
+    r2[i] = s * r2[i];
+  }
+  if constexpr (R::kStaged && kFull) {
+#pragma unroll
+    for (int l = 0; l < L; ++l) {
+      ring.put(p, in.stage, 2, l, C::at(p1, l));
+      ring.put(p, in.stage, 1, l, C::at(p2, l));
+      ring.put(p, in.stage, 0, l, C::at(r2, l));
+    }
+    ring.template leave<0>(p, o, k, in.stage);
+    return;
+  }
+  if (!o.on) return;
   const int64_t first = (o.b * p.steps + in.q.t0) * p.width + o.c;
   const int step = o.dir * (int)p.width * (int)sizeof(T);
   char *px = reinterpret_cast<char*>(static_cast<T*>(p.dx) + first),
        *pi = reinterpret_cast<char*>(static_cast<T*>(p.dig) + first),
        *pr = reinterpret_cast<char*>(static_cast<T*>(p.drg) + first);
 #pragma unroll
-  for (int l = L - 1; l >= 0; --l) {
-    Vec<N> dx[P], di[P], dr[P];
-#pragma unroll
-    for (int j = 0; j < P; ++j) {
-      const Vec<N> g = e[j] + widen<N>(in.dy[l], j);
-      e[j] = apply<kMask>(a[l][j], g, splat<N>(0.0f));
-      dx[j] = g * p1[l][j];
-      Vec<N> s = g * r1[l][j];
-      if (kMask) {  // (a gradient that is not finite is not spread to where nothing flows)
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          if (!((in.q.live >> l) & 1u)) dx[j].v[i] = 0.0f;
-          if (r1[l][j].v[i] == 0.0f) s.v[i] = 0.0f;
-        }
-      }
-      di[j] = dx[j] * p2[l][j];
-      acc[j] = acc[j] + s;
-      dr[j] = s * r2[l][j];
-    }
-    if (o.on && (kFull || ((in.q.inside >> l) & 1u))) {
+  for (int l = 0; l < L; ++l)
+    if (kFull || ((in.q.inside >> l) & 1u)) {
       const int64_t at = (int64_t)step * l;
-      store<T, V, N>(px + at, dx);
-      store<T, V, N>(pi + at, di);
-      store<T, V, N>(pr + at, dr);
+      store<T>(px + at, C::at(p1, l));
+      store<T>(pi + at, C::at(p2, l));
+      store<T>(pr + at, C::at(r2, l));
     }
-  }
 }
 
 template <class T, int V, int L, bool kMask, bool kFar, class R>
-__device__ __forceinline__ void backward_strip(const Args& p, const Lane& o, R& ring,
-                                               const Vec<Pairing<V, L>::N> (&rate)[Pairing<V, L>::P]) {
-  using Q = Pairing<V, L>;
-  constexpr int N = Q::N, P = Q::P;
-  Vec<N> e[P], acc[P];
-#pragma unroll
-  for (int j = 0; j < P; ++j) e[j] = acc[j] = splat<N>(0.0f);
-  if (p.dlast) read_row<V, N>(p.dlast + o.b * p.width + o.from, e);
-  if (p.strips > 1) wait_for_last();
-  if (o.rank >= p.strips) return;
-  start_of<V, N, kMask>(p, o, e);
+__device__ __forceinline__ void backward_strip(const Args& p, const Lane& o, R& ring, Vec<V> rate) {
+  using C = Cells<V, L>;
+  Vec<V> e = splat<V>(0.0f);
+  Vec<C::N> acc = splat<C::N>(0.0f);
+  if (p.dlast) e = read_row<V>(p.dlast + o.b * p.width + o.from);
+  if constexpr (V == 1) {
+    if (p.strips > 1) wait_for_last();
+    if (o.rank >= p.strips) return;
+    start_of<kMask>(p, o, e);
+  }
   using In = LoadedBack<T, V, L>;
-  if (!backward_walk<T, V, L, kMask, In>(p, o, ring, [&](In& in, auto full) {
-        backward_chunk<T, V, L, kMask, kFar, decltype(full)::value>(p, o, in, rate, e, acc);
+  if (!backward_walk<T, V, L, kMask, In>(p, o, ring, [&](int k, In& in, auto full) {
+        backward_chunk<T, V, L, kMask, kFar, decltype(full)::value>(p, o, ring, k, in, rate, e, acc);
       }))
     return;
   if (kMask) zero_rest<T, V, L, 3>(p, o, {p.dx, p.dig, p.drg});
   if (!o.on) return;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    if (o.rank == p.strips - 1 && p.dstate) p.dstate[o.b * p.width + o.c + v] = e[v / N].v[v % N];
-    p.dpart[(o.b * p.strips + o.rank) * p.width + o.c + v] = acc[v / N].v[v % N];
+    if (o.rank == p.strips - 1 && p.dstate) p.dstate[o.b * p.width + o.c + v] = e.v[v];
+    p.dpart[(o.b * p.strips + o.rank) * p.width + o.c + v] = V == C::N ? acc.v[v] : acc.v[0] + acc.v[C::N - 1];
   }
 }
 
 template <class T, int V, int L, bool kMask, bool kBulk>
-__global__ void __launch_bounds__(32 * kStrips) backward_kernel(const __grid_constant__ Args p,
+__global__ void __launch_bounds__(V == 2 ? 32 : 32 * backward_strips(kBulk, kMask, sizeof(T)),
+                                  V == 2 ? (kBulk ? 12 : 8) : backward_ctas(backward_strips(kBulk, kMask, sizeof(T)), kBulk, kMask, sizeof(T)))
+    backward_kernel(const __grid_constant__ Args p,
                                                                 const __grid_constant__ Maps m) {
-  using Q = Pairing<V, L>;
   let_next_start();
   const Lane o = lane_of<V, L, kMask, true>(p);
   auto ring = backward_ring<T, V, L, kBulk, false>(p, m, o);
-  Vec<Q::N> rate[Q::P];
-  if (rates<V, Q::N>(p, o, rate))
+  Vec<V> rate;
+  if (rates<V>(p, o, rate))
     backward_strip<T, V, L, kMask, true>(p, o, ring, rate);
   else
     backward_strip<T, V, L, kMask, false>(p, o, ring, rate);

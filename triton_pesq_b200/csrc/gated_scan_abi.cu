@@ -77,17 +77,6 @@ constexpr int64_t kWarpsForPairs = 148 * 12;
 constexpr int kFewestSteps = 32;
 constexpr int64_t kFewestBulk = 32;
 
-// What an SM holds by registers and shared memory, as CTAs of so many warps: cut rows
-// make one wave of them
-struct Resident {
-  int ctas, warps;
-};
-Resident resident(bool bulk, bool backward, bool mask, int dtype) {
-  if (!backward) return bulk ? Resident{3, 8} : Resident{2, 8};
-  if (!bulk) return Resident{3, 4};
-  return mask ? Resident{2, 4} : dtype == PESQ_F32 ? Resident{3, 4} : Resident{2, 8};
-}
-
 // Whether boxes can be copied: 16-byte addresses and strides, which a tensor map asks for
 bool boxes(const pesq_stream& s, const pesq_gated_scan_desc& d) {
   const int64_t e = element(d.dtype), most = INT64_C(1) << 39;
@@ -125,9 +114,16 @@ Geometry geometry(const pesq_gated_scan_desc& d, bool backward) {
   g.chunk = d.steps == 1 ? 1 : chunk_steps(g.vec, g.bulk);
   const int64_t chunks = (d.steps + g.chunk - 1) / g.chunk, warps = d.batch * g.ctiles;
   int64_t strips = 1;
-  const Resident sm = resident(g.bulk, backward, d.reset || d.lengths, d.dtype);
   if (warps < kWarpsEnough) {
-    strips = std::max<int64_t>(1, 148 * sm.ctas / warps) * sm.warps;
+    // one wave, in CTAs of four or eight strips: the more strips that gives, and eight where they are as many, since
+    // a strip goes through all the CTAs before its own
+    const bool mask = d.reset || d.lengths;
+    const int size = (int)element(d.dtype);
+    for (int w = 4; w <= (backward ? backward_strips(g.bulk, mask, size) : 8); w *= 2) {
+      const int ctas = backward ? backward_ctas(w, g.bulk, mask, size) : forward_ctas(w, g.bulk, size);
+      const int64_t n = std::max<int64_t>(1, 148 * ctas / warps) * w;
+      if (n >= strips) strips = n, g.warps = w;
+    }
     strips = std::max<int64_t>(1, std::min(strips, (d.steps + kFewestSteps - 1) / kFewestSteps));
   }
   g.row = !backward && g.vec == 1 && warps < kWarpsEnough && d.steps > kHeld && d.steps <= kHeld * kRowWarps;
@@ -135,8 +131,13 @@ Geometry geometry(const pesq_gated_scan_desc& d, bool backward) {
   const int64_t per = g.row ? kHeld / g.chunk : (chunks + strips - 1) / strips;
   g.strips = (int)((chunks + per - 1) / per);
   g.strip = (int)(per * g.chunk);
-  g.warps = g.row ? g.strips : std::min(g.strips, sm.warps);
+  g.warps = g.row ? g.strips : std::max(1, std::min(g.strips, g.warps));
   return g;
+}
+
+// A result, dense: as aligned as its way out wants it
+bool fits(const void* p, const Geometry& g, const pesq_gated_scan_desc& d) {
+  return g.bulk ? reinterpret_cast<uintptr_t>(p) % 16 == 0 : fits(p, g.vec, d);
 }
 
 // (a step stride of 0: one row of zeros, and what lies outside a map reads as zero)
@@ -238,6 +239,10 @@ int run(const pesq_gated_scan_desc& d, Args& a, const Geometry& g, const pesq_st
     if (!encode(m.x, d.x, d, g) || !encode(m.ig, d.input_gate, d, g) || !encode(m.rg, d.decay_gate, d, g) ||
         (backward && !encode(m.dy, *dy, d, g)))
       return set_error(PESQ_ERR_CUDA, "cuTensorMapEncodeTiled failed");
+    void* out[3] = {a.drg, a.dig, backward ? a.dx : a.y};
+    for (int i = backward ? 0 : 2; i < 3 && d.dtype != PESQ_F32 && !g.row; ++i)
+      if (!encode(m.out[i], {out[i], d.steps * d.width, d.width}, d, g))
+        return set_error(PESQ_ERR_CUDA, "cuTensorMapEncodeTiled failed");
   }
   const cudaError_t e = d.dtype == PESQ_F32    ? launch<float>(a, m, g, backward, mask, s)
                         : d.dtype == PESQ_BF16 ? launch<__nv_bfloat16>(a, m, g, backward, mask, s)
@@ -264,7 +269,7 @@ int pesq_gated_scan_forward(const pesq_gated_scan_desc* d, void* stream, void* y
   if (const int status = check(d)) return status;
   if (!y || !last) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL output");
   const Geometry g = geometry(*d, false);
-  if (!fits(y, g.vec, *d)) return set_error(PESQ_ERR_INVALID_ARGUMENT, "y is less aligned than the inputs");
+  if (!fits(y, g, *d)) return set_error(PESQ_ERR_INVALID_ARGUMENT, "y is less aligned than the inputs");
   if (missing(workspace, workspace_bytes, map_bytes(*d, g)) || (kept && missing(kept, kept_size, kept_bytes(*d, g))))
     return set_error(PESQ_ERR_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
   Args a{};
@@ -281,8 +286,8 @@ int pesq_gated_scan_backward(const pesq_gated_scan_desc* d, void* stream, const 
   if (const int status = check(d)) return status;
   if (!dx || !dinput_gate || !ddecay_gate || !ddecay) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL output");
   const Geometry g = geometry(*d, true);
-  if ((dy.data && (g.bulk ? !boxes(dy, *d) : !fits(dy, g.vec, *d))) || !fits(dx, g.vec, *d) || !fits(dinput_gate, g.vec, *d) ||
-      !fits(ddecay_gate, g.vec, *d))
+  if ((dy.data && (g.bulk ? !boxes(dy, *d) : !fits(dy, g.vec, *d))) || !fits(dx, g, *d) || !fits(dinput_gate, g, *d) ||
+      !fits(ddecay_gate, g, *d))
     return set_error(PESQ_ERR_INVALID_ARGUMENT, "a gradient is less aligned than the inputs");
   if (missing(kept, kept_size, kept_bytes(*d, g)))
     return set_error(PESQ_ERR_WORKSPACE, "the states that the forward kept are missing");

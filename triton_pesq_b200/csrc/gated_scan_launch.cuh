@@ -32,21 +32,25 @@ cudaError_t start(K kernel, const Args& p, const Maps& m, const Geometry& g, siz
 
 template <class T, int V, int L, bool kMask, bool kBulk>
 cudaError_t launch_vl(const Args& p, const Maps& m, const Geometry& g, bool backward, cudaStream_t s) {
+  constexpr bool kCuts = V == 1 && L > 1;  // only such rows are cut
+  const bool cut = kCuts && g.strips > 1;
   cudaError_t e = cudaSuccess;
-  const bool cut = g.strips > 1;
   if (!backward) {
-    const size_t smem = kBulk ? Ring<T, V, L, 3, false>::kBytes : 0;
-    if constexpr (V == 1 && L > 1) {
+    const size_t smem = kBulk ? Ring<T, V, L, 3, false, true>::kBytes : 0;
+    if constexpr (kCuts) {
       if (g.row) return start(forward_row_kernel<T, L, kMask, kBulk>, p, m, g, smem, false, s);
+      if (cut) e = start(forward_maps_kernel<T, L, kMask, kBulk>, p, m, g, smem, false, s);
     }
-    if (cut) e = start(forward_maps_kernel<T, V, L, kMask, kBulk>, p, m, g, smem, false, s);
     return e != cudaSuccess ? e : start(forward_kernel<T, V, L, kMask, kBulk>, p, m, g, smem, cut, s);
   }
-  if (cut)
-    e = start(backward_maps_kernel<T, V, L, kMask, kBulk>, p, m, g, kBulk ? Ring<T, V, L, 2, false>::kBytes : 0, false, s);
-  return e != cudaSuccess
-             ? e
-             : start(backward_kernel<T, V, L, kMask, kBulk>, p, m, g, kBulk ? Ring<T, V, L, 4, true>::kBytes : 0, cut, s);
+  if constexpr (kCuts) {
+    if (cut)
+      e = start(backward_maps_kernel<T, L, kMask, kBulk>, p, m, g, kBulk ? Ring<T, 1, L, 2, false, false>::kBytes : 0,
+                false, s);
+  }
+  return e != cudaSuccess ? e
+                          : start(backward_kernel<T, V, L, kMask, kBulk>, p, m, g,
+                                  kBulk ? Ring<T, V, L, 4, true, true>::kBytes : 0, cut, s);
 }
 
 template <class T, int V>
