@@ -67,10 +67,27 @@ def test_gated_scan_entry_checks_its_descriptor():
     assert lib.pesq_gated_scan_forward(ctypes.byref(d), None, None, one, None, 0, one, 1 << 30) == 1
     assert lib.pesq_gated_scan_forward(ctypes.byref(d), None, one, one, None, 0, one, 1 << 30) == 1
     assert "NULL" in _lib.last_error()
-    assert lib.pesq_gated_scan_forward(ctypes.byref(d), None, one, one, None, 0, None, 0) == _lib.PESQ_ERR_WORKSPACE
+    long = _scan(steps=1000)  # cut into strips; 100 steps go through one CTA, which needs no workspace
+    assert _sizes(d)[1][0] == 0 and _sizes(long)[1][0] > 0
+    assert lib.pesq_gated_scan_forward(ctypes.byref(long), None, one, one, None, 0, None, 0) == _lib.PESQ_ERR_WORKSPACE
     dy = _lib.Stream(data=None, batch_stride=0, step_stride=0)
     assert lib.pesq_gated_scan_backward(ctypes.byref(d), None, None, 0, dy, None, one, one, one, one, None, one,
                                         1 << 30) == _lib.PESQ_ERR_WORKSPACE
+
+
+def test_gated_scan_entry_checks_what_boxes_need_of_results():
+    """Streams that are copied in boxes ask for results that are 16-byte aligned."""
+    lib = _lib.library()
+    one, off = ctypes.c_void_p(16), ctypes.c_void_p(24)
+    dense = _lib.Stream(data=16, batch_stride=100 * 64, step_stride=64)
+    d = _scan(x=dense, input_gate=dense, decay_gate=dense)
+    assert lib.pesq_gated_scan_forward(ctypes.byref(d), None, off, one, None, 0, one, 1 << 30) == 1
+    assert "aligned" in _lib.last_error()
+    for k in range(3):
+        out = [off if i == k else one for i in range(3)]
+        assert lib.pesq_gated_scan_backward(ctypes.byref(d), None, one, 1 << 30, dense, None, *out, one, None, one,
+                                            1 << 30) == 1
+        assert "aligned" in _lib.last_error()
 
 
 def test_gated_scan_keeps_one_state_a_chunk():

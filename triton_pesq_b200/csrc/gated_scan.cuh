@@ -11,20 +11,36 @@
 // A warp owns V neighbouring channels per lane and a strip of consecutive steps,
 // and walks the strip in chunks of 8 or 16 steps with the state in registers:
 // everything of a step but one multiply-add is independent of the steps before it,
-// so a chunk's gates are worked out side by side, while the elements of the chunks
-// to come are on their way.  Warps wait for nobody but their own copies: no flag, no
-// atomic, and the order of every operation is fixed.
+// so a chunk's gates are worked out side by side, two steps (or channels) an instruction, while
+// the elements of the chunks to come are on their way.  Warps wait for nobody but their own
+// copies: no flag, no atomic, and the order of every operation is fixed.
 //
 // Elements come in two ways.  Where channels and strides allow (multiples of 16
-// bytes), a warp's chunks are boxes of 64 channels x 8 steps, or 32 x 16, that tensor copies bring to
-// a ring in shared memory: one instruction for a box, no registers held.  Otherwise every lane loads its own elements a chunk ahead.
+// bytes) and the row has 16 steps, a warp's chunks are boxes of 64 channels x 8 steps, or 32 x 16,
+// that tensor copies bring to a ring in shared memory: one instruction for a box, no registers held.
+// Otherwise every lane loads its own elements a chunk ahead (64 x 500 x 896 bfloat16: 86 us so, 77 by
+// boxes; copies of 4 bytes a lane to shared memory: 259 us where plain loads take 95).
 //
 // With rows and channels enough to fill the device a strip is the whole row,
 // and the data pass once.  Otherwise rows are cut into strips: the recurrence is
 // the composition of maps h -> A h + H, a first kernel (`maps`) works out every
-// strip's (A, H), and the second starts each strip from the state that the maps
-// before it give.  The strips of a CTA meet in shared memory, so a strip composes
-// the maps of the CTAs before its own and one more.
+// strip's (A, H), and the second, launched while the first still runs and waiting for its end, starts
+// each strip from the state that the maps before it give.  The strips of a CTA meet in shared memory,
+// so a strip composes the maps of the CTAs before its own and one more.  Rows of 33 to 512 steps that
+// would be cut go through one CTA of one launch instead, which holds its steps as (a, b) in registers.
+//
+// What bounds it.  The bytes, 4 elements a step forward and 7 backward, are the floor; an element
+// also takes 40 instruction slots forward and 65 backward, 5 of them special functions at a
+// quarter of the lanes a cycle.  With n warps a scheduler of 32 chunks each the time is 28 + 11 n us
+// forward and 36 + 18 n backward: a warp's work on every pipe in turn, of which n warps overlap the rest.
+// Measured (B200, cold caches, share of the bytes at the measured copy rate):
+//   64 x 500 x 896 bfloat16, uncut            forward 72 us, 49 %; backward 109 us, 57 %
+//   96 x 512 x 512 float32, uncut             forward 66 us, 93 %
+//   16 x 1000 x 512 float32, cut, boxes       forward 48 us, 42 %; backward 60 us, 58 %
+//   6 x 4001 x 385 float32, cut, plain loads  forward 62 us, 36 %; backward 87 us, 45 %
+//   1 x 32768 x 1040 bfloat16, cut, boxes     forward 124 us, 34 %; backward 146 us, 50 %
+//   8 x 500 x 768 bfloat16, one CTA a row     forward 21 us, 18 % (launch and one walk through the row)
+// (cut rows read the gates twice, which the floor does not count).
 //
 // Backward.  With g_t = dL/dh_t: g_t = dy_t + a_{t+1} g_{t+1}, the same kind of
 // scan from the end of the row, carried as e_t = a_t g_t.  Then
@@ -33,7 +49,7 @@
 //   ddecay = -rate sigmoid(decay) sum over rows and steps of dlog a r.
 // h is not read back from the rounded y: the forward keeps the state before every
 // chunk in 32 bits (1 / 8 or 1 / 16 of the elements), and the backward recomputes the
-// chunk from it.  beta -> 0 only together with log a, whose quotient goes to
+// chunk from it, by the same operations.  beta -> 0 only together with log a, whose quotient goes to
 // zero: the term is dropped there.
 #pragma once
 
@@ -137,7 +153,7 @@ constexpr float kNear = 0.25f;
 template <int N, int G>
 struct Gates {
   Vec<N> i[G], r[G], a[G], beta[G];
-  Vec<N> s[G];  // 1 / beta, or 1 / sqrt(kTiny) where beta is zero
+  Vec<N> s[G];  // 1 / beta; where beta is zero, 1 / sqrt(kTiny), which its uses multiply by beta
 };
 
 // The gates of G Vecs side by side: operation by operation rather than Vec by
@@ -179,8 +195,8 @@ __device__ __forceinline__ void decays(const Vec<N> (&r)[G], Vec<N> k, Vec<N> (&
   }
 }
 
-// 1 / (1 + exp(-v)); a reciprocal for each: one for the product of two would need
-// both exponentials to be held below overflow, which costs more
+// 1 / (1 + exp(-v)); a reciprocal for each: one for the product of two needs both
+// exponentials held below overflow, five operations more (64 x 500 x 896: 77 us, and 73 so)
 template <int N, int G>
 __device__ __forceinline__ void sigmoids(const Vec<N> (&v)[G], Vec<N> (&out)[G]) {
 #pragma unroll
@@ -241,11 +257,13 @@ template <int V, int L, bool kMask, bool kBack>
 __device__ __forceinline__ Lane lane_of(const Args& p) {
   Lane o;
   o.b = blockIdx.y;
-  const unsigned block = blockIdx.x / p.ctiles;  // CTA along the row
-  o.c = (int64_t)(blockIdx.x - block * p.ctiles) * (32 * V) + threadIdx.x * V;
+  const unsigned block = L == 1 ? 0 : blockIdx.x / p.ctiles;  // CTA along the row
+  // (a CTA's warps are strips of the row, but for single steps, which have none: neighbours in the channels)
+  const unsigned tile = L == 1 ? blockIdx.x * blockDim.y + threadIdx.y : blockIdx.x - block * p.ctiles;
+  o.c = (int64_t)tile * (32 * V) + threadIdx.x * V;
   o.on = o.c < p.width;
   o.from = o.on ? o.c : 0;
-  o.rank = block * blockDim.y + threadIdx.y;
+  o.rank = L == 1 ? 0 : block * blockDim.y + threadIdx.y;
   const int strip = kBack ? p.strips - 1 - o.rank : o.rank, steps = (int)p.steps;
   const int all = (steps + L - 1) / L;
   int per = p.strip / L;
@@ -484,7 +502,8 @@ __device__ __forceinline__ void zero_rest(const Args& p, const Lane& o, void* co
   for (int v = 0; v < V; ++v) z.v[v] = narrow<T>(0.0f);
   // (they lie at one end of the row)
   const int base = o.lo > 0 ? 0 : o.hi, per = (dead + p.strips - 1) / p.strips;
-  const int s0 = min((int)p.steps, min(base + dead, base + o.rank * per) * L), s1 = min((int)p.steps, min(base + dead, base + (o.rank + 1) * per) * L);
+  const int s0 = min((int)p.steps, min(base + dead, base + o.rank * per) * L);
+  const int s1 = min((int)p.steps, min(base + dead, base + (o.rank + 1) * per) * L);
   const int64_t t = p.reverse ? p.steps - 1 - s0 : s0, step = o.dir * p.width;
   const int64_t at = (o.b * p.steps + t) * p.width + o.c;
 #pragma unroll
@@ -515,7 +534,8 @@ __device__ __forceinline__ void walk(int n, R read, W work) {
 // A warp's ring of chunks in shared memory: kRing stages of S streams' boxes
 // [L][32 V] and, with kState, the states before the chunk.  With kOut, 16-bit results take the place
 // of the inputs in their stage and leave by tensor copies as well, which saves a thread their
-// addresses; the stage is filled again a chunk later.
+// addresses (64 x 500 x 896: backward 114 -> 109 us); the stage is filled again a chunk later.  32-bit
+// rings have two stages only, and their results leave from the registers.
 template <class T, int V, int L, int S, bool kState, bool kOut>
 struct Ring {
   static constexpr bool kStaged = kOut && sizeof(T) == 2;
@@ -727,8 +747,8 @@ __device__ __forceinline__ auto forward_ring(const Args& p, const Maps& m, const
 }
 
 template <class T, int L, bool kMask, bool kBulk>
-__global__ void __launch_bounds__(32 * kStrips, forward_ctas(8, kBulk, sizeof(T))) forward_maps_kernel(const __grid_constant__ Args p,
-                                                                    const __grid_constant__ Maps m) {
+__global__ void __launch_bounds__(32 * kStrips, forward_ctas(8, kBulk, sizeof(T)))
+    forward_maps_kernel(const __grid_constant__ Args p, const __grid_constant__ Maps m) {
   let_next_start();
   const Lane o = lane_of<1, L, kMask, false>(p);
   auto ring = forward_ring<T, 1, L, kBulk, false>(p, m, o);
@@ -787,8 +807,9 @@ __device__ __forceinline__ void forward_strip(const Args& p, const Lane& o, R& r
 }
 
 template <class T, int V, int L, bool kMask, bool kBulk>
-__global__ void __launch_bounds__(V == 2 ? 32 : 32 * kStrips, V == 2 ? (kBulk ? 16 : 11) : forward_ctas(8, kBulk, sizeof(T))) forward_kernel(const __grid_constant__ Args p,
-                                                               const __grid_constant__ Maps m) {
+__global__ void __launch_bounds__(V == 2 && L > 1 ? 32 : 32 * kStrips,
+                                  V == 2 && L > 1 ? (kBulk ? 16 : 11) : forward_ctas(8, kBulk, sizeof(T)))
+    forward_kernel(const __grid_constant__ Args p, const __grid_constant__ Maps m) {
   const Lane o = lane_of<V, L, kMask, false>(p);
   auto ring = forward_ring<T, V, L, kBulk, true>(p, m, o);
   Vec<V> rate;
@@ -800,7 +821,9 @@ __global__ void __launch_bounds__(V == 2 ? 32 : 32 * kStrips, V == 2 ? (kBulk ? 
 
 // A short row in one CTA: a warp holds its strip of kHeld steps as (a, b) in registers,
 // the strips' maps meet in shared memory, and the recursion is run from the state that
-// they give.  The data pass once, in one launch.
+// they give.  The data pass once, in one launch: 24 x 187 x 896 bfloat16 14.1 us, where strips in
+// two launches take 18.2.  With more rows than fill the device whole rows a warp are as good:
+// 32 x 500 x 896 47.6 us so, 45.7 as whole rows.
 template <class T, int L, bool kMask, bool kFar, class R>
 __device__ __forceinline__ void forward_row(const Args& p, const Lane& o, R& ring, Vec<1> rate) {
   using C = Cells<1, L>;
@@ -1022,8 +1045,8 @@ __global__ void __launch_bounds__(32 * kStrips) backward_maps_kernel(const __gri
 //   P1 = beta i, P2 = x (1 - i), R1 = r (a h_{t-1} - (a / beta)^2 b), R2 = rate (r - 1),
 // with b = beta i x, and s sums up to the decay gradient.
 template <class T, int V, int L, bool kMask, bool kFar, bool kFull, class R>
-__device__ __forceinline__ void backward_chunk(const Args& p, const Lane& o, const R& ring, int k, LoadedBack<T, V, L>& in,
-                                               Vec<V> rate, Vec<V>& e, Vec<Cells<V, L>::N>& acc) {
+__device__ __forceinline__ void backward_chunk(const Args& p, const Lane& o, const R& ring, int k,
+                                               LoadedBack<T, V, L>& in, Vec<V> rate, Vec<V>& e, Vec<Cells<V, L>::N>& acc) {
   using C = Cells<V, L>;
   constexpr int N = C::N, G = C::G;
   const Vec<N> minus = splat<N>(-1.0f);
@@ -1138,10 +1161,13 @@ __device__ __forceinline__ void backward_strip(const Args& p, const Lane& o, R& 
 }
 
 template <class T, int V, int L, bool kMask, bool kBulk>
-__global__ void __launch_bounds__(V == 2 ? 32 : 32 * backward_strips(kBulk, kMask, sizeof(T)),
-                                  V == 2 ? (kBulk ? 12 : 8) : backward_ctas(backward_strips(kBulk, kMask, sizeof(T)), kBulk, kMask, sizeof(T)))
-    backward_kernel(const __grid_constant__ Args p,
-                                                                const __grid_constant__ Maps m) {
+__global__ void __launch_bounds__(L == 1   ? 32 * kStrips
+                                  : V == 2 ? 32
+                                           : 32 * backward_strips(kBulk, kMask, sizeof(T)),
+                                  L == 1   ? 2
+                                  : V == 2 ? (kBulk ? 12 : 8)
+                                           : backward_ctas(backward_strips(kBulk, kMask, sizeof(T)), kBulk, kMask, sizeof(T)))
+    backward_kernel(const __grid_constant__ Args p, const __grid_constant__ Maps m) {
   let_next_start();
   const Lane o = lane_of<V, L, kMask, true>(p);
   auto ring = backward_ring<T, V, L, kBulk, false>(p, m, o);

@@ -69,13 +69,34 @@ bool fits(const pesq_stream& s, int vec, const pesq_gated_scan_desc& d) {
          (d.steps == 1 || s.step_stride % vec == 0);
 }
 
-// Rows and channels that make this many warps are not cut
-constexpr int64_t kWarpsEnough = 148 * 4;
-// and that many take pairs of channels
-constexpr int64_t kWarpsForPairs = 148 * 12;
-// the fewest steps of a strip, and of a row that is copied in boxes
-constexpr int kFewestSteps = 32;
-constexpr int64_t kFewestBulk = 32;
+// Rows and channels that make this many warps are not cut: their cost is a row's walk, cut ones' the
+// work of both kernels.  Forward and backward, whole / cut (us):
+//   float32 in boxes    308 x 2000 steps: 122 / 132, 169 / 151;  448 x 2000: 122 / 155, 173 / 196
+//   bfloat16 in boxes   448 x 2000: 128 / 124, 190 / 144;  672 x 2000: 148 / 151, 230 / 192;
+//                       896 x 2000: 149 / 200, 232 / 243
+//   float32 by lanes    520 x 2000: 204 / 175, 300 / 298;  624 x 2000: 212 / 224, 320 / 325
+//   bfloat16 by lanes   624 x 2000: 196 / 194, 282 / 239;  832 x 2000: 201 / 222, 292 / 271
+int64_t warps_enough(bool bulk, bool backward, int size) {
+  return backward && size == 2 ? 148 * 5 : bulk && size == 4 ? 148 * 5 / 2 : 148 * 4;
+}
+// Short rows go through one CTA each up to so many warps; that / a warp a row, us:
+//   float32 in boxes 308 x 500: 31 / 36, 448 x 500: 38 / 38;  bfloat16 448 x 500: 35 / 40, 560 x 500: 40 / 40
+int64_t warps_for_rows(bool bulk, int size) { return bulk && size == 4 ? 148 * 3 : 148 * 4; }
+// Rows and channel pairs that make so many warps take pairs of channels (forward and backward, pairs / single, us):
+//   float32 in boxes    672 x 500: 73 / 69, 118 / 131;  896 x 500: 81 / 94, 153 / 163;  3584 x 500: 302 / 322, 562 / 588
+//   float32 by lanes    1792 x 500: 202 / 175, 318 / 360;  2688 x 500: 259 / 255, 474 / 512
+//   bfloat16 by lanes   1792 x 500: 156 / 144, 226 / 262;  2688 x 500: 177 / 200, 316 / 354
+//   bfloat16 in boxes   4096 x 24: 23 / 27, 34 / 42;  4096 x 96: 49 / 52, 81 / 81;  4096 x 256: 111 / 113, 194 / 181;
+//                       1792 x 500: 122 / 114, 210 / 181
+int64_t warps_for_pairs(bool bulk, int size, int64_t steps) {
+  return bulk && size == 4 ? 148 * 5 : !bulk || steps < 96 ? 148 * 12 : INT64_MAX;
+}
+// The fewest steps of a strip (2 x 256 x 512, backward: 13.4 us, 15.1 with 32), and of a row that is copied
+// in boxes (512 x 24 x 512 bfloat16: 21.6 and 33.6 us, by lanes 25.6 and 37.9)
+constexpr int kFewestSteps = 16;
+constexpr int64_t kFewestBulk = 16;
+// Single steps: so many warps go in CTAs of eight, fewer in CTAs of one, which spread better
+constexpr int64_t kWarpsAtOnce = 148 * 32;
 
 // Whether boxes can be copied: 16-byte addresses and strides, which a tensor map asks for
 bool boxes(const pesq_stream& s, const pesq_gated_scan_desc& d) {
@@ -101,24 +122,23 @@ EncodeTiled encoder() {
 }
 
 // Chunks follow from the inputs alone, so that a backward call takes its forward's.
-// Pairs of channels where everything allows it and leaves warps enough.
 Geometry geometry(const pesq_gated_scan_desc& d, bool backward) {
   Geometry g{};
-  g.bulk = d.steps >= kFewestBulk && d.width * (int64_t)element(d.dtype) % 16 == 0 && boxes(d.x, d) &&
+  const int size = (int)element(d.dtype);
+  g.bulk = d.steps >= kFewestBulk && d.width * (int64_t)size % 16 == 0 && boxes(d.x, d) &&
            boxes(d.input_gate, d) && boxes(d.decay_gate, d);
-  g.vec = d.width % 2 == 0 && d.batch * ((d.width + 63) / 64) >= kWarpsForPairs && fits(d.x, 2, d) &&
-                  fits(d.input_gate, 2, d) && fits(d.decay_gate, 2, d)
-              ? 2
-              : 1;
+  const bool pairs = d.width % 2 == 0 && fits(d.x, 2, d) && fits(d.input_gate, 2, d) && fits(d.decay_gate, 2, d);
+  g.vec = pairs && d.batch * ((d.width + 63) / 64) >= warps_for_pairs(g.bulk, size, d.steps) ? 2 : 1;
   g.ctiles = (int)((d.width + 32 * g.vec - 1) / (32 * g.vec));
   g.chunk = d.steps == 1 ? 1 : chunk_steps(g.vec, g.bulk);
   const int64_t chunks = (d.steps + g.chunk - 1) / g.chunk, warps = d.batch * g.ctiles;
   int64_t strips = 1;
-  if (warps < kWarpsEnough) {
+  g.row = !backward && g.vec == 1 && warps < warps_for_rows(g.bulk, size) && d.steps > kHeld &&
+          d.steps <= kHeld * kRowWarps;
+  if (!g.row && warps < warps_enough(g.bulk, backward, size)) {
     // one wave, in CTAs of four or eight strips: the more strips that gives, and eight where they are as many, since
     // a strip goes through all the CTAs before its own
     const bool mask = d.reset || d.lengths;
-    const int size = (int)element(d.dtype);
     for (int w = 4; w <= (backward ? backward_strips(g.bulk, mask, size) : 8); w *= 2) {
       const int ctas = backward ? backward_ctas(w, g.bulk, mask, size) : forward_ctas(w, g.bulk, size);
       const int64_t n = std::max<int64_t>(1, 148 * ctas / warps) * w;
@@ -126,12 +146,13 @@ Geometry geometry(const pesq_gated_scan_desc& d, bool backward) {
     }
     strips = std::max<int64_t>(1, std::min(strips, (d.steps + kFewestSteps - 1) / kFewestSteps));
   }
-  g.row = !backward && g.vec == 1 && warps < kWarpsEnough && d.steps > kHeld && d.steps <= kHeld * kRowWarps;
   if (g.row) strips = (d.steps + kHeld - 1) / kHeld;
   const int64_t per = g.row ? kHeld / g.chunk : (chunks + strips - 1) / strips;
   g.strips = (int)((chunks + per - 1) / per);
   g.strip = (int)(per * g.chunk);
-  g.warps = g.row ? g.strips : std::max(1, std::min(g.strips, g.warps));
+  g.warps = g.row                                     ? g.strips
+            : d.steps == 1 && warps > kWarpsAtOnce ? std::min(g.ctiles, kStrips)
+                                                   : std::max(1, std::min(g.strips, g.warps));
   return g;
 }
 
@@ -158,7 +179,8 @@ bool encode(CUtensorMap& m, const pesq_stream& s, const pesq_gated_scan_desc& d,
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 // maps of strips and of CTAs of strips
 size_t map_bytes(const pesq_gated_scan_desc& d, const Geometry& g) {
-  return g.strips == 1 || g.row ? 0 : round16((size_t)(d.batch * (g.strips + (g.strips + g.warps - 1) / g.warps) * d.width) * 8);
+  if (g.strips == 1 || g.row) return 0;
+  return round16((size_t)(d.batch * (g.strips + (g.strips + g.warps - 1) / g.warps) * d.width) * 8);
 }
 size_t kept_bytes(const pesq_gated_scan_desc& d, const Geometry& g) {
   return round16((size_t)(d.batch * ((d.steps + g.chunk - 1) / g.chunk) * d.width) * 4);

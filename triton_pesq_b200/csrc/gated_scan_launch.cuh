@@ -21,7 +21,8 @@ cudaError_t start(K kernel, const Args& p, const Maps& m, const Geometry& g, siz
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t c{};
-  c.gridDim = dim3((unsigned)(g.ctiles * ((g.strips + warps - 1) / warps)), (unsigned)p.batch);
+  const int tiles = g.chunk == 1 ? (g.ctiles + warps - 1) / warps : g.ctiles * ((g.strips + warps - 1) / warps);
+  c.gridDim = dim3((unsigned)tiles, (unsigned)p.batch);
   c.blockDim = dim3(32, warps);
   c.dynamicSmemBytes = smem;
   c.stream = s;

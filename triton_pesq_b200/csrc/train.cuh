@@ -112,17 +112,6 @@ __device__ __forceinline__ Vec<N> widen(const Pack<T, M>& p, int j) {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// A 64-bit word published from one CTA to another: a naturally aligned 64-bit
-// access is single-copy atomic, so a word that carries its own tag needs no fence.
-__device__ __forceinline__ void put_word(unsigned long long* p, unsigned long long v) {
-  asm volatile("st.relaxed.gpu.global.b64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
-}
-__device__ __forceinline__ unsigned long long get_word(const unsigned long long* p) {
-  unsigned long long v;
-  asm volatile("ld.relaxed.gpu.global.b64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
-  return v;
-}
-
 }  // namespace train
 
 int set_error(int code, const char* msg);
