@@ -22,6 +22,15 @@
 // registers over the rows of a CTA; the CTAs' sums are added up in a fixed order by a
 // second kernel.  The gradient of a gate that the steps of a batch item share is summed
 // the same way.
+//
+// A row's sums are two rounds of shuffles, and barriers where a team has several warps, that its
+// loads and stores overlap only by the other teams of the SM and by the next row's loads.
+// Measured (B200, cold caches, share of the bytes at the measured copy rate):
+//   64 x 500 x 896, stream and block bfloat16   forward 56 us, 78 %; backward 103 us, 68 %
+//   64 x 500 x 385, float32                     forward 48 us, 78 %; backward 81 us, 74 %
+//   100000 x 64, bfloat16                       forward 18.5 us, backward 32.8 us
+//   4000 x 8192, bfloat16                       backward 278 us, 30 % (sums in shared memory, no next row)
+//   8 x 500 x 768, stream float32               forward 10.4 us a call (floor 5.6), launch included
 #pragma once
 
 #include <type_traits>
@@ -62,8 +71,8 @@ struct Args {
   float *part_u, *part_pre, *part_gate;  // [batch * units, width]; part_gate null where the gate is not shared
 };
 
-// Backward rows of so many threads leave a thread too few registers to hold the vectors,
-// the sums and the next row: those come from cache, go to shared memory, and wait
+// Backward rows of so many threads leave a thread too few registers (128, and 64 with 1024 threads) to hold
+// the vectors, the sums and the next row: those come from cache, go to shared memory, and wait
 template <int TEAM>
 constexpr bool kLeanRow = TEAM >= 512;
 
