@@ -155,8 +155,8 @@ struct Eight {
     const int t = threadIdx.x % TEAM;
     return kWide ? t * kEach + j : t + j * TEAM;
   }
-  __device__ __forceinline__ void load(const void* base, int64_t row, int width, bool take) {
-    const T* r = static_cast<const T*>(base) + row;
+  __device__ __forceinline__ void load(const void* row, int width, bool take) {
+    const T* r = static_cast<const T*>(row);
     if (kWide) {
       take = take && column(0) < width;
       const uint4* q = reinterpret_cast<const uint4*>(r + column(0));
@@ -259,20 +259,42 @@ __device__ __forceinline__ void activate(const E& g, int silu, Vec<2> (&value)[k
   }
 }
 
-// The row that a team works on in its k-th turn, dense and for an operand
+// The rows that a team works on in turn: every TEAMS-th of its CTA's
 template <int TEAM, int THREADS>
-struct Turn {
-  int64_t b, t;
-  bool on;
-  __device__ __forceinline__ Turn(const Args& p, int k) {
+struct Turns {
+  static constexpr int kTeams = THREADS / TEAM;
+  int64_t b, t;  // the team's first row
+  int rows;      // of the CTA
+  __device__ __forceinline__ Turns(const Args& p) {
     b = blockIdx.x / p.units;
-    const int unit = blockIdx.x - (int)b * p.units;
-    const int in = k * (THREADS / TEAM) + threadIdx.x / TEAM;
-    t = (int64_t)unit * p.span + in;
-    on = in < p.span && t < p.steps;
+    const int64_t first = (blockIdx.x - b * p.units) * p.span;
+    rows = (int)min((int64_t)p.span, p.steps - first);
+    t = first + threadIdx.x / TEAM;
   }
-  __device__ __forceinline__ int64_t of(const Rows& r) const { return b * r.sb + t * r.st; }
+  __device__ __forceinline__ bool on(int k) const { return k * kTeams + (int)threadIdx.x / TEAM < rows; }
+  // the first row of a dense result
   __device__ __forceinline__ int64_t dense(const Args& p) const { return (b * p.steps + t) * p.width; }
+};
+// An operand's rows.  With 16-bit blocks whose channels lie eight by eight the row's address is
+// kept and moved on (64 x 500 x 896: forward 58.5 -> 56.4 us, backward 110 -> 105); the others have no registers left for it
+// (64 x 500 x 385 float32: backward 81 -> 91 us) and work it out every time.
+template <class TB, bool kWide>
+constexpr bool kRunning = kWide && sizeof(TB) == 2;
+template <class T, bool kRuns, int TEAM, int THREADS>
+struct Cursor {
+  const char* at;
+  __device__ __forceinline__ Cursor(const Rows& r, const Turns<TEAM, THREADS>& of) : at(place(r, of, 0)) {}
+  static __device__ __forceinline__ const char* place(const Rows& r, const Turns<TEAM, THREADS>& of, int k) {
+    const int64_t row = of.b * r.sb + (of.t + (int64_t)k * of.kTeams) * r.st;
+    return static_cast<const char*>(r.p) + row * (int64_t)sizeof(T);
+  }
+  // the row of turn k, turns one after the other
+  __device__ __forceinline__ const char* row(const Rows& r, const Turns<TEAM, THREADS>& of, int k) {
+    if (!kRuns) return place(r, of, k);
+    const char* now = at;
+    at += of.kTeams * r.st * (int64_t)sizeof(T);
+    return now;
+  }
 };
 
 // ------------------------------------------------------------------- forward
@@ -286,9 +308,9 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(false,
   __shared__ __align__(16) float s_sum[2][32][8];
   int turn = 0;
   F post, pre, scale;
-  pre.load(p.pre, 0, p.width, true);
-  post.load(p.post, 0, p.width, p.post != nullptr);
-  scale.load(p.scale, 0, p.width, p.scale != nullptr);
+  pre.load(p.pre, p.width, true);
+  post.load(p.post, p.width, p.post != nullptr);
+  scale.load(p.scale, p.width, p.scale != nullptr);
   if (p.scale) {
 #pragma unroll
     for (int j = 0; j < kEach; j += 2) post.set(j, post.at(j) * scale.at(j), post.at(j + 1) * scale.at(j + 1));
@@ -297,18 +319,23 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(false,
   const float inv = 1.0f / (float)p.width;
   S x;
   B z, g;
-  Turn<TEAM, THREADS> now(p, 0);
-  x.load(p.stream.p, now.of(p.stream), p.width, now.on);
-  z.load(p.block.p, now.of(p.block), p.width, now.on && p.block.p);
-  g.load(p.gate.p, now.of(p.gate), p.width, now.on && p.gate.p);
+  const Turns<TEAM, THREADS> turn_of(p);
+  Cursor<TS, kRunning<TB, kWide>, TEAM, THREADS> at_x(p.stream, turn_of);
+  Cursor<TB, kRunning<TB, kWide>, TEAM, THREADS> at_z(p.block, turn_of), at_g(p.gate, turn_of);
+  const auto load = [&](int k, bool on, S& x, B& z, B& g) {
+    x.load(at_x.row(p.stream, turn_of, k), p.width, on);
+    z.load(at_z.row(p.block, turn_of, k), p.width, on && p.block.p);
+    g.load(at_g.row(p.gate, turn_of, k), p.width, on && p.gate.p);
+  };
+  int64_t to = turn_of.dense(p);
+  bool on = turn_of.on(0);
+  load(0, on, x, z, g);
 #pragma unroll 1
   for (int k = 0; k < turns; ++k) {
-    const Turn<TEAM, THREADS> next(p, k + 1);
+    const bool on1 = turn_of.on(k + 1);
     S x1;
     B z1, g1;
-    x1.load(p.stream.p, next.of(p.stream), p.width, next.on);
-    z1.load(p.block.p, next.of(p.block), p.width, next.on && p.block.p);
-    g1.load(p.gate.p, next.of(p.gate), p.width, next.on && p.gate.p);
+    load(k + 1, on1, x1, z1, g1);
 
     constexpr int H = kEach / 2;
     Vec<2> r[H], total = splat<2>(0.0f);
@@ -340,15 +367,16 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(false,
     sum[0] = total.v[0] + total.v[1];
     team_sum<1, TEAM>(sum, s_sum, turn);
     const Vec<2> rr = splat<2>(rsqrt_approx(fmaf(sum[0], inv, p.eps)));
-    if (now.on) {
+    if (on) {
       S out;
       B y;
 #pragma unroll
       for (int i = 0; i < H; ++i) out.set(2 * i, r[i]), y.set(2 * i, r[i] * (rr * pre.two(2 * i)));
-      if (p.out_stream) out.store(p.out_stream, now.dense(p), p.width);
-      y.store(p.out_normed, now.dense(p), p.width);
+      if (p.out_stream) out.store(p.out_stream, to, p.width);
+      y.store(p.out_normed, to, p.width);
     }
-    x = x1, z = z1, g = g1, now = next;
+    x = x1, z = z1, g = g1, on = on1;
+    to += (int64_t)TEAMS * p.width;
   }
 }
 
@@ -390,11 +418,11 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(true, 
   int turn = 0;
   F post, pre;  // post times scale
   const auto vectors = [&] {
-    pre.load(p.pre, 0, p.width, true);
-    post.load(p.post, 0, p.width, p.post != nullptr);
+    pre.load(p.pre, p.width, true);
+    post.load(p.post, p.width, p.post != nullptr);
     if (p.scale) {
       F scale;
-      scale.load(p.scale, 0, p.width, true);
+      scale.load(p.scale, p.width, true);
 #pragma unroll
       for (int j = 0; j < kEach; j += 2) post.set(j, post.at(j) * scale.at(j), post.at(j + 1) * scale.at(j + 1));
     }
@@ -415,25 +443,30 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(true, 
   const float inv = 1.0f / (float)p.width;
   S x, ds;
   B z, g, dy;
-  const auto load = [&](const Turn<TEAM, THREADS>& at, S& x, S& ds, B& z, B& g, B& dy) {
-    z.load(p.block.p, at.of(p.block), p.width, at.on && p.block.p);
-    g.load(p.gate.p, at.of(p.gate), p.width, at.on && p.gate.p);
-    x.load(p.stream.p, at.of(p.stream), p.width, at.on);
-    dy.load(p.dnormed.p, at.of(p.dnormed), p.width, at.on && p.dnormed.p);
-    ds.load(p.dstream.p, at.of(p.dstream), p.width, at.on && p.dstream.p);
+  const Turns<TEAM, THREADS> turn_of(p);
+  Cursor<TS, kRunning<TB, kWide>, TEAM, THREADS> at_x(p.stream, turn_of), at_ds(p.dstream, turn_of);
+  Cursor<TB, kRunning<TB, kWide>, TEAM, THREADS> at_z(p.block, turn_of), at_g(p.gate, turn_of),
+      at_dy(p.dnormed, turn_of);
+  const auto load = [&](int k, bool on, S& x, S& ds, B& z, B& g, B& dy) {
+    z.load(at_z.row(p.block, turn_of, k), p.width, on && p.block.p);
+    g.load(at_g.row(p.gate, turn_of, k), p.width, on && p.gate.p);
+    x.load(at_x.row(p.stream, turn_of, k), p.width, on);
+    dy.load(at_dy.row(p.dnormed, turn_of, k), p.width, on && p.dnormed.p);
+    ds.load(at_ds.row(p.dstream, turn_of, k), p.width, on && p.dstream.p);
   };
-  Turn<TEAM, THREADS> now(p, 0);
-  if (!kLean) load(now, x, ds, z, g, dy);
+  int64_t to = turn_of.dense(p);
+  bool on = turn_of.on(0);
+  if (!kLean) load(0, on, x, ds, z, g, dy);
 #pragma unroll 1
   for (int k = 0; k < turns; ++k) {
-    const Turn<TEAM, THREADS> next(p, k + 1);
+    const bool on1 = turn_of.on(k + 1);
     S x1, ds1;
     B z1, g1, dy1;
     if (kLean) {
-      load(now, x, ds, z, g, dy);
+      load(k, on, x, ds, z, g, dy);
       vectors();
     } else {
-      load(next, x1, ds1, z1, g1, dy1);
+      load(k + 1, on1, x1, ds1, z1, g1, dy1);
     }
 
     float rz = 0.0f;
@@ -443,7 +476,7 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(true, 
       for (int i = 0; i < H; ++i) total = fma(z.two(2 * i), z.two(2 * i), total);
       float one[1] = {total.v[0] + total.v[1]};
       team_sum<1, TEAM>(one, s_sum, turn);
-      rz = now.on ? rsqrt_approx(fmaf(one[0], inv, p.eps)) : 0.0f;
+      rz = on ? rsqrt_approx(fmaf(one[0], inv, p.eps)) : 0.0f;
     }
     // sums of r^2, q r, ds w, q w, r w
     Vec<2> value[H], slope[H], w[H], part[5];
@@ -470,7 +503,7 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(true, 
     for (int k5 = 0; k5 < 5; ++k5) sum[k5] = part[k5].v[0] + part[k5].v[1];
     team_sum5<TEAM>(sum, s_sum, turn);
     // (a row that is off is zeros, and adds zeros for any eps)
-    const float rr = now.on ? rsqrt_approx(fmaf(sum[0], inv, p.eps)) : 0.0f;
+    const float rr = on ? rsqrt_approx(fmaf(sum[0], inv, p.eps)) : 0.0f;
     const float mq = sum[1] * inv * rr * rr;                        // mean(q h) / rms
     const float mw = (sum[2] + rr * (sum[3] - mq * sum[4])) * inv;  // mean(dr w)
     Vec<2> dx[H], dz[H], dg[H];
@@ -492,26 +525,26 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(true, 
         acc_gate[i] = acc_gate[i] + dg[i];
       }
     }
-    if (now.on) {
-      const int64_t at = now.dense(p);
+    if (on) {
       S a;
       B b;
 #pragma unroll
       for (int i = 0; i < H; ++i) a.set(2 * i, dx[i]);
-      a.store(p.dx, at, p.width);
+      a.store(p.dx, to, p.width);
       if (p.dblock) {
 #pragma unroll
         for (int i = 0; i < H; ++i) b.set(2 * i, dz[i]);
-        b.store(p.dblock, at, p.width);
+        b.store(p.dblock, to, p.width);
       }
       if (p.dgate) {
 #pragma unroll
         for (int i = 0; i < H; ++i) b.set(2 * i, dg[i]);
-        b.store(p.dgate, at, p.width);
+        b.store(p.dgate, to, p.width);
       }
     }
     if (!kLean) x = x1, ds = ds1, z = z1, g = g1, dy = dy1;
-    now = next;
+    on = on1;
+    to += (int64_t)TEAMS * p.width;
   }
   if (kLean) {
 #pragma unroll
