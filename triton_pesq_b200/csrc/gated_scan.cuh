@@ -30,12 +30,12 @@
 // would be cut go through one CTA of one launch instead, which holds its steps as (a, b) in registers.
 //
 // What bounds it.  The bytes, 4 elements a step forward and 7 backward, are the floor; an element
-// also takes 40 instruction slots forward and 65 backward, 5 of them special functions at a
-// quarter of the lanes a cycle.  With n warps a scheduler of 32 chunks each the time is 28 + 11 n us
+// also takes 40 instruction slots forward and 65 backward, 5 of them special functions of eight
+// cycles a warp.  With n warps a scheduler of 32 chunks each the time is 28 + 11 n us
 // forward and 36 + 18 n backward: a warp's work on every pipe in turn, of which n warps overlap the rest.
 // Measured (B200, cold caches, share of the bytes at the measured copy rate):
 //   64 x 500 x 896 bfloat16, uncut            forward 72 us, 49 %; backward 109 us, 57 %
-//   96 x 512 x 512 float32, uncut             forward 66 us, 93 %
+//   96 x 512 x 512 float32, uncut, pairs      forward 77 us, 80 %; backward 138 us, 78 %
 //   16 x 1000 x 512 float32, cut, boxes       forward 48 us, 42 %; backward 60 us, 58 %
 //   6 x 4001 x 385 float32, cut, plain loads  forward 62 us, 36 %; backward 87 us, 45 %
 //   1 x 32768 x 1040 bfloat16, cut, boxes     forward 124 us, 34 %; backward 146 us, 50 %

@@ -83,7 +83,8 @@ int64_t warps_enough(bool bulk, bool backward, int size) {
 //   float32 in boxes 308 x 500: 31 / 36, 448 x 500: 38 / 38;  bfloat16 448 x 500: 35 / 40, 560 x 500: 40 / 40
 int64_t warps_for_rows(bool bulk, int size) { return bulk && size == 4 ? 148 * 3 : 148 * 4; }
 // Rows and channel pairs that make so many warps take pairs of channels (forward and backward, pairs / single, us):
-//   float32 in boxes    672 x 500: 73 / 69, 118 / 131;  896 x 500: 81 / 94, 153 / 163;  3584 x 500: 302 / 322, 562 / 588
+//   float32 in boxes    672 x 500: 73 / 69, 118 / 131;  768 x 512: 77 / 79, 138 / 146;  896 x 500: 81 / 91, 153 / 162;
+//                       1232 x 500: 118 / 144, 227 / 214;  2240 x 500: 206 / 212, 347 / 374
 //   float32 by lanes    1792 x 500: 202 / 175, 318 / 360;  2688 x 500: 259 / 255, 474 / 512
 //   bfloat16 by lanes   1792 x 500: 156 / 144, 226 / 262;  2688 x 500: 177 / 200, 316 / 354
 //   bfloat16 in boxes   4096 x 24: 23 / 27, 34 / 42;  4096 x 96: 49 / 52, 81 / 81;  4096 x 256: 111 / 113, 194 / 181;

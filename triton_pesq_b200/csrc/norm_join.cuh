@@ -26,10 +26,11 @@
 // A row's sums are two rounds of shuffles, and barriers where a team has several warps, that its
 // loads and stores overlap only by the other teams of the SM and by the next row's loads.
 // Measured (B200, cold caches, share of the bytes at the measured copy rate):
-//   64 x 500 x 896, stream and block bfloat16   forward 56 us, 78 %; backward 103 us, 68 %
+//   64 x 500 x 896, stream and block bfloat16   forward 56 us, 78 %; backward 105 us, 67 %
 //   64 x 500 x 385, float32                     forward 48 us, 78 %; backward 81 us, 74 %
 //   100000 x 64, bfloat16                       forward 18.5 us, backward 32.8 us
-//   4000 x 8192, bfloat16                       backward 278 us, 30 % (sums in shared memory, no next row)
+//   4000 x 8192, bfloat16                       forward 86 us, 58 %; backward 277 us, 29 % (sums in shared
+//                                               memory, no next row)
 //   8 x 500 x 768, stream float32               forward 10.4 us a call (floor 5.6), launch included
 #pragma once
 
