@@ -382,7 +382,9 @@ int pesq_gated_scan_forward(const pesq_gated_scan_desc* desc, void* stream, void
                             size_t kept_bytes, void* workspace, size_t workspace_bytes);
 /* dy.data and dlast may be NULL (zeros); dstate may be NULL (not wanted).
  * dx, dinput_gate, ddecay_gate: dense; ddecay: [width].  Gradients are at
- * least as aligned as the inputs, dy's strides too. */
+ * least as aligned as the inputs, dy's strides too.  kept_bytes: of the forward,
+ * as pesq_gated_scan_sizes gives it for the streams' addresses and strides there;
+ * of streams that are laid out otherwise here it is another number, and refused. */
 int pesq_gated_scan_backward(const pesq_gated_scan_desc* desc, void* stream, const void* kept, size_t kept_bytes,
                              pesq_stream dy, const float* dlast, void* dx, void* dinput_gate, void* ddecay_gate,
                              float* ddecay, float* dstate, void* workspace, size_t workspace_bytes);

@@ -359,3 +359,30 @@ def test_refusals(cuda_device):
     y, _ = gated_scan(x, ig, rg, decay)
     with pytest.raises(RuntimeError, match="second derivative"):
         torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dense_first", [False, True])
+def test_saved_streams_that_come_back_in_another_layout(cuda_device, dtype, dense_first):
+    """Hooks on what autograd saves (offloading, say) may hand the backward
+    tensors of other strides than the forward's."""
+
+    def strided(t):
+        out = torch.empty(t.shape[0], t.shape[1], t.shape[2] + 1, dtype=t.dtype, device=t.device)[..., 1:]
+        return out.copy_(t)
+
+    tensors, dy, dlast = inputs(2, 90, 64, dtype, seed=6)
+    dev = [t.to(cuda_device) for t in tensors]
+    relay = strided if dense_first else torch.Tensor.contiguous
+    if not dense_first:
+        dev[:3] = [strided(t) for t in dev[:3]]
+    dev = [t.requires_grad_(True) for t in dev]
+    streams = lambda t: t.dim() == 3 and t.dtype == dtype  # noqa: E731
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), lambda t: relay(t) if streams(t) else t):
+        y, last = gated_scan(*dev)
+    got = torch.autograd.grad((y, last), dev, (dy.to(cuda_device), dlast.to(cuda_device)))
+    wide = [t.double().requires_grad_(True) for t in tensors]
+    wy, wl = R.gated_scan(*wide, None, None, False, 8.0)
+    want = torch.autograd.grad((wy, wl), wide, (dy.double(), dlast.double()))
+    for name, g, w in zip(NAMES, got, want):
+        R.close(g, w, GTOL, "d " + name)

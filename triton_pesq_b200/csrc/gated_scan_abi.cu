@@ -312,8 +312,8 @@ int pesq_gated_scan_backward(const pesq_gated_scan_desc* d, void* stream, const 
   if ((dy.data && (g.bulk ? !boxes(dy, *d) : !fits(dy, g.vec, *d))) || !fits(dx, g, *d) || !fits(dinput_gate, g, *d) ||
       !fits(ddecay_gate, g, *d))
     return set_error(PESQ_ERR_INVALID_ARGUMENT, "a gradient is less aligned than the inputs");
-  if (missing(kept, kept_size, kept_bytes(*d, g)))
-    return set_error(PESQ_ERR_WORKSPACE, "the states that the forward kept are missing");
+  if (missing(kept, kept_size, kept_bytes(*d, g)) || kept_size != kept_bytes(*d, g))
+    return set_error(PESQ_ERR_WORKSPACE, "the states that the forward kept are missing, or of streams laid out otherwise");
   if (missing(workspace, workspace_bytes, back_bytes(*d, g)))
     return set_error(PESQ_ERR_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
   const cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -217,8 +217,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> gated_sca
   }
   size_t work = 0, states = 0, back = 0;
   check_status(pesq_gated_scan_sizes(&c.d, &work, &states, &back), "pesq_gated_scan_sizes");
-  at::Tensor ws = at::empty({static_cast<int64_t>(back)}, f32.dtype(at::kByte));
-  check_status(pesq_gated_scan_backward(&c.d, at::cuda::getCurrentCUDAStream(), kept.data_ptr(), kept.numel(), dys,
+  at::Tensor ws = at::empty({static_cast<int64_t>(back)}, f32.dtype(at::kByte)), before = kept;
+  // (the chunks that states are kept of follow from the streams' layout, and hooks on what autograd saves
+  // may bring the streams back in another)
+  if (kept.numel() != static_cast<int64_t>(states))
+    before = std::get<2>(gated_scan_forward(x, ig, rg, decay, state, reset, lengths, reverse, rate, true));
+  check_status(pesq_gated_scan_backward(&c.d, at::cuda::getCurrentCUDAStream(), before.data_ptr(), states, dys,
                                         dlast.defined() ? dlast.data_ptr<float>() : nullptr, dx.data_ptr(),
                                         dig.data_ptr(), drg.data_ptr(), ddecay.data_ptr<float>(),
                                         dstate.data_ptr<float>(), ws.data_ptr(), back),
