@@ -99,6 +99,27 @@ def test_lengths_with_nan_in_the_padding(cuda_device, dtype, steps, reverse):
     compare(tensors, dy, dlast, cuda_device, lengths=lengths, reset=reset, reverse=reverse)
 
 
+# every way through the rows: whole rows of single channels and of pairs, by boxes and by lanes; rows cut in
+# both directions or in the backward alone; rows of one CTA; many single steps
+WAYS = [((100, 40, 512), torch.float32), ((230, 33, 512), torch.bfloat16), ((100, 20, 1202), torch.float32),
+        ((100, 20, 1202), torch.float16), ((30, 50, 448), torch.float32), ((50, 150, 416), torch.bfloat16),
+        ((50, 100, 401), torch.float16), ((3, 700, 128), torch.float32), ((3, 700, 128), torch.bfloat16),
+        ((9, 500, 72), torch.bfloat16), ((80, 1, 4096), torch.float32), ((100, 1, 1601), torch.bfloat16)]
+
+
+@pytest.mark.parametrize("shape, dtype", WAYS)
+@pytest.mark.parametrize("masks, reverse", [(False, False), (True, False), (True, True)])
+def test_ways_through_the_rows(cuda_device, shape, dtype, masks, reverse):
+    batch, steps, _ = shape
+    tensors, dy, dlast = inputs(*shape, dtype, seed=sum(shape))
+    lengths = reset = None
+    if masks:
+        g = torch.Generator().manual_seed(3)
+        lengths = torch.randint(0, steps + 1, (batch,), generator=g)
+        reset = torch.rand(batch, steps, generator=g) < 0.02
+    compare(tensors, dy, dlast, cuda_device, lengths=lengths, reset=reset, reverse=reverse)
+
+
 def test_lengths_beyond_the_row_and_below_zero(cuda_device):
     tensors, _, _ = inputs(2, 20, 8, torch.float32)
     dev = [t.to(cuda_device) for t in tensors]
