@@ -37,8 +37,9 @@ def call(t, **kw):
     return norm_join(t[0], t[1], t[2], t[3], gate=t[4], scale=t[5], **kw)
 
 
-def compare(tensors, ds, dn, device, **kw):
-    mine = [None if t is None else t.to(device).requires_grad_(True) for t in tensors]
+def compare(tensors, ds, dn, device, place=None, **kw):
+    place = place or (lambda t: t.to(device))
+    mine = [None if t is None else place(t).requires_grad_(True) for t in tensors]
     stream, normed = call(mine, **kw)
     leaves = [t for t in mine if t is not None]
     got = torch.autograd.grad((stream, normed), leaves, (ds.to(device), dn.to(device)))
@@ -79,6 +80,26 @@ def test_gates_and_scales(cuda_device, gate, scale, shape):
     for types in ((F32, F32), (F32, BF16)):
         tensors, ds, dn = inputs(*shape, *types, seed=3, gate=gate, scale=scale)
         compare(tensors, ds, dn, cuda_device)
+
+
+@pytest.mark.parametrize("types", [(F32, F32), (BF16, BF16), (F32, F16)])
+@pytest.mark.parametrize("shape", [(2, 3001, 64), (3, 900, 256), (1, 2000, 896), (2, 500, 1600), (1, 500, 3000), (1, 400, 8192),
+                                   (2, 3001, 61), (1, 2000, 900)])
+@pytest.mark.parametrize("apart", [False, True])
+def test_teams_that_take_several_rows(cuda_device, types, shape, apart):
+    """More rows than the device holds teams for; with batch items apart,
+    a team's rows stay within one."""
+
+    tensors, ds, dn = inputs(*shape, *types, seed=8)
+    place = None
+    if apart:
+        def place(t):
+            if t.dim() < 3:
+                return t.to(cuda_device)
+            return torch.cat((t, torch.full_like(t[:, :3], float("nan"))), 1).to(cuda_device)[:, :-3]
+
+        assert place(ds).stride(0) > shape[1] * shape[2]
+    compare(tensors, ds, dn, cuda_device, place=place)
 
 
 def test_other_broadcasts_of_the_gate(cuda_device):
