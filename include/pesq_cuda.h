@@ -445,7 +445,7 @@ typedef struct pesq_adamw_desc {
   const float* grad_scale;  /* device, times every gradient; the step is skipped where it is not finite; NULL: 1 */
   double beta1, beta2;
   float lr, eps, weight_decay;
-  uint32_t seed;      /* of the 8-bit second moment's rounding */
+  uint32_t seed;      /* of the 8-bit moments' stochastic rounding */
 } pesq_adamw_desc;
 
 /* m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2,

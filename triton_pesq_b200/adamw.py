@@ -7,10 +7,11 @@ launch (csrc/adamw.cu), with moments in 32 or in 8 bits::
 The moments of all tensors lie in two flat buffers, a tensor's part beginning at
 a multiple of 256 values.  With 8 bits they are ``float8_e4m3fn`` in units of one
 float32 scale per 256 values (``scales[0]`` and ``scales[1]``), the second moment
-as its root; that root is rounded stochastically (a hash of position, step and
-``seed``), because nearest rounding would hold a value that changes by 1 / 2000 of
-itself a step for good.  The step count is on the device, so a step can be
-captured in a CUDA graph.  The reference has no optimiser.
+as its root.  Nearest rounding would hold what moves by less than half a rounding
+step at a time for good: that root, which changes by 1 / 2000 of itself a step, and the
+first moment where it is small (or ``b1`` above 15/16) and moves that little are rounded
+stochastically (a hash of position, step and ``seed``).  The step count is on the device, so a
+step can be captured in a CUDA graph.  The reference has no optimiser.
 """
 
 from __future__ import annotations
@@ -64,7 +65,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mo
         One float32 value on the GPU that multiplies every gradient (an unscaling
         or clipping factor).  Where it is not finite the step is skipped whole.
     seed
-        Of the 8-bit second moment's rounding.
+        Of the 8-bit moments' stochastic rounding.
     """
 
     (_op or _load())(params, grads, moment1, moment2, step, scales, [] if copies is None else copies, lr, betas[0],
@@ -117,7 +118,7 @@ class AdamWCuda(torch.optim.Optimizer):
     state_bits : int
         32, or 8 for float8 moments with a scale per 256 values
     seed : int
-        Of the 8-bit second moment's rounding
+        Of the 8-bit moments' stochastic rounding
 
     The step count is one for all parameters of a group and type, so a parameter
     that had no gradient at first is corrected as if it had been zero.  A captured

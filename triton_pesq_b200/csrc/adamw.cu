@@ -16,13 +16,19 @@
 // the arithmetic of the 8 bits (70 % of the issue slots) is as long as the bytes; 275,000 values in 52 tensors 7 us.
 //
 // 8 bits.  A block of 256 has a 32-bit scale, its largest magnitude / 448, and its
-// values are float8 (e4m3) in units of it.  The first moment is rounded to nearest:
-// it moves by a tenth of itself a step, more than half the rounding step, so it is not stuck.
+// values are float8 (e4m3) in units of it.  Nearest rounding holds a value for good that
+// moves by less than half a rounding step at a time; such a value is rounded stochastically,
+// with bits that are a hash of position, step and seed, so that its mean is right and a
+// run can be repeated.
+// The first moment moves by (1 - b1) (g - m).  Without a gradient that is more than half a step (1/16
+// of the value) where b1 <= 15/16 and the value is above 2^-6 units; there it is rounded to nearest,
+// and a gradient that stays the same is met to half a step / (1 - b1), 5/8 of the value for b1 = 0.9.
+// Below 2^-6 units the steps are 2^-9 throughout (codes of 1 to 4 steps times 0.9 round back
+// to themselves, and the parameter would move on without a gradient), and with a larger b1 nothing
+// need move that far: there a value that moves by less than half a step is rounded stochastically.
 // The second moment is kept as its root, which halves the range that 8 bits have to
 // span (2^-9 .. 448 of the root are 10 decades of the moment), and moves by less
-// than 1 / 2000 of itself a step, where nearest rounding (steps of 1/8) would
-// hold it for good: it is rounded stochastically, with bits that are a hash of
-// position, step and seed, so that its mean is right and a run can be repeated.
+// than 1 / 2000 of itself a step: it is always rounded stochastically.
 // A root that is not zero is never rounded to zero: the update would divide by
 // the gradient's own share alone and be too large by up to 1 / sqrt(1 - b2).  The hash
 // is the multiply-xorshift finaliser "lowbias32" (C. Wellons, "Prospecting for Hash
@@ -76,6 +82,7 @@ struct Args {
   double log_beta1, log_beta2;
   float beta1, beta2, rest1, rest2;  // betas, and 1 less them
   float lr, eps, decay;
+  float held1;           // units below which nearest rounding may hold the first moment
   unsigned seed;
   int last;              // of the call's launches
 };
@@ -104,12 +111,21 @@ __device__ __forceinline__ unsigned to_e4m3(const float* v) {  // nearest
 
 // u >= 0 to one of its two neighbours in e4m3, the upper with the probability of
 // its nearness: 20 random bits are added below the 3 mantissa bits that stay.
-// Below 2^-6, where the steps are 2^-9 throughout, that is done to u + 2^-6.  What is
-// above zero does not become zero.
+// Below 2^-6, where the steps are 2^-9 throughout, that is done to u + 2^-6.
 __device__ __forceinline__ float dither(float u, unsigned bits) {
   const float base = u < 0x1p-6f ? 0x1p-6f : 0.0f;
-  const float t = __uint_as_float((__float_as_uint(u + base) + (bits & 0xfffffu)) & ~0xfffffu) - base;
-  return u > 0.0f ? fmaxf(t, 0x1p-9f) : u;
+  return __uint_as_float((__float_as_uint(u + base) + (bits & 0xfffffu)) & ~0xfffffu) - base;
+}
+// The second moment's root: what is above zero does not become zero
+__device__ __forceinline__ float dither_root(float u, unsigned bits) {
+  return u > 0.0f ? fmaxf(dither(u, bits), 0x1p-9f) : u;
+}
+// The first moment, in units, that was `was` in the same units: left to nearest rounding
+// where it has moved by half a step or more.  The twelve upper bits of a hash; the root takes the others.
+__device__ __forceinline__ float dither_held(float m, float was, unsigned bits) {
+  const float u = fabsf(m), power = __uint_as_float(__float_as_uint(u) & 0x7f800000u);
+  if (!(fabsf(m - was) < 0x1p-4f * fmaxf(power, 0x1p-6f))) return m;
+  return copysignf(dither(u, bits >> 20 << 8 | 0x80u), m);
 }
 
 // Eight values of a tensor, as the words they were read as
@@ -309,10 +325,22 @@ __global__ void __launch_bounds__(kThreads, kCtas<kEight>) adamw_kernel(const __
         for (int j = 0; j < 8; ++j) top1 = max_nan(top1, fabsf(m[j])), top2 = max_nan(top2, r[j]);
         const float s1 = warp_max(top1) * (1.0f / kTop), s2 = warp_max(top2) * (1.0f / kTop);
         const float i1 = s1 > 1e-36f ? __frcp_rn(s1) : 0.0f, i2 = s2 > 1e-36f ? __frcp_rn(s2) : 0.0f;
+        float low1 = kTop;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           m[j] *= i1;
-          r[j] = dither(r[j] * i2, hash((unsigned)(place + j) + salt));
+          low1 = fminf(low1, fabsf(m[j]));
+          r[j] = dither_root(r[j] * i2, hash((unsigned)(place + j) + salt));
+        }
+        if (low1 < p.held1) {  // (rare where a gradient is there: 1 value in 10,000)
+          // (the codes are still in memory, which costs fewer registers than to keep them)
+          const uint2 c = *reinterpret_cast<const uint2*>(static_cast<const unsigned char*>(p.moment1) + place);
+          const float then = now.s1 * i1;
+          float was[8];
+          from_e4m3(c.x, was), from_e4m3(c.y, was + 4);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (fabsf(m[j]) < p.held1) m[j] = dither_held(m[j], was[j] * then, hash((unsigned)(place + j) + salt));
         }
         uint2 c1, c2;
         c1.x = to_e4m3(m), c1.y = to_e4m3(m + 4), c2.x = to_e4m3(r), c2.y = to_e4m3(r + 4);
@@ -412,6 +440,7 @@ int pesq_adamw_step(const pesq_adamw_desc* d, const pesq_adamw_tensor* tensors, 
   a.lr = d->lr;
   a.eps = d->eps;
   a.decay = d->weight_decay;
+  a.held1 = d->beta1 <= 0.9375 ? 0x1p-6f : INFINITY;
   a.seed = d->seed;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   Entry table[kLong];
