@@ -12,7 +12,7 @@
 // 256 values, so that the blocks of 256 of the buffer are the units of work, and one warp
 // takes a unit: eight values a lane.  A warp finds its tensor by bisection.
 // Measured (B200, share of the bytes at the measured copy rate): 35M values, 32-bit moments and
-// gradients 158 us, 95 %; 106M values, 8-bit moments, 16-bit gradients and copies 334 us, 78 %, where
+// gradients 158 us, 95 %; 106M values, 8-bit moments, 16-bit gradients and copies 329 us, 79 %, where
 // the arithmetic of the 8 bits (70 % of the issue slots) is as long as the bytes; 275,000 values in 52 tensors 7 us.
 //
 // 8 bits.  A block of 256 has a 32-bit scale, its largest magnitude / 448, and its
@@ -109,23 +109,22 @@ __device__ __forceinline__ unsigned to_e4m3(const float* v) {  // nearest
   return w;
 }
 
-// u >= 0 to one of its two neighbours in e4m3, the upper with the probability of
-// its nearness: 20 random bits are added below the 3 mantissa bits that stay.
-// Below 2^-6, where the steps are 2^-9 throughout, that is done to u + 2^-6.
+// u to one of its two neighbours in e4m3, the upper with the probability of its
+// nearness: 20 random bits are added below the 3 mantissa bits that stay.  From 2^-6 on
 __device__ __forceinline__ float dither(float u, unsigned bits) {
-  const float base = u < 0x1p-6f ? 0x1p-6f : 0.0f;
-  return __uint_as_float((__float_as_uint(u + base) + (bits & 0xfffffu)) & ~0xfffffu) - base;
+  return __uint_as_float((__float_as_uint(u) + (bits & 0xfffffu)) & ~0xfffffu);
 }
-// The second moment's root: what is above zero does not become zero
-__device__ __forceinline__ float dither_root(float u, unsigned bits) {
-  return u > 0.0f ? fmaxf(dither(u, bits), 0x1p-9f) : u;
+// below, where the steps are 2^-9 throughout
+__device__ __forceinline__ float dither_small(float u, unsigned bits) {
+  return floorf(fmaf((float)(bits & 0xfffffu), 0x1p-20f, u * 512.0f)) * 0x1p-9f;
 }
 // The first moment, in units, that was `was` in the same units: left to nearest rounding
 // where it has moved by half a step or more.  The twelve upper bits of a hash; the root takes the others.
 __device__ __forceinline__ float dither_held(float m, float was, unsigned bits) {
   const float u = fabsf(m), power = __uint_as_float(__float_as_uint(u) & 0x7f800000u);
   if (!(fabsf(m - was) < 0x1p-4f * fmaxf(power, 0x1p-6f))) return m;
-  return copysignf(dither(u, bits >> 20 << 8 | 0x80u), m);
+  const unsigned mine = bits >> 20 << 8 | 0x80u;
+  return copysignf(u < 0x1p-6f ? dither_small(u, mine) : dither(u, mine), m);
 }
 
 // Eight values of a tensor, as the words they were read as
@@ -325,12 +324,24 @@ __global__ void __launch_bounds__(kThreads, kCtas<kEight>) adamw_kernel(const __
         for (int j = 0; j < 8; ++j) top1 = max_nan(top1, fabsf(m[j])), top2 = max_nan(top2, r[j]);
         const float s1 = warp_max(top1) * (1.0f / kTop), s2 = warp_max(top2) * (1.0f / kTop);
         const float i1 = s1 > 1e-36f ? __frcp_rn(s1) : 0.0f, i2 = s2 > 1e-36f ? __frcp_rn(s2) : 0.0f;
-        float low1 = kTop;
+        float low1 = kTop, low2 = kTop;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          m[j] *= i1;
-          low1 = fminf(low1, fabsf(m[j]));
-          r[j] = dither_root(r[j] * i2, hash((unsigned)(place + j) + salt));
+          m[j] *= i1, r[j] *= i2;
+          low1 = fminf(low1, fabsf(m[j])), low2 = min_nan(low2, r[j]);
+        }
+        if (low2 >= 0x1p-6f) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) r[j] = dither(r[j], hash((unsigned)(place + j) + salt));
+        } else {  // (what is above zero does not become zero, and a NaN stays)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const unsigned h = hash((unsigned)(place + j) + salt);
+            if (r[j] >= 0x1p-6f)
+              r[j] = dither(r[j], h);
+            else if (r[j] > 0.0f)
+              r[j] = fmaxf(dither_small(r[j], h), 0x1p-9f);
+          }
         }
         if (low1 < p.held1) {  // (rare where a gradient is there: 1 value in 10,000)
           // (the codes are still in memory, which costs fewer registers than to keep them)
