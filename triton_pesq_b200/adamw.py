@@ -122,7 +122,9 @@ class AdamWCuda(torch.optim.Optimizer):
 
     The step count is one for all parameters of a group and type, so a parameter
     that had no gradient at first is corrected as if it had been zero.  A captured
-    step keeps the hyperparameters it was captured with.
+    step keeps the hyperparameters it was captured with.  16-bit parameters are written from
+    their masters by every step: what else writes to them after the first step is lost, unless
+    it writes to ``state[p]["master"]`` too.
     """
 
     def __init__(self, params, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
@@ -162,19 +164,35 @@ class AdamWCuda(torch.optim.Optimizer):
                     self.state[p] = views
         return flats
 
+    def _check_state(self, p: torch.Tensor, state: dict) -> None:
+        units = -(-p.numel() // BLOCK)
+        moment = torch.float32 if self.state_bits == 32 else torch.float8_e4m3fn
+        want = {"step": (torch.int64, (2,)), "moment1": (moment, (BLOCK * units,)), "moment2": (moment, (BLOCK * units,))}
+        if self.state_bits == 8:
+            want["scales"] = (torch.float32, (2, units))
+        if p.dtype != torch.float32:
+            want["master"] = (torch.float32, tuple(p.shape))
+        got = {k: (v.dtype, tuple(v.shape)) if isinstance(v, torch.Tensor) else type(v) for k, v in state.items()}
+        if got != want:
+            raise ValueError(f"This is not the state of a parameter of AdamWCuda with state_bits={self.state_bits}: needs "
+                             f"{want}, got {got}.")
+
     def load_state_dict(self, state_dict) -> None:
-        self._flats.clear()
-        self.state.clear()
-        kept = {}
-        # (float8 and int64 state is not to be cast to the parameters' type)
-        for key, value in state_dict["state"].items():
-            kept[key] = {k: v.clone() for k, v in value.items()}
-        super().load_state_dict({**state_dict, "state": {}})
+        """Takes the state of an ``AdamWCuda`` of the same ``state_bits`` on parameters of the same types and sizes;
+        anything else is refused with a ``ValueError`` and changes nothing."""
+
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
+        kept = {}
         for i, p in zip(ids, params):
-            if i in kept:
-                self.state[p] = {k: v.to(p.device) for k, v in kept[i].items()}
+            if i in state_dict["state"]:
+                state = state_dict["state"][i]
+                self._check_state(p, state)
+                kept[p] = {k: v.detach().to(p.device, copy=True) for k, v in state.items()}
+        # (the base class would cast float8 and int64 state to the parameters' type)
+        super().load_state_dict({**state_dict, "state": {}})
+        self._flats.clear()
+        self.state.update(kept)
 
     @torch.no_grad()
     def step(self, closure=None, grad_scale: Optional[torch.Tensor] = None):
