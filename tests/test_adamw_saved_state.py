@@ -1,4 +1,7 @@
-"""What an AdamWCuda takes as saved state."""
+"""What an AdamWCuda takes as saved state, and its copies."""
+
+import copy
+import io
 
 import pytest
 import torch
@@ -69,3 +72,41 @@ def test_state_of_another_kind_is_refused():
     assert not opt.state
     opt.load_state_dict(saved(32))
     assert len(opt.state) == 2
+
+
+def test_copies_keep_their_options():
+    opt = AdamWCuda(parameters(), state_bits=8, seed=5, lr=0.25)
+    opt.load_state_dict({**saved(8), "param_groups": opt.state_dict()["param_groups"]})
+    buffer = io.BytesIO()
+    torch.save(opt, buffer)
+    buffer.seek(0)
+    for other in (copy.deepcopy(opt), torch.load(buffer, weights_only=False)):
+        assert other.state_bits == 8 and other.seed == 5 and other.param_groups[0]["lr"] == 0.25
+        assert len(other.state) == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_copies_step_on_as_the_original(cuda_device, bits, dtype):
+    def advance(opt, seed):
+        g = torch.Generator(cuda_device).manual_seed(seed)
+        for group in opt.param_groups:
+            for p in group["params"]:
+                p.grad = torch.randn(p.shape, device=cuda_device, generator=g).to(p.dtype)
+        opt.step()
+
+    opt = AdamWCuda(parameters(cuda_device, dtype), lr=1e-2, state_bits=bits, seed=3)
+    advance(opt, 1)
+    buffer = io.BytesIO()
+    torch.save(opt, buffer)
+    buffer.seek(0)
+    others = [copy.deepcopy(opt), torch.load(buffer, weights_only=False)]
+    for seed in (2, 3):
+        for o in (opt, *others):
+            advance(o, seed)
+    for o in others:
+        for p, q in zip(opt.param_groups[0]["params"], o.param_groups[0]["params"]):
+            assert p is not q and torch.equal(p, q)
+            for k, t in opt.state[p].items():
+                assert torch.equal(t.contiguous().view(torch.uint8), o.state[q][k].contiguous().view(torch.uint8)), k

@@ -191,8 +191,15 @@ class AdamWCuda(torch.optim.Optimizer):
                 kept[p] = {k: v.detach().to(p.device, copy=True) for k, v in state.items()}
         # (the base class would cast float8 and int64 state to the parameters' type)
         super().load_state_dict({**state_dict, "state": {}})
-        self._flats.clear()
         self.state.update(kept)
+
+    def __getstate__(self) -> dict:
+        return {**super().__getstate__(), "state_bits": self.state_bits, "seed": self.seed}
+
+    def __setstate__(self, state: dict) -> None:
+        _load()
+        self._flats = {}  # (made from the state by the next step)
+        super().__setstate__(state)
 
     @torch.no_grad()
     def step(self, closure=None, grad_scale: Optional[torch.Tensor] = None):
