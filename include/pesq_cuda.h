@@ -439,7 +439,7 @@ typedef struct pesq_adamw_desc {
   int32_t grad_dtype; /* PESQ_F32, PESQ_BF16 or PESQ_F16 */
   int32_t state_bits; /* 32: float moments; 8: float8 (e4m3) moments, the second as its root, in units of scales */
   int64_t units;      /* units of 256 values that the moments' buffers hold */
-  void *moment1, *moment2;  /* [units * 256] */
+  void *moment1, *moment2;  /* [units * 256]; NULL where units is 0 */
   float *scale1, *scale2;   /* [units], 8 bits */
   int64_t* step;      /* device [2]: steps taken; 0 between calls (counts a launch's blocks) */
   const float* grad_scale;  /* device, times every gradient; the step is skipped where it is not finite; NULL: 1 */

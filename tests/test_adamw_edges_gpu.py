@@ -1,0 +1,37 @@
+"""AdamW steps at the edges of what there is to step."""
+
+import pytest
+import torch
+
+from triton_pesq_b200 import AdamWCuda, adamw_step
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("units", [0, 1])
+def test_a_step_without_values_counts(cuda_device, bits, units):
+    def state():
+        kind = torch.float32 if bits == 32 else torch.float8_e4m3fn
+        m, v = (torch.zeros(256 * units, device=cuda_device).to(kind) for _ in range(2))
+        scales = torch.zeros(2, units, device=cuda_device) if bits == 8 else None
+        return m, v, torch.tensor([4, 0], device=cuda_device), scales
+
+    empty = torch.zeros(0, device=cuda_device)
+    for params in ([], [empty], [empty, torch.zeros(3, 0, device=cuda_device)]):
+        m, v, step, scales = state()
+        adamw_step(params, [torch.zeros_like(p) for p in params], m, v, step, scales=scales)
+        assert step.tolist() == [5, 0]
+        adamw_step(params, [torch.zeros_like(p) for p in params], m, v, step, scales=scales,
+                   grad_scale=torch.full((1,), float("inf"), device=cuda_device))
+        assert step.tolist() == [5, 0]
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_group_of_empty_parameters_steps(cuda_device, bits):
+    empty, one = torch.nn.Parameter(torch.zeros(0, device=cuda_device)), torch.nn.Parameter(torch.ones(3, device=cuda_device))
+    opt = AdamWCuda([{"params": [empty]}, {"params": [one]}], state_bits=bits)
+    for n in (1, 2):
+        empty.grad, one.grad = torch.zeros_like(empty), torch.ones_like(one)
+        opt.step()
+        assert opt.state[empty]["step"].tolist() == opt.state[one]["step"].tolist() == [n, 0]

@@ -397,7 +397,8 @@ template <class G, bool kEight, int N>
 cudaError_t start(const Args& a, const Entry* e, cudaStream_t s) {
   Table<N> t;
   std::memcpy(t.e, e, sizeof(Entry) * a.count);
-  const int64_t blocks = (a.units + kThreads / 32 - 1) / (kThreads / 32);
+  // (one block at least: a step without values counts)
+  const int64_t blocks = std::max<int64_t>(1, (a.units + kThreads / 32 - 1) / (kThreads / 32));
   const unsigned grid = (unsigned)std::min<int64_t>(blocks, (int64_t)sms() * kCtas<kEight>);
   adamw_kernel<G, kEight, N><<<grid, kThreads, 0, s>>>(a, t);
   return cudaGetLastError();
@@ -417,7 +418,8 @@ int pesq_adamw_step(const pesq_adamw_desc* d, const pesq_adamw_tensor* tensors, 
   if (d->grad_dtype < PESQ_F32 || d->grad_dtype > PESQ_F16)
     return set_error(PESQ_ERR_INVALID_ARGUMENT, "unknown gradient type");
   if (d->state_bits != 8 && d->state_bits != 32) return set_error(PESQ_ERR_INVALID_ARGUMENT, "states have 8 or 32 bits");
-  if (!d->moment1 || !d->moment2 || !d->step || (d->state_bits == 8 && (!d->scale1 || !d->scale2)))
+  if (!d->step ||
+      (d->units > 0 && (!d->moment1 || !d->moment2 || (d->state_bits == 8 && (!d->scale1 || !d->scale2)))))
     return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL state");
   if (reinterpret_cast<uintptr_t>(d->moment1) % 16 || reinterpret_cast<uintptr_t>(d->moment2) % 16 ||
       reinterpret_cast<uintptr_t>(d->step) % 8)
@@ -456,7 +458,7 @@ int pesq_adamw_step(const pesq_adamw_desc* d, const pesq_adamw_tensor* tensors, 
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   Entry table[kLong];
   int64_t i = 0, before = 0;
-  do {  // (once at least: a step without values counts)
+  do {  // (once at least)
     a.count = 0;
     a.units = 0;
     a.first = before;
