@@ -35,3 +35,13 @@ def test_a_group_of_empty_parameters_steps(cuda_device, bits):
         empty.grad, one.grad = torch.zeros_like(empty), torch.ones_like(one)
         opt.step()
         assert opt.state[empty]["step"].tolist() == opt.state[one]["step"].tolist() == [n, 0]
+
+
+def test_small_gradients_without_eps(cuda_device):
+    """Gradients whose squares are below the normal range, eps = 0: the first step moves every value by lr.  The
+    second moment, 1e-43, is a multiple of 2**-149, so off by up to 0.7 % and its root by 0.35 %: 0.5 % is allowed."""
+
+    p, g = [torch.zeros(300, device=cuda_device)], [torch.full((300,), 1e-20, device=cuda_device)]
+    m, v = torch.zeros(512, device=cuda_device), torch.zeros(512, device=cuda_device)
+    adamw_step(p, g, m, v, torch.zeros(2, dtype=torch.int64, device=cuda_device), lr=1.0, eps=0.0, weight_decay=0.0)
+    assert float((p[0] + 1).abs().max()) <= 5e-3
