@@ -45,3 +45,24 @@ def test_small_gradients_without_eps(cuda_device):
     m, v = torch.zeros(512, device=cuda_device), torch.zeros(512, device=cuda_device)
     adamw_step(p, g, m, v, torch.zeros(2, dtype=torch.int64, device=cuda_device), lr=1.0, eps=0.0, weight_decay=0.0)
     assert float((p[0] + 1).abs().max()) <= 5e-3
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_first_step_is_not_captured(cuda_device, dtype):
+    """Its state would be made anew by every replay."""
+
+    w = torch.nn.Parameter(torch.ones(40, device=cuda_device, dtype=dtype))
+    w.grad = torch.ones_like(w)
+    opt = AdamWCuda([w])
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="captur"):
+        with torch.cuda.graph(graph):
+            opt.step()
+    del graph
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for _ in range(3):
+        graph.replay()
+    assert opt.state[w]["step"].tolist() == [4, 0]

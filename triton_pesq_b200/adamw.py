@@ -122,7 +122,8 @@ class AdamWCuda(torch.optim.Optimizer):
 
     The step count is one for all parameters of a group and type, so a parameter
     that had no gradient at first is corrected as if it had been zero.  A captured
-    step keeps the hyperparameters it was captured with.  16-bit parameters are written from
+    step keeps the hyperparameters it was captured with; the first step, and the first after
+    ``load_state_dict``, make the state's buffers and are refused in a capture.  16-bit parameters are written from
     their masters by every step: what else writes to them after the first step is lost, unless
     it writes to ``state[p]["master"]`` too.
     """
@@ -149,6 +150,9 @@ class AdamWCuda(torch.optim.Optimizer):
     def _flat(self, index: int) -> List[_Flat]:
         flats = self._flats.get(index)
         if flats is None:
+            if torch.cuda.is_current_stream_capturing():
+                # (a graph would take the state's making along, and every replay would begin anew)
+                raise RuntimeError("The first step of an AdamWCuda makes its state and cannot be captured: take one before.")
             kinds: Dict[tuple, List[torch.Tensor]] = {}
             for p in self.param_groups[index]["params"]:
                 if not p.is_cuda:
