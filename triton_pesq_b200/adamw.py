@@ -150,14 +150,14 @@ class AdamWCuda(torch.optim.Optimizer):
     def _flat(self, index: int) -> List[_Flat]:
         flats = self._flats.get(index)
         if flats is None:
-            if torch.cuda.is_current_stream_capturing():
-                # (a graph would take the state's making along, and every replay would begin anew)
-                raise RuntimeError("The first step of an AdamWCuda makes its state and cannot be captured: take one before.")
             kinds: Dict[tuple, List[torch.Tensor]] = {}
             for p in self.param_groups[index]["params"]:
                 if not p.is_cuda:
                     raise RuntimeError("AdamWCuda needs its parameters to live on a GPU.")
                 kinds.setdefault((p.device, p.dtype), []).append(p)
+            if kinds and torch.cuda.is_current_stream_capturing():
+                # (a graph would take the state's making along, and every replay would begin anew)
+                raise RuntimeError("The first step of an AdamWCuda makes its state and cannot be captured: take one before.")
             flats = self._flats[index] = [_Flat(ps, self.state_bits) for ps in kinds.values()]
             for f in flats:
                 for i, p in enumerate(f.params):
