@@ -66,3 +66,19 @@ def test_a_first_step_is_not_captured(cuda_device, dtype):
     for _ in range(3):
         graph.replay()
     assert opt.state[w]["step"].tolist() == [4, 0]
+
+
+def test_layouts_that_are_not_dense_are_refused_at_once(cuda_device):
+    weight = torch.nn.Conv2d(3, 4, 3).to(cuda_device, memory_format=torch.channels_last).weight
+    for p in (weight, torch.nn.Parameter(torch.ones(6, 4, device=cuda_device).t())):
+        with pytest.raises(RuntimeError, match="dense"):
+            AdamWCuda([p])
+        opt = AdamWCuda([torch.nn.Parameter(torch.ones(2, device=cuda_device))])
+        with pytest.raises(RuntimeError, match="dense"):
+            opt.add_param_group({"params": [p]})
+        assert len(opt.param_groups) == 1
+    with pytest.raises(RuntimeError, match="supports"):
+        opt.add_param_group({"params": [torch.nn.Parameter(torch.ones(2, device=cuda_device).double())]})
+    assert len(opt.param_groups) == 1
+    opt.add_param_group({"params": (torch.nn.Parameter(torch.ones(n, device=cuda_device)) for n in (1, 2))})
+    assert [len(g["params"]) for g in opt.param_groups] == [1, 2]

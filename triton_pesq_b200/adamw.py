@@ -48,7 +48,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mo
     Parameters
     ----------
     params
-        Dense float32 tensors on one GPU.
+        Float32 tensors on one GPU, dense in the order of their dimensions.
     grads
         Their gradients, all float32, bfloat16 or float16 (dense, or they are
         copied).  An empty tensor leaves its parameter and moments as they are.
@@ -111,8 +111,9 @@ class AdamWCuda(torch.optim.Optimizer):
     Parameters
     ----------
     params
-        Parameters or parameter groups, dense, on GPUs: float32, or bfloat16 /
-        float16, which are then the rounded copies of float32 masters in the state.
+        Parameters or parameter groups, on GPUs, dense in the order of their
+        dimensions (channels-last weights are not): float32, or bfloat16 / float16,
+        which are then the rounded copies of float32 masters in the state.
     lr, betas, eps, weight_decay
         As in ``torch.optim.AdamW``; each may differ between groups.
     state_bits : int
@@ -144,8 +145,15 @@ class AdamWCuda(torch.optim.Optimizer):
     def add_param_group(self, param_group) -> None:
         super().add_param_group(param_group)
         for p in self.param_groups[-1]["params"]:
+            why = None
             if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
-                raise RuntimeError(f"AdamWCuda supports float32, bfloat16 and float16 parameters, not {p.dtype}.")
+                why = f"AdamWCuda supports float32, bfloat16 and float16 parameters, not {p.dtype}."
+            elif not p.is_contiguous():
+                why = (f"AdamWCuda needs dense parameters in the order of their dimensions, got shape {tuple(p.shape)} "
+                       f"with strides {p.stride()}.")
+            if why:
+                self.param_groups.pop()
+                raise RuntimeError(why)
 
     def _flat(self, index: int) -> List[_Flat]:
         flats = self._flats.get(index)
