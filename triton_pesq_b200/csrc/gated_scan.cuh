@@ -238,6 +238,11 @@ __device__ __forceinline__ Vec<N> apply(Vec<N> a, Vec<N> h, Vec<N> b) {
   }
   return fma(a, h, b);
 }
+// The factor of a map that `a` comes after, as apply() looks at it: a = 0 cuts off what was not finite too
+template <bool kMask>
+__device__ __forceinline__ Vec<1> chain(Vec<1> a, Vec<1> A) {
+  return kMask && a.v[0] == 0.0f ? Vec<1>{{0.0f}} : A * a;
+}
 
 // What a lane works on, and where its strip lies.  Chunks are counted in the order of
 // the steps' scan.
@@ -470,14 +475,15 @@ __device__ __forceinline__ void join_maps(const Args& p, const Lane& o, Vec<1> A
   for (int w = 0; w < (int)threadIdx.y; ++w) {
     const float2 m = s_map[w][threadIdx.x];
     h = apply<kMask>(Vec<1>{{m.x}}, h, Vec<1>{{m.y}});
-    a.v[0] *= m.x;
+    a = chain<kMask>(Vec<1>{{m.x}}, a);
   }
   p.before[(o.b * p.strips + o.rank) * p.width + o.c] = make_float2(a.v[0], h.v[0]);
   if ((int)threadIdx.y == strips - 1 || o.rank == p.strips - 1) {
     const float2 m = s_map[threadIdx.y][threadIdx.x];
     h = apply<kMask>(Vec<1>{{m.x}}, h, Vec<1>{{m.y}});
     const int ctas = (p.strips + strips - 1) / strips;
-    p.total[(o.b * ctas + o.rank / strips) * p.width + o.c] = make_float2(a.v[0] * m.x, h.v[0]);
+    p.total[(o.b * ctas + o.rank / strips) * p.width + o.c] =
+        make_float2(chain<kMask>(Vec<1>{{m.x}}, a).v[0], h.v[0]);
   }
 }
 
@@ -725,7 +731,7 @@ __device__ __forceinline__ void forward_maps(const Args& p, const Lane& o, R& ri
 #pragma unroll
     for (int l = 0; l < L; ++l) {
       H = apply<kMask>(C::at(g.a, l), H, C::at(b, l));
-      A = A * C::at(g.a, l);
+      A = chain<kMask>(C::at(g.a, l), A);
     }
   });
   join_maps<kMask>(p, o, A, H);
@@ -862,7 +868,7 @@ __device__ __forceinline__ void forward_row(const Args& p, const Lane& o, R& rin
 #pragma unroll
     for (int l = 0; l < L; ++l) {
       H = apply<kMask>(C::at(a[c], l), H, C::at(b[c], l));
-      A = A * C::at(a[c], l);
+      A = chain<kMask>(C::at(a[c], l), A);
     }
   }
   if constexpr (!std::is_same<R, NoRing>::value) {
@@ -1003,7 +1009,7 @@ __device__ __forceinline__ void backward_maps(const Args& p, const Lane& o, R& r
       Vec<1> al = C::at(a, l);
       if (kMask && ((cut >> l) & 1u)) al = splat<1>(0.0f);
       E = apply<kMask>(al, E + widen<1>(in.dy[l], 0), splat<1>(0.0f));
-      A = A * al;
+      A = chain<kMask>(al, A);
     }
   });
   join_maps<kMask>(p, o, A, E);
