@@ -46,3 +46,21 @@ def test_what_a_reset_parts(cuda_device, shape, dtype, reverse, which, late):
         assert torch.equal(a[:, free], b[:, free])
     assert torch.equal(got[6], clean[6]) if late else torch.equal(got[1], clean[1])
     assert torch.isnan(got[0][:, order[cut + 2 if late else cut - 2]]).all()
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("reverse", [False, True])
+def test_a_reset_does_not_look_at_its_decay_gate(cuda_device, shape, reverse):
+    """a = 0 there whatever the gate holds: the gate's gradient is zero, and nothing else changes."""
+
+    batch, steps, width = shape
+    g = torch.Generator(cuda_device).manual_seed(1)
+    dev = [torch.randn(*shape, device=cuda_device, generator=g) for _ in range(3)]
+    dev += [torch.linspace(-5, 1, width, device=cuda_device), torch.randn(batch, width, device=cuda_device, generator=g)]
+    dy, dlast = torch.randn(*shape, device=cuda_device, generator=g), torch.ones(batch, width, device=cuda_device)
+    reset = torch.rand(batch, steps, device=cuda_device, generator=g) < 0.1
+    clean = call(dev, dy, dlast, reset, reverse)
+    dev[2] = torch.where(reset[:, :, None], float("nan"), dev[2])
+    for a, b in zip(call(dev, dy, dlast, reset, reverse), clean):
+        assert torch.equal(a, b)
+    assert not clean[4][reset].any()

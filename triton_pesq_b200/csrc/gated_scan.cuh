@@ -1103,12 +1103,12 @@ __device__ __forceinline__ void backward_chunk(const Args& p, const Lane& o, con
   for (int i = 0; i < G; ++i) {
     p1[i] = g[i] * p1[i];
     Vec<N> s = g[i] * r1[i];
-    if (kMask) {  // (a gradient that is not finite is not spread to where nothing flows)
+    if (kMask) {  // (a gradient, or a reset's decay gate, that is not finite is not spread to where nothing flows)
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         const int l = V == N ? i : i * N + j;
         if (!((in.q.live >> l) & 1u)) p1[i].v[j] = 0.0f;
-        if (r1[i].v[j] == 0.0f) s.v[j] = 0.0f;
+        if (r1[i].v[j] == 0.0f) s.v[j] = 0.0f, r2[i].v[j] = 0.0f;
       }
     }
     p2[i] = p1[i] * p2[i];

@@ -54,7 +54,7 @@ def gated_scan(x: torch.Tensor, input_gate: torch.Tensor, decay_gate: torch.Tens
     state
         float32 ``[batch, channel]``, the state before the first step (zeros).
     reset
-        bool ``[batch, step]``: the step forgets the state (``a = 0``), so that
+        bool ``[batch, step]``: the step forgets the state (``a = 0`` whatever its decay gate), so that
         several utterances can share a row.
     lengths
         int64 or int32 ``[batch]``: steps at or past a row's length leave its
