@@ -89,6 +89,13 @@ void no_second_derivative(const char* op) {
   TORCH_CHECK(!at::GradMode::is_enabled(), "The CUDA ", op, " has no second derivative (create_graph=True).");
 }
 
+bool has_tangent(const at::Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+bool has_tangent(const OptTensor& t) { return t.has_value() && has_tangent(*t); }
+template <class... Ts>
+void no_forward_mode(const char* op, const Ts&... inputs) {
+  TORCH_CHECK(!(has_tangent(inputs) || ...), "The CUDA ", op, " has no forward-mode derivative.");
+}
+
 bool wants_grad(const at::Tensor& t) { return t.requires_grad(); }
 bool wants_grad(const OptTensor& t) { return t.has_value() && t->defined() && t->requires_grad(); }
 
@@ -279,6 +286,7 @@ std::tuple<at::Tensor, at::Tensor> gated_scan(const at::Tensor& x, const at::Ten
                                               const at::Tensor& decay, const OptTensor& state, const OptTensor& reset,
                                               const OptTensor& lengths, bool reverse, double rate) {
   check_cuda(x, x, kScan, "x");
+  no_forward_mode(kScan, x, ig, rg, decay, state);
   if (at::GradMode::is_enabled() &&
       (wants_grad(x) || wants_grad(ig) || wants_grad(rg) || wants_grad(decay) || wants_grad(state))) {
     auto out = GatedScan::apply(x, ig, rg, decay, state, reset, lengths, reverse, rate);
@@ -462,6 +470,7 @@ std::tuple<at::Tensor, at::Tensor> norm_join(const at::Tensor& x, const OptTenso
                                              double eps, bool silu, int64_t dtype) {
   check_cuda(x, x, kJoin, "stream");
   TORCH_CHECK(x.dim() == 3, "The CUDA norm join needs `stream` [batch, step, channel], got ", x.sizes(), ".");
+  no_forward_mode(kJoin, x, z, g_, post, pre, scale);
   // one gate row for all steps of a batch item is summed by the kernels, any other broadcast by torch
   OptTensor g = g_;
   bool shared = false;

@@ -67,7 +67,7 @@ def gated_scan(x: torch.Tensor, input_gate: torch.Tensor, decay_gate: torch.Tens
     Returns
     -------
     ``(y, last)``: ``[batch, step, channel]`` in the type of ``x``, and the
-    float32 state after the last step.  Differentiable once, in all inputs but
+    float32 state after the last step.  Differentiable once, in reverse mode, in all inputs but
     the masks.
     """
 

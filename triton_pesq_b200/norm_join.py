@@ -66,7 +66,7 @@ def norm_join(stream: torch.Tensor, block: torch.Tensor, post_weight: torch.Tens
     Returns
     -------
     ``(stream', normed)``, in the types of ``stream`` and ``block``.  Differentiable
-    once in every operand.
+    once, in reverse mode, in every operand.
     """
 
     op = _op or _load()
