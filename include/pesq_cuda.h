@@ -364,7 +364,7 @@ typedef struct pesq_gated_scan_desc {
   int32_t dtype;      /* PESQ_F32, PESQ_BF16 or PESQ_F16: x, the gates, y and their gradients */
   int32_t reverse;    /* scan from the last step to the first */
   float rate;         /* > 0 */
-  int32_t reserved0;
+  int32_t kept_steps; /* of a backward: its forward's pesq_gated_scan_kept_steps; 0: of streams laid out as here */
   pesq_stream x, input_gate, decay_gate;
   const float* decay; /* [width] */
   const float* state; /* [batch, width], the state before the first step; NULL: zeros */
@@ -374,17 +374,21 @@ typedef struct pesq_gated_scan_desc {
 } pesq_gated_scan_desc;
 
 /* Bytes (16-byte aligned buffers) of a forward's workspace, of the states it
- * keeps for a backward call, and of the backward's workspace. */
+ * keeps for a backward call, which follow from the sizes alone, and of the
+ * backward's workspace. */
 int pesq_gated_scan_sizes(const pesq_gated_scan_desc* desc, size_t* forward, size_t* kept, size_t* backward);
+/* Steps between the states that a forward of these streams keeps, and the most
+ * that a forward of streams of these sizes, laid out in any way, may have left
+ * between them.  A backward takes states that are as close as its own streams' or closer. */
+int pesq_gated_scan_kept_steps(const pesq_gated_scan_desc* desc, int32_t* here, int32_t* most);
 /* y: [batch, steps, width] dense; last: [batch, width], the state after the
  * last step; kept: for the backward call, or NULL. */
 int pesq_gated_scan_forward(const pesq_gated_scan_desc* desc, void* stream, void* y, float* last, void* kept,
                             size_t kept_bytes, void* workspace, size_t workspace_bytes);
 /* dy.data and dlast may be NULL (zeros); dstate may be NULL (not wanted).
  * dx, dinput_gate, ddecay_gate: dense; ddecay: [width].  Gradients are at
- * least as aligned as the inputs, dy's strides too.  kept_bytes: of the forward,
- * as pesq_gated_scan_sizes gives it for the streams' addresses and strides there;
- * of streams that are laid out otherwise here it is another number, and refused. */
+ * least as aligned as the inputs, dy's strides too.  kept: of a forward of the
+ * same values; states that desc->kept_steps says are too far apart for these streams are refused. */
 int pesq_gated_scan_backward(const pesq_gated_scan_desc* desc, void* stream, const void* kept, size_t kept_bytes,
                              pesq_stream dy, const float* dlast, void* dx, void* dinput_gate, void* ddecay_gate,
                              float* ddecay, float* dstate, void* workspace, size_t workspace_bytes);

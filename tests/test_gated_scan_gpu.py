@@ -407,3 +407,40 @@ def test_saved_streams_that_come_back_in_another_layout(cuda_device, dtype, dens
     want = torch.autograd.grad((wy, wl), wide, (dy.double(), dlast.double()))
     for name, g, w in zip(NAMES, got, want):
         R.close(g, w, GTOL, "d " + name)
+
+
+@pytest.mark.parametrize("steps", [90, 300, 1000])
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dense_first", [False, True])
+def test_saved_streams_in_another_layout_with_lengths(cuda_device, steps, reverse, dense_first):
+    """The states that the forward keeps serve a backward of any layout, wherever the rows end: the same bits as
+    with one layout in both."""
+
+    def strided(t):
+        out = torch.empty(t.shape[0], t.shape[1], t.shape[2] + 1, dtype=t.dtype, device=t.device)[..., 1:]
+        return out.copy_(t)
+
+    lengths = torch.tensor([0, 1, 7, 8, 9, 15, 16, 17, 23, 24, 25, 31, 32, 33, 63, steps - 9, steps - 8, steps - 1, steps])
+    tensors, dy, dlast = inputs(len(lengths), steps, 64, torch.float32, seed=7)
+    dev, dy, dlast = [t.to(cuda_device) for t in tensors], dy.to(cuda_device), dlast.to(cuda_device)
+    first, then = (torch.Tensor.contiguous, strided) if dense_first else (strided, torch.Tensor.contiguous)
+
+    def call(at_first, later):
+        leaves = [(at_first(t) if t.dim() == 3 else t).detach().requires_grad_(True) for t in dev]
+        relay = lambda t: later(t) if t.dim() == 3 else t  # noqa: E731
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), relay):
+            y, last = gated_scan(*leaves, lengths=lengths.to(cuda_device), reverse=reverse)
+        return torch.autograd.grad((y, last), leaves, (dy, dlast))
+
+    want = call(then, then)
+    # states of a forward of which nothing is known
+    lasts = (*[first(t) for t in dev[:3]], *dev[3:], None, lengths.to(cuda_device), reverse, 8.0)
+    _, _, kept = torch.ops.pesq_cuda.gated_scan_forward(*lasts, True)
+    laters = (*[then(t) for t in dev[:3]], *lasts[3:])
+    for a, b in zip(torch.ops.pesq_cuda.gated_scan_backward(*laters, kept, 0, dy, dlast), want):
+        R.close(a, b.double(), 1e-5, "of an unknown forward")
+    for name, a, b in zip(NAMES, call(first, then), want):
+        if name == "decay":  # (a sum over strips, whose number is the layout's)
+            R.close(a, b.double(), 1e-5, name)
+        else:
+            R.close(a, b.double(), 1e-6, name)

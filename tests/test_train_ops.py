@@ -134,3 +134,33 @@ def test_adamw_entry_checks_its_descriptor():
                 {"beta1": float("nan")}, {"lr": -1.0}, {"eps": float("nan")}, {"weight_decay": -0.5}):
         assert step(**bad) == 1, bad
     assert step(n=257) == _lib.PESQ_ERR_WORKSPACE
+
+
+def test_gated_scan_keeps_the_same_whatever_the_layout():
+    """A tracer has shapes alone to go by."""
+    for steps, width in ((1, 64), (16, 64), (90, 64), (1000, 96), (300, 33)):
+        want = _sizes(_scan(batch=3, steps=steps, width=width))[1][1]
+        for dtype in (_lib.F32, _lib.BF16):
+            for at, stride in ((0, width), (16, width), (8, 3 * width), (2, width + 1)):
+                layout = _lib.Stream(data=4096 + at, batch_stride=steps * stride, step_stride=stride)
+                d = _scan(batch=3, steps=steps, width=width, dtype=dtype, x=layout, input_gate=layout, decay_gate=layout)
+                assert _sizes(d)[1][1] == want
+
+
+def test_gated_scan_says_how_far_apart_it_keeps_its_states():
+    """As far as chunks, which follow from the layout; a backward that needs them closer refuses them."""
+    lib, one = _lib.library(), ctypes.c_void_p(4096)
+    here, most = ctypes.c_int32(), ctypes.c_int32()
+    boxes = _lib.Stream(data=4096, batch_stride=100 * 64, step_stride=64)
+    lanes = _lib.Stream(data=4096 + 2, batch_stride=100 * 64, step_stride=64)
+    cases = ((boxes, 100, 64, 16, 16), (lanes, 100, 64, 8, 16), (lanes, 100, 63, 8, 8), (lanes, 10, 64, 8, 8), (boxes, 1, 64, 1, 1))
+    for stream, steps, width, want, longest in cases:
+        d = _scan(steps=steps, width=width, x=stream, input_gate=stream, decay_gate=stream)
+        assert lib.pesq_gated_scan_kept_steps(ctypes.byref(d), ctypes.byref(here), ctypes.byref(most)) == _lib.PESQ_OK
+        assert (here.value, most.value) == (want, longest)
+    assert lib.pesq_gated_scan_kept_steps(ctypes.byref(d), None, ctypes.byref(most)) == 1
+    d = _scan(x=lanes, input_gate=lanes, decay_gate=lanes, kept_steps=16)
+    none = _lib.Stream(data=None, batch_stride=0, step_stride=0)
+    assert lib.pesq_gated_scan_backward(ctypes.byref(d), None, one, 1 << 30, none, None, one, one, one, one, None, one,
+                                        1 << 30) == 1
+    assert "too far apart" in _lib.last_error()

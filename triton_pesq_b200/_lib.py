@@ -141,7 +141,7 @@ class GatedScanDesc(ctypes.Structure):
         ("dtype", ctypes.c_int32),
         ("reverse", ctypes.c_int32),
         ("rate", ctypes.c_float),
-        ("reserved0", ctypes.c_int32),
+        ("kept_steps", ctypes.c_int32),
         ("x", Stream),
         ("input_gate", Stream),
         ("decay_gate", Stream),
@@ -296,6 +296,10 @@ SIGNATURES = {
         [ctypes.POINTER(GatedScanDesc), ctypes.POINTER(ctypes.c_size_t), ctypes.POINTER(ctypes.c_size_t),
          ctypes.POINTER(ctypes.c_size_t)],
     ),
+    "pesq_gated_scan_kept_steps": (
+        ctypes.c_int,
+        [ctypes.POINTER(GatedScanDesc), ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32)],
+    ),
     "pesq_gated_scan_forward": (
         ctypes.c_int,
         [ctypes.POINTER(GatedScanDesc), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
@@ -414,18 +418,14 @@ def _register_fakes() -> None:
 
     @torch.library.register_fake("pesq_cuda::gated_scan_forward")
     def _gated_scan(x, input_gate, decay_gate, decay, state, reset, lengths, reverse, rate, keep):
-        kept = 0
-        if keep and x.numel():
-            desc = GatedScanDesc(batch=x.shape[0], steps=x.shape[1], width=x.shape[2], rate=1.0)
-            sizes = [ctypes.c_size_t() for _ in range(3)]
-            check(library().pesq_gated_scan_sizes(ctypes.byref(desc), *[ctypes.byref(n) for n in sizes]),
-                  "pesq_gated_scan_sizes")
-            kept = sizes[1].value
+        # room for a state before every eighth step, to 16 bytes
+        kept = (x.shape[0] * ((x.shape[1] + 7) // 8) * x.shape[2] * 4 + 15) // 16 * 16 if keep else 0
         return (x.new_empty(x.shape), x.new_empty((x.shape[0], x.shape[2]), dtype=torch.float32),
                 x.new_empty((kept,), dtype=torch.uint8))
 
     @torch.library.register_fake("pesq_cuda::gated_scan_backward")
-    def _gated_scan_backward(x, input_gate, decay_gate, decay, state, reset, lengths, reverse, rate, kept, dy, dlast):
+    def _gated_scan_backward(x, input_gate, decay_gate, decay, state, reset, lengths, reverse, rate, kept, kept_steps, dy,
+                             dlast):
         return (x.new_empty(x.shape), x.new_empty(x.shape), x.new_empty(x.shape),
                 x.new_empty((x.shape[2],), dtype=torch.float32),
                 x.new_empty((x.shape[0], x.shape[2]), dtype=torch.float32))

@@ -49,8 +49,10 @@
 //   ddecay = -rate sigmoid(decay) sum over rows and steps of dlog a r.
 // h is not read back from the rounded y: the forward keeps the state before every
 // chunk in 32 bits (1 / 8 or 1 / 16 of the elements), and the backward recomputes the
-// chunk from it, by the same operations.  beta -> 0 only together with log a, whose quotient goes to
-// zero: the term is dropped there.
+// chunk from it, by the same operations.  Chunks follow from the streams' addresses and strides, which
+// may be others by the time of the backward, while a tracer needs the buffer's size from shapes alone: it
+// has room for a state before every eighth step, of which chunks of 16 fill every other one.
+// beta -> 0 only together with log a, whose quotient goes to zero: the term is dropped there.
 #pragma once
 
 #include <cuda.h>
@@ -69,6 +71,7 @@ using namespace train;
 // steps of a chunk, by the channels of a lane: in shared memory sixteen elements of each
 // stream either way, in registers no more than 8 steps
 constexpr int chunk_steps(int vec, bool bulk) { return bulk ? 16 / vec : 8; }
+constexpr int kKept = 8;  // steps between the places for states that a forward keeps
 constexpr int kStrips = 8;  // strips (warps) of a CTA at most, where rows are cut
 // CTAs of so many strips (4 or 8) that an SM holds by registers and shared memory, of elements of `size` bytes
 constexpr int forward_ctas(int strips, bool bulk, int size) {
@@ -107,7 +110,7 @@ struct Args {
   // and of a CTA's strips, [batch][CTA][width]; ranks count in the order of the scan at hand
   float2* before;
   float2* total;
-  float* kept;                // state before every chunk, [batch][chunk][width]
+  float* kept;                // state before every chunk, [batch][its first step / 8][width]
   // forward
   void* y;
   float* last;
@@ -139,6 +142,12 @@ __device__ __forceinline__ float softplus(float v) {
   p = fmaf(q, p, 1.0f / 3);
   p = fmaf(q, p, 1.0f);
   return max_nan(v, 0.0f) + 2.0f * s * p;
+}
+
+// The place of the state before chunk k
+template <int L>
+__device__ __forceinline__ int64_t kept_at(const Args& p, int64_t b, int k) {
+  return (b * ((p.steps + kKept - 1) / kKept) + (int64_t)k * (L > kKept ? L / kKept : 1)) * p.width;
 }
 
 // The decay gate that steps past the length and outside the row read as
@@ -277,7 +286,8 @@ __device__ __forceinline__ Lane lane_of(const Args& p) {
   o.dir = p.reverse ? -1 : 1;
   if (kMask && p.lengths) {
     o.len = (int)max(INT64_C(0), min(p.lengths[o.b], p.steps));
-    o.lo = p.reverse ? (steps - o.len) / L : 0;
+    // (from a multiple of 16 steps on with chunks of eight too, for the states that chunks of 16 ask for)
+    o.lo = p.reverse ? (steps - o.len) / 16 * 16 / L : 0;
     o.hi = o.len == 0 ? o.lo : p.reverse ? all : (o.len + L - 1) / L;
     per = (o.hi - o.lo + p.strips - 1) / p.strips;
   }
@@ -575,7 +585,7 @@ struct Ring {
           "l"(map[i]), "r"(smem_u32(bar + stage)), "r"(c0), "r"(t0), "r"((int)o.b)
           : "memory");
     if (kState)
-      bulk_g2s(to + S * kBox, p.kept + (o.b * ((p.steps + L - 1) / L) + k) * p.width + o.c, state, bar + stage);
+      bulk_g2s(to + S * kBox, p.kept + kept_at<L>(p, o.b, k) + o.c, state, bar + stage);
   }
   // one stream of the stage, in scan order
   __device__ __forceinline__ void get(const Args& p, int stage, int i, Pack<T, V> (&out)[L]) const {
@@ -771,7 +781,7 @@ __device__ __forceinline__ void forward_chunk(const Args& p, const Lane& o, cons
                                               Vec<V> rate, Vec<V>& h) {
   using C = Cells<V, L>;
   if (p.kept && o.on) {
-    float* keep = p.kept + (o.b * ((p.steps + L - 1) / L) + k) * p.width + o.c;
+    float* keep = p.kept + kept_at<L>(p, o.b, k) + o.c;
 #pragma unroll
     for (int v = 0; v < V; ++v) keep[v] = h.v[v];
   }
@@ -889,7 +899,7 @@ __device__ __forceinline__ void forward_row(const Args& p, const Lane& o, R& rin
   for (int c = 0; c < NC; ++c) {
     if (c >= o.count) continue;
     const Chunk q = chunk_of<L, kMask>(p, o, o.first + c);
-    if (p.kept) p.kept[(o.b * ((p.steps + L - 1) / L) + o.first + c) * p.width + o.c] = h.v[0];
+    if (p.kept) p.kept[kept_at<L>(p, o.b, o.first + c) + o.c] = h.v[0];
     char* y = reinterpret_cast<char*>(static_cast<T*>(p.y) + (o.b * p.steps + q.t0) * p.width + o.c);
     const int step = o.dir * (int)p.width * (int)sizeof(T);
 #pragma unroll
@@ -958,7 +968,7 @@ struct LoadedBack {
     load<T, V, L, kFull>(ig, p.ig, o, q);
     load<T, V, L, kFull>(x, p.x, o, q);
     load<T, V, L, kFull>(dy, p.dy, o, q);
-    h = read_row<V>(p.kept + (o.b * ((p.steps + L - 1) / L) + k) * p.width + o.from);
+    h = read_row<V>(p.kept + kept_at<L>(p, o.b, k) + o.from);
   }
 };
 

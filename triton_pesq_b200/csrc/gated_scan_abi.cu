@@ -123,7 +123,6 @@ EncodeTiled encoder() {
   return fn;
 }
 
-// Chunks follow from the inputs alone, so that a backward call takes its forward's.
 Geometry geometry(const pesq_gated_scan_desc& d, bool backward) {
   Geometry g{};
   const int size = (int)element(d.dtype);
@@ -184,8 +183,8 @@ size_t map_bytes(const pesq_gated_scan_desc& d, const Geometry& g) {
   if (g.strips == 1 || g.row) return 0;
   return round16((size_t)(d.batch * (g.strips + (g.strips + g.warps - 1) / g.warps) * d.width) * 8);
 }
-size_t kept_bytes(const pesq_gated_scan_desc& d, const Geometry& g) {
-  return round16((size_t)(d.batch * ((d.steps + g.chunk - 1) / g.chunk) * d.width) * 4);
+size_t kept_bytes(const pesq_gated_scan_desc& d) {  // (of the sizes alone)
+  return round16((size_t)(d.batch * ((d.steps + kKept - 1) / kKept) * d.width) * 4);
 }
 size_t part_bytes(const pesq_gated_scan_desc& d, const Geometry& g) {
   return round16((size_t)(d.batch * g.strips * d.width) * 4);
@@ -283,8 +282,18 @@ int pesq_gated_scan_sizes(const pesq_gated_scan_desc* d, size_t* forward, size_t
   if (const int status = check(d)) return status;
   const Geometry g = geometry(*d, false);
   *forward = map_bytes(*d, g);
-  *kept = kept_bytes(*d, g);
+  *kept = kept_bytes(*d);
   *backward = back_bytes(*d, geometry(*d, true));
+  return PESQ_OK;
+}
+
+int pesq_gated_scan_kept_steps(const pesq_gated_scan_desc* d, int32_t* here, int32_t* most) {
+  if (!here || !most) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL argument");
+  if (const int status = check(d)) return status;
+  *here = geometry(*d, false).chunk;
+  pesq_gated_scan_desc dense = *d;  // what tensor copies take is what has the longest chunks
+  dense.x = dense.input_gate = dense.decay_gate = {reinterpret_cast<const void*>(256), d->steps * d->width, d->width};
+  *most = std::max(*here, (int32_t)geometry(dense, false).chunk);
   return PESQ_OK;
 }
 
@@ -294,7 +303,7 @@ int pesq_gated_scan_forward(const pesq_gated_scan_desc* d, void* stream, void* y
   if (!y || !last) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL output");
   const Geometry g = geometry(*d, false);
   if (!fits(y, g, *d)) return set_error(PESQ_ERR_INVALID_ARGUMENT, "y is less aligned than the inputs");
-  if (missing(workspace, workspace_bytes, map_bytes(*d, g)) || (kept && missing(kept, kept_size, kept_bytes(*d, g))))
+  if (missing(workspace, workspace_bytes, map_bytes(*d, g)) || (kept && missing(kept, kept_size, kept_bytes(*d))))
     return set_error(PESQ_ERR_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
   Args a{};
   if (const int status = prepare(*d, g, static_cast<char*>(workspace), a)) return status;
@@ -313,8 +322,10 @@ int pesq_gated_scan_backward(const pesq_gated_scan_desc* d, void* stream, const 
   if ((dy.data && (g.bulk ? !boxes(dy, *d) : !fits(dy, g.vec, *d))) || !fits(dx, g, *d) || !fits(dinput_gate, g, *d) ||
       !fits(ddecay_gate, g, *d))
     return set_error(PESQ_ERR_INVALID_ARGUMENT, "a gradient is less aligned than the inputs");
-  if (missing(kept, kept_size, kept_bytes(*d, g)) || kept_size != kept_bytes(*d, g))
-    return set_error(PESQ_ERR_WORKSPACE, "the states that the forward kept are missing, or of streams laid out otherwise");
+  if (missing(kept, kept_size, kept_bytes(*d)))
+    return set_error(PESQ_ERR_WORKSPACE, "the states that the forward kept are missing");
+  if (d->kept_steps > g.chunk)
+    return set_error(PESQ_ERR_INVALID_ARGUMENT, "the forward kept its states too far apart for streams laid out like these");
   if (missing(workspace, workspace_bytes, back_bytes(*d, g)))
     return set_error(PESQ_ERR_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
   const cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -166,6 +166,9 @@ struct ScanCall {
   bool empty() const { return d.batch == 0 || d.steps == 0 || d.width == 0; }
 };
 
+// Steps between the states that this thread's last forward kept; 0 where a tracer stood in for it
+thread_local int64_t scan_kept_steps = 0;
+
 // (y, last, the states kept for the backward where `keep`)
 std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_scan_forward(const at::Tensor& x, const at::Tensor& ig,
                                                                   const at::Tensor& rg, const at::Tensor& decay,
@@ -192,13 +195,18 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_scan_forward(const at::Tens
   check_status(pesq_gated_scan_forward(&c.d, at::cuda::getCurrentCUDAStream(), y.data_ptr(), last.data_ptr<float>(),
                                        keep ? states.data_ptr() : nullptr, kept, work ? ws.data_ptr() : nullptr, work),
                "pesq_gated_scan_forward");
+  if (keep) {
+    int32_t here = 0, most = 0;
+    check_status(pesq_gated_scan_kept_steps(&c.d, &here, &most), "pesq_gated_scan_kept_steps");
+    scan_kept_steps = here;
+  }
   return {y, last, states};
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> gated_scan_backward(
     const at::Tensor& x, const at::Tensor& ig, const at::Tensor& rg, const at::Tensor& decay, const OptTensor& state,
     const OptTensor& reset, const OptTensor& lengths, bool reverse, double rate, const at::Tensor& kept,
-    const OptTensor& dy_, const OptTensor& dlast_) {
+    int64_t kept_steps, const OptTensor& dy_, const OptTensor& dlast_) {
   ScanCall c(x, ig, rg, decay, state, reset, lengths, reverse, rate);
   c10::cuda::CUDAGuard guard(x.device());
   const auto f32 = x.options().dtype(at::kFloat);
@@ -224,10 +232,15 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> gated_sca
   }
   size_t work = 0, states = 0, back = 0;
   check_status(pesq_gated_scan_sizes(&c.d, &work, &states, &back), "pesq_gated_scan_sizes");
+  check_cuda(kept, x, kScan, "kept");
+  TORCH_CHECK(kept.scalar_type() == at::kByte && kept.is_contiguous() && kept.numel() == static_cast<int64_t>(states),
+              "The CUDA gated scan needs the states that its forward kept.");
   at::Tensor ws = at::empty({static_cast<int64_t>(back)}, f32.dtype(at::kByte)), before = kept;
-  // (the chunks that states are kept of follow from the streams' layout, and hooks on what autograd saves
-  // may bring the streams back in another)
-  if (kept.numel() != static_cast<int64_t>(states))
+  // (hooks on what autograd saves, or a compiler, may bring the streams back in another layout than the forward's,
+  // one that asks for states closer together)
+  int32_t here = 0, most = 0;
+  check_status(pesq_gated_scan_kept_steps(&c.d, &here, &most), "pesq_gated_scan_kept_steps");
+  if ((kept_steps > 0 ? kept_steps : most) > here)
     before = std::get<2>(gated_scan_forward(x, ig, rg, decay, state, reset, lengths, reverse, rate, true));
   check_status(pesq_gated_scan_backward(&c.d, at::cuda::getCurrentCUDAStream(), before.data_ptr(), states, dys,
                                         dlast.defined() ? dlast.data_ptr<float>() : nullptr, dx.data_ptr(),
@@ -255,12 +268,14 @@ struct GatedScan : public torch::autograd::Function<GatedScan> {
                                const at::Tensor& decay, const OptTensor& state, const OptTensor& reset,
                                const OptTensor& lengths, bool reverse, double rate) {
     at::AutoDispatchBelowADInplaceOrView below;
+    scan_kept_steps = 0;
     auto [y, last, kept] = scan_forward_op().call(x, ig, rg, decay, state, reset, lengths, reverse, rate, true);
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({x, ig, rg, decay, state.value_or(at::Tensor()), reset.value_or(at::Tensor()),
                             lengths.value_or(at::Tensor()), kept});
     ctx->saved_data["reverse"] = reverse;
     ctx->saved_data["rate"] = rate;
+    ctx->saved_data["kept_steps"] = scan_kept_steps;
     return {y, last};
   }
 
@@ -271,8 +286,8 @@ struct GatedScan : public torch::autograd::Function<GatedScan> {
     if (!g[0].defined() && !g[1].defined()) return out;
     auto [dx, dig, drg, ddecay, dstate] = scan_backward_op().call(
         s[0], s[1], s[2], s[3], optional_of(s[4]), optional_of(s[5]), optional_of(s[6]),
-        ctx->saved_data["reverse"].toBool(), ctx->saved_data["rate"].toDouble(), s[7], optional_of(g[0]),
-        optional_of(g[1]));
+        ctx->saved_data["reverse"].toBool(), ctx->saved_data["rate"].toDouble(), s[7],
+        ctx->saved_data["kept_steps"].toInt(), optional_of(g[0]), optional_of(g[1]));
     out[0] = dx;
     out[1] = dig;
     out[2] = drg;
@@ -596,7 +611,7 @@ TORCH_LIBRARY_FRAGMENT(pesq_cuda, m) {
   m.def((std::string("gated_scan") + scan_in + ") -> (Tensor, Tensor)").c_str());
   m.def((std::string("gated_scan_forward") + scan_in + ", bool keep) -> (Tensor, Tensor, Tensor)").c_str());
   m.def((std::string("gated_scan_backward") + scan_in +
-         ", Tensor kept, Tensor? dy, Tensor? dlast) -> (Tensor, Tensor, Tensor, Tensor, Tensor)")
+         ", Tensor kept, int kept_steps, Tensor? dy, Tensor? dlast) -> (Tensor, Tensor, Tensor, Tensor, Tensor)")
             .c_str());
   const char* join_in = "(Tensor stream, Tensor? block, Tensor? gate, Tensor? post, Tensor pre, Tensor? scale, float eps, bool silu";
   m.def((std::string("norm_join") + join_in + ", int dtype) -> (Tensor, Tensor)").c_str());
