@@ -60,6 +60,13 @@ void check_float(const at::Tensor& t, const char* op, const char* name) {
               ".");
 }
 
+bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+void check_gradient(const at::Tensor& t, const at::Tensor& of, at::IntArrayRef want, const char* op, const char* name) {
+  check_cuda(t, of, op, name);
+  check_shape(t, want, op, name);
+}
+
 // channels adjacent, steps less than 2 GiB apart
 at::Tensor rows(const at::Tensor& t) {
   const int64_t far = INT64_C(0x7fffffff) / t.element_size();
@@ -214,7 +221,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> gated_sca
              drg = at::empty(x.sizes(), x.options());
   at::Tensor ddecay = at::empty({c.d.width}, f32), dstate = at::empty({c.d.batch, c.d.width}, f32);
   at::Tensor dlast;
-  if (dlast_.has_value() && dlast_->defined()) dlast = dlast_->contiguous();
+  if (given(dy_)) check_gradient(*dy_, x, x.sizes(), kScan, "dy");
+  if (given(dlast_)) {
+    check_gradient(*dlast_, x, {c.d.batch, c.d.width}, kScan, "dlast");
+    dlast = dlast_->to(at::kFloat).contiguous();
+  }
   if (c.empty()) {
     ddecay.zero_();
     if (dlast.defined()) {
@@ -226,7 +237,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> gated_sca
   }
   at::Tensor dy;
   pesq_stream dys{nullptr, 0, 0};
-  if (dy_.has_value() && dy_->defined()) {
+  if (given(dy_)) {
     dy = aligned(rows(dy_->to(x.scalar_type())));
     dys = stream_of(dy);
   }
@@ -314,8 +325,6 @@ std::tuple<at::Tensor, at::Tensor> gated_scan(const at::Tensor& x, const at::Ten
 // ------------------------------------------------------------------- norm join
 
 constexpr const char* kJoin = "norm join";
-
-bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
 
 struct JoinCall {
   at::Tensor x, z, g, post, pre, scale;
@@ -413,10 +422,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
   at::Tensor ds, dn;
   pesq_stream s{nullptr, 0, 0}, n{nullptr, 0, 0};
   if (given(dstream_)) {
+    check_gradient(*dstream_, x, x.sizes(), kJoin, "dstream");
     ds = rows(dstream_->to(x.scalar_type()));
     s = stream_of(ds);
   }
   if (given(dnormed_)) {
+    check_gradient(*dnormed_, x, x.sizes(), kJoin, "dnormed");
     dn = rows(dnormed_->to(c.out));
     n = stream_of(dn);
   }
