@@ -360,7 +360,7 @@ typedef struct pesq_stream {
  * (csrc/gated_scan.cuh).  The reference has fixed-coefficient recurrences only
  * (torch_pesq/triton_ops/iir.py). */
 typedef struct pesq_gated_scan_desc {
-  int64_t batch, steps, width;
+  int64_t batch, steps, width; /* batch: up to 65535 (the torch op takes more, in parts); width: up to 2^24 */
   int32_t dtype;      /* PESQ_F32, PESQ_BF16 or PESQ_F16: x, the gates, y and their gradients */
   int32_t reverse;    /* scan from the last step to the first */
   float rate;         /* > 0 */

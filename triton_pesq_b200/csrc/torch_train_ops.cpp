@@ -171,6 +171,29 @@ struct ScanCall {
   }
 
   bool empty() const { return d.batch == 0 || d.steps == 0 || d.width == 0; }
+
+  // Rows go to the C entries in parts of about one size, which they then treat alike: as few as their
+  // limit of 65535 rows allows, and a multiple of 8 rows each, so that a part of what is kept is aligned
+  int64_t parts() const { return (d.batch + 65527) / 65528; }
+  int64_t part_rows() const { return ((d.batch + parts() - 1) / parts() + 7) / 8 * 8; }
+  // bytes of the states that a forward keeps of n rows
+  int64_t kept(int64_t n) const { return (n * ((d.steps + 7) / 8) * d.width * 4 + 15) / 16 * 16; }
+  pesq_gated_scan_desc part(int64_t first) const {
+    pesq_gated_scan_desc e = d;
+    e.batch = std::min(part_rows(), d.batch - first);
+    const auto move = [&](pesq_stream& s) {
+      s.data = static_cast<const char*>(s.data) + first * s.batch_stride * x.element_size();
+    };
+    move(e.x), move(e.input_gate), move(e.decay_gate);
+    if (e.state) e.state += first * d.width;
+    if (e.reset) e.reset += first * d.reset_batch_stride;
+    if (e.lengths) e.lengths += first;
+    return e;
+  }
+  // where the results of the rows from `first` on go, of a dense tensor
+  static char* at(const at::Tensor& t, int64_t first) {
+    return t.defined() ? static_cast<char*>(t.data_ptr()) + first * t.stride(0) * t.element_size() : nullptr;
+  }
 };
 
 // Steps between the states that this thread's last forward kept; 0 where a tracer stood in for it
@@ -196,16 +219,22 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_scan_forward(const at::Tens
     return {y, last, at::empty({0}, bytes)};
   }
   size_t work = 0, kept = 0, back = 0;
-  check_status(pesq_gated_scan_sizes(&c.d, &work, &kept, &back), "pesq_gated_scan_sizes");
-  at::Tensor states = at::empty({keep ? static_cast<int64_t>(kept) : 0}, bytes), ws;
+  pesq_gated_scan_desc d = c.part(0);
+  check_status(pesq_gated_scan_sizes(&d, &work, &kept, &back), "pesq_gated_scan_sizes");
+  at::Tensor states = at::empty({keep ? c.kept(c.d.batch) : 0}, bytes), ws;
   if (work) ws = at::empty({static_cast<int64_t>(work)}, bytes);
-  check_status(pesq_gated_scan_forward(&c.d, at::cuda::getCurrentCUDAStream(), y.data_ptr(), last.data_ptr<float>(),
-                                       keep ? states.data_ptr() : nullptr, kept, work ? ws.data_ptr() : nullptr, work),
-               "pesq_gated_scan_forward");
   if (keep) {
     int32_t here = 0, most = 0;
-    check_status(pesq_gated_scan_kept_steps(&c.d, &here, &most), "pesq_gated_scan_kept_steps");
+    check_status(pesq_gated_scan_kept_steps(&d, &here, &most), "pesq_gated_scan_kept_steps");
     scan_kept_steps = here;
+  }
+  for (int64_t first = 0; first < c.d.batch; first += c.part_rows()) {
+    if (first > 0) d = c.part(first);
+    check_status(pesq_gated_scan_forward(&d, at::cuda::getCurrentCUDAStream(), ScanCall::at(y, first),
+                                         last.data_ptr<float>() + first * c.d.width,
+                                         keep ? static_cast<char*>(states.data_ptr()) + c.kept(first) : nullptr,
+                                         keep ? c.kept(d.batch) : 0, work ? ws.data_ptr() : nullptr, work),
+                 "pesq_gated_scan_forward");
   }
   return {y, last, states};
 }
@@ -242,22 +271,32 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> gated_sca
     dys = stream_of(dy);
   }
   size_t work = 0, states = 0, back = 0;
-  check_status(pesq_gated_scan_sizes(&c.d, &work, &states, &back), "pesq_gated_scan_sizes");
+  pesq_gated_scan_desc d = c.part(0);
+  check_status(pesq_gated_scan_sizes(&d, &work, &states, &back), "pesq_gated_scan_sizes");
   check_cuda(kept, x, kScan, "kept");
-  TORCH_CHECK(kept.scalar_type() == at::kByte && kept.is_contiguous() && kept.numel() == static_cast<int64_t>(states),
+  TORCH_CHECK(kept.scalar_type() == at::kByte && kept.is_contiguous() && kept.numel() == c.kept(c.d.batch),
               "The CUDA gated scan needs the states that its forward kept.");
   at::Tensor ws = at::empty({static_cast<int64_t>(back)}, f32.dtype(at::kByte)), before = kept;
   // (hooks on what autograd saves, or a compiler, may bring the streams back in another layout than the forward's,
   // one that asks for states closer together)
   int32_t here = 0, most = 0;
-  check_status(pesq_gated_scan_kept_steps(&c.d, &here, &most), "pesq_gated_scan_kept_steps");
+  check_status(pesq_gated_scan_kept_steps(&d, &here, &most), "pesq_gated_scan_kept_steps");
   if ((kept_steps > 0 ? kept_steps : most) > here)
     before = std::get<2>(gated_scan_forward(x, ig, rg, decay, state, reset, lengths, reverse, rate, true));
-  check_status(pesq_gated_scan_backward(&c.d, at::cuda::getCurrentCUDAStream(), before.data_ptr(), states, dys,
-                                        dlast.defined() ? dlast.data_ptr<float>() : nullptr, dx.data_ptr(),
-                                        dig.data_ptr(), drg.data_ptr(), ddecay.data_ptr<float>(),
-                                        dstate.data_ptr<float>(), ws.data_ptr(), back),
-               "pesq_gated_scan_backward");
+  at::Tensor sums = c.parts() > 1 ? at::empty({c.parts(), c.d.width}, f32) : ddecay.unsqueeze(0);
+  for (int64_t first = 0, k = 0; first < c.d.batch; first += c.part_rows(), ++k) {
+    if (first > 0) d = c.part(first);
+    pesq_stream part = dys;
+    if (part.data) part.data = ScanCall::at(dy, first);
+    check_status(pesq_gated_scan_backward(&d, at::cuda::getCurrentCUDAStream(),
+                                          static_cast<const char*>(before.data_ptr()) + c.kept(first), c.kept(d.batch), part,
+                                          dlast.defined() ? dlast.data_ptr<float>() + first * c.d.width : nullptr,
+                                          ScanCall::at(dx, first), ScanCall::at(dig, first), ScanCall::at(drg, first),
+                                          sums.data_ptr<float>() + k * c.d.width,
+                                          dstate.data_ptr<float>() + first * c.d.width, ws.data_ptr(), back),
+                 "pesq_gated_scan_backward");
+  }
+  if (c.parts() > 1) ddecay = sums.sum(0);
   return {dx, dig, drg, ddecay, dstate};
 }
 

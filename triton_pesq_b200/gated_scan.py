@@ -46,7 +46,7 @@ def gated_scan(x: torch.Tensor, input_gate: torch.Tensor, decay_gate: torch.Tens
     Parameters
     ----------
     x, input_gate, decay_gate
-        ``[batch, step, channel]``, float32, bfloat16 or float16, one type.  Any
+        ``[batch, step, channel]``, float32, bfloat16 or float16, one type, up to 2**24 channels.  Any
         strides: slices of one projection are read where they lie (a tensor
         whose channels are not adjacent is copied).  The gates are logits.
     decay
