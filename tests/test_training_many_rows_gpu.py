@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from triton_pesq_b200 import gated_scan
+from triton_pesq_b200 import gated_scan, norm_join
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +38,19 @@ def test_gated_scan(cuda_device, batch, shape):
         else:  # (sums of `batch` terms in 32 bits, of about the same size and any sign)
             want = sum(p[k].double() for p in parts)
             assert float((a - want).abs().max()) <= 1e-5 * batch**0.5
+
+
+def test_norm_join_shared_gate(cuda_device):
+    batch, steps, width = 70001, 2, 8
+    g = torch.Generator(cuda_device).manual_seed(1)
+    x, z = (torch.randn(batch, steps, width, device=cuda_device, generator=g) for _ in range(2))
+    gate, v = torch.randn(batch, 1, width, device=cuda_device, generator=g), torch.ones(width, device=cuda_device)
+
+    def call(rows):
+        leaf = gate[rows].detach().requires_grad_(True)
+        out = norm_join(x[rows], z[rows], v, v, gate=leaf)
+        return (*out, *torch.autograd.grad(sum((o * x[rows]).sum() for o in out), leaf))
+
+    got, parts = call(slice(None)), [call(slice(0, 40000)), call(slice(40000, None))]
+    for k, a in enumerate(got):
+        assert torch.equal(a, torch.cat([p[k] for p in parts]))
