@@ -77,6 +77,13 @@ struct Args {
 template <int TEAM>
 constexpr bool kLeanRow = TEAM >= 512;
 
+// 1 / sqrt(mean), of means below the normal range too (rows of 1e-20, eps = 0)
+__device__ __forceinline__ float inverse_root(float mean) {
+  float y;
+  asm("rsqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(mean));
+  return y;
+}
+
 // Sums of K values over a team: by shuffles within a warp, through shared
 // memory across warps (two buffers in turn, so that one barrier a round is enough).
 template <int K, int TEAM>
@@ -346,7 +353,7 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(false,
       for (int i = 0; i < H; ++i) total = fma(z.two(2 * i), z.two(2 * i), total);
       sum[0] = total.v[0] + total.v[1];
       team_sum<1, TEAM>(sum, s_sum, turn);
-      const Vec<2> rz = splat<2>(rsqrt_approx(fmaf(sum[0], inv, p.eps)));
+      const Vec<2> rz = splat<2>(inverse_root(fmaf(sum[0], inv, p.eps)));
       Vec<2> w[H];
 #pragma unroll
       for (int i = 0; i < H; ++i) w[i] = z.two(2 * i) * (rz * post.two(2 * i));
@@ -367,7 +374,7 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(false,
     for (int i = 0; i < H; ++i) total = fma(r[i], r[i], total);
     sum[0] = total.v[0] + total.v[1];
     team_sum<1, TEAM>(sum, s_sum, turn);
-    const Vec<2> rr = splat<2>(rsqrt_approx(fmaf(sum[0], inv, p.eps)));
+    const Vec<2> rr = splat<2>(inverse_root(fmaf(sum[0], inv, p.eps)));
     if (on) {
       S out;
       B y;
@@ -477,7 +484,7 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(true, 
       for (int i = 0; i < H; ++i) total = fma(z.two(2 * i), z.two(2 * i), total);
       float one[1] = {total.v[0] + total.v[1]};
       team_sum<1, TEAM>(one, s_sum, turn);
-      rz = on ? rsqrt_approx(fmaf(one[0], inv, p.eps)) : 0.0f;
+      rz = on ? inverse_root(fmaf(one[0], inv, p.eps)) : 0.0f;
     }
     // sums of r^2, q r, ds w, q w, r w
     Vec<2> value[H], slope[H], w[H], part[5];
@@ -504,7 +511,7 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(true, 
     for (int k5 = 0; k5 < 5; ++k5) sum[k5] = part[k5].v[0] + part[k5].v[1];
     team_sum5<TEAM>(sum, s_sum, turn);
     // (a row that is off is zeros, and adds zeros for any eps)
-    const float rr = on ? rsqrt_approx(fmaf(sum[0], inv, p.eps)) : 0.0f;
+    const float rr = on ? inverse_root(fmaf(sum[0], inv, p.eps)) : 0.0f;
     const float mq = sum[1] * inv * rr * rr;                        // mean(q h) / rms
     const float mw = (sum[2] + rr * (sum[3] - mq * sum[4])) * inv;  // mean(dr w)
     Vec<2> dx[H], dz[H], dg[H];
