@@ -650,6 +650,12 @@ def iir_check(handle: int, stream: int = 0) -> int:
     return int(failed.value)
 
 
+def widened(vector):
+    """A module's vector as the training operators take it: 16-bit ones in float32, anything else as it is."""
+
+    return vector.float() if vector is not None and vector.is_floating_point() and vector.itemsize == 2 else vector
+
+
 def gated_scan_check(stream: int = 0) -> int:
     """Synchronise ``stream`` and return (and clear) the current device's gated scan error word."""
 

@@ -94,7 +94,7 @@ class GatedScanCuda(torch.nn.Module):
     Attributes
     ----------
     decay : torch.nn.Parameter
-        float32 ``[channels]``
+        float32 ``[channels]``; of a module in 16 bits it is widened for the call
     """
 
     def __init__(self, channels: int, rate: float = 8.0, reverse: bool = False, fast: float = 0.9,
@@ -116,7 +116,7 @@ class GatedScanCuda(torch.nn.Module):
                 lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """Sequences ``[batch, step, channel]``; see :func:`gated_scan`."""
 
-        return gated_scan(x, input_gate, decay_gate, self.decay, state, reset=reset, lengths=lengths,
+        return gated_scan(x, input_gate, decay_gate, _lib.widened(self.decay), state, reset=reset, lengths=lengths,
                           reverse=self.reverse, rate=self.rate)
 
     def step(self, x: torch.Tensor, input_gate: torch.Tensor, decay_gate: torch.Tensor,

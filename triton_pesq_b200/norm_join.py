@@ -107,7 +107,7 @@ class NormJoinCuda(torch.nn.Module):
     post_weight, pre_weight : torch.nn.Parameter
         float32 ``[channels]``, ones
     scale : Optional[torch.nn.Parameter]
-        float32 ``[channels]``
+        float32 ``[channels]``; the vectors of a module in 16 bits are widened for the call
     """
 
     def __init__(self, channels: int, eps: float = 1e-6, activation: str = "sigmoid", scale: Optional[float] = 1.0):
@@ -128,8 +128,8 @@ class NormJoinCuda(torch.nn.Module):
                 gate: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """See :func:`norm_join`."""
 
-        return norm_join(stream, block, self.post_weight, self.pre_weight, gate=gate, scale=self.scale, eps=self.eps,
-                         activation=self.activation)
+        return norm_join(stream, block, _lib.widened(self.post_weight), _lib.widened(self.pre_weight), gate=gate,
+                         scale=_lib.widened(self.scale), eps=self.eps, activation=self.activation)
 
     def extra_repr(self) -> str:
         return f"channels={self.channels}, eps={self.eps}, activation={self.activation}"
