@@ -363,7 +363,7 @@ typedef struct pesq_gated_scan_desc {
   int64_t batch, steps, width; /* batch: up to 65535 (the torch op takes more, in parts); width: up to 2^24 */
   int32_t dtype;      /* PESQ_F32, PESQ_BF16 or PESQ_F16: x, the gates, y and their gradients */
   int32_t reverse;    /* scan from the last step to the first */
-  float rate;         /* > 0 */
+  float rate;         /* above 0, up to 1e6 */
   int32_t kept_steps; /* of a backward: its forward's pesq_gated_scan_kept_steps; 0: of streams laid out as here */
   pesq_stream x, input_gate, decay_gate;
   const float* decay; /* [width] */

@@ -164,3 +164,11 @@ def test_gated_scan_says_how_far_apart_it_keeps_its_states():
     assert lib.pesq_gated_scan_backward(ctypes.byref(d), None, one, 1 << 30, none, None, one, one, one, one, None, one,
                                         1 << 30) == 1
     assert "too far apart" in _lib.last_error()
+
+
+def test_rates_that_no_call_takes_are_refused_by_the_module():
+    for rate in (1.1e6, float("inf"), float("nan"), -1.0):
+        with pytest.raises(ValueError, match="1e6"):
+            GatedScanCuda(4, rate=rate)
+    assert _sizes(_scan(rate=1e6))[0] == _lib.PESQ_OK
+    assert _sizes(_scan(rate=1.1e6))[0] == _lib.PESQ_ERR_INVALID_ARGUMENT and "1e6" in _lib.last_error()

@@ -55,7 +55,7 @@ int check(const pesq_gated_scan_desc* d) {
   if (d->batch < 1 || d->steps < 1 || d->width < 1)
     return set_error(PESQ_ERR_INVALID_ARGUMENT, "batch, steps and width must be at least 1");
   if (d->dtype < PESQ_F32 || d->dtype > PESQ_F16) return set_error(PESQ_ERR_INVALID_ARGUMENT, "unknown element type");
-  if (!(d->rate > 0.0f) || d->rate > 1e6f) return set_error(PESQ_ERR_INVALID_ARGUMENT, "rate must be positive");
+  if (!(d->rate > 0.0f) || d->rate > 1e6f) return set_error(PESQ_ERR_INVALID_ARGUMENT, "rate must lie above 0 and not above 1e6");
   if (d->batch > 65535 || d->width > (1 << 24) || d->steps > INT32_MAX - 64)
     return set_error(PESQ_ERR_UNSUPPORTED, "more than 65535 rows, 2^24 channels or 2^31 steps in one call");
   return PESQ_OK;

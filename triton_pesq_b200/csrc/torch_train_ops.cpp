@@ -129,7 +129,7 @@ struct ScanCall {
     TORCH_CHECK(ig_.scalar_type() == x_.scalar_type() && rg_.scalar_type() == x_.scalar_type(),
                 "The CUDA gated scan needs `x` and the gates in one type, got ", x_.scalar_type(), ", ",
                 ig_.scalar_type(), " and ", rg_.scalar_type(), ".");
-    TORCH_CHECK_VALUE(rate > 0.0 && rate <= 1e6, "The CUDA gated scan needs a positive `rate`, got ", rate, ".");
+    TORCH_CHECK_VALUE(rate > 0.0 && rate <= 1e6, "The CUDA gated scan needs a `rate` above 0 and up to 1e6, got ", rate, ".");
     x = rows(x_);
     ig = rows(ig_);
     rg = rows(rg_);

@@ -17,7 +17,6 @@ recurrences only (torch_pesq/triton_ops/iir.py).
 
 from __future__ import annotations
 
-import math
 from typing import Optional, Tuple
 
 import torch
@@ -62,7 +61,7 @@ def gated_scan(x: torch.Tensor, input_gate: torch.Tensor, decay_gate: torch.Tens
     reverse
         Scan from the last step to the first.
     rate
-        Positive factor of the log decay.
+        Factor of the log decay, above 0 and up to 1e6.
 
     Returns
     -------
@@ -85,7 +84,7 @@ class GatedScanCuda(torch.nn.Module):
     channels : int
         Width of the recurrence
     rate : float
-        Positive factor of the log decay
+        Factor of the log decay, above 0 and up to 1e6
     reverse : bool
         Scan from the last step to the first
     fast, slow : float
@@ -102,8 +101,8 @@ class GatedScanCuda(torch.nn.Module):
         super().__init__()
         if int(channels) < 1:
             raise ValueError("`channels` has to be positive.")
-        if not (rate > 0 and math.isfinite(rate)):
-            raise ValueError("`rate` has to be positive.")
+        if not 0 < rate <= 1e6:
+            raise ValueError("`rate` has to lie above 0 and not above 1e6.")
         if not 0 < fast <= slow < 1:
             raise ValueError("The initial decays have to satisfy 0 < fast <= slow < 1.")
         self.channels, self.rate, self.reverse = int(channels), float(rate), bool(reverse)
