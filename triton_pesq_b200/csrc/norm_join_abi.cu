@@ -144,14 +144,14 @@ size_t part_bytes(const pesq_norm_join_desc& d) {
   return round16((size_t)rows * d.width * 4);
 }
 
-Rows rows_of(const pesq_stream& s, const Plan& q) {
+Rows rows_of(const pesq_stream& s) {
   return {s.data, s.batch_stride, s.step_stride};
 }
 
 void fill(Args& a, const pesq_norm_join_desc& d, const Plan& q) {
-  a.stream = rows_of(d.stream, q);
-  a.block = rows_of(d.block, q);
-  a.gate = rows_of(d.gate, q);
+  a.stream = rows_of(d.stream);
+  a.block = rows_of(d.block);
+  a.gate = rows_of(d.gate);
   if (d.gate_shared) a.gate.st = 0;
   a.post = d.post;
   a.pre = d.pre;
@@ -212,8 +212,8 @@ int pesq_norm_join_backward(const pesq_norm_join_desc* d, void* stream, pesq_str
   q.g.wide = q.g.wide && wide(dx) && wide(dblock) && wide(dgate);
   Args a{};
   fill(a, *d, q);
-  a.dstream = rows_of(dstream, q);
-  a.dnormed = rows_of(dnormed, q);
+  a.dstream = rows_of(dstream);
+  a.dnormed = rows_of(dnormed);
   a.dx = dx;
   a.dblock = d->block.data ? dblock : nullptr;
   a.dgate = d->gate.data && !d->gate_shared ? dgate : nullptr;

@@ -116,7 +116,6 @@ __device__ __forceinline__ Vec<N> widen(const Pack<T, M>& p, int j) {
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 }  // namespace train
 
