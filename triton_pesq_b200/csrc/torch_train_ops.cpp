@@ -283,7 +283,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> gated_sca
   check_status(pesq_gated_scan_kept_steps(&d, &here, &most), "pesq_gated_scan_kept_steps");
   if ((kept_steps > 0 ? kept_steps : most) > here)
     before = std::get<2>(gated_scan_forward(x, ig, rg, decay, state, reset, lengths, reverse, rate, true));
-  at::Tensor sums = c.parts() > 1 ? at::empty({c.parts(), c.d.width}, f32) : ddecay.unsqueeze(0);
+  at::Tensor sums;  // of the parts
+  if (c.parts() > 1) sums = at::empty({c.parts(), c.d.width}, f32);
   for (int64_t first = 0, k = 0; first < c.d.batch; first += c.part_rows(), ++k) {
     if (first > 0) d = c.part(first);
     pesq_stream part = dys;
@@ -292,7 +293,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> gated_sca
                                           static_cast<const char*>(before.data_ptr()) + c.kept(first), c.kept(d.batch), part,
                                           dlast.defined() ? dlast.data_ptr<float>() + first * c.d.width : nullptr,
                                           ScanCall::at(dx, first), ScanCall::at(dig, first), ScanCall::at(drg, first),
-                                          sums.data_ptr<float>() + k * c.d.width,
+                                          c.parts() > 1 ? sums.data_ptr<float>() + k * c.d.width : ddecay.data_ptr<float>(),
                                           dstate.data_ptr<float>() + first * c.d.width, ws.data_ptr(), back),
                  "pesq_gated_scan_backward");
   }
