@@ -24,55 +24,52 @@ namespace {
 constexpr int kMaxWidth = 8192;  // one CTA of 1024 threads holds a row
 
 // Columns of the CTAs' sums, in a fixed order: 32 columns a block, every thread a
-// stride of the rows, then a tree.  Kinds of sums, which blockIdx.y begins with and takes a grid's height
-// further: 0 the pre vector, 1 the post and scale vectors, 2 + b the shared gate of batch item b.
+// stride of the rows, then a tree.  first + blockIdx.y: 0 the pre vector, 1 the post and scale
+// vectors, 2 + b the shared gate of batch item b.
 struct SumArgs {
   const float *pre, *u, *gate, *post, *scale;
   float *dpre, *dpost, *dscale;
   void* dgate;
-  int64_t rows, per_item, kinds;
+  int64_t rows, per_item, first;
   int width, dtype;
 };
-constexpr int kSumRows = 32, kMostKinds = 65535;  // (of a launch at once)
+constexpr int kSumRows = 32, kMostSums = 65535;  // (of a launch)
 __global__ void __launch_bounds__(32 * kSumRows) vectors_kernel(const __grid_constant__ SumArgs p) {
   __shared__ float s[kSumRows][33];
   const int c = blockIdx.x * 32 + threadIdx.x;
+  const int64_t which = p.first + blockIdx.y;
+  const float* part = which == 0 ? p.pre : which == 1 ? p.u : p.gate + (which - 2) * p.per_item * p.width;
+  const int64_t rows = which < 2 ? p.rows : p.per_item;
+  if (!part) return;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // for the kernel before, which this one is launched close to
-  for (int64_t which = blockIdx.y; which < p.kinds; which += gridDim.y) {
-    const float* part = which == 0 ? p.pre : which == 1 ? p.u : p.gate + (which - 2) * p.per_item * p.width;
-    const int64_t rows = which < 2 ? p.rows : p.per_item;
-    if (!part) continue;
-    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (c < p.width) {
-      int64_t r = threadIdx.y;
-      for (; r + 3 * kSumRows < rows; r += 4 * kSumRows) {
+  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (c < p.width) {
+    int64_t r = threadIdx.y;
+    for (; r + 3 * kSumRows < rows; r += 4 * kSumRows) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) acc[k] += part[(r + k * kSumRows) * p.width + c];
-      }
-      for (; r < rows; r += kSumRows) acc[0] += part[r * p.width + c];
+      for (int k = 0; k < 4; ++k) acc[k] += part[(r + k * kSumRows) * p.width + c];
     }
-    s[threadIdx.y][threadIdx.x] = (acc[0] + acc[1]) + (acc[2] + acc[3]);
-    __syncthreads();
-    if (threadIdx.y == 0 && c < p.width) {
-      float v = 0.0f;
+    for (; r < rows; r += kSumRows) acc[0] += part[r * p.width + c];
+  }
+  s[threadIdx.y][threadIdx.x] = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+  __syncthreads();
+  if (threadIdx.y != 0 || c >= p.width) return;
+  float v = 0.0f;
 #pragma unroll
-      for (int k = 0; k < kSumRows; ++k) v += s[k][threadIdx.x];
-      if (which == 0) {
-        p.dpre[c] = v;
-      } else if (which == 1) {
-        p.dpost[c] = p.scale ? v * p.scale[c] : v;
-        if (p.dscale) p.dscale[c] = v * p.post[c];
-      } else {
-        const int64_t at = (which - 2) * p.width + c;
-        if (p.dtype == PESQ_F32)
-          static_cast<float*>(p.dgate)[at] = v;
-        else if (p.dtype == PESQ_BF16)
-          static_cast<__nv_bfloat16*>(p.dgate)[at] = __float2bfloat16_rn(v);
-        else
-          static_cast<__half*>(p.dgate)[at] = __float2half_rn(v);
-      }
-    }
-    __syncthreads();
+  for (int k = 0; k < kSumRows; ++k) v += s[k][threadIdx.x];
+  if (which == 0) {
+    p.dpre[c] = v;
+  } else if (which == 1) {
+    p.dpost[c] = p.scale ? v * p.scale[c] : v;
+    if (p.dscale) p.dscale[c] = v * p.post[c];
+  } else {
+    const int64_t at = (which - 2) * p.width + c;
+    if (p.dtype == PESQ_F32)
+      static_cast<float*>(p.dgate)[at] = v;
+    else if (p.dtype == PESQ_BF16)
+      static_cast<__nv_bfloat16*>(p.dgate)[at] = __float2bfloat16_rn(v);
+    else
+      static_cast<__half*>(p.dgate)[at] = __float2half_rn(v);
   }
 }
 
@@ -238,18 +235,19 @@ int pesq_norm_join_backward(const pesq_norm_join_desc* d, void* stream, pesq_str
     t.per_item = q.units;
     t.width = (int)d->width;
     t.dtype = d->dtype;
-    t.kinds = 2 + (a.part_gate ? q.batch : 0);
-    const dim3 grid((unsigned)((d->width + 31) / 32), (unsigned)std::min<int64_t>(t.kinds, kMostKinds));
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t c{};
-    c.gridDim = grid;
     c.blockDim = dim3(32, kSumRows);
     c.stream = s;
     c.attrs = &at;
     c.numAttrs = 1;
-    e = cudaLaunchKernelEx(&c, vectors_kernel, t);
+    const int64_t sums = 2 + (a.part_gate ? q.batch : 0);
+    for (; e == cudaSuccess && t.first < sums; t.first += kMostSums) {
+      c.gridDim = dim3((unsigned)((d->width + 31) / 32), (unsigned)std::min<int64_t>(sums - t.first, kMostSums));
+      e = cudaLaunchKernelEx(&c, vectors_kernel, t);
+    }
   }
   return e == cudaSuccess ? PESQ_OK : set_error(PESQ_ERR_CUDA, cudaGetErrorString(e));
 }
