@@ -12,7 +12,7 @@
 // 256 values, so that the blocks of 256 of the buffer are the units of work, and one warp
 // takes a unit: eight values a lane.  A warp finds its tensor by bisection.
 // Measured (B200, share of the bytes at the measured copy rate): 35M values, 32-bit moments and
-// gradients 158 us, 95 %; 106M values, 8-bit moments, 16-bit gradients and copies 329 us, 79 %, where
+// gradients 157 us, 96 %; 106M values, 8-bit moments, 16-bit gradients and copies 329 us, 79 %, where
 // the arithmetic of the 8 bits (70 % of the issue slots) is as long as the bytes; 275,000 values in 52 tensors 7 us.
 //
 // 8 bits.  A block of 256 has a 32-bit scale, its largest magnitude / 448, and its

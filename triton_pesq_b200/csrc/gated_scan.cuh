@@ -27,20 +27,26 @@
 // strip's (A, H), and the second, launched while the first still runs and waiting for its end, starts
 // each strip from the state that the maps before it give.  The strips of a CTA meet in shared memory,
 // so a strip composes the maps of the CTAs before its own and one more.  Rows of 33 to 512 steps that
-// would be cut go through one CTA of one launch instead, which holds its steps as (a, b) in registers.
+// would be cut go through one CTA for every 32 channels in one launch instead, which holds its steps as (a, b) in
+// registers: of up to 512 threads, one an SM.
 //
 // What bounds it.  The bytes, 4 elements a step forward and 7 backward, are the floor; an element
 // also takes 40 instruction slots forward and 65 backward, 5 of them special functions of eight
 // cycles a warp.  With n warps a scheduler of 32 chunks each the time is 28 + 11 n us
 // forward and 36 + 18 n backward: a warp's work on every pipe in turn, of which n warps overlap the rest.
-// Measured (B200, cold caches, share of the bytes at the measured copy rate):
-//   64 x 500 x 896 bfloat16, uncut            forward 72 us, 49 %; backward 109 us, 57 %
-//   96 x 512 x 512 float32, uncut, pairs      forward 77 us, 80 %; backward 138 us, 78 %
-//   16 x 1000 x 512 float32, cut, boxes       forward 48 us, 42 %; backward 60 us, 58 %
-//   6 x 4001 x 385 float32, cut, plain loads  forward 62 us, 36 %; backward 87 us, 45 %
-//   1 x 32768 x 1040 bfloat16, cut, boxes     forward 124 us, 34 %; backward 146 us, 50 %
-//   8 x 500 x 768 bfloat16, one CTA a row     forward 21 us, 18 % (launch and one walk through the row)
-// (cut rows read the gates twice, which the floor does not count).
+// Measured (B200, cold caches, the call's kernels alone with the 6 us of a launch, channels that stay
+// below kNear; bytes at the measured copy rate):
+//                                             forward (bytes alone)    backward
+//   64 x 500 x 896 bfloat16, uncut            73.8 us (35.1)           110.6 us (61.4)
+//   96 x 512 x 512 float32, uncut, pairs      77.8 (61.6)              139.3 (107.8)
+//   16 x 1000 x 512 float32, cut, boxes       49.2 (20.0)              61.5 (35.1)
+//   6 x 4001 x 385 float32, cut, plain loads  63.5 (22.6)              85 (39.6)
+//   1 x 32768 x 1040 bfloat16, cut, boxes     129.1 (41.7)             142 (73.0)
+//   1 x 65537 x 129 float32, cut, plain loads 61.5 (20.7)              79.9 (36.2)   the fifth warp across: one lane
+//   1 x 65537 x 128 float32, cut, boxes       51.2 (20.5)              63.5 (35.9)
+//   8 x 500 x 768 bfloat16, one CTA each      22.5 (3.8)               26.7 (6.6)    192 CTAs forward: two rounds
+// Cut rows read x and both gates twice forward, the decay gate and dy twice backward, which the bytes alone
+// do not count.  Channels above kNear take the exponential: 64 x 500 x 896 81.9 and 116.7 us.
 //
 // Backward.  With g_t = dL/dh_t: g_t = dy_t + a_{t+1} g_{t+1}, the same kind of
 // scan from the end of the row, carried as e_t = a_t g_t.  Then

@@ -25,13 +25,18 @@
 //
 // A row's sums are two rounds of shuffles, and barriers where a team has several warps, that its
 // loads and stores overlap only by the other teams of the SM and by the next row's loads.
-// Measured (B200, cold caches, share of the bytes at the measured copy rate):
-//   64 x 500 x 896, stream and block bfloat16   forward 56 us, 78 %; backward 105 us, 67 %
-//   64 x 500 x 385, float32                     forward 48 us, 78 %; backward 81 us, 74 %
-//   100000 x 64, bfloat16                       forward 18.5 us, backward 32.8 us
-//   4000 x 8192, bfloat16                       forward 86 us, 58 %; backward 277 us, 29 % (sums in shared
-//                                               memory, no next row)
-//   8 x 500 x 768, stream float32               forward 10.4 us a call (floor 5.6), launch included
+// Measured (B200, cold caches, the call's kernels alone; bytes at the measured copy rate):
+//                                    forward (bytes alone)     backward
+//   64 x 500 x 896 bfloat16          55.3 us (43.9)            106.5 us (70.2)
+//   64 x 500 x 385 float32           49.2 (37.7)               82.0 (60.3)
+//   100000 x 64 bfloat16             20.5 (9.8)                34.7 (15.7)
+//   6 x 1500 x 385, shared gate      18.5 (8.5)                32.8 (12.7)
+//   16000 x 1024 bfloat16            34.8 (25.1)               63.5 (40.1)
+//   16000 x 1040 bfloat16            53.3 (25.4)               129.1 (40.7)  teams of 256, 130 of them with channels
+//   8000 x 2048 bfloat16             36.9 (25.1)               77.9 (40.1)   8 warps an SM
+//   4000 x 8192 bfloat16             88.0 (50.1)               268.7 (80.2)  sums in shared memory, no next row
+//   8 x 500 x 768, float32 stream    14.3 (6.6)                26.7 (10.3)   of which a launch is 6
+//   the norm alone, 64 x 500 x 896   34.8 (17.5)               75.8 (26.3)
 #pragma once
 
 #include <type_traits>
@@ -46,9 +51,11 @@ using namespace train;
 
 constexpr int kEach = 8;      // channels of a thread
 constexpr int kThreads = 128; // of a CTA, unless a row takes more
-// CTAs that an SM holds, which the registers of a thread follow from: 72 in the forward (96
+// CTAs that an SM holds, which the registers of a thread follow from.  Teams up to 128: 72 in the forward (96
 // where every channel is addressed by itself), 168 in the backward, where 16 warps of 128
-// registers spill and take 25 % longer than 12 that do not
+// registers spill and take 25 % longer than 12 that do not.  Wider teams are a CTA each, as many as those registers
+// allow and one at least: in the backward one of 256 threads (194 to 236 registers), of 512 (128) or of 1024 (64, which
+// spills).  Nothing was tried to fill the SM better there.
 constexpr int ctas(bool backward, bool wide, int team) {
   const int threads = team > kThreads ? team : kThreads, sm = backward ? 384 : wide ? 896 : 640;
   return sm / threads > 0 ? sm / threads : 1;
