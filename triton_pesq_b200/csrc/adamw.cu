@@ -122,9 +122,10 @@ __device__ __forceinline__ float dither_small(float u, unsigned bits) {
 // where it has moved by half a step or more.  The twelve upper bits of a hash; the root takes the others.
 __device__ __forceinline__ float dither_held(float m, float was, unsigned bits) {
   const float u = fabsf(m), power = __uint_as_float(__float_as_uint(u) & 0x7f800000u);
-  if (!(fabsf(m - was) < 0x1p-4f * fmaxf(power, 0x1p-6f))) return m;
   const unsigned mine = bits >> 20 << 8 | 0x80u;
-  return copysignf(u < 0x1p-6f ? dither_small(u, mine) : dither(u, mine), m);
+  float to = dither(u, mine);
+  if (u < 0x1p-6f) to = dither_small(u, mine);
+  return fabsf(m - was) < 0x1p-4f * fmaxf(power, 0x1p-6f) ? copysignf(to, m) : m;
 }
 
 // Eight values of a tensor, as the words they were read as
@@ -330,28 +331,32 @@ __global__ void __launch_bounds__(kThreads, kCtas<kEight>) adamw_kernel(const __
           m[j] *= i1, r[j] *= i2;
           low1 = fminf(low1, fabsf(m[j])), low2 = min_nan(low2, r[j]);
         }
-        if (low2 >= 0x1p-6f) {
+        bool held = low1 < p.held1;
+        if (held && low1 == 0.0f) {  // (zeros stay)
+          held = false;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) held = held || (m[j] != 0.0f && fabsf(m[j]) < p.held1);
+        }
+        if (!held && low2 >= 0x1p-6f) {  // (rarely not with b1 <= 15/16; above, always: 106M values 385 us)
 #pragma unroll
           for (int j = 0; j < 8; ++j) r[j] = dither(r[j], hash((unsigned)(place + j) + salt));
-        } else {  // (what is above zero does not become zero, and a NaN stays)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const unsigned h = hash((unsigned)(place + j) + salt);
-            if (r[j] >= 0x1p-6f)
-              r[j] = dither(r[j], h);
-            else if (r[j] > 0.0f)
-              r[j] = fmaxf(dither_small(r[j], h), 0x1p-9f);
-          }
-        }
-        if (low1 < p.held1) {  // (rare where a gradient is there: 1 value in 10,000)
+        } else {
           // (the codes are still in memory, which costs fewer registers than to keep them)
           const uint2 c = *reinterpret_cast<const uint2*>(static_cast<const unsigned char*>(p.moment1) + place);
           const float then = now.s1 * i1;
           float was[8];
           from_e4m3(c.x, was), from_e4m3(c.y, was + 4);
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (fabsf(m[j]) < p.held1) m[j] = dither_held(m[j], was[j] * then, hash((unsigned)(place + j) + salt));
+          for (int j = 0; j < 8; ++j) {
+            const unsigned h = hash((unsigned)(place + j) + salt);
+            const float to = dither_held(m[j], was[j] * then, h);
+            m[j] = fabsf(m[j]) < p.held1 ? to : m[j];
+            // (what is above zero does not become zero, and a NaN stays)
+            if (r[j] >= 0x1p-6f)
+              r[j] = dither(r[j], h);
+            else if (r[j] > 0.0f)
+              r[j] = fmaxf(dither_small(r[j], h), 0x1p-9f);
+          }
         }
         uint2 c1, c2;
         c1.x = to_e4m3(m), c1.y = to_e4m3(m + 4), c2.x = to_e4m3(r), c2.y = to_e4m3(r + 4);
