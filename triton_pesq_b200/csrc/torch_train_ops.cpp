@@ -4,8 +4,8 @@
 // Every operator is three ops: the one a caller uses (composite: it records an
 // autograd node when a gradient is wanted), and the forward and backward it is
 // made of, which allocate with torch's caching allocator, take the current
-// stream and call the C ABI.  Shapes, types and devices are checked in the
-// forward; the backward gets what the forward has checked.
+// stream and call the C ABI.  Both check the shapes, types and devices of what
+// they are given.
 #include <algorithm>
 #include <limits>
 
