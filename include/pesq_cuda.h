@@ -457,6 +457,37 @@ typedef struct pesq_adamw_desc {
  * over all tensors in one launch (csrc/adamw.cu; one more for every further 800 tensors). */
 int pesq_adamw_step(const pesq_adamw_desc* desc, const pesq_adamw_tensor* tensors, int64_t count, void* stream);
 
+/* A [batch, step, head, channel] stream: element strides of batch, step and
+ * head (any, negative or zero too); channels are adjacent. */
+typedef struct pesq_heads {
+  const void* data;
+  int64_t batch_stride;
+  int64_t step_stride;
+  int64_t head_stride;
+} pesq_heads;
+
+/* Layer norm over the channels,
+ *   y = (x - mean(x)) / sqrt(mean((x - mean(x))^2) + eps) weight + bias
+ * with a weight (and bias) for each head and channel; one head for one of each
+ * channel (csrc/layer_norm.cuh). */
+typedef struct pesq_layer_norm_desc {
+  int64_t batch, steps, heads, width; /* width: 1 .. 8192; heads * width: up to 2^20 */
+  int32_t dtype;     /* of x and its gradient: PESQ_F32, or `out_dtype` */
+  int32_t out_dtype; /* of y and its gradient */
+  float eps;
+  int32_t reserved0;
+  pesq_heads x;
+  const float *weight, *bias; /* [heads, width]; bias NULL: zeros */
+} pesq_layer_norm_desc;
+
+/* y: [batch, steps, heads, width] dense. */
+int pesq_layer_norm_forward(const pesq_layer_norm_desc* desc, void* stream, void* y);
+/* Bytes of a backward's workspace. */
+int pesq_layer_norm_workspace(const pesq_layer_norm_desc* desc, size_t* bytes);
+/* dx: dense; dweight, dbias: [heads, width]; dbias may be NULL without a bias. */
+int pesq_layer_norm_backward(const pesq_layer_norm_desc* desc, void* stream, pesq_heads dy, void* dx, float* dweight,
+                             float* dbias, void* workspace, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

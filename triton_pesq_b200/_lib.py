@@ -174,6 +174,31 @@ class NormJoinDesc(ctypes.Structure):
     ]
 
 
+class Heads(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("batch_stride", ctypes.c_int64),
+        ("step_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+    ]
+
+
+class LayerNormDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int64),
+        ("steps", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("width", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("reserved0", ctypes.c_int32),
+        ("x", Heads),
+        ("weight", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+    ]
+
+
 class AdamwTensor(ctypes.Structure):
     _fields_ = [
         ("param", ctypes.c_void_p),
@@ -320,6 +345,13 @@ SIGNATURES = {
         [ctypes.POINTER(NormJoinDesc), ctypes.c_void_p, Stream, Stream, ctypes.c_void_p, ctypes.c_void_p,
          ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t],
     ),
+    "pesq_layer_norm_forward": (ctypes.c_int, [ctypes.POINTER(LayerNormDesc), ctypes.c_void_p, ctypes.c_void_p]),
+    "pesq_layer_norm_workspace": (ctypes.c_int, [ctypes.POINTER(LayerNormDesc), ctypes.POINTER(ctypes.c_size_t)]),
+    "pesq_layer_norm_backward": (
+        ctypes.c_int,
+        [ctypes.POINTER(LayerNormDesc), ctypes.c_void_p, Heads, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+         ctypes.c_void_p, ctypes.c_size_t],
+    ),
     "pesq_adamw_step": (
         ctypes.c_int,
         [ctypes.POINTER(AdamwDesc), ctypes.POINTER(AdamwTensor), ctypes.c_int64, ctypes.c_void_p],
@@ -445,6 +477,14 @@ def _register_fakes() -> None:
 
         return like(stream), like(block), like(gate), like(post), like(pre), like(scale)
 
+
+    @torch.library.register_fake("pesq_cuda::layer_norm_forward")
+    def _layer_norm(x, weight, bias, eps, dtype):
+        return x.new_empty(x.shape, dtype=dtypes[dtype])
+
+    @torch.library.register_fake("pesq_cuda::layer_norm_backward")
+    def _layer_norm_backward(x, weight, bias, eps, dtype, dy):
+        return x.new_empty(x.shape), weight.new_empty(weight.shape), weight.new_empty((0,) if bias is None else bias.shape)
 
     @torch.library.register_fake("pesq_cuda::adamw_step")
     def _adamw_step(params, grads, moment1, moment2, step, scales, copies, lr, beta1, beta2, eps, weight_decay,

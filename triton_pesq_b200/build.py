@@ -30,7 +30,8 @@ CUDA_SOURCES = ["front.cu", "align.cu", "back.cu", "spectrum.cu", "chain.cu", "r
                 "resample_abi.cu", "iir_abi.cu", "iir_ka.cu", "iir_kb.cu", "iir_kc.cu", "iir_kd.cu", "iir_ke.cu",
                 "iir_kf.cu", "gated_scan_f32.cu", "gated_scan_bf16.cu", "gated_scan_f16.cu", "gated_scan_abi.cu",
                 "norm_join_f32.cu", "norm_join_bf16.cu", "norm_join_f16.cu", "norm_join_f32_bf16.cu", "norm_join_f32_f16.cu",
-                "norm_join_abi.cu", "adamw.cu"]
+                "norm_join_abi.cu", "adamw.cu", "layer_norm_f32.cu", "layer_norm_bf16.cu", "layer_norm_f16.cu",
+                "layer_norm_f32_bf16.cu", "layer_norm_f32_f16.cu", "layer_norm_abi.cu"]
 NVCC_FLAGS = [
     "-std=c++17",
     "-O3",
@@ -115,7 +116,8 @@ def build_torch_ops(force: bool = False, verbose: bool = False) -> str:
     ctypes.CDLL(LIB, mode=ctypes.RTLD_GLOBAL)
     cpp_extension.load(
         name="pesq_torch_ops",
-        sources=[os.path.join(CSRC, "torch_ops.cpp"), os.path.join(CSRC, "torch_train_ops.cpp")],
+        sources=[os.path.join(CSRC, "torch_ops.cpp"), os.path.join(CSRC, "torch_train_ops.cpp"),
+                 os.path.join(CSRC, "torch_layer_ops.cpp")],
         extra_cflags=["-O2", "-std=c++17"],
         extra_ldflags=[f"-L{HERE}", "-lpesq_cuda", "-Wl,-rpath,\\$$ORIGIN"],
         build_directory=bdir,

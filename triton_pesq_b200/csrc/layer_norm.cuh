@@ -1,0 +1,241 @@
+// Layer norm over the last dimension of [batch, step, head, channel], with a weight (and bias) for each
+// channel, or for each head and channel:
+//
+//   y = h weight + bias,   h = (x - mean(x)) / sqrt(mean((x - mean(x))^2) + eps)
+//
+// A team of threads keeps a row in registers, eight channels a thread, as the join of norm_join.cuh does: x
+// is read once, the mean subtracted before the squares are summed (two rounds of sums), and the next row is on its
+// way while one is worked on.  The backward recomputes the statistics instead of reading them, and takes with
+// q = dy weight the second round's three sums together:
+//
+//   dx = (q - mean(q) - h mean(q h)) / sqrt(..),   dweight = sum over rows of dy h,   dbias = of dy
+//
+// The vectors' sums stay in registers over the rows of a team, which all belong to one head; a CTA's teams of the
+// same head are added up in shared memory, and the CTAs' sums in a fixed order by a second kernel, so that a
+// result is the same every time.  The bound is memory.
+#pragma once
+
+#include "norm_join.cuh"
+
+namespace pesq {
+namespace lnorm {
+
+using namespace train;
+using njoin::Eight;
+using njoin::inverse_root;
+using njoin::kEach;
+using njoin::team_sum;
+
+constexpr int kThreads = 128;  // of a CTA, unless a row takes more
+
+// An operand's rows: strides of batch, step and head in elements
+struct Rows {
+  const void* p;
+  int64_t sb, st, sh;
+};
+
+struct Args {
+  Rows x, dy;
+  const float *weight, *bias;  // [heads, width]; bias may be null
+  int64_t batch, steps;
+  int heads, width;
+  int block_heads;   // heads of a CTA
+  int head_blocks;   // CTAs side by side over the heads
+  int64_t units;     // CTAs over the rows, of each of which `span` rows
+  int64_t span;
+  float eps;
+  void* y;           // forward, dense
+  void* dx;          // backward, dense
+  float *part_weight, *part_bias;  // [units, heads, width]; part_bias null without a bias
+};
+
+// CTAs that an SM holds, which the registers of a thread follow from
+constexpr int ctas(bool backward, int team) {
+  const int threads = team > kThreads ? team : kThreads, sm = backward ? 512 : 1024;
+  return sm / threads > 0 ? sm / threads : 1;
+}
+
+// The rows that a team works on in turn: those of one head, every kSlots-th of its CTA's
+template <int TEAM, int THREADS>
+struct Turns {
+  static constexpr int kTeams = THREADS / TEAM;
+  int head, slots;     // rows that the CTA's teams of one head take at once
+  int64_t row, end;    // of [batch * steps]
+  __device__ __forceinline__ Turns(const Args& p) {
+    const int team = threadIdx.x / TEAM, block = blockIdx.x % p.head_blocks;
+    const int64_t unit = blockIdx.x / p.head_blocks;
+    slots = kTeams / p.block_heads;
+    head = block * p.block_heads + team % p.block_heads;
+    const bool on = team < slots * p.block_heads && head < p.heads;
+    row = unit * p.span + team / p.block_heads;
+    end = on ? min(p.batch * p.steps, (unit + 1) * p.span) : 0;
+    if (!on) head = 0;
+  }
+};
+template <class T>
+__device__ __forceinline__ const char* place(const Rows& r, const Args& p, int64_t row, int head) {
+  // (one batch item where the items' rows lie as one run, so that most calls divide by nothing here)
+  const int64_t b = p.batch == 1 ? 0 : row / p.steps, t = row - b * p.steps;
+  return static_cast<const char*>(r.p) + (b * r.sb + t * r.st + head * r.sh) * (int64_t)sizeof(T);
+}
+
+template <class TX, class TY, int TEAM, bool kWide>
+__global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(false, TEAM))
+    forward_kernel(const __grid_constant__ Args p) {
+  constexpr int THREADS = TEAM > kThreads ? TEAM : kThreads, H = kEach / 2;
+  using X = Eight<TX, TEAM, kWide>;
+  using Y = Eight<TY, TEAM, kWide>;
+  using F = Eight<float, TEAM, kWide>;
+  __shared__ __align__(16) float s_sum[2][32][8];
+  int turn = 0;
+  Turns<TEAM, THREADS> of(p);
+  F weight, bias;
+  weight.load(p.weight + (int64_t)of.head * p.width, p.width, true);
+  bias.load(p.bias + (int64_t)of.head * p.width, p.width, p.bias != nullptr);
+  const float inv = 1.0f / (float)p.width;
+  const int64_t turns = (p.span + of.slots - 1) / of.slots;
+  X x;
+  bool on = of.row < of.end;
+  x.load(place<TX>(p.x, p, on ? of.row : 0, of.head), p.width, on);
+#pragma unroll 1
+  for (int64_t k = 0; k < turns; ++k) {
+    const int64_t next = of.row + of.slots;
+    const bool on1 = next < of.end;
+    X x1;
+    x1.load(place<TX>(p.x, p, on1 ? next : 0, of.head), p.width, on1);
+    Vec<2> d[H], total = splat<2>(0.0f);
+#pragma unroll
+    for (int i = 0; i < H; ++i) total = total + x.two(2 * i);
+    float sum[1] = {total.v[0] + total.v[1]};
+    team_sum<1, TEAM>(sum, s_sum, turn);
+    const float mean = sum[0] * inv;
+    total = splat<2>(0.0f);
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) d[i].v[j] = X::column(2 * i + j) < p.width ? x.at(2 * i + j) - mean : 0.0f;
+      total = fma(d[i], d[i], total);
+    }
+    sum[0] = total.v[0] + total.v[1];
+    team_sum<1, TEAM>(sum, s_sum, turn);
+    const Vec<2> r = splat<2>(inverse_root(fmaf(sum[0], inv, p.eps)));
+    if (on) {
+      Y y;
+#pragma unroll
+      for (int i = 0; i < H; ++i) y.set(2 * i, fma(d[i] * r, weight.two(2 * i), bias.two(2 * i)));
+      y.store(p.y, (of.row * p.heads + of.head) * p.width, p.width);
+    }
+    x = x1, on = on1, of.row = next;
+  }
+}
+
+// What the CTA's teams of each head hold, added up, to the CTA's row of `part`
+template <int TEAM, int TEAMS, bool kWide>
+__device__ __forceinline__ void store_part(const Vec<2> (&v)[kEach / 2], float* part, const Args& p, float* s_part) {
+  using F = Eight<float, TEAM, kWide>;
+  F f;
+#pragma unroll
+  for (int i = 0; i < kEach / 2; ++i) f.set(2 * i, v[i]);
+  const int64_t unit = blockIdx.x / p.head_blocks;
+  const int first = blockIdx.x % p.head_blocks * p.block_heads, heads = min(p.block_heads, p.heads - first);
+  float* to = part + (unit * p.heads + first) * p.width;
+  if (TEAMS == 1) {
+    f.store(to, 0, p.width);
+    return;
+  }
+  f.store(s_part, (int64_t)(threadIdx.x / TEAM) * kEach * TEAM, kEach * TEAM);
+  __syncthreads();
+  const int slots = TEAMS / p.block_heads;
+  for (int c = threadIdx.x; c < heads * p.width; c += TEAM * TEAMS) {
+    const int head = c / p.width, at = c - head * p.width;
+    float t = 0.0f;
+    for (int w = 0; w < slots; ++w) t += s_part[(w * p.block_heads + head) * kEach * TEAM + at];
+    to[c] = t;
+  }
+  __syncthreads();
+}
+
+template <class TX, class TY, int TEAM, bool kWide>
+__global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(true, TEAM))
+    backward_kernel(const __grid_constant__ Args p) {
+  constexpr int THREADS = TEAM > kThreads ? TEAM : kThreads, TEAMS = THREADS / TEAM, H = kEach / 2;
+  using X = Eight<TX, TEAM, kWide>;
+  using Y = Eight<TY, TEAM, kWide>;
+  using F = Eight<float, TEAM, kWide>;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __shared__ __align__(16) float s_sum[2][32][8];
+  __shared__ __align__(16) float s_part[TEAMS > 1 ? THREADS * kEach : 4];
+  int turn = 0;
+  Turns<TEAM, THREADS> of(p);
+  F weight;
+  weight.load(p.weight + (int64_t)of.head * p.width, p.width, true);
+  Vec<2> acc_weight[H], acc_bias[H];
+#pragma unroll
+  for (int i = 0; i < H; ++i) acc_weight[i] = acc_bias[i] = splat<2>(0.0f);
+  const float inv = 1.0f / (float)p.width;
+  const int64_t turns = (p.span + of.slots - 1) / of.slots;
+  X x;
+  Y dy;
+  bool on = of.row < of.end;
+  x.load(place<TX>(p.x, p, on ? of.row : 0, of.head), p.width, on);
+  dy.load(place<TY>(p.dy, p, on ? of.row : 0, of.head), p.width, on);
+#pragma unroll 1
+  for (int64_t k = 0; k < turns; ++k) {
+    const int64_t next = of.row + of.slots;
+    const bool on1 = next < of.end;
+    X x1;
+    Y dy1;
+    x1.load(place<TX>(p.x, p, on1 ? next : 0, of.head), p.width, on1);
+    dy1.load(place<TY>(p.dy, p, on1 ? next : 0, of.head), p.width, on1);
+    Vec<2> d[H], total = splat<2>(0.0f);
+#pragma unroll
+    for (int i = 0; i < H; ++i) total = total + x.two(2 * i);
+    float sum[1] = {total.v[0] + total.v[1]};
+    team_sum<1, TEAM>(sum, s_sum, turn);
+    const float mean = sum[0] * inv;
+    // sums of d^2, q, q d
+    Vec<2> part[3];
+#pragma unroll
+    for (int k3 = 0; k3 < 3; ++k3) part[k3] = splat<2>(0.0f);
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) d[i].v[j] = X::column(2 * i + j) < p.width ? x.at(2 * i + j) - mean : 0.0f;
+      const Vec<2> q = dy.two(2 * i) * weight.two(2 * i);
+      part[0] = fma(d[i], d[i], part[0]);
+      part[1] = part[1] + q;
+      part[2] = fma(q, d[i], part[2]);
+    }
+    float three[3];
+#pragma unroll
+    for (int k3 = 0; k3 < 3; ++k3) three[k3] = part[k3].v[0] + part[k3].v[1];
+    team_sum<3, TEAM>(three, s_sum, turn);
+    // (a row that is off is zeros, and adds zeros for any eps)
+    const float r = on ? inverse_root(fmaf(three[0], inv, p.eps)) : 0.0f;
+    const Vec<2> rr = splat<2>(r), mq = splat<2>(-three[1] * inv), mh = splat<2>(-three[2] * inv * r);
+    X dx;
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      const Vec<2> h = d[i] * rr, q = fma(dy.two(2 * i), weight.two(2 * i), mq);
+      dx.set(2 * i, rr * fma(h, mh, q));
+      acc_weight[i] = fma(dy.two(2 * i), h, acc_weight[i]);
+      acc_bias[i] = acc_bias[i] + dy.two(2 * i);
+    }
+    if (on) dx.store(p.dx, (of.row * p.heads + of.head) * p.width, p.width);
+    x = x1, dy = dy1, on = on1, of.row = next;
+  }
+  store_part<TEAM, TEAMS, kWide>(acc_weight, p.part_weight, p, s_part);
+  if (p.part_bias) store_part<TEAM, TEAMS, kWide>(acc_bias, p.part_bias, p, s_part);
+}
+
+struct Geometry {
+  int team;
+  bool wide;
+  int64_t blocks;
+};
+
+template <class TX, class TY>
+cudaError_t launch(const Args& p, const Geometry& g, bool backward, cudaStream_t s);
+
+}  // namespace lnorm
+}  // namespace pesq

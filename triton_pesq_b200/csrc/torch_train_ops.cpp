@@ -9,63 +9,11 @@
 #include <algorithm>
 #include <limits>
 
-#include <ATen/ATen.h>
-#include <ATen/cuda/CUDAContext.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/library.h>
-
-#include "../../include/pesq_cuda.h"
+#include "torch_checks.h"
 
 namespace {
 
-using OptTensor = std::optional<at::Tensor>;
-using torch::autograd::AutogradContext;
-using torch::autograd::Variable;
-using torch::autograd::variable_list;
-
-void check_status(int status, const char* what) {
-  if (status == PESQ_OK) return;
-  const char* msg = pesq_last_error();
-  if (status == PESQ_ERR_INVALID_ARGUMENT) TORCH_CHECK_VALUE(false, what, ": ", msg);
-  TORCH_CHECK(false, what, " failed (status ", status, "): ", msg);
-}
-
-int dtype_code(const at::Tensor& t, const char* op, const char* name) {
-  switch (t.scalar_type()) {
-    case at::kFloat:
-      return PESQ_F32;
-    case at::kBFloat16:
-      return PESQ_BF16;
-    case at::kHalf:
-      return PESQ_F16;
-    default:
-      TORCH_CHECK(false, "The CUDA ", op, " supports float32, bfloat16 and float16, `", name, "` is ", t.scalar_type(),
-                  ".");
-  }
-}
-
-void check_cuda(const at::Tensor& t, const at::Tensor& first, const char* op, const char* name) {
-  TORCH_CHECK(t.is_cuda(), "The CUDA ", op, " needs `", name, "` to live on a GPU.");
-  TORCH_CHECK(t.device() == first.device(), "The CUDA ", op, " needs all tensors on one device, `", name, "` is on ",
-              t.device(), ", not ", first.device(), ".");
-}
-
-void check_shape(const at::Tensor& t, at::IntArrayRef want, const char* op, const char* name) {
-  TORCH_CHECK_VALUE(t.sizes() == want, "The CUDA ", op, " needs `", name, "` of shape ", want, ", got ", t.sizes(), ".");
-}
-
-void check_float(const at::Tensor& t, const char* op, const char* name) {
-  TORCH_CHECK(t.scalar_type() == at::kFloat, "The CUDA ", op, " needs `", name, "` in float32, it is ", t.scalar_type(),
-              ".");
-}
-
-bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
-
-void check_gradient(const at::Tensor& t, const at::Tensor& of, at::IntArrayRef want, const char* op, const char* name) {
-  check_cuda(t, of, op, name);
-  check_shape(t, want, op, name);
-}
+using namespace pesq_torch;
 
 // channels adjacent, steps less than 2 GiB apart
 at::Tensor rows(const at::Tensor& t) {
@@ -87,24 +35,6 @@ at::Tensor aligned(const at::Tensor& t) {
 }
 
 pesq_stream stream_of(const at::Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1)}; }
-
-const float* floats(const OptTensor& t) { return t.has_value() && t->defined() ? t->data_ptr<float>() : nullptr; }
-
-OptTensor optional_of(const Variable& v) { return v.defined() ? OptTensor(v) : std::nullopt; }
-
-void no_second_derivative(const char* op) {
-  TORCH_CHECK(!at::GradMode::is_enabled(), "The CUDA ", op, " has no second derivative (create_graph=True).");
-}
-
-bool has_tangent(const at::Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
-bool has_tangent(const OptTensor& t) { return t.has_value() && has_tangent(*t); }
-template <class... Ts>
-void no_forward_mode(const char* op, const Ts&... inputs) {
-  TORCH_CHECK(!(has_tangent(inputs) || ...), "The CUDA ", op, " has no forward-mode derivative.");
-}
-
-bool wants_grad(const at::Tensor& t) { return t.requires_grad(); }
-bool wants_grad(const OptTensor& t) { return t.has_value() && t->defined() && t->requires_grad(); }
 
 // ------------------------------------------------------------------ gated scan
 
