@@ -488,6 +488,40 @@ int pesq_layer_norm_workspace(const pesq_layer_norm_desc* desc, size_t* bytes);
 int pesq_layer_norm_backward(const pesq_layer_norm_desc* desc, void* stream, pesq_heads dy, void* dx, float* dweight,
                              float* dbias, void* workspace, size_t workspace_bytes);
 
+/* Linear attention with a decay for each head, along the steps of every row,
+ *   S_t = exp(g_t) S_{t-1} + k_t v_t^T,  y_t = scale S_t^T q_t
+ * (csrc/linear_attention.cuh).  A log decay of -inf, like a reset, forgets the
+ * state. */
+typedef struct pesq_linear_attention_desc {
+  int64_t batch, steps, heads, key, value; /* batch * heads: up to 2^22; key, value: 1 .. 128 */
+  int32_t dtype;        /* PESQ_F32, PESQ_BF16 or PESQ_F16: q, k, v, y and their gradients */
+  int32_t reverse;      /* scan from the last step to the first */
+  float scale;
+  int32_t decay_shared; /* one log decay for all steps of a head: its batch and step strides are not used */
+  pesq_heads q, k, v;
+  const float* log_decay; /* g, by element strides */
+  int64_t decay_batch_stride, decay_step_stride, decay_head_stride;
+  const float* state;     /* [batch, heads, key, value], the state before the first step; NULL: zeros */
+  const uint8_t* reset;   /* nonzero: the step forgets the state; NULL: none */
+  int64_t reset_batch_stride, reset_step_stride;
+  const int64_t* lengths; /* [batch]: steps at or past it keep the state and give 0; NULL: all steps */
+} pesq_linear_attention_desc;
+
+/* Bytes (16-byte aligned buffers) of a forward's workspace, of the states it
+ * keeps for a backward call, and of the backward's workspace; they follow from
+ * the sizes, the type and decay_shared. */
+int pesq_linear_attention_sizes(const pesq_linear_attention_desc* desc, size_t* forward, size_t* kept, size_t* backward);
+/* y: [batch, steps, heads, value] dense; last: [batch, heads, key, value], the
+ * state after the last step, or NULL; kept: for the backward call, or NULL. */
+int pesq_linear_attention_forward(const pesq_linear_attention_desc* desc, void* stream, void* y, float* last, void* kept,
+                                  size_t kept_bytes, void* workspace, size_t workspace_bytes);
+/* dlast may be NULL (zeros); dstate may be NULL (not wanted).  dq, dk, dv:
+ * dense; ddecay: [heads] where the decay is shared, else [batch, steps, heads].
+ * kept: of a forward of the same values. */
+int pesq_linear_attention_backward(const pesq_linear_attention_desc* desc, void* stream, const void* kept,
+                                   size_t kept_bytes, pesq_heads dy, const float* dlast, void* dq, void* dk, void* dv,
+                                   float* ddecay, float* dstate, void* workspace, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -5,7 +5,7 @@ import ctypes
 import pytest
 import torch
 
-from triton_pesq_b200 import LayerNormCuda, _lib, layer_norm
+from triton_pesq_b200 import LayerNormCuda, LinearAttentionCuda, _lib, layer_norm, linear_attention
 
 
 def test_layer_norm_without_a_gpu():
@@ -46,3 +46,68 @@ def test_layer_norm_entry_checks_its_descriptor():
     assert lib.pesq_layer_norm_backward(ctypes.byref(d), None, none, one, one, None, one, 1 << 30) == 1
     assert lib.pesq_layer_norm_backward(ctypes.byref(d), None, x, one, one, None, one, 8) == _lib.PESQ_ERR_WORKSPACE
     assert lib.pesq_layer_norm_backward(ctypes.byref(d), None, x, one, one, None, ctypes.c_void_p(24), 1 << 30) == 3
+
+
+def test_linear_attention_without_a_gpu():
+    x = torch.zeros(1, 2, 3, 4)
+    with pytest.raises(RuntimeError, match="GPU"):
+        linear_attention(x, x, x, torch.zeros(3))
+    for kw in ({"heads": 0, "key": 4}, {"heads": 2, "key": 0}, {"heads": 2, "key": 129}, {"heads": 2, "key": 4, "slow": 1.0},
+               {"heads": 2, "key": 4, "fast": 0.99, "slow": 0.9}):
+        with pytest.raises(ValueError):
+            LinearAttentionCuda(**kw)
+    module = LinearAttentionCuda(5, 16)
+    a = torch.exp(module.log_decay())
+    assert (a[1:] > a[:-1]).all() and "heads=5" in repr(module)
+    assert float(torch.exp(LinearAttentionCuda(1, 16).log_decay())) == pytest.approx(0.875)
+
+
+def test_linear_attention_entry_checks_its_descriptor():
+    lib = _lib.library()
+
+    def make(**kw):
+        d = _lib.LinearAttentionDesc(batch=2, steps=100, heads=3, key=64, value=48, dtype=_lib.BF16, scale=1.0)
+        for k, v in kw.items():
+            setattr(d, k, v)
+        return d
+
+    def sizes(d):
+        out = [ctypes.c_size_t() for _ in range(3)]
+        return lib.pesq_linear_attention_sizes(ctypes.byref(d), *[ctypes.byref(n) for n in out]), [n.value for n in out]
+
+    assert sizes(make())[0] == _lib.PESQ_OK
+    for bad in ({"batch": 0}, {"steps": 0}, {"heads": -1}, {"key": 0}, {"value": 0}, {"dtype": 3}, {"scale": float("nan")},
+                {"scale": float("inf")}):
+        assert sizes(make(**bad))[0] == 1, bad
+    for large in ({"key": 129}, {"value": 129}, {"batch": 1 << 22}, {"batch": 1 << 40}, {"steps": 1 << 31}):
+        assert sizes(make(**large))[0] == 2, large
+    assert lib.pesq_linear_attention_sizes(ctypes.byref(make()), None, None, None) == 1
+    # a state of 32 bits before every chunk of 64 steps (of 32 where float32 keys and values are wide), of padded widths
+    for kw, chunks, width in (({}, 2, 64 * 64), ({"dtype": _lib.F32}, 2, 64 * 64), ({"key": 128, "value": 100}, 2, 128 * 128),
+                              ({"key": 128, "value": 100, "dtype": _lib.F32}, 4, 128 * 128), ({"key": 3, "value": 33}, 2, 32 * 64)):
+        assert sizes(make(**kw))[1][1] == 2 * 3 * chunks * width * 4
+    # short rows need no workspace, long ones that are few do, and a head's decay gradient always
+    assert sizes(make())[1][::2] == [0, 0]
+    assert sizes(make(decay_shared=1))[1][2] > 0
+    long = make(steps=5000)
+    assert min(sizes(long)[1]) > 0
+    one, odd = ctypes.c_void_p(16), ctypes.c_void_p(18)
+    x = _lib.Heads(data=16, batch_stride=19200, step_stride=192, head_stride=64)
+    none = _lib.Heads(data=None)
+    full = dict(q=x, k=x, v=x, log_decay=16)
+
+    def forward(d, y=one, kept=None, kept_bytes=0, ws=one, ws_bytes=1 << 30):
+        return lib.pesq_linear_attention_forward(ctypes.byref(d), None, y, one, kept, kept_bytes, ws, ws_bytes)
+
+    assert forward(make()) == 1 and forward(make(**full), y=None) == 1 and forward(make(**full), y=odd) == 1
+    assert forward(make(**{**full, "q": _lib.Heads(data=17)})) == 1
+    assert forward(make(**full), kept=one, kept_bytes=100) == _lib.PESQ_ERR_WORKSPACE
+    assert forward(make(steps=5000, **full), ws=None, ws_bytes=0) == _lib.PESQ_ERR_WORKSPACE
+
+    def backward(d, kept=one, kept_bytes=1 << 30, dy=x, dq=one, ws=one, ws_bytes=1 << 30):
+        return lib.pesq_linear_attention_backward(ctypes.byref(d), None, kept, kept_bytes, dy, None, dq, one, one, one, None,
+                                                  ws, ws_bytes)
+
+    assert backward(make(**full), dy=none) == 1 and backward(make(**full), dq=None) == 1 and backward(make(**full), dq=odd) == 1
+    assert backward(make(**full), kept=None) == 3 and backward(make(**full), kept_bytes=64) == 3
+    assert backward(make(decay_shared=1, **full), ws=None) == 3

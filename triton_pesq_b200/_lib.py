@@ -199,6 +199,32 @@ class LayerNormDesc(ctypes.Structure):
     ]
 
 
+class LinearAttentionDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int64),
+        ("steps", ctypes.c_int64),
+        ("heads", ctypes.c_int64),
+        ("key", ctypes.c_int64),
+        ("value", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("reverse", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("decay_shared", ctypes.c_int32),
+        ("q", Heads),
+        ("k", Heads),
+        ("v", Heads),
+        ("log_decay", ctypes.c_void_p),
+        ("decay_batch_stride", ctypes.c_int64),
+        ("decay_step_stride", ctypes.c_int64),
+        ("decay_head_stride", ctypes.c_int64),
+        ("state", ctypes.c_void_p),
+        ("reset", ctypes.c_void_p),
+        ("reset_batch_stride", ctypes.c_int64),
+        ("reset_step_stride", ctypes.c_int64),
+        ("lengths", ctypes.c_void_p),
+    ]
+
+
 class AdamwTensor(ctypes.Structure):
     _fields_ = [
         ("param", ctypes.c_void_p),
@@ -352,6 +378,22 @@ SIGNATURES = {
         [ctypes.POINTER(LayerNormDesc), ctypes.c_void_p, Heads, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
          ctypes.c_void_p, ctypes.c_size_t],
     ),
+    "pesq_linear_attention_sizes": (
+        ctypes.c_int,
+        [ctypes.POINTER(LinearAttentionDesc), ctypes.POINTER(ctypes.c_size_t), ctypes.POINTER(ctypes.c_size_t),
+         ctypes.POINTER(ctypes.c_size_t)],
+    ),
+    "pesq_linear_attention_forward": (
+        ctypes.c_int,
+        [ctypes.POINTER(LinearAttentionDesc), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+         ctypes.c_size_t, ctypes.c_void_p, ctypes.c_size_t],
+    ),
+    "pesq_linear_attention_backward": (
+        ctypes.c_int,
+        [ctypes.POINTER(LinearAttentionDesc), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, Heads, ctypes.c_void_p,
+         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+         ctypes.c_size_t],
+    ),
     "pesq_adamw_step": (
         ctypes.c_int,
         [ctypes.POINTER(AdamwDesc), ctypes.POINTER(AdamwTensor), ctypes.c_int64, ctypes.c_void_p],
@@ -485,6 +527,28 @@ def _register_fakes() -> None:
     @torch.library.register_fake("pesq_cuda::layer_norm_backward")
     def _layer_norm_backward(x, weight, bias, eps, dtype, dy):
         return x.new_empty(x.shape), weight.new_empty(weight.shape), weight.new_empty((0,) if bias is None else bias.shape)
+
+    @torch.library.register_fake("pesq_cuda::linear_attention_forward")
+    def _linear_attention(q, k, v, log_decay, state, reset, lengths, reverse, scale, keep):
+        batch, steps, heads, key = q.shape
+        value = v.shape[3]
+
+        def padded(n):
+            return 32 if n <= 32 else 64 if n <= 64 else 128
+
+        # a state before every chunk, in 32 bits
+        chunk = 32 if q.dtype == torch.float32 and padded(key) == 128 and padded(value) == 128 else 64
+        kept = batch * heads * ((steps + chunk - 1) // chunk) * padded(key) * padded(value) * 4 if keep else 0
+        if key == 0 or value == 0:
+            kept = 0
+        return (v.new_empty(v.shape), q.new_empty((batch, heads, key, value), dtype=torch.float32),
+                q.new_empty((kept,), dtype=torch.uint8))
+
+    @torch.library.register_fake("pesq_cuda::linear_attention_backward")
+    def _linear_attention_backward(q, k, v, log_decay, state, reset, lengths, reverse, scale, kept, dy, dlast):
+        return (q.new_empty(q.shape), q.new_empty(q.shape), v.new_empty(v.shape), log_decay.new_empty(log_decay.shape),
+                q.new_empty((q.shape[0], q.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32))
+
 
     @torch.library.register_fake("pesq_cuda::adamw_step")
     def _adamw_step(params, grads, moment1, moment2, step, scales, copies, lr, beta1, beta2, eps, weight_decay,

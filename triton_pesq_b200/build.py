@@ -31,7 +31,10 @@ CUDA_SOURCES = ["front.cu", "align.cu", "back.cu", "spectrum.cu", "chain.cu", "r
                 "iir_kf.cu", "gated_scan_f32.cu", "gated_scan_bf16.cu", "gated_scan_f16.cu", "gated_scan_abi.cu",
                 "norm_join_f32.cu", "norm_join_bf16.cu", "norm_join_f16.cu", "norm_join_f32_bf16.cu", "norm_join_f32_f16.cu",
                 "norm_join_abi.cu", "adamw.cu", "layer_norm_f32.cu", "layer_norm_bf16.cu", "layer_norm_f16.cu",
-                "layer_norm_f32_bf16.cu", "layer_norm_f32_f16.cu", "layer_norm_abi.cu"]
+                "layer_norm_f32_bf16.cu", "layer_norm_f32_f16.cu", "layer_norm_abi.cu",
+                "linear_attention_forward_f32.cu", "linear_attention_forward_bf16.cu", "linear_attention_forward_f16.cu",
+                "linear_attention_backward_f32.cu", "linear_attention_backward_bf16.cu", "linear_attention_backward_f16.cu",
+                "linear_attention_abi.cu"]
 NVCC_FLAGS = [
     "-std=c++17",
     "-O3",

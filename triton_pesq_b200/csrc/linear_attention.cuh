@@ -1,0 +1,1345 @@
+// Linear attention with a decay for each head, per row (batch item and head) of
+// [batch, step, head, channel] streams, in scan order:
+//
+//   S_t = exp(g_t) S_{t-1} + k_t v_t^T,   y_t = scale S_t^T q_t
+//
+// In chunks of C steps, with G_i the sum of the chunk's g up to step i and L_ij = exp(G_i - G_j) for
+// j <= i (0 elsewhere), this is matrix products:
+//
+//   Y  = scale ((Q K^T) o L) V + scale diag(e^G) Q S
+//   S' = e^{G_C} S + (diag(e^{G_C - G}) K)^T V
+//
+// and, with dS the gradient of the state at the chunk's end,
+//
+//   dQ = scale ((dY V^T) o L) K + scale diag(e^G) dY S^T
+//   dK = scale ((dY V^T) o L)^T Q + diag(e^{G_C - G}) V dS^T
+//   dV = scale ((Q K^T) o L)^T dY + diag(e^{G_C - G}) K dS
+//   dS' = e^{G_C} dS + scale (diag(e^G) Q)^T dY
+//
+// The gradient of g_t is what flows through step t from before it to it and later: with
+// W = scale (Q K^T) o (dY V^T) o L without its diagonal,
+//
+//   dg_t = sum_{i >= t > j} W_ij + sum_{i >= t} scale e^{G_i} q_i S dy_i + sum_{j < t} e^{G_C - G_j} k_j dS v_j
+//          + e^{G_C} <S, dS>
+//
+// in which the chunk's own sums alone are prefix sums, so that nothing large cancels over a long row.
+//
+// A CTA walks the chunks of a row, or of a part of a row where rows are few, with the state in the registers of its
+// warps as 32-bit sums and a copy in shared memory as an operand of the next chunk's products.  Parts begin from states
+// that a sweep over keys and values alone, and a join over the parts, made before.  A forward that a
+// backward follows keeps the state before every chunk, which the backward reads beside its own, the gradient of the
+// state, that it carries from the row's end.  The backward forms (Q K^T) and (dY V^T) once by rows and once by columns,
+// so that every product's left operand is in the registers of the warp that made it.
+//
+// Numbers.  All sums, the state and the decays are 32 bits; G is summed in 64 bits and kept as two floats, so that
+// differences of it are as exact as the steps' own (a reset is a step of -200 in log2, which exp2 turns to 0).
+// Products go through the matrix instructions in the operands' own type where both are inputs.  What is computed (the
+// weighted products, the state, the decayed keys) goes in as two bfloat16 terms beside bfloat16 inputs (2^-17 off),
+// as two tf32 terms (2^-22) beside float16, whose range the products and states exceed, and float32, whose inputs are also
+// two terms.
+#pragma once
+
+#include <type_traits>
+
+#include "../../include/pesq_cuda.h"
+#include "train.cuh"
+
+namespace pesq {
+namespace lattn {
+
+using namespace train;
+
+constexpr float kCut = -200.0f;  // log2 of a decay that is zero: exp2 of it and less is 0, and sums of it stay exact
+
+// ------------------------------------------------------------------------------------------- arguments
+
+struct Operand {
+  const void* p;
+  int64_t sb, st, sh;  // strides of batch, step and head, in elements
+  int unit;            // bytes that a row's pieces are loaded in: 16, 8, 4 or 2
+};
+
+struct Args {
+  Operand q, k, v, dy;
+  const float* decay;  // log decays
+  int64_t decay_sb, decay_st, decay_sh;
+  const uint8_t* reset;
+  int64_t reset_sb, reset_st;
+  const int64_t* lengths;
+  const float* state;  // [batch, heads, key, value], or null
+  int64_t steps;
+  int heads, key, value;
+  int reverse;
+  float scale;
+  int chunks, parts, part_chunks, slices;  // of a row; chunks of a part; CTAs side by side over the values
+  float *starts, *factors;  // [rows, parts, DK, DV], [rows, parts]: of a sweep and its join
+  void* kept;               // states before the chunks
+  // results
+  void* y;
+  float* last;              // or null: not wanted
+  void *dq, *dk, *dv;
+  float* ddecay;            // [batch, step, heads], or
+  double* chunk_ddecay;     // its sums over the steps of every chunk, [rows, chunks], where a head has one decay
+  const float* dlast;
+  float* dstate;
+};
+
+// ----------------------------------------------------------------------------------------- instructions
+
+__device__ __forceinline__ uint32_t smem_of(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+template <bool kTrans>
+__device__ __forceinline__ void ldmatrix(uint32_t (&r)[4], const void* p) {
+  if (kTrans)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(smem_of(p)) : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(smem_of(p)) : "memory");
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+// Sixteen columns of the contraction as two of eight.  A thread's pairs of columns 2c, 2c + 1 stand where the instruction has
+// columns c and c + 4: in both operands, so that the sum is the same.
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[8], const uint32_t (&b)[4]) {
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[4 * s]), "r"(a[4 * s + 2]), "r"(a[4 * s + 1]), "r"(a[4 * s + 3]), "r"(b[2 * s]), "r"(b[2 * s + 1]));
+}
+
+// two values as bfloat16 terms hi + lo
+__device__ __forceinline__ void split_bf16(float x, float y, uint32_t& hi, uint32_t& lo) {
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(y), "f"(x));
+  const float dx = x - __uint_as_float(hi << 16), dy = y - __uint_as_float(hi & 0xffff0000u);
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(dy), "f"(dx));
+}
+// a value as tf32 terms
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
+}
+__device__ __forceinline__ float2 floats_of(uint32_t pair, __nv_bfloat16) {
+  return make_float2(__uint_as_float(pair << 16), __uint_as_float(pair & 0xffff0000u));
+}
+__device__ __forceinline__ float2 floats_of(uint32_t pair, __half) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&pair));
+}
+
+// ------------------------------------------------------------------------------------------- operands
+//
+// A thread's share of a 16 x 16 left operand is four pairs of adjacent columns: rows g and g + 8 (g = lane / 4)
+// of columns 2c, 2c + 1 (c = lane % 4), then the same rows of columns 2c + 8, 2c + 9.  Of a 16 x 8 right operand two
+// pairs of adjacent rows of column g.  The same of every type; what is computed in a product's
+// layout (rows g, g + 8 of columns 2c, 2c + 1 of eight) is two of these eighths of a left operand.
+
+template <class T>
+constexpr bool kHalfWord = sizeof(T) == 2;
+
+// left operand: an input
+template <class T>
+struct InA {
+  uint32_t x[4];
+};
+template <>
+struct InA<float> {
+  uint32_t hi[8], lo[8];
+};
+template <class T>
+struct InB {
+  uint32_t x[2];
+};
+template <>
+struct InB<float> {
+  uint32_t hi[4], lo[4];
+};
+// computed: of two terms
+template <class T>
+struct Made {
+  uint32_t hi[8], lo[8];
+};
+template <>
+struct Made<__nv_bfloat16> {
+  uint32_t hi[4], lo[4];
+};
+template <class T>
+struct MadeB {
+  uint32_t hi[4], lo[4];
+};
+template <>
+struct MadeB<__nv_bfloat16> {
+  uint32_t hi[2], lo[2];
+};
+
+template <class T>
+__device__ __forceinline__ void make(Made<T>& m, const float (&x)[8]) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) split_bf16(x[2 * i], x[2 * i + 1], m.hi[i], m.lo[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) split_tf32(x[i], m.hi[i], m.lo[i]);
+  }
+}
+
+// The raw values of a left operand whose rows are a tile's rows (kTrans: columns)
+template <class T, int LD, bool kTrans>
+__device__ __forceinline__ void load_a(float (&x)[8], const T* tile, int m0, int k0) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  if constexpr (kHalfWord<T>) {
+    uint32_t r[4];
+    const T* at = kTrans ? tile + (k0 + (lane >> 4) * 8 + (lane & 7)) * LD + m0 + (lane >> 3 & 1) * 8
+                         : tile + (m0 + (lane & 15)) * LD + k0 + (lane >> 4) * 8;
+    ldmatrix<kTrans>(r, at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = floats_of(r[i], T{});
+      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int m = m0 + g + (i & 1) * 8, k = k0 + 2 * c + (i >> 1) * 8;
+      if (kTrans) {
+        x[2 * i] = tile[k * LD + m], x[2 * i + 1] = tile[(k + 1) * LD + m];
+      } else {
+        const float2 f = *reinterpret_cast<const float2*>(tile + m * LD + k);
+        x[2 * i] = f.x, x[2 * i + 1] = f.y;
+      }
+    }
+  }
+}
+template <class T, int LD>
+__device__ __forceinline__ void load_a(InA<T>& a, const T* tile, int m0, int k0) {
+  if constexpr (kHalfWord<T>) {
+    const int lane = threadIdx.x & 31;
+    ldmatrix<false>(a.x, tile + (m0 + (lane & 15)) * LD + k0 + (lane >> 4) * 8);
+  } else {
+    float x[8];
+    load_a<T, LD, false>(x, tile, m0, k0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) split_tf32(x[i], a.hi[i], a.lo[i]);
+  }
+}
+// two right operands, of columns n0 .. n0 + 7 and n0 + 8 .. n0 + 15: columns are a tile's rows (kTrans: columns)
+template <class T, int LD, bool kTrans>
+__device__ __forceinline__ void load_words(uint32_t (&r)[4], const T* tile, int n0, int k0) {
+  const int lane = threadIdx.x & 31, a = lane >> 4, b = lane >> 3 & 1, row = lane & 7;
+  ldmatrix<kTrans>(r, kTrans ? tile + (k0 + b * 8 + row) * LD + n0 + a * 8 : tile + (n0 + a * 8 + row) * LD + k0 + b * 8);
+}
+template <int LD, bool kTrans>
+__device__ __forceinline__ void load_floats(float (&x)[8], const float* tile, int n0, int k0) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int n = n0 + g + (i >> 1) * 8, k = k0 + 2 * c + (i & 1) * 8;
+    if (kTrans) {
+      x[2 * i] = tile[k * LD + n], x[2 * i + 1] = tile[(k + 1) * LD + n];
+    } else {
+      const float2 f = *reinterpret_cast<const float2*>(tile + n * LD + k);
+      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    }
+  }
+}
+template <class T, int LD, bool kTrans>
+__device__ __forceinline__ void load_b(InB<T> (&b)[2], const T* tile, int n0, int k0) {
+  if constexpr (kHalfWord<T>) {
+    uint32_t r[4];
+    load_words<T, LD, kTrans>(r, tile, n0, k0);
+    b[0].x[0] = r[0], b[0].x[1] = r[1], b[1].x[0] = r[2], b[1].x[1] = r[3];
+  } else {
+    float x[8];
+    load_floats<LD, kTrans>(x, tile, n0, k0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) split_tf32(x[i], b[i >> 2].hi[i & 3], b[i >> 2].lo[i & 3]);
+  }
+}
+
+// The state as an operand: two planes of bfloat16, or 32 bits
+template <class T>
+using Stored = std::conditional_t<std::is_same<T, __nv_bfloat16>::value, __nv_bfloat16, float>;
+template <class T>
+constexpr int kPlanes = std::is_same<T, __nv_bfloat16>::value ? 2 : 1;
+
+template <class T, int LD, int PLANE, bool kTrans>
+__device__ __forceinline__ void load_state(MadeB<T> (&b)[2], const Stored<T>* s, int n0, int k0) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    uint32_t r[4];
+    load_words<__nv_bfloat16, LD, kTrans>(r, s, n0, k0);
+    b[0].hi[0] = r[0], b[0].hi[1] = r[1], b[1].hi[0] = r[2], b[1].hi[1] = r[3];
+    load_words<__nv_bfloat16, LD, kTrans>(r, s + PLANE, n0, k0);
+    b[0].lo[0] = r[0], b[0].lo[1] = r[1], b[1].lo[0] = r[2], b[1].lo[1] = r[3];
+  } else {
+    float x[8];
+    load_floats<LD, kTrans>(x, s, n0, k0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) split_tf32(x[i], b[i >> 2].hi[i & 3], b[i >> 2].lo[i & 3]);
+  }
+}
+template <class T, int LD, int PLANE>
+__device__ __forceinline__ void store_state(Stored<T>* s, int row, int col, float x, float y) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    uint32_t hi, lo;
+    split_bf16(x, y, hi, lo);
+    *reinterpret_cast<uint32_t*>(s + row * LD + col) = hi;
+    *reinterpret_cast<uint32_t*>(s + PLANE + row * LD + col) = lo;
+  } else {
+    *reinterpret_cast<float2*>(s + row * LD + col) = make_float2(x, y);
+  }
+}
+template <class T, int LD, int PLANE>
+__device__ __forceinline__ float2 read_state(const Stored<T>* s, int row, int col) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const float2 a = floats_of(*reinterpret_cast<const uint32_t*>(s + row * LD + col), __nv_bfloat16{});
+    const float2 b = floats_of(*reinterpret_cast<const uint32_t*>(s + PLANE + row * LD + col), __nv_bfloat16{});
+    return make_float2(a.x + b.x, a.y + b.y);
+  } else {
+    return *reinterpret_cast<const float2*>(s + row * LD + col);
+  }
+}
+
+// ------------------------------------------------------------------------------------------- products
+
+template <class T>
+__device__ __forceinline__ void widen_a(uint32_t (&w)[8], const InA<T>& a) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = floats_of(a.x[i], T{});
+    w[2 * i] = __float_as_uint(f.x), w[2 * i + 1] = __float_as_uint(f.y);
+  }
+}
+// input times input
+template <class T>
+__device__ __forceinline__ void mma(float (&c)[4], const InA<T>& a, const InB<T>& b) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    mma_bf16(c, a.x, b.x);
+  } else if constexpr (std::is_same<T, __half>::value) {
+    mma_f16(c, a.x, b.x);
+  } else {
+    mma_tf32(c, a.lo, b.hi);
+    mma_tf32(c, a.hi, b.lo);
+    mma_tf32(c, a.hi, b.hi);
+  }
+}
+// computed times input
+template <class T>
+__device__ __forceinline__ void mma(float (&c)[4], const Made<T>& a, const InB<T>& b) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    mma_bf16(c, a.lo, b.x);
+    mma_bf16(c, a.hi, b.x);
+  } else if constexpr (std::is_same<T, __half>::value) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float2 f = floats_of(b.x[i], T{});
+      w[2 * i] = __float_as_uint(f.x), w[2 * i + 1] = __float_as_uint(f.y);
+    }
+    mma_tf32(c, a.lo, w);
+    mma_tf32(c, a.hi, w);
+  } else {
+    mma_tf32(c, a.lo, b.hi);
+    mma_tf32(c, a.hi, b.lo);
+    mma_tf32(c, a.hi, b.hi);
+  }
+}
+// input times state
+template <class T>
+__device__ __forceinline__ void mma(float (&c)[4], const InA<T>& a, const MadeB<T>& b) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    mma_bf16(c, a.x, b.lo);
+    mma_bf16(c, a.x, b.hi);
+  } else if constexpr (std::is_same<T, __half>::value) {
+    uint32_t w[8];
+    widen_a(w, a);
+    mma_tf32(c, w, b.lo);
+    mma_tf32(c, w, b.hi);
+  } else {
+    mma_tf32(c, a.lo, b.hi);
+    mma_tf32(c, a.hi, b.lo);
+    mma_tf32(c, a.hi, b.hi);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ geometry
+
+template <class T, int D>
+constexpr int kLd = D + (sizeof(T) == 2 ? 8 : 4);  // 16 bytes of padding: eight rows' pieces lie in different banks
+
+// One row's steps: of the n that count, scan order s is time t; those past them follow in both orders
+struct Row {
+  int64_t b, steps, n;
+  int h, reverse;
+  __device__ __forceinline__ Row(const Args& p, int64_t row) {
+    b = row / p.heads;
+    h = (int)(row - b * p.heads);
+    steps = p.steps;
+    n = steps;
+    if (p.lengths) n = max((int64_t)0, min(steps, p.lengths[b]));
+    reverse = p.reverse;
+  }
+  __device__ __forceinline__ int64_t time(int64_t s) const { return reverse && s < n ? n - 1 - s : s; }
+};
+
+// Rows s0 .. s0 + C - 1 of an operand to a tile, zeros for steps past the row's length.  The columns past `cols` are
+// zeros from before.
+template <class T, int D, int C, int THREADS>
+__device__ __forceinline__ void load_tile(T* tile, const Operand& o, int first, int cols, const Row& row, int64_t s0) {
+  constexpr int LD = kLd<T, D>, kPer = D * (int)sizeof(T) / 16;  // 16-byte pieces of a row
+  constexpr int kRows = THREADS / kPer;
+  static_assert(THREADS % kPer == 0 && C % kRows == 0 || kRows > C, "");
+  const int piece = threadIdx.x % kPer, bytes = cols * (int)sizeof(T) - piece * 16;
+  if (bytes <= 0) return;
+  const char* base = static_cast<const char*>(o.p) + (row.b * o.sb + row.h * o.sh + first) * (int64_t)sizeof(T) + piece * 16;
+#pragma unroll
+  for (int r0 = 0; r0 < C; r0 += kRows) {
+    const int r = r0 + threadIdx.x / kPer;
+    if (kRows > C && r >= C) break;
+    const int64_t s = s0 + r;
+    const bool live = s < row.n;
+    const char* from = live ? base + row.time(s) * o.st * (int64_t)sizeof(T) : static_cast<const char*>(o.p);
+    char* to = reinterpret_cast<char*>(tile + r * LD) + piece * 16;
+    if (o.unit == 16) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_of(to)), "l"(from), "r"(live ? 16 : 0) : "memory");
+    } else if (o.unit == 8) {
+#pragma unroll
+      for (int x = 0; x < 16; x += 8)
+        if (x < bytes)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_of(to + x)), "l"(live ? from + x : from), "r"(live ? 8 : 0) : "memory");
+    } else if (o.unit == 4) {
+#pragma unroll
+      for (int x = 0; x < 16; x += 4)
+        if (x < bytes)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_of(to + x)), "l"(live ? from + x : from), "r"(live ? 4 : 0) : "memory");
+    } else {
+#pragma unroll
+      for (int x = 0; x < 16; x += 2)
+        if (x < bytes) *reinterpret_cast<uint16_t*>(to + x) = live ? *reinterpret_cast<const uint16_t*>(from + x) : (uint16_t)0;
+    }
+  }
+}
+__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+
+// Decays of a chunk's steps, by one warp.  Between load (early) and store lies the latency of the loads.
+template <int C>
+struct Decays {
+  static constexpr int E = C / 32;
+  float g[E];
+  __device__ __forceinline__ void load(const Args& p, const Row& row, int64_t s0) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int64_t s = s0 + lane * E + e;
+      g[e] = 0.0f;
+      if (s < row.n) {
+        const int64_t t = row.time(s);
+        g[e] = p.decay[row.b * p.decay_sb + t * p.decay_st + row.h * p.decay_sh];
+        if (p.reset && p.reset[row.b * p.reset_sb + t * p.reset_st]) g[e] = -INFINITY;
+      }
+    }
+  }
+  __device__ __forceinline__ static double log2_of(float g) {
+    return g * kLog2e < kCut ? (double)kCut : (double)g * 1.4426950408889634;  // (a NaN stays one)
+  }
+  // sums as two floats, e^{G_i}, e^{G_C - G_j}
+  __device__ __forceinline__ void store(float2* sums, float* before, float* after) const {
+    const int lane = threadIdx.x & 31;
+    double own[E], total = 0.0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) own[e] = total += log2_of(g[e]);
+    double up = total;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const double v = __shfl_up_sync(0xffffffffu, up, off);
+      if (lane >= off) up += v;
+    }
+    const double all = __shfl_sync(0xffffffffu, up, 31);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const double at = up - total + own[e];
+      const float hi = (float)at;
+      sums[lane * E + e] = make_float2(hi, (float)(at - hi));
+      before[lane * E + e] = exp2_approx(hi);
+      after[lane * E + e] = exp2_approx((float)(all - at));
+    }
+  }
+};
+__device__ __forceinline__ float between(float2 i, float2 j) { return exp2_approx((i.x - j.x) + (i.y - j.y)); }
+// a factor of zero cuts off whatever it multiplies
+__device__ __forceinline__ float decayed(float factor, float x) { return factor == 0.0f ? 0.0f : factor * x; }
+
+// A warp's part of a DK x DV state: kTiles tiles of 16 rows, kCols columns
+template <int DK, int DV, int WARPS>
+struct StateShape {
+  static constexpr int kRowWarps = WARPS < DK / 16 ? WARPS : DK / 16;
+  static constexpr int kColWarps = WARPS / kRowWarps;
+  static constexpr int kTiles = DK / 16 / kRowWarps;
+  static constexpr int kCols = DV / kColWarps;
+  static_assert(kCols % 16 == 0, "");
+};
+template <int DK, int DV, int WARPS>
+struct State {
+  using Shape = StateShape<DK, DV, WARPS>;
+  float x[Shape::kTiles][Shape::kCols / 8][4];
+
+  static __device__ __forceinline__ int row0() { return (threadIdx.x >> 5) % Shape::kRowWarps * Shape::kTiles * 16; }
+  static __device__ __forceinline__ int col0() { return (threadIdx.x >> 5) / Shape::kRowWarps * Shape::kCols; }
+  // f(row, column, value of it, of the next column), rows and columns of the state
+  template <class F>
+  __device__ __forceinline__ void each(F f) {
+    const int g = (threadIdx.x & 31) >> 2, c = threadIdx.x & 3;
+#pragma unroll
+    for (int m = 0; m < Shape::kTiles; ++m)
+#pragma unroll
+      for (int n = 0; n < Shape::kCols / 8; ++n)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+          f(row0() + m * 16 + g + half * 8, col0() + n * 8 + 2 * c, x[m][n][2 * half], x[m][n][2 * half + 1]);
+  }
+  // from a dense [key, value] matrix's columns from `first`, or zeros
+  __device__ __forceinline__ void read(const float* from, int key, int value, int first) {
+    each([&](int r, int c, float& a, float& b) {
+      const bool in = from && r < key;
+      a = in && first + c < value ? from[(int64_t)r * value + first + c] : 0.0f;
+      b = in && first + c + 1 < value ? from[(int64_t)r * value + first + c + 1] : 0.0f;
+    });
+  }
+  __device__ __forceinline__ void write(float* to, int key, int value, int first) {
+    each([&](int r, int c, float& a, float& b) {
+      if (r < key && first + c < value) to[(int64_t)r * value + first + c] = a;
+      if (r < key && first + c + 1 < value) to[(int64_t)r * value + first + c + 1] = b;
+    });
+  }
+  // S = factor S + sum over the chunk's steps of weight a b^T
+  template <class T, int C>
+  __device__ __forceinline__ void update(const T* a, const T* b, const float* weights, float factor, float scale) {
+    const int c = threadIdx.x & 3;
+#pragma unroll
+    for (int m = 0; m < Shape::kTiles; ++m)
+#pragma unroll
+      for (int n = 0; n < Shape::kCols / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[m][n][e] = decayed(factor, x[m][n][e]);
+#pragma unroll
+    for (int k = 0; k < C; k += 16) {
+      const float2 w0 = *reinterpret_cast<const float2*>(weights + k + 2 * c);
+      const float2 w1 = *reinterpret_cast<const float2*>(weights + k + 8 + 2 * c);
+      Made<T> left[Shape::kTiles];
+#pragma unroll
+      for (int m = 0; m < Shape::kTiles; ++m) {
+        float f[8];
+        load_a<T, kLd<T, DK>, true>(f, a, row0() + m * 16, k);
+        f[0] *= w0.x * scale, f[1] *= w0.y * scale, f[2] *= w0.x * scale, f[3] *= w0.y * scale;
+        f[4] *= w1.x * scale, f[5] *= w1.y * scale, f[6] *= w1.x * scale, f[7] *= w1.y * scale;
+        make(left[m], f);
+      }
+#pragma unroll
+      for (int n = 0; n < Shape::kCols / 16; ++n) {
+        InB<T> right[2];
+        load_b<T, kLd<T, DV>, true>(right, b, col0() + n * 16, k);
+#pragma unroll
+        for (int m = 0; m < Shape::kTiles; ++m) {
+          mma(x[m][2 * n], left[m], right[0]);
+          mma(x[m][2 * n + 1], left[m], right[1]);
+        }
+      }
+    }
+  }
+  // to shared memory, as an operand
+  template <class T>
+  __device__ __forceinline__ void publish(Stored<T>* s) {
+    each([&](int r, int c, float& a, float& b) { store_state<T, kLd<Stored<T>, DV>, DK * kLd<Stored<T>, DV>>(s, r, c, a, b); });
+  }
+};
+
+// Bytes of the state before a chunk: two planes of 16 bits, or 32, of [DK][DV]
+__host__ __device__ constexpr int64_t kept_bytes(int DK, int DV) { return (int64_t)4 * DK * DV; }
+
+template <class T>
+__device__ __forceinline__ void store_pair(void* base, int64_t at, int col, int cols, float x, float y) {
+  T* to = static_cast<T*>(base) + at + col;
+  if (cols % 2 == 0) {
+    if (col < cols) {
+      Pack<T, 2> v;
+      v.v[0] = narrow<T>(x), v.v[1] = narrow<T>(y);
+      *reinterpret_cast<Pack<T, 2>*>(to) = v;
+    }
+  } else {
+    if (col < cols) to[0] = narrow<T>(x);
+    if (col + 1 < cols) to[1] = narrow<T>(y);
+  }
+}
+
+template <int THREADS>
+__device__ __forceinline__ void clear(void* p, int bytes) {
+  uint4* q = static_cast<uint4*>(p);
+  for (int i = threadIdx.x; i < bytes / 16; i += THREADS) q[i] = make_uint4(0u, 0u, 0u, 0u);
+}
+
+// ------------------------------------------------------------------------------------------- forward
+
+template <class T, int DK, int DV, int C>
+struct ForwardShared {
+  static constexpr int kTiles = (2 * C * kLd<T, DK> + C * kLd<T, DV>) * (int)sizeof(T);
+  static constexpr int kState = kPlanes<T> * DK * kLd<Stored<T>, DV> * (int)sizeof(Stored<T>);
+  static constexpr int kDecays = 2 * C * 16;  // two chunks' sums, e^G and e^{G_C - G}
+  // the next chunk's tiles come in while one is worked on, where three CTAs an SM have the room
+  static constexpr int kStages = 2 * kTiles + kState + kDecays <= (75 << 10) ? 2 : 1;
+  static constexpr int kBytes = kStages * kTiles + kState + kDecays;
+};
+
+template <class T, int DK, int DV, int C>
+__global__ void __launch_bounds__(128) forward_kernel(const __grid_constant__ Args p) {
+  constexpr int THREADS = 128, WARPS = 4, RG = C / 16, WC = WARPS / RG, NY = DV / WC / 8;
+  using Sh = ForwardShared<T, DK, DV, C>;
+  constexpr int LDK = kLd<T, DK>, LDV = kLd<T, DV>, LDS = kLd<Stored<T>, DV>, PLANE = DK * LDS;
+  extern __shared__ __align__(16) char shared[];
+  char* tiles = shared;
+  Stored<T>* s_state = reinterpret_cast<Stored<T>*>(shared + Sh::kStages * Sh::kTiles);
+  char* decays = shared + Sh::kStages * Sh::kTiles + Sh::kState;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  const int rg = warp % RG, wc = warp / RG;
+
+  const int slice = blockIdx.x % p.slices;
+  const int64_t unit = blockIdx.x / p.slices, index = unit / p.parts;
+  const int part = (int)(unit - index * p.parts);
+  const Row row(p, index);
+  const int first = slice * DV, cols = min(DV, p.value - first);
+  const int c0 = part * p.part_chunks, c1 = min(p.chunks, c0 + p.part_chunks);
+  const int padded = DV * p.slices;  // columns of the states in memory
+
+  clear<THREADS>(shared, Sh::kStages * Sh::kTiles);
+  State<DK, DV, WARPS> S;
+  const float* from = p.state ? p.state + index * p.key * p.value : nullptr;
+  if (p.parts > 1)
+    S.read(p.starts + (index * p.parts + part) * DK * padded, DK, padded, first);
+  else
+    S.read(from, p.key, p.value, first);
+  S.template publish<T>(s_state);
+  __syncthreads();
+
+  const auto q_of = [&](int stage) { return reinterpret_cast<T*>(tiles + stage * Sh::kTiles); };
+  const auto load = [&](int chunk, int stage) {
+    T* q = q_of(stage);
+    const int64_t s0 = (int64_t)chunk * C;
+    if (s0 < row.n) {
+      load_tile<T, DK, C, THREADS>(q, p.q, 0, p.key, row, s0);
+      load_tile<T, DK, C, THREADS>(q + C * LDK, p.k, 0, p.key, row, s0);
+      load_tile<T, DV, C, THREADS>(q + 2 * C * LDK, p.v, first, cols, row, s0);
+    }
+    copies_issued();
+  };
+  const auto sums_of = [&](int chunk) { return reinterpret_cast<float2*>(decays + (chunk & 1) * C * 16); };
+  Decays<C> next;
+  load(c0, 0);
+  if (warp == WARPS - 1) {
+    next.load(p, row, (int64_t)c0 * C);
+    next.store(sums_of(c0), reinterpret_cast<float*>(sums_of(c0) + C), reinterpret_cast<float*>(sums_of(c0) + C) + C);
+  }
+#pragma unroll 1
+  for (int chunk = c0; chunk < c1; ++chunk) {
+    const int stage = Sh::kStages == 2 ? (chunk - c0) & 1 : 0;
+    const int64_t s0 = (int64_t)chunk * C;
+    copies_done();
+    __syncthreads();  // the chunk's tiles, decays and state are there
+    if (Sh::kStages == 2 && chunk + 1 < c1) load(chunk + 1, stage ^ 1);
+    if (warp == WARPS - 1 && chunk + 1 < c1) next.load(p, row, s0 + C);
+    const T *q = q_of(stage), *k = q + C * LDK, *v = q + 2 * C * LDK;
+    const float2* sums = sums_of(chunk);
+    const float *before = reinterpret_cast<const float*>(sums + C), *after = before + C;
+    const bool live = s0 < row.n;
+    if (live && p.kept) {
+      // the state before the chunk, for the backward: 16-byte pieces of the operand's planes
+      constexpr int kPieces = DV * (int)sizeof(Stored<T>) / 16;
+      char* to = static_cast<char*>(p.kept) + (index * p.chunks + chunk) * kept_bytes(DK, padded) + first * (int)sizeof(Stored<T>);
+      for (int i = threadIdx.x; i < kPlanes<T> * DK * kPieces; i += THREADS) {
+        const int r = i / kPieces, piece = i % kPieces;  // (rows of both planes, one after the other)
+        *reinterpret_cast<uint4*>(to + (int64_t)r * padded * (int)sizeof(Stored<T>) + piece * 16) =
+            *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(s_state + r * LDS) + piece * 16);
+      }
+    }
+    float y[NY][4];
+#pragma unroll
+    for (int n = 0; n < NY; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[n][e] = 0.0f;
+    if (live) {
+      float a[C / 8][4];
+#pragma unroll
+      for (int n = 0; n < C / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[n][e] = 0.0f;
+#pragma unroll
+      for (int kk = 0; kk < DK; kk += 16) {
+        InA<T> left;
+        load_a<T, LDK>(left, q, rg * 16, kk);
+#pragma unroll
+        for (int n = 0; n < C / 16; ++n) {
+          if (n > rg) break;
+          InB<T> right[2];
+          load_b<T, LDK, false>(right, k, n * 16, kk);
+          mma(a[2 * n], left, right[0]);
+          mma(a[2 * n + 1], left, right[1]);
+        }
+#pragma unroll
+        for (int n = 0; n < NY / 2; ++n) {
+          MadeB<T> right[2];
+          load_state<T, LDS, PLANE, true>(right, s_state, wc * NY * 8 + n * 16, kk);
+          mma(y[2 * n], left, right[0]);
+          mma(y[2 * n + 1], left, right[1]);
+        }
+      }
+      const int i0 = rg * 16 + g, i1 = i0 + 8;
+      const float b0 = before[i0] * p.scale, b1 = before[i1] * p.scale;
+#pragma unroll
+      for (int n = 0; n < NY; ++n) {
+        y[n][0] = decayed(b0, y[n][0]), y[n][1] = decayed(b0, y[n][1]);
+        y[n][2] = decayed(b1, y[n][2]), y[n][3] = decayed(b1, y[n][3]);
+      }
+      const float2 sum0 = sums[i0], sum1 = sums[i1];
+#pragma unroll
+      for (int n = 0; n < C / 16; ++n) {
+        if (n > rg) break;
+        float x[8];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int j = n * 16 + half * 8 + 2 * c;
+          const float4 two = *reinterpret_cast<const float4*>(sums + j);
+          const float2 s0j = make_float2(two.x, two.y), s1j = make_float2(two.z, two.w);
+          const float(&at)[4] = a[2 * n + half];
+          x[4 * half] = j <= i0 ? at[0] * (p.scale * between(sum0, s0j)) : 0.0f;
+          x[4 * half + 1] = j + 1 <= i0 ? at[1] * (p.scale * between(sum0, s1j)) : 0.0f;
+          x[4 * half + 2] = j <= i1 ? at[2] * (p.scale * between(sum1, s0j)) : 0.0f;
+          x[4 * half + 3] = j + 1 <= i1 ? at[3] * (p.scale * between(sum1, s1j)) : 0.0f;
+        }
+        Made<T> left;
+        make(left, x);
+#pragma unroll
+        for (int m = 0; m < NY / 2; ++m) {
+          InB<T> right[2];
+          load_b<T, LDV, true>(right, v, wc * NY * 8 + m * 16, n * 16);
+          mma(y[2 * m], left, right[0]);
+          mma(y[2 * m + 1], left, right[1]);
+        }
+      }
+      S.template update<T, C>(k, v, after, before[C - 1], 1.0f);
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int64_t s = s0 + rg * 16 + g + half * 8;
+      if (s >= row.steps) continue;
+      const int64_t at = ((row.b * row.steps + row.time(s)) * p.heads + row.h) * p.value;
+      const bool in = s < row.n;
+#pragma unroll
+      for (int n = 0; n < NY; ++n)
+        store_pair<T>(p.y, at, first + wc * NY * 8 + n * 8 + 2 * c, p.value, in ? y[n][2 * half] : 0.0f,
+                      in ? y[n][2 * half + 1] : 0.0f);
+    }
+    if (warp == WARPS - 1 && chunk + 1 < c1) {
+      float2* to = sums_of(chunk + 1);
+      next.store(to, reinterpret_cast<float*>(to + C), reinterpret_cast<float*>(to + C) + C);
+    }
+    __syncthreads();  // the chunk's tiles and state are read
+    if (live) S.template publish<T>(s_state);
+    if (Sh::kStages == 1 && chunk + 1 < c1) load(chunk + 1, 0);
+  }
+  if (p.last && c1 == p.chunks) S.write(p.last + index * p.key * p.value, p.key, p.value, first);
+}
+
+// ------------------------------------------------------------------------------------- states of parts
+
+// What a part's steps add to the state, and its decay: from keys and values in scan order (kBackward: from queries and
+// the upstream gradient, from the end)
+template <class T, int DK, int DV, int C>
+struct SweepShared {
+  static constexpr int kTiles = C * (kLd<T, DK> + kLd<T, DV>) * (int)sizeof(T);
+  static constexpr int kDecays = 2 * C * 16;
+  static constexpr int kBytes = 2 * kTiles + kDecays;
+};
+template <class T, int DK, int DV, int C, bool kBackward>
+__global__ void __launch_bounds__(128) sweep_kernel(const __grid_constant__ Args p) {
+  constexpr int THREADS = 128, WARPS = 4;
+  using Sh = SweepShared<T, DK, DV, C>;
+  constexpr int LDK = kLd<T, DK>;
+  extern __shared__ __align__(16) char shared[];
+  char* decays = shared + 2 * Sh::kTiles;
+  const int warp = threadIdx.x >> 5;
+  const int slice = blockIdx.x % p.slices;
+  const int64_t unit = blockIdx.x / p.slices, index = unit / p.parts;
+  const int part = (int)(unit - index * p.parts);
+  const Row row(p, index);
+  const int first = slice * DV, cols = min(DV, p.value - first), padded = DV * p.slices;
+  const int c0 = part * p.part_chunks, c1 = min(p.chunks, c0 + p.part_chunks);
+  if (part == (kBackward ? 0 : p.parts - 1)) return;  // (nothing begins from it)
+  clear<THREADS>(shared, 2 * Sh::kTiles);
+  State<DK, DV, WARPS> S;
+  S.read(nullptr, 0, 0, 0);
+  float factor = 1.0f;
+  __syncthreads();
+  const auto load = [&](int chunk, int stage) {
+    T* a = reinterpret_cast<T*>(shared + stage * Sh::kTiles);
+    const int64_t s0 = (int64_t)chunk * C;
+    if (s0 < row.n) {
+      load_tile<T, DK, C, THREADS>(a, kBackward ? p.q : p.k, 0, p.key, row, s0);
+      load_tile<T, DV, C, THREADS>(a + C * LDK, kBackward ? p.dy : p.v, first, cols, row, s0);
+    }
+    copies_issued();
+  };
+  const int count = c1 - c0;
+  const auto chunk_of = [&](int i) { return kBackward ? c1 - 1 - i : c0 + i; };
+  const auto sums_of = [&](int i) { return reinterpret_cast<float2*>(decays + (i & 1) * C * 16); };
+  Decays<C> next;
+  const auto store = [&](int i) {
+    float2* to = sums_of(i);
+    next.store(to, reinterpret_cast<float*>(to + C), reinterpret_cast<float*>(to + C) + C);
+  };
+  load(chunk_of(0), 0);
+  if (warp == WARPS - 1) {
+    next.load(p, row, (int64_t)chunk_of(0) * C);
+    store(0);
+  }
+#pragma unroll 1
+  for (int i = 0; i < count; ++i) {
+    copies_done();
+    __syncthreads();
+    if (i + 1 < count) {
+      load(chunk_of(i + 1), (i + 1) & 1);
+      if (warp == WARPS - 1) next.load(p, row, (int64_t)chunk_of(i + 1) * C);
+    }
+    if ((int64_t)chunk_of(i) * C < row.n) {
+      const T* a = reinterpret_cast<const T*>(shared + (i & 1) * Sh::kTiles);
+      const float *before = reinterpret_cast<const float*>(sums_of(i) + C), *after = before + C;
+      S.template update<T, C>(a, a + C * LDK, kBackward ? before : after, before[C - 1], kBackward ? p.scale : 1.0f);
+      factor *= before[C - 1];
+    }
+    if (warp == WARPS - 1 && i + 1 < count) store(i + 1);
+    __syncthreads();
+  }
+  S.write(p.starts + (index * p.parts + part) * DK * padded, DK, padded, first);
+  if (threadIdx.x == 0 && slice == 0) p.factors[index * p.parts + part] = factor;
+}
+
+// What the parts add, to the states that they begin from; a thread takes an element of a row's state
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ Args p, int DK, int DV, int backward) {
+  const int64_t size = (int64_t)DK * DV, per = (size + kThreads - 1) / kThreads;
+  const int64_t index = blockIdx.x / per, at = (blockIdx.x - index * per) * kThreads + threadIdx.x;
+  if (at >= size) return;
+  const int r = (int)(at / DV), c = (int)(at - (int64_t)r * DV);
+  const float* from = backward ? p.dlast : p.state;
+  float s = from && r < p.key && c < p.value ? from[(index * p.key + r) * p.value + c] : 0.0f;
+  float* starts = p.starts + index * p.parts * size + at;
+  const float* factors = p.factors + index * p.parts;
+  for (int i = 0; i < p.parts; ++i) {
+    const int part = backward ? p.parts - 1 - i : i;
+    const float add = i + 1 < p.parts ? starts[part * size] : 0.0f;
+    starts[part * size] = s;
+    if (i + 1 < p.parts) s = decayed(factors[part], s) + add;
+  }
+}
+
+// ------------------------------------------------------------------------------------------ backward
+
+template <class T, int DK, int DV>
+constexpr int kBackWarps = DK > 64 || DV > 64 ? 8 : 4;
+
+template <class T, int DK, int DV, int C>
+struct BackwardShared {
+  static constexpr int WARPS = kBackWarps<T, DK, DV>, WC = WARPS / (C / 16);
+  static constexpr int kTiles = 2 * C * (kLd<T, DK> + kLd<T, DV>) * (int)sizeof(T);
+  static constexpr int kState = kPlanes<T> * DK * kLd<Stored<T>, DV> * (int)sizeof(Stored<T>);
+  static constexpr int kDecays = 2 * C * 16;
+  static constexpr int kSums = ((2 * WC + C / 16 + 1) * C + WARPS) * 4;
+  static constexpr int kBytes = kTiles + 2 * kState + kDecays + kSums;
+};
+
+template <class T, int DK, int DV, int C>
+__global__ void __launch_bounds__(32 * kBackWarps<T, DK, DV>) backward_kernel(const __grid_constant__ Args p) {
+  using Sh = BackwardShared<T, DK, DV, C>;
+  constexpr int WARPS = Sh::WARPS, THREADS = 32 * WARPS, RG = C / 16, WC = Sh::WC, NK = DK / WC / 8, NV = DV / WC / 8;
+  constexpr int LDK = kLd<T, DK>, LDV = kLd<T, DV>, LDS = kLd<Stored<T>, DV>, PLANE = DK * LDS;
+  extern __shared__ __align__(16) char shared[];
+  T *q = reinterpret_cast<T*>(shared), *k = q + C * LDK, *v = k + C * LDK, *dy = v + C * LDV;
+  Stored<T>* s_state = reinterpret_cast<Stored<T>*>(shared + Sh::kTiles);  // before the chunk
+  Stored<T>* s_grad = reinterpret_cast<Stored<T>*>(shared + Sh::kTiles + Sh::kState);
+  char* decays = shared + Sh::kTiles + 2 * Sh::kState;
+  float* s_far = reinterpret_cast<float*>(decays + Sh::kDecays);  // [WC][C]: scale e^{G_i} q_i S dy_i
+  float* s_end = s_far + WC * C;                                  // [WC][C]: e^{G_C - G_j} k_j dS v_j
+  float* s_row = s_end + WC * C;                                  // [RG][C]: sums of W over the warp's j, of each i
+  float* s_col = s_row + RG * C;                                  // [C]: over i, of each j
+  float* s_all = s_col + C;                                       // [WARPS]: <S, dS>
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  const int rg = warp % RG, wc = warp / RG;
+
+  const int64_t index = blockIdx.x / p.parts;
+  const int part = (int)(blockIdx.x - index * p.parts);
+  const Row row(p, index);
+  const int c0 = part * p.part_chunks, c1 = min(p.chunks, c0 + p.part_chunks);
+
+  clear<THREADS>(shared, Sh::kTiles);
+  State<DK, DV, WARPS> S;  // the gradient of the state
+  const float* from = p.dlast ? p.dlast + index * p.key * p.value : nullptr;
+  if (p.parts > 1)
+    S.read(p.starts + (index * p.parts + part) * DK * DV, DK, DV, 0);
+  else
+    S.read(from, p.key, p.value, 0);
+  S.template publish<T>(s_grad);
+  __syncthreads();
+
+  const auto load = [&](int chunk) {
+    const int64_t s0 = (int64_t)chunk * C;
+    if (s0 < row.n) {
+      load_tile<T, DK, C, THREADS>(q, p.q, 0, p.key, row, s0);
+      load_tile<T, DK, C, THREADS>(k, p.k, 0, p.key, row, s0);
+      load_tile<T, DV, C, THREADS>(v, p.v, 0, p.value, row, s0);
+      load_tile<T, DV, C, THREADS>(dy, p.dy, 0, p.value, row, s0);
+      constexpr int kPieces = DV * (int)sizeof(Stored<T>) / 16;
+      const char* at = static_cast<const char*>(p.kept) + (index * p.chunks + chunk) * kept_bytes(DK, DV);
+      for (int i = threadIdx.x; i < kPlanes<T> * DK * kPieces; i += THREADS) {
+        const int r = i / kPieces, piece = i % kPieces;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                         smem_of(reinterpret_cast<const char*>(s_state + r * LDS) + piece * 16)),
+                     "l"(at + (int64_t)i * 16) : "memory");
+      }
+    }
+    copies_issued();
+  };
+  const auto sums_of = [&](int chunk) { return reinterpret_cast<float2*>(decays + (chunk & 1) * C * 16); };
+  Decays<C> now, next;
+  const auto store = [&](int chunk) {
+    float2* to = sums_of(chunk);
+    next.store(to, reinterpret_cast<float*>(to + C), reinterpret_cast<float*>(to + C) + C);
+    now = next;
+  };
+  load(c1 - 1);
+  if (warp == WARPS - 1) {
+    next.load(p, row, (int64_t)(c1 - 1) * C);
+    store(c1 - 1);
+  }
+#pragma unroll 1
+  for (int chunk = c1 - 1; chunk >= c0; --chunk) {
+    const int64_t s0 = (int64_t)chunk * C;
+    copies_done();
+    __syncthreads();
+    if (warp == WARPS - 1 && chunk > c0) next.load(p, row, s0 - C);
+    const float2* sums = sums_of(chunk);
+    const float *before = reinterpret_cast<const float*>(sums + C), *after = before + C;
+    const bool live = s0 < row.n;
+    const int i0 = rg * 16 + g, i1 = i0 + 8;
+    const float2 sum0 = sums[i0], sum1 = sums[i1];
+    const int64_t t0 = row.time(s0 + i0), t1 = row.time(s0 + i1);
+    const int64_t at0 = (row.b * row.steps + t0) * p.heads + row.h, at1 = (row.b * row.steps + t1) * p.heads + row.h;
+    const bool in0 = s0 + i0 < row.steps, in1 = s0 + i1 < row.steps;
+    const bool on0 = s0 + i0 < row.n, on1 = s0 + i1 < row.n;
+    const auto put = [&](void* to, int width, int col, const float (&x)[4]) {
+      if (in0) store_pair<T>(to, at0 * width, col, width, on0 ? x[0] : 0.0f, on0 ? x[1] : 0.0f);
+      if (in1) store_pair<T>(to, at1 * width, col, width, on1 ? x[2] : 0.0f, on1 ? x[3] : 0.0f);
+    };
+    if (live) {
+      // by rows i: dQ
+      float d[C / 8][4], out[NK][4];
+#pragma unroll
+      for (int n = 0; n < C / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[n][e] = 0.0f;
+#pragma unroll
+      for (int n = 0; n < NK; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[n][e] = 0.0f;
+#pragma unroll
+      for (int kk = 0; kk < DV; kk += 16) {
+        InA<T> left;
+        load_a<T, LDV>(left, dy, rg * 16, kk);
+#pragma unroll
+        for (int n = 0; n < C / 16; ++n) {
+          if (n > rg) break;
+          InB<T> right[2];
+          load_b<T, LDV, false>(right, v, n * 16, kk);
+          mma(d[2 * n], left, right[0]);
+          mma(d[2 * n + 1], left, right[1]);
+        }
+#pragma unroll
+        for (int n = 0; n < NK / 2; ++n) {
+          MadeB<T> right[2];
+          load_state<T, LDS, PLANE, false>(right, s_state, wc * NK * 8 + n * 16, kk);
+          mma(out[2 * n], left, right[0]);
+          mma(out[2 * n + 1], left, right[1]);
+        }
+      }
+      const float b0 = before[i0] * p.scale, b1 = before[i1] * p.scale;
+      float far0 = 0.0f, far1 = 0.0f;
+#pragma unroll
+      for (int n = 0; n < NK; ++n) {
+        const int col = wc * NK * 8 + n * 8 + 2 * c;
+        out[n][0] = decayed(b0, out[n][0]), out[n][1] = decayed(b0, out[n][1]);
+        out[n][2] = decayed(b1, out[n][2]), out[n][3] = decayed(b1, out[n][3]);
+        far0 = fmaf(out[n][0], widen(q[i0 * LDK + col]), fmaf(out[n][1], widen(q[i0 * LDK + col + 1]), far0));
+        far1 = fmaf(out[n][2], widen(q[i1 * LDK + col]), fmaf(out[n][3], widen(q[i1 * LDK + col + 1]), far1));
+      }
+#pragma unroll
+      for (int off = 1; off < 4; off <<= 1) {
+        far0 += __shfl_xor_sync(0xffffffffu, far0, off);
+        far1 += __shfl_xor_sync(0xffffffffu, far1, off);
+      }
+      if (c == 0) s_far[wc * C + i0] = far0, s_far[wc * C + i1] = far1;
+#pragma unroll
+      for (int n = 0; n < C / 16; ++n) {
+        if (n > rg) break;
+        float x[8];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int j = n * 16 + half * 8 + 2 * c;
+          const float4 two = *reinterpret_cast<const float4*>(sums + j);
+          const float2 s0j = make_float2(two.x, two.y), s1j = make_float2(two.z, two.w);
+          const float(&at)[4] = d[2 * n + half];
+          x[4 * half] = j <= i0 ? at[0] * (p.scale * between(sum0, s0j)) : 0.0f;
+          x[4 * half + 1] = j + 1 <= i0 ? at[1] * (p.scale * between(sum0, s1j)) : 0.0f;
+          x[4 * half + 2] = j <= i1 ? at[2] * (p.scale * between(sum1, s0j)) : 0.0f;
+          x[4 * half + 3] = j + 1 <= i1 ? at[3] * (p.scale * between(sum1, s1j)) : 0.0f;
+        }
+        Made<T> left;
+        make(left, x);
+#pragma unroll
+        for (int m = 0; m < NK / 2; ++m) {
+          InB<T> right[2];
+          load_b<T, LDK, true>(right, k, wc * NK * 8 + m * 16, n * 16);
+          mma(out[2 * m], left, right[0]);
+          mma(out[2 * m + 1], left, right[1]);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NK; ++n) put(p.dq, p.key, wc * NK * 8 + n * 8 + 2 * c, out[n]);
+    }
+    if (live) {
+      // by rows j: dV and dK
+      float a[C / 8][4], d[C / 8][4], dv[NV][4], dk[NK][4];
+#pragma unroll
+      for (int n = 0; n < C / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[n][e] = d[n][e] = 0.0f;
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dv[n][e] = 0.0f;
+#pragma unroll
+      for (int kk = 0; kk < DK; kk += 16) {
+        InA<T> left;
+        load_a<T, LDK>(left, k, rg * 16, kk);
+#pragma unroll
+        for (int n = 0; n < C / 16; ++n) {
+          if (n < rg) continue;
+          InB<T> right[2];
+          load_b<T, LDK, false>(right, q, n * 16, kk);
+          mma(a[2 * n], left, right[0]);
+          mma(a[2 * n + 1], left, right[1]);
+        }
+#pragma unroll
+        for (int n = 0; n < NV / 2; ++n) {
+          MadeB<T> right[2];
+          load_state<T, LDS, PLANE, true>(right, s_grad, wc * NV * 8 + n * 16, kk);
+          mma(dv[2 * n], left, right[0]);
+          mma(dv[2 * n + 1], left, right[1]);
+        }
+      }
+      const float w0 = after[i0], w1 = after[i1];
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        dv[n][0] = decayed(w0, dv[n][0]), dv[n][1] = decayed(w0, dv[n][1]);
+        dv[n][2] = decayed(w1, dv[n][2]), dv[n][3] = decayed(w1, dv[n][3]);
+      }
+#pragma unroll
+      for (int n = 0; n < NK; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dk[n][e] = 0.0f;
+#pragma unroll
+      for (int kk = 0; kk < DV; kk += 16) {
+        InA<T> left;
+        load_a<T, LDV>(left, v, rg * 16, kk);
+#pragma unroll
+        for (int n = 0; n < C / 16; ++n) {
+          if (n < rg) continue;
+          InB<T> right[2];
+          load_b<T, LDV, false>(right, dy, n * 16, kk);
+          mma(d[2 * n], left, right[0]);
+          mma(d[2 * n + 1], left, right[1]);
+        }
+#pragma unroll
+        for (int n = 0; n < NK / 2; ++n) {
+          MadeB<T> right[2];
+          load_state<T, LDS, PLANE, false>(right, s_grad, wc * NK * 8 + n * 16, kk);
+          mma(dk[2 * n], left, right[0]);
+          mma(dk[2 * n + 1], left, right[1]);
+        }
+      }
+      float end0 = 0.0f, end1 = 0.0f;
+#pragma unroll
+      for (int n = 0; n < NK; ++n) {
+        const int col = wc * NK * 8 + n * 8 + 2 * c;
+        dk[n][0] = decayed(w0, dk[n][0]), dk[n][1] = decayed(w0, dk[n][1]);
+        dk[n][2] = decayed(w1, dk[n][2]), dk[n][3] = decayed(w1, dk[n][3]);
+        end0 = fmaf(dk[n][0], widen(k[i0 * LDK + col]), fmaf(dk[n][1], widen(k[i0 * LDK + col + 1]), end0));
+        end1 = fmaf(dk[n][2], widen(k[i1 * LDK + col]), fmaf(dk[n][3], widen(k[i1 * LDK + col + 1]), end1));
+      }
+      float col0 = 0.0f, col1 = 0.0f;  // sums of W over i, of j = i0 and i1
+#pragma unroll
+      for (int n = 0; n < C / 16; ++n) {
+        if (n < rg) continue;
+        float x[8], z[8];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int i = n * 16 + half * 8 + 2 * c;
+          const float4 two = *reinterpret_cast<const float4*>(sums + i);
+          const float2 s0i = make_float2(two.x, two.y), s1i = make_float2(two.z, two.w);
+          const float f0 = i0 <= i ? p.scale * between(s0i, sum0) : 0.0f, f1 = i0 <= i + 1 ? p.scale * between(s1i, sum0) : 0.0f;
+          const float f2 = i1 <= i ? p.scale * between(s0i, sum1) : 0.0f, f3 = i1 <= i + 1 ? p.scale * between(s1i, sum1) : 0.0f;
+          const float(&at)[4] = a[2 * n + half];
+          const float(&to)[4] = d[2 * n + half];
+          x[4 * half] = f0 == 0.0f ? 0.0f : at[0] * f0, x[4 * half + 1] = f1 == 0.0f ? 0.0f : at[1] * f1;
+          x[4 * half + 2] = f2 == 0.0f ? 0.0f : at[2] * f2, x[4 * half + 3] = f3 == 0.0f ? 0.0f : at[3] * f3;
+          z[4 * half] = f0 == 0.0f ? 0.0f : to[0] * f0, z[4 * half + 1] = f1 == 0.0f ? 0.0f : to[1] * f1;
+          z[4 * half + 2] = f2 == 0.0f ? 0.0f : to[2] * f2, z[4 * half + 3] = f3 == 0.0f ? 0.0f : to[3] * f3;
+          const float u0 = i == i0 ? 0.0f : x[4 * half] * to[0], u1 = i + 1 == i0 ? 0.0f : x[4 * half + 1] * to[1];
+          const float u2 = i == i1 ? 0.0f : x[4 * half + 2] * to[2], u3 = i + 1 == i1 ? 0.0f : x[4 * half + 3] * to[3];
+          if (wc == 0) {
+            col0 += u0 + u1, col1 += u2 + u3;
+            float r0 = u0 + u2, r1 = u1 + u3;
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) {
+              r0 += __shfl_xor_sync(0xffffffffu, r0, off);
+              r1 += __shfl_xor_sync(0xffffffffu, r1, off);
+            }
+            if (g == 0) s_row[rg * C + i] = r0, s_row[rg * C + i + 1] = r1;
+          }
+        }
+        Made<T> left;
+        make(left, x);
+#pragma unroll
+        for (int m = 0; m < NV / 2; ++m) {
+          InB<T> right[2];
+          load_b<T, LDV, true>(right, dy, wc * NV * 8 + m * 16, n * 16);
+          mma(dv[2 * m], left, right[0]);
+          mma(dv[2 * m + 1], left, right[1]);
+        }
+        make(left, z);
+#pragma unroll
+        for (int m = 0; m < NK / 2; ++m) {
+          InB<T> right[2];
+          load_b<T, LDK, true>(right, q, wc * NK * 8 + m * 16, n * 16);
+          mma(dk[2 * m], left, right[0]);
+          mma(dk[2 * m + 1], left, right[1]);
+        }
+      }
+#pragma unroll
+      for (int off = 1; off < 4; off <<= 1) {
+        end0 += __shfl_xor_sync(0xffffffffu, end0, off);
+        end1 += __shfl_xor_sync(0xffffffffu, end1, off);
+        col0 += __shfl_xor_sync(0xffffffffu, col0, off);
+        col1 += __shfl_xor_sync(0xffffffffu, col1, off);
+      }
+      if (c == 0) {
+        s_end[wc * C + i0] = end0, s_end[wc * C + i1] = end1;
+        if (wc == 0) s_col[i0] = col0, s_col[i1] = col1;
+      }
+#pragma unroll
+      for (int n = 0; n < NV; ++n) put(p.dv, p.value, wc * NV * 8 + n * 8 + 2 * c, dv[n]);
+#pragma unroll
+      for (int n = 0; n < NK; ++n) put(p.dk, p.key, wc * NK * 8 + n * 8 + 2 * c, dk[n]);
+      // what passes the chunk whole
+      float all = 0.0f;
+      S.each([&](int r, int col, float& x, float& y) {
+        const float2 s = read_state<T, LDS, PLANE>(s_state, r, col);
+        all = fmaf(x, s.x, fmaf(y, s.y, all));
+      });
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) all += __shfl_xor_sync(0xffffffffu, all, off);
+      if (lane == 0) s_all[warp] = decayed(before[C - 1], all);
+      S.template update<T, C>(q, dy, before, before[C - 1], p.scale);
+    } else {
+      const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int n = 0; n < NK; ++n) {
+        put(p.dq, p.key, wc * NK * 8 + n * 8 + 2 * c, zero);
+        put(p.dk, p.key, wc * NK * 8 + n * 8 + 2 * c, zero);
+      }
+#pragma unroll
+      for (int n = 0; n < NV; ++n) put(p.dv, p.value, wc * NV * 8 + n * 8 + 2 * c, zero);
+    }
+    __syncthreads();  // the chunk's tiles, states and sums are read or written
+    if (warp == WARPS - 1) {
+      // the decays' gradients: prefix sums over the chunk's steps in 64 bits
+      constexpr int E = C / 32;
+      double back = 0.0, ahead = 0.0, own_back[E], own_ahead[E], through = 0.0;
+      if (live) {
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) through += s_all[w];
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int t = lane * E + e;
+        own_back[e] = back, own_ahead[e] = ahead;  // of the steps before this one
+        if (live) {
+          float rows = 0.0f;
+#pragma unroll
+          for (int r = 0; r < RG; ++r)
+            if (r <= t / 16) rows += s_row[r * C + t];
+          back += (double)s_col[t] - (double)rows;
+#pragma unroll
+          for (int w = 0; w < WC; ++w) back += s_end[w * C + t], ahead += s_far[w * C + t];
+        }
+      }
+      double up_back = back, up_ahead = ahead;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const double x = __shfl_up_sync(0xffffffffu, up_back, off), y = __shfl_up_sync(0xffffffffu, up_ahead, off);
+        if (lane >= off) up_back += x, up_ahead += y;
+      }
+      const double all_ahead = __shfl_sync(0xffffffffu, up_ahead, 31);
+      double sum = 0.0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int64_t s = s0 + lane * E + e;
+        const double x = (up_back - back + own_back[e]) + (all_ahead - (up_ahead - ahead + own_ahead[e])) + through;
+        const bool cut = !(now.g[e] * kLog2e >= kCut) && now.g[e] == now.g[e];
+        const double out = s < row.n && !cut ? x : 0.0;
+        sum += out;
+        if (p.ddecay && s < row.steps) p.ddecay[(row.b * row.steps + row.time(s)) * p.heads + row.h] = (float)out;
+      }
+      if (p.chunk_ddecay) {
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        if (lane == 0) p.chunk_ddecay[index * p.chunks + chunk] = sum;
+      }
+      if (chunk > c0) store(chunk - 1);
+    }
+    if (live) S.template publish<T>(s_grad);
+    if (chunk > c0) load(chunk - 1);
+  }
+  if (p.dstate && part == 0) S.write(p.dstate + index * p.key * p.value, p.key, p.value, 0);
+}
+
+// ---------------------------------------------------------------------------------------- single steps
+
+// Few steps, one after the other, with the state in registers: a CTA takes a row's columns by 32, a thread four
+// adjacent columns of every 16th row.
+constexpr int kStepColumns = 32;
+template <class T, int DK>
+__global__ void __launch_bounds__(128) steps_kernel(const __grid_constant__ Args p) {
+  constexpr int kGroups = 16, kEach = DK / kGroups;
+  __shared__ float s_part[2][4][kStepColumns];
+  const int blocks = (p.value + kStepColumns - 1) / kStepColumns;
+  const int64_t index = blockIdx.x / blocks;
+  const int first = (int)(blockIdx.x - index * blocks) * kStepColumns;
+  const Row row(p, index);
+  const int group = threadIdx.x / 8, col = first + threadIdx.x % 8 * 4, warp = threadIdx.x >> 5;
+  const bool whole = p.value % 4 == 0;
+  const int64_t state = index * p.key * p.value;
+  float S[kEach][4];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int r = e * kGroups + group;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) S[e][j] = 0.0f;
+    if (p.state && r < p.key && col < p.value) {
+      const float* at = p.state + state + (int64_t)r * p.value + col;
+      if (whole && reinterpret_cast<uintptr_t>(p.state) % 16 == 0) {
+        const float4 f = *reinterpret_cast<const float4*>(at);
+        S[e][0] = f.x, S[e][1] = f.y, S[e][2] = f.z, S[e][3] = f.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (col + j < p.value) S[e][j] = at[j];
+      }
+    }
+  }
+  const T *q = static_cast<const T*>(p.q.p), *k = static_cast<const T*>(p.k.p), *v = static_cast<const T*>(p.v.p);
+  for (int64_t s = 0; s < row.steps; ++s) {
+    const int64_t t = row.time(s);
+    const bool live = s < row.n;
+    float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (live) {
+      float x[4], kk[kEach], qq[kEach];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        x[j] = col + j < p.value ? widen(v[row.b * p.v.sb + t * p.v.st + row.h * p.v.sh + col + j]) : 0.0f;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int r = e * kGroups + group;
+        kk[e] = r < p.key ? widen(k[row.b * p.k.sb + t * p.k.st + row.h * p.k.sh + r]) : 0.0f;
+        qq[e] = r < p.key ? widen(q[row.b * p.q.sb + t * p.q.st + row.h * p.q.sh + r]) : 0.0f;
+      }
+      float g = p.decay[row.b * p.decay_sb + t * p.decay_st + row.h * p.decay_sh];
+      if (p.reset && p.reset[row.b * p.reset_sb + t * p.reset_st]) g = -INFINITY;
+      const float a = g * kLog2e < kCut ? 0.0f : expf(g);
+#pragma unroll
+      for (int e = 0; e < kEach; ++e)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          S[e][j] = fmaf(kk[e], x[j], decayed(a, S[e][j]));
+          y[j] = fmaf(qq[e], S[e][j], y[j]);
+        }
+    }
+    // over the groups: those of a warp by shuffles, the warps through shared memory (two buffers in turn)
+#pragma unroll
+    for (int off = 8; off < 32; off <<= 1)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] += __shfl_xor_sync(0xffffffffu, y[j], off);
+    float(*part)[kStepColumns] = s_part[s & 1];
+    if ((threadIdx.x & 31) < 8) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) part[warp][threadIdx.x % 8 * 4 + j] = y[j];
+    }
+    __syncthreads();
+    if (threadIdx.x < kStepColumns && first + threadIdx.x < p.value) {
+      const float sum = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
+      static_cast<T*>(p.y)[((row.b * row.steps + t) * p.heads + row.h) * p.value + first + threadIdx.x] =
+          narrow<T>(live ? p.scale * sum : 0.0f);
+    }
+  }
+  if (!p.last) return;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int r = e * kGroups + group;
+    if (r >= p.key || col >= p.value) continue;
+    float* at = p.last + state + (int64_t)r * p.value + col;
+    if (whole && reinterpret_cast<uintptr_t>(p.last) % 16 == 0) {
+      *reinterpret_cast<float4*>(at) = make_float4(S[e][0], S[e][1], S[e][2], S[e][3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (col + j < p.value) at[j] = S[e][j];
+    }
+  }
+}
+
+// -------------------------------------------------------------------------------------------- launches
+
+enum Kind { kForward, kSweep, kSweepBackward, kSteps };
+
+struct Geometry {
+  int dk, dv;  // padded; dv of a CTA
+  int chunk;
+  int64_t blocks;
+};
+
+template <class T>
+cudaError_t forward_of(const Args& p, const Geometry& g, Kind kind, cudaStream_t s);
+template <class T>
+cudaError_t backward_of(const Args& p, const Geometry& g, cudaStream_t s);
+
+// Steps of a chunk.  Two tiles of 32-bit queries and values of 128 columns beside two states fill an SM's shared memory
+// at 32 steps; everything else has 64.
+constexpr int chunk_of(int dtype, int dk, int dv) { return dtype == PESQ_F32 && dk == 128 && dv == 128 ? 32 : 64; }
+
+}  // namespace lattn
+}  // namespace pesq

@@ -1,0 +1,251 @@
+// C ABI of the linear attention: checks, geometry, workspace, and the sums of the decays' gradients.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "linear_attention.cuh"
+
+using namespace pesq::lattn;
+using pesq::set_error;
+
+namespace pesq {
+namespace lattn {
+extern template cudaError_t forward_of<float>(const Args&, const Geometry&, Kind, cudaStream_t);
+extern template cudaError_t forward_of<__nv_bfloat16>(const Args&, const Geometry&, Kind, cudaStream_t);
+extern template cudaError_t forward_of<__half>(const Args&, const Geometry&, Kind, cudaStream_t);
+extern template cudaError_t backward_of<float>(const Args&, const Geometry&, cudaStream_t);
+extern template cudaError_t backward_of<__nv_bfloat16>(const Args&, const Geometry&, cudaStream_t);
+extern template cudaError_t backward_of<__half>(const Args&, const Geometry&, cudaStream_t);
+}  // namespace lattn
+}  // namespace pesq
+
+namespace {
+
+constexpr int kMaxWidth = 128;  // of keys and of values
+constexpr int kFewSteps = 8;    // that single steps take, where no backward follows
+constexpr int kJoinThreads = 256;
+
+// The decay's gradient of a head: the chunks' sums of its rows, in a fixed order
+constexpr int kSumThreads = 256;
+__global__ void __launch_bounds__(kSumThreads) decay_kernel(const double* parts, float* out, int64_t batch, int heads, int chunks) {
+  __shared__ double s[kSumThreads];
+  const int head = blockIdx.x;
+  double v = 0.0;
+  for (int64_t i = threadIdx.x; i < batch * chunks; i += kSumThreads) {
+    const int64_t b = i / chunks;
+    v += parts[(b * heads + head) * chunks + (i - b * chunks)];
+  }
+  s[threadIdx.x] = v;
+  __syncthreads();
+  for (int n = kSumThreads / 2; n > 0; n >>= 1) {
+    if (threadIdx.x < n) s[threadIdx.x] += s[threadIdx.x + n];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) out[head] = (float)s[0];
+}
+
+int64_t element(int dtype) { return dtype == PESQ_F32 ? 4 : 2; }
+int padded(int64_t n) { return n <= 32 ? 32 : n <= 64 ? 64 : 128; }
+
+int check(const pesq_linear_attention_desc* d) {
+  if (!d) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL descriptor");
+  if (d->batch < 1 || d->steps < 1 || d->heads < 1 || d->key < 1 || d->value < 1)
+    return set_error(PESQ_ERR_INVALID_ARGUMENT, "batch, steps, heads, key and value must be at least 1");
+  if (d->key > kMaxWidth || d->value > kMaxWidth)
+    return set_error(PESQ_ERR_UNSUPPORTED, "keys and values of at most 128 channels");
+  if (d->dtype < PESQ_F32 || d->dtype > PESQ_F16) return set_error(PESQ_ERR_INVALID_ARGUMENT, "unknown type");
+  if (!(d->scale - d->scale == 0.0f)) return set_error(PESQ_ERR_INVALID_ARGUMENT, "scale must be finite");
+  if (d->batch > INT32_MAX || d->heads > INT32_MAX || d->batch * d->heads > 1 << 22 || d->steps > INT32_MAX)
+    return set_error(PESQ_ERR_UNSUPPORTED, "more than 2^22 rows or 2^31 - 1 steps in a call");
+  return PESQ_OK;
+}
+
+struct Plan {
+  Geometry g;
+  int chunks, parts, part_chunks, slices;
+  int64_t rows;
+  size_t starts, factors, sums;  // bytes of the workspace's pieces
+  size_t bytes() const { return starts + factors + sums; }
+};
+
+size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+
+// Rows fill the device by themselves from about one CTA an SM; fewer are cut in parts of four chunks or more, as many as make
+// two CTAs an SM.
+Plan plan(const pesq_linear_attention_desc& d, bool backward) {
+  Plan q{};
+  q.rows = d.batch * d.heads;
+  const int dk = padded(d.key), dv = padded(d.value);
+  q.g.dk = dk;
+  q.g.dv = backward ? dv : std::min(dv, 64);
+  q.slices = dv / q.g.dv;
+  q.g.chunk = chunk_of(d.dtype, dk, dv);
+  q.chunks = (int)((d.steps + q.g.chunk - 1) / q.g.chunk);
+  const int64_t ctas = q.rows * q.slices;
+  const int64_t parts = ctas >= 148 ? 1 : std::min<int64_t>((2 * 148 + ctas - 1) / ctas, std::max(1, q.chunks / 4));
+  q.part_chunks = (int)((q.chunks + parts - 1) / parts);
+  q.parts = (q.chunks + q.part_chunks - 1) / q.part_chunks;
+  q.g.blocks = ctas * q.parts;
+  if (q.parts > 1) {
+    q.starts = round16((size_t)q.rows * q.parts * dk * dv * 4);
+    q.factors = round16((size_t)q.rows * q.parts * 4);
+  }
+  if (backward && d.decay_shared) q.sums = round16((size_t)q.rows * q.chunks * 8);
+  return q;
+}
+
+size_t kept_size(const pesq_linear_attention_desc& d) {
+  const Plan q = plan(d, false);
+  return (size_t)q.rows * q.chunks * kept_bytes(padded(d.key), padded(d.value));
+}
+
+Operand operand(const pesq_heads& s, const pesq_linear_attention_desc& d, int64_t width) {
+  Operand o{s.data, s.batch_stride, s.step_stride, s.head_stride, 0};
+  const int64_t size = element(d.dtype);
+  const int64_t all = (int64_t)reinterpret_cast<uintptr_t>(s.data) | width * size | (d.batch > 1 ? s.batch_stride * size : 0) |
+                      (d.steps > 1 ? s.step_stride * size : 0) | (d.heads > 1 ? s.head_stride * size : 0);
+  o.unit = all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2;
+  return o;
+}
+
+Args arguments(const pesq_linear_attention_desc& d, const Plan& q, void* workspace) {
+  Args a{};
+  a.q = operand(d.q, d, d.key);
+  a.k = operand(d.k, d, d.key);
+  a.v = operand(d.v, d, d.value);
+  a.decay = d.log_decay;
+  a.decay_sb = d.decay_shared ? 0 : d.decay_batch_stride;
+  a.decay_st = d.decay_shared ? 0 : d.decay_step_stride;
+  a.decay_sh = d.decay_head_stride;
+  a.reset = d.reset;
+  a.reset_sb = d.reset_batch_stride;
+  a.reset_st = d.reset_step_stride;
+  a.lengths = d.lengths;
+  a.state = d.state;
+  a.steps = d.steps;
+  a.heads = (int)d.heads;
+  a.key = (int)d.key;
+  a.value = (int)d.value;
+  a.reverse = d.reverse != 0;
+  a.scale = d.scale;
+  a.chunks = q.chunks;
+  a.parts = q.parts;
+  a.part_chunks = q.part_chunks;
+  a.slices = q.slices;
+  char* ws = static_cast<char*>(workspace);
+  a.starts = reinterpret_cast<float*>(ws);
+  a.factors = reinterpret_cast<float*>(ws + q.starts);
+  a.chunk_ddecay = q.sums ? reinterpret_cast<double*>(ws + q.starts + q.factors) : nullptr;
+  return a;
+}
+
+cudaError_t forward(const Args& a, const Geometry& g, int dtype, Kind kind, cudaStream_t s) {
+  return dtype == PESQ_F32    ? forward_of<float>(a, g, kind, s)
+         : dtype == PESQ_BF16 ? forward_of<__nv_bfloat16>(a, g, kind, s)
+                              : forward_of<__half>(a, g, kind, s);
+}
+
+// the states that the parts begin from
+cudaError_t sweep(Args a, const Plan& q, int dtype, bool backward, cudaStream_t s) {
+  Geometry g = q.g;
+  const int dv = q.g.dv * q.slices;
+  g.dv = std::min(dv, 64);
+  a.slices = dv / g.dv;
+  g.blocks = q.rows * q.parts * a.slices;
+  cudaError_t e = forward(a, g, dtype, backward ? kSweepBackward : kSweep, s);
+  if (e != cudaSuccess) return e;
+  const int64_t per = ((int64_t)g.dk * dv + kJoinThreads - 1) / kJoinThreads;
+  join_kernel<kJoinThreads><<<(unsigned)(q.rows * per), kJoinThreads, 0, s>>>(a, g.dk, dv, backward);
+  return cudaGetLastError();
+}
+
+int check_operands(const pesq_linear_attention_desc* d) {
+  if (!d->q.data || !d->k.data || !d->v.data || !d->log_decay) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL operand");
+  const uintptr_t all = reinterpret_cast<uintptr_t>(d->q.data) | reinterpret_cast<uintptr_t>(d->k.data) |
+                        reinterpret_cast<uintptr_t>(d->v.data);
+  if (all % element(d->dtype)) return set_error(PESQ_ERR_INVALID_ARGUMENT, "an operand that is not aligned to its type");
+  return PESQ_OK;
+}
+int check_workspace(const void* workspace, size_t bytes, size_t need) {
+  if (need && (!workspace || bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
+    return set_error(PESQ_ERR_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
+  return PESQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int pesq_linear_attention_sizes(const pesq_linear_attention_desc* d, size_t* forward, size_t* kept, size_t* backward) {
+  if (!forward || !kept || !backward) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL argument");
+  if (const int status = check(d)) return status;
+  *forward = plan(*d, false).bytes();
+  *kept = kept_size(*d);
+  *backward = plan(*d, true).bytes();
+  return PESQ_OK;
+}
+
+int pesq_linear_attention_forward(const pesq_linear_attention_desc* d, void* stream, void* y, float* last, void* kept,
+                                  size_t kept_bytes, void* workspace, size_t workspace_bytes) {
+  if (const int status = check(d)) return status;
+  if (const int status = check_operands(d)) return status;
+  if (!y) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL result");
+  if (reinterpret_cast<uintptr_t>(y) % 4) return set_error(PESQ_ERR_INVALID_ARGUMENT, "a result that is not 4-byte aligned");
+  if (kept && (kept_bytes < kept_size(*d) || reinterpret_cast<uintptr_t>(kept) % 16))
+    return set_error(PESQ_ERR_WORKSPACE, "room for the kept states too small or not 16-byte aligned");
+  Plan q = plan(*d, false);
+  if (const int status = check_workspace(workspace, workspace_bytes, q.bytes())) return status;
+  Args a = arguments(*d, q, workspace);
+  a.y = y;
+  a.last = last;
+  a.kept = kept;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaSuccess;
+  if (!kept && d->steps <= kFewSteps) {
+    Geometry g = q.g;
+    g.blocks = q.rows * ((d->value + kStepColumns - 1) / kStepColumns);
+    e = forward(a, g, d->dtype, kSteps, s);
+  } else {
+    if (q.parts > 1) e = sweep(a, q, d->dtype, false, s);
+    if (e == cudaSuccess) e = forward(a, q.g, d->dtype, kForward, s);
+  }
+  return e == cudaSuccess ? PESQ_OK : set_error(PESQ_ERR_CUDA, cudaGetErrorString(e));
+}
+
+int pesq_linear_attention_backward(const pesq_linear_attention_desc* d, void* stream, const void* kept, size_t kept_bytes,
+                                   pesq_heads dy, const float* dlast, void* dq, void* dk, void* dv, float* ddecay,
+                                   float* dstate, void* workspace, size_t workspace_bytes) {
+  if (const int status = check(d)) return status;
+  if (const int status = check_operands(d)) return status;
+  if (!dy.data || !dq || !dk || !dv || !ddecay) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL operand");
+  if (reinterpret_cast<uintptr_t>(dy.data) % element(d->dtype))
+    return set_error(PESQ_ERR_INVALID_ARGUMENT, "an operand that is not aligned to its type");
+  if ((reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv)) % 4)
+    return set_error(PESQ_ERR_INVALID_ARGUMENT, "a result that is not 4-byte aligned");
+  if (!kept || kept_bytes < kept_size(*d) || reinterpret_cast<uintptr_t>(kept) % 16)
+    return set_error(PESQ_ERR_WORKSPACE, "kept states missing, too small or not 16-byte aligned");
+  Plan q = plan(*d, true);
+  if (const int status = check_workspace(workspace, workspace_bytes, q.bytes())) return status;
+  Args a = arguments(*d, q, workspace);
+  a.dy = operand(dy, *d, d->value);
+  a.kept = const_cast<void*>(kept);
+  a.dq = dq;
+  a.dk = dk;
+  a.dv = dv;
+  a.ddecay = d->decay_shared ? nullptr : ddecay;
+  a.dlast = dlast;
+  a.dstate = dstate;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = q.parts > 1 ? sweep(a, q, d->dtype, true, s) : cudaSuccess;
+  if (e == cudaSuccess)
+    e = d->dtype == PESQ_F32    ? backward_of<float>(a, q.g, s)
+        : d->dtype == PESQ_BF16 ? backward_of<__nv_bfloat16>(a, q.g, s)
+                                : backward_of<__half>(a, q.g, s);
+  if (e == cudaSuccess && d->decay_shared) {
+    decay_kernel<<<(unsigned)d->heads, kSumThreads, 0, s>>>(a.chunk_ddecay, ddecay, d->batch, (int)d->heads, q.chunks);
+    e = cudaGetLastError();
+  }
+  return e == cudaSuccess ? PESQ_OK : set_error(PESQ_ERR_CUDA, cudaGetErrorString(e));
+}
+
+}  // extern "C"

@@ -1,0 +1,65 @@
+// Instantiation of the linear attention's kernels for one type (the forward and the backward of each in a translation
+// unit of its own, so that they compile in parallel).
+#pragma once
+
+#include "linear_attention.cuh"
+
+namespace pesq {
+namespace lattn {
+
+template <class K>
+cudaError_t start(K kernel, const Args& p, int64_t grid, int threads, int smem, cudaStream_t s) {
+  if (smem > 48 << 10) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+  }
+  kernel<<<(unsigned)grid, threads, smem, s>>>(p);
+  return cudaGetLastError();
+}
+
+template <class T, int DK, int DV, int C>
+cudaError_t launch_forward(const Args& p, const Geometry& g, Kind kind, cudaStream_t s) {
+  switch (kind) {
+    case kForward: return start(forward_kernel<T, DK, DV, C>, p, g.blocks, 128, ForwardShared<T, DK, DV, C>::kBytes, s);
+    case kSweep: return start(sweep_kernel<T, DK, DV, C, false>, p, g.blocks, 128, SweepShared<T, DK, DV, C>::kBytes, s);
+    default: return start(sweep_kernel<T, DK, DV, C, true>, p, g.blocks, 128, SweepShared<T, DK, DV, C>::kBytes, s);
+  }
+}
+
+template <class T, int DK>
+cudaError_t forward_width(const Args& p, const Geometry& g, Kind kind, cudaStream_t s) {
+  if (kind == kSteps) return start(steps_kernel<T, DK>, p, g.blocks, 128, 0, s);
+  if constexpr (std::is_same<T, float>::value && DK == 128) {
+    if (g.chunk == 32) return launch_forward<T, DK, 64, 32>(p, g, kind, s);
+  }
+  return g.dv == 32 ? launch_forward<T, DK, 32, 64>(p, g, kind, s) : launch_forward<T, DK, 64, 64>(p, g, kind, s);
+}
+
+// the forward, the sweeps of both directions and single steps
+template <class T>
+cudaError_t forward_of(const Args& p, const Geometry& g, Kind kind, cudaStream_t s) {
+  return g.dk == 32   ? forward_width<T, 32>(p, g, kind, s)
+         : g.dk == 64 ? forward_width<T, 64>(p, g, kind, s)
+                      : forward_width<T, 128>(p, g, kind, s);
+}
+
+template <class T, int DK, int DV>
+cudaError_t launch_backward(const Args& p, const Geometry& g, cudaStream_t s) {
+  constexpr int dtype = std::is_same<T, float>::value ? PESQ_F32 : PESQ_BF16, C = chunk_of(dtype, DK, DV);
+  return start(backward_kernel<T, DK, DV, C>, p, g.blocks, 32 * kBackWarps<T, DK, DV>, BackwardShared<T, DK, DV, C>::kBytes, s);
+}
+template <class T, int DK>
+cudaError_t backward_width(const Args& p, const Geometry& g, cudaStream_t s) {
+  return g.dv == 32   ? launch_backward<T, DK, 32>(p, g, s)
+         : g.dv == 64 ? launch_backward<T, DK, 64>(p, g, s)
+                      : launch_backward<T, DK, 128>(p, g, s);
+}
+template <class T>
+cudaError_t backward_of(const Args& p, const Geometry& g, cudaStream_t s) {
+  return g.dk == 32   ? backward_width<T, 32>(p, g, s)
+         : g.dk == 64 ? backward_width<T, 64>(p, g, s)
+                      : backward_width<T, 128>(p, g, s);
+}
+
+}  // namespace lattn
+}  // namespace pesq

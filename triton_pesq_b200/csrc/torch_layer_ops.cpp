@@ -1,4 +1,4 @@
-// torch custom ops of the layer norm over the C ABI of
+// torch custom ops of the layer norm and the linear attention over the C ABI of
 // libpesq_cuda.so, with their autograd nodes: as in torch_train_ops.cpp, the op that
 // a caller uses, and the forward and backward it is made of.
 #include <algorithm>
@@ -159,7 +159,228 @@ at::Tensor layer_norm(const at::Tensor& x_, const at::Tensor& weight_, const Opt
   return y.sizes() == x_.sizes() ? y : y.view(x_.sizes());
 }
 
+// ------------------------------------------------------------ linear attention
+
+constexpr const char* kAttention = "linear attention";
+
+struct AttentionCall {
+  at::Tensor q, k, v, decay, state, reset, lengths;
+  pesq_linear_attention_desc d{};
+
+  AttentionCall(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_, const at::Tensor& decay_,
+                const OptTensor& state_, const OptTensor& reset_, const OptTensor& lengths_, bool reverse, double scale) {
+    check_cuda(q_, q_, kAttention, "q");
+    d.dtype = dtype_code(q_, kAttention, "q");
+    TORCH_CHECK(q_.dim() == 4, "The CUDA linear attention needs `q` [batch, step, head, key], got ", q_.sizes(), ".");
+    check_cuda(k_, q_, kAttention, "k");
+    check_cuda(v_, q_, kAttention, "v");
+    check_cuda(decay_, q_, kAttention, "log_decay");
+    check_shape(k_, q_.sizes(), kAttention, "k");
+    TORCH_CHECK_VALUE(v_.dim() == 4 && v_.sizes().slice(0, 3) == q_.sizes().slice(0, 3),
+                      "The CUDA linear attention needs `v` [batch, step, head, value] beside `q` of shape ", q_.sizes(), ", got ",
+                      v_.sizes(), ".");
+    TORCH_CHECK(k_.scalar_type() == q_.scalar_type() && v_.scalar_type() == q_.scalar_type(),
+                "The CUDA linear attention needs `q`, `k` and `v` in one type, got ", q_.scalar_type(), ", ",
+                k_.scalar_type(), " and ", v_.scalar_type(), ".");
+    check_float(decay_, kAttention, "log_decay");
+    TORCH_CHECK_VALUE(scale - scale == 0.0, "The CUDA linear attention needs a finite `scale`, got ", scale, ".");
+    q = rows(q_);
+    k = rows(k_);
+    v = rows(v_);
+    decay = decay_;
+    d.batch = q.size(0);
+    d.steps = q.size(1);
+    d.heads = q.size(2);
+    d.key = q.size(3);
+    d.value = v.size(3);
+    d.decay_shared = decay.dim() == 1;
+    if (d.decay_shared) {
+      check_shape(decay, {d.heads}, kAttention, "log_decay");
+      d.decay_head_stride = decay.stride(0);
+    } else {
+      const int64_t want[3] = {d.batch, d.steps, d.heads};
+      check_shape(decay, want, kAttention, "log_decay");
+      d.decay_batch_stride = decay.stride(0);
+      d.decay_step_stride = decay.stride(1);
+      d.decay_head_stride = decay.stride(2);
+    }
+    d.log_decay = decay.data_ptr<float>();
+    if (given(state_)) {
+      check_cuda(*state_, q_, kAttention, "state");
+      check_float(*state_, kAttention, "state");
+      const int64_t want[4] = {d.batch, d.heads, d.key, d.value};
+      check_shape(*state_, want, kAttention, "state");
+      state = state_->contiguous();
+      d.state = state.data_ptr<float>();
+    }
+    if (given(reset_)) {
+      check_cuda(*reset_, q_, kAttention, "reset");
+      check_shape(*reset_, {d.batch, d.steps}, kAttention, "reset");
+      TORCH_CHECK(reset_->scalar_type() == at::kBool, "The CUDA linear attention needs `reset` in bool, it is ",
+                  reset_->scalar_type(), ".");
+      reset = *reset_;
+      d.reset = static_cast<const uint8_t*>(reset.data_ptr());
+      d.reset_batch_stride = reset.stride(0);
+      d.reset_step_stride = reset.stride(1);
+    }
+    if (given(lengths_)) {
+      check_cuda(*lengths_, q_, kAttention, "lengths");
+      check_shape(*lengths_, {d.batch}, kAttention, "lengths");
+      TORCH_CHECK(lengths_->scalar_type() == at::kLong || lengths_->scalar_type() == at::kInt,
+                  "The CUDA linear attention needs `lengths` in int64 or int32, it is ", lengths_->scalar_type(), ".");
+      lengths = lengths_->to(at::kLong).contiguous();
+      d.lengths = lengths.data_ptr<int64_t>();
+    }
+    d.reverse = reverse;
+    d.scale = static_cast<float>(scale);
+    d.q = heads_of(q);
+    d.k = heads_of(k);
+    d.v = heads_of(v);
+  }
+
+  bool empty() const { return q.numel() == 0 || v.numel() == 0; }
+  at::Tensor matrix() const { return at::empty({d.batch, d.heads, d.key, d.value}, q.options().dtype(at::kFloat)); }
+};
+
+// (y, last, the states kept for the backward where `keep`)
+std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_attention_forward(const at::Tensor& q, const at::Tensor& k,
+                                                                        const at::Tensor& v, const at::Tensor& decay,
+                                                                        const OptTensor& state, const OptTensor& reset,
+                                                                        const OptTensor& lengths, bool reverse, double scale,
+                                                                        bool keep) {
+  AttentionCall c(q, k, v, decay, state, reset, lengths, reverse, scale);
+  c10::cuda::CUDAGuard guard(q.device());
+  const auto bytes = q.options().dtype(at::kByte);
+  at::Tensor y = at::empty(v.sizes(), v.options()), last = c.matrix();
+  if (c.empty()) {
+    y.zero_();  // (no keys: nothing is ever in the state)
+    if (c.d.state) {
+      last.copy_(c.state);
+    } else {
+      last.zero_();
+    }
+    return {y, last, at::empty({0}, bytes)};
+  }
+  size_t work = 0, kept = 0, back = 0;
+  check_status(pesq_linear_attention_sizes(&c.d, &work, &kept, &back), "pesq_linear_attention_sizes");
+  at::Tensor states = at::empty({keep ? static_cast<int64_t>(kept) : 0}, bytes), ws;
+  if (work) ws = at::empty({static_cast<int64_t>(work)}, bytes);
+  check_status(pesq_linear_attention_forward(&c.d, at::cuda::getCurrentCUDAStream(), y.data_ptr(), last.data_ptr<float>(),
+                                             keep ? states.data_ptr() : nullptr, keep ? kept : 0,
+                                             work ? ws.data_ptr() : nullptr, work),
+               "pesq_linear_attention_forward");
+  return {y, last, states};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> linear_attention_backward(
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& decay, const OptTensor& state,
+    const OptTensor& reset, const OptTensor& lengths, bool reverse, double scale, const at::Tensor& kept_,
+    const OptTensor& dy_, const OptTensor& dlast_) {
+  AttentionCall c(q, k, v, decay, state, reset, lengths, reverse, scale);
+  c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(q.sizes(), q.options()),
+             dv = at::empty(v.sizes(), v.options()), ddecay = at::empty(decay.sizes(), decay.options()), dstate = c.matrix();
+  at::Tensor dlast, dy;
+  if (given(dy_)) check_gradient(*dy_, q, v.sizes(), kAttention, "dy");
+  if (given(dlast_)) {
+    check_gradient(*dlast_, q, dstate.sizes(), kAttention, "dlast");
+    dlast = dlast_->to(at::kFloat).contiguous();
+  }
+  if (c.empty()) {
+    for (at::Tensor* t : {&dq, &dk, &dv, &ddecay}) t->zero_();
+    if (dlast.defined()) {
+      dstate.copy_(dlast);
+    } else {
+      dstate.zero_();
+    }
+    return {dq, dk, dv, ddecay, dstate};
+  }
+  dy = given(dy_) ? rows(dy_->to(q.scalar_type())) : at::zeros({1}, q.options()).expand(v.sizes());
+  if (dy.stride(3) != 1 && dy.size(3) > 1) dy = dy.contiguous();
+  size_t work = 0, kept = 0, back = 0;
+  check_status(pesq_linear_attention_sizes(&c.d, &work, &kept, &back), "pesq_linear_attention_sizes");
+  check_cuda(kept_, q, kAttention, "kept");
+  TORCH_CHECK(kept_.scalar_type() == at::kByte && kept_.is_contiguous() && kept_.numel() == static_cast<int64_t>(kept),
+              "The CUDA linear attention needs the states that its forward kept.");
+  at::Tensor ws;
+  if (back) ws = at::empty({static_cast<int64_t>(back)}, q.options().dtype(at::kByte));
+  check_status(pesq_linear_attention_backward(&c.d, at::cuda::getCurrentCUDAStream(), kept_.data_ptr(), kept, heads_of(dy),
+                                              dlast.defined() ? dlast.data_ptr<float>() : nullptr, dq.data_ptr(),
+                                              dk.data_ptr(), dv.data_ptr(), ddecay.data_ptr<float>(),
+                                              dstate.data_ptr<float>(), back ? ws.data_ptr() : nullptr, back),
+               "pesq_linear_attention_backward");
+  return {dq, dk, dv, ddecay, dstate};
+}
+
+const auto& attention_forward_op() {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("pesq_cuda::linear_attention_forward", "")
+                       .typed<decltype(linear_attention_forward)>();
+  return op;
+}
+const auto& attention_backward_op() {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("pesq_cuda::linear_attention_backward", "")
+                       .typed<decltype(linear_attention_backward)>();
+  return op;
+}
+
+struct LinearAttention : public torch::autograd::Function<LinearAttention> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                               const at::Tensor& decay, const OptTensor& state, const OptTensor& reset,
+                               const OptTensor& lengths, bool reverse, double scale) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [y, last, kept] = attention_forward_op().call(q, k, v, decay, state, reset, lengths, reverse, scale, true);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({q, k, v, decay, state.value_or(at::Tensor()), reset.value_or(at::Tensor()),
+                            lengths.value_or(at::Tensor()), kept});
+    ctx->saved_data["reverse"] = reverse;
+    ctx->saved_data["scale"] = scale;
+    return {y, last};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    no_second_derivative(kAttention);
+    const auto s = ctx->get_saved_variables();
+    variable_list out(9);
+    if (!g[0].defined() && !g[1].defined()) return out;
+    auto [dq, dk, dv, ddecay, dstate] = attention_backward_op().call(
+        s[0], s[1], s[2], s[3], optional_of(s[4]), optional_of(s[5]), optional_of(s[6]),
+        ctx->saved_data["reverse"].toBool(), ctx->saved_data["scale"].toDouble(), s[7], optional_of(g[0]), optional_of(g[1]));
+    out[0] = dq;
+    out[1] = dk;
+    out[2] = dv;
+    out[3] = ddecay;
+    if (s[4].defined()) out[4] = dstate;
+    return out;
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> linear_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                    const at::Tensor& decay, const OptTensor& state, const OptTensor& reset,
+                                                    const OptTensor& lengths, bool reverse, double scale) {
+  check_cuda(q, q, kAttention, "q");
+  no_forward_mode(kAttention, q, k, v, decay, state);
+  if (at::GradMode::is_enabled() &&
+      (wants_grad(q) || wants_grad(k) || wants_grad(v) || wants_grad(decay) || wants_grad(state))) {
+    auto out = LinearAttention::apply(q, k, v, decay, state, reset, lengths, reverse, scale);
+    return {out[0], out[1]};
+  }
+  auto [y, last, kept] = attention_forward_op().call(q, k, v, decay, state, reset, lengths, reverse, scale, false);
+  return {y, last};
+}
+
 }  // namespace
+
+TORCH_LIBRARY_FRAGMENT(pesq_cuda, m) {
+  const char* in = "(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? state, Tensor? reset, Tensor? lengths, "
+                   "bool reverse, float scale";
+  m.def((std::string("linear_attention") + in + ") -> (Tensor, Tensor)").c_str());
+  m.def((std::string("linear_attention_forward") + in + ", bool keep) -> (Tensor, Tensor, Tensor)").c_str());
+  m.def((std::string("linear_attention_backward") + in +
+         ", Tensor kept, Tensor? dy, Tensor? dlast) -> (Tensor, Tensor, Tensor, Tensor, Tensor)")
+            .c_str());
+}
 
 TORCH_LIBRARY_FRAGMENT(pesq_cuda, m) {
   m.def("layer_norm(Tensor x, Tensor weight, Tensor? bias, float eps, int dtype) -> Tensor");
@@ -170,9 +391,12 @@ TORCH_LIBRARY_FRAGMENT(pesq_cuda, m) {
 
 TORCH_LIBRARY_IMPL(pesq_cuda, CompositeImplicitAutograd, m) {
   m.impl("layer_norm", &layer_norm);
+  m.impl("linear_attention", &linear_attention);
 }
 
 TORCH_LIBRARY_IMPL(pesq_cuda, CUDA, m) {
   m.impl("layer_norm_forward", &layer_norm_forward);
   m.impl("layer_norm_backward", &layer_norm_backward);
+  m.impl("linear_attention_forward", &linear_attention_forward);
+  m.impl("linear_attention_backward", &linear_attention_backward);
 }
