@@ -522,6 +522,53 @@ int pesq_linear_attention_backward(const pesq_linear_attention_desc* desc, void*
                                    size_t kept_bytes, pesq_heads dy, const float* dlast, void* dq, void* dk, void* dv,
                                    float* ddecay, float* dstate, void* workspace, size_t workspace_bytes);
 
+/* Orthogonalised updates (Muon): of a matrix p with gradient g,
+ *   m = momentum m + (1 - momentum) g,  U = momentum m + (1 - momentum) g (nesterov) or m
+ *   X = U / max(|U|, eps);  `steps` times  X = a X + (b A + c A A) X,  A = X X^T (on the shorter side)
+ *   p = p (1 - lr weight_decay) - lr adjust X
+ * over all matrices together (csrc/muon.cu). */
+#define PESQ_MUON_ORIGINAL 0  /* adjust = sqrt(max(1, rows / cols)) */
+#define PESQ_MUON_MATCH_RMS 1 /* adjust = 0.2 sqrt(max(rows, cols)): the root mean square of an AdamW step */
+typedef struct pesq_muon_tensor {
+  float* param;      /* [rows, cols] */
+  const void* grad;  /* [rows, cols], of grad_dtype; NULL leaves the matrix and its momentum as they are */
+  float* momentum;   /* [rows, cols] */
+  void* copy;        /* [rows, cols], the new values in the gradients' 16-bit type; or NULL */
+  int64_t rows, cols; /* 1 .. 32768 */
+} pesq_muon_tensor;
+
+typedef struct pesq_muon_desc {
+  int32_t grad_dtype; /* PESQ_F32, PESQ_BF16 or PESQ_F16 */
+  int32_t nesterov;
+  int32_t adjust;
+  int32_t steps;      /* 1 .. 100 */
+  double momentum;
+  float lr, weight_decay;
+  float eps;          /* above 0 */
+  float a, b, c;      /* -16 .. 16 */
+  const float* grad_scale; /* device, times every gradient; the step is skipped where it is not finite; NULL: 1 */
+} pesq_muon_desc;
+
+/* Bytes of a step's workspace. */
+int pesq_muon_workspace(const pesq_muon_desc* desc, const pesq_muon_tensor* tensors, int64_t count, size_t* bytes);
+int pesq_muon_step(const pesq_muon_desc* desc, const pesq_muon_tensor* tensors, int64_t count, void* stream,
+                   void* workspace, size_t workspace_bytes);
+
+/* The iteration alone, of `count` dense matrices. */
+typedef struct pesq_orthogonalize_desc {
+  int64_t count, rows, cols; /* rows, cols: 1 .. 32768 */
+  int32_t dtype;             /* of x and out */
+  int32_t steps;
+  float eps, a, b, c;
+} pesq_orthogonalize_desc;
+int pesq_orthogonalize_workspace(const pesq_orthogonalize_desc* desc, size_t* bytes);
+int pesq_orthogonalize(const pesq_orthogonalize_desc* desc, void* stream, const void* x, void* out, void* workspace,
+                       size_t workspace_bytes);
+/* Synchronises `stream`, then reads and clears the current device's error
+ * word: nonzero when a bounded wait of an earlier call ran out (that call's results
+ * are then wrong). */
+int pesq_muon_check(void* stream, uint32_t* failed);
+
 #ifdef __cplusplus
 }
 #endif

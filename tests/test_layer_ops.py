@@ -5,7 +5,8 @@ import ctypes
 import pytest
 import torch
 
-from triton_pesq_b200 import LayerNormCuda, LinearAttentionCuda, _lib, layer_norm, linear_attention
+from triton_pesq_b200 import (LayerNormCuda, LinearAttentionCuda, MuonCuda, _lib, layer_norm, linear_attention, muon_step,
+                              orthogonalize)
 
 
 def test_layer_norm_without_a_gpu():
@@ -111,3 +112,58 @@ def test_linear_attention_entry_checks_its_descriptor():
     assert backward(make(**full), dy=none) == 1 and backward(make(**full), dq=None) == 1 and backward(make(**full), dq=odd) == 1
     assert backward(make(**full), kept=None) == 3 and backward(make(**full), kept_bytes=64) == 3
     assert backward(make(decay_shared=1, **full), ws=None) == 3
+
+
+def test_muon_without_a_gpu():
+    p = torch.nn.Parameter(torch.ones(4, 4))
+    p.grad = torch.ones(4, 4)
+    with pytest.raises(RuntimeError, match="GPU"):
+        MuonCuda([p]).step()
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        orthogonalize(p)
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        muon_step([p.detach()], [p.grad], [torch.zeros(4, 4)])
+    for kw in ({"lr": -1.0}, {"momentum": 1.0}, {"weight_decay": -0.1}, {"coefficients": (1.0, 2.0)}, {"coefficients": (20.0, 0.0, 0.0)},
+               {"eps": 0.0}, {"eps": float("inf")}, {"steps": 0}, {"steps": 101}, {"adjust": "x"}):
+        with pytest.raises(ValueError):
+            MuonCuda([torch.nn.Parameter(torch.ones(2, 2))], **kw)
+    for bad in (torch.ones(3), torch.ones(2, 2, 2), torch.ones(0, 3), torch.ones(2, 3).T, torch.ones(2, 2).double()):
+        with pytest.raises(RuntimeError):
+            MuonCuda([torch.nn.Parameter(bad)])
+    good = MuonCuda([p])
+    with pytest.raises(ValueError, match="momentum"):
+        good.load_state_dict({**good.state_dict(), "state": {0: {"momentum": torch.zeros(4, 4), "master": torch.zeros(4, 4)}}})
+
+
+def test_muon_entry_checks_its_descriptor():
+    lib = _lib.library()
+    size = ctypes.c_size_t()
+
+    def workspace(count=1, rows=100, cols=200, param=16, grad=16, momentum=16, copy=None, **kw):
+        d = _lib.MuonDesc(grad_dtype=_lib.F32, nesterov=1, adjust=0, steps=5, momentum=0.95, lr=0.02, weight_decay=0.1, eps=1e-7, a=3.4,
+                          b=-4.8, c=2.0)
+        for k, v in kw.items():
+            setattr(d, {"beta": "momentum"}.get(k, k), v)
+        t = (_lib.MuonTensor * 1)(_lib.MuonTensor(param=param, grad=grad, momentum=momentum, copy=copy, rows=rows, cols=cols))
+        return lib.pesq_muon_workspace(ctypes.byref(d), t, count, ctypes.byref(size)), d, t
+
+    assert workspace()[0] == _lib.PESQ_OK
+    # X before and after a step, A and the polynomial, in tiles of 128, 4 bytes a value; and a norm's sums
+    assert size.value == (2 * 128 * 256 + 2 * 128 * 128) * 4 + 8 * -(-100 * 200 // 8192)
+    for bad in ({"count": -1}, {"rows": 0}, {"cols": 0}, {"param": None}, {"momentum": None}, {"copy": 16}, {"grad_dtype": 3},
+                {"steps": 0}, {"steps": 101}, {"adjust": 2}, {"beta": 1.0}, {"beta": float("nan")}, {"lr": -1.0},
+                {"weight_decay": float("nan")}, {"eps": 0.0}, {"eps": float("inf")}, {"a": 17.0}, {"b": float("nan")}):
+        assert workspace(**bad)[0] == 1, bad
+    assert workspace(rows=32769)[0] == 2 and workspace(cols=1 << 40)[0] == 2
+    assert workspace(grad=None, param=None)[0] == _lib.PESQ_OK and size.value == 0
+    _, d, t = workspace()
+    assert lib.pesq_muon_workspace(ctypes.byref(d), t, 1, None) == 1
+    assert lib.pesq_muon_step(ctypes.byref(d), t, 1, None, None, 0) == _lib.PESQ_ERR_WORKSPACE
+    assert lib.pesq_muon_step(ctypes.byref(d), t, 1, None, ctypes.c_void_p(8), 1 << 40) == _lib.PESQ_ERR_WORKSPACE
+    assert lib.pesq_muon_step(None, None, 0, None, None, 0) == 1
+    o = _lib.OrthogonalizeDesc(count=2, rows=100, cols=200, dtype=_lib.BF16, steps=5, eps=1e-7, a=3.4, b=-4.8, c=2.0)
+    assert lib.pesq_orthogonalize_workspace(ctypes.byref(o), ctypes.byref(size)) == _lib.PESQ_OK
+    assert lib.pesq_orthogonalize(ctypes.byref(o), None, None, ctypes.c_void_p(16), ctypes.c_void_p(16), 1 << 40) == 1
+    assert lib.pesq_orthogonalize(ctypes.byref(o), None, ctypes.c_void_p(16), ctypes.c_void_p(16), ctypes.c_void_p(16), 100) == 3
+    o.count = 0
+    assert lib.pesq_orthogonalize_workspace(ctypes.byref(o), ctypes.byref(size)) == 1

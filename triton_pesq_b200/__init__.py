@@ -20,9 +20,10 @@ from .iir import IIRCuda
 from .layer_norm import LayerNormCuda, layer_norm
 from .linear_attention import LinearAttentionCuda, linear_attention
 from .loss import PesqLossCuda
+from .muon import MuonCuda, muon_step, orthogonalize
 from .norm_join import NormJoinCuda, norm_join, pre_norm
 from .resample import ResampleCuda
 
 __all__ = ["PesqLossCuda", "ResampleCuda", "IIRCuda", "GatedScanCuda", "gated_scan", "NormJoinCuda",
            "norm_join", "pre_norm", "AdamWCuda", "adamw_step", "LayerNormCuda", "layer_norm",
-           "LinearAttentionCuda", "linear_attention"]
+           "LinearAttentionCuda", "linear_attention", "MuonCuda", "muon_step", "orthogonalize"]

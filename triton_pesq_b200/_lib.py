@@ -225,6 +225,48 @@ class LinearAttentionDesc(ctypes.Structure):
     ]
 
 
+class MuonTensor(ctypes.Structure):
+    _fields_ = [
+        ("param", ctypes.c_void_p),
+        ("grad", ctypes.c_void_p),
+        ("momentum", ctypes.c_void_p),
+        ("copy", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+        ("cols", ctypes.c_int64),
+    ]
+
+
+class MuonDesc(ctypes.Structure):
+    _fields_ = [
+        ("grad_dtype", ctypes.c_int32),
+        ("nesterov", ctypes.c_int32),
+        ("adjust", ctypes.c_int32),
+        ("steps", ctypes.c_int32),
+        ("momentum", ctypes.c_double),
+        ("lr", ctypes.c_float),
+        ("weight_decay", ctypes.c_float),
+        ("eps", ctypes.c_float),
+        ("a", ctypes.c_float),
+        ("b", ctypes.c_float),
+        ("c", ctypes.c_float),
+        ("grad_scale", ctypes.c_void_p),
+    ]
+
+
+class OrthogonalizeDesc(ctypes.Structure):
+    _fields_ = [
+        ("count", ctypes.c_int64),
+        ("rows", ctypes.c_int64),
+        ("cols", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("steps", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("a", ctypes.c_float),
+        ("b", ctypes.c_float),
+        ("c", ctypes.c_float),
+    ]
+
+
 class AdamwTensor(ctypes.Structure):
     _fields_ = [
         ("param", ctypes.c_void_p),
@@ -394,6 +436,22 @@ SIGNATURES = {
          ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
          ctypes.c_size_t],
     ),
+    "pesq_muon_workspace": (
+        ctypes.c_int,
+        [ctypes.POINTER(MuonDesc), ctypes.POINTER(MuonTensor), ctypes.c_int64, ctypes.POINTER(ctypes.c_size_t)],
+    ),
+    "pesq_muon_step": (
+        ctypes.c_int,
+        [ctypes.POINTER(MuonDesc), ctypes.POINTER(MuonTensor), ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
+         ctypes.c_size_t],
+    ),
+    "pesq_orthogonalize_workspace": (ctypes.c_int, [ctypes.POINTER(OrthogonalizeDesc), ctypes.POINTER(ctypes.c_size_t)]),
+    "pesq_orthogonalize": (
+        ctypes.c_int,
+        [ctypes.POINTER(OrthogonalizeDesc), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+         ctypes.c_size_t],
+    ),
+    "pesq_muon_check": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint32)]),
     "pesq_adamw_step": (
         ctypes.c_int,
         [ctypes.POINTER(AdamwDesc), ctypes.POINTER(AdamwTensor), ctypes.c_int64, ctypes.c_void_p],
@@ -548,6 +606,16 @@ def _register_fakes() -> None:
     def _linear_attention_backward(q, k, v, log_decay, state, reset, lengths, reverse, scale, kept, dy, dlast):
         return (q.new_empty(q.shape), q.new_empty(q.shape), v.new_empty(v.shape), log_decay.new_empty(log_decay.shape),
                 q.new_empty((q.shape[0], q.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32))
+
+
+    @torch.library.register_fake("pesq_cuda::muon_step")
+    def _muon_step(params, grads, momenta, copies, lr, momentum, nesterov, weight_decay, a, b, c, eps, steps, adjust,
+                   grad_scale):
+        return None
+
+    @torch.library.register_fake("pesq_cuda::orthogonalize")
+    def _orthogonalize(x, a, b, c, eps, steps):
+        return x.new_empty(x.shape)
 
 
     @torch.library.register_fake("pesq_cuda::adamw_step")
@@ -765,4 +833,12 @@ def gated_scan_check(stream: int = 0) -> int:
 
     failed = ctypes.c_uint32(0)
     check(library().pesq_gated_scan_check(ctypes.c_void_p(stream), ctypes.byref(failed)), "pesq_gated_scan_check")
+    return int(failed.value)
+
+
+def muon_check(stream: int = 0) -> int:
+    """Synchronise ``stream`` and return (and clear) the current device's Muon error word."""
+
+    failed = ctypes.c_uint32(0)
+    check(library().pesq_muon_check(ctypes.c_void_p(stream), ctypes.byref(failed)), "pesq_muon_check")
     return int(failed.value)

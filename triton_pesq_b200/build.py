@@ -34,7 +34,7 @@ CUDA_SOURCES = ["front.cu", "align.cu", "back.cu", "spectrum.cu", "chain.cu", "r
                 "layer_norm_f32_bf16.cu", "layer_norm_f32_f16.cu", "layer_norm_abi.cu",
                 "linear_attention_forward_f32.cu", "linear_attention_forward_bf16.cu", "linear_attention_forward_f16.cu",
                 "linear_attention_backward_f32.cu", "linear_attention_backward_bf16.cu", "linear_attention_backward_f16.cu",
-                "linear_attention_abi.cu"]
+                "linear_attention_abi.cu", "muon.cu"]
 NVCC_FLAGS = [
     "-std=c++17",
     "-O3",

@@ -1,4 +1,4 @@
-// torch custom ops of the layer norm and the linear attention over the C ABI of
+// torch custom ops of the layer norm, the linear attention and Muon over the C ABI of
 // libpesq_cuda.so, with their autograd nodes: as in torch_train_ops.cpp, the op that
 // a caller uses, and the forward and backward it is made of.
 #include <algorithm>
@@ -370,7 +370,129 @@ std::tuple<at::Tensor, at::Tensor> linear_attention(const at::Tensor& q, const a
   return {y, last};
 }
 
+// ------------------------------------------------------------------------ Muon
+
+constexpr const char* kMuon = "Muon step";
+constexpr const char* kOrthogonalize = "orthogonalisation";
+
+void check_dense(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_contiguous(), "The CUDA Muon step needs dense `", name, "`.");
+}
+
+void muon_step(at::TensorList params, at::TensorList grads, at::TensorList momenta, at::TensorList copies, double lr,
+               double momentum, bool nesterov, double weight_decay, double a, double b, double c, double eps, int64_t steps,
+               int64_t adjust, const OptTensor& grad_scale) {
+  TORCH_CHECK_VALUE(params.size() == grads.size() && params.size() == momenta.size(),
+                    "The CUDA Muon step needs a gradient and a momentum for every parameter, got ", params.size(), ", ",
+                    grads.size(), " and ", momenta.size(), ".");
+  TORCH_CHECK_VALUE(copies.empty() || copies.size() == params.size(),
+                    "The CUDA Muon step needs a copy for every parameter or none, got ", copies.size(), ".");
+  if (params.empty()) return;
+  const at::Tensor& first = params[0];
+  check_cuda(first, first, kMuon, "params");
+  c10::cuda::CUDAGuard guard(first.device());
+  pesq_muon_desc d{};
+  d.nesterov = nesterov;
+  d.adjust = static_cast<int32_t>(adjust);
+  TORCH_CHECK_VALUE(steps >= 1 && steps <= 100, "The CUDA Muon step takes between 1 and 100 steps, got ", steps, ".");
+  d.steps = static_cast<int32_t>(steps);
+  d.momentum = momentum;
+  d.lr = static_cast<float>(lr);
+  d.weight_decay = static_cast<float>(weight_decay);
+  d.eps = static_cast<float>(eps);
+  d.a = static_cast<float>(a), d.b = static_cast<float>(b), d.c = static_cast<float>(c);
+  if (given(grad_scale)) {
+    check_cuda(*grad_scale, first, kMuon, "grad_scale");
+    check_float(*grad_scale, kMuon, "grad_scale");
+    TORCH_CHECK_VALUE(grad_scale->numel() == 1, "The CUDA Muon step needs one `grad_scale`.");
+    d.grad_scale = grad_scale->data_ptr<float>();
+  }
+  std::vector<pesq_muon_tensor> table;
+  std::vector<at::Tensor> dense;  // gradients that had to be copied
+  table.reserve(params.size());
+  bool typed = false;
+  at::ScalarType type = at::kFloat;
+  for (size_t i = 0; i < params.size(); ++i) {
+    const at::Tensor &p = params[i], &m = momenta[i];
+    at::Tensor g = grads[i];
+    check_cuda(p, first, kMuon, "params");
+    check_float(p, kMuon, "params");
+    TORCH_CHECK_VALUE(p.dim() == 2, "The CUDA Muon step needs matrices, got `params` of shape ", p.sizes(), ".");
+    check_dense(p, "params");
+    if (!g.defined() || g.numel() == 0) continue;
+    check_cuda(g, first, kMuon, "grads");
+    check_shape(g, p.sizes(), kMuon, "grads");
+    check_cuda(m, first, kMuon, "momenta");
+    check_float(m, kMuon, "momenta");
+    check_shape(m, p.sizes(), kMuon, "momenta");
+    check_dense(m, "momenta");
+    if (!typed) type = g.scalar_type(), d.grad_dtype = dtype_code(g, kMuon, "grads"), typed = true;
+    TORCH_CHECK(g.scalar_type() == type, "The CUDA Muon step needs gradients of one type, got ", type, " and ",
+                g.scalar_type(), ".");
+    if (!g.is_contiguous()) {
+      dense.push_back(g.contiguous());
+      g = dense.back();
+    }
+    pesq_muon_tensor e{p.data_ptr<float>(), g.data_ptr(), m.data_ptr<float>(), nullptr, p.size(0), p.size(1)};
+    if (!copies.empty()) {
+      const at::Tensor& q = copies[i];
+      check_cuda(q, first, kMuon, "copies");
+      check_shape(q, p.sizes(), kMuon, "copies");
+      check_dense(q, "copies");
+      TORCH_CHECK(q.scalar_type() == type && type != at::kFloat,
+                  "The CUDA Muon step needs copies in the gradients' 16-bit type, they are ", q.scalar_type(), ".");
+      e.copy = q.data_ptr();
+    }
+    table.push_back(e);
+  }
+  const int64_t count = static_cast<int64_t>(table.size());
+  size_t bytes = 0;
+  check_status(pesq_muon_workspace(&d, table.data(), count, &bytes), "pesq_muon_workspace");
+  if (!count) return;
+  at::Tensor ws = at::empty({static_cast<int64_t>(bytes)}, first.options().dtype(at::kByte));
+  for (size_t i = 0; i < params.size(); ++i) {
+    if (!grads[i].defined() || grads[i].numel() == 0) continue;
+    params[i].unsafeGetTensorImpl()->bump_version();
+    momenta[i].unsafeGetTensorImpl()->bump_version();
+    if (!copies.empty()) copies[i].unsafeGetTensorImpl()->bump_version();
+  }
+  check_status(pesq_muon_step(&d, table.data(), count, at::cuda::getCurrentCUDAStream(), ws.data_ptr(), bytes),
+               "pesq_muon_step");
+}
+
+at::Tensor orthogonalize(const at::Tensor& x_, double a, double b, double c, double eps, int64_t steps) {
+  check_cuda(x_, x_, kOrthogonalize, "x");
+  pesq_orthogonalize_desc d{};
+  d.dtype = dtype_code(x_, kOrthogonalize, "x");
+  TORCH_CHECK_VALUE(x_.dim() >= 2, "The CUDA orthogonalisation needs `x` [..., row, column], got ", x_.sizes(), ".");
+  TORCH_CHECK_VALUE(steps >= 1 && steps <= 100, "The CUDA orthogonalisation takes between 1 and 100 steps, got ", steps, ".");
+  c10::cuda::CUDAGuard guard(x_.device());
+  const at::Tensor x = x_.contiguous();
+  at::Tensor out = at::empty(x.sizes(), x.options());
+  if (x.numel() == 0) return out;
+  d.rows = x.size(-2);
+  d.cols = x.size(-1);
+  d.count = x.numel() / (d.rows * d.cols);
+  d.steps = static_cast<int32_t>(steps);
+  d.eps = static_cast<float>(eps);
+  d.a = static_cast<float>(a), d.b = static_cast<float>(b), d.c = static_cast<float>(c);
+  size_t bytes = 0;
+  check_status(pesq_orthogonalize_workspace(&d, &bytes), "pesq_orthogonalize_workspace");
+  at::Tensor ws = at::empty({static_cast<int64_t>(bytes)}, x.options().dtype(at::kByte));
+  check_status(pesq_orthogonalize(&d, at::cuda::getCurrentCUDAStream(), x.data_ptr(), out.data_ptr(), ws.data_ptr(), bytes),
+               "pesq_orthogonalize");
+  return out;
+}
+
 }  // namespace
+
+TORCH_LIBRARY_FRAGMENT(pesq_cuda, m) {
+  m.def(
+      "muon_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] momenta, Tensor(c!)[] copies, float lr, float momentum, "
+      "bool nesterov, float weight_decay, float a, float b, float c, float eps, int steps, int adjust, Tensor? grad_scale) "
+      "-> ()");
+  m.def("orthogonalize(Tensor x, float a, float b, float c, float eps, int steps) -> Tensor");
+}
 
 TORCH_LIBRARY_FRAGMENT(pesq_cuda, m) {
   const char* in = "(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? state, Tensor? reset, Tensor? lengths, "
@@ -399,4 +521,6 @@ TORCH_LIBRARY_IMPL(pesq_cuda, CUDA, m) {
   m.impl("layer_norm_backward", &layer_norm_backward);
   m.impl("linear_attention_forward", &linear_attention_forward);
   m.impl("linear_attention_backward", &linear_attention_backward);
+  m.impl("muon_step", &muon_step);
+  m.impl("orthogonalize", &orthogonalize);
 }
