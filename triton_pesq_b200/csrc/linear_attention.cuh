@@ -396,36 +396,47 @@ struct Row {
 template <class T, int D, int C, int THREADS>
 __device__ __forceinline__ void load_tile(T* tile, const Operand& o, int first, int cols, const Row& row, int64_t s0) {
   constexpr int LD = kLd<T, D>, kPer = D * (int)sizeof(T) / 16;  // 16-byte pieces of a row
-  constexpr int kRows = THREADS / kPer;
-  static_assert(THREADS % kPer == 0 && C % kRows == 0 || kRows > C, "");
-  const int piece = threadIdx.x % kPer, bytes = cols * (int)sizeof(T) - piece * 16;
-  if (bytes <= 0) return;
+  constexpr int kRows = THREADS / kPer < C ? THREADS / kPer : C;
+  static_assert(THREADS % kPer == 0 && C % kRows == 0, "");
+  const int piece = threadIdx.x % kPer, r0 = threadIdx.x / kPer, bytes = cols * (int)sizeof(T) - piece * 16;
+  if (bytes <= 0 || r0 >= kRows) return;
   const char* base = static_cast<const char*>(o.p) + (row.b * o.sb + row.h * o.sh + first) * (int64_t)sizeof(T) + piece * 16;
+  const uint32_t to0 = smem_of(tile) + r0 * LD * (int)sizeof(T) + piece * 16;
+  const int64_t step = row.reverse ? -o.st * (int64_t)sizeof(T) : o.st * (int64_t)sizeof(T);
+  const char* from = base + row.time(s0 + r0) * o.st * (int64_t)sizeof(T);
+  if (o.unit == 16 && s0 + C <= row.n) {
 #pragma unroll
-  for (int r0 = 0; r0 < C; r0 += kRows) {
-    const int r = r0 + threadIdx.x / kPer;
-    if (kRows > C && r >= C) break;
-    const int64_t s = s0 + r;
-    const bool live = s < row.n;
-    const char* from = live ? base + row.time(s) * o.st * (int64_t)sizeof(T) : static_cast<const char*>(o.p);
-    char* to = reinterpret_cast<char*>(tile + r * LD) + piece * 16;
+    for (int k = 0; k < C / kRows; ++k) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to0 + k * kRows * LD * (int)sizeof(T)), "l"(from) : "memory");
+      from += kRows * step;
+    }
+    return;
+  }
+#pragma unroll 1
+  for (int k = 0; k < C / kRows; ++k) {
+    const bool live = s0 + r0 + k * kRows < row.n;
+    const uint32_t to = to0 + k * kRows * LD * (int)sizeof(T);
+    // (a piece that is not live is zeros, of any address)
+    const char* at = live ? from : static_cast<const char*>(o.p);
     if (o.unit == 16) {
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_of(to)), "l"(from), "r"(live ? 16 : 0) : "memory");
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(at), "r"(live ? 16 : 0) : "memory");
     } else if (o.unit == 8) {
 #pragma unroll
       for (int x = 0; x < 16; x += 8)
         if (x < bytes)
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_of(to + x)), "l"(live ? from + x : from), "r"(live ? 8 : 0) : "memory");
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to + x), "l"(live ? at + x : at), "r"(live ? 8 : 0) : "memory");
     } else if (o.unit == 4) {
 #pragma unroll
       for (int x = 0; x < 16; x += 4)
         if (x < bytes)
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_of(to + x)), "l"(live ? from + x : from), "r"(live ? 4 : 0) : "memory");
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + x), "l"(live ? at + x : at), "r"(live ? 4 : 0) : "memory");
     } else {
+      char* generic = reinterpret_cast<char*>(tile + (r0 + k * kRows) * LD) + piece * 16;
 #pragma unroll
       for (int x = 0; x < 16; x += 2)
-        if (x < bytes) *reinterpret_cast<uint16_t*>(to + x) = live ? *reinterpret_cast<const uint16_t*>(from + x) : (uint16_t)0;
+        if (x < bytes) *reinterpret_cast<uint16_t*>(generic + x) = live ? *reinterpret_cast<const uint16_t*>(at + x) : (uint16_t)0;
     }
+    from += kRows * step;
   }
 }
 __device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -452,8 +463,9 @@ struct Decays {
   __device__ __forceinline__ static double log2_of(float g) {
     return g * kLog2e < kCut ? (double)kCut : (double)g * 1.4426950408889634;  // (a NaN stays one)
   }
-  // sums as two floats, e^{G_i}, e^{G_C - G_j}
-  __device__ __forceinline__ void store(float2* sums, float* before, float* after) const {
+  // sums as two floats, e^{G_i}, e^{G_C - G_j}, and e^{G_e - G_j} to the last step e of j's sixteen
+  __device__ __forceinline__ void store(float2* sums) const {
+    float *before = reinterpret_cast<float*>(sums + C), *after = before + C, *tail = after + C;
     const int lane = threadIdx.x & 31;
     double own[E], total = 0.0;
 #pragma unroll
@@ -464,7 +476,7 @@ struct Decays {
       const double v = __shfl_up_sync(0xffffffffu, up, off);
       if (lane >= off) up += v;
     }
-    const double all = __shfl_sync(0xffffffffu, up, 31);
+    const double all = __shfl_sync(0xffffffffu, up, 31), ends = __shfl_sync(0xffffffffu, up, lane | (16 / E - 1));
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const double at = up - total + own[e];
@@ -472,10 +484,61 @@ struct Decays {
       sums[lane * E + e] = make_float2(hi, (float)(at - hi));
       before[lane * E + e] = exp2_approx(hi);
       after[lane * E + e] = exp2_approx((float)(all - at));
+      tail[lane * E + e] = exp2_approx((float)(ends - at));
     }
   }
 };
+template <int C>
+constexpr int kDecayBytes = 2 * C * 20;  // of two chunks
 __device__ __forceinline__ float between(float2 i, float2 j) { return exp2_approx((i.x - j.x) + (i.y - j.y)); }
+// Weights scale L of a thread's eighths of a 16 x 16 block, as `make` takes them: rows i0, i1 = i0 + 8 of steps i, columns of
+// steps j0 + 2c, + 1, + 8, + 9.  Where every i is past every j, L is e^{G_i - G_e} e^{G_e - G_j} with e the last of the
+// sixteen j, both of them 1 at most: two exponentials a thread instead of eight.
+__device__ __forceinline__ void weights_by_row(float (&w)[8], const float2* sums, const float* tail, int i0, int j0, bool diagonal,
+                                               float scale) {
+  const int j = j0 + 2 * (threadIdx.x & 3);
+  const float2 sum0 = sums[i0], sum1 = sums[i0 + 8];
+  if (!diagonal) {
+    const float2 end = sums[j0 + 15];
+    const float f0 = scale * between(sum0, end), f1 = scale * between(sum1, end);
+    const float2 t0 = *reinterpret_cast<const float2*>(tail + j), t1 = *reinterpret_cast<const float2*>(tail + j + 8);
+    w[0] = f0 * t0.x, w[1] = f0 * t0.y, w[2] = f1 * t0.x, w[3] = f1 * t0.y;
+    w[4] = f0 * t1.x, w[5] = f0 * t1.y, w[6] = f1 * t1.x, w[7] = f1 * t1.y;
+    return;
+  }
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int at = j + 8 * half;
+    const float4 two = *reinterpret_cast<const float4*>(sums + at);
+    const float2 a = make_float2(two.x, two.y), b = make_float2(two.z, two.w);
+    w[4 * half] = at <= i0 ? scale * between(sum0, a) : 0.0f;
+    w[4 * half + 1] = at + 1 <= i0 ? scale * between(sum0, b) : 0.0f;
+    w[4 * half + 2] = at <= i0 + 8 ? scale * between(sum1, a) : 0.0f;
+    w[4 * half + 3] = at + 1 <= i0 + 8 ? scale * between(sum1, b) : 0.0f;
+  }
+}
+// The same of the transpose: rows of steps j = j0, j0 + 8, columns of steps i0 + 2c ..
+__device__ __forceinline__ void weights_by_column(float (&w)[8], const float2* sums, const float* tail, int j0, int i0, int block,
+                                                  bool diagonal, float scale) {
+  const int i = i0 + 2 * (threadIdx.x & 3);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int at = i + 8 * half;
+    const float4 two = *reinterpret_cast<const float4*>(sums + at);
+    const float2 a = make_float2(two.x, two.y), b = make_float2(two.z, two.w);
+    if (!diagonal) {
+      const float2 end = sums[block + 15];  // (of j's sixteen)
+      const float f0 = scale * between(a, end), f1 = scale * between(b, end), t0 = tail[j0], t1 = tail[j0 + 8];
+      w[4 * half] = f0 * t0, w[4 * half + 1] = f1 * t0, w[4 * half + 2] = f0 * t1, w[4 * half + 3] = f1 * t1;
+    } else {
+      const float2 sum0 = sums[j0], sum1 = sums[j0 + 8];
+      w[4 * half] = j0 <= at ? scale * between(a, sum0) : 0.0f;
+      w[4 * half + 1] = j0 <= at + 1 ? scale * between(b, sum0) : 0.0f;
+      w[4 * half + 2] = j0 + 8 <= at ? scale * between(a, sum1) : 0.0f;
+      w[4 * half + 3] = j0 + 8 <= at + 1 ? scale * between(b, sum1) : 0.0f;
+    }
+  }
+}
 // a factor of zero cuts off whatever it multiplies
 __device__ __forceinline__ float decayed(float factor, float x) { return factor == 0.0f ? 0.0f : factor * x; }
 
@@ -493,6 +556,7 @@ struct State {
   using Shape = StateShape<DK, DV, WARPS>;
   float x[Shape::kTiles][Shape::kCols / 8][4];
 
+  // (warps past the first WARPS have no part in it)
   static __device__ __forceinline__ int row0() { return (threadIdx.x >> 5) % Shape::kRowWarps * Shape::kTiles * 16; }
   static __device__ __forceinline__ int col0() { return (threadIdx.x >> 5) / Shape::kRowWarps * Shape::kCols; }
   // f(row, column, value of it, of the next column), rows and columns of the state
@@ -521,37 +585,45 @@ struct State {
       if (r < key && first + c + 1 < value) to[(int64_t)r * value + first + c + 1] = b;
     });
   }
-  // S = factor S + sum over the chunk's steps of weight a b^T
+  // S = factor S + sum over the chunk's steps of weight a b^T.  The chunk's sum is made by itself and added, rounded: the
+  // instruction cuts off what its accumulator does not hold, which over the chunks that a slow head remembers is 1e-5.
   template <class T, int C>
   __device__ __forceinline__ void update(const T* a, const T* b, const float* weights, float factor, float scale) {
     const int c = threadIdx.x & 3;
+    constexpr int kBlocks = C / 16, kTogether = std::is_same<T, __nv_bfloat16>::value ? kBlocks : 2;  // of registers' worth
 #pragma unroll
-    for (int m = 0; m < Shape::kTiles; ++m)
+    for (int m = 0; m < Shape::kTiles; ++m) {
 #pragma unroll
-      for (int n = 0; n < Shape::kCols / 8; ++n)
+      for (int k0 = 0; k0 < kBlocks; k0 += kTogether) {
+        Made<T> left[kTogether];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[m][n][e] = decayed(factor, x[m][n][e]);
+        for (int k = 0; k < kTogether; ++k) {
+          const int at = (k0 + k) * 16;
+          const float2 w0 = *reinterpret_cast<const float2*>(weights + at + 2 * c);
+          const float2 w1 = *reinterpret_cast<const float2*>(weights + at + 8 + 2 * c);
+          float f[8];
+          load_a<T, kLd<T, DK>, true>(f, a, row0() + m * 16, at);
+          f[0] *= w0.x * scale, f[1] *= w0.y * scale, f[2] *= w0.x * scale, f[3] *= w0.y * scale;
+          f[4] *= w1.x * scale, f[5] *= w1.y * scale, f[6] *= w1.x * scale, f[7] *= w1.y * scale;
+          make(left[k], f);
+        }
 #pragma unroll
-    for (int k = 0; k < C; k += 16) {
-      const float2 w0 = *reinterpret_cast<const float2*>(weights + k + 2 * c);
-      const float2 w1 = *reinterpret_cast<const float2*>(weights + k + 8 + 2 * c);
-      Made<T> left[Shape::kTiles];
+        for (int n = 0; n < Shape::kCols / 16; ++n) {
+          float sum[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-      for (int m = 0; m < Shape::kTiles; ++m) {
-        float f[8];
-        load_a<T, kLd<T, DK>, true>(f, a, row0() + m * 16, k);
-        f[0] *= w0.x * scale, f[1] *= w0.y * scale, f[2] *= w0.x * scale, f[3] *= w0.y * scale;
-        f[4] *= w1.x * scale, f[5] *= w1.y * scale, f[6] *= w1.x * scale, f[7] *= w1.y * scale;
-        make(left[m], f);
-      }
+          for (int k = 0; k < kTogether; ++k) {
+            InB<T> right[2];
+            load_b<T, kLd<T, DV>, true>(right, b, col0() + n * 16, (k0 + k) * 16);
+            mma(sum[0], left[k], right[0]);
+            mma(sum[1], left[k], right[1]);
+          }
 #pragma unroll
-      for (int n = 0; n < Shape::kCols / 16; ++n) {
-        InB<T> right[2];
-        load_b<T, kLd<T, DV>, true>(right, b, col0() + n * 16, k);
+          for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int m = 0; m < Shape::kTiles; ++m) {
-          mma(x[m][2 * n], left[m], right[0]);
-          mma(x[m][2 * n + 1], left[m], right[1]);
+            for (int e = 0; e < 4; ++e) {
+              float& s = x[m][2 * n + half][e];
+              s = (k0 == 0 ? decayed(factor, s) : s) + sum[half][e];
+            }
         }
       }
     }
@@ -566,19 +638,38 @@ struct State {
 // Bytes of the state before a chunk: two planes of 16 bits, or 32, of [DK][DV]
 __host__ __device__ constexpr int64_t kept_bytes(int DK, int DV) { return (int64_t)4 * DK * DV; }
 
-template <class T>
-__device__ __forceinline__ void store_pair(void* base, int64_t at, int col, int cols, float x, float y) {
-  T* to = static_cast<T*>(base) + at + col;
-  if (cols % 2 == 0) {
-    if (col < cols) {
-      Pack<T, 2> v;
-      v.v[0] = narrow<T>(x), v.v[1] = narrow<T>(y);
-      *reinterpret_cast<Pack<T, 2>*>(to) = v;
+// A warp's 16 rows of N times 8 columns from col (the thread's first) to rows of `width`: those of steps s and s + 8, where
+// they are within the row; zeros past its length
+template <class T, int N>
+__device__ __forceinline__ void store_rows(void* base, const Args& p, const Row& row, int64_t s, int width, int col, const float (&x)[N][4]) {
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int64_t at = s + 8 * half;
+    if (at >= row.steps) continue;
+    const bool live = at < row.n;
+    T* to = static_cast<T*>(base) + ((row.b * row.steps + row.time(at)) * p.heads + row.h) * width + col;
+    const int left = width - col;
+    if (width % 2 == 0) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        Pack<T, 2> v;
+        v.v[0] = narrow<T>(live ? x[n][2 * half] : 0.0f), v.v[1] = narrow<T>(live ? x[n][2 * half + 1] : 0.0f);
+        if (n * 8 < left) *reinterpret_cast<Pack<T, 2>*>(to + n * 8) = v;
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        if (n * 8 < left) to[n * 8] = narrow<T>(live ? x[n][2 * half] : 0.0f);
+        if (n * 8 + 1 < left) to[n * 8 + 1] = narrow<T>(live ? x[n][2 * half + 1] : 0.0f);
+      }
     }
-  } else {
-    if (col < cols) to[0] = narrow<T>(x);
-    if (col + 1 < cols) to[1] = narrow<T>(y);
   }
+}
+// two adjacent values of a tile
+template <class T>
+__device__ __forceinline__ float2 two_of(const T* at) {
+  if constexpr (kHalfWord<T>) return floats_of(*reinterpret_cast<const uint32_t*>(at), T{});
+  else return *reinterpret_cast<const float2*>(at);
 }
 
 template <int THREADS>
@@ -587,20 +678,45 @@ __device__ __forceinline__ void clear(void* p, int bytes) {
   for (int i = threadIdx.x; i < bytes / 16; i += THREADS) q[i] = make_uint4(0u, 0u, 0u, 0u);
 }
 
+// Loops over the channels of a contraction.  Where a product is many instructions, code that repeats them outgrows the
+// instruction cache (two thirds of the stalls of a float32 forward)
+template <class T>
+constexpr int kUnroll = std::is_same<T, __nv_bfloat16>::value ? 4 : 1;
+
+// 16 rows of a from m0 times 16 rows of b from n0, over their D channels
+template <class T, int D>
+__device__ __forceinline__ void products(float (&sum)[2][4], const T* a, int m0, const T* b, int n0) {
+#pragma unroll kUnroll<T>
+  for (int kk = 0; kk < D; kk += 16) {
+    InA<T> left;
+    InB<T> right[2];
+    load_a<T, kLd<T, D>>(left, a, m0, kk);
+    load_b<T, kLd<T, D>, false>(right, b, n0, kk);
+    mma(sum[0], left, right[0]);
+    mma(sum[1], left, right[1]);
+  }
+}
+
 // ------------------------------------------------------------------------------------------- forward
 
+#ifndef FWD_LIMIT
+#define FWD_LIMIT 55
+#endif
+#ifndef FWD_CTAS
+#define FWD_CTAS 4
+#endif
 template <class T, int DK, int DV, int C>
 struct ForwardShared {
   static constexpr int kTiles = (2 * C * kLd<T, DK> + C * kLd<T, DV>) * (int)sizeof(T);
   static constexpr int kState = kPlanes<T> * DK * kLd<Stored<T>, DV> * (int)sizeof(Stored<T>);
-  static constexpr int kDecays = 2 * C * 16;  // two chunks' sums, e^G and e^{G_C - G}
-  // the next chunk's tiles come in while one is worked on, where three CTAs an SM have the room
-  static constexpr int kStages = 2 * kTiles + kState + kDecays <= (75 << 10) ? 2 : 1;
+  static constexpr int kDecays = kDecayBytes<C>;
+  // the next chunk's tiles come in while one is worked on, where four CTAs an SM have the room
+  static constexpr int kStages = 2 * kTiles + kState + kDecays <= (FWD_LIMIT << 10) ? 2 : 1;
   static constexpr int kBytes = kStages * kTiles + kState + kDecays;
 };
 
 template <class T, int DK, int DV, int C>
-__global__ void __launch_bounds__(128) forward_kernel(const __grid_constant__ Args p) {
+__global__ void __launch_bounds__(128, DK == 128 ? 2 : FWD_CTAS) forward_kernel(const __grid_constant__ Args p) {
   constexpr int THREADS = 128, WARPS = 4, RG = C / 16, WC = WARPS / RG, NY = DV / WC / 8;
   using Sh = ForwardShared<T, DK, DV, C>;
   constexpr int LDK = kLd<T, DK>, LDV = kLd<T, DV>, LDS = kLd<Stored<T>, DV>, PLANE = DK * LDS;
@@ -640,12 +756,12 @@ __global__ void __launch_bounds__(128) forward_kernel(const __grid_constant__ Ar
     }
     copies_issued();
   };
-  const auto sums_of = [&](int chunk) { return reinterpret_cast<float2*>(decays + (chunk & 1) * C * 16); };
+  const auto sums_of = [&](int chunk) { return reinterpret_cast<float2*>(decays + (chunk & 1) * C * 20); };
   Decays<C> next;
   load(c0, 0);
   if (warp == WARPS - 1) {
     next.load(p, row, (int64_t)c0 * C);
-    next.store(sums_of(c0), reinterpret_cast<float*>(sums_of(c0) + C), reinterpret_cast<float*>(sums_of(c0) + C) + C);
+    next.store(sums_of(c0));
   }
 #pragma unroll 1
   for (int chunk = c0; chunk < c1; ++chunk) {
@@ -657,7 +773,7 @@ __global__ void __launch_bounds__(128) forward_kernel(const __grid_constant__ Ar
     if (warp == WARPS - 1 && chunk + 1 < c1) next.load(p, row, s0 + C);
     const T *q = q_of(stage), *k = q + C * LDK, *v = q + 2 * C * LDK;
     const float2* sums = sums_of(chunk);
-    const float *before = reinterpret_cast<const float*>(sums + C), *after = before + C;
+    const float *before = reinterpret_cast<const float*>(sums + C), *after = before + C, *tail = after + C;
     const bool live = s0 < row.n;
     if (live && p.kept) {
       // the state before the chunk, for the backward: 16-byte pieces of the operand's planes
@@ -675,23 +791,11 @@ __global__ void __launch_bounds__(128) forward_kernel(const __grid_constant__ Ar
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[n][e] = 0.0f;
     if (live) {
-      float a[C / 8][4];
-#pragma unroll
-      for (int n = 0; n < C / 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) a[n][e] = 0.0f;
-#pragma unroll
+      const int i0 = rg * 16 + g;
+#pragma unroll kUnroll<T>
       for (int kk = 0; kk < DK; kk += 16) {
         InA<T> left;
         load_a<T, LDK>(left, q, rg * 16, kk);
-#pragma unroll
-        for (int n = 0; n < C / 16; ++n) {
-          if (n > rg) break;
-          InB<T> right[2];
-          load_b<T, LDK, false>(right, k, n * 16, kk);
-          mma(a[2 * n], left, right[0]);
-          mma(a[2 * n + 1], left, right[1]);
-        }
 #pragma unroll
         for (int n = 0; n < NY / 2; ++n) {
           MadeB<T> right[2];
@@ -700,29 +804,21 @@ __global__ void __launch_bounds__(128) forward_kernel(const __grid_constant__ Ar
           mma(y[2 * n + 1], left, right[1]);
         }
       }
-      const int i0 = rg * 16 + g, i1 = i0 + 8;
-      const float b0 = before[i0] * p.scale, b1 = before[i1] * p.scale;
+      const float b0 = before[i0] * p.scale, b1 = before[i0 + 8] * p.scale;
 #pragma unroll
       for (int n = 0; n < NY; ++n) {
         y[n][0] = decayed(b0, y[n][0]), y[n][1] = decayed(b0, y[n][1]);
         y[n][2] = decayed(b1, y[n][2]), y[n][3] = decayed(b1, y[n][3]);
       }
-      const float2 sum0 = sums[i0], sum1 = sums[i1];
+      // sixteen steps j at a time, up to the warp's own
+#pragma unroll 1
+      for (int n = 0; n <= rg; ++n) {
+        float a[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+        products<T, DK>(a, q, rg * 16, k, n * 16);
+        float w[8], x[8];
+        weights_by_row(w, sums, tail, i0, n * 16, n == rg, p.scale);
 #pragma unroll
-      for (int n = 0; n < C / 16; ++n) {
-        if (n > rg) break;
-        float x[8];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int j = n * 16 + half * 8 + 2 * c;
-          const float4 two = *reinterpret_cast<const float4*>(sums + j);
-          const float2 s0j = make_float2(two.x, two.y), s1j = make_float2(two.z, two.w);
-          const float(&at)[4] = a[2 * n + half];
-          x[4 * half] = j <= i0 ? at[0] * (p.scale * between(sum0, s0j)) : 0.0f;
-          x[4 * half + 1] = j + 1 <= i0 ? at[1] * (p.scale * between(sum0, s1j)) : 0.0f;
-          x[4 * half + 2] = j <= i1 ? at[2] * (p.scale * between(sum1, s0j)) : 0.0f;
-          x[4 * half + 3] = j + 1 <= i1 ? at[3] * (p.scale * between(sum1, s1j)) : 0.0f;
-        }
+        for (int e = 0; e < 8; ++e) x[e] = w[e] == 0.0f ? 0.0f : a[e >> 2][e & 3] * w[e];
         Made<T> left;
         make(left, x);
 #pragma unroll
@@ -735,20 +831,9 @@ __global__ void __launch_bounds__(128) forward_kernel(const __grid_constant__ Ar
       }
       S.template update<T, C>(k, v, after, before[C - 1], 1.0f);
     }
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int64_t s = s0 + rg * 16 + g + half * 8;
-      if (s >= row.steps) continue;
-      const int64_t at = ((row.b * row.steps + row.time(s)) * p.heads + row.h) * p.value;
-      const bool in = s < row.n;
-#pragma unroll
-      for (int n = 0; n < NY; ++n)
-        store_pair<T>(p.y, at, first + wc * NY * 8 + n * 8 + 2 * c, p.value, in ? y[n][2 * half] : 0.0f,
-                      in ? y[n][2 * half + 1] : 0.0f);
-    }
+    store_rows<T>(p.y, p, row, s0 + rg * 16 + g, p.value, first + wc * NY * 8 + 2 * c, y);
     if (warp == WARPS - 1 && chunk + 1 < c1) {
-      float2* to = sums_of(chunk + 1);
-      next.store(to, reinterpret_cast<float*>(to + C), reinterpret_cast<float*>(to + C) + C);
+      next.store(sums_of(chunk + 1));
     }
     __syncthreads();  // the chunk's tiles and state are read
     if (live) S.template publish<T>(s_state);
@@ -764,7 +849,7 @@ __global__ void __launch_bounds__(128) forward_kernel(const __grid_constant__ Ar
 template <class T, int DK, int DV, int C>
 struct SweepShared {
   static constexpr int kTiles = C * (kLd<T, DK> + kLd<T, DV>) * (int)sizeof(T);
-  static constexpr int kDecays = 2 * C * 16;
+  static constexpr int kDecays = kDecayBytes<C>;
   static constexpr int kBytes = 2 * kTiles + kDecays;
 };
 template <class T, int DK, int DV, int C, bool kBackward>
@@ -798,11 +883,10 @@ __global__ void __launch_bounds__(128) sweep_kernel(const __grid_constant__ Args
   };
   const int count = c1 - c0;
   const auto chunk_of = [&](int i) { return kBackward ? c1 - 1 - i : c0 + i; };
-  const auto sums_of = [&](int i) { return reinterpret_cast<float2*>(decays + (i & 1) * C * 16); };
+  const auto sums_of = [&](int i) { return reinterpret_cast<float2*>(decays + (i & 1) * C * 20); };
   Decays<C> next;
   const auto store = [&](int i) {
-    float2* to = sums_of(i);
-    next.store(to, reinterpret_cast<float*>(to + C), reinterpret_cast<float*>(to + C) + C);
+    next.store(sums_of(i));
   };
   load(chunk_of(0), 0);
   if (warp == WARPS - 1) {
@@ -841,33 +925,49 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
   float s = from && r < p.key && c < p.value ? from[(index * p.key + r) * p.value + c] : 0.0f;
   float* starts = p.starts + index * p.parts * size + at;
   const float* factors = p.factors + index * p.parts;
-  for (int i = 0; i < p.parts; ++i) {
-    const int part = backward ? p.parts - 1 - i : i;
-    const float add = i + 1 < p.parts ? starts[part * size] : 0.0f;
-    starts[part * size] = s;
-    if (i + 1 < p.parts) s = decayed(factors[part], s) + add;
+  constexpr int kAhead = 8;  // parts whose loads are on their way together
+  for (int i0 = 0; i0 < p.parts; i0 += kAhead) {
+    float add[kAhead], factor[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = i0 + k, part = backward ? p.parts - 1 - i : i;
+      const bool in = i + 1 < p.parts;
+      add[k] = in ? starts[part * size] : 0.0f;
+      factor[k] = in ? factors[part] : 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = i0 + k, part = backward ? p.parts - 1 - i : i;
+      if (i >= p.parts) break;
+      starts[part * size] = s;
+      s = decayed(factor[k], s) + add[k];
+    }
   }
 }
 
 // ------------------------------------------------------------------------------------------ backward
 
+// Half the warps work by rows i (dQ, and the state's gradient, which takes about as long as the rest of the other half),
+// half by rows j (dK and dV).
 template <class T, int DK, int DV>
-constexpr int kBackWarps = DK > 64 || DV > 64 ? 8 : 4;
+constexpr int kSide = DK > 64 || DV > 64 ? 8 : 4;
 
 template <class T, int DK, int DV, int C>
 struct BackwardShared {
-  static constexpr int WARPS = kBackWarps<T, DK, DV>, WC = WARPS / (C / 16);
+  static constexpr int SIDE = kSide<T, DK, DV>, WC = SIDE / (C / 16);
   static constexpr int kTiles = 2 * C * (kLd<T, DK> + kLd<T, DV>) * (int)sizeof(T);
   static constexpr int kState = kPlanes<T> * DK * kLd<Stored<T>, DV> * (int)sizeof(Stored<T>);
-  static constexpr int kDecays = 2 * C * 16;
-  static constexpr int kSums = ((2 * WC + C / 16 + 1) * C + WARPS) * 4;
+  static constexpr int kDecays = kDecayBytes<C>;
+  static constexpr int kSums = ((2 * WC + C / 16 + 1) * C + SIDE) * 4;
   static constexpr int kBytes = kTiles + 2 * kState + kDecays + kSums;
 };
 
 template <class T, int DK, int DV, int C>
-__global__ void __launch_bounds__(32 * kBackWarps<T, DK, DV>) backward_kernel(const __grid_constant__ Args p) {
+__global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ? 2 : 1)
+    backward_kernel(const __grid_constant__ Args p) {
   using Sh = BackwardShared<T, DK, DV, C>;
-  constexpr int WARPS = Sh::WARPS, THREADS = 32 * WARPS, RG = C / 16, WC = Sh::WC, NK = DK / WC / 8, NV = DV / WC / 8;
+  constexpr int SIDE = Sh::SIDE, WARPS = 2 * SIDE, THREADS = 32 * WARPS, RG = C / 16, WC = Sh::WC;
+  constexpr int NK = DK / WC / 8, NV = DV / WC / 8;
   constexpr int LDK = kLd<T, DK>, LDV = kLd<T, DV>, LDS = kLd<Stored<T>, DV>, PLANE = DK * LDS;
   extern __shared__ __align__(16) char shared[];
   T *q = reinterpret_cast<T*>(shared), *k = q + C * LDK, *v = k + C * LDK, *dy = v + C * LDV;
@@ -876,11 +976,12 @@ __global__ void __launch_bounds__(32 * kBackWarps<T, DK, DV>) backward_kernel(co
   char* decays = shared + Sh::kTiles + 2 * Sh::kState;
   float* s_far = reinterpret_cast<float*>(decays + Sh::kDecays);  // [WC][C]: scale e^{G_i} q_i S dy_i
   float* s_end = s_far + WC * C;                                  // [WC][C]: e^{G_C - G_j} k_j dS v_j
-  float* s_row = s_end + WC * C;                                  // [RG][C]: sums of W over the warp's j, of each i
+  float* s_row = s_end + WC * C;                                  // [RG][C]: sums of W over sixteen j, of each i
   float* s_col = s_row + RG * C;                                  // [C]: over i, of each j
-  float* s_all = s_col + C;                                       // [WARPS]: <S, dS>
+  float* s_all = s_col + C;                                       // [SIDE]: <S, dS>
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
-  const int rg = warp % RG, wc = warp / RG;
+  const bool by_rows = warp < SIDE;
+  const int rg = warp % SIDE % RG, wc = warp % SIDE / RG;
 
   const int64_t index = blockIdx.x / p.parts;
   const int part = (int)(blockIdx.x - index * p.parts);
@@ -888,13 +989,15 @@ __global__ void __launch_bounds__(32 * kBackWarps<T, DK, DV>) backward_kernel(co
   const int c0 = part * p.part_chunks, c1 = min(p.chunks, c0 + p.part_chunks);
 
   clear<THREADS>(shared, Sh::kTiles);
-  State<DK, DV, WARPS> S;  // the gradient of the state
-  const float* from = p.dlast ? p.dlast + index * p.key * p.value : nullptr;
-  if (p.parts > 1)
-    S.read(p.starts + (index * p.parts + part) * DK * DV, DK, DV, 0);
-  else
-    S.read(from, p.key, p.value, 0);
-  S.template publish<T>(s_grad);
+  State<DK, DV, SIDE> S;  // the gradient of the state, of the warps by rows
+  if (by_rows) {
+    const float* from = p.dlast ? p.dlast + index * p.key * p.value : nullptr;
+    if (p.parts > 1)
+      S.read(p.starts + (index * p.parts + part) * DK * DV, DK, DV, 0);
+    else
+      S.read(from, p.key, p.value, 0);
+    S.template publish<T>(s_grad);
+  }
   __syncthreads();
 
   const auto load = [&](int chunk) {
@@ -904,9 +1007,10 @@ __global__ void __launch_bounds__(32 * kBackWarps<T, DK, DV>) backward_kernel(co
       load_tile<T, DK, C, THREADS>(k, p.k, 0, p.key, row, s0);
       load_tile<T, DV, C, THREADS>(v, p.v, 0, p.value, row, s0);
       load_tile<T, DV, C, THREADS>(dy, p.dy, 0, p.value, row, s0);
-      constexpr int kPieces = DV * (int)sizeof(Stored<T>) / 16;
+      constexpr int kPieces = DV * (int)sizeof(Stored<T>) / 16, kAll = kPlanes<T> * DK * kPieces;
       const char* at = static_cast<const char*>(p.kept) + (index * p.chunks + chunk) * kept_bytes(DK, DV);
-      for (int i = threadIdx.x; i < kPlanes<T> * DK * kPieces; i += THREADS) {
+#pragma unroll 4
+      for (int i = threadIdx.x; i < kAll; i += THREADS) {
         const int r = i / kPieces, piece = i % kPieces;
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
                          smem_of(reinterpret_cast<const char*>(s_state + r * LDS) + piece * 16)),
@@ -915,11 +1019,10 @@ __global__ void __launch_bounds__(32 * kBackWarps<T, DK, DV>) backward_kernel(co
     }
     copies_issued();
   };
-  const auto sums_of = [&](int chunk) { return reinterpret_cast<float2*>(decays + (chunk & 1) * C * 16); };
+  const auto sums_of = [&](int chunk) { return reinterpret_cast<float2*>(decays + (chunk & 1) * C * 20); };
   Decays<C> now, next;
   const auto store = [&](int chunk) {
-    float2* to = sums_of(chunk);
-    next.store(to, reinterpret_cast<float*>(to + C), reinterpret_cast<float*>(to + C) + C);
+    next.store(sums_of(chunk));
     now = next;
   };
   load(c1 - 1);
@@ -934,255 +1037,204 @@ __global__ void __launch_bounds__(32 * kBackWarps<T, DK, DV>) backward_kernel(co
     __syncthreads();
     if (warp == WARPS - 1 && chunk > c0) next.load(p, row, s0 - C);
     const float2* sums = sums_of(chunk);
-    const float *before = reinterpret_cast<const float*>(sums + C), *after = before + C;
+    const float *before = reinterpret_cast<const float*>(sums + C), *after = before + C, *tail = after + C;
     const bool live = s0 < row.n;
-    const int i0 = rg * 16 + g, i1 = i0 + 8;
-    const float2 sum0 = sums[i0], sum1 = sums[i1];
-    const int64_t t0 = row.time(s0 + i0), t1 = row.time(s0 + i1);
-    const int64_t at0 = (row.b * row.steps + t0) * p.heads + row.h, at1 = (row.b * row.steps + t1) * p.heads + row.h;
-    const bool in0 = s0 + i0 < row.steps, in1 = s0 + i1 < row.steps;
-    const bool on0 = s0 + i0 < row.n, on1 = s0 + i1 < row.n;
-    const auto put = [&](void* to, int width, int col, const float (&x)[4]) {
-      if (in0) store_pair<T>(to, at0 * width, col, width, on0 ? x[0] : 0.0f, on0 ? x[1] : 0.0f);
-      if (in1) store_pair<T>(to, at1 * width, col, width, on1 ? x[2] : 0.0f, on1 ? x[3] : 0.0f);
-    };
-    if (live) {
-      // by rows i: dQ
-      float d[C / 8][4], out[NK][4];
-#pragma unroll
-      for (int n = 0; n < C / 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) d[n][e] = 0.0f;
+    const int i0 = rg * 16 + g;  // the warp's rows are i0 and i0 + 8, i or j
+    if (by_rows) {
+      float dq[NK][4];
 #pragma unroll
       for (int n = 0; n < NK; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) out[n][e] = 0.0f;
+        for (int e = 0; e < 4; ++e) dq[n][e] = 0.0f;
+      if (live) {
+#pragma unroll kUnroll<T>
+        for (int kk = 0; kk < DV; kk += 16) {
+          InA<T> left;
+          load_a<T, LDV>(left, dy, rg * 16, kk);
 #pragma unroll
-      for (int kk = 0; kk < DV; kk += 16) {
-        InA<T> left;
-        load_a<T, LDV>(left, dy, rg * 16, kk);
+          for (int n = 0; n < NK / 2; ++n) {
+            MadeB<T> right[2];
+            load_state<T, LDS, PLANE, false>(right, s_state, wc * NK * 8 + n * 16, kk);
+            mma(dq[2 * n], left, right[0]);
+            mma(dq[2 * n + 1], left, right[1]);
+          }
+        }
+        const float b0 = before[i0] * p.scale, b1 = before[i0 + 8] * p.scale;
+        float far0 = 0.0f, far1 = 0.0f;
 #pragma unroll
-        for (int n = 0; n < C / 16; ++n) {
-          if (n > rg) break;
-          InB<T> right[2];
-          load_b<T, LDV, false>(right, v, n * 16, kk);
-          mma(d[2 * n], left, right[0]);
-          mma(d[2 * n + 1], left, right[1]);
+        for (int n = 0; n < NK; ++n) {
+          const int col = wc * NK * 8 + n * 8 + 2 * c;
+          const float2 q0 = two_of(q + i0 * LDK + col), q1 = two_of(q + (i0 + 8) * LDK + col);
+          dq[n][0] = decayed(b0, dq[n][0]), dq[n][1] = decayed(b0, dq[n][1]);
+          dq[n][2] = decayed(b1, dq[n][2]), dq[n][3] = decayed(b1, dq[n][3]);
+          far0 = fmaf(dq[n][0], q0.x, fmaf(dq[n][1], q0.y, far0));
+          far1 = fmaf(dq[n][2], q1.x, fmaf(dq[n][3], q1.y, far1));
         }
 #pragma unroll
-        for (int n = 0; n < NK / 2; ++n) {
-          MadeB<T> right[2];
-          load_state<T, LDS, PLANE, false>(right, s_state, wc * NK * 8 + n * 16, kk);
-          mma(out[2 * n], left, right[0]);
-          mma(out[2 * n + 1], left, right[1]);
+        for (int off = 1; off < 4; off <<= 1) {
+          far0 += __shfl_xor_sync(0xffffffffu, far0, off);
+          far1 += __shfl_xor_sync(0xffffffffu, far1, off);
+        }
+        if (c == 0) s_far[wc * C + i0] = far0, s_far[wc * C + i0 + 8] = far1;
+#pragma unroll 1
+        for (int n = 0; n <= rg; ++n) {
+          float d[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+          products<T, DV>(d, dy, rg * 16, v, n * 16);
+          float w[8], x[8];
+          weights_by_row(w, sums, tail, i0, n * 16, n == rg, p.scale);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = w[e] == 0.0f ? 0.0f : d[e >> 2][e & 3] * w[e];
+          Made<T> left;
+          make(left, x);
+#pragma unroll
+          for (int m = 0; m < NK / 2; ++m) {
+            InB<T> right[2];
+            load_b<T, LDK, true>(right, k, wc * NK * 8 + m * 16, n * 16);
+            mma(dq[2 * m], left, right[0]);
+            mma(dq[2 * m + 1], left, right[1]);
+          }
         }
       }
-      const float b0 = before[i0] * p.scale, b1 = before[i1] * p.scale;
-      float far0 = 0.0f, far1 = 0.0f;
+      store_rows<T>(p.dq, p, row, s0 + i0, p.key, wc * NK * 8 + 2 * c, dq);
+      if (live) {
+        // what passes the chunk whole
+        float all = 0.0f;
+        S.each([&](int r, int col, float& x, float& y) {
+          const float2 s = read_state<T, LDS, PLANE>(s_state, r, col);
+          all = fmaf(x, s.x, fmaf(y, s.y, all));
+        });
 #pragma unroll
-      for (int n = 0; n < NK; ++n) {
-        const int col = wc * NK * 8 + n * 8 + 2 * c;
-        out[n][0] = decayed(b0, out[n][0]), out[n][1] = decayed(b0, out[n][1]);
-        out[n][2] = decayed(b1, out[n][2]), out[n][3] = decayed(b1, out[n][3]);
-        far0 = fmaf(out[n][0], widen(q[i0 * LDK + col]), fmaf(out[n][1], widen(q[i0 * LDK + col + 1]), far0));
-        far1 = fmaf(out[n][2], widen(q[i1 * LDK + col]), fmaf(out[n][3], widen(q[i1 * LDK + col + 1]), far1));
+        for (int off = 1; off < 32; off <<= 1) all += __shfl_xor_sync(0xffffffffu, all, off);
+        if (lane == 0) s_all[warp] = decayed(before[C - 1], all);
+        S.template update<T, C>(q, dy, before, before[C - 1], p.scale);
       }
-#pragma unroll
-      for (int off = 1; off < 4; off <<= 1) {
-        far0 += __shfl_xor_sync(0xffffffffu, far0, off);
-        far1 += __shfl_xor_sync(0xffffffffu, far1, off);
-      }
-      if (c == 0) s_far[wc * C + i0] = far0, s_far[wc * C + i1] = far1;
-#pragma unroll
-      for (int n = 0; n < C / 16; ++n) {
-        if (n > rg) break;
-        float x[8];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int j = n * 16 + half * 8 + 2 * c;
-          const float4 two = *reinterpret_cast<const float4*>(sums + j);
-          const float2 s0j = make_float2(two.x, two.y), s1j = make_float2(two.z, two.w);
-          const float(&at)[4] = d[2 * n + half];
-          x[4 * half] = j <= i0 ? at[0] * (p.scale * between(sum0, s0j)) : 0.0f;
-          x[4 * half + 1] = j + 1 <= i0 ? at[1] * (p.scale * between(sum0, s1j)) : 0.0f;
-          x[4 * half + 2] = j <= i1 ? at[2] * (p.scale * between(sum1, s0j)) : 0.0f;
-          x[4 * half + 3] = j + 1 <= i1 ? at[3] * (p.scale * between(sum1, s1j)) : 0.0f;
-        }
-        Made<T> left;
-        make(left, x);
-#pragma unroll
-        for (int m = 0; m < NK / 2; ++m) {
-          InB<T> right[2];
-          load_b<T, LDK, true>(right, k, wc * NK * 8 + m * 16, n * 16);
-          mma(out[2 * m], left, right[0]);
-          mma(out[2 * m + 1], left, right[1]);
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < NK; ++n) put(p.dq, p.key, wc * NK * 8 + n * 8 + 2 * c, out[n]);
-    }
-    if (live) {
-      // by rows j: dV and dK
-      float a[C / 8][4], d[C / 8][4], dv[NV][4], dk[NK][4];
-#pragma unroll
-      for (int n = 0; n < C / 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) a[n][e] = d[n][e] = 0.0f;
+    } else {
+      float dv[NV][4], dk[NK][4];
 #pragma unroll
       for (int n = 0; n < NV; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) dv[n][e] = 0.0f;
 #pragma unroll
-      for (int kk = 0; kk < DK; kk += 16) {
-        InA<T> left;
-        load_a<T, LDK>(left, k, rg * 16, kk);
-#pragma unroll
-        for (int n = 0; n < C / 16; ++n) {
-          if (n < rg) continue;
-          InB<T> right[2];
-          load_b<T, LDK, false>(right, q, n * 16, kk);
-          mma(a[2 * n], left, right[0]);
-          mma(a[2 * n + 1], left, right[1]);
-        }
-#pragma unroll
-        for (int n = 0; n < NV / 2; ++n) {
-          MadeB<T> right[2];
-          load_state<T, LDS, PLANE, true>(right, s_grad, wc * NV * 8 + n * 16, kk);
-          mma(dv[2 * n], left, right[0]);
-          mma(dv[2 * n + 1], left, right[1]);
-        }
-      }
-      const float w0 = after[i0], w1 = after[i1];
-#pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        dv[n][0] = decayed(w0, dv[n][0]), dv[n][1] = decayed(w0, dv[n][1]);
-        dv[n][2] = decayed(w1, dv[n][2]), dv[n][3] = decayed(w1, dv[n][3]);
-      }
-#pragma unroll
       for (int n = 0; n < NK; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) dk[n][e] = 0.0f;
+      if (live) {
+#pragma unroll kUnroll<T>
+        for (int kk = 0; kk < DK; kk += 16) {
+          InA<T> left;
+          load_a<T, LDK>(left, k, rg * 16, kk);
 #pragma unroll
-      for (int kk = 0; kk < DV; kk += 16) {
-        InA<T> left;
-        load_a<T, LDV>(left, v, rg * 16, kk);
-#pragma unroll
-        for (int n = 0; n < C / 16; ++n) {
-          if (n < rg) continue;
-          InB<T> right[2];
-          load_b<T, LDV, false>(right, dy, n * 16, kk);
-          mma(d[2 * n], left, right[0]);
-          mma(d[2 * n + 1], left, right[1]);
-        }
-#pragma unroll
-        for (int n = 0; n < NK / 2; ++n) {
-          MadeB<T> right[2];
-          load_state<T, LDS, PLANE, false>(right, s_grad, wc * NK * 8 + n * 16, kk);
-          mma(dk[2 * n], left, right[0]);
-          mma(dk[2 * n + 1], left, right[1]);
-        }
-      }
-      float end0 = 0.0f, end1 = 0.0f;
-#pragma unroll
-      for (int n = 0; n < NK; ++n) {
-        const int col = wc * NK * 8 + n * 8 + 2 * c;
-        dk[n][0] = decayed(w0, dk[n][0]), dk[n][1] = decayed(w0, dk[n][1]);
-        dk[n][2] = decayed(w1, dk[n][2]), dk[n][3] = decayed(w1, dk[n][3]);
-        end0 = fmaf(dk[n][0], widen(k[i0 * LDK + col]), fmaf(dk[n][1], widen(k[i0 * LDK + col + 1]), end0));
-        end1 = fmaf(dk[n][2], widen(k[i1 * LDK + col]), fmaf(dk[n][3], widen(k[i1 * LDK + col + 1]), end1));
-      }
-      float col0 = 0.0f, col1 = 0.0f;  // sums of W over i, of j = i0 and i1
-#pragma unroll
-      for (int n = 0; n < C / 16; ++n) {
-        if (n < rg) continue;
-        float x[8], z[8];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int i = n * 16 + half * 8 + 2 * c;
-          const float4 two = *reinterpret_cast<const float4*>(sums + i);
-          const float2 s0i = make_float2(two.x, two.y), s1i = make_float2(two.z, two.w);
-          const float f0 = i0 <= i ? p.scale * between(s0i, sum0) : 0.0f, f1 = i0 <= i + 1 ? p.scale * between(s1i, sum0) : 0.0f;
-          const float f2 = i1 <= i ? p.scale * between(s0i, sum1) : 0.0f, f3 = i1 <= i + 1 ? p.scale * between(s1i, sum1) : 0.0f;
-          const float(&at)[4] = a[2 * n + half];
-          const float(&to)[4] = d[2 * n + half];
-          x[4 * half] = f0 == 0.0f ? 0.0f : at[0] * f0, x[4 * half + 1] = f1 == 0.0f ? 0.0f : at[1] * f1;
-          x[4 * half + 2] = f2 == 0.0f ? 0.0f : at[2] * f2, x[4 * half + 3] = f3 == 0.0f ? 0.0f : at[3] * f3;
-          z[4 * half] = f0 == 0.0f ? 0.0f : to[0] * f0, z[4 * half + 1] = f1 == 0.0f ? 0.0f : to[1] * f1;
-          z[4 * half + 2] = f2 == 0.0f ? 0.0f : to[2] * f2, z[4 * half + 3] = f3 == 0.0f ? 0.0f : to[3] * f3;
-          const float u0 = i == i0 ? 0.0f : x[4 * half] * to[0], u1 = i + 1 == i0 ? 0.0f : x[4 * half + 1] * to[1];
-          const float u2 = i == i1 ? 0.0f : x[4 * half + 2] * to[2], u3 = i + 1 == i1 ? 0.0f : x[4 * half + 3] * to[3];
-          if (wc == 0) {
-            col0 += u0 + u1, col1 += u2 + u3;
-            float r0 = u0 + u2, r1 = u1 + u3;
-#pragma unroll
-            for (int off = 4; off < 32; off <<= 1) {
-              r0 += __shfl_xor_sync(0xffffffffu, r0, off);
-              r1 += __shfl_xor_sync(0xffffffffu, r1, off);
-            }
-            if (g == 0) s_row[rg * C + i] = r0, s_row[rg * C + i + 1] = r1;
+          for (int n = 0; n < NV / 2; ++n) {
+            MadeB<T> right[2];
+            load_state<T, LDS, PLANE, true>(right, s_grad, wc * NV * 8 + n * 16, kk);
+            mma(dv[2 * n], left, right[0]);
+            mma(dv[2 * n + 1], left, right[1]);
           }
         }
-        Made<T> left;
-        make(left, x);
+#pragma unroll kUnroll<T>
+        for (int kk = 0; kk < DV; kk += 16) {
+          InA<T> left;
+          load_a<T, LDV>(left, v, rg * 16, kk);
 #pragma unroll
-        for (int m = 0; m < NV / 2; ++m) {
-          InB<T> right[2];
-          load_b<T, LDV, true>(right, dy, wc * NV * 8 + m * 16, n * 16);
-          mma(dv[2 * m], left, right[0]);
-          mma(dv[2 * m + 1], left, right[1]);
+          for (int n = 0; n < NK / 2; ++n) {
+            MadeB<T> right[2];
+            load_state<T, LDS, PLANE, false>(right, s_grad, wc * NK * 8 + n * 16, kk);
+            mma(dk[2 * n], left, right[0]);
+            mma(dk[2 * n + 1], left, right[1]);
+          }
         }
-        make(left, z);
+        const float w0 = after[i0], w1 = after[i0 + 8];
 #pragma unroll
-        for (int m = 0; m < NK / 2; ++m) {
-          InB<T> right[2];
-          load_b<T, LDK, true>(right, q, wc * NK * 8 + m * 16, n * 16);
-          mma(dk[2 * m], left, right[0]);
-          mma(dk[2 * m + 1], left, right[1]);
+        for (int n = 0; n < NV; ++n) {
+          dv[n][0] = decayed(w0, dv[n][0]), dv[n][1] = decayed(w0, dv[n][1]);
+          dv[n][2] = decayed(w1, dv[n][2]), dv[n][3] = decayed(w1, dv[n][3]);
+        }
+        float end0 = 0.0f, end1 = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NK; ++n) {
+          const int col = wc * NK * 8 + n * 8 + 2 * c;
+          const float2 k0 = two_of(k + i0 * LDK + col), k1 = two_of(k + (i0 + 8) * LDK + col);
+          dk[n][0] = decayed(w0, dk[n][0]), dk[n][1] = decayed(w0, dk[n][1]);
+          dk[n][2] = decayed(w1, dk[n][2]), dk[n][3] = decayed(w1, dk[n][3]);
+          end0 = fmaf(dk[n][0], k0.x, fmaf(dk[n][1], k0.y, end0));
+          end1 = fmaf(dk[n][2], k1.x, fmaf(dk[n][3], k1.y, end1));
+        }
+        float col0 = 0.0f, col1 = 0.0f;  // sums of W over i, of j = i0 and i0 + 8
+#pragma unroll 1
+        for (int n = rg; n < RG; ++n) {
+          float a[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+          float d[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+          products<T, DK>(a, k, rg * 16, q, n * 16);
+          products<T, DV>(d, v, rg * 16, dy, n * 16);
+          float w[8], x[8], z[8];
+          weights_by_column(w, sums, tail, i0, n * 16, rg * 16, n == rg, p.scale);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            x[e] = w[e] == 0.0f ? 0.0f : a[e >> 2][e & 3] * w[e];
+            z[e] = w[e] == 0.0f ? 0.0f : d[e >> 2][e & 3] * w[e];
+          }
+          if (wc == 0) {
+            const bool same = n == rg;  // (W has no diagonal)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const int i = n * 16 + half * 8 + 2 * c;
+              const float u0 = same && i == i0 ? 0.0f : x[4 * half] * d[half][0];
+              const float u1 = same && i + 1 == i0 ? 0.0f : x[4 * half + 1] * d[half][1];
+              const float u2 = same && i == i0 + 8 ? 0.0f : x[4 * half + 2] * d[half][2];
+              const float u3 = same && i + 1 == i0 + 8 ? 0.0f : x[4 * half + 3] * d[half][3];
+              col0 += u0 + u1, col1 += u2 + u3;
+              float r0 = u0 + u2, r1 = u1 + u3;
+#pragma unroll
+              for (int off = 4; off < 32; off <<= 1) {
+                r0 += __shfl_xor_sync(0xffffffffu, r0, off);
+                r1 += __shfl_xor_sync(0xffffffffu, r1, off);
+              }
+              if (g == 0) *reinterpret_cast<float2*>(s_row + rg * C + i) = make_float2(r0, r1);
+            }
+          }
+          Made<T> left;
+          make(left, x);
+#pragma unroll
+          for (int m = 0; m < NV / 2; ++m) {
+            InB<T> right[2];
+            load_b<T, LDV, true>(right, dy, wc * NV * 8 + m * 16, n * 16);
+            mma(dv[2 * m], left, right[0]);
+            mma(dv[2 * m + 1], left, right[1]);
+          }
+          make(left, z);
+#pragma unroll
+          for (int m = 0; m < NK / 2; ++m) {
+            InB<T> right[2];
+            load_b<T, LDK, true>(right, q, wc * NK * 8 + m * 16, n * 16);
+            mma(dk[2 * m], left, right[0]);
+            mma(dk[2 * m + 1], left, right[1]);
+          }
+        }
+#pragma unroll
+        for (int off = 1; off < 4; off <<= 1) {
+          end0 += __shfl_xor_sync(0xffffffffu, end0, off);
+          end1 += __shfl_xor_sync(0xffffffffu, end1, off);
+          col0 += __shfl_xor_sync(0xffffffffu, col0, off);
+          col1 += __shfl_xor_sync(0xffffffffu, col1, off);
+        }
+        if (c == 0) {
+          s_end[wc * C + i0] = end0, s_end[wc * C + i0 + 8] = end1;
+          if (wc == 0) s_col[i0] = col0, s_col[i0 + 8] = col1;
         }
       }
-#pragma unroll
-      for (int off = 1; off < 4; off <<= 1) {
-        end0 += __shfl_xor_sync(0xffffffffu, end0, off);
-        end1 += __shfl_xor_sync(0xffffffffu, end1, off);
-        col0 += __shfl_xor_sync(0xffffffffu, col0, off);
-        col1 += __shfl_xor_sync(0xffffffffu, col1, off);
-      }
-      if (c == 0) {
-        s_end[wc * C + i0] = end0, s_end[wc * C + i1] = end1;
-        if (wc == 0) s_col[i0] = col0, s_col[i1] = col1;
-      }
-#pragma unroll
-      for (int n = 0; n < NV; ++n) put(p.dv, p.value, wc * NV * 8 + n * 8 + 2 * c, dv[n]);
-#pragma unroll
-      for (int n = 0; n < NK; ++n) put(p.dk, p.key, wc * NK * 8 + n * 8 + 2 * c, dk[n]);
-      // what passes the chunk whole
-      float all = 0.0f;
-      S.each([&](int r, int col, float& x, float& y) {
-        const float2 s = read_state<T, LDS, PLANE>(s_state, r, col);
-        all = fmaf(x, s.x, fmaf(y, s.y, all));
-      });
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) all += __shfl_xor_sync(0xffffffffu, all, off);
-      if (lane == 0) s_all[warp] = decayed(before[C - 1], all);
-      S.template update<T, C>(q, dy, before, before[C - 1], p.scale);
-    } else {
-      const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int n = 0; n < NK; ++n) {
-        put(p.dq, p.key, wc * NK * 8 + n * 8 + 2 * c, zero);
-        put(p.dk, p.key, wc * NK * 8 + n * 8 + 2 * c, zero);
-      }
-#pragma unroll
-      for (int n = 0; n < NV; ++n) put(p.dv, p.value, wc * NV * 8 + n * 8 + 2 * c, zero);
+      store_rows<T>(p.dv, p, row, s0 + i0, p.value, wc * NV * 8 + 2 * c, dv);
+      store_rows<T>(p.dk, p, row, s0 + i0, p.key, wc * NK * 8 + 2 * c, dk);
     }
     __syncthreads();  // the chunk's tiles, states and sums are read or written
+    if (chunk > c0) load(chunk - 1);
+    if (by_rows && live) S.template publish<T>(s_grad);
     if (warp == WARPS - 1) {
       // the decays' gradients: prefix sums over the chunk's steps in 64 bits
       constexpr int E = C / 32;
       double back = 0.0, ahead = 0.0, own_back[E], own_ahead[E], through = 0.0;
       if (live) {
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) through += s_all[w];
+        for (int w = 0; w < SIDE; ++w) through += s_all[w];
       }
 #pragma unroll
       for (int e = 0; e < E; ++e) {
@@ -1222,10 +1274,8 @@ __global__ void __launch_bounds__(32 * kBackWarps<T, DK, DV>) backward_kernel(co
       }
       if (chunk > c0) store(chunk - 1);
     }
-    if (live) S.template publish<T>(s_grad);
-    if (chunk > c0) load(chunk - 1);
   }
-  if (p.dstate && part == 0) S.write(p.dstate + index * p.key * p.value, p.key, p.value, 0);
+  if (by_rows && p.dstate && part == 0) S.write(p.dstate + index * p.key * p.value, p.key, p.value, 0);
 }
 
 // ---------------------------------------------------------------------------------------- single steps

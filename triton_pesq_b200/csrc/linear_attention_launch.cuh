@@ -46,7 +46,7 @@ cudaError_t forward_of(const Args& p, const Geometry& g, Kind kind, cudaStream_t
 template <class T, int DK, int DV>
 cudaError_t launch_backward(const Args& p, const Geometry& g, cudaStream_t s) {
   constexpr int dtype = std::is_same<T, float>::value ? PESQ_F32 : PESQ_BF16, C = chunk_of(dtype, DK, DV);
-  return start(backward_kernel<T, DK, DV, C>, p, g.blocks, 32 * kBackWarps<T, DK, DV>, BackwardShared<T, DK, DV, C>::kBytes, s);
+  return start(backward_kernel<T, DK, DV, C>, p, g.blocks, 64 * kSide<T, DK, DV>, BackwardShared<T, DK, DV, C>::kBytes, s);
 }
 template <class T, int DK>
 cudaError_t backward_width(const Args& p, const Geometry& g, cudaStream_t s) {
