@@ -100,12 +100,12 @@ __device__ __forceinline__ void ldmatrix(uint32_t (&r)[4], const void* p) {
                  : "r"(smem_of(p)) : "memory");
 }
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
@@ -114,7 +114,7 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], c
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[8], const uint32_t (&b)[4]) {
 #pragma unroll
   for (int s = 0; s < 2; ++s)
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[4 * s]), "r"(a[4 * s + 2]), "r"(a[4 * s + 1]), "r"(a[4 * s + 3]), "r"(b[2 * s]), "r"(b[2 * s + 1]));
 }
@@ -542,6 +542,20 @@ __device__ __forceinline__ void weights_by_column(float (&w)[8], const float2* s
 // a factor of zero cuts off whatever it multiplies
 __device__ __forceinline__ float decayed(float factor, float x) { return factor == 0.0f ? 0.0f : factor * x; }
 
+// 16 rows of N times 8 columns times their rows' factors
+template <int N>
+__device__ __forceinline__ void decay_rows(float (&x)[N][4], float f0, float f1) {
+  if (__any_sync(0xffffffffu, f0 == 0.0f || f1 == 0.0f)) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      if (f0 == 0.0f) x[n][0] = x[n][1] = 0.0f;
+      if (f1 == 0.0f) x[n][2] = x[n][3] = 0.0f;
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < N; ++n) x[n][0] *= f0, x[n][1] *= f0, x[n][2] *= f1, x[n][3] *= f1;
+}
+
 // A warp's part of a DK x DV state: kTiles tiles of 16 rows, kCols columns
 template <int DK, int DV, int WARPS>
 struct StateShape {
@@ -590,6 +604,14 @@ struct State {
   template <class T, int C>
   __device__ __forceinline__ void update(const T* a, const T* b, const float* weights, float factor, float scale) {
     const int c = threadIdx.x & 3;
+    if (factor == 0.0f) {  // (cuts off whatever the state holds)
+#pragma unroll
+      for (int m = 0; m < Shape::kTiles; ++m)
+#pragma unroll
+        for (int n = 0; n < Shape::kCols / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[m][n][e] = 0.0f;
+    }
     constexpr int kBlocks = C / 16, kTogether = std::is_same<T, __nv_bfloat16>::value ? kBlocks : 2;  // of registers' worth
 #pragma unroll
     for (int m = 0; m < Shape::kTiles; ++m) {
@@ -622,7 +644,7 @@ struct State {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               float& s = x[m][2 * n + half][e];
-              s = (k0 == 0 ? decayed(factor, s) : s) + sum[half][e];
+              s = k0 == 0 ? fmaf(factor, s, sum[half][e]) : s + sum[half][e];
             }
         }
       }
@@ -638,6 +660,17 @@ struct State {
 // Bytes of the state before a chunk: two planes of 16 bits, or 32, of [DK][DV]
 __host__ __device__ constexpr int64_t kept_bytes(int DK, int DV) { return (int64_t)4 * DK * DV; }
 
+__device__ __forceinline__ uint32_t narrow_pair(float x, float y, __nv_bfloat16) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t narrow_pair(float x, float y, __half) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+  return r;
+}
+__device__ __forceinline__ float2 narrow_pair(float x, float y, float) { return make_float2(x, y); }
 // A warp's 16 rows of N times 8 columns from col (the thread's first) to rows of `width`: those of steps s and s + 8, where
 // they are within the row; zeros past its length
 template <class T, int N>
@@ -650,11 +683,15 @@ __device__ __forceinline__ void store_rows(void* base, const Args& p, const Row&
     T* to = static_cast<T*>(base) + ((row.b * row.steps + row.time(at)) * p.heads + row.h) * width + col;
     const int left = width - col;
     if (width % 2 == 0) {
+      using Pair = decltype(narrow_pair(0.0f, 0.0f, T{}));
+      Pair* pairs = reinterpret_cast<Pair*>(to);
+      if (live && (N - 1) * 8 < left) {
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
-        Pack<T, 2> v;
-        v.v[0] = narrow<T>(live ? x[n][2 * half] : 0.0f), v.v[1] = narrow<T>(live ? x[n][2 * half + 1] : 0.0f);
-        if (n * 8 < left) *reinterpret_cast<Pack<T, 2>*>(to + n * 8) = v;
+        for (int n = 0; n < N; ++n) pairs[n * 4] = narrow_pair(x[n][2 * half], x[n][2 * half + 1], T{});
+      } else {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+          if (n * 8 < left) pairs[n * 4] = narrow_pair(live ? x[n][2 * half] : 0.0f, live ? x[n][2 * half + 1] : 0.0f, T{});
       }
     } else {
 #pragma unroll
@@ -699,24 +736,19 @@ __device__ __forceinline__ void products(float (&sum)[2][4], const T* a, int m0,
 
 // ------------------------------------------------------------------------------------------- forward
 
-#ifndef FWD_LIMIT
-#define FWD_LIMIT 55
-#endif
-#ifndef FWD_CTAS
-#define FWD_CTAS 4
-#endif
 template <class T, int DK, int DV, int C>
 struct ForwardShared {
   static constexpr int kTiles = (2 * C * kLd<T, DK> + C * kLd<T, DV>) * (int)sizeof(T);
   static constexpr int kState = kPlanes<T> * DK * kLd<Stored<T>, DV> * (int)sizeof(Stored<T>);
   static constexpr int kDecays = kDecayBytes<C>;
-  // the next chunk's tiles come in while one is worked on, where four CTAs an SM have the room
-  static constexpr int kStages = 2 * kTiles + kState + kDecays <= (FWD_LIMIT << 10) ? 2 : 1;
+  // the next chunk's tiles come in while one is worked on, where three CTAs an SM have the room (896 rows of 500 steps 159 us
+  // forward, four CTAs with one set of tiles 169; 448 rows 99 and 87)
+  static constexpr int kStages = 2 * kTiles + kState + kDecays <= (75 << 10) ? 2 : 1;
   static constexpr int kBytes = kStages * kTiles + kState + kDecays;
 };
 
 template <class T, int DK, int DV, int C>
-__global__ void __launch_bounds__(128, DK == 128 ? 2 : FWD_CTAS) forward_kernel(const __grid_constant__ Args p) {
+__global__ void __launch_bounds__(128, DK > 64 ? 2 : 3) forward_kernel(const __grid_constant__ Args p) {
   constexpr int THREADS = 128, WARPS = 4, RG = C / 16, WC = WARPS / RG, NY = DV / WC / 8;
   using Sh = ForwardShared<T, DK, DV, C>;
   constexpr int LDK = kLd<T, DK>, LDV = kLd<T, DV>, LDS = kLd<Stored<T>, DV>, PLANE = DK * LDS;
@@ -804,12 +836,7 @@ __global__ void __launch_bounds__(128, DK == 128 ? 2 : FWD_CTAS) forward_kernel(
           mma(y[2 * n + 1], left, right[1]);
         }
       }
-      const float b0 = before[i0] * p.scale, b1 = before[i0 + 8] * p.scale;
-#pragma unroll
-      for (int n = 0; n < NY; ++n) {
-        y[n][0] = decayed(b0, y[n][0]), y[n][1] = decayed(b0, y[n][1]);
-        y[n][2] = decayed(b1, y[n][2]), y[n][3] = decayed(b1, y[n][3]);
-      }
+      decay_rows(y, before[i0] * p.scale, before[i0 + 8] * p.scale);
       // sixteen steps j at a time, up to the warp's own
 #pragma unroll 1
       for (int n = 0; n <= rg; ++n) {
@@ -818,7 +845,7 @@ __global__ void __launch_bounds__(128, DK == 128 ? 2 : FWD_CTAS) forward_kernel(
         float w[8], x[8];
         weights_by_row(w, sums, tail, i0, n * 16, n == rg, p.scale);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = w[e] == 0.0f ? 0.0f : a[e >> 2][e & 3] * w[e];
+        for (int e = 0; e < 8; ++e) x[e] = a[e >> 2][e & 3] * w[e];
         Made<T> left;
         make(left, x);
 #pragma unroll
@@ -1059,14 +1086,12 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
             mma(dq[2 * n + 1], left, right[1]);
           }
         }
-        const float b0 = before[i0] * p.scale, b1 = before[i0 + 8] * p.scale;
+        decay_rows(dq, before[i0] * p.scale, before[i0 + 8] * p.scale);
         float far0 = 0.0f, far1 = 0.0f;
 #pragma unroll
         for (int n = 0; n < NK; ++n) {
           const int col = wc * NK * 8 + n * 8 + 2 * c;
           const float2 q0 = two_of(q + i0 * LDK + col), q1 = two_of(q + (i0 + 8) * LDK + col);
-          dq[n][0] = decayed(b0, dq[n][0]), dq[n][1] = decayed(b0, dq[n][1]);
-          dq[n][2] = decayed(b1, dq[n][2]), dq[n][3] = decayed(b1, dq[n][3]);
           far0 = fmaf(dq[n][0], q0.x, fmaf(dq[n][1], q0.y, far0));
           far1 = fmaf(dq[n][2], q1.x, fmaf(dq[n][3], q1.y, far1));
         }
@@ -1083,7 +1108,7 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
           float w[8], x[8];
           weights_by_row(w, sums, tail, i0, n * 16, n == rg, p.scale);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = w[e] == 0.0f ? 0.0f : d[e >> 2][e & 3] * w[e];
+          for (int e = 0; e < 8; ++e) x[e] = d[e >> 2][e & 3] * w[e];
           Made<T> left;
           make(left, x);
 #pragma unroll
@@ -1143,19 +1168,13 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
             mma(dk[2 * n + 1], left, right[1]);
           }
         }
-        const float w0 = after[i0], w1 = after[i0 + 8];
-#pragma unroll
-        for (int n = 0; n < NV; ++n) {
-          dv[n][0] = decayed(w0, dv[n][0]), dv[n][1] = decayed(w0, dv[n][1]);
-          dv[n][2] = decayed(w1, dv[n][2]), dv[n][3] = decayed(w1, dv[n][3]);
-        }
+        decay_rows(dv, after[i0], after[i0 + 8]);
+        decay_rows(dk, after[i0], after[i0 + 8]);
         float end0 = 0.0f, end1 = 0.0f;
 #pragma unroll
         for (int n = 0; n < NK; ++n) {
           const int col = wc * NK * 8 + n * 8 + 2 * c;
           const float2 k0 = two_of(k + i0 * LDK + col), k1 = two_of(k + (i0 + 8) * LDK + col);
-          dk[n][0] = decayed(w0, dk[n][0]), dk[n][1] = decayed(w0, dk[n][1]);
-          dk[n][2] = decayed(w1, dk[n][2]), dk[n][3] = decayed(w1, dk[n][3]);
           end0 = fmaf(dk[n][0], k0.x, fmaf(dk[n][1], k0.y, end0));
           end1 = fmaf(dk[n][2], k1.x, fmaf(dk[n][3], k1.y, end1));
         }
@@ -1170,8 +1189,8 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
           weights_by_column(w, sums, tail, i0, n * 16, rg * 16, n == rg, p.scale);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            x[e] = w[e] == 0.0f ? 0.0f : a[e >> 2][e & 3] * w[e];
-            z[e] = w[e] == 0.0f ? 0.0f : d[e >> 2][e & 3] * w[e];
+            x[e] = a[e >> 2][e & 3] * w[e];
+            z[e] = d[e >> 2][e & 3] * w[e];
           }
           if (wc == 0) {
             const bool same = n == rg;  // (W has no diagonal)
