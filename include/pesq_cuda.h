@@ -508,8 +508,8 @@ typedef struct pesq_linear_attention_desc {
 } pesq_linear_attention_desc;
 
 /* Bytes (16-byte aligned buffers) of a forward's workspace, of the states it
- * keeps for a backward call, and of the backward's workspace; they follow from
- * the sizes, the type and decay_shared. */
+ * keeps for a backward call, and of the backward's workspace; the states follow from
+ * the sizes and the type alone. */
 int pesq_linear_attention_sizes(const pesq_linear_attention_desc* desc, size_t* forward, size_t* kept, size_t* backward);
 /* y: [batch, steps, heads, value] dense; last: [batch, heads, key, value], the
  * state after the last step, or NULL; kept: for the backward call, or NULL. */

@@ -3,9 +3,9 @@
 //
 //   y = h weight + bias,   h = (x - mean(x)) / sqrt(mean((x - mean(x))^2) + eps)
 //
-// A team of threads keeps a row in registers, eight channels a thread, as the join of norm_join.cuh does: x
+// A team of threads keeps a row in registers, up to 32 channels a thread in groups of eight: x
 // is read once, the mean subtracted before the squares are summed (two rounds of sums), and the next row is on its
-// way while one is worked on.  The backward recomputes the statistics instead of reading them, and takes with
+// way while one is worked on.  A warp is a team for up to 1024 channels, so that its sums are shuffles without barriers.  The backward recomputes the statistics instead of reading them, and takes with
 // q = dy weight the second round's three sums together:
 //
 //   dx = (q - mean(q) - h mean(q h)) / sqrt(..),   dweight = sum over rows of dy h,   dbias = of dy
@@ -29,13 +29,13 @@ using njoin::team_sum;
 constexpr int kThreads = 128;  // of a CTA, unless a row takes more
 
 // An operand's rows: strides of batch, step and head in elements
-struct Rows {
+struct Strided {
   const void* p;
   int64_t sb, st, sh;
 };
 
 struct Args {
-  Rows x, dy;
+  Strided x, dy;
   const float *weight, *bias;  // [heads, width]; bias may be null
   int64_t batch, steps;
   int heads, width;
@@ -50,10 +50,27 @@ struct Args {
 };
 
 // CTAs that an SM holds, which the registers of a thread follow from
-constexpr int ctas(bool backward, int team) {
-  const int threads = team > kThreads ? team : kThreads, sm = backward ? 512 : 1024;
+constexpr int ctas(bool backward, int team, int groups) {
+  const int threads = team > kThreads ? team : kThreads, sm = groups == 4 ? (backward ? 256 : 384) : (backward ? 512 : 1024);
   return sm / threads > 0 ? sm / threads : 1;
 }
+
+// A thread's channels of a row: groups of eight, 8 TEAM channels apart
+template <class T, int TEAM, int GROUPS, bool kWide>
+struct Row {
+  using E = Eight<T, TEAM, kWide>;
+  static constexpr int kApart = kEach * TEAM;
+  E e[GROUPS];
+  __device__ __forceinline__ void load(const void* row, int width, bool take) {
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) e[g].load(static_cast<const T*>(row) + g * kApart, width - g * kApart, take);
+  }
+  __device__ __forceinline__ void store(void* base, int64_t row, int width) const {
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) e[g].store(base, row + g * kApart, width - g * kApart);
+  }
+  static __device__ __forceinline__ bool in(int g, int j, int width) { return E::column(j) < width - g * kApart; }
+};
 
 // The rows that a team works on in turn: those of one head, every kSlots-th of its CTA's
 template <int TEAM, int THREADS>
@@ -73,19 +90,19 @@ struct Turns {
   }
 };
 template <class T>
-__device__ __forceinline__ const char* place(const Rows& r, const Args& p, int64_t row, int head) {
+__device__ __forceinline__ const char* place(const Strided& r, const Args& p, int64_t row, int head) {
   // (one batch item where the items' rows lie as one run, so that most calls divide by nothing here)
   const int64_t b = p.batch == 1 ? 0 : row / p.steps, t = row - b * p.steps;
   return static_cast<const char*>(r.p) + (b * r.sb + t * r.st + head * r.sh) * (int64_t)sizeof(T);
 }
 
-template <class TX, class TY, int TEAM, bool kWide>
-__global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(false, TEAM))
+template <class TX, class TY, int TEAM, int GROUPS, bool kWide>
+__global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(false, TEAM, GROUPS))
     forward_kernel(const __grid_constant__ Args p) {
   constexpr int THREADS = TEAM > kThreads ? TEAM : kThreads, H = kEach / 2;
-  using X = Eight<TX, TEAM, kWide>;
-  using Y = Eight<TY, TEAM, kWide>;
-  using F = Eight<float, TEAM, kWide>;
+  using X = Row<TX, TEAM, GROUPS, kWide>;
+  using Y = Row<TY, TEAM, GROUPS, kWide>;
+  using F = Row<float, TEAM, GROUPS, kWide>;
   __shared__ __align__(16) float s_sum[2][32][8];
   int turn = 0;
   Turns<TEAM, THREADS> of(p);
@@ -103,26 +120,32 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(false,
     const bool on1 = next < of.end;
     X x1;
     x1.load(place<TX>(p.x, p, on1 ? next : 0, of.head), p.width, on1);
-    Vec<2> d[H], total = splat<2>(0.0f);
+    Vec<2> d[GROUPS][H], total = splat<2>(0.0f);
 #pragma unroll
-    for (int i = 0; i < H; ++i) total = total + x.two(2 * i);
+    for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+      for (int i = 0; i < H; ++i) total = total + x.e[g].two(2 * i);
     float sum[1] = {total.v[0] + total.v[1]};
     team_sum<1, TEAM>(sum, s_sum, turn);
     const float mean = sum[0] * inv;
     total = splat<2>(0.0f);
 #pragma unroll
-    for (int i = 0; i < H; ++i) {
+    for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) d[i].v[j] = X::column(2 * i + j) < p.width ? x.at(2 * i + j) - mean : 0.0f;
-      total = fma(d[i], d[i], total);
-    }
+      for (int i = 0; i < H; ++i) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) d[g][i].v[j] = X::in(g, 2 * i + j, p.width) ? x.e[g].at(2 * i + j) - mean : 0.0f;
+        total = fma(d[g][i], d[g][i], total);
+      }
     sum[0] = total.v[0] + total.v[1];
     team_sum<1, TEAM>(sum, s_sum, turn);
     const Vec<2> r = splat<2>(inverse_root(fmaf(sum[0], inv, p.eps)));
     if (on) {
       Y y;
 #pragma unroll
-      for (int i = 0; i < H; ++i) y.set(2 * i, fma(d[i] * r, weight.two(2 * i), bias.two(2 * i)));
+      for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+        for (int i = 0; i < H; ++i) y.e[g].set(2 * i, fma(d[g][i] * r, weight.e[g].two(2 * i), bias.e[g].two(2 * i)));
       y.store(p.y, (of.row * p.heads + of.head) * p.width, p.width);
     }
     x = x1, on = on1, of.row = next;
@@ -130,12 +153,15 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(false,
 }
 
 // What the CTA's teams of each head hold, added up, to the CTA's row of `part`
-template <int TEAM, int TEAMS, bool kWide>
-__device__ __forceinline__ void store_part(const Vec<2> (&v)[kEach / 2], float* part, const Args& p, float* s_part) {
-  using F = Eight<float, TEAM, kWide>;
+template <int TEAM, int GROUPS, int TEAMS, bool kWide>
+__device__ __forceinline__ void store_part(const Vec<2> (&v)[GROUPS][kEach / 2], float* part, const Args& p, float* s_part) {
+  using F = Row<float, TEAM, GROUPS, kWide>;
+  constexpr int kRow = kEach * TEAM * GROUPS;
   F f;
 #pragma unroll
-  for (int i = 0; i < kEach / 2; ++i) f.set(2 * i, v[i]);
+  for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+    for (int i = 0; i < kEach / 2; ++i) f.e[g].set(2 * i, v[g][i]);
   const int64_t unit = blockIdx.x / p.head_blocks;
   const int first = blockIdx.x % p.head_blocks * p.block_heads, heads = min(p.block_heads, p.heads - first);
   float* to = part + (unit * p.heads + first) * p.width;
@@ -143,35 +169,37 @@ __device__ __forceinline__ void store_part(const Vec<2> (&v)[kEach / 2], float* 
     f.store(to, 0, p.width);
     return;
   }
-  f.store(s_part, (int64_t)(threadIdx.x / TEAM) * kEach * TEAM, kEach * TEAM);
+  f.store(s_part, (int64_t)(threadIdx.x / TEAM) * kRow, kRow);
   __syncthreads();
   const int slots = TEAMS / p.block_heads;
   for (int c = threadIdx.x; c < heads * p.width; c += TEAM * TEAMS) {
     const int head = c / p.width, at = c - head * p.width;
     float t = 0.0f;
-    for (int w = 0; w < slots; ++w) t += s_part[(w * p.block_heads + head) * kEach * TEAM + at];
+    for (int w = 0; w < slots; ++w) t += s_part[(w * p.block_heads + head) * kRow + at];
     to[c] = t;
   }
   __syncthreads();
 }
 
-template <class TX, class TY, int TEAM, bool kWide>
-__global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(true, TEAM))
+template <class TX, class TY, int TEAM, int GROUPS, bool kWide>
+__global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(true, TEAM, GROUPS))
     backward_kernel(const __grid_constant__ Args p) {
   constexpr int THREADS = TEAM > kThreads ? TEAM : kThreads, TEAMS = THREADS / TEAM, H = kEach / 2;
-  using X = Eight<TX, TEAM, kWide>;
-  using Y = Eight<TY, TEAM, kWide>;
-  using F = Eight<float, TEAM, kWide>;
+  using X = Row<TX, TEAM, GROUPS, kWide>;
+  using Y = Row<TY, TEAM, GROUPS, kWide>;
+  using F = Row<float, TEAM, GROUPS, kWide>;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ __align__(16) float s_sum[2][32][8];
-  __shared__ __align__(16) float s_part[TEAMS > 1 ? THREADS * kEach : 4];
+  __shared__ __align__(16) float s_part[TEAMS > 1 ? THREADS * kEach * GROUPS : 4];
   int turn = 0;
   Turns<TEAM, THREADS> of(p);
   F weight;
   weight.load(p.weight + (int64_t)of.head * p.width, p.width, true);
-  Vec<2> acc_weight[H], acc_bias[H];
+  Vec<2> acc_weight[GROUPS][H], acc_bias[GROUPS][H];
 #pragma unroll
-  for (int i = 0; i < H; ++i) acc_weight[i] = acc_bias[i] = splat<2>(0.0f);
+  for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+    for (int i = 0; i < H; ++i) acc_weight[g][i] = acc_bias[g][i] = splat<2>(0.0f);
   const float inv = 1.0f / (float)p.width;
   const int64_t turns = (p.span + of.slots - 1) / of.slots;
   X x;
@@ -187,9 +215,11 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(true, 
     Y dy1;
     x1.load(place<TX>(p.x, p, on1 ? next : 0, of.head), p.width, on1);
     dy1.load(place<TY>(p.dy, p, on1 ? next : 0, of.head), p.width, on1);
-    Vec<2> d[H], total = splat<2>(0.0f);
+    Vec<2> d[GROUPS][H], total = splat<2>(0.0f);
 #pragma unroll
-    for (int i = 0; i < H; ++i) total = total + x.two(2 * i);
+    for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+      for (int i = 0; i < H; ++i) total = total + x.e[g].two(2 * i);
     float sum[1] = {total.v[0] + total.v[1]};
     team_sum<1, TEAM>(sum, s_sum, turn);
     const float mean = sum[0] * inv;
@@ -198,14 +228,16 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(true, 
 #pragma unroll
     for (int k3 = 0; k3 < 3; ++k3) part[k3] = splat<2>(0.0f);
 #pragma unroll
-    for (int i = 0; i < H; ++i) {
+    for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) d[i].v[j] = X::column(2 * i + j) < p.width ? x.at(2 * i + j) - mean : 0.0f;
-      const Vec<2> q = dy.two(2 * i) * weight.two(2 * i);
-      part[0] = fma(d[i], d[i], part[0]);
-      part[1] = part[1] + q;
-      part[2] = fma(q, d[i], part[2]);
-    }
+      for (int i = 0; i < H; ++i) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) d[g][i].v[j] = X::in(g, 2 * i + j, p.width) ? x.e[g].at(2 * i + j) - mean : 0.0f;
+        const Vec<2> q = dy.e[g].two(2 * i) * weight.e[g].two(2 * i);
+        part[0] = fma(d[g][i], d[g][i], part[0]);
+        part[1] = part[1] + q;
+        part[2] = fma(q, d[g][i], part[2]);
+      }
     float three[3];
 #pragma unroll
     for (int k3 = 0; k3 < 3; ++k3) three[k3] = part[k3].v[0] + part[k3].v[1];
@@ -215,21 +247,23 @@ __global__ void __launch_bounds__(TEAM > kThreads ? TEAM : kThreads, ctas(true, 
     const Vec<2> rr = splat<2>(r), mq = splat<2>(-three[1] * inv), mh = splat<2>(-three[2] * inv * r);
     X dx;
 #pragma unroll
-    for (int i = 0; i < H; ++i) {
-      const Vec<2> h = d[i] * rr, q = fma(dy.two(2 * i), weight.two(2 * i), mq);
-      dx.set(2 * i, rr * fma(h, mh, q));
-      acc_weight[i] = fma(dy.two(2 * i), h, acc_weight[i]);
-      acc_bias[i] = acc_bias[i] + dy.two(2 * i);
-    }
+    for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        const Vec<2> y = dy.e[g].two(2 * i), h = d[g][i] * rr, q = fma(y, weight.e[g].two(2 * i), mq);
+        dx.e[g].set(2 * i, rr * fma(h, mh, q));
+        acc_weight[g][i] = fma(y, h, acc_weight[g][i]);
+        acc_bias[g][i] = acc_bias[g][i] + y;
+      }
     if (on) dx.store(p.dx, (of.row * p.heads + of.head) * p.width, p.width);
     x = x1, dy = dy1, on = on1, of.row = next;
   }
-  store_part<TEAM, TEAMS, kWide>(acc_weight, p.part_weight, p, s_part);
-  if (p.part_bias) store_part<TEAM, TEAMS, kWide>(acc_bias, p.part_bias, p, s_part);
+  store_part<TEAM, GROUPS, TEAMS, kWide>(acc_weight, p.part_weight, p, s_part);
+  if (p.part_bias) store_part<TEAM, GROUPS, TEAMS, kWide>(acc_bias, p.part_bias, p, s_part);
 }
 
 struct Geometry {
-  int team;
+  int team, groups;  // threads of a row, eights of channels of a thread
   bool wide;
   int64_t blocks;
 };

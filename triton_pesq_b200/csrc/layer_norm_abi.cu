@@ -20,7 +20,7 @@ extern template cudaError_t launch<float, __half>(const Args&, const Geometry&, 
 
 namespace {
 
-constexpr int kMaxWidth = 8192;          // one CTA of 1024 threads holds a row
+constexpr int kMaxWidth = 8192;          // one CTA of 256 threads holds a row
 constexpr int64_t kMaxVector = 1 << 20;  // heads times channels
 
 // Columns of the CTAs' sums, in a fixed order: 32 columns a block, every thread a stride of the rows, then a tree.
@@ -81,11 +81,10 @@ bool wide(const pesq_heads& s, const pesq_layer_norm_desc& d, int dtype) {
 }
 bool wide(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-int team_of(int64_t width) {
-  int team = 4;
-  for (int t : {8, 16, 32, 64, 128, 256, 512, 1024})
-    if (team * kEach < width) team = t;
-  return team;
+// threads of a row, and eights of channels of each
+void team_of(int64_t width, Geometry& g) {
+  g.team = 4, g.groups = 1;
+  while (g.team * g.groups * kEach < width) (g.team < 32 || g.groups == 4 ? g.team : g.groups) *= 2;
 }
 
 struct Plan {
@@ -104,7 +103,7 @@ Plan plan(const pesq_layer_norm_desc& d, bool backward, const pesq_heads* dy) {
   const bool flat = joined(d.x, d) && joined(g, d);
   q.batch = flat ? 1 : d.batch;
   q.steps = flat ? d.batch * d.steps : d.steps;
-  q.g.team = team_of(d.width);
+  team_of(d.width, q.g);
   q.g.wide = d.width % kEach == 0 && wide(d.x, d, d.dtype) && wide(g, d, d.out_dtype) && wide(d.weight) && wide(d.bias);
   const int threads = std::max(q.g.team, kThreads), teams = threads / q.g.team;
   double best = -1.0;
@@ -115,7 +114,7 @@ Plan plan(const pesq_layer_norm_desc& d, bool backward, const pesq_heads* dy) {
   }
   const int slots = teams / q.block_heads;
   const int64_t rows = d.batch * d.steps;
-  const int64_t most = std::max<int64_t>(1, 148 * ctas(backward, q.g.team) / q.head_blocks);
+  const int64_t most = std::max<int64_t>(1, 148 * ctas(backward, q.g.team, q.g.groups) / q.head_blocks);
   const int64_t units = std::min<int64_t>(most, (rows + slots - 1) / slots);
   q.span = (rows + units - 1) / units;
   q.units = (rows + q.span - 1) / q.span;
@@ -128,7 +127,7 @@ size_t part_bytes(const pesq_layer_norm_desc& d) {
   return ((size_t)q.units * d.heads * d.width * 4 + 15) / 16 * 16;
 }
 
-Rows rows_of(const pesq_heads& s) { return {s.data, s.batch_stride, s.step_stride, s.head_stride}; }
+Strided rows_of(const pesq_heads& s) { return {s.data, s.batch_stride, s.step_stride, s.head_stride}; }
 
 Args arguments(const pesq_layer_norm_desc& d, const Plan& q) {
   Args a{};

@@ -23,6 +23,8 @@ namespace {
 
 constexpr int kMaxWidth = 128;  // of keys and of values
 constexpr int kFewSteps = 8;    // that single steps take, where no backward follows
+constexpr int kFewChunks = 6;   // that are not cut in parts
+constexpr int kRagged = 4;
 constexpr int kJoinThreads = 256;
 
 // The decay's gradient of a head: the chunks' sums of its rows, in a fixed order
@@ -70,8 +72,26 @@ struct Plan {
 
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 
-// Rows fill the device by themselves from about one CTA an SM; fewer are cut in parts of four chunks or more, as many as make
-// two CTAs an SM.
+// CTAs of a kernel that an SM holds: what their shared memory leaves, and their registers
+int resident(int dtype, const Geometry& g, bool backward) {
+  const int size = (int)element(dtype), pad = size == 2 ? 8 : 4;
+  const int state = dtype == PESQ_BF16 ? 2 * g.dk * (g.dv + 8) * 2 : g.dk * (g.dv + 4) * 4, sums = 60 * g.chunk;
+  const int wide = g.dk > 64 || (backward && g.dv > 64);
+  int bytes;
+  if (backward) {
+    bytes = 2 * g.chunk * (g.dk + g.dv + 2 * pad) * size + 2 * state + sums;
+  } else {
+    const int tiles = g.chunk * (2 * g.dk + g.dv + 3 * pad) * size;
+    bytes = (2 * tiles + state + 40 * g.chunk <= 75 << 10 ? 2 : 1) * tiles + state + 40 * g.chunk;
+  }
+  return std::max(1, std::min((228 << 10) / (bytes + 1024), (backward ? 2 : 3) - wide));
+}
+
+// Rows are cut in parts, as many as the device holds at once, where that is four times the rows or more forward
+// and twice backward: the parts' sweep and join take about 0.6 of a forward's time and 0.3 of a backward's, and some
+// 10 us (12 x 8 rows of 500 steps of 64 x 64 in bfloat16: one part 43 us, four 42; 128 rows: 43 and three 58; 16: 41 and eight 24).
+// Rows of different lengths are cut four times as often, since parts past a row's end leave their place to others (30
+// rows of up to 4001 steps of 96 x 128 in float16, trained: parts for one filling 953 us, for four 594).
 Plan plan(const pesq_linear_attention_desc& d, bool backward) {
   Plan q{};
   q.rows = d.batch * d.heads;
@@ -81,8 +101,9 @@ Plan plan(const pesq_linear_attention_desc& d, bool backward) {
   q.slices = dv / q.g.dv;
   q.g.chunk = chunk_of(d.dtype, dk, dv);
   q.chunks = (int)((d.steps + q.g.chunk - 1) / q.g.chunk);
-  const int64_t ctas = q.rows * q.slices;
-  const int64_t parts = ctas >= 148 ? 1 : std::min<int64_t>((2 * 148 + ctas - 1) / ctas, std::max(1, q.chunks / 4));
+  const int64_t ctas = q.rows * q.slices, room = 148 * resident(d.dtype, q.g, backward) / ctas;
+  const bool cut = q.chunks >= kFewChunks && room >= (backward ? 2 : 4);
+  const int64_t parts = cut ? std::min<int64_t>(d.lengths ? kRagged * room : room, q.chunks) : 1;
   q.part_chunks = (int)((q.chunks + parts - 1) / parts);
   q.parts = (q.chunks + q.part_chunks - 1) / q.part_chunks;
   q.g.blocks = ctas * q.parts;

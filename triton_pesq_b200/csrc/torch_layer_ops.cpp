@@ -25,10 +25,14 @@ struct NormCall {
   pesq_layer_norm_desc d{};
   at::ScalarType out;
 
-  // x [batch, step, head, channel], weight and bias [head, channel]
+  // x [..., channel], weight and bias [channel]; or [..., head, channel] and [head, channel]
   NormCall(const at::Tensor& x_, const at::Tensor& weight_, const OptTensor& bias_, double eps, int64_t dtype) {
     check_cuda(x_, x_, kNorm, "x");
-    TORCH_CHECK(x_.dim() == 4, "The CUDA layer norm needs `x` [batch, step, head, channel], got ", x_.sizes(), ".");
+    const int64_t dims = x_.dim(), own = weight_.dim();
+    TORCH_CHECK_VALUE(own == 1 || own == 2, "The CUDA layer norm needs `weight` [channel] or [head, channel], got ",
+                      weight_.sizes(), ".");
+    TORCH_CHECK_VALUE(dims >= own && x_.sizes().slice(dims - own) == weight_.sizes(),
+                      "The CUDA layer norm needs `x` whose last sizes are `weight`'s ", weight_.sizes(), ", got ", x_.sizes(), ".");
     d.dtype = dtype_code(x_, kNorm, "x");
     TORCH_CHECK_VALUE(dtype >= PESQ_F32 && dtype <= PESQ_F16, "The CUDA layer norm has no type ", dtype, ".");
     d.out_dtype = static_cast<int32_t>(dtype);
@@ -37,12 +41,15 @@ struct NormCall {
                 "The CUDA layer norm needs `x` in float32 or in the result's type, it is ", x_.scalar_type(), ".");
     TORCH_CHECK_VALUE(eps >= 0.0, "The CUDA layer norm needs an `eps` that is not negative, got ", eps, ".");
     d.eps = static_cast<float>(eps);
+    heads = own == 2;
     x = rows(x_);
-    d.batch = x.size(0);
-    d.steps = x.size(1);
-    d.heads = x.size(2);
-    d.width = x.size(3);
-    d.x = heads_of(x);
+    d.width = x.size(-1);
+    d.heads = heads ? x.size(-2) : 1;
+    lead = dims - own;
+    d.batch = lead == 2 ? x.size(0) : 1;
+    d.steps = 1;
+    for (int64_t k = lead == 2 ? 1 : 0; k < lead; ++k) d.steps *= x.size(k);
+    d.x = strides_of(x);
     weight = vector(weight_, "weight");
     d.weight = weight.data_ptr<float>();
     if (given(bias_)) {
@@ -51,14 +58,26 @@ struct NormCall {
     }
   }
 
-  at::Tensor vector(const at::Tensor& t, const char* name) {
+  // of up to two leading dimensions any strides, of more a dense tensor; channels adjacent
+  at::Tensor rows(const at::Tensor& t) const {
+    const int64_t leading = t.dim() - (heads ? 2 : 1);
+    return leading <= 2 && (t.size(-1) <= 1 || t.stride(-1) == 1) ? t : t.contiguous();
+  }
+  pesq_heads strides_of(const at::Tensor& t) const {
+    const int64_t row = d.heads * d.width;
+    return {t.data_ptr(), lead == 2 ? t.stride(0) : 0, lead == 2 ? t.stride(1) : lead == 1 ? t.stride(0) : row,
+            heads ? t.stride(-2) : d.width};
+  }
+  at::Tensor vector(const at::Tensor& t, const char* name) const {
     check_cuda(t, x, kNorm, name);
     check_float(t, kNorm, name);
-    check_shape(t, {x.size(2), x.size(3)}, kNorm, name);
+    check_shape(t, x.sizes().slice(lead), kNorm, name);
     return t.contiguous();
   }
 
   bool empty() const { return x.numel() == 0; }
+  bool heads = false;
+  int64_t lead = 0;  // dimensions before the weight's
 };
 
 at::Tensor layer_norm_forward(const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias, double eps,
@@ -84,11 +103,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm_backward(const at::Ten
     dbias.zero_();
     return {dx, dweight, dbias};
   }
-  const at::Tensor dy = rows(dy_.to(c.out));
+  const at::Tensor dy = c.rows(dy_.scalar_type() == c.out ? dy_ : dy_.to(c.out));
   size_t bytes = 0;
   check_status(pesq_layer_norm_workspace(&c.d, &bytes), "pesq_layer_norm_workspace");
   at::Tensor ws = at::empty({static_cast<int64_t>(bytes)}, x.options().dtype(at::kByte));
-  check_status(pesq_layer_norm_backward(&c.d, at::cuda::getCurrentCUDAStream(), heads_of(dy), dx.data_ptr(),
+  check_status(pesq_layer_norm_backward(&c.d, at::cuda::getCurrentCUDAStream(), c.strides_of(dy), dx.data_ptr(),
                                         dweight.data_ptr<float>(), c.bias.defined() ? dbias.data_ptr<float>() : nullptr,
                                         ws.data_ptr(), bytes),
                "pesq_layer_norm_backward");
@@ -134,29 +153,14 @@ struct LayerNorm : public torch::autograd::Function<LayerNorm> {
   }
 };
 
-// x [..., channel] with weight [channel], or [..., head, channel] with [head, channel]; dtype < 0: x's
-at::Tensor layer_norm(const at::Tensor& x_, const at::Tensor& weight_, const OptTensor& bias_, double eps, int64_t dtype) {
-  check_cuda(x_, x_, kNorm, "x");
-  const int64_t dims = x_.dim(), vector = weight_.dim();
-  TORCH_CHECK_VALUE(vector == 1 || vector == 2, "The CUDA layer norm needs `weight` [channel] or [head, channel], got ",
-                    weight_.sizes(), ".");
-  TORCH_CHECK_VALUE(dims >= vector && x_.sizes().slice(dims - vector) == weight_.sizes(),
-                    "The CUDA layer norm needs `x` whose last sizes are `weight`'s ", weight_.sizes(), ", got ", x_.sizes(), ".");
-  if (given(bias_)) check_shape(*bias_, weight_.sizes(), kNorm, "bias");
-  no_forward_mode(kNorm, x_, weight_, bias_);
-  if (dtype < 0) dtype = dtype_code(x_, kNorm, "x");
-  at::Tensor x = x_, weight = weight_;
-  OptTensor bias = bias_;
-  if (vector == 1) {
-    weight = weight.unsqueeze(0);
-    if (given(bias)) bias = bias->unsqueeze(0);
-    x = x.unsqueeze(dims - 1);
-  }
-  while (x.dim() < 4) x = x.unsqueeze(0);
-  if (x.dim() > 4) x = x.flatten(0, x.dim() - 4);
-  const bool grad = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias));
-  const at::Tensor y = grad ? LayerNorm::apply(x, weight, bias, eps, dtype) : norm_forward_op().call(x, weight, bias, eps, dtype);
-  return y.sizes() == x_.sizes() ? y : y.view(x_.sizes());
+// dtype < 0: x's
+at::Tensor layer_norm(const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias, double eps, int64_t dtype) {
+  check_cuda(x, x, kNorm, "x");
+  no_forward_mode(kNorm, x, weight, bias);
+  if (dtype < 0) dtype = dtype_code(x, kNorm, "x");
+  if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias)))
+    return LayerNorm::apply(x, weight, bias, eps, dtype);
+  return norm_forward_op().call(x, weight, bias, eps, dtype);
 }
 
 // ------------------------------------------------------------ linear attention
