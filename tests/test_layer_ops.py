@@ -148,8 +148,8 @@ def test_muon_entry_checks_its_descriptor():
         return lib.pesq_muon_workspace(ctypes.byref(d), t, count, ctypes.byref(size)), d, t
 
     assert workspace()[0] == _lib.PESQ_OK
-    # X before and after a step, A and the polynomial, in tiles of 128, 4 bytes a value; and a norm's sums
-    assert size.value == (2 * 128 * 256 + 2 * 128 * 128) * 4 + 8 * -(-100 * 200 // 8192)
+    # X before and after a step, A, b + c A and the polynomial, in tiles of 128, 4 bytes a value; a norm's sums and a counter
+    assert size.value == (2 * 128 * 256 + 3 * 128 * 128) * 4 + 8 * -(-100 * 200 // 8192) + 16
     for bad in ({"count": -1}, {"rows": 0}, {"cols": 0}, {"param": None}, {"momentum": None}, {"copy": 16}, {"grad_dtype": 3},
                 {"steps": 0}, {"steps": 101}, {"adjust": 2}, {"beta": 1.0}, {"beta": float("nan")}, {"lr": -1.0},
                 {"weight_decay": float("nan")}, {"eps": 0.0}, {"eps": float("inf")}, {"a": 17.0}, {"b": float("nan")}):

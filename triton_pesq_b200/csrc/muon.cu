@@ -20,10 +20,13 @@
 // behind each other, zeros past the matrix' edge.  So an operand is a plain bulk copy of 32 KB, odd sizes need nothing
 // anywhere, and the one layout serves X X^T (64 columns of the contraction side by side) and B X (X's rows are the contraction:
 // the same bytes read as a transposed operand).  A and the polynomial are symmetric: the tiles below and on the diagonal are
-// computed, and written mirrored too, which takes 10 n^2 m products of a square matrix' step instead of 14.
+// computed, and written mirrored too, which takes 10 n^3 operations of a square matrix' step instead of 14.  Beside A goes
+// b + c A, so that the polynomial but for its a on the diagonal is one product of the two.
 //
 // A CTA takes tiles in turn: a thread issues copies three stages ahead, a thread issues products, four warps
-// empty the accumulators, of which there are two, so that a tile's end overlaps the next one's products.  All waits are
+// empty the accumulators, of which there are two, so that a tile's end overlaps the next one's products.  All products of
+// a call are one cooperative launch, whose CTAs wait for one another between the products of a step (15 launches of a
+// small model's step took 230 us of the host's time).  All waits are
 // bounded; one that runs out sets an error word and the CTA returns.
 #include <cuda_runtime.h>
 
@@ -65,7 +68,7 @@ struct Item {
   float* momentum;
   const void* grad;  // or the matrix to orthogonalise
   void* out;         // the parameter's copy in the gradient's type, or the result, or null
-  int64_t x[2], a, b;  // workspace offsets of X (before and after a step), A, the polynomial
+  int64_t x[2], a, c, b;  // workspace offsets of X (before and after a step), A, what it is multiplied with, the polynomial
   int rows, cols;
   int n, m, nt, mt;    // shorter and longer side, in tiles of 128
   int flipped;         // X is the matrix' transpose
@@ -73,38 +76,40 @@ struct Item {
   int first_prep, first_square, first_wide;  // tile, of the second pass, of symmetric products, of updates
   float step;          // lr times adjust
 };
-struct Args {
-  int count, dtype, nesterov;
-  int total;           // tiles, or blocks, of the launch
-  int mode, from;      // of a product; which X it reads
+struct Call {
+  int count, dtype, nesterov, steps;
+  int squares, wides;  // tiles of symmetric products, of updates
   char* ws;
   double* norms;       // sums of squares of the first pass' blocks
+  uint32_t* arrived;   // CTAs at the ends of the products so far
   const float* grad_scale;
   float beta, rest, decay;  // momentum, 1 - momentum, 1 - lr wd
   float eps, ca, cb, cc;
   uint32_t* error;
-  Item item[kItems];
 };
-static_assert(sizeof(Args) < 32000, "kernel parameters");
+// Kernel parameters; a launch of few matrices takes the short table
+template <int N>
+struct Args : Call {
+  Item item[N];
+};
+constexpr int kShort = 16;
+static_assert(sizeof(Args<kItems>) < 32000, "kernel parameters");
 
 __device__ uint32_t g_error;
 
-__device__ __forceinline__ float load(const void* p, int dtype, int64_t i) {
-  return dtype == PESQ_F32    ? static_cast<const float*>(p)[i]
-         : dtype == PESQ_BF16 ? widen(static_cast<const __nv_bfloat16*>(p)[i])
-                              : widen(static_cast<const __half*>(p)[i]);
-}
-__device__ __forceinline__ void store(void* p, int dtype, int64_t i, float v) {
+// f(a value of the gradients' type)
+template <class F>
+__device__ __forceinline__ void with_type(int dtype, F f) {
   if (dtype == PESQ_F32)
-    static_cast<float*>(p)[i] = v;
+    f(float{});
   else if (dtype == PESQ_BF16)
-    static_cast<__nv_bfloat16*>(p)[i] = narrow<__nv_bfloat16>(v);
+    f(__nv_bfloat16{});
   else
-    static_cast<__half*>(p)[i] = narrow<__half>(v);
+    f(__half{});
 }
 // the last item whose first is not above at
-template <int Item::*kFirst>
-__device__ __forceinline__ int find(const Args& p, int at) {
+template <int Item::*kFirst, int N>
+__device__ __forceinline__ int find(const Args<N>& p, int at) {
   int lo = 0, hi = p.count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) / 2;
@@ -114,7 +119,7 @@ __device__ __forceinline__ int find(const Args& p, int at) {
   return lo;
 }
 // the factor of the gradients; `skip` where it is not finite
-__device__ __forceinline__ float scale_of(const Args& p, bool& skip) {
+__device__ __forceinline__ float scale_of(const Call& p, bool& skip) {
   const float s = p.grad_scale ? *p.grad_scale : 1.0f;
   skip = !(s - s == 0.0f);
   return s;
@@ -124,34 +129,48 @@ __device__ __forceinline__ void depend() { asm volatile("griddepcontrol.wait;" :
 
 // ------------------------------------------------------------------------------- momentum and its norm
 
-__device__ __forceinline__ float update_of(const Args& p, const Item& it, int64_t i, float s) {
-  if (!it.momentum) return load(it.grad, p.dtype, i);
-  const float m = it.momentum[i];
-  return p.nesterov ? fmaf(p.beta, m, p.rest * (s * load(it.grad, p.dtype, i))) : m;
-}
+// the matrix that is orthogonalised
+__device__ __forceinline__ float update_of(const Call& p, float m, float g) { return p.nesterov ? fmaf(p.beta, m, p.rest * g) : m; }
 
-__global__ void __launch_bounds__(kPrepThreads) momentum_kernel(const __grid_constant__ Args p) {
+template <int N>
+__global__ void __launch_bounds__(kPrepThreads) momentum_kernel(const __grid_constant__ Args<N> p) {
+  constexpr int kTogether = 8;  // values of a thread whose loads are on their way together
   __shared__ double s_sum[kPrepThreads / 32];
   dependents();
   depend();
   const Item& it = p.item[find<&Item::first_norm>(p, blockIdx.x)];
   const int64_t numel = (int64_t)it.rows * it.cols, first = (int64_t)(blockIdx.x - it.first_norm) * kNormValues;
-  const int64_t end = min(numel, first + kNormValues);
   bool skip;
   const float s = scale_of(p, skip);
   double sum = 0.0;
-  for (int64_t i = first + threadIdx.x; i < end; i += kPrepThreads) {
-    float u;
-    if (it.momentum) {
-      const float g = s * load(it.grad, p.dtype, i);
-      const float m = fmaf(p.beta, it.momentum[i], p.rest * g);
-      if (!skip) it.momentum[i] = m;
-      u = p.nesterov ? fmaf(p.beta, m, p.rest * g) : m;
-    } else {
-      u = load(it.grad, p.dtype, i);
+  with_type(p.dtype, [&](auto zero) {
+    using G = decltype(zero);
+    const G* grad = static_cast<const G*>(it.grad) + first + threadIdx.x;
+    float* momentum = it.momentum ? it.momentum + first + threadIdx.x : nullptr;
+    const int left = (int)min((int64_t)kNormValues, numel - first) - (int)threadIdx.x;
+#pragma unroll 1
+    for (int i0 = 0; i0 < kNormValues / kPrepThreads; i0 += kTogether) {
+      float g[kTogether], m[kTogether];
+#pragma unroll
+      for (int k = 0; k < kTogether; ++k) {
+        const int at = (i0 + k) * kPrepThreads;
+        g[k] = at < left ? widen(grad[at]) : 0.0f;
+        m[k] = at < left && momentum ? momentum[at] : 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < kTogether; ++k) {
+        const int at = (i0 + k) * kPrepThreads;
+        float u = g[k];
+        if (momentum) {
+          g[k] *= s;
+          m[k] = fmaf(p.beta, m[k], p.rest * g[k]);
+          if (at < left && !skip) momentum[at] = m[k];
+          u = update_of(p, m[k], g[k]);
+        }
+        if (at < left) sum = fma((double)u, (double)u, sum);
+      }
     }
-    sum = fma((double)u, (double)u, sum);
-  }
+  });
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
   if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x / 32] = sum;
@@ -159,6 +178,7 @@ __global__ void __launch_bounds__(kPrepThreads) momentum_kernel(const __grid_con
   if (threadIdx.x == 0) {
     for (int w = 1; w < kPrepThreads / 32; ++w) sum += s_sum[w];
     p.norms[blockIdx.x] = sum;
+    if (blockIdx.x == 0) *p.arrived = 0;
   }
 }
 
@@ -177,7 +197,8 @@ __device__ __forceinline__ void split8(const float (&v)[8], Eight& hi, Eight& lo
 __device__ __forceinline__ int at(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
 
 // X in tiles; a block takes one
-__global__ void __launch_bounds__(kPrepThreads) prepare_kernel(const __grid_constant__ Args p) {
+template <int N>
+__global__ void __launch_bounds__(kPrepThreads) prepare_kernel(const __grid_constant__ Args<N> p) {
   __shared__ double s_sum[kPrepThreads];
   dependents();
   const int index = find<&Item::first_prep>(p, blockIdx.x);
@@ -197,21 +218,33 @@ __global__ void __launch_bounds__(kPrepThreads) prepare_kernel(const __grid_cons
   const double norm = sqrt(s_sum[0]);
   const float inverse = (float)(kScale / (norm > p.eps || norm != norm ? norm : (double)p.eps));
   char* to = p.ws + it.x[0] + (int64_t)tile * kPair;
-  // neighbouring threads: rows of a flipped matrix, chunks of a row of another
-  for (int i = threadIdx.x; i < kTile * 8; i += kPrepThreads) {
-    const int row = it.flipped ? i % kTile : i / 8, chunk = it.flipped ? i / kTile : i % 8;
-    const int r = rt * kTile + row, c = ct * kDepth + chunk * 8;
-    float v[8];
+  with_type(p.dtype, [&](auto zero) {
+    using G = decltype(zero);
+    const G* grad = static_cast<const G*>(it.grad);
+    // neighbouring threads: rows of a flipped matrix, chunks of a row of another
+#pragma unroll 2
+    for (int i = threadIdx.x; i < kTile * 8; i += kPrepThreads) {
+      const int row = it.flipped ? i % kTile : i / 8, chunk = it.flipped ? i / kTile : i % 8;
+      const int r = rt * kTile + row, c = ct * kDepth + chunk * 8;
+      const int64_t first = it.flipped ? (int64_t)c * it.cols + r : (int64_t)r * it.cols + c, apart = it.flipped ? it.cols : 1;
+      float g[8], m[8], v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const bool in = r < it.n && c + j < it.m;
-      v[j] = in ? update_of(p, it, it.flipped ? (int64_t)(c + j) * it.cols + r : (int64_t)r * it.cols + c + j, s) * inverse : 0.0f;
+      for (int j = 0; j < 8; ++j) {
+        const bool in = r < it.n && c + j < it.m;
+        g[j] = in ? widen(grad[first + j * apart]) : 0.0f;
+        m[j] = in && it.momentum ? it.momentum[first + j * apart] : 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = (it.momentum ? update_of(p, m[j], s * g[j]) : g[j]) * inverse;
+        if (!(r < it.n && c + j < it.m)) v[j] = 0.0f;
+      }
+      Eight hi, lo;
+      split8(v, hi, lo);
+      *reinterpret_cast<Eight*>(to + at(row, chunk)) = hi;
+      *reinterpret_cast<Eight*>(to + kPlane + at(row, chunk)) = lo;
     }
-    Eight hi, lo;
-    split8(v, hi, lo);
-    *reinterpret_cast<Eight*>(to + at(row, chunk)) = hi;
-    *reinterpret_cast<Eight*>(to + kPlane + at(row, chunk)) = lo;
-  }
+  });
 }
 
 // ------------------------------------------------------------------------------------------ products
@@ -257,15 +290,16 @@ __device__ __forceinline__ void load32(uint32_t (&v)[32], uint32_t address) {
 // A tile of a launch: its matrix, its place, and how long its contraction is
 struct Tile {
   int index, i, j, depth;
-  __device__ __forceinline__ Tile(const Args& p, int t) {
-    if (p.mode < kUpdate) {
+  template <int N>
+  __device__ __forceinline__ Tile(const Args<N>& p, int mode, int t) {
+    if (mode < kUpdate) {
       index = find<&Item::first_square>(p, t);
       const Item& it = p.item[index];
       t -= it.first_square;
       i = 0;
       while (t > i) t -= ++i;  // rows of 1, 2, 3, ... tiles
       j = t;
-      depth = ((p.mode == kGram ? it.m : it.n) + kDepth - 1) / kDepth;
+      depth = ((mode == kGram ? it.m : it.n) + kDepth - 1) / kDepth;
     } else {
       index = find<&Item::first_wide>(p, t);
       const Item& it = p.item[index];
@@ -277,77 +311,133 @@ struct Tile {
   }
 };
 
-// What four warps make of 32 columns of a tile's accumulators
-__device__ __forceinline__ void finish(const Args& p, const Item& it, const Tile& t, int row, int col, const float (&acc)[32],
-                                       float s_decay, bool skip) {
-  const int r = t.i * kTile + row, lane = threadIdx.x & 31;
-  if (p.mode == kLast) {
-    // (X is the result or its transpose: either way a thread has a row of X)
+// Eight columns of a row to a tile, and where mirrored to the tile across the diagonal too, whose rows are the columns here:
+// neighbouring lanes, which hold neighbouring rows, exchange halves, so that each stores two columns of one row
+__device__ __forceinline__ void put(char* to, char* over, bool mirrored, int row, int col, const float (&v)[8]) {
+  Eight plane[2];
+  split8(v, plane[0], plane[1]);
+  const int lane = threadIdx.x & 31, chunk = col % kDepth / 8, column = row % kDepth & ~1;
 #pragma unroll
-    for (int k = 0; k < 32; ++k) {
-      const int c = t.j * kTile + col + k;
-      if (r >= it.n || c >= it.m || skip) continue;
-      const float x = acc[k] * (1.0f / (kScale * kScale));
-      const int64_t to = it.flipped ? (int64_t)c * it.cols + r : (int64_t)r * it.cols + c;
-      if (it.param) {
-        const float v = fmaf(-it.step, x, it.param[to] * s_decay);
-        it.param[to] = v;
-        if (it.out) store(it.out, p.dtype, to, v);
-      } else {
-        store(it.out, p.dtype, to, x);
-      }
-    }
-    return;
-  }
-  const int tiles = p.mode == kUpdate ? 2 * it.mt : 2 * it.nt;  // side by side
-  const int64_t base = p.mode == kGram ? it.a : p.mode == kPolynomial ? it.b : it.x[p.from ^ 1];
-  const int64_t place = ((int64_t)t.i * tiles + t.j * 2 + col / kDepth) * kPair;
-  char* to = p.ws + base + place;
+  for (int q = 0; q < 2; ++q) {
+    *reinterpret_cast<Eight*>(to + q * kPlane + at(row, chunk)) = plane[q];
+    if (!mirrored) continue;
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(plane[q].h);
 #pragma unroll
-  for (int k = 0; k < 32; k += 8) {
-    const int chunk = col % kDepth / 8 + k / 8;
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = acc[k + j] * (1.0f / kScale);
-    if (p.mode == kPolynomial) {
-      const char* from = p.ws + it.a + place;
-      const Eight hi = *reinterpret_cast<const Eight*>(from + at(row, chunk));
-      const Eight lo = *reinterpret_cast<const Eight*>(from + kPlane + at(row, chunk));
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int c = t.j * kTile + col + k + j;
-        v[j] = fmaf(p.cc, v[j], p.cb * (__half2float(hi.h[j]) + __half2float(lo.h[j])));
-        if (c == r && r < it.n) v[j] += p.ca * kScale;
-      }
-    }
-    Eight hi, lo;
-    split8(v, hi, lo);
-    *reinterpret_cast<Eight*>(to + at(row, chunk)) = hi;
-    *reinterpret_cast<Eight*>(to + kPlane + at(row, chunk)) = lo;
-    if (p.mode < kUpdate && t.i != t.j) {
-      // mirrored: rows are the columns here.  Neighbouring lanes, which hold neighbouring rows, exchange halves, so that each
-      // stores two columns of one row
-      char* over = p.ws + base + ((int64_t)t.j * tiles + t.i * 2 + row / kDepth) * kPair;
-      const int column = row % kDepth & ~1;
-#pragma unroll
-      for (int plane = 0; plane < 2; ++plane) {
-        const uint32_t* words = reinterpret_cast<const uint32_t*>(plane ? lo.h : hi.h);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t other = __shfl_xor_sync(0xffffffffu, words[j], 1);
-          const uint32_t pair = lane & 1 ? __byte_perm(other, words[j], 0x7632) : __byte_perm(words[j], other, 0x5410);
-          const int mine = col + k + 2 * j + (lane & 1);
-          *reinterpret_cast<uint32_t*>(over + plane * kPlane + at(mine, column / 8) + column % 8 * 2) = pair;
-        }
-      }
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, words[j], 1);
+      const uint32_t pair = lane & 1 ? __byte_perm(other, words[j], 0x7632) : __byte_perm(words[j], other, 0x5410);
+      *reinterpret_cast<uint32_t*>(over + q * kPlane + at(col + 2 * j + (lane & 1), column / 8) + column % 8 * 2) = pair;
     }
   }
 }
 
-__global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_constant__ Args p) {
+// What four warps make of 32 columns of a tile's accumulators: a thread has a row
+__device__ __forceinline__ void finish(const Call& p, int mode, int from, const Item& it, const Tile& t, int row, int col,
+                                       const float (&acc)[32], bool skip) {
+  const int r = t.i * kTile + row, c0 = t.j * kTile + col;
+  if (mode == kLast) {
+    // (X is the result or its transpose.  All loads before all stores, as they may be the same memory)
+    if (r >= it.n || skip) return;
+    const int64_t first = it.flipped ? (int64_t)c0 * it.cols + r : (int64_t)r * it.cols + c0, apart = it.flipped ? it.cols : 1;
+    const int left = it.m - c0;
+    float v[32];
+    if (it.param) {
+      float* param = it.param + first;
+      const bool fours = !it.flipped && left >= 32 && reinterpret_cast<uintptr_t>(param) % 16 == 0;
+      if (fours) {
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(param + k);
+          v[k] = f.x, v[k + 1] = f.y, v[k + 2] = f.z, v[k + 3] = f.w;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] = k < left ? param[k * apart] : 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < 32; ++k) v[k] = fmaf(-it.step, acc[k] * (1.0f / (kScale * kScale)), v[k] * p.decay);
+      if (fours) {
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(param + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+          if (k < left) param[k * apart] = v[k];
+      }
+      if (!it.out) return;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 32; ++k) v[k] = acc[k] * (1.0f / (kScale * kScale));
+    }
+    with_type(p.dtype, [&](auto zero) {
+      using G = decltype(zero);
+      G* out = static_cast<G*>(it.out) + first;
+      if (apart == 1 && left >= 32 && reinterpret_cast<uintptr_t>(out) % 16 == 0) {
+        constexpr int kEach = 16 / sizeof(G);
+#pragma unroll
+        for (int k = 0; k < 32; k += kEach) {
+          Pack<G, kEach> q;
+#pragma unroll
+          for (int j = 0; j < kEach; ++j) q.v[j] = narrow<G>(v[k + j]);
+          *reinterpret_cast<Pack<G, kEach>*>(out + k) = q;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+          if (k < left) out[k * apart] = narrow<G>(v[k]);
+      }
+    });
+    return;
+  }
+  const int tiles = mode == kUpdate ? 2 * it.mt : 2 * it.nt;  // side by side
+  const int64_t place = ((int64_t)t.i * tiles + t.j * 2 + col / kDepth) * kPair;
+  const int64_t across = ((int64_t)t.j * tiles + t.i * 2 + row / kDepth) * kPair;
+  const bool mirrored = mode < kUpdate && t.i != t.j;
+  char* const to = p.ws + (mode == kGram ? it.a : mode == kPolynomial ? it.b : it.x[from ^ 1]);
+#pragma unroll
+  for (int k = 0; k < 32; k += 8) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = acc[k + j] * (1.0f / kScale);
+      if (mode == kPolynomial && c0 + k + j == r && r < it.n) v[j] += p.ca * kScale;
+    }
+    put(to + place, to + across, mirrored, row, col + k, v);
+    if (mode == kGram) {  // and what A is multiplied with: b + c A, so that the polynomial's tiles are products alone
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = p.cc * v[j] + (c0 + k + j == r && r < it.n ? p.cb * kScale : 0.0f);
+      put(p.ws + it.c + place, p.ws + it.c + across, mirrored, row, col + k, v);
+    }
+  }
+}
+
+// All CTAs of the launch at the same point, what they wrote visible to the copies that they issue next.  False where some
+// did not come in time
+constexpr uint32_t kPolls = 1u << 21;  // (a second or two)
+__device__ __forceinline__ bool meet(uint32_t* arrived, uint32_t want, volatile uint32_t& s_stop) {
+  asm volatile("fence.proxy.async;" ::: "memory");
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0 && !s_stop) {
+    asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(arrived) : "memory");
+    uint32_t seen = 0;
+    for (uint32_t i = 0; i < kPolls; ++i) {
+      asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(arrived) : "memory");
+      if (seen >= want) break;
+    }
+    if (seen < want) s_stop = 1;
+  }
+  __syncthreads();
+  asm volatile("fence.proxy.async;" ::: "memory");
+  return !s_stop;
+}
+
+template <int N>
+__global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_constant__ Args<N> p) {
   extern __shared__ char raw[];
   __shared__ __align__(8) uint64_t full[kStages], empty[kStages], ready[2], spent[2], drained;
   __shared__ uint32_t s_tmem;
+  __shared__ volatile uint32_t s_stop;
   char* const tiles = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -355,6 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
     for (int s = 0; s < 2; ++s) init(ready + s, 1), init(spent + s, 4);
     init(&drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    s_stop = 0;
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(&s_tmem)) : "memory");
@@ -364,128 +455,145 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = s_tmem;
-  dependents();
-  depend();
-  bool good = true;
-  if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0, issued = 0;
-      uint32_t parity = 1;
-      for (int t = blockIdx.x; t < p.total && good; t += gridDim.x) {
-        const Tile tile(p, t);
-        const Item& it = p.item[tile.index];
-        const bool wide = p.mode >= kUpdate, same = !wide && tile.i == tile.j;
-        const int64_t left = p.mode == kGram ? it.x[p.from] : p.mode == kPolynomial ? it.a : it.b;
-        const int across = p.mode == kGram ? 2 * it.mt : 2 * it.nt;
-        const char *a = p.ws + left + (int64_t)tile.i * across * kPair, *b = p.ws + left + (int64_t)tile.j * across * kPair;
-        for (int k = 0; k < tile.depth; ++k) {
-          if (!mbar_wait(empty + stage, parity)) {
-            good = false;
-            break;
+  // where the role of this thread is in its ring: copies or products of stages, accumulators
+  int stage = 0, half = 0;
+  uint32_t parity = warp == 0 ? 1 : 0, half_parity = warp == 1 ? 1 : 0;
+  int issued = 0;
+  bool good = true, skip;
+  scale_of(p, skip);
+  uint32_t met = 0;
+#pragma unroll 1
+  for (int product_index = 0; product_index < 3 * p.steps; ++product_index) {
+    const int step = product_index / 3, from = step & 1;
+    const int mode = product_index % 3 < 2 ? product_index % 3 : step + 1 < p.steps ? kUpdate : kLast;
+    const int total = mode < kUpdate ? p.squares : p.wides;
+    const bool wide = mode >= kUpdate;
+    if (warp == 0) {
+      if (lane == 0) {
+        for (int t = blockIdx.x; t < total && good; t += gridDim.x) {
+          const Tile tile(p, mode, t);
+          const Item& it = p.item[tile.index];
+          const bool same = mode == kGram && tile.i == tile.j;
+          const int64_t left = mode == kGram ? it.x[from] : mode == kPolynomial ? it.a : it.b;
+          const int across = mode == kGram ? 2 * it.mt : 2 * it.nt;
+          const char* a = p.ws + left + (int64_t)tile.i * across * kPair;
+          const char* b = p.ws + (mode == kPolynomial ? it.c : left) + (int64_t)tile.j * across * kPair;
+          for (int k = 0; k < tile.depth; ++k) {
+            if (!mbar_wait(empty + stage, parity)) {
+              good = false;
+              break;
+            }
+            char* to = tiles + stage * kStage;
+            mbar_arrive_expect_tx(full + stage, same ? kPair : 2 * kPair);
+            bulk_g2s(to, a + (int64_t)k * kPair, kPair, full + stage);
+            if (wide) {
+              // 64 rows of two tiles of X side by side
+              const char* x = p.ws + it.x[from] + ((int64_t)(k / 2) * 2 * it.mt + tile.j * 2) * kPair + (k & 1) * (kPlane / 2);
+              for (int plane = 0; plane < 2; ++plane)
+                for (int side = 0; side < 2; ++side)
+                  bulk_g2s(to + kPair + plane * kPlane + side * (kPlane / 2), x + side * kPair + plane * kPlane, kPlane / 2, full + stage);
+            } else if (!same) {
+              bulk_g2s(to + kPair, b + (int64_t)k * kPair, kPair, full + stage);
+            }
+            if (issued < kStages) ++issued;
+            if (++stage == kStages) stage = 0, parity ^= 1;
           }
-          char* to = tiles + stage * kStage;
-          mbar_arrive_expect_tx(full + stage, same ? kPair : 2 * kPair);
-          bulk_g2s(to, a + (int64_t)k * kPair, kPair, full + stage);
-          if (wide) {
-            // 64 rows of two tiles of X side by side
-            const char* x = p.ws + it.x[p.from] + ((int64_t)(k / 2) * 2 * it.mt + tile.j * 2) * kPair + (k & 1) * (kPlane / 2);
-            for (int plane = 0; plane < 2; ++plane)
-              for (int side = 0; side < 2; ++side)
-                bulk_g2s(to + kPair + plane * kPlane + side * (kPlane / 2), x + side * kPair + plane * kPlane, kPlane / 2, full + stage);
-          } else if (!same) {
-            bulk_g2s(to + kPair, b + (int64_t)k * kPair, kPair, full + stage);
+        }
+        if (!good) {  // (what is in flight lands before the CTA ends)
+          atomicOr(p.error, 1u);
+          s_stop = 1;
+          for (int s = 1; s <= issued; ++s) {
+            // the copies s stages back, whose phase is that of the parity they were issued with
+            const int back = (stage + kStages - s) % kStages;
+            mbar_wait(full + back, back < stage ? parity ^ 1 : parity);
           }
-          if (issued < kStages) ++issued;
-          if (++stage == kStages) stage = 0, parity ^= 1;
         }
       }
-      if (!good) {  // (what is in flight lands before the CTA ends)
-        atomicOr(p.error, 1u);
-        for (int s = 1; s <= issued; ++s) {
-          // the copies s stages back, whose phase is that of the parity they were issued with
-          const int back = (stage + kStages - s) % kStages;
-          mbar_wait(full + back, back < stage ? parity ^ 1 : parity);
+    } else if (warp == 1) {
+      if (lane == 0) {
+        for (int t = blockIdx.x; t < total && good; t += gridDim.x) {
+          const Tile tile(p, mode, t);
+          const bool same = mode == kGram && tile.i == tile.j;
+          const uint32_t instruction = kInstruction | (wide ? kTransposedB : 0);
+          for (int k = 0; k < tile.depth; ++k) {
+            if (k % kSegment == 0 && !mbar_wait(spent + half, half_parity) || !mbar_wait(full + stage, parity)) {
+              good = false;
+              break;
+            }
+            const uint32_t to = tmem + half * kTile;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t a = smem_u32(tiles + stage * kStage), b = same ? a : a + kPair;
+#pragma unroll
+            for (int s = 0; s < kDepth / 16; ++s) {
+              const uint32_t as = a + s * 32, bs = b + s * (wide ? 2048 : 32);
+              const uint64_t a_hi = descriptor(as, false), a_lo = descriptor(as + kPlane, false);
+              const uint64_t b_hi = descriptor(bs, wide), b_lo = descriptor(bs + kPlane, wide);
+              product(to, a_lo, b_hi, instruction, k % kSegment > 0 || s > 0);
+              product(to, a_hi, b_lo, instruction, true);
+              product(to, a_hi, b_hi, instruction, true);
+            }
+            commit(empty + stage);
+            if (++stage == kStages) stage = 0, parity ^= 1;
+            if ((k + 1) % kSegment == 0 || k + 1 == tile.depth) {
+              commit(ready + half);
+              half ^= 1;
+              if (half == 0) half_parity ^= 1;
+            }
+          }
+        }
+        if (!good) {  // (what is issued ends before its memory goes)
+          atomicOr(p.error, 2u);
+          s_stop = 1;
+          commit(&drained);
+          mbar_wait(&drained, 0);
         }
       }
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      int stage = 0, half = 0;
-      uint32_t parity = 0, spent_parity = 1;
-      for (int t = blockIdx.x; t < p.total && good; t += gridDim.x) {
-        const Tile tile(p, t);
-        const bool wide = p.mode >= kUpdate, same = !wide && tile.i == tile.j;
-        const uint32_t instruction = kInstruction | (wide ? kTransposedB : 0);
-        for (int k = 0; k < tile.depth; ++k) {
-          if (k % kSegment == 0 && !mbar_wait(spent + half, spent_parity) || !mbar_wait(full + stage, parity)) {
-            good = false;
-            break;
-          }
-          const uint32_t to = tmem + half * kTile;
+    } else {
+      const int quarter = warp & 3;
+      for (int t = blockIdx.x; t < total && good; t += gridDim.x) {
+        const Tile tile(p, mode, t);
+        float acc[kTile / 32][32];
+#pragma unroll
+        for (int c = 0; c < kTile / 32; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; ++e) acc[c][e] = 0.0f;
+        for (int k = 0; k < tile.depth; k += kSegment) {
+          good = __all_sync(0xffffffffu, mbar_wait(ready + half, half_parity));
+          if (!good) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t a = smem_u32(tiles + stage * kStage), b = same ? a : a + kPair;
 #pragma unroll
-          for (int s = 0; s < kDepth / 16; ++s) {
-            const uint32_t as = a + s * 32, bs = b + s * (wide ? 2048 : 32);
-            const uint64_t a_hi = descriptor(as, false), a_lo = descriptor(as + kPlane, false);
-            const uint64_t b_hi = descriptor(bs, wide), b_lo = descriptor(bs + kPlane, wide);
-            product(to, a_lo, b_hi, instruction, k % kSegment > 0 || s > 0);
-            product(to, a_hi, b_lo, instruction, true);
-            product(to, a_hi, b_hi, instruction, true);
+          for (int c = 0; c < kTile / 32; ++c) {
+            uint32_t part[32];
+            load32(part, tmem + half * kTile + c * 32 + ((uint32_t)(quarter * 32) << 16));
+#pragma unroll
+            for (int e = 0; e < 32; ++e) acc[c][e] += __uint_as_float(part[e]);
           }
-          commit(empty + stage);
-          if (++stage == kStages) stage = 0, parity ^= 1;
-          if ((k + 1) % kSegment == 0 || k + 1 == tile.depth) {
-            commit(ready + half);
-            half ^= 1;
-            if (half == 0) spent_parity ^= 1;
-          }
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) arrive(spent + half);
+          half ^= 1;
+          if (half == 0) half_parity ^= 1;
         }
-      }
-      if (!good) {  // (what is issued ends before its memory goes)
-        atomicOr(p.error, 2u);
-        commit(&drained);
-        mbar_wait(&drained, 0);
-      }
-    }
-  } else {
-    const int quarter = warp & 3;
-    int half = 0;
-    uint32_t parity = 0;
-    bool skip;
-    scale_of(p, skip);
-    for (int t = blockIdx.x; t < p.total && good; t += gridDim.x) {
-      const Tile tile(p, t);
-      float acc[kTile / 32][32];
-#pragma unroll
-      for (int c = 0; c < kTile / 32; ++c)
-#pragma unroll
-        for (int e = 0; e < 32; ++e) acc[c][e] = 0.0f;
-      for (int k = 0; k < tile.depth; k += kSegment) {
-        good = __all_sync(0xffffffffu, mbar_wait(ready + half, parity));
         if (!good) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-        for (int c = 0; c < kTile / 32; ++c) {
-          uint32_t part[32];
-          load32(part, tmem + half * kTile + c * 32 + ((uint32_t)(quarter * 32) << 16));
-#pragma unroll
-          for (int e = 0; e < 32; ++e) acc[c][e] += __uint_as_float(part[e]);
-        }
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) arrive(spent + half);
-        half ^= 1;
-        if (half == 0) parity ^= 1;
+        for (int c = 0; c < kTile / 32; ++c)
+          finish(p, mode, from, p.item[tile.index], tile, quarter * 32 + lane, c * 32, acc[c], skip);
       }
-      if (!good) break;
-#pragma unroll
-      for (int c = 0; c < kTile / 32; ++c)
-        finish(p, p.item[tile.index], tile, quarter * 32 + lane, c * 32, acc[c], p.decay, skip);
+      if (!good && lane == 0) {
+        atomicOr(p.error, 4u);
+        s_stop = 1;
+      }
     }
-    if (!good && lane == 0) atomicOr(p.error, 4u);
+    __syncwarp();
+    met += gridDim.x;
+    if (product_index + 1 < 3 * p.steps) {
+      good = meet(p.arrived, met, s_stop) && good;
+      if (s_stop) {
+        if (threadIdx.x == 0) atomicOr(p.error, 8u);
+        break;
+      }
+    }
   }
-  __syncwarp();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (warp == 1) {
@@ -506,11 +614,17 @@ int sms() {
   return cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess ? n : 148;
 }
 
-template <class... A>
-cudaError_t start(void (*kernel)(A...), int grid, int threads, int smem, cudaStream_t s, const A&... args) {
+// close behind the kernel before, or with all CTAs on the device at once
+template <class A>
+cudaError_t start(void (*kernel)(A), int grid, int threads, int smem, bool together, cudaStream_t s, const A& args) {
   cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
+  if (together) {
+    at.id = cudaLaunchAttributeCooperative;
+    at.val.cooperative = 1;
+  } else {
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+  }
   cudaLaunchConfig_t c{};
   c.gridDim = dim3((unsigned)grid);
   c.blockDim = dim3((unsigned)threads);
@@ -518,7 +632,7 @@ cudaError_t start(void (*kernel)(A...), int grid, int threads, int smem, cudaStr
   c.stream = s;
   c.attrs = &at;
   c.numAttrs = 1;
-  return cudaLaunchKernelEx(&c, kernel, args...);
+  return cudaLaunchKernelEx(&c, kernel, args);
 }
 
 struct Matrix {
@@ -532,7 +646,7 @@ struct Matrix {
 int64_t tiles_of(int64_t n) { return (n + kTile - 1) / kTile; }
 int64_t matrix_bytes(int64_t rows, int64_t cols) {
   const int64_t nt = tiles_of(std::min(rows, cols)), mt = tiles_of(std::max(rows, cols));
-  return (2 * nt * mt + 2 * nt * nt) * 2 * kPair;
+  return (2 * nt * mt + 3 * nt * nt) * 2 * kPair;
 }
 int64_t norm_blocks(int64_t rows, int64_t cols) { return (rows * cols + kNormValues - 1) / kNormValues; }
 
@@ -556,61 +670,66 @@ void groups(const std::vector<Matrix>& all, F f) {
 }
 size_t workspace_of(const std::vector<Matrix>& all) {
   int64_t most = 0;
-  groups(all, [&](size_t, size_t, int64_t bytes, int64_t norms) { most = std::max(most, bytes + norms * 8); });
+  groups(all, [&](size_t, size_t, int64_t bytes, int64_t norms) { most = std::max(most, bytes + norms * 8 + 16); });
   return (size_t)most;
 }
 
-cudaError_t run(const std::vector<Matrix>& all, Args& a, int steps, void* workspace, cudaStream_t s) {
-  cudaError_t e = cudaFuncSetAttribute(products_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared);
-  groups(all, [&](size_t first, size_t n, int64_t bytes, int64_t) {
+template <int N>
+cudaError_t run_group(const Call& call, const Matrix* all, int n, int64_t bytes, int64_t norm_count, cudaStream_t s) {
+  Args<N> a{};
+  static_cast<Call&>(a) = call;
+  a.count = n;
+  a.norms = reinterpret_cast<double*>(a.ws + bytes);
+  a.arrived = reinterpret_cast<uint32_t*>(a.norms + norm_count);
+  int64_t at = 0;
+  int norms = 0, preps = 0;
+  for (int k = 0; k < n; ++k) {
+    const Matrix& m = all[k];
+    Item& it = a.item[k];
+    it.param = m.param;
+    it.momentum = m.momentum;
+    it.grad = m.grad;
+    it.out = m.out;
+    it.rows = (int)m.rows;
+    it.cols = (int)m.cols;
+    it.flipped = m.rows > m.cols;
+    it.n = std::min(it.rows, it.cols);
+    it.m = std::max(it.rows, it.cols);
+    it.nt = (int)tiles_of(it.n);
+    it.mt = (int)tiles_of(it.m);
+    it.step = m.step;
+    const int64_t x = (int64_t)it.nt * 2 * it.mt * kPair, square = (int64_t)it.nt * 2 * it.nt * kPair;
+    it.x[0] = at;
+    it.x[1] = at + x;
+    it.a = at + 2 * x;
+    it.c = it.a + square;
+    it.b = it.c + square;
+    at = it.b + square;
+    it.first_norm = norms;
+    it.norms = (int)norm_blocks(m.rows, m.cols);
+    it.first_prep = preps;
+    it.first_square = a.squares;
+    it.first_wide = a.wides;
+    norms += it.norms;
+    preps += it.nt * 2 * it.mt;
+    a.squares += it.nt * (it.nt + 1) / 2;
+    a.wides += it.nt * it.mt;
+  }
+  cudaError_t e = cudaFuncSetAttribute(products_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared);
+  if (e == cudaSuccess) e = start(momentum_kernel<N>, norms, kPrepThreads, 0, false, s, a);
+  if (e == cudaSuccess) e = start(prepare_kernel<N>, preps, kPrepThreads, 0, false, s, a);
+  if (e == cudaSuccess)
+    e = start(products_kernel<N>, std::min(sms(), std::max(a.squares, a.wides)), kThreads, kShared, true, s, a);
+  return e;
+}
+
+cudaError_t run(const std::vector<Matrix>& all, Call& call, void* workspace, cudaStream_t s) {
+  call.ws = static_cast<char*>(workspace);
+  cudaError_t e = cudaSuccess;
+  groups(all, [&](size_t first, size_t n, int64_t bytes, int64_t norms) {
     if (e != cudaSuccess) return;
-    a.count = (int)n;
-    a.ws = static_cast<char*>(workspace);
-    a.norms = reinterpret_cast<double*>(a.ws + bytes);
-    int64_t at = 0;
-    int norms = 0, preps = 0, squares = 0, wides = 0;
-    for (size_t k = 0; k < n; ++k) {
-      const Matrix& m = all[first + k];
-      Item& it = a.item[k];
-      it = Item{};
-      it.param = m.param;
-      it.momentum = m.momentum;
-      it.grad = m.grad;
-      it.out = m.out;
-      it.rows = (int)m.rows;
-      it.cols = (int)m.cols;
-      it.flipped = m.rows > m.cols;
-      it.n = std::min(it.rows, it.cols);
-      it.m = std::max(it.rows, it.cols);
-      it.nt = (int)tiles_of(it.n);
-      it.mt = (int)tiles_of(it.m);
-      it.step = m.step;
-      const int64_t x = (int64_t)it.nt * 2 * it.mt * kPair, square = (int64_t)it.nt * 2 * it.nt * kPair;
-      it.x[0] = at;
-      it.x[1] = at + x;
-      it.a = at + 2 * x;
-      it.b = it.a + square;
-      at = it.b + square;
-      it.first_norm = norms;
-      it.norms = (int)norm_blocks(m.rows, m.cols);
-      it.first_prep = preps;
-      it.first_square = squares;
-      it.first_wide = wides;
-      norms += it.norms;
-      preps += it.nt * 2 * it.mt;
-      squares += it.nt * (it.nt + 1) / 2;
-      wides += it.nt * it.mt;
-    }
-    e = start(momentum_kernel, norms, kPrepThreads, 0, s, a);
-    if (e == cudaSuccess) e = start(prepare_kernel, preps, kPrepThreads, 0, s, a);
-    for (int step = 0; step < steps && e == cudaSuccess; ++step) {
-      a.from = step & 1;
-      for (int mode : {(int)kGram, (int)kPolynomial, step + 1 < steps ? (int)kUpdate : (int)kLast}) {
-        a.mode = mode;
-        a.total = mode < kUpdate ? squares : wides;
-        if (e == cudaSuccess) e = start(products_kernel, std::min(sms(), a.total), kThreads, kShared, s, a);
-      }
-    }
+    e = n <= kShort ? run_group<kShort>(call, &all[first], (int)n, bytes, norms, s)
+                    : run_group<kItems>(call, &all[first], (int)n, bytes, norms, s);
   });
   return e;
 }
@@ -700,8 +819,9 @@ int pesq_muon_step(const pesq_muon_desc* d, const pesq_muon_tensor* tensors, int
     if (const int status = muon_matrices(d, tensors, count, all)) return status;
     if (all.empty()) return (int)PESQ_OK;
     if (const int status = check_workspace(workspace, workspace_bytes, workspace_of(all))) return status;
-    Args a{};
+    Call a{};
     a.dtype = d->grad_dtype;
+    a.steps = d->steps;
     a.nesterov = d->nesterov != 0;
     a.grad_scale = d->grad_scale;
     a.beta = (float)d->momentum;
@@ -711,7 +831,7 @@ int pesq_muon_step(const pesq_muon_desc* d, const pesq_muon_tensor* tensors, int
     a.ca = d->a, a.cb = d->b, a.cc = d->c;
     a.error = error_word();
     if (!a.error) return set_error(PESQ_ERR_CUDA, "no error word");
-    const cudaError_t e = run(all, a, d->steps, workspace, static_cast<cudaStream_t>(stream));
+    const cudaError_t e = run(all, a, workspace, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? (int)PESQ_OK : set_error(PESQ_ERR_CUDA, cudaGetErrorString(e));
   });
 }
@@ -733,13 +853,14 @@ int pesq_orthogonalize(const pesq_orthogonalize_desc* d, void* stream, const voi
     if (!x || !out) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL operand");
     if (const int status = stack(d, x, out, all)) return status;
     if (const int status = check_workspace(workspace, workspace_bytes, workspace_of(all))) return status;
-    Args a{};
+    Call a{};
     a.dtype = d->dtype;
+    a.steps = d->steps;
     a.eps = d->eps;
     a.ca = d->a, a.cb = d->b, a.cc = d->c;
     a.error = error_word();
     if (!a.error) return set_error(PESQ_ERR_CUDA, "no error word");
-    const cudaError_t e = run(all, a, d->steps, workspace, static_cast<cudaStream_t>(stream));
+    const cudaError_t e = run(all, a, workspace, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? (int)PESQ_OK : set_error(PESQ_ERR_CUDA, cudaGetErrorString(e));
   });
 }
