@@ -23,8 +23,9 @@
 // computed, and written mirrored too, which takes 10 n^3 operations of a square matrix' step instead of 14.  Beside A goes
 // b + c A, so that the polynomial but for its a on the diagonal is one product of the two.
 //
-// A CTA takes tiles in turn: a thread issues copies three stages ahead, a thread issues products, four warps
-// empty the accumulators, of which there are two, so that a tile's end overlaps the next one's products.  All products of
+// A CTA takes tiles in turn: a thread issues copies three stages ahead, a thread issues products, sixteen warps
+// empty the accumulators, of which there are two, so that a tile's end overlaps the next one's products (each a quarter of
+// the columns: four warps with all of them took twice as long over a small model's tiles).  All products of
 // a call are one cooperative launch, whose CTAs wait for one another between the products of a step (15 launches of a
 // small model's step took 230 us of the host's time).  All waits are
 // bounded; one that runs out sets an error word and the CTA returns.
@@ -51,7 +52,8 @@ constexpr int kTile = 128, kDepth = 64;               // rows of a tile, columns
 constexpr int kPlane = kTile * kDepth * 2;            // bytes of a tile's hi or lo terms
 constexpr int kPair = 2 * kPlane;
 constexpr int kStages = 3, kStage = 2 * kPair;        // both operands
-constexpr int kThreads = 192;                         // copies, products, four warps of results
+constexpr int kReaders = 16;                          // warps of results: four for each quarter of the columns
+constexpr int kThreads = 64 + 32 * kReaders;          // copies, products, results
 constexpr int kShared = kStages * kStage + 1024;      // (aligned to 1024 in the kernel)
 constexpr int kSegment = 2;                           // stages whose products are summed in tensor memory
 constexpr float kScale = 1024.0f;                     // of what is kept
@@ -442,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) init(full + s, 1), init(empty + s, 1);
-    for (int s = 0; s < 2; ++s) init(ready + s, 1), init(spent + s, 4);
+    for (int s = 0; s < 2; ++s) init(ready + s, 1), init(spent + s, kReaders);
     init(&drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     s_stop = 0;
@@ -549,35 +551,28 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
         }
       }
     } else {
-      const int quarter = warp & 3;
+      const int quarter = warp & 3, col = (warp - 2) / 4 * 32;  // its lanes of tensor memory, and columns
       for (int t = blockIdx.x; t < total && good; t += gridDim.x) {
         const Tile tile(p, mode, t);
-        float acc[kTile / 32][32];
+        float acc[32];
 #pragma unroll
-        for (int c = 0; c < kTile / 32; ++c)
-#pragma unroll
-          for (int e = 0; e < 32; ++e) acc[c][e] = 0.0f;
+        for (int e = 0; e < 32; ++e) acc[e] = 0.0f;
         for (int k = 0; k < tile.depth; k += kSegment) {
           good = __all_sync(0xffffffffu, mbar_wait(ready + half, half_parity));
           if (!good) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-          for (int c = 0; c < kTile / 32; ++c) {
-            uint32_t part[32];
-            load32(part, tmem + half * kTile + c * 32 + ((uint32_t)(quarter * 32) << 16));
-#pragma unroll
-            for (int e = 0; e < 32; ++e) acc[c][e] += __uint_as_float(part[e]);
-          }
+          uint32_t part[32];
+          load32(part, tmem + half * kTile + col + ((uint32_t)(quarter * 32) << 16));
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           __syncwarp();
           if (lane == 0) arrive(spent + half);
           half ^= 1;
           if (half == 0) half_parity ^= 1;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) acc[e] += __uint_as_float(part[e]);
         }
         if (!good) break;
-#pragma unroll
-        for (int c = 0; c < kTile / 32; ++c)
-          finish(p, mode, from, p.item[tile.index], tile, quarter * 32 + lane, c * 32, acc[c], skip);
+        finish(p, mode, from, p.item[tile.index], tile, quarter * 32 + lane, col, acc, skip);
       }
       if (!good && lane == 0) {
         atomicOr(p.error, 4u);
