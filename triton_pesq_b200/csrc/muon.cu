@@ -59,6 +59,9 @@ constexpr int kSegment = 2;                           // stages whose products a
 constexpr float kScale = 1024.0f;                     // of what is kept
 constexpr int kMost = 32768;                          // rows or columns
 constexpr int kItems = 128;                           // matrices of a launch
+constexpr int kNarrowStages = 3;                      // of one operand, beside two squares, of the narrow kernel
+constexpr int kNarrowShared = 4 * kPair + kNarrowStages * kPair + 1024;
+constexpr int kNarrowTiles = 8;                       // across, of the matrices that it takes
 constexpr int64_t kGroupBytes = INT64_C(256) << 20;   // of their workspace, where there are several
 constexpr int kNormValues = 8192;                     // of a block of the first pass
 constexpr int kPrepThreads = 256;
@@ -413,6 +416,20 @@ __device__ __forceinline__ void finish(const Call& p, int mode, int from, const 
   }
 }
 
+// The three products of a step, 16 columns of the contraction after the other
+__device__ __forceinline__ void products_of(uint32_t to, uint32_t a, uint32_t b, bool transposed, bool add) {
+  const uint32_t instruction = kInstruction | (transposed ? kTransposedB : 0);
+#pragma unroll
+  for (int s = 0; s < kDepth / 16; ++s) {
+    const uint32_t as = a + s * 32, bs = b + s * (transposed ? 2048 : 32);
+    const uint64_t a_hi = descriptor(as, false), a_lo = descriptor(as + kPlane, false);
+    const uint64_t b_hi = descriptor(bs, transposed), b_lo = descriptor(bs + kPlane, transposed);
+    product(to, a_lo, b_hi, instruction, add || s > 0);
+    product(to, a_hi, b_lo, instruction, true);
+    product(to, a_hi, b_hi, instruction, true);
+  }
+}
+
 // All CTAs of the launch at the same point, what they wrote visible to the copies that they issue next.  False where some
 // did not come in time
 constexpr uint32_t kPolls = 1u << 21;  // (a second or two)
@@ -516,24 +533,14 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
         for (int t = blockIdx.x; t < total && good; t += gridDim.x) {
           const Tile tile(p, mode, t);
           const bool same = mode == kGram && tile.i == tile.j;
-          const uint32_t instruction = kInstruction | (wide ? kTransposedB : 0);
           for (int k = 0; k < tile.depth; ++k) {
             if (k % kSegment == 0 && !mbar_wait(spent + half, half_parity) || !mbar_wait(full + stage, parity)) {
               good = false;
               break;
             }
-            const uint32_t to = tmem + half * kTile;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t a = smem_u32(tiles + stage * kStage), b = same ? a : a + kPair;
-#pragma unroll
-            for (int s = 0; s < kDepth / 16; ++s) {
-              const uint32_t as = a + s * 32, bs = b + s * (wide ? 2048 : 32);
-              const uint64_t a_hi = descriptor(as, false), a_lo = descriptor(as + kPlane, false);
-              const uint64_t b_hi = descriptor(bs, wide), b_lo = descriptor(bs + kPlane, wide);
-              product(to, a_lo, b_hi, instruction, k % kSegment > 0 || s > 0);
-              product(to, a_hi, b_lo, instruction, true);
-              product(to, a_hi, b_hi, instruction, true);
-            }
+            const uint32_t a = smem_u32(tiles + stage * kStage);
+            products_of(tmem + half * kTile, a, same ? a : a + kPair, wide, k % kSegment > 0);
             commit(empty + stage);
             if (++stage == kStages) stage = 0, parity ^= 1;
             if ((k + 1) % kSegment == 0 || k + 1 == tile.depth) {
@@ -597,6 +604,194 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
   }
 }
 
+// Eight columns of a row of a square in shared memory: two tiles of 64 columns
+__device__ __forceinline__ void put_shared(char* square, int row, int col, const float (&v)[8]) {
+  Eight hi, lo;
+  split8(v, hi, lo);
+  char* to = square + col / kDepth * kPair + at(row, col % kDepth / 8);
+  *reinterpret_cast<Eight*>(to) = hi;
+  *reinterpret_cast<Eight*>(to + kPlane) = lo;
+}
+
+template <int N>
+__global__ void __launch_bounds__(kThreads, 1) narrow_kernel(const __grid_constant__ Args<N> p) {
+  extern __shared__ char raw[];
+  __shared__ __align__(8) uint64_t full[kNarrowStages], empty[kNarrowStages], ready[2], spent[2], made, drained;
+  __shared__ uint32_t s_tmem;
+  __shared__ volatile uint32_t s_stop;
+  char* const squares = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);  // A, then the polynomial; b + c A
+  char* const ring = squares + 4 * kPair;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kNarrowStages; ++s) init(full + s, 1), init(empty + s, 1);
+    for (int s = 0; s < 2; ++s) init(ready + s, 1), init(spent + s, kReaders);
+    init(&made, kReaders);
+    init(&drained, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    s_stop = 0;
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(&s_tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  }
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = s_tmem;
+  int stage = 0, half = 0, issued = 0;
+  uint32_t parity = warp == 0 ? 1 : 0, half_parity = warp == 1 ? 1 : 0, made_parity = 0, met = 0;
+  bool good = true, skip;
+  scale_of(p, skip);
+#pragma unroll 1
+  for (int step = 0; step < p.steps; ++step) {
+    const int from = step & 1;
+    if (warp == 0) {
+      if (lane == 0) {
+        for (int t = blockIdx.x; t < p.wides && good; t += gridDim.x) {
+          const Tile tile(p, kUpdate, t);
+          const Item& it = p.item[tile.index];
+          const char* x = p.ws + it.x[from];
+          const int gram = (it.m + kDepth - 1) / kDepth;
+          for (int k = 0; k < gram + tile.depth; ++k) {
+            if (!mbar_wait(empty + stage, parity)) {
+              good = false;
+              break;
+            }
+            char* to = ring + stage * kPair;
+            mbar_arrive_expect_tx(full + stage, kPair);
+            if (k < gram) {
+              bulk_g2s(to, x + (int64_t)k * kPair, kPair, full + stage);
+            } else {  // 64 rows of two tiles of X side by side
+              const char* rows = x + (int64_t)tile.j * 2 * kPair + (k - gram) * (kPlane / 2);
+              for (int plane = 0; plane < 2; ++plane)
+                for (int side = 0; side < 2; ++side)
+                  bulk_g2s(to + plane * kPlane + side * (kPlane / 2), rows + side * kPair + plane * kPlane, kPlane / 2, full + stage);
+            }
+            if (issued < kNarrowStages) ++issued;
+            if (++stage == kNarrowStages) stage = 0, parity ^= 1;
+          }
+        }
+        if (!good) {  // (what is in flight lands before the CTA ends)
+          atomicOr(p.error, 1u);
+          s_stop = 1;
+          for (int s = 1; s <= issued; ++s) {
+            const int back = (stage + kNarrowStages - s) % kNarrowStages;
+            mbar_wait(full + back, back < stage ? parity ^ 1 : parity);
+          }
+        }
+      }
+    } else if (warp == 1) {
+      if (lane == 0) {
+        const uint32_t square = smem_u32(squares);
+        for (int t = blockIdx.x; t < p.wides && good; t += gridDim.x) {
+          const Tile tile(p, kUpdate, t);
+          const int gram = (p.item[tile.index].m + kDepth - 1) / kDepth;
+          // A: X X^T, then the polynomial: A (b + c A), then X': the polynomial times X
+          for (int part = 0; part < 3 && good; ++part) {
+            const int depth = part == 0 ? gram : tile.depth;
+            if (part > 0) {
+              good = mbar_wait(&made, made_parity);
+              made_parity ^= 1;
+            }
+            for (int k = 0; k < depth && good; ++k) {
+              if (k % kSegment == 0) good = mbar_wait(spent + half, half_parity);
+              if (part != 1) good = good && mbar_wait(full + stage, parity);
+              if (!good) break;
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+              const uint32_t own = smem_u32(ring + stage * kPair);
+              products_of(tmem + half * kTile, part == 0 ? own : square + k * kPair, part == 1 ? square + (2 + k) * kPair : own,
+                          part == 2, k % kSegment > 0);
+              if (part != 1) {
+                commit(empty + stage);
+                if (++stage == kNarrowStages) stage = 0, parity ^= 1;
+              }
+              if ((k + 1) % kSegment == 0 || k + 1 == depth) {
+                commit(ready + half);
+                half ^= 1;
+                if (half == 0) half_parity ^= 1;
+              }
+            }
+          }
+        }
+        if (!good) {  // (what is issued ends before its memory goes)
+          atomicOr(p.error, 2u);
+          s_stop = 1;
+          commit(&drained);
+          mbar_wait(&drained, 0);
+        }
+      }
+    } else {
+      const int quarter = warp & 3, col = (warp - 2) / 4 * 32, row = quarter * 32 + lane;
+      for (int t = blockIdx.x; t < p.wides && good; t += gridDim.x) {
+        const Tile tile(p, kUpdate, t);
+        const Item& it = p.item[tile.index];
+        const int gram = (it.m + kDepth - 1) / kDepth;
+#pragma unroll 1
+        for (int part = 0; part < 3 && good; ++part) {
+          const int depth = part == 0 ? gram : tile.depth;
+          float acc[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) acc[e] = 0.0f;
+          for (int k = 0; k < depth; k += kSegment) {
+            good = __all_sync(0xffffffffu, mbar_wait(ready + half, half_parity));
+            if (!good) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            uint32_t sum[32];
+            load32(sum, tmem + half * kTile + col + ((uint32_t)(quarter * 32) << 16));
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) arrive(spent + half);
+            half ^= 1;
+            if (half == 0) half_parity ^= 1;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) acc[e] += __uint_as_float(sum[e]);
+          }
+          if (!good) break;
+          if (part == 2) {
+            finish(p, step + 1 < p.steps ? kUpdate : kLast, from, it, tile, row, col, acc, skip);
+            break;
+          }
+          const float one = part == 0 ? 0.0f : p.ca * kScale;
+#pragma unroll
+          for (int k = 0; k < 32; k += 8) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = acc[k + j] * (1.0f / kScale) + (col + k + j == row && row < it.n ? one : 0.0f);
+            put_shared(squares, row, col + k, v);
+            if (part == 0) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[j] = p.cc * v[j] + (col + k + j == row && row < it.n ? p.cb * kScale : 0.0f);
+              put_shared(squares + 2 * kPair, row, col + k, v);
+            }
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) arrive(&made);
+        }
+      }
+      if (!good && lane == 0) {
+        atomicOr(p.error, 4u);
+        s_stop = 1;
+      }
+    }
+    __syncwarp();
+    met += gridDim.x;
+    if (step + 1 < p.steps) {
+      good = meet(p.arrived, met, s_stop) && good;
+      if (s_stop) {
+        if (threadIdx.x == 0) atomicOr(p.error, 8u);
+        break;
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem) : "memory");
+  }
+}
+
 // --------------------------------------------------------------------------------------------- launches
 
 uint32_t* error_word() {
@@ -645,7 +840,11 @@ int64_t matrix_bytes(int64_t rows, int64_t cols) {
 }
 int64_t norm_blocks(int64_t rows, int64_t cols) { return (rows * cols + kNormValues - 1) / kNormValues; }
 
-// Matrices that go together: as many as the table and the workspace's share hold
+bool narrow(const Matrix& m) {
+  return std::min(m.rows, m.cols) <= kTile && std::max(m.rows, m.cols) <= kNarrowTiles * kTile;
+}
+
+// Matrices that go together, narrow ones or others: as many as the table and the workspace's share hold
 template <class F>
 void groups(const std::vector<Matrix>& all, F f) {
   for (size_t first = 0; first < all.size();) {
@@ -654,7 +853,7 @@ void groups(const std::vector<Matrix>& all, F f) {
     while (first + n < all.size() && n < kItems) {
       const Matrix& m = all[first + n];
       const int64_t more = matrix_bytes(m.rows, m.cols);
-      if (n > 0 && bytes + more > kGroupBytes) break;
+      if (n > 0 && (bytes + more > kGroupBytes || narrow(m) != narrow(all[first]))) break;
       bytes += more;
       norms += norm_blocks(m.rows, m.cols);
       ++n;
@@ -710,11 +909,13 @@ cudaError_t run_group(const Call& call, const Matrix* all, int n, int64_t bytes,
     a.squares += it.nt * (it.nt + 1) / 2;
     a.wides += it.nt * it.mt;
   }
-  cudaError_t e = cudaFuncSetAttribute(products_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared);
+  const bool thin = narrow(all[0]);  // (all of them)
+  void (*const kernel)(Args<N>) = thin ? narrow_kernel<N> : products_kernel<N>;
+  const int shared = thin ? kNarrowShared : kShared, tiles = thin ? a.wides : std::max(a.squares, a.wides);
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
   if (e == cudaSuccess) e = start(momentum_kernel<N>, norms, kPrepThreads, 0, false, s, a);
   if (e == cudaSuccess) e = start(prepare_kernel<N>, preps, kPrepThreads, 0, false, s, a);
-  if (e == cudaSuccess)
-    e = start(products_kernel<N>, std::min(sms(), std::max(a.squares, a.wides)), kThreads, kShared, true, s, a);
+  if (e == cudaSuccess) e = start(kernel, std::min(sms(), tiles), kThreads, shared, true, s, a);
   return e;
 }
 
@@ -768,6 +969,7 @@ int muon_matrices(const pesq_muon_desc* d, const pesq_muon_tensor* tensors, int6
                                                           : 0.2 * std::sqrt((double)std::max(t.rows, t.cols));
     all.push_back({t.param, t.momentum, t.grad, t.copy, t.rows, t.cols, (float)(d->lr * adjust)});
   }
+  std::stable_partition(all.begin(), all.end(), narrow);
   return PESQ_OK;
 }
 
