@@ -51,9 +51,13 @@ struct Args {
 
 // CTAs that an SM holds, which the registers of a thread follow from
 constexpr int ctas(bool backward, int team, int groups) {
-  const int threads = team > kThreads ? team : kThreads, sm = groups == 4 ? (backward ? 256 : 384) : (backward ? 512 : 1024);
+  const int threads = team > kThreads ? team : kThreads;
+  const int sm = groups == 4 ? (backward ? 256 : 384) : groups == 2 ? (backward ? 384 : 640) : (backward ? 512 : 1024);
   return sm / threads > 0 ? sm / threads : 1;
 }
+
+// Eights of channels of a thread at most: channel by channel (kWide false) a backward of four spills
+constexpr int most_groups(bool wide) { return wide ? 4 : 2; }
 
 // A thread's channels of a row: groups of eight, 8 TEAM channels apart
 template <class T, int TEAM, int GROUPS, bool kWide>

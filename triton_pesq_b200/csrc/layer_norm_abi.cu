@@ -84,7 +84,7 @@ bool wide(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 // threads of a row, and eights of channels of each
 void team_of(int64_t width, Geometry& g) {
   g.team = 4, g.groups = 1;
-  while (g.team * g.groups * kEach < width) (g.team < 32 || g.groups == 4 ? g.team : g.groups) *= 2;
+  while (g.team * g.groups * kEach < width) (g.team < 32 || g.groups == most_groups(g.wide) ? g.team : g.groups) *= 2;
 }
 
 struct Plan {
@@ -96,15 +96,16 @@ struct Plan {
 // As many CTAs as the device holds at once, each with its share of the rows, but none with less than a row a team.
 // A CTA's teams take the heads side by side: of the numbers of heads that leave the fewest teams idle the largest, so that
 // neighbouring heads, whose rows are neighbours in memory, are read together.
-Plan plan(const pesq_layer_norm_desc& d, bool backward, const pesq_heads* dy) {
+Plan plan(const pesq_layer_norm_desc& d, bool backward, const pesq_heads* dy, const void* result) {
   Plan q{};
   const pesq_heads none{nullptr, 0, 0, 0};
   const pesq_heads& g = dy ? *dy : none;
   const bool flat = joined(d.x, d) && joined(g, d);
   q.batch = flat ? 1 : d.batch;
   q.steps = flat ? d.batch * d.steps : d.steps;
+  q.g.wide = d.width % kEach == 0 && wide(d.x, d, d.dtype) && wide(g, d, d.out_dtype) && wide(d.weight) && wide(d.bias) &&
+             wide(result);
   team_of(d.width, q.g);
-  q.g.wide = d.width % kEach == 0 && wide(d.x, d, d.dtype) && wide(g, d, d.out_dtype) && wide(d.weight) && wide(d.bias);
   const int threads = std::max(q.g.team, kThreads), teams = threads / q.g.team;
   double best = -1.0;
   for (int h = 1; h <= std::min<int64_t>(teams, d.heads); ++h) {
@@ -123,8 +124,8 @@ Plan plan(const pesq_layer_norm_desc& d, bool backward, const pesq_heads* dy) {
 }
 
 size_t part_bytes(const pesq_layer_norm_desc& d) {
-  const Plan q = plan(d, true, nullptr);  // (its units follow from the sizes alone)
-  return ((size_t)q.units * d.heads * d.width * 4 + 15) / 16 * 16;
+  // (however the operands lie, no more CTAs than this over the rows: four an SM, and the fewest of a head)
+  return ((size_t)(148 * 4) * d.heads * d.width * 4 + 15) / 16 * 16;
 }
 
 Strided rows_of(const pesq_heads& s) { return {s.data, s.batch_stride, s.step_stride, s.head_stride}; }
@@ -162,8 +163,7 @@ extern "C" {
 int pesq_layer_norm_forward(const pesq_layer_norm_desc* d, void* stream, void* y) {
   if (const int status = check(d)) return status;
   if (!d->x.data || !d->weight || !y) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL operand");
-  Plan q = plan(*d, false, nullptr);
-  q.g.wide = q.g.wide && wide(y);
+  const Plan q = plan(*d, false, nullptr, y);
   Args a = arguments(*d, q);
   a.y = y;
   const cudaError_t e = run(a, q, *d, false, static_cast<cudaStream_t>(stream));
@@ -184,8 +184,7 @@ int pesq_layer_norm_backward(const pesq_layer_norm_desc* d, void* stream, pesq_h
     return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL operand");
   if (!workspace || workspace_bytes < part_bytes(*d) * 2 || reinterpret_cast<uintptr_t>(workspace) % 16)
     return set_error(PESQ_ERR_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
-  Plan q = plan(*d, true, &dy);
-  q.g.wide = q.g.wide && wide(dx);
+  const Plan q = plan(*d, true, &dy, dx);
   Args a = arguments(*d, q);
   a.dy = rows_of(dy);
   a.dx = dx;

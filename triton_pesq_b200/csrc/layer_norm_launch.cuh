@@ -7,33 +7,39 @@
 namespace pesq {
 namespace lnorm {
 
-template <class TX, class TY, int TEAM, int GROUPS>
+template <class TX, class TY, int TEAM, int GROUPS, bool kWide>
 cudaError_t launch_team(const Args& p, const Geometry& g, bool backward, cudaStream_t s) {
-  const unsigned grid = (unsigned)g.blocks;
   constexpr int threads = TEAM > kThreads ? TEAM : kThreads;
   if (backward)
-    g.wide ? backward_kernel<TX, TY, TEAM, GROUPS, true><<<grid, threads, 0, s>>>(p)
-           : backward_kernel<TX, TY, TEAM, GROUPS, false><<<grid, threads, 0, s>>>(p);
+    backward_kernel<TX, TY, TEAM, GROUPS, kWide><<<(unsigned)g.blocks, threads, 0, s>>>(p);
   else
-    g.wide ? forward_kernel<TX, TY, TEAM, GROUPS, true><<<grid, threads, 0, s>>>(p)
-           : forward_kernel<TX, TY, TEAM, GROUPS, false><<<grid, threads, 0, s>>>(p);
+    forward_kernel<TX, TY, TEAM, GROUPS, kWide><<<(unsigned)g.blocks, threads, 0, s>>>(p);
   return cudaGetLastError();
+}
+
+template <class TX, class TY, bool kWide>
+cudaError_t launch_width(const Args& p, const Geometry& g, bool backward, cudaStream_t s) {
+  constexpr int kMost = most_groups(kWide);
+  switch (g.team) {
+    case 4: return launch_team<TX, TY, 4, 1, kWide>(p, g, backward, s);
+    case 8: return launch_team<TX, TY, 8, 1, kWide>(p, g, backward, s);
+    case 16: return launch_team<TX, TY, 16, 1, kWide>(p, g, backward, s);
+    case 32:
+      if (g.groups == 1) return launch_team<TX, TY, 32, 1, kWide>(p, g, backward, s);
+      if (g.groups == 2) return launch_team<TX, TY, 32, 2, kWide>(p, g, backward, s);
+      return launch_team<TX, TY, 32, kMost, kWide>(p, g, backward, s);
+    case 64: return launch_team<TX, TY, 64, kMost, kWide>(p, g, backward, s);
+    case 128: return launch_team<TX, TY, 128, kMost, kWide>(p, g, backward, s);
+    case 256: return launch_team<TX, TY, 256, kMost, kWide>(p, g, backward, s);
+    default:
+      if constexpr (kMost < 4) return launch_team<TX, TY, 512, kMost, kWide>(p, g, backward, s);
+      return cudaErrorInvalidConfiguration;
+  }
 }
 
 template <class TX, class TY>
 cudaError_t launch(const Args& p, const Geometry& g, bool backward, cudaStream_t s) {
-  switch (g.team) {
-    case 4: return launch_team<TX, TY, 4, 1>(p, g, backward, s);
-    case 8: return launch_team<TX, TY, 8, 1>(p, g, backward, s);
-    case 16: return launch_team<TX, TY, 16, 1>(p, g, backward, s);
-    case 32:
-      return g.groups == 1   ? launch_team<TX, TY, 32, 1>(p, g, backward, s)
-             : g.groups == 2 ? launch_team<TX, TY, 32, 2>(p, g, backward, s)
-                             : launch_team<TX, TY, 32, 4>(p, g, backward, s);
-    case 64: return launch_team<TX, TY, 64, 4>(p, g, backward, s);
-    case 128: return launch_team<TX, TY, 128, 4>(p, g, backward, s);
-    default: return launch_team<TX, TY, 256, 4>(p, g, backward, s);
-  }
+  return g.wide ? launch_width<TX, TY, true>(p, g, backward, s) : launch_width<TX, TY, false>(p, g, backward, s);
 }
 
 }  // namespace lnorm
