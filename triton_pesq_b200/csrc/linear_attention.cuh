@@ -412,6 +412,39 @@ __device__ __forceinline__ void load_tile(T* tile, const Operand& o, int first, 
     }
     return;
   }
+  if constexpr (sizeof(T) == 2) {
+    if (o.unit == 2) {
+      // the aligned words that hold some of the piece, shifted into place; those of several rows on their way together
+      constexpr int kTogether = C / kRows < 4 ? C / kRows : 4;
+      const int count = min(16, bytes) / 2;  // elements
+#pragma unroll 1
+      for (int k0 = 0; k0 < C / kRows; k0 += kTogether) {
+        uint32_t w[kTogether][5];
+#pragma unroll
+        for (int k = 0; k < kTogether; ++k) {
+          const bool live = s0 + r0 + (k0 + k) * kRows < row.n;
+          const uintptr_t at = reinterpret_cast<uintptr_t>(from) + (k0 + k) * kRows * step;
+          const uint32_t* words = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
+          const int last = (int)((at & 3) + 2 * count + 3) / 4;  // words
+#pragma unroll
+          for (int i = 0; i < 5; ++i) w[k][i] = live && i < last ? words[i] : 0u;
+        }
+#pragma unroll
+        for (int k = 0; k < kTogether; ++k) {
+          const uint32_t shift = ((reinterpret_cast<uintptr_t>(from) + (k0 + k) * kRows * step) & 2) * 8;
+          uint32_t v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            v[i] = __funnelshift_r(w[k][i], w[k][i + 1], shift);
+            v[i] = 2 * i + 1 < count ? v[i] : 2 * i < count ? v[i] & 0xffffu : 0u;
+          }
+          *reinterpret_cast<uint4*>(reinterpret_cast<char*>(tile + (r0 + (k0 + k) * kRows) * LD) + piece * 16) =
+              make_uint4(v[0], v[1], v[2], v[3]);
+        }
+      }
+      return;
+    }
+  }
 #pragma unroll 1
   for (int k = 0; k < C / kRows; ++k) {
     const bool live = s0 + r0 + k * kRows < row.n;
@@ -425,16 +458,11 @@ __device__ __forceinline__ void load_tile(T* tile, const Operand& o, int first, 
       for (int x = 0; x < 16; x += 8)
         if (x < bytes)
           asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to + x), "l"(live ? at + x : at), "r"(live ? 8 : 0) : "memory");
-    } else if (o.unit == 4) {
+    } else {
 #pragma unroll
       for (int x = 0; x < 16; x += 4)
         if (x < bytes)
           asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + x), "l"(live ? at + x : at), "r"(live ? 4 : 0) : "memory");
-    } else {
-      char* generic = reinterpret_cast<char*>(tile + (r0 + k * kRows) * LD) + piece * 16;
-#pragma unroll
-      for (int x = 0; x < 16; x += 2)
-        if (x < bytes) *reinterpret_cast<uint16_t*>(generic + x) = live ? *reinterpret_cast<const uint16_t*>(at + x) : (uint16_t)0;
     }
     from += kRows * step;
   }
@@ -571,19 +599,29 @@ struct State {
   float x[Shape::kTiles][Shape::kCols / 8][4];
 
   // (warps past the first WARPS have no part in it)
-  static __device__ __forceinline__ int row0() { return (threadIdx.x >> 5) % Shape::kRowWarps * Shape::kTiles * 16; }
-  static __device__ __forceinline__ int col0() { return (threadIdx.x >> 5) / Shape::kRowWarps * Shape::kCols; }
-  // f(row, column, value of it, of the next column), rows and columns of the state
+  // its tiles of 16 rows and blocks of 16 columns lie in turn with the other warps', so that a state narrower than DK x DV
+  // is shared out evenly too
+  static __device__ __forceinline__ int row_of(int tile) {
+    return (tile * Shape::kRowWarps + (int)(threadIdx.x >> 5) % Shape::kRowWarps) * 16;
+  }
+  static __device__ __forceinline__ int col_of(int block) {
+    return (block * Shape::kColWarps + (int)(threadIdx.x >> 5) / Shape::kRowWarps) * 16;
+  }
+  // f(row, column, value of it, of the next column), rows and columns of the state, of tiles within `rows` and `cols`
   template <class F>
-  __device__ __forceinline__ void each(F f) {
+  __device__ __forceinline__ void each(F f, int rows = DK, int cols = DV) {
     const int g = (threadIdx.x & 31) >> 2, c = threadIdx.x & 3;
 #pragma unroll
-    for (int m = 0; m < Shape::kTiles; ++m)
+    for (int m = 0; m < Shape::kTiles; ++m) {
+      if (row_of(m) >= rows) continue;
 #pragma unroll
-      for (int n = 0; n < Shape::kCols / 8; ++n)
+      for (int n = 0; n < Shape::kCols / 8; ++n) {
+        if (col_of(n / 2) >= cols) continue;
 #pragma unroll
         for (int half = 0; half < 2; ++half)
-          f(row0() + m * 16 + g + half * 8, col0() + n * 8 + 2 * c, x[m][n][2 * half], x[m][n][2 * half + 1]);
+          f(row_of(m) + g + half * 8, col_of(n / 2) + n % 2 * 8 + 2 * c, x[m][n][2 * half], x[m][n][2 * half + 1]);
+      }
+    }
   }
   // from a dense [key, value] matrix's columns from `first`, or zeros
   __device__ __forceinline__ void read(const float* from, int key, int value, int first) {
@@ -602,7 +640,7 @@ struct State {
   // S = factor S + sum over the chunk's steps of weight a b^T.  The chunk's sum is made by itself and added, rounded: the
   // instruction cuts off what its accumulator does not hold, which over the chunks that a slow head remembers is 1e-5.
   template <class T, int C>
-  __device__ __forceinline__ void update(const T* a, const T* b, const float* weights, float factor, float scale) {
+  __device__ __forceinline__ void update(const T* a, const T* b, const float* weights, float factor, float scale, int rows, int cols) {
     const int c = threadIdx.x & 3;
     if (factor == 0.0f) {  // (cuts off whatever the state holds)
 #pragma unroll
@@ -615,6 +653,7 @@ struct State {
     constexpr int kBlocks = C / 16, kTogether = std::is_same<T, __nv_bfloat16>::value ? kBlocks : 2;  // of registers' worth
 #pragma unroll
     for (int m = 0; m < Shape::kTiles; ++m) {
+      if (row_of(m) >= rows) continue;
 #pragma unroll
       for (int k0 = 0; k0 < kBlocks; k0 += kTogether) {
         Made<T> left[kTogether];
@@ -624,18 +663,19 @@ struct State {
           const float2 w0 = *reinterpret_cast<const float2*>(weights + at + 2 * c);
           const float2 w1 = *reinterpret_cast<const float2*>(weights + at + 8 + 2 * c);
           float f[8];
-          load_a<T, kLd<T, DK>, true>(f, a, row0() + m * 16, at);
+          load_a<T, kLd<T, DK>, true>(f, a, row_of(m), at);
           f[0] *= w0.x * scale, f[1] *= w0.y * scale, f[2] *= w0.x * scale, f[3] *= w0.y * scale;
           f[4] *= w1.x * scale, f[5] *= w1.y * scale, f[6] *= w1.x * scale, f[7] *= w1.y * scale;
           make(left[k], f);
         }
 #pragma unroll
         for (int n = 0; n < Shape::kCols / 16; ++n) {
+          if (col_of(n) >= cols) continue;
           float sum[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
           for (int k = 0; k < kTogether; ++k) {
             InB<T> right[2];
-            load_b<T, kLd<T, DV>, true>(right, b, col0() + n * 16, (k0 + k) * 16);
+            load_b<T, kLd<T, DV>, true>(right, b, col_of(n), (k0 + k) * 16);
             mma(sum[0], left[k], right[0]);
             mma(sum[1], left[k], right[1]);
           }
@@ -652,8 +692,9 @@ struct State {
   }
   // to shared memory, as an operand
   template <class T>
-  __device__ __forceinline__ void publish(Stored<T>* s) {
-    each([&](int r, int c, float& a, float& b) { store_state<T, kLd<Stored<T>, DV>, DK * kLd<Stored<T>, DV>>(s, r, c, a, b); });
+  __device__ __forceinline__ void publish(Stored<T>* s, int rows, int cols) {
+    each([&](int r, int c, float& a, float& b) { store_state<T, kLd<Stored<T>, DV>, DK * kLd<Stored<T>, DV>>(s, r, c, a, b); },
+         rows, cols);
   }
 };
 
@@ -671,10 +712,12 @@ __device__ __forceinline__ uint32_t narrow_pair(float x, float y, __half) {
   return r;
 }
 __device__ __forceinline__ float2 narrow_pair(float x, float y, float) { return make_float2(x, y); }
-// A warp's 16 rows of N times 8 columns from col (the thread's first) to rows of `width`: those of steps s and s + 8, where
-// they are within the row; zeros past its length
-template <class T, int N>
+// A warp's 16 rows of N times 8 columns to rows of `width`: those of steps s and s + 8, where they are within the row; zeros
+// past its length.  The columns are blocks of 16, WC blocks apart, the thread's first at col
+template <class T, int WC, int N>
 __device__ __forceinline__ void store_rows(void* base, const Args& p, const Row& row, int64_t s, int width, int col, const float (&x)[N][4]) {
+  constexpr auto column = [](int n) { return n / 2 * WC * 16 + n % 2 * 8; };
+  constexpr int kLast = (N - 1) / 2 * WC * 16 + (N - 1) % 2 * 8;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int64_t at = s + 8 * half;
@@ -685,19 +728,19 @@ __device__ __forceinline__ void store_rows(void* base, const Args& p, const Row&
     if (width % 2 == 0) {
       using Pair = decltype(narrow_pair(0.0f, 0.0f, T{}));
       Pair* pairs = reinterpret_cast<Pair*>(to);
-      if (live && (N - 1) * 8 < left) {
+      if (live && kLast < left) {
 #pragma unroll
-        for (int n = 0; n < N; ++n) pairs[n * 4] = narrow_pair(x[n][2 * half], x[n][2 * half + 1], T{});
+        for (int n = 0; n < N; ++n) pairs[column(n) / 2] = narrow_pair(x[n][2 * half], x[n][2 * half + 1], T{});
       } else {
 #pragma unroll
         for (int n = 0; n < N; ++n)
-          if (n * 8 < left) pairs[n * 4] = narrow_pair(live ? x[n][2 * half] : 0.0f, live ? x[n][2 * half + 1] : 0.0f, T{});
+          if (column(n) < left) pairs[column(n) / 2] = narrow_pair(live ? x[n][2 * half] : 0.0f, live ? x[n][2 * half + 1] : 0.0f, T{});
       }
     } else {
 #pragma unroll
       for (int n = 0; n < N; ++n) {
-        if (n * 8 < left) to[n * 8] = narrow<T>(live ? x[n][2 * half] : 0.0f);
-        if (n * 8 + 1 < left) to[n * 8 + 1] = narrow<T>(live ? x[n][2 * half + 1] : 0.0f);
+        if (column(n) < left) to[column(n)] = narrow<T>(live ? x[n][2 * half] : 0.0f);
+        if (column(n) + 1 < left) to[column(n) + 1] = narrow<T>(live ? x[n][2 * half + 1] : 0.0f);
       }
     }
   }
@@ -720,11 +763,12 @@ __device__ __forceinline__ void clear(void* p, int bytes) {
 template <class T>
 constexpr int kUnroll = std::is_same<T, __nv_bfloat16>::value ? 4 : 1;
 
-// 16 rows of a from m0 times 16 rows of b from n0, over their D channels
+// 16 rows of a from m0 times 16 rows of b from n0, over their channels, `width` of at most D
 template <class T, int D>
-__device__ __forceinline__ void products(float (&sum)[2][4], const T* a, int m0, const T* b, int n0) {
+__device__ __forceinline__ void products(float (&sum)[2][4], const T* a, int m0, const T* b, int n0, int width) {
 #pragma unroll kUnroll<T>
   for (int kk = 0; kk < D; kk += 16) {
+    if (kk >= width) break;
     InA<T> left;
     InB<T> right[2];
     load_a<T, kLd<T, D>>(left, a, m0, kk);
@@ -733,6 +777,61 @@ __device__ __forceinline__ void products(float (&sum)[2][4], const T* a, int m0,
     mma(sum[1], left, right[1]);
   }
 }
+
+// 16 rows of a from m0, over their channels, `width` of at most D, times a state's columns (kTrans; else its rows), those of the
+// blocks of 16 in turn from wc that lie within `cols`
+template <class T, int D, int LDS, int PLANE, bool kTrans, int WC, int N>
+__device__ __forceinline__ void times_state(float (&out)[N][4], const T* a, int m0, const Stored<T>* state, int wc, int width, int cols) {
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[n][e] = 0.0f;
+#pragma unroll kUnroll<T>
+  for (int kk = 0; kk < D; kk += 16) {
+    if (kk >= width) break;
+    InA<T> left;
+    load_a<T, kLd<T, D>>(left, a, m0, kk);
+#pragma unroll
+    for (int n = 0; n < N / 2; ++n) {
+      if ((n * WC + wc) * 16 >= cols) continue;
+      MadeB<T> right[2];
+      load_state<T, LDS, PLANE, kTrans>(right, state, (n * WC + wc) * 16, kk);
+      mma(out[2 * n], left, right[0]);
+      mma(out[2 * n + 1], left, right[1]);
+    }
+  }
+}
+// A computed 16 x 16 block times 16 rows of b from k0, the same columns of it
+template <class T, int LD, int WC, int N>
+__device__ __forceinline__ void add_product(float (&out)[N][4], const Made<T>& left, const T* b, int k0, int wc, int cols) {
+#pragma unroll
+  for (int n = 0; n < N / 2; ++n) {
+    if ((n * WC + wc) * 16 >= cols) continue;
+    InB<T> right[2];
+    load_b<T, LD, true>(right, b, (n * WC + wc) * 16, k0);
+    mma(out[2 * n], left, right[0]);
+    mma(out[2 * n + 1], left, right[1]);
+  }
+}
+// sums over the same columns of x times a tile's rows i0 and i0 + 8; in every lane of a row
+template <class T, int LD, int WC, int N>
+__device__ __forceinline__ float2 row_sums(const float (&x)[N][4], const T* tile, int i0, int wc) {
+  float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const T* at = tile + i0 * LD + (n / 2 * WC + wc) * 16 + n % 2 * 8 + 2 * (threadIdx.x & 3);
+    const float2 a = two_of(at), b = two_of(at + 8 * LD);
+    s0 = fmaf(x[n][0], a.x, fmaf(x[n][1], a.y, s0));
+    s1 = fmaf(x[n][2], b.x, fmaf(x[n][3], b.y, s1));
+  }
+#pragma unroll
+  for (int off = 1; off < 4; off <<= 1) {
+    s0 += __shfl_xor_sync(0xffffffffu, s0, off);
+    s1 += __shfl_xor_sync(0xffffffffu, s1, off);
+  }
+  return make_float2(s0, s1);
+}
+__device__ __forceinline__ int sixteens(int n) { return (n + 15) & ~15; }
 
 // ------------------------------------------------------------------------------------------- forward
 
@@ -747,7 +846,9 @@ struct ForwardShared {
   static constexpr int kBytes = kStages * kTiles + kState + kDecays;
 };
 
-template <class T, int DK, int DV, int C>
+// kWhole: keys and values fill DK and DV (the loops over less would keep the compiler from mixing their rounds: 20 % of a
+// forward and 35 % of a backward)
+template <class T, int DK, int DV, int C, bool kWhole>
 __global__ void __launch_bounds__(128, DK > 64 ? 2 : 3) forward_kernel(const __grid_constant__ Args p) {
   constexpr int THREADS = 128, WARPS = 4, RG = C / 16, WC = WARPS / RG, NY = DV / WC / 8;
   using Sh = ForwardShared<T, DK, DV, C>;
@@ -766,6 +867,7 @@ __global__ void __launch_bounds__(128, DK > 64 ? 2 : 3) forward_kernel(const __g
   const int first = slice * DV, cols = min(DV, p.value - first);
   const int c0 = part * p.part_chunks, c1 = min(p.chunks, c0 + p.part_chunks);
   const int padded = DV * p.slices;  // columns of the states in memory
+  const int key = kWhole ? DK : sixteens(p.key), value = kWhole ? DV : sixteens(cols);
 
   clear<THREADS>(shared, Sh::kStages * Sh::kTiles);
   State<DK, DV, WARPS> S;
@@ -774,7 +876,7 @@ __global__ void __launch_bounds__(128, DK > 64 ? 2 : 3) forward_kernel(const __g
     S.read(p.starts + (index * p.parts + part) * DK * padded, DK, padded, first);
   else
     S.read(from, p.key, p.value, first);
-  S.template publish<T>(s_state);
+  S.template publish<T>(s_state, key, value);
   __syncthreads();
 
   const auto q_of = [&](int stage) { return reinterpret_cast<T*>(tiles + stage * Sh::kTiles); };
@@ -810,60 +912,48 @@ __global__ void __launch_bounds__(128, DK > 64 ? 2 : 3) forward_kernel(const __g
     if (live && p.kept) {
       // the state before the chunk, for the backward: 16-byte pieces of the operand's planes
       constexpr int kPieces = DV * (int)sizeof(Stored<T>) / 16;
-      char* to = static_cast<char*>(p.kept) + (index * p.chunks + chunk) * kept_bytes(DK, padded) + first * (int)sizeof(Stored<T>);
-      for (int i = threadIdx.x; i < kPlanes<T> * DK * kPieces; i += THREADS) {
-        const int r = i / kPieces, piece = i % kPieces;  // (rows of both planes, one after the other)
-        *reinterpret_cast<uint4*>(to + (int64_t)r * padded * (int)sizeof(Stored<T>) + piece * 16) =
-            *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(s_state + r * LDS) + piece * 16);
+      const int piece = threadIdx.x % kPieces, apart = padded * (int)sizeof(Stored<T>);
+      char* to = static_cast<char*>(p.kept) + (index * p.chunks + chunk) * kept_bytes(DK, padded) + first * (int)sizeof(Stored<T>) + piece * 16;
+      if (piece * 16 < value * (int)sizeof(Stored<T>)) {
+#pragma unroll
+        for (int plane = 0; plane < kPlanes<T>; ++plane)
+#pragma unroll 4
+          for (int r = threadIdx.x / kPieces; r < key; r += THREADS / kPieces)
+            *reinterpret_cast<uint4*>(to + (int64_t)(plane * DK + r) * apart) =
+                *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(s_state + plane * PLANE + r * LDS) + piece * 16);
       }
     }
     float y[NY][4];
-#pragma unroll
-    for (int n = 0; n < NY; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[n][e] = 0.0f;
     if (live) {
       const int i0 = rg * 16 + g;
-#pragma unroll kUnroll<T>
-      for (int kk = 0; kk < DK; kk += 16) {
-        InA<T> left;
-        load_a<T, LDK>(left, q, rg * 16, kk);
-#pragma unroll
-        for (int n = 0; n < NY / 2; ++n) {
-          MadeB<T> right[2];
-          load_state<T, LDS, PLANE, true>(right, s_state, wc * NY * 8 + n * 16, kk);
-          mma(y[2 * n], left, right[0]);
-          mma(y[2 * n + 1], left, right[1]);
-        }
-      }
+      times_state<T, DK, LDS, PLANE, true, WC>(y, q, rg * 16, s_state, wc, key, value);
       decay_rows(y, before[i0] * p.scale, before[i0 + 8] * p.scale);
       // sixteen steps j at a time, up to the warp's own
 #pragma unroll 1
       for (int n = 0; n <= rg; ++n) {
         float a[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-        products<T, DK>(a, q, rg * 16, k, n * 16);
+        products<T, DK>(a, q, rg * 16, k, n * 16, key);
         float w[8], x[8];
         weights_by_row(w, sums, tail, i0, n * 16, n == rg, p.scale);
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = a[e >> 2][e & 3] * w[e];
         Made<T> left;
         make(left, x);
-#pragma unroll
-        for (int m = 0; m < NY / 2; ++m) {
-          InB<T> right[2];
-          load_b<T, LDV, true>(right, v, wc * NY * 8 + m * 16, n * 16);
-          mma(y[2 * m], left, right[0]);
-          mma(y[2 * m + 1], left, right[1]);
-        }
+        add_product<T, LDV, WC>(y, left, v, n * 16, wc, value);
       }
-      S.template update<T, C>(k, v, after, before[C - 1], 1.0f);
+      S.template update<T, C>(k, v, after, before[C - 1], 1.0f, key, value);
+    } else {
+#pragma unroll
+      for (int n = 0; n < NY; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[n][e] = 0.0f;
     }
-    store_rows<T>(p.y, p, row, s0 + rg * 16 + g, p.value, first + wc * NY * 8 + 2 * c, y);
+    store_rows<T, WC>(p.y, p, row, s0 + rg * 16 + g, p.value, first + wc * 16 + 2 * c, y);
     if (warp == WARPS - 1 && chunk + 1 < c1) {
       next.store(sums_of(chunk + 1));
     }
     __syncthreads();  // the chunk's tiles and state are read
-    if (live) S.template publish<T>(s_state);
+    if (live) S.template publish<T>(s_state, key, value);
     if (Sh::kStages == 1 && chunk + 1 < c1) load(chunk + 1, 0);
   }
   if (p.last && c1 == p.chunks) S.write(p.last + index * p.key * p.value, p.key, p.value, first);
@@ -879,7 +969,7 @@ struct SweepShared {
   static constexpr int kDecays = kDecayBytes<C>;
   static constexpr int kBytes = 2 * kTiles + kDecays;
 };
-template <class T, int DK, int DV, int C, bool kBackward>
+template <class T, int DK, int DV, int C, bool kWhole, bool kBackward>
 __global__ void __launch_bounds__(128) sweep_kernel(const __grid_constant__ Args p) {
   constexpr int THREADS = 128, WARPS = 4;
   using Sh = SweepShared<T, DK, DV, C>;
@@ -931,7 +1021,8 @@ __global__ void __launch_bounds__(128) sweep_kernel(const __grid_constant__ Args
     if ((int64_t)chunk_of(i) * C < row.n) {
       const T* a = reinterpret_cast<const T*>(shared + (i & 1) * Sh::kTiles);
       const float *before = reinterpret_cast<const float*>(sums_of(i) + C), *after = before + C;
-      S.template update<T, C>(a, a + C * LDK, kBackward ? before : after, before[C - 1], kBackward ? p.scale : 1.0f);
+      S.template update<T, C>(a, a + C * LDK, kBackward ? before : after, before[C - 1], kBackward ? p.scale : 1.0f,
+                              kWhole ? DK : sixteens(p.key), kWhole ? DV : sixteens(cols));
       factor *= before[C - 1];
     }
     if (warp == WARPS - 1 && i + 1 < count) store(i + 1);
@@ -989,7 +1080,7 @@ struct BackwardShared {
   static constexpr int kBytes = kTiles + 2 * kState + kDecays + kSums;
 };
 
-template <class T, int DK, int DV, int C>
+template <class T, int DK, int DV, int C, bool kWhole>
 __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ? 2 : 1)
     backward_kernel(const __grid_constant__ Args p) {
   using Sh = BackwardShared<T, DK, DV, C>;
@@ -1015,6 +1106,8 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
   const Row row(p, index);
   const int c0 = part * p.part_chunks, c1 = min(p.chunks, c0 + p.part_chunks);
 
+  const int key = kWhole ? DK : sixteens(p.key), value = kWhole ? DV : sixteens(p.value);
+
   clear<THREADS>(shared, Sh::kTiles);
   State<DK, DV, SIDE> S;  // the gradient of the state, of the warps by rows
   if (by_rows) {
@@ -1023,7 +1116,7 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
       S.read(p.starts + (index * p.parts + part) * DK * DV, DK, DV, 0);
     else
       S.read(from, p.key, p.value, 0);
-    S.template publish<T>(s_grad);
+    S.template publish<T>(s_grad, key, value);
   }
   __syncthreads();
 
@@ -1034,14 +1127,17 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
       load_tile<T, DK, C, THREADS>(k, p.k, 0, p.key, row, s0);
       load_tile<T, DV, C, THREADS>(v, p.v, 0, p.value, row, s0);
       load_tile<T, DV, C, THREADS>(dy, p.dy, 0, p.value, row, s0);
-      constexpr int kPieces = DV * (int)sizeof(Stored<T>) / 16, kAll = kPlanes<T> * DK * kPieces;
-      const char* at = static_cast<const char*>(p.kept) + (index * p.chunks + chunk) * kept_bytes(DK, DV);
+      constexpr int kPieces = DV * (int)sizeof(Stored<T>) / 16;
+      const int piece = threadIdx.x % kPieces;
+      const char* at = static_cast<const char*>(p.kept) + (index * p.chunks + chunk) * kept_bytes(DK, DV) + piece * 16;
+      if (piece * 16 < value * (int)sizeof(Stored<T>)) {
+#pragma unroll
+        for (int plane = 0; plane < kPlanes<T>; ++plane)
 #pragma unroll 4
-      for (int i = threadIdx.x; i < kAll; i += THREADS) {
-        const int r = i / kPieces, piece = i % kPieces;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                         smem_of(reinterpret_cast<const char*>(s_state + r * LDS) + piece * 16)),
-                     "l"(at + (int64_t)i * 16) : "memory");
+          for (int r = threadIdx.x / kPieces; r < key; r += THREADS / kPieces)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                             smem_of(reinterpret_cast<const char*>(s_state + plane * PLANE + r * LDS) + piece * 16)),
+                         "l"(at + (int64_t)(plane * DK + r) * (DV * (int)sizeof(Stored<T>))) : "memory");
       }
     }
     copies_issued();
@@ -1069,122 +1165,58 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
     const int i0 = rg * 16 + g;  // the warp's rows are i0 and i0 + 8, i or j
     if (by_rows) {
       float dq[NK][4];
-#pragma unroll
-      for (int n = 0; n < NK; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) dq[n][e] = 0.0f;
       if (live) {
-#pragma unroll kUnroll<T>
-        for (int kk = 0; kk < DV; kk += 16) {
-          InA<T> left;
-          load_a<T, LDV>(left, dy, rg * 16, kk);
-#pragma unroll
-          for (int n = 0; n < NK / 2; ++n) {
-            MadeB<T> right[2];
-            load_state<T, LDS, PLANE, false>(right, s_state, wc * NK * 8 + n * 16, kk);
-            mma(dq[2 * n], left, right[0]);
-            mma(dq[2 * n + 1], left, right[1]);
-          }
-        }
+        times_state<T, DV, LDS, PLANE, false, WC>(dq, dy, rg * 16, s_state, wc, value, key);
         decay_rows(dq, before[i0] * p.scale, before[i0 + 8] * p.scale);
-        float far0 = 0.0f, far1 = 0.0f;
-#pragma unroll
-        for (int n = 0; n < NK; ++n) {
-          const int col = wc * NK * 8 + n * 8 + 2 * c;
-          const float2 q0 = two_of(q + i0 * LDK + col), q1 = two_of(q + (i0 + 8) * LDK + col);
-          far0 = fmaf(dq[n][0], q0.x, fmaf(dq[n][1], q0.y, far0));
-          far1 = fmaf(dq[n][2], q1.x, fmaf(dq[n][3], q1.y, far1));
-        }
-#pragma unroll
-        for (int off = 1; off < 4; off <<= 1) {
-          far0 += __shfl_xor_sync(0xffffffffu, far0, off);
-          far1 += __shfl_xor_sync(0xffffffffu, far1, off);
-        }
-        if (c == 0) s_far[wc * C + i0] = far0, s_far[wc * C + i0 + 8] = far1;
+        const float2 far = row_sums<T, LDK, WC>(dq, q, i0, wc);
+        if (c == 0) s_far[wc * C + i0] = far.x, s_far[wc * C + i0 + 8] = far.y;
 #pragma unroll 1
         for (int n = 0; n <= rg; ++n) {
           float d[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-          products<T, DV>(d, dy, rg * 16, v, n * 16);
+          products<T, DV>(d, dy, rg * 16, v, n * 16, value);
           float w[8], x[8];
           weights_by_row(w, sums, tail, i0, n * 16, n == rg, p.scale);
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = d[e >> 2][e & 3] * w[e];
           Made<T> left;
           make(left, x);
-#pragma unroll
-          for (int m = 0; m < NK / 2; ++m) {
-            InB<T> right[2];
-            load_b<T, LDK, true>(right, k, wc * NK * 8 + m * 16, n * 16);
-            mma(dq[2 * m], left, right[0]);
-            mma(dq[2 * m + 1], left, right[1]);
-          }
+          add_product<T, LDK, WC>(dq, left, k, n * 16, wc, key);
         }
+      } else {
+#pragma unroll
+        for (int n = 0; n < NK; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dq[n][e] = 0.0f;
       }
-      store_rows<T>(p.dq, p, row, s0 + i0, p.key, wc * NK * 8 + 2 * c, dq);
+      store_rows<T, WC>(p.dq, p, row, s0 + i0, p.key, wc * 16 + 2 * c, dq);
       if (live) {
         // what passes the chunk whole
         float all = 0.0f;
         S.each([&](int r, int col, float& x, float& y) {
           const float2 s = read_state<T, LDS, PLANE>(s_state, r, col);
           all = fmaf(x, s.x, fmaf(y, s.y, all));
-        });
+        }, key, value);
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) all += __shfl_xor_sync(0xffffffffu, all, off);
         if (lane == 0) s_all[warp] = decayed(before[C - 1], all);
-        S.template update<T, C>(q, dy, before, before[C - 1], p.scale);
+        S.template update<T, C>(q, dy, before, before[C - 1], p.scale, key, value);
       }
     } else {
       float dv[NV][4], dk[NK][4];
-#pragma unroll
-      for (int n = 0; n < NV; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) dv[n][e] = 0.0f;
-#pragma unroll
-      for (int n = 0; n < NK; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) dk[n][e] = 0.0f;
       if (live) {
-#pragma unroll kUnroll<T>
-        for (int kk = 0; kk < DK; kk += 16) {
-          InA<T> left;
-          load_a<T, LDK>(left, k, rg * 16, kk);
-#pragma unroll
-          for (int n = 0; n < NV / 2; ++n) {
-            MadeB<T> right[2];
-            load_state<T, LDS, PLANE, true>(right, s_grad, wc * NV * 8 + n * 16, kk);
-            mma(dv[2 * n], left, right[0]);
-            mma(dv[2 * n + 1], left, right[1]);
-          }
-        }
-#pragma unroll kUnroll<T>
-        for (int kk = 0; kk < DV; kk += 16) {
-          InA<T> left;
-          load_a<T, LDV>(left, v, rg * 16, kk);
-#pragma unroll
-          for (int n = 0; n < NK / 2; ++n) {
-            MadeB<T> right[2];
-            load_state<T, LDS, PLANE, false>(right, s_grad, wc * NK * 8 + n * 16, kk);
-            mma(dk[2 * n], left, right[0]);
-            mma(dk[2 * n + 1], left, right[1]);
-          }
-        }
+        times_state<T, DK, LDS, PLANE, true, WC>(dv, k, rg * 16, s_grad, wc, key, value);
+        times_state<T, DV, LDS, PLANE, false, WC>(dk, v, rg * 16, s_grad, wc, value, key);
         decay_rows(dv, after[i0], after[i0 + 8]);
         decay_rows(dk, after[i0], after[i0 + 8]);
-        float end0 = 0.0f, end1 = 0.0f;
-#pragma unroll
-        for (int n = 0; n < NK; ++n) {
-          const int col = wc * NK * 8 + n * 8 + 2 * c;
-          const float2 k0 = two_of(k + i0 * LDK + col), k1 = two_of(k + (i0 + 8) * LDK + col);
-          end0 = fmaf(dk[n][0], k0.x, fmaf(dk[n][1], k0.y, end0));
-          end1 = fmaf(dk[n][2], k1.x, fmaf(dk[n][3], k1.y, end1));
-        }
+        const float2 end = row_sums<T, LDK, WC>(dk, k, i0, wc);
+        if (c == 0) s_end[wc * C + i0] = end.x, s_end[wc * C + i0 + 8] = end.y;
         float col0 = 0.0f, col1 = 0.0f;  // sums of W over i, of j = i0 and i0 + 8
 #pragma unroll 1
         for (int n = rg; n < RG; ++n) {
           float a[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
           float d[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-          products<T, DK>(a, k, rg * 16, q, n * 16);
-          products<T, DV>(d, v, rg * 16, dy, n * 16);
+          products<T, DK>(a, k, rg * 16, q, n * 16, key);
+          products<T, DV>(d, v, rg * 16, dy, n * 16, value);
           float w[8], x[8], z[8];
           weights_by_column(w, sums, tail, i0, n * 16, rg * 16, n == rg, p.scale);
 #pragma unroll
@@ -1213,40 +1245,32 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
           }
           Made<T> left;
           make(left, x);
-#pragma unroll
-          for (int m = 0; m < NV / 2; ++m) {
-            InB<T> right[2];
-            load_b<T, LDV, true>(right, dy, wc * NV * 8 + m * 16, n * 16);
-            mma(dv[2 * m], left, right[0]);
-            mma(dv[2 * m + 1], left, right[1]);
-          }
+          add_product<T, LDV, WC>(dv, left, dy, n * 16, wc, value);
           make(left, z);
-#pragma unroll
-          for (int m = 0; m < NK / 2; ++m) {
-            InB<T> right[2];
-            load_b<T, LDK, true>(right, q, wc * NK * 8 + m * 16, n * 16);
-            mma(dk[2 * m], left, right[0]);
-            mma(dk[2 * m + 1], left, right[1]);
-          }
+          add_product<T, LDK, WC>(dk, left, q, n * 16, wc, key);
         }
 #pragma unroll
         for (int off = 1; off < 4; off <<= 1) {
-          end0 += __shfl_xor_sync(0xffffffffu, end0, off);
-          end1 += __shfl_xor_sync(0xffffffffu, end1, off);
           col0 += __shfl_xor_sync(0xffffffffu, col0, off);
           col1 += __shfl_xor_sync(0xffffffffu, col1, off);
         }
-        if (c == 0) {
-          s_end[wc * C + i0] = end0, s_end[wc * C + i0 + 8] = end1;
-          if (wc == 0) s_col[i0] = col0, s_col[i0 + 8] = col1;
-        }
+        if (c == 0 && wc == 0) s_col[i0] = col0, s_col[i0 + 8] = col1;
+      } else {
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dv[n][e] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NK; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dk[n][e] = 0.0f;
       }
-      store_rows<T>(p.dv, p, row, s0 + i0, p.value, wc * NV * 8 + 2 * c, dv);
-      store_rows<T>(p.dk, p, row, s0 + i0, p.key, wc * NK * 8 + 2 * c, dk);
+      store_rows<T, WC>(p.dv, p, row, s0 + i0, p.value, wc * 16 + 2 * c, dv);
+      store_rows<T, WC>(p.dk, p, row, s0 + i0, p.key, wc * 16 + 2 * c, dk);
     }
     __syncthreads();  // the chunk's tiles, states and sums are read or written
     if (chunk > c0) load(chunk - 1);
-    if (by_rows && live) S.template publish<T>(s_grad);
+    if (by_rows && live) S.template publish<T>(s_grad, key, value);
     if (warp == WARPS - 1) {
       // the decays' gradients: prefix sums over the chunk's steps in 64 bits
       constexpr int E = C / 32;
