@@ -1,10 +1,10 @@
 """A causal speech enhancer trained on the PESQ loss, and run frame by frame.
 
-    python examples/enhancer.py [--steps 200] [--state-bits 8]
+    python examples/enhancer.py [--steps 200] [--state-bits 8] [--mixer attention] [--muon]
 
 The network estimates a mask on the magnitude spectrum (512-sample frames, hop
-256) with blocks of a gated linear recurrence.  It is trained with
-``PesqLossCuda`` and ``AdamWCuda`` on synthetic speech in noise; afterwards the same
+256) with blocks of a gated linear recurrence, or of linear attention whose heads are normed.  It is trained with
+``PesqLossCuda`` and ``AdamWCuda``, or ``MuonCuda`` for its matrices, on synthetic speech in noise; afterwards the same
 weights run one frame at a time with the recurrences' states carried along, as
 a live stream would, and give the same masks.
 """
@@ -17,7 +17,8 @@ import torch
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
-from triton_pesq_b200 import AdamWCuda, GatedScanCuda, NormJoinCuda, PesqLossCuda, pre_norm  # noqa: E402
+from triton_pesq_b200 import (AdamWCuda, GatedScanCuda, LayerNormCuda, LinearAttentionCuda, MuonCuda, NormJoinCuda,  # noqa: E402
+                              PesqLossCuda, pre_norm)
 from triton_pesq_b200.signals import add_noise, speech_like  # noqa: E402
 
 N_FFT, HOP = 512, 256
@@ -41,13 +42,33 @@ class Block(torch.nn.Module):
         return stream, normed, state
 
 
+class AttentionBlock(torch.nn.Module):
+    """The same with linear attention: every head remembers for another time, and its output is normed by itself."""
+
+    def __init__(self, width: int, heads: int = 4):
+        super().__init__()
+        self.heads, self.channels = heads, width // heads
+        self.inner = torch.nn.Linear(width, 4 * width)
+        self.attention = LinearAttentionCuda(heads, self.channels)
+        self.norm = LayerNormCuda(self.channels, heads=heads)
+        self.outer = torch.nn.Linear(width, width)
+        self.join = NormJoinCuda(width, activation="silu", scale=0.5)
+
+    def forward(self, stream, normed, state=None):
+        *qkv, gate = self.inner(normed).chunk(4, dim=2)
+        y, state = self.attention(*(t.unflatten(2, (self.heads, self.channels)) for t in qkv), state)
+        stream, normed = self.join(stream, self.outer(self.norm(y).flatten(2)), gate)
+        return stream, normed, state
+
+
 class Enhancer(torch.nn.Module):
-    def __init__(self, width: int = 96, blocks: int = 3):
+    def __init__(self, width: int = 96, blocks: int = 3, mixer: str = "scan"):
         super().__init__()
         bins = N_FFT // 2 + 1
         self.embed = torch.nn.Linear(bins, width)
         self.weight = torch.nn.Parameter(torch.ones(width))
-        self.blocks = torch.nn.ModuleList(Block(width) for _ in range(blocks))
+        block = {"scan": Block, "attention": AttentionBlock}[mixer]
+        self.blocks = torch.nn.ModuleList(block(width) for _ in range(blocks))
         self.head = torch.nn.Linear(width, bins)
         self.register_buffer("window", torch.hann_window(N_FFT))
 
@@ -83,22 +104,28 @@ class Enhancer(torch.nn.Module):
         return torch.cat(out, dim=1)
 
 
-def train(model, steps: int, batch: int = 8, seconds: float = 2.0, state_bits: int = 32, lr: float = 3e-3, seed: int = 0):
+def train(model, steps: int, batch: int = 8, seconds: float = 2.0, state_bits: int = 32, lr: float = 3e-3, seed: int = 0,
+          muon: bool = False):
     """Trains on synthetic speech at 0 to 10 dB; returns the losses."""
 
     device = next(model.parameters()).device
     loss_fn = PesqLossCuda(0.5, sample_rate=16000).to(device)
-    optimiser = AdamWCuda(model.parameters(), lr=lr, state_bits=state_bits, seed=seed)
+    matrices = [p for b in model.blocks for p in b.parameters() if p.dim() == 2 and muon]
+    rest = [p for p in model.parameters() if not any(p is m for m in matrices)]
+    optimisers = [AdamWCuda(rest, lr=lr, state_bits=state_bits, seed=seed)]
+    if matrices:
+        optimisers.append(MuonCuda(matrices, lr=lr, weight_decay=1e-2, adjust="match_rms_adamw"))
     samples, losses = int(16000 * seconds), []
     for step in range(steps):
         clean = speech_like(batch, samples, 16000, seed=seed + step % 16)
         noisy = add_noise(clean, float(step % 11), seed=1000 + seed + step % 16).to(device)
         clean = clean.to(device)
-        optimiser.zero_grad()
+        model.zero_grad()
         enhanced = model(noisy)
         loss = loss_fn(clean, enhanced).mean()
         loss.backward()
-        optimiser.step()
+        for optimiser in optimisers:
+            optimiser.step()
         losses.append(loss.detach())
     return torch.stack(losses).cpu()
 
@@ -107,10 +134,12 @@ def main():
     parser = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     parser.add_argument("--steps", type=int, default=200)
     parser.add_argument("--state-bits", type=int, default=8, choices=(8, 32))
+    parser.add_argument("--mixer", default="scan", choices=("scan", "attention"))
+    parser.add_argument("--muon", action="store_true", help="step the blocks' matrices by orthogonalised updates")
     args = parser.parse_args()
     torch.manual_seed(0)
-    model = Enhancer().cuda()
-    losses = train(model, args.steps, state_bits=args.state_bits)
+    model = Enhancer(mixer=args.mixer).cuda()
+    losses = train(model, args.steps, state_bits=args.state_bits, muon=args.muon)
     print(f"loss of the first ten steps {losses[:10].mean():.3f}, of the last ten {losses[-10:].mean():.3f}")
     noisy = add_noise(speech_like(1, 32000, 16000, seed=99), 5.0, seed=98).cuda()
     magnitude = model.spectrum(noisy).abs()
