@@ -187,16 +187,19 @@ __global__ void __launch_bounds__(kPrepThreads) momentum_kernel(const __grid_con
   }
 }
 
-__device__ __forceinline__ void split(float v, __half& hi, __half& lo) {
-  hi = __float2half_rn(v);
-  lo = __float2half_rn(v - __half2float(hi));
-}
 struct alignas(16) Eight {
-  __half h[8];
+  uint32_t w[4];  // two float16 each
 };
+// Eight values as their terms.  The upper term's value is the value's own bits rounded to 11, half away from zero, which a conversion back
+// would take twice as long for (conversions are what bounds this); below 2^-14, where float16 holds fewer, the terms are off by up to 2^-25.
 __device__ __forceinline__ void split8(const float (&v)[8], Eight& hi, Eight& lo) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) split(v[j], hi.h[j], lo.h[j]);
+  for (int j = 0; j < 4; ++j) {
+    const float a = v[2 * j], b = v[2 * j + 1];
+    const float x = __uint_as_float((__float_as_uint(a) + 0x1000u) & 0xffffe000u), y = __uint_as_float((__float_as_uint(b) + 0x1000u) & 0xffffe000u);
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(hi.w[j]) : "f"(y), "f"(x));
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(lo.w[j]) : "f"(b - y), "f"(a - x));
+  }
 }
 // where columns 8 chunk .. of a row of a tile's plane lie
 __device__ __forceinline__ int at(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
@@ -326,7 +329,7 @@ __device__ __forceinline__ void put(char* to, char* over, bool mirrored, int row
   for (int q = 0; q < 2; ++q) {
     *reinterpret_cast<Eight*>(to + q * kPlane + at(row, chunk)) = plane[q];
     if (!mirrored) continue;
-    const uint32_t* words = reinterpret_cast<const uint32_t*>(plane[q].h);
+    const uint32_t* words = plane[q].w;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint32_t other = __shfl_xor_sync(0xffffffffu, words[j], 1);
@@ -336,7 +339,13 @@ __device__ __forceinline__ void put(char* to, char* over, bool mirrored, int row
   }
 }
 
-// What four warps make of 32 columns of a tile's accumulators: a thread has a row
+__device__ __forceinline__ void add_diagonal(float (&v)[8], int at, float x) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j == at) v[j] += x;
+}
+
+// What a warp makes of 32 columns of a tile's accumulators: a thread has a row
 __device__ __forceinline__ void finish(const Call& p, int mode, int from, const Item& it, const Tile& t, int row, int col,
                                        const float (&acc)[32], bool skip) {
   const int r = t.i * kTile + row, c0 = t.j * kTile + col;
@@ -399,18 +408,18 @@ __device__ __forceinline__ void finish(const Call& p, int mode, int from, const 
   const int64_t across = ((int64_t)t.j * tiles + t.i * 2 + row / kDepth) * kPair;
   const bool mirrored = mode < kUpdate && t.i != t.j;
   char* const to = p.ws + (mode == kGram ? it.a : mode == kPolynomial ? it.b : it.x[from ^ 1]);
+  const bool diagonal = mode < kUpdate && t.i == t.j && col == row / 32 * 32 && r < it.n;
 #pragma unroll
   for (int k = 0; k < 32; k += 8) {
     float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v[j] = acc[k + j] * (1.0f / kScale);
-      if (mode == kPolynomial && c0 + k + j == r && r < it.n) v[j] += p.ca * kScale;
-    }
+    for (int j = 0; j < 8; ++j) v[j] = acc[k + j] * (1.0f / kScale);
+    if (mode == kPolynomial && diagonal) add_diagonal(v, row % 32 - k, p.ca * kScale);
     put(to + place, to + across, mirrored, row, col + k, v);
     if (mode == kGram) {  // and what A is multiplied with: b + c A, so that the polynomial's tiles are products alone
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = p.cc * v[j] + (c0 + k + j == r && r < it.n ? p.cb * kScale : 0.0f);
+      for (int j = 0; j < 8; ++j) v[j] *= p.cc;
+      if (diagonal) add_diagonal(v, row % 32 - k, p.cb * kScale);
       put(p.ws + it.c + place, p.ws + it.c + across, mirrored, row, col + k, v);
     }
   }
