@@ -73,6 +73,7 @@ struct Args {
   float scale;
   int chunks, parts, part_chunks, slices;  // of a row; chunks of a part; CTAs side by side over the values
   float *starts, *factors;  // [rows, parts, DK, DV], [rows, parts]: of a sweep and its join
+  int joined;               // a join has made the states that the parts begin from; else they are made from the sweep's
   void* kept;               // states before the chunks
   // results
   void* y;
@@ -637,6 +638,30 @@ struct State {
       if (r < key && first + c + 1 < value) to[(int64_t)r * value + first + c + 1] = b;
     });
   }
+  // What a part begins from: the row's state `from`, and what the parts before it in scan order (after it, kBackward) add
+  template <bool kBackward>
+  __device__ __forceinline__ void begin(const Args& p, int64_t index, int part, const float* from, int padded, int first) {
+    if (p.parts == 1) {
+      read(from, p.key, p.value, first);
+      return;
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // for the sweep, or the join, which this kernel is launched close to
+    const float* starts = p.starts + index * p.parts * DK * padded;
+    if (p.joined) {
+      read(starts + (int64_t)part * DK * padded, DK, padded, first);
+      return;
+    }
+    read(from, p.key, p.value, first);
+#pragma unroll 1
+    for (int i = kBackward ? p.parts - 1 : 0; i != part; i += kBackward ? -1 : 1) {
+      const float factor = p.factors[index * p.parts + i];
+      const float* add = starts + (int64_t)i * DK * padded + first;
+      each([&](int r, int c, float& a, float& b) {
+        const float2 more = *reinterpret_cast<const float2*>(add + (int64_t)r * padded + c);
+        a = decayed(factor, a) + more.x, b = decayed(factor, b) + more.y;
+      });
+    }
+  }
   // S = factor S + sum over the chunk's steps of weight a b^T.  The chunk's sum is made by itself and added, rounded: the
   // instruction cuts off what its accumulator does not hold, which over the chunks that a slow head remembers is 1e-5.
   template <class T, int C>
@@ -871,11 +896,7 @@ __global__ void __launch_bounds__(128, DK > 64 ? 2 : 3) forward_kernel(const __g
 
   clear<THREADS>(shared, Sh::kStages * Sh::kTiles);
   State<DK, DV, WARPS> S;
-  const float* from = p.state ? p.state + index * p.key * p.value : nullptr;
-  if (p.parts > 1)
-    S.read(p.starts + (index * p.parts + part) * DK * padded, DK, padded, first);
-  else
-    S.read(from, p.key, p.value, first);
+  S.template begin<false>(p, index, part, p.state ? p.state + index * p.key * p.value : nullptr, padded, first);
   S.template publish<T>(s_state, key, value);
   __syncthreads();
 
@@ -983,6 +1004,7 @@ __global__ void __launch_bounds__(128) sweep_kernel(const __grid_constant__ Args
   const Row row(p, index);
   const int first = slice * DV, cols = min(DV, p.value - first), padded = DV * p.slices;
   const int c0 = part * p.part_chunks, c1 = min(p.chunks, c0 + p.part_chunks);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (part == (kBackward ? 0 : p.parts - 1)) return;  // (nothing begins from it)
   clear<THREADS>(shared, 2 * Sh::kTiles);
   State<DK, DV, WARPS> S;
@@ -1035,6 +1057,7 @@ __global__ void __launch_bounds__(128) sweep_kernel(const __grid_constant__ Args
 // What the parts add, to the states that they begin from; a thread takes an element of a row's state
 template <int kThreads>
 __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ Args p, int DK, int DV, int backward) {
+  asm volatile("griddepcontrol.launch_dependents;\ngriddepcontrol.wait;" ::: "memory");
   const int64_t size = (int64_t)DK * DV, per = (size + kThreads - 1) / kThreads;
   const int64_t index = blockIdx.x / per, at = (blockIdx.x - index * per) * kThreads + threadIdx.x;
   if (at >= size) return;
@@ -1111,12 +1134,10 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
   clear<THREADS>(shared, Sh::kTiles);
   State<DK, DV, SIDE> S;  // the gradient of the state, of the warps by rows
   if (by_rows) {
-    const float* from = p.dlast ? p.dlast + index * p.key * p.value : nullptr;
-    if (p.parts > 1)
-      S.read(p.starts + (index * p.parts + part) * DK * DV, DK, DV, 0);
-    else
-      S.read(from, p.key, p.value, 0);
+    S.template begin<true>(p, index, part, p.dlast ? p.dlast + index * p.key * p.value : nullptr, DV, 0);
     S.template publish<T>(s_grad, key, value);
+  } else if (p.parts > 1) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
   }
   __syncthreads();
 

@@ -25,6 +25,7 @@ constexpr int kMaxWidth = 128;  // of keys and of values
 constexpr int kFewSteps = 8;    // that single steps take, where no backward follows
 constexpr int kFewChunks = 6;   // that are not cut in parts
 constexpr int kRagged = 4;
+constexpr int kFewParts = 4;    // that make the states they begin from themselves, without a join
 constexpr int kJoinThreads = 256;
 
 // The decay's gradient of a head: the chunks' sums of its rows, in a fixed order
@@ -153,6 +154,7 @@ Args arguments(const pesq_linear_attention_desc& d, const Plan& q, void* workspa
   a.parts = q.parts;
   a.part_chunks = q.part_chunks;
   a.slices = q.slices;
+  a.joined = q.parts > kFewParts;
   char* ws = static_cast<char*>(workspace);
   a.starts = reinterpret_cast<float*>(ws);
   a.factors = reinterpret_cast<float*>(ws + q.starts);
@@ -175,9 +177,18 @@ cudaError_t sweep(Args a, const Plan& q, int dtype, bool backward, cudaStream_t 
   g.blocks = q.rows * q.parts * a.slices;
   cudaError_t e = forward(a, g, dtype, backward ? kSweepBackward : kSweep, s);
   if (e != cudaSuccess) return e;
+  if (!a.joined) return cudaSuccess;
   const int64_t per = ((int64_t)g.dk * dv + kJoinThreads - 1) / kJoinThreads;
-  join_kernel<kJoinThreads><<<(unsigned)(q.rows * per), kJoinThreads, 0, s>>>(a, g.dk, dv, backward);
-  return cudaGetLastError();
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3((unsigned)(q.rows * per));
+  c.blockDim = dim3(kJoinThreads);
+  c.stream = s;
+  c.attrs = &at;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, join_kernel<kJoinThreads>, a, g.dk, dv, (int)backward);
 }
 
 int check_operands(const pesq_linear_attention_desc* d) {

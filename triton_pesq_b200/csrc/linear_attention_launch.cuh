@@ -7,22 +7,31 @@
 namespace pesq {
 namespace lattn {
 
-template <class K>
-cudaError_t start(K kernel, const Args& p, int64_t grid, int threads, int smem, cudaStream_t s) {
+// close: to the kernel before, whose results it waits for itself
+inline cudaError_t start(void (*kernel)(Args), const Args& p, int64_t grid, int threads, int smem, bool close, cudaStream_t s) {
   if (smem > 48 << 10) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
   }
-  kernel<<<(unsigned)grid, threads, smem, s>>>(p);
-  return cudaGetLastError();
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = close;
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3((unsigned)grid);
+  c.blockDim = dim3((unsigned)threads);
+  c.dynamicSmemBytes = (size_t)smem;
+  c.stream = s;
+  c.attrs = &at;
+  c.numAttrs = close ? 1 : 0;
+  return cudaLaunchKernelEx(&c, kernel, p);
 }
 
 template <class T, int DK, int DV, int C, bool kWhole>
 cudaError_t launch_forward(const Args& p, const Geometry& g, Kind kind, cudaStream_t s) {
   switch (kind) {
-    case kForward: return start(forward_kernel<T, DK, DV, C, kWhole>, p, g.blocks, 128, ForwardShared<T, DK, DV, C>::kBytes, s);
-    case kSweep: return start(sweep_kernel<T, DK, DV, C, kWhole, false>, p, g.blocks, 128, SweepShared<T, DK, DV, C>::kBytes, s);
-    default: return start(sweep_kernel<T, DK, DV, C, kWhole, true>, p, g.blocks, 128, SweepShared<T, DK, DV, C>::kBytes, s);
+    case kForward: return start(forward_kernel<T, DK, DV, C, kWhole>, p, g.blocks, 128, ForwardShared<T, DK, DV, C>::kBytes, p.parts > 1, s);
+    case kSweep: return start(sweep_kernel<T, DK, DV, C, kWhole, false>, p, g.blocks, 128, SweepShared<T, DK, DV, C>::kBytes, false, s);
+    default: return start(sweep_kernel<T, DK, DV, C, kWhole, true>, p, g.blocks, 128, SweepShared<T, DK, DV, C>::kBytes, false, s);
   }
 }
 
@@ -41,7 +50,7 @@ cudaError_t launch_forward(const Args& p, const Geometry& g, Kind kind, cudaStre
 
 template <class T, int DK>
 cudaError_t forward_width(const Args& p, const Geometry& g, Kind kind, cudaStream_t s) {
-  if (kind == kSteps) return start(steps_kernel<T, DK>, p, g.blocks, 128, 0, s);
+  if (kind == kSteps) return start(steps_kernel<T, DK>, p, g.blocks, 128, 0, false, s);
   if constexpr (std::is_same<T, float>::value && DK == 128) {
     if (g.chunk == 32) return launch_forward<T, DK, 64, 32>(p, g, kind, s);
   }
@@ -61,9 +70,9 @@ cudaError_t launch_backward(const Args& p, const Geometry& g, cudaStream_t s) {
   constexpr int dtype = std::is_same<T, float>::value ? PESQ_F32 : PESQ_BF16, C = chunk_of(dtype, DK, DV);
   constexpr int kThreads = 64 * kSide<T, DK, DV>, kBytes = BackwardShared<T, DK, DV, C>::kBytes;
   if constexpr (!kAlwaysWhole<T>) {
-    if (p.key <= DK - 16 || p.value <= DV - 16) return start(backward_kernel<T, DK, DV, C, false>, p, g.blocks, kThreads, kBytes, s);
+    if (p.key <= DK - 16 || p.value <= DV - 16) return start(backward_kernel<T, DK, DV, C, false>, p, g.blocks, kThreads, kBytes, p.parts > 1, s);
   }
-  return start(backward_kernel<T, DK, DV, C, true>, p, g.blocks, kThreads, kBytes, s);
+  return start(backward_kernel<T, DK, DV, C, true>, p, g.blocks, kThreads, kBytes, p.parts > 1, s);
 }
 template <class T, int DK>
 cudaError_t backward_width(const Args& p, const Geometry& g, cudaStream_t s) {
