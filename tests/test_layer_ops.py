@@ -49,6 +49,16 @@ def test_layer_norm_entry_checks_its_descriptor():
     assert lib.pesq_layer_norm_backward(ctypes.byref(d), None, x, one, one, None, ctypes.c_void_p(24), 1 << 30) == 3
 
 
+@pytest.mark.parametrize("heads,width", [(1, 1), (1, 8192), (14, 64), (128, 8192), (1000, 64), (16384, 64), (1 << 20, 1), (100000, 7)])
+@pytest.mark.parametrize("steps", [1, 1000, 1 << 20])
+def test_layer_norm_workspace_stays_small(heads, width, steps):
+    """One CTA's sums are of its own heads: twice as many vectors as CTAs at most, however many heads there are."""
+    d = _lib.LayerNormDesc(batch=1, steps=steps, heads=heads, width=width, dtype=_lib.F32, out_dtype=_lib.F32, eps=0.0)
+    size = ctypes.c_size_t()
+    assert _lib.library().pesq_layer_norm_workspace(ctypes.byref(d), ctypes.byref(size)) == _lib.PESQ_OK
+    assert 2 * 4 * heads * width <= size.value <= 1 << 25
+
+
 def test_linear_attention_without_a_gpu():
     x = torch.zeros(1, 2, 3, 4)
     with pytest.raises(RuntimeError, match="GPU"):

@@ -96,15 +96,7 @@ struct Plan {
 // As many CTAs as the device holds at once, each with its share of the rows, but none with less than a row a team.
 // A CTA's teams take the heads side by side: of the numbers of heads that leave the fewest teams idle the largest, so that
 // neighbouring heads, whose rows are neighbours in memory, are read together.
-Plan plan(const pesq_layer_norm_desc& d, bool backward, const pesq_heads* dy, const void* result) {
-  Plan q{};
-  const pesq_heads none{nullptr, 0, 0, 0};
-  const pesq_heads& g = dy ? *dy : none;
-  const bool flat = joined(d.x, d) && joined(g, d);
-  q.batch = flat ? 1 : d.batch;
-  q.steps = flat ? d.batch * d.steps : d.steps;
-  q.g.wide = d.width % kEach == 0 && wide(d.x, d, d.dtype) && wide(g, d, d.out_dtype) && wide(d.weight) && wide(d.bias) &&
-             wide(result);
+void share(const pesq_layer_norm_desc& d, bool backward, Plan& q) {
   team_of(d.width, q.g);
   const int threads = std::max(q.g.team, kThreads), teams = threads / q.g.team;
   double best = -1.0;
@@ -120,12 +112,31 @@ Plan plan(const pesq_layer_norm_desc& d, bool backward, const pesq_heads* dy, co
   q.span = (rows + units - 1) / units;
   q.units = (rows + q.span - 1) / q.span;
   q.g.blocks = q.units * q.head_blocks;
+}
+
+Plan plan(const pesq_layer_norm_desc& d, bool backward, const pesq_heads* dy, const void* result) {
+  Plan q{};
+  const pesq_heads none{nullptr, 0, 0, 0};
+  const pesq_heads& g = dy ? *dy : none;
+  const bool flat = joined(d.x, d) && joined(g, d);
+  q.batch = flat ? 1 : d.batch;
+  q.steps = flat ? d.batch * d.steps : d.steps;
+  q.g.wide = d.width % kEach == 0 && wide(d.x, d, d.dtype) && wide(g, d, d.out_dtype) && wide(d.weight) && wide(d.bias) &&
+             wide(result);
+  share(d, backward, q);
   return q;
 }
 
+// of the CTAs' sums of one vector, however the operands lie
 size_t part_bytes(const pesq_layer_norm_desc& d) {
-  // (however the operands lie, no more CTAs than this over the rows: four an SM, and the fewest of a head)
-  return ((size_t)(148 * 4) * d.heads * d.width * 4 + 15) / 16 * 16;
+  int64_t units = 0;
+  for (const bool wide : {false, true}) {
+    Plan q{};
+    q.g.wide = wide;
+    share(d, true, q);
+    units = std::max(units, q.units);
+  }
+  return ((size_t)units * d.heads * d.width * 4 + 15) / 16 * 16;
 }
 
 Strided rows_of(const pesq_heads& s) { return {s.data, s.batch_stride, s.step_stride, s.head_stride}; }
