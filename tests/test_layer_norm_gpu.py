@@ -167,6 +167,52 @@ def test_the_same_every_time_and_a_captured_step(cuda_device):
         assert torch.equal(a, e)
 
 
+def test_two_streams_at_once(cuda_device):
+    inputs = [[t.to(cuda_device) for t in make((3, 900, 6, 48), (6, 48), BF16, BF16, seed=s)] for s in (5, 6)]
+
+    def step(x, w, b, dy):
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        y = layer_norm(*leaves)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    want = [step(*t) for t in inputs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in inputs], []
+    for t, stream in zip(inputs, streams):
+        with torch.cuda.stream(stream):
+            got.append([step(*t) for _ in range(10)])
+    torch.cuda.synchronize()
+    for runs, e in zip(got, want):
+        for run in runs:
+            assert all(torch.equal(a, b) for a, b in zip(run, e))
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """The last rows of more than 2^31 elements, and rows 2^31 elements and more apart, are what they are alone."""
+
+    rows, width = (1 << 24) + 77, 128
+    w, b = (torch.linspace(0.5, 1.5, width, device=cuda_device, requires_grad=True) for _ in range(2))
+    x = torch.randn(1, rows, width, device=cuda_device, dtype=BF16).requires_grad_(True)
+    y = layer_norm(x, w, b)
+    dy = torch.zeros_like(y)
+    tail = x.detach()[:, -50:].clone().requires_grad_(True)
+    want = layer_norm(tail, w, b)
+    assert torch.equal(y[:, -50:], want)
+    dy[:, -50:] = 1 + torch.arange(width, device=cuda_device) % 3
+    got = torch.autograd.grad(y, (x, w, b), dy)
+    alone = torch.autograd.grad(want, (tail, w, b), dy[:, -50:].clone())
+    assert torch.equal(got[0][:, -50:], alone[0]) and not got[0][:, :-50].any()
+    for a, e in zip(got[1:], alone[1:]):
+        R.close(a, e.double(), VTOL, "vectors")
+    del x, y, dy, got
+    far = torch.zeros((1 << 32) + 4096, device=cuda_device, dtype=BF16)
+    for strides in (((1 << 32), 64, 1), (1024, 1 << 31, 1)):
+        view = torch.as_strided(far, (2, 3, 64) if strides[1] == 64 else (4, 3, 64), strides)
+        dense = torch.randn(view.shape, device=cuda_device, dtype=BF16)
+        view.copy_(dense)
+        assert torch.equal(layer_norm(view, w.detach()[:64], b.detach()[:64]), layer_norm(dense, w.detach()[:64], b.detach()[:64]))
+
+
 def test_no_rows(cuda_device):
     for shape in ((0, 4, 8), (2, 0, 8), (2, 3, 0)):
         x = torch.zeros(shape, device=cuda_device, requires_grad=True)

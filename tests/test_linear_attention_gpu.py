@@ -314,6 +314,43 @@ def test_two_streams_at_once(cuda_device):
         assert torch.equal(a[0], e[0]) and torch.equal(a[1], e[1])
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_offsets_past_32_bits(cuda_device, dtype):
+    """The last steps of operands of more than 2^31 elements, and operands whose steps, heads and rows lie as far apart."""
+
+    steps, heads, width, tail = (1 << 20) + 200, 32, 64, 300
+    x = torch.randn(1, steps, heads, width, device=cuda_device, dtype=dtype) * 0.3
+    decay = torch.linspace(-0.6, -0.4, heads, device=cuda_device)
+    v = x.detach().requires_grad_(True)
+    y, last = linear_attention(x, x, v, decay)
+    # (what came 128 steps before is e^-51 of what it was)
+    end = x[:, -tail:].cpu().double()
+    wv = end.clone().requires_grad_(True)
+    want, wlast = definition(end, end, wv, decay.cpu().double())
+    R.close(y[:, -tail + 128:], want[:, 128:], TOL[dtype], "y")
+    R.close(last, wlast, TOL[dtype], "last")
+    dlast = torch.randn_like(last)
+    got = torch.autograd.grad(last, v, dlast)[0]
+    alone = torch.autograd.grad(wlast, wv, dlast.cpu().double())[0]
+    R.close(got[:, -tail:], alone, TOL[dtype] * 2, "dv")
+    assert not got[:, :1000].any()
+    del x, v, y, got
+    far = torch.zeros((1 << 32) + (1 << 14), device=cuda_device, dtype=dtype)
+    for strides in ((1 << 32, 256, 64, 1), (1 << 13, 1 << 30, 64, 1), (1 << 13, 64, 1 << 31, 1)):
+        shape = (2, 5 if strides[1] == 1 << 30 else 30, 3 if strides[2] == 1 << 31 else 2, 64)
+        last_at = sum((n - 1) * s for n, s in zip(shape, strides))
+        if last_at >= far.numel():
+            shape = (2, 4, 2, 64)
+        view = torch.as_strided(far, shape, strides)
+        dense = torch.randn(shape, device=cuda_device, dtype=dtype)
+        view.copy_(dense)
+        decay = torch.linspace(-0.5, -0.1, shape[2], device=cuda_device)
+        for n in (shape[1], 1):
+            v, d = view[:, :n], dense[:, :n]
+            for a, e in zip(linear_attention(v, v, v, decay), linear_attention(d, d, d, decay)):
+                assert torch.equal(a, e)
+
+
 def test_nothing_to_do(cuda_device):
     for shape in ((0, 4, 2, 8, 8), (2, 0, 2, 8, 8), (2, 3, 0, 8, 8), (2, 3, 2, 0, 8), (2, 3, 2, 8, 0)):
         (q, k, v, g, s), dy, dlast, kw = make(*shape[:3], max(shape[3], 1), max(shape[4], 1), F32)

@@ -85,6 +85,34 @@ def test_scales_ranks_and_steps(cuda_device):
     near(orthogonalize(x.to(cuda_device), steps=8, coefficients=cubic), newton_schulz(x.double(), steps=8, coefficients=cubic), "cubic")
 
 
+def test_the_least_eps(cuda_device):
+    """A reciprocal that is just in float32's range: 1 / eps is, 2^10 / eps is not."""
+
+    x = 1e-37 * matrix(60, 100, seed=7)
+    for eps in (2e-38, 1.2e-38):
+        near(orthogonalize(x.to(cuda_device), eps=eps), newton_schulz(x.double(), eps=eps), "above eps")
+        tiny = 1e-3 * x
+        # (subnormal inputs are as exact as their last bit, 1.4e-45, beside a norm of some 1e-38)
+        near(orthogonalize(tiny.to(cuda_device), eps=eps), newton_schulz(tiny.double(), eps=eps), "below eps")
+    with pytest.raises(ValueError, match="eps"):
+        orthogonalize(x.to(cuda_device), eps=1e-39)
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """A matrix whose tiles lie more than 2^32 bytes into the workspace."""
+
+    x = matrix(8192, 32768, seed=8).to(cuda_device)
+    got = orthogonalize(x, steps=2)
+    assert _lib.muon_check() == 0
+    want = newton_schulz(x.double(), steps=2)
+    size = torch.linalg.matrix_norm(want)
+    off = torch.linalg.matrix_norm(got.double() - want)
+    # (two steps' slopes: 3.4445^2 of what is added to a norm of 1, and 20 as above)
+    assert off <= (12 + 20 * size) * 2.0**-21 + R.ROUND[F32] * size, (off, size)
+    rows = torch.linalg.vector_norm(got.double() - want, dim=1) / torch.linalg.vector_norm(want, dim=1)
+    assert rows.max() < 2.0**-15
+
+
 def test_what_is_not_finite_stays_in_its_matrix(cuda_device):
     x = matrix(3, 70, 50).to(cuda_device)
     want = orthogonalize(x)

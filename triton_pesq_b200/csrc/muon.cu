@@ -13,7 +13,7 @@
 // usual coefficients, far from float16's largest, and the lo term of an element of 2^-10 still has its bits.
 // The accumulator of the instruction cuts off what it does not hold instead of rounding it, which adds up over a long
 // contraction (2.3e-5 of the result of a 385 x 1155 matrix, 5.0e-5 of 1280 x 3840).  So it sums 128 columns alone, and the
-// warps that read it add those sums in registers, rounded (7.1e-6 and 4.0e-6; float32 products 2.8e-6 and 3.6e-6).
+// warps that read it add those sums in registers, rounded (4.4e-6 and 2.9e-6; float32 products 2.8e-6 and 3.6e-6).
 //
 // Products run on tcgen05 with the accumulator in tensor memory, in tiles of 128 x 128.  Matrices lie in the workspace as the
 // tiles that the instruction reads from shared memory: 128 rows of 64 columns in the 128-byte swizzle, hi and lo
@@ -32,6 +32,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <vector>
 
@@ -224,7 +225,7 @@ __global__ void __launch_bounds__(kPrepThreads) prepare_kernel(const __grid_cons
   bool skip;
   const float s = scale_of(p, skip);
   const double norm = sqrt(s_sum[0]);
-  const float inverse = (float)(kScale / (norm > p.eps || norm != norm ? norm : (double)p.eps));
+  const float inverse = (float)(1.0 / (norm > p.eps || norm != norm ? norm : (double)p.eps));  // (times 2^10 it may be past float32)
   char* to = p.ws + it.x[0] + (int64_t)tile * kPair;
   with_type(p.dtype, [&](auto zero) {
     using G = decltype(zero);
@@ -244,7 +245,7 @@ __global__ void __launch_bounds__(kPrepThreads) prepare_kernel(const __grid_cons
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        v[j] = (it.momentum ? update_of(p, m[j], s * g[j]) : g[j]) * inverse;
+        v[j] = (it.momentum ? update_of(p, m[j], s * g[j]) : g[j]) * inverse * kScale;
         if (!(r < it.n && c + j < it.m)) v[j] = 0.0f;
       }
       Eight hi, lo;
@@ -942,7 +943,8 @@ cudaError_t run(const std::vector<Matrix>& all, Call& call, void* workspace, cud
 int check_iteration(int dtype, int steps, float eps, float a, float b, float c) {
   if (dtype < PESQ_F32 || dtype > PESQ_F16) return set_error(PESQ_ERR_INVALID_ARGUMENT, "unknown type");
   if (steps < 1 || steps > 100) return set_error(PESQ_ERR_INVALID_ARGUMENT, "between 1 and 100 steps");
-  if (!(eps > 0.0f) || !(eps - eps == 0.0f)) return set_error(PESQ_ERR_INVALID_ARGUMENT, "eps must be positive and finite");
+  if (!(eps >= FLT_MIN) || !(eps - eps == 0.0f))
+    return set_error(PESQ_ERR_INVALID_ARGUMENT, "eps must be positive, finite and no subnormal");
   for (float x : {a, b, c})
     if (!(std::fabs(x) <= 16.0f)) return set_error(PESQ_ERR_INVALID_ARGUMENT, "coefficients must lie between -16 and 16");
   return PESQ_OK;

@@ -47,9 +47,10 @@ def orthogonalize(x: torch.Tensor, *, coefficients: Tuple[float, float, float] =
     x
         float32, bfloat16 or float16, up to 32768 rows and columns.
     coefficients
-        Of the polynomial, each between -16 and 16.
+        Of the polynomial ``c0 + c1 s^2 + c2 s^4`` of the singular values s, each between -16 and 16.  The values, the polynomial on
+        them and ``c1 + c2 s^2`` have to stay below 60, the operands' range: a result of larger ones is not finite.
     eps
-        Least norm that a matrix is divided by, above 0.
+        Least norm that a matrix is divided by, 1.2e-38 or more.
     steps
         Between 1 and 100.
 
@@ -126,8 +127,8 @@ class MuonCuda(torch.optim.Optimizer):
             raise ValueError("`momentum` has to lie in [0, 1).")
         if len(coefficients) != 3 or not all(abs(c) <= 16 for c in coefficients):
             raise ValueError("`coefficients` have to be three values between -16 and 16.")
-        if not 0 < eps < float("inf"):
-            raise ValueError("`eps` has to be positive and finite.")
+        if not torch.finfo(torch.float32).tiny <= eps < float("inf"):
+            raise ValueError("`eps` has to be positive, finite and no subnormal.")
         if not 1 <= int(steps) <= 100:
             raise ValueError("`steps` has to lie between 1 and 100.")
         if adjust not in ADJUSTMENTS:
