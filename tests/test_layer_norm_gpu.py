@@ -65,6 +65,14 @@ def test_wide_rows(cuda_device, width):
 
 
 @pytest.mark.parametrize("types", [(F32, F32), (BF16, BF16), (F32, F16)])
+@pytest.mark.parametrize("width", [1025, 1032, 1155, 1500, 1536, 1537, 2304, 2500, 2561, 4104, 5121, 6136, 6145, 8001])
+def test_rows_of_several_warps(cuda_device, types, width):
+    """Every number of warps, with rows enough that a team takes several."""
+
+    compare(*make((2, 400, width), (width,), *types, seed=width), cuda_device)
+
+
+@pytest.mark.parametrize("types", [(F32, F32), (BF16, BF16), (F32, F16)])
 @pytest.mark.parametrize("shape", [(2, 3, 1, 16), (2, 5, 2, 64), (3, 700, 14, 64), (1, 900, 9, 33), (2, 50, 17, 8), (1, 40, 300, 24),
                                    (1, 30, 5, 512), (2, 21, 3, 1500), (5, 1, 12, 77)])
 @pytest.mark.parametrize("bias", [True, False])

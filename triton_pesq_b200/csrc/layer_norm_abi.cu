@@ -81,10 +81,19 @@ bool wide(const pesq_heads& s, const pesq_layer_norm_desc& d, int dtype) {
 }
 bool wide(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-// threads of a row, and eights of channels of each
+// Threads of a row, and eights of channels of each.  Above a warp any number of warps that keeps few lanes idle, not a power of two
+// (24006 x 1155 float32 to float16: three warps 40 us forward and 60 backward, four 47 and 74; 1160, of 16 bytes: three warps of two
+// eights 38 and 55, two of four 39 and 63)
 void team_of(int64_t width, Geometry& g) {
+  const int most = most_groups(g.wide);
   g.team = 4, g.groups = 1;
-  while (g.team * g.groups * kEach < width) (g.team < 32 || g.groups == most_groups(g.wide) ? g.team : g.groups) *= 2;
+  while (g.team * g.groups * kEach < width && (g.team < 32 || g.groups < most)) (g.team < 32 ? g.team : g.groups) *= 2;
+  if (g.team * g.groups * kEach >= width) return;
+  for (const int warps : {2, 3, 4, 5, 6, 8, 12, 16}) {
+    g.team = 32 * warps;
+    if (g.team * g.groups * kEach >= width) break;
+  }
+  if (g.groups == 4 && width <= 3 * 32 * 2 * kEach) g.team = 96, g.groups = 2;
 }
 
 struct Plan {
@@ -98,7 +107,7 @@ struct Plan {
 // neighbouring heads, whose rows are neighbours in memory, are read together.
 void share(const pesq_layer_norm_desc& d, bool backward, Plan& q) {
   team_of(d.width, q.g);
-  const int threads = std::max(q.g.team, kThreads), teams = threads / q.g.team;
+  const int threads = threads_of(q.g.team), teams = threads / q.g.team;
   double best = -1.0;
   for (int h = 1; h <= std::min<int64_t>(teams, d.heads); ++h) {
     const int64_t blocks = (d.heads + h - 1) / h;
@@ -107,7 +116,7 @@ void share(const pesq_layer_norm_desc& d, bool backward, Plan& q) {
   }
   const int slots = teams / q.block_heads;
   const int64_t rows = d.batch * d.steps;
-  const int64_t most = std::max<int64_t>(1, 148 * ctas(backward, q.g.team, q.g.groups) / q.head_blocks);
+  const int64_t most = std::max<int64_t>(1, 148 * ctas(backward, q.g.wide, q.g.team, q.g.groups) / q.head_blocks);
   const int64_t units = std::min<int64_t>(most, (rows + slots - 1) / slots);
   q.span = (rows + units - 1) / units;
   q.units = (rows + q.span - 1) / q.span;

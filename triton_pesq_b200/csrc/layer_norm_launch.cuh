@@ -9,7 +9,7 @@ namespace lnorm {
 
 template <class TX, class TY, int TEAM, int GROUPS, bool kWide>
 cudaError_t launch_team(const Args& p, const Geometry& g, bool backward, cudaStream_t s) {
-  constexpr int threads = TEAM > kThreads ? TEAM : kThreads;
+  constexpr int threads = threads_of(TEAM);
   if (backward)
     backward_kernel<TX, TY, TEAM, GROUPS, kWide><<<(unsigned)g.blocks, threads, 0, s>>>(p);
   else
@@ -29,10 +29,18 @@ cudaError_t launch_width(const Args& p, const Geometry& g, bool backward, cudaSt
       if (g.groups == 2) return launch_team<TX, TY, 32, 2, kWide>(p, g, backward, s);
       return launch_team<TX, TY, 32, kMost, kWide>(p, g, backward, s);
     case 64: return launch_team<TX, TY, 64, kMost, kWide>(p, g, backward, s);
+    case 96:
+      if (g.groups == 2) return launch_team<TX, TY, 96, 2, kWide>(p, g, backward, s);
+      return launch_team<TX, TY, 96, kMost, kWide>(p, g, backward, s);
     case 128: return launch_team<TX, TY, 128, kMost, kWide>(p, g, backward, s);
+    case 160: return launch_team<TX, TY, 160, kMost, kWide>(p, g, backward, s);
+    case 192: return launch_team<TX, TY, 192, kMost, kWide>(p, g, backward, s);
     case 256: return launch_team<TX, TY, 256, kMost, kWide>(p, g, backward, s);
     default:
-      if constexpr (kMost < 4) return launch_team<TX, TY, 512, kMost, kWide>(p, g, backward, s);
+      if constexpr (kMost < 4) {
+        if (g.team == 384) return launch_team<TX, TY, 384, kMost, kWide>(p, g, backward, s);
+        return launch_team<TX, TY, 512, kMost, kWide>(p, g, backward, s);
+      }
       return cudaErrorInvalidConfiguration;
   }
 }
