@@ -71,8 +71,9 @@ struct Args {
   int heads, key, value;
   int reverse;
   float scale;
-  int chunks, parts, part_chunks, slices;  // of a row; chunks of a part; CTAs side by side over the values
-  float *starts, *factors;  // [rows, parts, DK, DV], [rows, parts]: of a sweep and its join
+  int chunks, parts, part_chunks, slices;  // of a row; of a row that is cut; chunks of a part; CTAs side by side over the values
+  int64_t whole;            // the first rows, which are not cut
+  float *starts, *factors;  // [cut rows, parts, DK, DV], [cut rows, parts]: of a sweep and its join
   int joined;               // a join has made the states that the parts begin from; else they are made from the sweep's
   void* kept;               // states before the chunks
   // results
@@ -392,6 +393,19 @@ struct Row {
   __device__ __forceinline__ int64_t time(int64_t s) const { return reverse && s < n ? n - 1 - s : s; }
 };
 
+// What a CTA works on: a whole row, or a part of one of those after
+struct Span {
+  int64_t index;
+  int part, c0, c1;
+  __device__ __forceinline__ Span(const Args& p, int64_t unit) {
+    const bool cut = unit >= p.whole;
+    index = cut ? p.whole + (unit - p.whole) / p.parts : unit;
+    part = cut ? (int)((unit - p.whole) % p.parts) : 0;
+    c0 = part * p.part_chunks;
+    c1 = cut ? min(p.chunks, c0 + p.part_chunks) : p.chunks;
+  }
+};
+
 // Rows s0 .. s0 + C - 1 of an operand to a tile, zeros for steps past the row's length.  The columns past `cols` are
 // zeros from before.
 template <class T, int D, int C, int THREADS>
@@ -641,12 +655,13 @@ struct State {
   // What a part begins from: the row's state `from`, and what the parts before it in scan order (after it, kBackward) add
   template <bool kBackward>
   __device__ __forceinline__ void begin(const Args& p, int64_t index, int part, const float* from, int padded, int first) {
-    if (p.parts == 1) {
+    if (index < p.whole) {
       read(from, p.key, p.value, first);
       return;
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");  // for the sweep, or the join, which this kernel is launched close to
-    const float* starts = p.starts + index * p.parts * DK * padded;
+    const int64_t cut = (index - p.whole) * p.parts;
+    const float* starts = p.starts + cut * DK * padded;
     if (p.joined) {
       read(starts + (int64_t)part * DK * padded, DK, padded, first);
       return;
@@ -654,7 +669,7 @@ struct State {
     read(from, p.key, p.value, first);
 #pragma unroll 1
     for (int i = kBackward ? p.parts - 1 : 0; i != part; i += kBackward ? -1 : 1) {
-      const float factor = p.factors[index * p.parts + i];
+      const float factor = p.factors[cut + i];
       const float* add = starts + (int64_t)i * DK * padded + first;
       each([&](int r, int c, float& a, float& b) {
         const float2 more = *reinterpret_cast<const float2*>(add + (int64_t)r * padded + c);
@@ -886,11 +901,11 @@ __global__ void __launch_bounds__(128, DK > 64 ? 2 : 3) forward_kernel(const __g
   const int rg = warp % RG, wc = warp / RG;
 
   const int slice = blockIdx.x % p.slices;
-  const int64_t unit = blockIdx.x / p.slices, index = unit / p.parts;
-  const int part = (int)(unit - index * p.parts);
+  const Span span(p, blockIdx.x / p.slices);
+  const int64_t index = span.index;
+  const int part = span.part, c0 = span.c0, c1 = span.c1;
   const Row row(p, index);
   const int first = slice * DV, cols = min(DV, p.value - first);
-  const int c0 = part * p.part_chunks, c1 = min(p.chunks, c0 + p.part_chunks);
   const int padded = DV * p.slices;  // columns of the states in memory
   const int key = kWhole ? DK : sixteens(p.key), value = kWhole ? DV : sixteens(cols);
 
@@ -999,11 +1014,11 @@ __global__ void __launch_bounds__(128) sweep_kernel(const __grid_constant__ Args
   char* decays = shared + 2 * Sh::kTiles;
   const int warp = threadIdx.x >> 5;
   const int slice = blockIdx.x % p.slices;
-  const int64_t unit = blockIdx.x / p.slices, index = unit / p.parts;
-  const int part = (int)(unit - index * p.parts);
-  const Row row(p, index);
+  const int64_t unit = blockIdx.x / p.slices;  // of the rows that are cut
+  const Span span(p, p.whole + unit);
+  const int part = span.part, c0 = span.c0, c1 = span.c1;
+  const Row row(p, span.index);
   const int first = slice * DV, cols = min(DV, p.value - first), padded = DV * p.slices;
-  const int c0 = part * p.part_chunks, c1 = min(p.chunks, c0 + p.part_chunks);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (part == (kBackward ? 0 : p.parts - 1)) return;  // (nothing begins from it)
   clear<THREADS>(shared, 2 * Sh::kTiles);
@@ -1050,8 +1065,8 @@ __global__ void __launch_bounds__(128) sweep_kernel(const __grid_constant__ Args
     if (warp == WARPS - 1 && i + 1 < count) store(i + 1);
     __syncthreads();
   }
-  S.write(p.starts + (index * p.parts + part) * DK * padded, DK, padded, first);
-  if (threadIdx.x == 0 && slice == 0) p.factors[index * p.parts + part] = factor;
+  S.write(p.starts + unit * DK * padded, DK, padded, first);
+  if (threadIdx.x == 0 && slice == 0) p.factors[unit] = factor;
 }
 
 // What the parts add, to the states that they begin from; a thread takes an element of a row's state
@@ -1059,13 +1074,13 @@ template <int kThreads>
 __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ Args p, int DK, int DV, int backward) {
   asm volatile("griddepcontrol.launch_dependents;\ngriddepcontrol.wait;" ::: "memory");
   const int64_t size = (int64_t)DK * DV, per = (size + kThreads - 1) / kThreads;
-  const int64_t index = blockIdx.x / per, at = (blockIdx.x - index * per) * kThreads + threadIdx.x;
+  const int64_t cut = blockIdx.x / per, index = p.whole + cut, at = (blockIdx.x - cut * per) * kThreads + threadIdx.x;
   if (at >= size) return;
   const int r = (int)(at / DV), c = (int)(at - (int64_t)r * DV);
   const float* from = backward ? p.dlast : p.state;
   float s = from && r < p.key && c < p.value ? from[(index * p.key + r) * p.value + c] : 0.0f;
-  float* starts = p.starts + index * p.parts * size + at;
-  const float* factors = p.factors + index * p.parts;
+  float* starts = p.starts + cut * p.parts * size + at;
+  const float* factors = p.factors + cut * p.parts;
   constexpr int kAhead = 8;  // parts whose loads are on their way together
   for (int i0 = 0; i0 < p.parts; i0 += kAhead) {
     float add[kAhead], factor[kAhead];
@@ -1124,10 +1139,10 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
   const bool by_rows = warp < SIDE;
   const int rg = warp % SIDE % RG, wc = warp % SIDE / RG;
 
-  const int64_t index = blockIdx.x / p.parts;
-  const int part = (int)(blockIdx.x - index * p.parts);
+  const Span span(p, blockIdx.x);
+  const int64_t index = span.index;
+  const int part = span.part, c0 = span.c0, c1 = span.c1;
   const Row row(p, index);
-  const int c0 = part * p.part_chunks, c1 = min(p.chunks, c0 + p.part_chunks);
 
   const int key = kWhole ? DK : sixteens(p.key), value = kWhole ? DV : sixteens(p.value);
 
@@ -1136,7 +1151,7 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
   if (by_rows) {
     S.template begin<true>(p, index, part, p.dlast ? p.dlast + index * p.key * p.value : nullptr, DV, 0);
     S.template publish<T>(s_grad, key, value);
-  } else if (p.parts > 1) {
+  } else if (index >= p.whole) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
   }
   __syncthreads();

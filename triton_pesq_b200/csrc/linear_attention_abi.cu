@@ -66,7 +66,7 @@ int check(const pesq_linear_attention_desc* d) {
 struct Plan {
   Geometry g;
   int chunks, parts, part_chunks, slices;
-  int64_t rows;
+  int64_t rows, whole;  // of them not cut
   size_t starts, factors, sums;  // bytes of the workspace's pieces
   size_t bytes() const { return starts + factors + sums; }
 };
@@ -102,15 +102,19 @@ Plan plan(const pesq_linear_attention_desc& d, bool backward) {
   q.slices = dv / q.g.dv;
   q.g.chunk = chunk_of(d.dtype, dk, dv);
   q.chunks = (int)((d.steps + q.g.chunk - 1) / q.g.chunk);
-  const int64_t ctas = q.rows * q.slices, room = 148 * resident(d.dtype, q.g, backward) / ctas;
-  const bool cut = q.chunks >= kFewChunks && room >= (backward ? 2 : 4);
-  const int64_t parts = cut ? std::min<int64_t>(d.lengths ? kRagged * room : room, q.chunks) : 1;
+  const int64_t hold = 148 * resident(d.dtype, q.g, backward) / q.slices;  // rows that the device holds at once
+  int64_t last = q.rows < hold ? q.rows : d.lengths ? 0 : q.rows % hold;
+  int64_t parts = 1;
+  if (q.chunks >= kFewChunks && last > 0 && hold / last >= (backward ? 2 : 4))
+    parts = std::min<int64_t>((d.lengths ? kRagged : 1) * (hold / last), q.chunks);
   q.part_chunks = (int)((q.chunks + parts - 1) / parts);
   q.parts = (q.chunks + q.part_chunks - 1) / q.part_chunks;
-  q.g.blocks = ctas * q.parts;
+  if (q.parts == 1) last = 0;
+  q.whole = q.rows - last;
+  q.g.blocks = (q.whole + last * q.parts) * q.slices;
   if (q.parts > 1) {
-    q.starts = round16((size_t)q.rows * q.parts * dk * dv * 4);
-    q.factors = round16((size_t)q.rows * q.parts * 4);
+    q.starts = round16((size_t)last * q.parts * dk * dv * 4);
+    q.factors = round16((size_t)last * q.parts * 4);
   }
   if (backward && d.decay_shared) q.sums = round16((size_t)q.rows * q.chunks * 8);
   return q;
@@ -153,6 +157,7 @@ Args arguments(const pesq_linear_attention_desc& d, const Plan& q, void* workspa
   a.chunks = q.chunks;
   a.parts = q.parts;
   a.part_chunks = q.part_chunks;
+  a.whole = q.whole;
   a.slices = q.slices;
   a.joined = q.parts > kFewParts;
   char* ws = static_cast<char*>(workspace);
@@ -174,7 +179,7 @@ cudaError_t sweep(Args a, const Plan& q, int dtype, bool backward, cudaStream_t 
   const int dv = q.g.dv * q.slices;
   g.dv = std::min(dv, 64);
   a.slices = dv / g.dv;
-  g.blocks = q.rows * q.parts * a.slices;
+  g.blocks = (q.rows - q.whole) * q.parts * a.slices;
   cudaError_t e = forward(a, g, dtype, backward ? kSweepBackward : kSweep, s);
   if (e != cudaSuccess) return e;
   if (!a.joined) return cudaSuccess;
@@ -183,7 +188,7 @@ cudaError_t sweep(Args a, const Plan& q, int dtype, bool backward, cudaStream_t 
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t c{};
-  c.gridDim = dim3((unsigned)(q.rows * per));
+  c.gridDim = dim3((unsigned)((q.rows - q.whole) * per));
   c.blockDim = dim3(kJoinThreads);
   c.stream = s;
   c.attrs = &at;
