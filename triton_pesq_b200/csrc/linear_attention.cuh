@@ -482,6 +482,7 @@ __device__ __forceinline__ void load_tile(T* tile, const Operand& o, int first, 
     from += kRows * step;
   }
 }
+__device__ __forceinline__ void prefetch(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 __device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
@@ -1178,6 +1179,23 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
     }
     copies_issued();
   };
+  // There is no room for a chunk's tiles while another's are worked on: they come as far as the L2 cache meanwhile (896 rows of 500
+  // steps of 64 x 64: bfloat16 364 us without, 356 with; float16 616 and 571)
+  const auto fetch = [&](int chunk) {
+    const int64_t s0 = (int64_t)chunk * C;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < 4 * C; i += THREADS) {
+      const Operand& o = i < C ? p.q : i < 2 * C ? p.k : i < 3 * C ? p.v : p.dy;
+      const int64_t s = s0 + i % C;
+      if (s >= row.n) continue;
+      const char* at = static_cast<const char*>(o.p) + (row.b * o.sb + row.time(s) * o.st + row.h * o.sh) * (int64_t)sizeof(T);
+      for (int x = 0; x < (i < 2 * C ? p.key : p.value) * (int)sizeof(T); x += 128) prefetch(at + x);
+    }
+    if (s0 < row.n) {
+      const char* at = static_cast<const char*>(p.kept) + (index * p.chunks + chunk) * kept_bytes(DK, DV);
+      for (int x = threadIdx.x * 128; x < kPlanes<T> * DK * DV * (int)sizeof(Stored<T>); x += THREADS * 128) prefetch(at + x);
+    }
+  };
   const auto sums_of = [&](int chunk) { return reinterpret_cast<float2*>(decays + (chunk & 1) * C * 20); };
   Decays<C> now, next;
   const auto store = [&](int chunk) {
@@ -1194,6 +1212,7 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
     const int64_t s0 = (int64_t)chunk * C;
     copies_done();
     __syncthreads();
+    if (chunk > c0) fetch(chunk - 1);
     if (warp == WARPS - 1 && chunk > c0) next.load(p, row, s0 - C);
     const float2* sums = sums_of(chunk);
     const float *before = reinterpret_cast<const float*>(sums + C), *after = before + C, *tail = after + C;
