@@ -124,6 +124,15 @@ def test_rows_in_parts(cuda_device, dtype, shape, gated, reverse):
     compare(*make(*shape, dtype, gated=gated, reset=gated, lengths=reverse, seed=9), cuda_device, reverse=reverse)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape,gated,reverse", [((45, 390, 10, 16, 24), True, True), ((30, 400, 10, 24, 16), False, False),
+                                                 ((23, 385, 10, 16, 72), True, False)])
+def test_rows_left_over_from_full_rounds(cuda_device, dtype, shape, gated, reverse):
+    """A few rows more than the device holds at once, of the forward, of the backward, and of two CTAs a row: cut, the others whole."""
+
+    compare(*make(*shape, dtype, gated=gated, reset=gated, seed=10), cuda_device, reverse=reverse)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("steps", [1, 2, 7, 8, 9])
 @pytest.mark.parametrize("widths", [(64, 64), (31, 33), (128, 100), (5, 3)])
