@@ -139,6 +139,17 @@ __device__ __forceinline__ float2 floats_of(uint32_t pair, __half) {
   return __half22float2(*reinterpret_cast<const __half2*>(&pair));
 }
 
+__device__ __forceinline__ uint32_t narrow_pair(float x, float y, __nv_bfloat16) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t narrow_pair(float x, float y, __half) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+  return r;
+}
+
 // ------------------------------------------------------------------------------------------- operands
 //
 // A thread's share of a 16 x 16 left operand is four pairs of adjacent columns: rows g and g + 8 (g = lane / 4)
@@ -175,6 +186,14 @@ template <>
 struct Made<__nv_bfloat16> {
   uint32_t hi[4], lo[4];
 };
+// What goes into a state, which is an output in 32 bits: of three terms of bfloat16 (of two, 2.2e-6 of the last state are off instead of
+// 1.2e-7; 364 + 139 us and 381 + 145 of the 896 rows below)
+template <class T>
+struct Finest : Made<T> {};
+template <>
+struct Finest<__nv_bfloat16> : Made<__nv_bfloat16> {
+  uint32_t least[4];
+};
 template <class T>
 struct MadeB {
   uint32_t hi[4], lo[4];
@@ -192,6 +211,20 @@ __device__ __forceinline__ void make(Made<T>& m, const float (&x)[8]) {
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) split_tf32(x[i], m.hi[i], m.lo[i]);
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void make(Finest<T>& m, const float (&x)[8]) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      split_bf16(x[2 * i], x[2 * i + 1], m.hi[i], m.lo[i]);
+      const float2 hi = floats_of(m.hi[i], T{}), lo = floats_of(m.lo[i], T{});
+      m.least[i] = narrow_pair((x[2 * i] - hi.x) - lo.x, (x[2 * i + 1] - hi.y) - lo.y, T{});
+    }
+  } else {
+    make(static_cast<Made<T>&>(m), x);
   }
 }
 
@@ -289,13 +322,17 @@ __device__ __forceinline__ void load_state(MadeB<T> (&b)[2], const Stored<T>* s,
     for (int i = 0; i < 8; ++i) split_tf32(x[i], b[i >> 2].hi[i & 3], b[i >> 2].lo[i & 3]);
   }
 }
-template <class T, int LD, int PLANE>
+template <class T, int LD, int PLANE, int PLANES>
 __device__ __forceinline__ void store_state(Stored<T>* s, int row, int col, float x, float y) {
   if constexpr (std::is_same<T, __nv_bfloat16>::value) {
     uint32_t hi, lo;
     split_bf16(x, y, hi, lo);
     *reinterpret_cast<uint32_t*>(s + row * LD + col) = hi;
     *reinterpret_cast<uint32_t*>(s + PLANE + row * LD + col) = lo;
+    if constexpr (PLANES == 3) {
+      const float2 a = floats_of(hi, T{}), b = floats_of(lo, T{});
+      *reinterpret_cast<uint32_t*>(s + 2 * PLANE + row * LD + col) = narrow_pair((x - a.x) - b.x, (y - a.y) - b.y, T{});
+    }
   } else {
     *reinterpret_cast<float2*>(s + row * LD + col) = make_float2(x, y);
   }
@@ -354,6 +391,11 @@ __device__ __forceinline__ void mma(float (&c)[4], const Made<T>& a, const InB<T
     mma_tf32(c, a.hi, b.lo);
     mma_tf32(c, a.hi, b.hi);
   }
+}
+template <class T>
+__device__ __forceinline__ void mma(float (&c)[4], const Finest<T>& a, const InB<T>& b) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) mma_bf16(c, a.least, b.x);
+  mma(c, static_cast<const Made<T>&>(a), b);
 }
 // input times state
 template <class T>
@@ -691,13 +733,13 @@ struct State {
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[m][n][e] = 0.0f;
     }
-    constexpr int kBlocks = C / 16, kTogether = std::is_same<T, __nv_bfloat16>::value ? kBlocks : 2;  // of registers' worth
+    constexpr int kBlocks = C / 16, kTogether = 2;  // of registers' worth
 #pragma unroll
     for (int m = 0; m < Shape::kTiles; ++m) {
       if (row_of(m) >= rows) continue;
 #pragma unroll
       for (int k0 = 0; k0 < kBlocks; k0 += kTogether) {
-        Made<T> left[kTogether];
+        Finest<T> left[kTogether];
 #pragma unroll
         for (int k = 0; k < kTogether; ++k) {
           const int at = (k0 + k) * 16;
@@ -732,26 +774,16 @@ struct State {
     }
   }
   // to shared memory, as an operand
-  template <class T>
+  template <class T, int PLANES = kPlanes<T>>
   __device__ __forceinline__ void publish(Stored<T>* s, int rows, int cols) {
-    each([&](int r, int c, float& a, float& b) { store_state<T, kLd<Stored<T>, DV>, DK * kLd<Stored<T>, DV>>(s, r, c, a, b); },
-         rows, cols);
+    constexpr int LD = kLd<Stored<T>, DV>;
+    each([&](int r, int c, float& a, float& b) { store_state<T, LD, DK * LD, PLANES>(s, r, c, a, b); }, rows, cols);
   }
 };
 
 // Bytes of the state before a chunk: two planes of 16 bits, or 32, of [DK][DV]
 __host__ __device__ constexpr int64_t kept_bytes(int DK, int DV) { return (int64_t)4 * DK * DV; }
 
-__device__ __forceinline__ uint32_t narrow_pair(float x, float y, __nv_bfloat16) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
-  return r;
-}
-__device__ __forceinline__ uint32_t narrow_pair(float x, float y, __half) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
-  return r;
-}
 __device__ __forceinline__ float2 narrow_pair(float x, float y, float) { return make_float2(x, y); }
 // A warp's 16 rows of N times 8 columns to rows of `width`: those of steps s and s + 8, where they are within the row; zeros
 // past its length.  The columns are blocks of 16, WC blocks apart, the thread's first at col
@@ -821,7 +853,7 @@ __device__ __forceinline__ void products(float (&sum)[2][4], const T* a, int m0,
 
 // 16 rows of a from m0, over their channels, `width` of at most D, times a state's columns (kTrans; else its rows), those of the
 // blocks of 16 in turn from wc that lie within `cols`
-template <class T, int D, int LDS, int PLANE, bool kTrans, int WC, int N>
+template <class T, int D, int LDS, int PLANE, bool kTrans, int WC, int PLANES = kPlanes<T>, int N>
 __device__ __forceinline__ void times_state(float (&out)[N][4], const T* a, int m0, const Stored<T>* state, int wc, int width, int cols) {
 #pragma unroll
   for (int n = 0; n < N; ++n)
@@ -836,6 +868,12 @@ __device__ __forceinline__ void times_state(float (&out)[N][4], const T* a, int 
     for (int n = 0; n < N / 2; ++n) {
       if ((n * WC + wc) * 16 >= cols) continue;
       MadeB<T> right[2];
+      if constexpr (PLANES == 3) {
+        InB<T> least[2];
+        load_b<T, LDS, kTrans>(least, state + 2 * PLANE, (n * WC + wc) * 16, kk);
+        mma(out[2 * n], left, least[0]);
+        mma(out[2 * n + 1], left, least[1]);
+      }
       load_state<T, LDS, PLANE, kTrans>(right, state, (n * WC + wc) * 16, kk);
       mma(out[2 * n], left, right[0]);
       mma(out[2 * n + 1], left, right[1]);
@@ -1109,6 +1147,13 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
 template <class T, int DK, int DV>
 constexpr int kSide = DK > 64 || DV > 64 ? 8 : 4;
 
+// Planes of the state's gradient.  The decays' gradients are sums of k dS v, of which two terms of bfloat16 would leave 1.3e-6
+// (with the third 7e-7, of the states that the forward keeps in two; 364 us and 389 of 896 rows of 500 steps of 64 x 64).  128 x 128
+// have room for two
+constexpr int grad_planes(bool bf16, int dk, int dv) { return !bf16 ? 1 : dk * dv < 128 * 128 ? 3 : 2; }
+template <class T, int DK, int DV>
+constexpr int kGradPlanes = grad_planes(std::is_same<T, __nv_bfloat16>::value, DK, DV);
+
 template <class T, int DK, int DV, int C>
 struct BackwardShared {
   static constexpr int SIDE = kSide<T, DK, DV>, WC = SIDE / (C / 16);
@@ -1116,7 +1161,8 @@ struct BackwardShared {
   static constexpr int kState = kPlanes<T> * DK * kLd<Stored<T>, DV> * (int)sizeof(Stored<T>);
   static constexpr int kDecays = kDecayBytes<C>;
   static constexpr int kSums = ((2 * WC + C / 16 + 1) * C + SIDE) * 4;
-  static constexpr int kBytes = kTiles + 2 * kState + kDecays + kSums;
+  static constexpr int kGrad = kState / kPlanes<T> * kGradPlanes<T, DK, DV>;
+  static constexpr int kBytes = kTiles + kState + kGrad + kDecays + kSums;
 };
 
 template <class T, int DK, int DV, int C, bool kWhole>
@@ -1130,7 +1176,7 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
   T *q = reinterpret_cast<T*>(shared), *k = q + C * LDK, *v = k + C * LDK, *dy = v + C * LDV;
   Stored<T>* s_state = reinterpret_cast<Stored<T>*>(shared + Sh::kTiles);  // before the chunk
   Stored<T>* s_grad = reinterpret_cast<Stored<T>*>(shared + Sh::kTiles + Sh::kState);
-  char* decays = shared + Sh::kTiles + 2 * Sh::kState;
+  char* decays = shared + Sh::kTiles + Sh::kState + Sh::kGrad;
   float* s_far = reinterpret_cast<float*>(decays + Sh::kDecays);  // [WC][C]: scale e^{G_i} q_i S dy_i
   float* s_end = s_far + WC * C;                                  // [WC][C]: e^{G_C - G_j} k_j dS v_j
   float* s_row = s_end + WC * C;                                  // [RG][C]: sums of W over sixteen j, of each i
@@ -1151,7 +1197,7 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
   State<DK, DV, SIDE> S;  // the gradient of the state, of the warps by rows
   if (by_rows) {
     S.template begin<true>(p, index, part, p.dlast ? p.dlast + index * p.key * p.value : nullptr, DV, 0);
-    S.template publish<T>(s_grad, key, value);
+    S.template publish<T, kGradPlanes<T, DK, DV>>(s_grad, key, value);
   } else if (index >= p.whole) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
   }
@@ -1260,7 +1306,7 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
       float dv[NV][4], dk[NK][4];
       if (live) {
         times_state<T, DK, LDS, PLANE, true, WC>(dv, k, rg * 16, s_grad, wc, key, value);
-        times_state<T, DV, LDS, PLANE, false, WC>(dk, v, rg * 16, s_grad, wc, value, key);
+        times_state<T, DV, LDS, PLANE, false, WC, kGradPlanes<T, DK, DV>>(dk, v, rg * 16, s_grad, wc, value, key);
         decay_rows(dv, after[i0], after[i0 + 8]);
         decay_rows(dk, after[i0], after[i0 + 8]);
         const float2 end = row_sums<T, LDK, WC>(dk, k, i0, wc);
@@ -1325,7 +1371,7 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
     }
     __syncthreads();  // the chunk's tiles, states and sums are read or written
     if (chunk > c0) load(chunk - 1);
-    if (by_rows && live) S.template publish<T>(s_grad, key, value);
+    if (by_rows && live) S.template publish<T, kGradPlanes<T, DK, DV>>(s_grad, key, value);
     if (warp == WARPS - 1) {
       // the decays' gradients: prefix sums over the chunk's steps in 64 bits
       constexpr int E = C / 32;

@@ -80,7 +80,9 @@ int resident(int dtype, const Geometry& g, bool backward) {
   const int wide = g.dk > 64 || (backward && g.dv > 64);
   int bytes;
   if (backward) {
-    bytes = 2 * g.chunk * (g.dk + g.dv + 2 * pad) * size + 2 * state + sums;
+    const bool bf16 = dtype == PESQ_BF16;
+    const int grad = state / (bf16 ? 2 : 1) * grad_planes(bf16, g.dk, g.dv);
+    bytes = 2 * g.chunk * (g.dk + g.dv + 2 * pad) * size + state + grad + sums;
   } else {
     const int tiles = g.chunk * (2 * g.dk + g.dv + 3 * pad) * size;
     bytes = (2 * tiles + state + 40 * g.chunk <= 75 << 10 ? 2 : 1) * tiles + state + 40 * g.chunk;
