@@ -12,8 +12,9 @@
 // accumulator.  Values are kept times 2^10: elements of X and A are at most about 1.2, those of the polynomial about 8, for the
 // usual coefficients, far from float16's largest, and the lo term of an element of 2^-10 still has its bits.
 // The accumulator of the instruction cuts off what it does not hold instead of rounding it, which adds up over a long
-// contraction (2.3e-5 of the result of a 385 x 1155 matrix, 5.0e-5 of 1280 x 3840).  So it sums 128 columns alone, and the
-// warps that read it add those sums in registers, rounded (4.4e-6 and 2.9e-6; float32 products 2.8e-6 and 3.6e-6).
+// contraction (2.3e-5 of the result of a 385 x 1155 matrix, 5.0e-5 of 1280 x 3840).  So it sums 64 columns alone, and the
+// warps that read it add those sums in registers, rounded (2.5e-6 and 1.5e-6; with 128 columns 4.3e-6 and 2.8e-6 in 4 % less time;
+// float32 products 2.8e-6 and 3.6e-6).
 //
 // Products run on tcgen05 with the accumulator in tensor memory, in tiles of 128 x 128.  Matrices lie in the workspace as the
 // tiles that the instruction reads from shared memory: 128 rows of 64 columns in the 128-byte swizzle, hi and lo
@@ -56,7 +57,7 @@ constexpr int kStages = 3, kStage = 2 * kPair;        // both operands
 constexpr int kReaders = 16;                          // warps of results: four for each quarter of the columns
 constexpr int kThreads = 64 + 32 * kReaders;          // copies, products, results
 constexpr int kShared = kStages * kStage + 1024;      // (aligned to 1024 in the kernel)
-constexpr int kSegment = 2;                           // stages whose products are summed in tensor memory
+constexpr int kSegment = 1;                           // stages whose products are summed in tensor memory
 constexpr float kScale = 1024.0f;                     // of what is kept
 constexpr int kMost = 32768;                          // rows or columns
 constexpr int kItems = 128;                           // matrices of a launch
@@ -429,14 +430,14 @@ __device__ __forceinline__ void finish(const Call& p, int mode, int from, const 
 // The three products of a step, 16 columns of the contraction after the other
 __device__ __forceinline__ void products_of(uint32_t to, uint32_t a, uint32_t b, bool transposed, bool add) {
   const uint32_t instruction = kInstruction | (transposed ? kTransposedB : 0);
+  // (the lower terms first: what the accumulator cuts off is a share of what it holds)
 #pragma unroll
-  for (int s = 0; s < kDepth / 16; ++s) {
-    const uint32_t as = a + s * 32, bs = b + s * (transposed ? 2048 : 32);
-    const uint64_t a_hi = descriptor(as, false), a_lo = descriptor(as + kPlane, false);
-    const uint64_t b_hi = descriptor(bs, transposed), b_lo = descriptor(bs + kPlane, transposed);
-    product(to, a_lo, b_hi, instruction, add || s > 0);
-    product(to, a_hi, b_lo, instruction, true);
-    product(to, a_hi, b_hi, instruction, true);
+  for (int pair = 0; pair < 3; ++pair) {
+#pragma unroll
+    for (int s = 0; s < kDepth / 16; ++s) {
+      const uint32_t as = a + s * 32 + (pair == 0 ? kPlane : 0), bs = b + s * (transposed ? 2048 : 32) + (pair == 1 ? kPlane : 0);
+      product(to, descriptor(as, false), descriptor(bs, transposed), instruction, add || pair > 0 || s > 0);
+    }
   }
 }
 
