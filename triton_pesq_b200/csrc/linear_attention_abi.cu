@@ -93,6 +93,8 @@ int resident(int dtype, const Geometry& g, bool backward) {
 // Rows are cut in parts, as many as the device holds at once, where that is four times the rows or more forward
 // and twice backward: the parts' sweep and join take about 0.6 of a forward's time and 0.3 of a backward's, and some
 // 10 us (12 x 8 rows of 500 steps of 64 x 64 in bfloat16: one part 43 us, four 42; 128 rows: 43 and three 58; 16: 41 and eight 24).
+// Rows beyond full rounds of the device are cut by the same rule, and the others walked whole beside them (896 rows are six a SM
+// and eight more, bfloat16: 150 us forward and 390 backward with a round of their own, 139 and 364 cut).
 // Rows of different lengths are cut four times as often, since parts past a row's end leave their place to others (30
 // rows of up to 4001 steps of 96 x 128 in float16, trained: parts for one filling 953 us, for four 594).
 Plan plan(const pesq_linear_attention_desc& d, bool backward) {
