@@ -15,7 +15,8 @@
 // same head are added up in shared memory, and the CTAs' sums in a fixed order by a second kernel, so that a
 // result is the same every time.
 //
-// The bound is memory; what is in the way of it is instructions (16 bits to 32 and back, masks, addresses: issue slots 60 % full).
+// The bound is memory; what is in the way of it are rounds of sums and loads that 12 to 45 % of an SM's warps, whose registers hold
+// the rows, have to hide, and instructions (16 bits to 32 and back, masks: issue slots 45 to 57 % full).
 // Forward and backward on cold caches, with the bytes alone at the copy rate in brackets: 32000 x 896 bfloat16 26 (18) and 40 us
 // (27), 32000 x 14 heads of 64 28 (18) and 46 (27), 24006 x 1155 float32 to float16 40 (26) and 60 (43).  More rows on their way
 // (two to four) did not help, and took twice as long channel by channel (32000 x 895: 33 and 76 us), whose registers they leave no room for.
@@ -86,7 +87,7 @@ struct Row {
     for (int g = 0; g < GROUPS; ++g) e[g].store(base, row + g * kApart, width - g * kApart);
   }
   // Channels j and j + 1 (j even) of group g less the mean; those past the width, which are zero, stay so.  Where a group is in the row
-  // or out of it as a whole one selection takes the place of eight: instructions are what bounds these kernels
+  // or out of it as a whole one selection takes the place of eight (a backward of 32000 x 896 bfloat16 42 us, then 40)
   __device__ __forceinline__ Vec<2> less(int g, int j, float mean, int width) const {
     const int left = width - g * kApart;
     if (kWide) return e[g].two(j) + splat<2>(E::column(0) < left ? -mean : 0.0f);
