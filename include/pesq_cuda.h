@@ -544,7 +544,7 @@ typedef struct pesq_muon_desc {
   int32_t steps;      /* 1 .. 100 */
   double momentum;
   float lr, weight_decay;
-  float eps;          /* above 0 */
+  float eps;          /* 1.2e-38 (float32's least normal value) or more */
   float a, b, c;      /* -16 .. 16 */
   const float* grad_scale; /* device, times every gradient; the step is skipped where it is not finite; NULL: 1 */
 } pesq_muon_desc;
@@ -559,7 +559,7 @@ typedef struct pesq_orthogonalize_desc {
   int64_t count, rows, cols; /* rows, cols: 1 .. 32768 */
   int32_t dtype;             /* of x and out */
   int32_t steps;
-  float eps, a, b, c;
+  float eps, a, b, c;        /* as of a pesq_muon_desc */
 } pesq_orthogonalize_desc;
 int pesq_orthogonalize_workspace(const pesq_orthogonalize_desc* desc, size_t* bytes);
 int pesq_orthogonalize(const pesq_orthogonalize_desc* desc, void* stream, const void* x, void* out, void* workspace,

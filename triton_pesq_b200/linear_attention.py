@@ -43,7 +43,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
     Parameters
     ----------
     q, k
-        ``[batch, step, head, key]``, float32, bfloat16 or float16, one type, up to 128 channels.  Any strides:
+        ``[batch, step, head, key]``, float32, bfloat16 or float16, one type, up to 128 channels and 2^22 heads over the batch.  Any strides:
         slices of one projection, or heads that are shared by expansion, are read where they lie (a tensor whose channels
         are not adjacent is copied).
     v
