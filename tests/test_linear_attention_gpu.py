@@ -323,6 +323,23 @@ def test_two_streams_at_once(cuda_device):
         assert torch.equal(a[0], e[0]) and torch.equal(a[1], e[1])
 
 
+@pytest.mark.parametrize("shape", [(3, 400, 4, 64, 64), (2, 300, 2, 128, 100), (1, 1300, 2, 32, 16)])
+def test_states_beside_bfloat16_are_of_32_bits(cuda_device, shape):
+    """The last state and the first one's gradient, by their norm.  Three terms hold 24 bits, and a state is a chunk's sum (in
+    four to eight pieces, each cut off at 2^-23 of it) and a decay a chunk: some ten roundings of random sign, 10**0.5 * 2^-23."""
+
+    (q, k, v, decay, state), dy, dlast, kw = make(*shape, BF16, gated=True, seed=12)
+    mine = [t.to(cuda_device) for t in (q, k, v, decay)]
+    first, wide = state.to(cuda_device).requires_grad_(True), state.double().requires_grad_(True)
+    y, last = linear_attention(*mine, first, **kw)
+    wy, wlast = definition(*(t.double() for t in (q, k, v, decay)), wide, **kw)
+    got = torch.autograd.grad((y, last), first, (dy.to(cuda_device), dlast.to(cuda_device)))[0]
+    want = torch.autograd.grad((wy, wlast), wide, (dy.double(), dlast.double()))[0]
+    for name, x, e in (("last", last, wlast), ("d state", got, want)):
+        off = float((x.detach().cpu().double() - e).norm() / e.norm())
+        assert off <= 10**0.5 * 2.0**-23, (name, off)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_offsets_past_32_bits(cuda_device, dtype):
     """The last steps of operands of more than 2^31 elements, and operands whose steps, heads and rows lie as far apart."""
