@@ -1,0 +1,51 @@
+"""Operands of the layer operators' C entries that are less aligned than what the kernels load and store: refused on the host,
+before any launch.  The addresses are not memory: where there is a GPU the tests are skipped, so that nothing is ever launched on
+them."""
+
+import ctypes
+
+import pytest
+import torch
+
+from triton_pesq_b200 import _lib
+
+pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="a call that is not refused would be launched")
+
+INVALID = 1
+ONE = ctypes.c_void_p(64)
+
+
+def at(address):
+    return ctypes.c_void_p(address)
+
+
+def attention(dtype, key, value, **kw):
+    x = _lib.Heads(data=64, batch_stride=19200, step_stride=192, head_stride=64)
+    d = _lib.LinearAttentionDesc(batch=2, steps=100, heads=3, key=key, value=value, dtype=dtype, scale=1.0, q=x, k=x, v=x, log_decay=64)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return ctypes.byref(d), x
+
+
+def attention_forward(d, y=ONE, last=ONE):
+    return _lib.library().pesq_linear_attention_forward(d, None, y, last, None, 0, ONE, 1 << 40)
+
+
+def attention_backward(d, dy, dq=ONE, dk=ONE, dv=ONE, ddecay=ONE, dstate=ONE, dlast=ONE):
+    return _lib.library().pesq_linear_attention_backward(d, None, ONE, 1 << 40, dy, dlast, dq, dk, dv, ddecay, dstate, ONE, 1 << 40)
+
+
+@pytest.mark.parametrize("dtype,size", [(_lib.F32, 4), (_lib.BF16, 2), (_lib.F16, 2)])
+def test_attention_results_of_even_width_are_stored_in_pairs(dtype, size):
+    """Two adjacent elements of a row of even width are one store; rows of odd width go element by element."""
+
+    for off in (size, size // 2, 1):
+        d, x = attention(dtype, 64, 48)
+        assert attention_forward(d, y=at(64 + off)) == INVALID
+        for name in ("dq", "dk", "dv"):
+            assert attention_backward(d, x, **{name: at(64 + off)}) == INVALID, (name, off)
+    for off in (size // 2, 1):
+        d, x = attention(dtype, 33, 47)
+        assert attention_forward(d, y=at(64 + off)) == INVALID
+        for name in ("dq", "dk", "dv"):
+            assert attention_backward(d, x, **{name: at(64 + off)}) == INVALID, (name, off)

@@ -1,0 +1,68 @@
+"""The layer operators' C entries with results and operands that are aligned to no more than their checks ask for."""
+
+import ctypes
+
+import pytest
+import torch
+
+from triton_pesq_b200 import _lib, linear_attention
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+CODES = {F32: _lib.F32, BF16: _lib.BF16, F16: _lib.F16}
+
+
+def place(t, off):
+    """t's values as a dense tensor that begins `off` elements past a 512-byte boundary, with a canary on both sides."""
+
+    room = torch.full((off + t.numel() + 8,), 7.0, dtype=t.dtype, device=t.device)
+    assert room.data_ptr() % 512 == 0
+    room[off:off + t.numel()] = t.flatten()
+    return room, room[off:off + t.numel()].view(t.shape)
+
+
+def untouched(room, off, numel):
+    return bool((room[:off] == 7).all()) and bool((room[off + numel:] == 7).all())
+
+
+def heads(t):
+    return _lib.Heads(data=t.data_ptr(), batch_stride=t.stride(0), step_stride=t.stride(1), head_stride=t.stride(2))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("key,value", [(32, 24), (33, 47), (24, 33)])
+@pytest.mark.parametrize("steps", [5, 130])
+def test_attention(cuda_device, dtype, key, value, steps):
+    """Results of even width two elements past a boundary, of odd width one: as the torch entry's, bit for bit."""
+
+    g = torch.Generator().manual_seed(1)
+    batch, count = 2, 3
+    q, k = (torch.randn(batch, steps, count, key, generator=g).to(dtype).to(cuda_device) for _ in range(2))
+    v, dy = (torch.randn(batch, steps, count, value, generator=g).to(dtype).to(cuda_device) for _ in range(2))
+    decay = torch.tensor([-0.1, -0.5, -0.01], device=cuda_device)
+    state, dlast = (torch.randn(batch, count, key, value, generator=g).to(cuda_device) for _ in range(2))
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v, decay, state)]
+    want = linear_attention(*leaves)
+    grads = torch.autograd.grad(want, leaves, (dy, dlast))
+    lib, stream = _lib.library(), torch.cuda.current_stream().cuda_stream
+    d = _lib.LinearAttentionDesc(batch=batch, steps=steps, heads=count, key=key, value=value, dtype=CODES[dtype], scale=1.0,
+                                 decay_shared=1, q=heads(q), k=heads(k), v=heads(v), decay_head_stride=1)
+    # (32-bit operands one element past a boundary)
+    inputs = [place(t, 1)[1] for t in (decay, state, dlast)]
+    d.log_decay, d.state = inputs[0].data_ptr(), inputs[1].data_ptr()
+    sizes = [ctypes.c_size_t() for _ in range(3)]
+    _lib.check(lib.pesq_linear_attention_sizes(ctypes.byref(d), *[ctypes.byref(n) for n in sizes]), "sizes")
+    work, kept, back = (torch.empty(n.value + 16, dtype=torch.uint8, device=cuda_device) for n in sizes)
+    off = {key: 2 if key % 2 == 0 else 1, value: 2 if value % 2 == 0 else 1}
+    rooms = [(place(torch.zeros_like(t), o), o, e) for t, o, e in
+             ((v, off[value], want[0]), (state, 1, want[1]), (q, off[key], grads[0]), (q, off[key], grads[1]), (v, off[value], grads[2]),
+              (decay, 1, grads[3]), (state, 1, grads[4]))]
+    y, last, dq, dk, dv, ddecay, dstate = (ctypes.c_void_p(r[0][1].data_ptr()) for r in rooms)
+    _lib.check(lib.pesq_linear_attention_forward(ctypes.byref(d), ctypes.c_void_p(stream), y, last, ctypes.c_void_p(kept.data_ptr()),
+                                                 kept.numel(), ctypes.c_void_p(work.data_ptr()), work.numel()), "forward")
+    _lib.check(lib.pesq_linear_attention_backward(ctypes.byref(d), ctypes.c_void_p(stream), ctypes.c_void_p(kept.data_ptr()), kept.numel(),
+                                                  heads(dy), ctypes.c_void_p(inputs[2].data_ptr()), dq, dk, dv, ddecay, dstate,
+                                                  ctypes.c_void_p(back.data_ptr()), back.numel()), "backward")
+    for ((room, got), o, e) in rooms:
+        assert torch.equal(got, e) and untouched(room, o, got.numel())

@@ -207,6 +207,10 @@ int check_operands(const pesq_linear_attention_desc* d) {
   if (all % element(d->dtype)) return set_error(PESQ_ERR_INVALID_ARGUMENT, "an operand that is not aligned to its type");
   return PESQ_OK;
 }
+// A dense result, whose rows of even width are stored two elements at a time
+bool fits(const void* result, const pesq_linear_attention_desc& d, int64_t width) {
+  return reinterpret_cast<uintptr_t>(result) % (element(d.dtype) * (width % 2 == 0 ? 2 : 1)) == 0;
+}
 int check_workspace(const void* workspace, size_t bytes, size_t need) {
   if (need && (!workspace || bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
     return set_error(PESQ_ERR_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
@@ -231,7 +235,8 @@ int pesq_linear_attention_forward(const pesq_linear_attention_desc* d, void* str
   if (const int status = check(d)) return status;
   if (const int status = check_operands(d)) return status;
   if (!y) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL result");
-  if (reinterpret_cast<uintptr_t>(y) % 4) return set_error(PESQ_ERR_INVALID_ARGUMENT, "a result that is not 4-byte aligned");
+  if (!fits(y, *d, d->value))
+    return set_error(PESQ_ERR_INVALID_ARGUMENT, "y has to be aligned to its type, and where its width is even to two elements");
   if (kept && (kept_bytes < kept_size(*d) || reinterpret_cast<uintptr_t>(kept) % 16))
     return set_error(PESQ_ERR_WORKSPACE, "room for the kept states too small or not 16-byte aligned");
   Plan q = plan(*d, false);
@@ -261,8 +266,8 @@ int pesq_linear_attention_backward(const pesq_linear_attention_desc* d, void* st
   if (!dy.data || !dq || !dk || !dv || !ddecay) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL operand");
   if (reinterpret_cast<uintptr_t>(dy.data) % element(d->dtype))
     return set_error(PESQ_ERR_INVALID_ARGUMENT, "an operand that is not aligned to its type");
-  if ((reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv)) % 4)
-    return set_error(PESQ_ERR_INVALID_ARGUMENT, "a result that is not 4-byte aligned");
+  if (!fits(dq, *d, d->key) || !fits(dk, *d, d->key) || !fits(dv, *d, d->value))
+    return set_error(PESQ_ERR_INVALID_ARGUMENT, "a gradient has to be aligned to its type, and where its width is even to two elements");
   if (!kept || kept_bytes < kept_size(*d) || reinterpret_cast<uintptr_t>(kept) % 16)
     return set_error(PESQ_ERR_WORKSPACE, "kept states missing, too small or not 16-byte aligned");
   Plan q = plan(*d, true);
