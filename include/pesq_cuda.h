@@ -513,8 +513,8 @@ typedef struct pesq_linear_attention_desc {
 int pesq_linear_attention_sizes(const pesq_linear_attention_desc* desc, size_t* forward, size_t* kept, size_t* backward);
 /* y: [batch, steps, heads, value] dense; last: [batch, heads, key, value], the
  * state after the last step, or NULL; kept: for the backward call, or NULL.
- * y is aligned to two elements where `value` is even, else to one; so are the
- * backward's dq and dk of `key`, and dv of `value`. */
+ * Operands are aligned to their types; y to two elements where `value` is even, and
+ * so are the backward's dq and dk where `key` is, dv where `value` is. */
 int pesq_linear_attention_forward(const pesq_linear_attention_desc* desc, void* stream, void* y, float* last, void* kept,
                                   size_t kept_bytes, void* workspace, size_t workspace_bytes);
 /* dlast may be NULL (zeros); dstate may be NULL (not wanted).  dq, dk, dv:

@@ -49,3 +49,20 @@ def test_attention_results_of_even_width_are_stored_in_pairs(dtype, size):
         assert attention_forward(d, y=at(64 + off)) == INVALID
         for name in ("dq", "dk", "dv"):
             assert attention_backward(d, x, **{name: at(64 + off)}) == INVALID, (name, off)
+
+
+def test_attention_operands_are_aligned_to_their_types():
+    good, x = attention(_lib.F32, 64, 48)
+    for dtype, off in ((_lib.F32, 2), (_lib.BF16, 1)):
+        odd = _lib.Heads(data=64 + off, batch_stride=19200, step_stride=192, head_stride=64)
+        for name in ("q", "k", "v"):
+            d, _ = attention(dtype, 64, 48, **{name: odd})
+            assert attention_forward(d) == INVALID and attention_backward(d, x) == INVALID, name
+        d, _ = attention(dtype, 64, 48)
+        assert attention_backward(d, odd) == INVALID
+    for name, address in (("log_decay", 66), ("state", 66), ("lengths", 68)):
+        d, _ = attention(_lib.BF16, 64, 48, **{name: address})
+        assert attention_forward(d) == INVALID and attention_backward(d, x) == INVALID, name
+    assert attention_forward(good, last=at(66)) == INVALID
+    for name in ("dlast", "ddecay", "dstate"):
+        assert attention_backward(good, x, **{name: at(66)}) == INVALID, name

@@ -200,16 +200,18 @@ cudaError_t sweep(Args a, const Plan& q, int dtype, bool backward, cudaStream_t 
   return cudaLaunchKernelEx(&c, join_kernel<kJoinThreads>, a, g.dk, dv, (int)backward);
 }
 
+bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 int check_operands(const pesq_linear_attention_desc* d) {
   if (!d->q.data || !d->k.data || !d->v.data || !d->log_decay) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL operand");
-  const uintptr_t all = reinterpret_cast<uintptr_t>(d->q.data) | reinterpret_cast<uintptr_t>(d->k.data) |
-                        reinterpret_cast<uintptr_t>(d->v.data);
-  if (all % element(d->dtype)) return set_error(PESQ_ERR_INVALID_ARGUMENT, "an operand that is not aligned to its type");
+  const int64_t size = element(d->dtype);
+  if (!aligned(d->q.data, size) || !aligned(d->k.data, size) || !aligned(d->v.data, size) || !aligned(d->log_decay, 4) ||
+      !aligned(d->state, 4) || !aligned(d->lengths, 8))
+    return set_error(PESQ_ERR_INVALID_ARGUMENT, "an operand that is not aligned to its type");
   return PESQ_OK;
 }
 // A dense result, whose rows of even width are stored two elements at a time
 bool fits(const void* result, const pesq_linear_attention_desc& d, int64_t width) {
-  return reinterpret_cast<uintptr_t>(result) % (element(d.dtype) * (width % 2 == 0 ? 2 : 1)) == 0;
+  return aligned(result, element(d.dtype) * (width % 2 == 0 ? 2 : 1));
 }
 int check_workspace(const void* workspace, size_t bytes, size_t need) {
   if (need && (!workspace || bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
@@ -237,6 +239,7 @@ int pesq_linear_attention_forward(const pesq_linear_attention_desc* d, void* str
   if (!y) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL result");
   if (!fits(y, *d, d->value))
     return set_error(PESQ_ERR_INVALID_ARGUMENT, "y has to be aligned to its type, and where its width is even to two elements");
+  if (!aligned(last, 4)) return set_error(PESQ_ERR_INVALID_ARGUMENT, "the last state is not aligned to its type");
   if (kept && (kept_bytes < kept_size(*d) || reinterpret_cast<uintptr_t>(kept) % 16))
     return set_error(PESQ_ERR_WORKSPACE, "room for the kept states too small or not 16-byte aligned");
   Plan q = plan(*d, false);
@@ -264,7 +267,7 @@ int pesq_linear_attention_backward(const pesq_linear_attention_desc* d, void* st
   if (const int status = check(d)) return status;
   if (const int status = check_operands(d)) return status;
   if (!dy.data || !dq || !dk || !dv || !ddecay) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL operand");
-  if (reinterpret_cast<uintptr_t>(dy.data) % element(d->dtype))
+  if (!aligned(dy.data, element(d->dtype)) || !aligned(dlast, 4) || !aligned(ddecay, 4) || !aligned(dstate, 4))
     return set_error(PESQ_ERR_INVALID_ARGUMENT, "an operand that is not aligned to its type");
   if (!fits(dq, *d, d->key) || !fits(dk, *d, d->key) || !fits(dv, *d, d->value))
     return set_error(PESQ_ERR_INVALID_ARGUMENT, "a gradient has to be aligned to its type, and where its width is even to two elements");
