@@ -480,7 +480,7 @@ typedef struct pesq_layer_norm_desc {
   const float *weight, *bias; /* [heads, width]; bias NULL: zeros */
 } pesq_layer_norm_desc;
 
-/* y: [batch, steps, heads, width] dense. */
+/* y: [batch, steps, heads, width] dense.  All operands are aligned to their types. */
 int pesq_layer_norm_forward(const pesq_layer_norm_desc* desc, void* stream, void* y);
 /* Bytes of a backward's workspace. */
 int pesq_layer_norm_workspace(const pesq_layer_norm_desc* desc, size_t* bytes);

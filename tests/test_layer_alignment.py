@@ -66,3 +66,23 @@ def test_attention_operands_are_aligned_to_their_types():
     assert attention_forward(good, last=at(66)) == INVALID
     for name in ("dlast", "ddecay", "dstate"):
         assert attention_backward(good, x, **{name: at(66)}) == INVALID, name
+
+
+def test_layer_norm_operands_are_aligned_to_their_types():
+    lib = _lib.library()
+
+    def call(out=_lib.BF16, x=64, weight=64, bias=64, dy=64, dx=64, dweight=64, dbias=64, y=64):
+        """Of float32, with gradients of `out`: (the forward's answer, the backward's)."""
+
+        d = _lib.LayerNormDesc(batch=2, steps=3, heads=1, width=64, dtype=_lib.F32, out_dtype=out, eps=1e-6, weight=weight, bias=bias,
+                               x=_lib.Heads(data=x, batch_stride=192, step_stride=64, head_stride=64))
+        g = _lib.Heads(data=dy, batch_stride=192, step_stride=64, head_stride=64)
+        return (lib.pesq_layer_norm_forward(ctypes.byref(d), None, at(y)),
+                lib.pesq_layer_norm_backward(ctypes.byref(d), None, g, at(dx), at(dweight), at(dbias), ONE, 1 << 40))
+
+    for name in ("x", "weight", "bias"):
+        assert call(**{name: 66}) == (INVALID, INVALID), name
+    assert call(y=65, dy=65) == (INVALID, INVALID)
+    assert call(out=_lib.F32, y=66, dy=66) == (INVALID, INVALID)
+    for name in ("dx", "dweight", "dbias"):
+        assert call(y=65, **{name: 66}) == (INVALID, INVALID), name

@@ -5,7 +5,7 @@ import ctypes
 import pytest
 import torch
 
-from triton_pesq_b200 import _lib, linear_attention
+from triton_pesq_b200 import _lib, layer_norm, linear_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -66,3 +66,35 @@ def test_attention(cuda_device, dtype, key, value, steps):
                                                   ctypes.c_void_p(back.data_ptr()), back.numel()), "backward")
     for ((room, got), o, e) in rooms:
         assert torch.equal(got, e) and untouched(room, o, got.numel())
+
+
+@pytest.mark.parametrize("dtype,out", [(F32, F32), (BF16, BF16), (F16, F16), (F32, BF16)])
+@pytest.mark.parametrize("width", [64, 33, 1155])
+def test_layer_norm(cuda_device, dtype, out, width):
+    """All operands and results one element past a boundary.  Sums may run in another order than those of whole pieces of 16
+    bytes: ten roundings of 32 bits of the largest value (times four for what a gradient is the difference of, times the root of 150 rows for
+    the vectors' sums), and one to the type."""
+
+    g = torch.Generator().manual_seed(2)
+    batch, steps = 3, 50
+    x = torch.randn(batch, steps, 1, width, generator=g).to(dtype).to(cuda_device)
+    dy = torch.randn(batch, steps, 1, width, generator=g).to(out).to(cuda_device)
+    weight, bias = (torch.randn(width, generator=g).to(cuda_device) for _ in range(2))
+    leaves = [x.clone().requires_grad_(True), weight.clone().requires_grad_(True), bias.clone().requires_grad_(True)]
+    want = layer_norm(*leaves, dtype=out)
+    grads = torch.autograd.grad(want, leaves, dy)
+    lib, stream = _lib.library(), torch.cuda.current_stream().cuda_stream
+    x, dy, weight, bias = (place(t, 1)[1] for t in (x, dy, weight, bias))
+    d = _lib.LayerNormDesc(batch=batch, steps=steps, heads=1, width=width, dtype=CODES[dtype], out_dtype=CODES[out], eps=1e-5, x=heads(x),
+                           weight=weight.data_ptr(), bias=bias.data_ptr())
+    size = ctypes.c_size_t()
+    _lib.check(lib.pesq_layer_norm_workspace(ctypes.byref(d), ctypes.byref(size)), "workspace")
+    work = torch.empty(size.value, dtype=torch.uint8, device=cuda_device)
+    rooms = [(place(torch.zeros_like(e), 1), e) for e in (want, *grads)]
+    y, dx, dweight, dbias = (ctypes.c_void_p(r[0][1].data_ptr()) for r in rooms)
+    _lib.check(lib.pesq_layer_norm_forward(ctypes.byref(d), ctypes.c_void_p(stream), y), "forward")
+    _lib.check(lib.pesq_layer_norm_backward(ctypes.byref(d), ctypes.c_void_p(stream), heads(dy), dx, dweight, dbias,
+                                            ctypes.c_void_p(work.data_ptr()), work.numel()), "backward")
+    for (room, got), e in rooms:
+        allowed = torch.finfo(e.dtype).eps * e.abs().double() + 10 * 2.0**-24 * float(e.abs().max()) * (12 if e.dim() == 1 else 4)
+        assert bool(((got.double() - e.double()).abs() <= allowed).all()) and untouched(room, 1, got.numel())

@@ -71,6 +71,15 @@ int check(const pesq_layer_norm_desc* d) {
   return PESQ_OK;
 }
 
+// To its type, which is all that channel by channel wants
+bool aligned(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % element(dtype) == 0; }
+int check_operands(const pesq_layer_norm_desc* d) {
+  if (!d->x.data || !d->weight) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL operand");
+  if (!aligned(d->x.data, d->dtype) || !aligned(d->weight, PESQ_F32) || !aligned(d->bias, PESQ_F32))
+    return set_error(PESQ_ERR_INVALID_ARGUMENT, "an operand that is not aligned to its type");
+  return PESQ_OK;
+}
+
 bool joined(const pesq_heads& s, const pesq_layer_norm_desc& d) {
   return !s.data || d.batch == 1 || s.batch_stride == d.steps * s.step_stride;
 }
@@ -182,7 +191,9 @@ extern "C" {
 
 int pesq_layer_norm_forward(const pesq_layer_norm_desc* d, void* stream, void* y) {
   if (const int status = check(d)) return status;
-  if (!d->x.data || !d->weight || !y) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL operand");
+  if (const int status = check_operands(d)) return status;
+  if (!y) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL result");
+  if (!aligned(y, d->out_dtype)) return set_error(PESQ_ERR_INVALID_ARGUMENT, "a result that is not aligned to its type");
   const Plan q = plan(*d, false, nullptr, y);
   Args a = arguments(*d, q);
   a.y = y;
@@ -200,8 +211,10 @@ int pesq_layer_norm_workspace(const pesq_layer_norm_desc* d, size_t* bytes) {
 int pesq_layer_norm_backward(const pesq_layer_norm_desc* d, void* stream, pesq_heads dy, void* dx, float* dweight,
                              float* dbias, void* workspace, size_t workspace_bytes) {
   if (const int status = check(d)) return status;
-  if (!d->x.data || !d->weight || !dy.data || !dx || !dweight || (d->bias && !dbias))
-    return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL operand");
+  if (const int status = check_operands(d)) return status;
+  if (!dy.data || !dx || !dweight || (d->bias && !dbias)) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL operand");
+  if (!aligned(dy.data, d->out_dtype) || !aligned(dx, d->dtype) || !aligned(dweight, PESQ_F32) || !aligned(dbias, PESQ_F32))
+    return set_error(PESQ_ERR_INVALID_ARGUMENT, "a gradient that is not aligned to its type");
   if (!workspace || workspace_bytes < part_bytes(*d) * 2 || reinterpret_cast<uintptr_t>(workspace) % 16)
     return set_error(PESQ_ERR_WORKSPACE, "workspace missing, too small or not 16-byte aligned");
   const Plan q = plan(*d, true, &dy, dx);
