@@ -86,3 +86,20 @@ def test_layer_norm_operands_are_aligned_to_their_types():
     assert call(out=_lib.F32, y=66, dy=66) == (INVALID, INVALID)
     for name in ("dx", "dweight", "dbias"):
         assert call(y=65, **{name: 66}) == (INVALID, INVALID), name
+
+
+def test_muon_tensors_are_aligned_to_their_types():
+    lib = _lib.library()
+
+    def step(dtype=_lib.BF16, **kw):
+        d = _lib.MuonDesc(grad_dtype=dtype, nesterov=1, adjust=0, steps=5, momentum=0.95, lr=0.02, weight_decay=0.1, eps=1e-7, a=3.4, b=-4.8,
+                          c=2.0, grad_scale=kw.pop("grad_scale", None))
+        t = (_lib.MuonTensor * 1)(_lib.MuonTensor(**{**dict(param=64, grad=64, momentum=64, copy=None, rows=100, cols=200), **kw}))
+        return lib.pesq_muon_step(ctypes.byref(d), t, 1, None, ONE, 1 << 40)
+
+    for kw in ({"param": 66}, {"momentum": 66}, {"grad": 65}, {"copy": 65}, {"grad_scale": 66}, {"dtype": _lib.F32, "grad": 66}):
+        assert step(**kw) == INVALID, kw
+    for dtype, off in ((_lib.F32, 2), (_lib.F16, 1)):
+        o = _lib.OrthogonalizeDesc(count=2, rows=100, cols=200, dtype=dtype, steps=5, eps=1e-7, a=3.4, b=-4.8, c=2.0)
+        assert lib.pesq_orthogonalize(ctypes.byref(o), None, at(64 + off), ONE, ONE, 1 << 40) == INVALID
+        assert lib.pesq_orthogonalize(ctypes.byref(o), None, ONE, at(64 + off), ONE, 1 << 40) == INVALID

@@ -5,7 +5,7 @@ import ctypes
 import pytest
 import torch
 
-from triton_pesq_b200 import _lib, layer_norm, linear_attention
+from triton_pesq_b200 import _lib, layer_norm, linear_attention, muon_step, orthogonalize
 
 pytestmark = pytest.mark.gpu
 
@@ -98,3 +98,22 @@ def test_layer_norm(cuda_device, dtype, out, width):
     for (room, got), e in rooms:
         allowed = torch.finfo(e.dtype).eps * e.abs().double() + 10 * 2.0**-24 * float(e.abs().max()) * (12 if e.dim() == 1 else 4)
         assert bool(((got.double() - e.double()).abs() <= allowed).all()) and untouched(room, 1, got.numel())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("shape", [(96, 257), (385, 200)])
+def test_muon(cuda_device, dtype, shape):
+    """Tensors one element past a boundary, through the torch entries: the same bits."""
+
+    g = torch.Generator().manual_seed(3)
+    param, momentum, grad = (torch.randn(shape, generator=g).to(cuda_device) for _ in range(3))
+    grad = grad.to(dtype)
+    copy = None if dtype == F32 else torch.zeros_like(grad)
+    tensors = [param, grad, momentum, *([] if copy is None else [copy])]
+    rooms = [place(t, 1) for t in tensors]
+    moved = [r[1] for r in rooms]
+    for p, gr, m, *c in (tensors, moved):
+        muon_step([p], [gr], [m], copies=c or None, lr=0.1)
+    for a, e, (room, _) in zip(moved, tensors, rooms):
+        assert torch.equal(a, e) and untouched(room, 1, e.numel())
+    assert torch.equal(orthogonalize(place(grad, 1)[1]), orthogonalize(grad)) and _lib.muon_check() == 0

@@ -957,6 +957,8 @@ int check_sizes(int64_t rows, int64_t cols) {
   if (rows > kMost || cols > kMost) return set_error(PESQ_ERR_UNSUPPORTED, "at most 32768 rows and columns");
   return PESQ_OK;
 }
+// (what lies at 16 bytes is read and written in fours, all else value by value)
+bool aligned(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % (dtype == PESQ_F32 ? 4 : 2) == 0; }
 int check_workspace(const void* workspace, size_t bytes, size_t need) {
   // (its tiles are read by bulk copies, and by instructions that want rows of eight in 1024 bytes, of the copy)
   if (!workspace || bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)
@@ -970,6 +972,7 @@ int muon_matrices(const pesq_muon_desc* d, const pesq_muon_tensor* tensors, int6
   if (!(d->momentum >= 0.0) || !(d->momentum < 1.0)) return set_error(PESQ_ERR_INVALID_ARGUMENT, "momentum must lie in [0, 1)");
   if (!(d->lr >= 0.0f) || !(d->weight_decay >= 0.0f))
     return set_error(PESQ_ERR_INVALID_ARGUMENT, "lr and weight_decay must not be negative");
+  if (!aligned(d->grad_scale, PESQ_F32)) return set_error(PESQ_ERR_INVALID_ARGUMENT, "grad_scale is not aligned to its type");
   if (d->adjust != PESQ_MUON_ORIGINAL && d->adjust != PESQ_MUON_MATCH_RMS)
     return set_error(PESQ_ERR_INVALID_ARGUMENT, "unknown adjustment");
   for (int64_t i = 0; i < count; ++i) {
@@ -977,6 +980,8 @@ int muon_matrices(const pesq_muon_desc* d, const pesq_muon_tensor* tensors, int6
     if (!t.grad) continue;
     if (!t.param || !t.momentum) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL parameter or momentum");
     if (t.copy && d->grad_dtype == PESQ_F32) return set_error(PESQ_ERR_INVALID_ARGUMENT, "copies are of 16-bit gradients' type");
+    if (!aligned(t.param, PESQ_F32) || !aligned(t.momentum, PESQ_F32) || !aligned(t.grad, d->grad_dtype) || !aligned(t.copy, d->grad_dtype))
+      return set_error(PESQ_ERR_INVALID_ARGUMENT, "a tensor that is not aligned to its type");
     if (const int status = check_sizes(t.rows, t.cols)) return status;
     const double ratio = (double)t.rows / (double)t.cols;
     const double adjust = d->adjust == PESQ_MUON_ORIGINAL ? std::sqrt(std::max(1.0, ratio))
@@ -991,6 +996,7 @@ int stack(const pesq_orthogonalize_desc* d, const void* x, void* out, std::vecto
   if (!d) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL descriptor");
   if (const int status = check_iteration(d->dtype, d->steps, d->eps, d->a, d->b, d->c)) return status;
   if (const int status = check_sizes(d->rows, d->cols)) return status;
+  if (!aligned(x, d->dtype) || !aligned(out, d->dtype)) return set_error(PESQ_ERR_INVALID_ARGUMENT, "a stack that is not aligned to its type");
   if (d->count < 1 || d->count > 1 << 20) return set_error(PESQ_ERR_INVALID_ARGUMENT, "between 1 and 2^20 matrices");
   const int64_t bytes = d->rows * d->cols * (d->dtype == PESQ_F32 ? 4 : 2);
   for (int64_t i = 0; i < d->count; ++i)
