@@ -110,7 +110,8 @@ def train(model, steps: int, batch: int = 8, seconds: float = 2.0, state_bits: i
 
     device = next(model.parameters()).device
     loss_fn = PesqLossCuda(0.5, sample_rate=16000).to(device)
-    matrices = [p for b in model.blocks for p in b.parameters() if p.dim() == 2 and muon]
+    # (a norm's weights [head, channel] are a vector for each head, no matrix)
+    matrices = [m.weight for m in model.blocks.modules() if isinstance(m, torch.nn.Linear) and muon]
     rest = [p for p in model.parameters() if not any(p is m for m in matrices)]
     optimisers = [AdamWCuda(rest, lr=lr, state_bits=state_bits, seed=seed)]
     if matrices:
