@@ -168,6 +168,10 @@ class MuonCuda(torch.optim.Optimizer):
         """Takes the state of a ``MuonCuda`` on parameters of the same types and sizes; anything else is refused with a
         ``ValueError`` and changes nothing."""
 
+        for g in state_dict["param_groups"]:
+            missing = sorted(set(self.defaults) - set(g))
+            if missing:
+                raise ValueError(f"These are not the parameter groups of a MuonCuda: {missing} are missing.")
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         kept = {}
