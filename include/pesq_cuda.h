@@ -528,7 +528,8 @@ int pesq_linear_attention_backward(const pesq_linear_attention_desc* desc, void*
  *   m = momentum m + (1 - momentum) g,  U = momentum m + (1 - momentum) g (nesterov) or m
  *   X = U / max(|U|, eps);  `steps` times  X = a X + (b A + c A A) X,  A = X X^T (on the shorter side)
  *   p = p (1 - lr weight_decay) - lr adjust X
- * over all matrices together (csrc/muon.cu).  All pointers are aligned to their types. */
+ * over all matrices together (csrc/muon.cu).  All pointers are aligned to their types;
+ * parameters, momenta and copies share no memory. */
 #define PESQ_MUON_ORIGINAL 0  /* adjust = sqrt(max(1, rows / cols)) */
 #define PESQ_MUON_MATCH_RMS 1 /* adjust = 0.2 sqrt(max(rows, cols)): the root mean square of an AdamW step */
 typedef struct pesq_muon_tensor {

@@ -37,6 +37,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <utility>
 #include <vector>
 
 #include "../../include/pesq_cuda.h"
@@ -992,6 +993,21 @@ int muon_matrices(const pesq_muon_desc* d, const pesq_muon_tensor* tensors, int6
   return PESQ_OK;
 }
 
+// Whether two of what a step writes are the same memory, or some of it: matrices are worked on at the same time
+bool overlap(const std::vector<Matrix>& all, int grad_dtype) {
+  std::vector<std::pair<const char*, const char*>> written;
+  written.reserve(3 * all.size());
+  for (const Matrix& m : all) {
+    const int64_t n = m.rows * m.cols;
+    for (const float* p : {m.param, m.momentum}) written.push_back({reinterpret_cast<const char*>(p), reinterpret_cast<const char*>(p + n)});
+    if (m.out) written.push_back({static_cast<const char*>(m.out), static_cast<const char*>(m.out) + n * (grad_dtype == PESQ_F32 ? 4 : 2)});
+  }
+  std::sort(written.begin(), written.end());
+  for (size_t i = 1; i < written.size(); ++i)
+    if (written[i].first < written[i - 1].second) return true;
+  return false;
+}
+
 int stack(const pesq_orthogonalize_desc* d, const void* x, void* out, std::vector<Matrix>& all) {
   if (!d) return set_error(PESQ_ERR_INVALID_ARGUMENT, "NULL descriptor");
   if (const int status = check_iteration(d->dtype, d->steps, d->eps, d->a, d->b, d->c)) return status;
@@ -1036,6 +1052,7 @@ int pesq_muon_step(const pesq_muon_desc* d, const pesq_muon_tensor* tensors, int
     if (const int status = muon_matrices(d, tensors, count, all)) return status;
     if (all.empty()) return (int)PESQ_OK;
     if (const int status = check_workspace(workspace, workspace_bytes, workspace_of(all))) return status;
+    if (overlap(all, d->grad_dtype)) return set_error(PESQ_ERR_INVALID_ARGUMENT, "parameters, momenta and copies must not share memory");
     Call a{};
     a.dtype = d->grad_dtype;
     a.steps = d->steps;

@@ -454,14 +454,14 @@ void muon_step(at::TensorList params, at::TensorList grads, at::TensorList momen
   check_status(pesq_muon_workspace(&d, table.data(), count, &bytes), "pesq_muon_workspace");
   if (!count) return;
   at::Tensor ws = at::empty({static_cast<int64_t>(bytes)}, first.options().dtype(at::kByte));
+  check_status(pesq_muon_step(&d, table.data(), count, at::cuda::getCurrentCUDAStream(), ws.data_ptr(), bytes),
+               "pesq_muon_step");
   for (size_t i = 0; i < params.size(); ++i) {
     if (!grads[i].defined() || grads[i].numel() == 0) continue;
     params[i].unsafeGetTensorImpl()->bump_version();
     momenta[i].unsafeGetTensorImpl()->bump_version();
     if (!copies.empty()) copies[i].unsafeGetTensorImpl()->bump_version();
   }
-  check_status(pesq_muon_step(&d, table.data(), count, at::cuda::getCurrentCUDAStream(), ws.data_ptr(), bytes),
-               "pesq_muon_step");
 }
 
 at::Tensor orthogonalize(const at::Tensor& x_, double a, double b, double c, double eps, int64_t steps) {

@@ -74,7 +74,8 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
     Parameters
     ----------
     params
-        Float32 matrices on one GPU, dense in the order of their dimensions, each given once.
+        Float32 matrices on one GPU, dense in the order of their dimensions, each given once: what is written must not
+        share memory.
     grads
         Their gradients, all float32, bfloat16 or float16 (dense, or they are
         copied).  An empty tensor leaves its matrix and momentum as they are.
