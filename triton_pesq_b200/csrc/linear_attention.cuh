@@ -35,15 +35,20 @@
 // Numbers.  All sums, the state and the decays are 32 bits; G is summed in 64 bits and kept as two floats, so that
 // differences of it are as exact as the steps' own (a reset is a step of -200 in log2, which exp2 turns to 0).
 // Products go through the matrix instructions in the operands' own type where both are inputs.  What is computed (the
-// weighted products, the state, the decayed keys) goes in as two bfloat16 terms beside bfloat16 inputs (2^-17 off),
-// as two tf32 terms (2^-22) beside float16, whose range the products and states exceed, and float32, whose inputs are also
-// two terms.  What becomes an output in 32 bits (states, decays' gradients) has a third bfloat16 term where that shows.
+// weighted products, the state, the decayed keys) goes in as terms.  Beside bfloat16: three of bfloat16, which hold all bits, for what
+// becomes an output of 32 bits (states, and the products with a state or its gradient that a decay's gradient sums), two (2^-18 off at
+// most) for what is rounded to bfloat16 itself: 1e-4 of such an output's norm is rounded the other way, 5e-5 with three terms, which
+// take 16 % more time of both directions.  Two of tf32 (2^-22) beside float16, whose range the products and states exceed, and
+// float32, whose inputs are also two terms.
 //
-// Bound.  The bytes alone would take 36 us forward and 63 backward of 896 rows of 500 steps of 64 x 64 in bfloat16, which take 139
-// to 145 and 390: neither memory (20 to 30 % of its rate) nor the matrix instructions (30 %) are full.  Shared memory's pipe is the
-// fullest (60 %), since every warp reads the chunk's operands and the state for 16 rows, and the rest is latency between
-// barriers with 12 to 16 warps an SM, whose registers are what holds the state.  Of other splits none was faster: 32 rows a warp
-// (forward 200 us, then 150), eight warps a chunk (171, then 139), a quarter more CTAs with one set of tiles.
+// Bound.  The bytes alone would take 36 us forward and 63 backward of 896 rows of 500 steps of 64 x 64 in bfloat16, which take 157
+// and 405 (all other figures of this file are of its stages, and given as shares of the time then): neither memory (20 to 30 % of its rate)
+// nor the matrix instructions (30 %) are full.  Shared memory's pipe is the fullest (60 %), since every warp reads the chunk's operands
+// and the state for 16 rows, and the rest is latency between barriers with 12 to 16 warps an SM, whose registers are what holds the state.
+// The backward is held to 128 registers by its 16 warps an SM, and spills: 504 bytes stored and 328 read a thread of 64 x 64 in
+// bfloat16, 580 and 400 in float16, 836 and 516 in float32, 1.5 to 2 KB and 0.9 to 1.5 of 128 x 128 (1 and 0.7 in float32).
+// Of other splits none was faster: 32 rows a warp (a third slower forward), eight warps a chunk (a quarter), a quarter more CTAs with one
+// set of tiles.
 #pragma once
 
 #include <type_traits>
@@ -134,6 +139,14 @@ __device__ __forceinline__ void split_bf16(float x, float y, uint32_t& hi, uint3
   const float dx = x - __uint_as_float(hi << 16), dy = y - __uint_as_float(hi & 0xffff0000u);
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(dy), "f"(dx));
 }
+// and the term that they leave: with it all bits of 32
+__device__ __forceinline__ uint32_t least_bf16(float x, float y, uint32_t hi, uint32_t lo) {
+  uint32_t least;
+  const float dx = (x - __uint_as_float(hi << 16)) - __uint_as_float(lo << 16);
+  const float dy = (y - __uint_as_float(hi & 0xffff0000u)) - __uint_as_float(lo & 0xffff0000u);
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(least) : "f"(dy), "f"(dx));
+  return least;
+}
 // a value as tf32 terms
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
@@ -194,7 +207,7 @@ struct Made<__nv_bfloat16> {
   uint32_t hi[4], lo[4];
 };
 // What goes into a state, which is an output in 32 bits: of three terms of bfloat16 (of two, 2.2e-6 of the last state are off instead of
-// 1.2e-7; 364 + 139 us and 381 + 145 of the 896 rows below)
+// 1.2e-7, in 4 % less time)
 template <class T>
 struct Finest : Made<T> {};
 template <>
@@ -207,7 +220,7 @@ struct MadeB {
 };
 template <>
 struct MadeB<__nv_bfloat16> {
-  uint32_t hi[2], lo[2];
+  uint32_t hi[2], lo[2], least[2];  // (the least where a product takes three)
 };
 
 template <class T>
@@ -227,8 +240,7 @@ __device__ __forceinline__ void make(Finest<T>& m, const float (&x)[8]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       split_bf16(x[2 * i], x[2 * i + 1], m.hi[i], m.lo[i]);
-      const float2 hi = floats_of(m.hi[i], T{}), lo = floats_of(m.lo[i], T{});
-      m.least[i] = narrow_pair((x[2 * i] - hi.x) - lo.x, (x[2 * i + 1] - hi.y) - lo.y, T{});
+      m.least[i] = least_bf16(x[2 * i], x[2 * i + 1], m.hi[i], m.lo[i]);
     }
   } else {
     make(static_cast<Made<T>&>(m), x);
@@ -308,48 +320,73 @@ __device__ __forceinline__ void load_b(InB<T> (&b)[2], const T* tile, int n0, in
   }
 }
 
-// The state as an operand: two planes of bfloat16, or 32 bits
-template <class T>
-using Stored = std::conditional_t<std::is_same<T, __nv_bfloat16>::value, __nv_bfloat16, float>;
-template <class T>
-constexpr int kPlanes = std::is_same<T, __nv_bfloat16>::value ? 2 : 1;
+// The state as an operand in shared memory: beside bfloat16 planes of its terms, two forward and three backward, whose products
+// with it go into the decays' gradients (of two, those are 1e-6 to 3e-6 off, of three 3e-7, in 4 % more time of a backward of 64 x 64); else,
+// and where three planes of two states have no room (128 x 128), 32 bits, which every warp splits that reads them (459 us with two planes,
+// 607 with 32 bits, 802 with tf32 terms, of 192 rows of 1000 steps)
+template <class T, bool kFlat>
+using Stored = std::conditional_t<std::is_same<T, __nv_bfloat16>::value && !kFlat, __nv_bfloat16, float>;
+template <class S>
+constexpr bool kInPlanes = sizeof(S) == 2;
 
-template <class T, int LD, int PLANE, bool kTrans>
-__device__ __forceinline__ void load_state(MadeB<T> (&b)[2], const Stored<T>* s, int n0, int k0) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+// kTerms: of bfloat16, two or three
+template <class T, int LD, int PLANE, bool kTrans, int kTerms, class S>
+__device__ __forceinline__ void load_state(MadeB<T> (&b)[2], const S* s, int n0, int k0) {
+  if constexpr (kInPlanes<S>) {
     uint32_t r[4];
     load_words<__nv_bfloat16, LD, kTrans>(r, s, n0, k0);
     b[0].hi[0] = r[0], b[0].hi[1] = r[1], b[1].hi[0] = r[2], b[1].hi[1] = r[3];
     load_words<__nv_bfloat16, LD, kTrans>(r, s + PLANE, n0, k0);
     b[0].lo[0] = r[0], b[0].lo[1] = r[1], b[1].lo[0] = r[2], b[1].lo[1] = r[3];
+    if constexpr (kTerms == 3) {
+      load_words<__nv_bfloat16, LD, kTrans>(r, s + 2 * PLANE, n0, k0);
+      b[0].least[0] = r[0], b[0].least[1] = r[1], b[1].least[0] = r[2], b[1].least[1] = r[3];
+    }
   } else {
     float x[8];
     load_floats<LD, kTrans>(x, s, n0, k0);
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) split_tf32(x[i], b[i >> 2].hi[i & 3], b[i >> 2].lo[i & 3]);
+      for (int i = 0; i < 4; ++i) {
+        split_bf16(x[2 * i], x[2 * i + 1], b[i >> 1].hi[i & 1], b[i >> 1].lo[i & 1]);
+        if constexpr (kTerms == 3) b[i >> 1].least[i & 1] = least_bf16(x[2 * i], x[2 * i + 1], b[i >> 1].hi[i & 1], b[i >> 1].lo[i & 1]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) split_tf32(x[i], b[i >> 2].hi[i & 3], b[i >> 2].lo[i & 3]);
+    }
   }
 }
-template <class T, int LD, int PLANE, int PLANES>
-__device__ __forceinline__ void store_state(Stored<T>* s, int row, int col, float x, float y) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+// Two or four adjacent values to planes of their terms, or as they are
+template <int LD, int PLANE, int kPlanes, class S>
+__device__ __forceinline__ void store_state(S* s, int row, int col, float x, float y) {
+  if constexpr (kInPlanes<S>) {
     uint32_t hi, lo;
     split_bf16(x, y, hi, lo);
     *reinterpret_cast<uint32_t*>(s + row * LD + col) = hi;
     *reinterpret_cast<uint32_t*>(s + PLANE + row * LD + col) = lo;
-    if constexpr (PLANES == 3) {
-      const float2 a = floats_of(hi, T{}), b = floats_of(lo, T{});
-      *reinterpret_cast<uint32_t*>(s + 2 * PLANE + row * LD + col) = narrow_pair((x - a.x) - b.x, (y - a.y) - b.y, T{});
-    }
+    if constexpr (kPlanes == 3) *reinterpret_cast<uint32_t*>(s + 2 * PLANE + row * LD + col) = least_bf16(x, y, hi, lo);
   } else {
     *reinterpret_cast<float2*>(s + row * LD + col) = make_float2(x, y);
   }
 }
-template <class T, int LD, int PLANE>
-__device__ __forceinline__ float2 read_state(const Stored<T>* s, int row, int col) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    const float2 a = floats_of(*reinterpret_cast<const uint32_t*>(s + row * LD + col), __nv_bfloat16{});
-    const float2 b = floats_of(*reinterpret_cast<const uint32_t*>(s + PLANE + row * LD + col), __nv_bfloat16{});
-    return make_float2(a.x + b.x, a.y + b.y);
+template <int PLANE>
+__device__ __forceinline__ void store_state(__nv_bfloat16* at, float4 v) {
+  uint2 hi, lo;
+  split_bf16(v.x, v.y, hi.x, lo.x);
+  split_bf16(v.z, v.w, hi.y, lo.y);
+  *reinterpret_cast<uint2*>(at) = hi;
+  *reinterpret_cast<uint2*>(at + PLANE) = lo;
+  *reinterpret_cast<uint2*>(at + 2 * PLANE) = make_uint2(least_bf16(v.x, v.y, hi.x, lo.x), least_bf16(v.z, v.w, hi.y, lo.y));
+}
+// (all bits of them: of three planes)
+template <int LD, int PLANE, class S>
+__device__ __forceinline__ float2 read_state(const S* s, int row, int col) {
+  if constexpr (kInPlanes<S>) {
+    const float2 a = floats_of(*reinterpret_cast<const uint32_t*>(s + row * LD + col), S{});
+    const float2 b = floats_of(*reinterpret_cast<const uint32_t*>(s + PLANE + row * LD + col), S{});
+    const float2 c = floats_of(*reinterpret_cast<const uint32_t*>(s + 2 * PLANE + row * LD + col), S{});
+    return make_float2(a.x + (b.x + c.x), a.y + (b.y + c.y));
   } else {
     return *reinterpret_cast<const float2*>(s + row * LD + col);
   }
@@ -405,9 +442,10 @@ __device__ __forceinline__ void mma(float (&c)[4], const Finest<T>& a, const InB
   mma(c, static_cast<const Made<T>&>(a), b);
 }
 // input times state
-template <class T>
+template <int kTerms, class T>
 __device__ __forceinline__ void mma(float (&c)[4], const InA<T>& a, const MadeB<T>& b) {
   if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    if constexpr (kTerms == 3) mma_bf16(c, a.x, b.least);
     mma_bf16(c, a.x, b.lo);
     mma_bf16(c, a.x, b.hi);
   } else if constexpr (std::is_same<T, __half>::value) {
@@ -781,14 +819,14 @@ struct State {
     }
   }
   // to shared memory, as an operand
-  template <class T, int PLANES = kPlanes<T>>
-  __device__ __forceinline__ void publish(Stored<T>* s, int rows, int cols) {
-    constexpr int LD = kLd<Stored<T>, DV>;
-    each([&](int r, int c, float& a, float& b) { store_state<T, LD, DK * LD, PLANES>(s, r, c, a, b); }, rows, cols);
+  template <int kPlanes, class S>
+  __device__ __forceinline__ void publish(S* s, int rows, int cols) {
+    constexpr int LD = kLd<S, DV>;
+    each([&](int r, int c, float& a, float& b) { store_state<LD, DK * LD, kPlanes>(s, r, c, a, b); }, rows, cols);
   }
 };
 
-// Bytes of the state before a chunk: two planes of 16 bits, or 32, of [DK][DV]
+// Bytes of the state before a chunk: 32 bits of [DK][DV]
 __host__ __device__ constexpr int64_t kept_bytes(int DK, int DV) { return (int64_t)4 * DK * DV; }
 
 __device__ __forceinline__ float2 narrow_pair(float x, float y, float) { return make_float2(x, y); }
@@ -840,8 +878,8 @@ __device__ __forceinline__ void clear(void* p, int bytes) {
 
 // Loops over the channels of a contraction.  Where a product is many instructions, code that repeats them outgrows the
 // instruction cache (two thirds of the stalls of a float32 forward)
-template <class T>
-constexpr int kUnroll = std::is_same<T, __nv_bfloat16>::value ? 4 : 1;
+template <class T, class S = T>
+constexpr int kUnroll = std::is_same<T, __nv_bfloat16>::value && kHalfWord<S> ? 4 : 1;
 
 // 16 rows of a from m0 times 16 rows of b from n0, over their channels, `width` of at most D
 template <class T, int D>
@@ -860,13 +898,13 @@ __device__ __forceinline__ void products(float (&sum)[2][4], const T* a, int m0,
 
 // 16 rows of a from m0, over their channels, `width` of at most D, times a state's columns (kTrans; else its rows), those of the
 // blocks of 16 in turn from wc that lie within `cols`
-template <class T, int D, int LDS, int PLANE, bool kTrans, int WC, int PLANES = kPlanes<T>, int N>
-__device__ __forceinline__ void times_state(float (&out)[N][4], const T* a, int m0, const Stored<T>* state, int wc, int width, int cols) {
+template <class T, int D, int LDS, int PLANE, bool kTrans, int WC, int kTerms, class S, int N>
+__device__ __forceinline__ void times_state(float (&out)[N][4], const T* a, int m0, const S* state, int wc, int width, int cols) {
 #pragma unroll
   for (int n = 0; n < N; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e) out[n][e] = 0.0f;
-#pragma unroll kUnroll<T>
+#pragma unroll (kUnroll<T, S>)
   for (int kk = 0; kk < D; kk += 16) {
     if (kk >= width) break;
     InA<T> left;
@@ -875,15 +913,9 @@ __device__ __forceinline__ void times_state(float (&out)[N][4], const T* a, int 
     for (int n = 0; n < N / 2; ++n) {
       if ((n * WC + wc) * 16 >= cols) continue;
       MadeB<T> right[2];
-      if constexpr (PLANES == 3) {
-        InB<T> least[2];
-        load_b<T, LDS, kTrans>(least, state + 2 * PLANE, (n * WC + wc) * 16, kk);
-        mma(out[2 * n], left, least[0]);
-        mma(out[2 * n + 1], left, least[1]);
-      }
-      load_state<T, LDS, PLANE, kTrans>(right, state, (n * WC + wc) * 16, kk);
-      mma(out[2 * n], left, right[0]);
-      mma(out[2 * n + 1], left, right[1]);
+      load_state<T, LDS, PLANE, kTrans, kTerms>(right, state, (n * WC + wc) * 16, kk);
+      mma<kTerms>(out[2 * n], left, right[0]);
+      mma<kTerms>(out[2 * n + 1], left, right[1]);
     }
   }
 }
@@ -924,10 +956,12 @@ __device__ __forceinline__ int sixteens(int n) { return (n + 15) & ~15; }
 template <class T, int DK, int DV, int C>
 struct ForwardShared {
   static constexpr int kTiles = (2 * C * kLd<T, DK> + C * kLd<T, DV>) * (int)sizeof(T);
-  static constexpr int kState = kPlanes<T> * DK * kLd<Stored<T>, DV> * (int)sizeof(Stored<T>);
+  using S = Stored<T, false>;
+  static constexpr int kPlanes = kInPlanes<S> ? 2 : 1;
+  static constexpr int kState = kPlanes * DK * kLd<S, DV> * (int)sizeof(S);
   static constexpr int kDecays = kDecayBytes<C>;
-  // the next chunk's tiles come in while one is worked on, where three CTAs an SM have the room (896 rows of 500 steps 159 us
-  // forward, four CTAs with one set of tiles 169; 448 rows 99 and 87)
+  // the next chunk's tiles come in while one is worked on, where three CTAs an SM have the room (of 896 rows of 500 steps
+  // four CTAs with one set of tiles are 6 % slower, of 448 rows 12 % faster)
   static constexpr int kStages = 2 * kTiles + kState + kDecays <= (75 << 10) ? 2 : 1;
   static constexpr int kBytes = kStages * kTiles + kState + kDecays;
 };
@@ -938,10 +972,10 @@ template <class T, int DK, int DV, int C, bool kWhole>
 __global__ void __launch_bounds__(128, DK > 64 ? 2 : 3) forward_kernel(const __grid_constant__ Args p) {
   constexpr int THREADS = 128, WARPS = 4, RG = C / 16, WC = WARPS / RG, NY = DV / WC / 8;
   using Sh = ForwardShared<T, DK, DV, C>;
-  constexpr int LDK = kLd<T, DK>, LDV = kLd<T, DV>, LDS = kLd<Stored<T>, DV>, PLANE = DK * LDS;
+  constexpr int LDK = kLd<T, DK>, LDV = kLd<T, DV>, LDS = kLd<typename Sh::S, DV>, PLANE = DK * LDS;
   extern __shared__ __align__(16) char shared[];
   char* tiles = shared;
-  Stored<T>* s_state = reinterpret_cast<Stored<T>*>(shared + Sh::kStages * Sh::kTiles);
+  auto* s_state = reinterpret_cast<typename Sh::S*>(shared + Sh::kStages * Sh::kTiles);
   char* decays = shared + Sh::kStages * Sh::kTiles + Sh::kState;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const int rg = warp % RG, wc = warp / RG;
@@ -958,7 +992,7 @@ __global__ void __launch_bounds__(128, DK > 64 ? 2 : 3) forward_kernel(const __g
   clear<THREADS>(shared, Sh::kStages * Sh::kTiles);
   State<DK, DV, WARPS> S;
   S.template begin<false>(p, index, part, p.state ? p.state + index * p.key * p.value : nullptr, padded, first);
-  S.template publish<T>(s_state, key, value);
+  S.template publish<Sh::kPlanes>(s_state, key, value);
   __syncthreads();
 
   const auto q_of = [&](int stage) { return reinterpret_cast<T*>(tiles + stage * Sh::kTiles); };
@@ -991,24 +1025,25 @@ __global__ void __launch_bounds__(128, DK > 64 ? 2 : 3) forward_kernel(const __g
     const float2* sums = sums_of(chunk);
     const float *before = reinterpret_cast<const float*>(sums + C), *after = before + C, *tail = after + C;
     const bool live = s0 < row.n;
-    if (live && p.kept) {
-      // the state before the chunk, for the backward: 16-byte pieces of the operand's planes
-      constexpr int kPieces = DV * (int)sizeof(Stored<T>) / 16;
-      const int piece = threadIdx.x % kPieces, apart = padded * (int)sizeof(Stored<T>);
-      char* to = static_cast<char*>(p.kept) + (index * p.chunks + chunk) * kept_bytes(DK, padded) + first * (int)sizeof(Stored<T>) + piece * 16;
-      if (piece * 16 < value * (int)sizeof(Stored<T>)) {
-#pragma unroll
-        for (int plane = 0; plane < kPlanes<T>; ++plane)
+    if (live && p.kept) {  // the state before the chunk, for the backward
+      float* to = reinterpret_cast<float*>(static_cast<char*>(p.kept) + (index * p.chunks + chunk) * kept_bytes(DK, padded)) + first;
+      if constexpr (kInPlanes<typename Sh::S>) {
+        S.each([&](int r, int col, float& a, float& b) { *reinterpret_cast<float2*>(to + (int64_t)r * padded + col) = make_float2(a, b); },
+               key, value);
+      } else {
+        constexpr int kPieces = DV / 4;
+        const int piece = threadIdx.x % kPieces * 4;
+        if (piece < value) {
 #pragma unroll 4
           for (int r = threadIdx.x / kPieces; r < key; r += THREADS / kPieces)
-            *reinterpret_cast<uint4*>(to + (int64_t)(plane * DK + r) * apart) =
-                *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(s_state + plane * PLANE + r * LDS) + piece * 16);
+            *reinterpret_cast<float4*>(to + (int64_t)r * padded + piece) = *reinterpret_cast<const float4*>(s_state + r * LDS + piece);
+        }
       }
     }
     float y[NY][4];
     if (live) {
       const int i0 = rg * 16 + g;
-      times_state<T, DK, LDS, PLANE, true, WC>(y, q, rg * 16, s_state, wc, key, value);
+      times_state<T, DK, LDS, PLANE, true, WC, 2>(y, q, rg * 16, s_state, wc, key, value);
       decay_rows(y, before[i0] * p.scale, before[i0 + 8] * p.scale);
       // sixteen steps j at a time, up to the warp's own
 #pragma unroll 1
@@ -1035,7 +1070,7 @@ __global__ void __launch_bounds__(128, DK > 64 ? 2 : 3) forward_kernel(const __g
       next.store(sums_of(chunk + 1));
     }
     __syncthreads();  // the chunk's tiles and state are read
-    if (live) S.template publish<T>(s_state, key, value);
+    if (live) S.template publish<Sh::kPlanes>(s_state, key, value);
     if (Sh::kStages == 1 && chunk + 1 < c1) load(chunk + 1, 0);
   }
   if (p.last && c1 == p.chunks) S.write(p.last + index * p.key * p.value, p.key, p.value, first);
@@ -1154,22 +1189,16 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
 template <class T, int DK, int DV>
 constexpr int kSide = DK > 64 || DV > 64 ? 8 : 4;
 
-// Planes of the state's gradient.  The decays' gradients are sums of k dS v, of which two terms of bfloat16 would leave 1.3e-6
-// (with the third 7e-7, of the states that the forward keeps in two; 364 us and 389 of 896 rows of 500 steps of 64 x 64).  128 x 128
-// have room for two
-constexpr int grad_planes(bool bf16, int dk, int dv) { return !bf16 ? 1 : dk * dv < 128 * 128 ? 3 : 2; }
-template <class T, int DK, int DV>
-constexpr int kGradPlanes = grad_planes(std::is_same<T, __nv_bfloat16>::value, DK, DV);
-
 template <class T, int DK, int DV, int C>
 struct BackwardShared {
   static constexpr int SIDE = kSide<T, DK, DV>, WC = SIDE / (C / 16);
   static constexpr int kTiles = 2 * C * (kLd<T, DK> + kLd<T, DV>) * (int)sizeof(T);
-  static constexpr int kState = kPlanes<T> * DK * kLd<Stored<T>, DV> * (int)sizeof(Stored<T>);
+  // (beside bfloat16 two states of three planes, 209 KB of 128 x 128)
+  using S = Stored<T, DK * DV == 128 * 128>;
+  static constexpr int kState = (kInPlanes<S> ? 3 : 1) * DK * kLd<S, DV> * (int)sizeof(S);
   static constexpr int kDecays = kDecayBytes<C>;
   static constexpr int kSums = ((2 * WC + C / 16 + 1) * C + SIDE) * 4;
-  static constexpr int kGrad = kState / kPlanes<T> * kGradPlanes<T, DK, DV>;
-  static constexpr int kBytes = kTiles + kState + kGrad + kDecays + kSums;
+  static constexpr int kBytes = kTiles + 2 * kState + kDecays + kSums;
 };
 
 template <class T, int DK, int DV, int C, bool kWhole>
@@ -1178,12 +1207,13 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
   using Sh = BackwardShared<T, DK, DV, C>;
   constexpr int SIDE = Sh::SIDE, WARPS = 2 * SIDE, THREADS = 32 * WARPS, RG = C / 16, WC = Sh::WC;
   constexpr int NK = DK / WC / 8, NV = DV / WC / 8;
-  constexpr int LDK = kLd<T, DK>, LDV = kLd<T, DV>, LDS = kLd<Stored<T>, DV>, PLANE = DK * LDS;
+  constexpr int LDK = kLd<T, DK>, LDV = kLd<T, DV>, LDS = kLd<typename Sh::S, DV>, PLANE = DK * LDS;
+  constexpr bool kPlanes = kInPlanes<typename Sh::S>;
   extern __shared__ __align__(16) char shared[];
   T *q = reinterpret_cast<T*>(shared), *k = q + C * LDK, *v = k + C * LDK, *dy = v + C * LDV;
-  Stored<T>* s_state = reinterpret_cast<Stored<T>*>(shared + Sh::kTiles);  // before the chunk
-  Stored<T>* s_grad = reinterpret_cast<Stored<T>*>(shared + Sh::kTiles + Sh::kState);
-  char* decays = shared + Sh::kTiles + Sh::kState + Sh::kGrad;
+  auto* s_state = reinterpret_cast<typename Sh::S*>(shared + Sh::kTiles);  // before the chunk
+  auto* s_grad = reinterpret_cast<typename Sh::S*>(shared + Sh::kTiles + Sh::kState);
+  char* decays = shared + Sh::kTiles + 2 * Sh::kState;
   float* s_far = reinterpret_cast<float*>(decays + Sh::kDecays);  // [WC][C]: scale e^{G_i} q_i S dy_i
   float* s_end = s_far + WC * C;                                  // [WC][C]: e^{G_C - G_j} k_j dS v_j
   float* s_row = s_end + WC * C;                                  // [RG][C]: sums of W over sixteen j, of each i
@@ -1204,12 +1234,15 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
   State<DK, DV, SIDE> S;  // the gradient of the state, of the warps by rows
   if (by_rows) {
     S.template begin<true>(p, index, part, p.dlast ? p.dlast + index * p.key * p.value : nullptr, DV, 0);
-    S.template publish<T, kGradPlanes<T, DK, DV>>(s_grad, key, value);
+    S.template publish<3>(s_grad, key, value);
   } else if (index >= p.whole) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
   }
   __syncthreads();
 
+  const auto kept_of = [&](int chunk) {
+    return reinterpret_cast<const float*>(static_cast<const char*>(p.kept) + (index * p.chunks + chunk) * kept_bytes(DK, DV));
+  };
   const auto load = [&](int chunk) {
     const int64_t s0 = (int64_t)chunk * C;
     if (s0 < row.n) {
@@ -1217,23 +1250,36 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
       load_tile<T, DK, C, THREADS>(k, p.k, 0, p.key, row, s0);
       load_tile<T, DV, C, THREADS>(v, p.v, 0, p.value, row, s0);
       load_tile<T, DV, C, THREADS>(dy, p.dy, 0, p.value, row, s0);
-      constexpr int kPieces = DV * (int)sizeof(Stored<T>) / 16;
-      const int piece = threadIdx.x % kPieces;
-      const char* at = static_cast<const char*>(p.kept) + (index * p.chunks + chunk) * kept_bytes(DK, DV) + piece * 16;
-      if (piece * 16 < value * (int)sizeof(Stored<T>)) {
-#pragma unroll
-        for (int plane = 0; plane < kPlanes<T>; ++plane)
+      if constexpr (!kPlanes) {
+        constexpr int kPieces = DV / 4;
+        const int piece = threadIdx.x % kPieces * 4;
+        const float* at = kept_of(chunk) + piece;
+        if (piece < value) {
 #pragma unroll 4
           for (int r = threadIdx.x / kPieces; r < key; r += THREADS / kPieces)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                             smem_of(reinterpret_cast<const char*>(s_state + plane * PLANE + r * LDS) + piece * 16)),
-                         "l"(at + (int64_t)(plane * DK + r) * (DV * (int)sizeof(Stored<T>))) : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_of(s_state + r * LDS + piece)), "l"(at + (int64_t)r * DV) : "memory");
+        }
       }
     }
     copies_issued();
   };
+  // The state before a chunk to its planes, by the warps that hold no state
+  const auto split = [&](int chunk) {
+    if constexpr (kPlanes) {
+      constexpr int kPieces = DV / 4, kRows = 32 * SIDE / kPieces;
+      static_assert(DK % kRows == 0, "");
+      if (by_rows || (int64_t)chunk * C >= row.n) return;
+      const int t = threadIdx.x - 32 * SIDE;
+      const float4* at = reinterpret_cast<const float4*>(kept_of(chunk)) + t;
+      float4 v[DK / kRows];
+#pragma unroll
+      for (int i = 0; i < DK / kRows; ++i) v[i] = at[i * 32 * SIDE];
+#pragma unroll
+      for (int i = 0; i < DK / kRows; ++i) store_state<PLANE>(s_state + (t / kPieces + i * kRows) * LDS + t % kPieces * 4, v[i]);
+    }
+  };
   // There is no room for a chunk's tiles while another's are worked on: they come as far as the L2 cache meanwhile (896 rows of 500
-  // steps of 64 x 64: bfloat16 364 us without, 356 with; float16 616 and 571)
+  // steps of 64 x 64: 2 % of bfloat16's time, 7 % of float16's)
   const auto fetch = [&](int chunk) {
     const int64_t s0 = (int64_t)chunk * C;
 #pragma unroll 1
@@ -1245,8 +1291,8 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
       for (int x = 0; x < (i < 2 * C ? p.key : p.value) * (int)sizeof(T); x += 128) prefetch(at + x);
     }
     if (s0 < row.n) {
-      const char* at = static_cast<const char*>(p.kept) + (index * p.chunks + chunk) * kept_bytes(DK, DV);
-      for (int x = threadIdx.x * 128; x < kPlanes<T> * DK * DV * (int)sizeof(Stored<T>); x += THREADS * 128) prefetch(at + x);
+      const char* at = reinterpret_cast<const char*>(kept_of(chunk));
+      for (int x = threadIdx.x * 128; x < DK * DV * 4; x += THREADS * 128) prefetch(at + x);
     }
   };
   const auto sums_of = [&](int chunk) { return reinterpret_cast<float2*>(decays + (chunk & 1) * C * 20); };
@@ -1256,6 +1302,7 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
     now = next;
   };
   load(c1 - 1);
+  split(c1 - 1);
   if (warp == WARPS - 1) {
     next.load(p, row, (int64_t)(c1 - 1) * C);
     store(c1 - 1);
@@ -1274,7 +1321,7 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
     if (by_rows) {
       float dq[NK][4];
       if (live) {
-        times_state<T, DV, LDS, PLANE, false, WC>(dq, dy, rg * 16, s_state, wc, value, key);
+        times_state<T, DV, LDS, PLANE, false, WC, 3>(dq, dy, rg * 16, s_state, wc, value, key);
         decay_rows(dq, before[i0] * p.scale, before[i0 + 8] * p.scale);
         const float2 far = row_sums<T, LDK, WC>(dq, q, i0, wc);
         if (c == 0) s_far[wc * C + i0] = far.x, s_far[wc * C + i0 + 8] = far.y;
@@ -1301,7 +1348,7 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
         // what passes the chunk whole
         float all = 0.0f;
         S.each([&](int r, int col, float& x, float& y) {
-          const float2 s = read_state<T, LDS, PLANE>(s_state, r, col);
+          const float2 s = read_state<LDS, PLANE>(s_state, r, col);
           all = fmaf(x, s.x, fmaf(y, s.y, all));
         }, key, value);
 #pragma unroll
@@ -1312,8 +1359,8 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
     } else {
       float dv[NV][4], dk[NK][4];
       if (live) {
-        times_state<T, DK, LDS, PLANE, true, WC>(dv, k, rg * 16, s_grad, wc, key, value);
-        times_state<T, DV, LDS, PLANE, false, WC, kGradPlanes<T, DK, DV>>(dk, v, rg * 16, s_grad, wc, value, key);
+        times_state<T, DK, LDS, PLANE, true, WC, 2>(dv, k, rg * 16, s_grad, wc, key, value);
+        times_state<T, DV, LDS, PLANE, false, WC, 3>(dk, v, rg * 16, s_grad, wc, value, key);
         decay_rows(dv, after[i0], after[i0 + 8]);
         decay_rows(dk, after[i0], after[i0 + 8]);
         const float2 end = row_sums<T, LDK, WC>(dk, k, i0, wc);
@@ -1377,8 +1424,8 @@ __global__ void __launch_bounds__(64 * kSide<T, DK, DV>, kSide<T, DK, DV> == 4 ?
       store_rows<T, WC>(p.dk, p, row, s0 + i0, p.key, wc * 16 + 2 * c, dk);
     }
     __syncthreads();  // the chunk's tiles, states and sums are read or written
-    if (chunk > c0) load(chunk - 1);
-    if (by_rows && live) S.template publish<T, kGradPlanes<T, DK, DV>>(s_grad, key, value);
+    if (chunk > c0) load(chunk - 1), split(chunk - 1);
+    if (by_rows && live) S.template publish<3>(s_grad, key, value);
     if (warp == WARPS - 1) {
       // the decays' gradients: prefix sums over the chunk's steps in 64 bits
       constexpr int E = C / 32;

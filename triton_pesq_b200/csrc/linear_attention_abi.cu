@@ -76,13 +76,12 @@ size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 // CTAs of a kernel that an SM holds: what their shared memory leaves, and their registers
 int resident(int dtype, const Geometry& g, bool backward) {
   const int size = (int)element(dtype), pad = size == 2 ? 8 : 4;
-  const int state = dtype == PESQ_BF16 ? 2 * g.dk * (g.dv + 8) * 2 : g.dk * (g.dv + 4) * 4, sums = 60 * g.chunk;
+  const bool planes = dtype == PESQ_BF16 && !(backward && g.dk * g.dv == 128 * 128);
+  const int state = planes ? (backward ? 3 : 2) * g.dk * (g.dv + 8) * 2 : g.dk * (g.dv + 4) * 4, sums = 60 * g.chunk;
   const int wide = g.dk > 64 || (backward && g.dv > 64);
   int bytes;
   if (backward) {
-    const bool bf16 = dtype == PESQ_BF16;
-    const int grad = state / (bf16 ? 2 : 1) * grad_planes(bf16, g.dk, g.dv);
-    bytes = 2 * g.chunk * (g.dk + g.dv + 2 * pad) * size + state + grad + sums;
+    bytes = 2 * g.chunk * (g.dk + g.dv + 2 * pad) * size + 2 * state + sums;
   } else {
     const int tiles = g.chunk * (2 * g.dk + g.dv + 3 * pad) * size;
     bytes = (2 * tiles + state + 40 * g.chunk <= 75 << 10 ? 2 : 1) * tiles + state + 40 * g.chunk;
@@ -94,7 +93,7 @@ int resident(int dtype, const Geometry& g, bool backward) {
 // and twice backward: the parts' sweep and join take about 0.6 of a forward's time and 0.3 of a backward's, and some
 // 10 us (12 x 8 rows of 500 steps of 64 x 64 in bfloat16: one part 43 us, four 42; 128 rows: 43 and three 58; 16: 41 and eight 24).
 // Rows beyond full rounds of the device are cut by the same rule, and the others walked whole beside them (896 rows are six a SM
-// and eight more, bfloat16: 150 us forward and 390 backward with a round of their own, 139 and 364 cut).
+// and eight more, bfloat16: a round of their own takes 8 % longer forward and 7 % backward than cut).
 // Rows of different lengths are cut four times as often, since parts past a row's end leave their place to others (30
 // rows of up to 4001 steps of 96 x 128 in float16, trained: parts for one filling 953 us, for four 594).
 Plan plan(const pesq_linear_attention_desc& d, bool backward) {
