@@ -2,7 +2,8 @@
 
 Bounds.  The states' own roundings, which decay with them, are some ten of random sign: sqrt(10) * 2^-23.  A decay's gradient
 beside 16 bits sums products over up to 128 channels, whose instruction cuts off what its accumulator does not hold: at most
-24 times (eight steps of three terms, 16 of two) half of 2^-24 of the sum on average."""
+24 times (eight steps of three terms, 16 of two) half of 2^-24 of the sum on average.  Of float32 a product leaves out the product of two lower
+terms, 2^-22 at most, and its sums are rounded: with the states' roundings 2^-22 more."""
 
 import pytest
 import torch
@@ -44,6 +45,16 @@ def test_gradients_of_decays_beside_16_bits(cuda_device, dtype, shape):
             assert far(a, e) <= STATES + 24 * 2.0**-25, far(a, e)
         elif a.dtype == F32:
             assert far(a, e) <= STATES, (name, far(a, e))
+
+
+@pytest.mark.parametrize("shape", [(3, 5, 6, 18, 9), (3, 300, 4, 64, 64), (2, 300, 4, 100, 64), (2, 300, 4, 64, 128), (2, 300, 4, 128, 128),
+                                   (1, 888, 13, 115, 110), (8, 500, 12, 64, 64)])
+@pytest.mark.parametrize("reset", [False, True])
+def test_float32(cuda_device, shape, reset):
+    for decays in (0.2, 0.02):
+        names, got, want = both(shape, F32, cuda_device, 32, reset=reset, decays=decays)
+        for name, a, e in zip(names, got, want):
+            assert far(a, e) <= STATES + 2.0**-22, (name, far(a, e))
 
 
 def test_steps_without_a_backward(cuda_device):

@@ -39,14 +39,14 @@
 // becomes an output of 32 bits (states, and the products with a state or its gradient that a decay's gradient sums), two (2^-18 off at
 // most) for what is rounded to bfloat16 itself: 1e-4 of such an output's norm is rounded the other way, 5e-5 with three terms, which
 // take 16 % more time of both directions.  Two of tf32 (2^-22) beside float16, whose range the products and states exceed, and
-// float32, whose inputs are also two terms.
+// float32, whose inputs are also two terms, and whose sums are made apart and added rounded.
 //
 // Bound.  The bytes alone would take 36 us forward and 63 backward of 896 rows of 500 steps of 64 x 64 in bfloat16, which take 157
 // and 405 (all other figures of this file are of its stages, and given as shares of the time then): neither memory (20 to 30 % of its rate)
 // nor the matrix instructions (30 %) are full.  Shared memory's pipe is the fullest (60 %), since every warp reads the chunk's operands
 // and the state for 16 rows, and the rest is latency between barriers with 12 to 16 warps an SM, whose registers are what holds the state.
 // The backward is held to 128 registers by its 16 warps an SM, and spills: 504 bytes stored and 328 read a thread of 64 x 64 in
-// bfloat16, 580 and 400 in float16, 836 and 516 in float32, 1.5 to 2 KB and 0.9 to 1.5 of 128 x 128 (1 and 0.7 in float32).
+// bfloat16, 580 and 400 in float16, 1012 and 628 in float32, 1.5 to 2 KB and 0.9 to 1.5 of 128 x 128 (1 and 0.7 in float32).
 // Of other splits none was faster: 32 rows a warp (a third slower forward), eight warps a chunk (a quarter), a quarter more CTAs with one
 // set of tiles.
 #pragma once
@@ -131,6 +131,18 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[8], 
     asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[4 * s]), "r"(a[4 * s + 2]), "r"(a[4 * s + 1]), "r"(a[4 * s + 3]), "r"(b[2 * s]), "r"(b[2 * s + 1]));
+}
+
+// Both of two tf32 terms, as a sum of its own that is added rounded: the instruction cuts off what its accumulator does not hold
+// (over 128 columns 1.2e-6 of a float32 result, 3e-7 so)
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&ahi)[8], const uint32_t (&alo)[8], const uint32_t (&bhi)[4],
+                                         const uint32_t (&blo)[4]) {
+  float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  mma_tf32(t, alo, bhi);
+  mma_tf32(t, ahi, blo);
+  mma_tf32(t, ahi, bhi);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c[e] += t[e];
 }
 
 // two values as bfloat16 terms hi + lo
@@ -410,9 +422,7 @@ __device__ __forceinline__ void mma(float (&c)[4], const InA<T>& a, const InB<T>
   } else if constexpr (std::is_same<T, __half>::value) {
     mma_f16(c, a.x, b.x);
   } else {
-    mma_tf32(c, a.lo, b.hi);
-    mma_tf32(c, a.hi, b.lo);
-    mma_tf32(c, a.hi, b.hi);
+    mma_tf32(c, a.hi, a.lo, b.hi, b.lo);
   }
 }
 // computed times input
@@ -431,9 +441,7 @@ __device__ __forceinline__ void mma(float (&c)[4], const Made<T>& a, const InB<T
     mma_tf32(c, a.lo, w);
     mma_tf32(c, a.hi, w);
   } else {
-    mma_tf32(c, a.lo, b.hi);
-    mma_tf32(c, a.hi, b.lo);
-    mma_tf32(c, a.hi, b.hi);
+    mma_tf32(c, a.hi, a.lo, b.hi, b.lo);
   }
 }
 template <class T>
@@ -454,9 +462,7 @@ __device__ __forceinline__ void mma(float (&c)[4], const InA<T>& a, const MadeB<
     mma_tf32(c, w, b.lo);
     mma_tf32(c, w, b.hi);
   } else {
-    mma_tf32(c, a.lo, b.hi);
-    mma_tf32(c, a.hi, b.lo);
-    mma_tf32(c, a.hi, b.hi);
+    mma_tf32(c, a.hi, a.lo, b.hi, b.lo);
   }
 }
 
