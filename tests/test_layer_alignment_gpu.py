@@ -96,7 +96,7 @@ def test_layer_norm(cuda_device, dtype, out, width):
     _lib.check(lib.pesq_layer_norm_backward(ctypes.byref(d), ctypes.c_void_p(stream), heads(dy), dx, dweight, dbias,
                                             ctypes.c_void_p(work.data_ptr()), work.numel()), "backward")
     for (room, got), e in rooms:
-        allowed = torch.finfo(e.dtype).eps * e.abs().double() + 10 * 2.0**-24 * float(e.abs().max()) * (12 if e.dim() == 1 else 4)
+        allowed = torch.finfo(e.dtype).eps * e.abs().double() + 10 * 2.0**-24 * float(e.detach().abs().max()) * (12 if e.dim() == 1 else 4)
         assert bool(((got.double() - e.double()).abs() <= allowed).all()) and untouched(room, 1, got.numel())
 
 

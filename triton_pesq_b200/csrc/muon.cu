@@ -12,9 +12,9 @@
 // accumulator.  Values are kept times 2^10: elements of X and A are at most about 1.2, those of the polynomial about 8, for the
 // usual coefficients, far from float16's largest, and the lo term of an element of 2^-10 still has its bits.
 // The accumulator of the instruction cuts off what it does not hold instead of rounding it, which adds up over a long
-// contraction (2.3e-5 of the result of a 385 x 1155 matrix, 5.0e-5 of 1280 x 3840).  So it sums 64 columns alone, and the
-// warps that read it add those sums in registers, rounded (2.5e-6 and 1.5e-6; with 128 columns 4.3e-6 and 2.8e-6 in 4 % less time;
-// float32 products 2.8e-6 and 3.6e-6).
+// contraction (2.3e-5 of the result of a 385 x 1155 matrix, 5.0e-5 of 1280 x 3840).  So it sums 64 columns alone (of narrow matrices
+// 32 or 16), and the warps that read it add those sums in registers, rounded (2.5e-6 and 1.5e-6; with 128 columns 4.3e-6 and 2.8e-6 in
+// 4 % less time, with 32 1.6e-6 of 385 x 1155 in 20 % more; float32 products 2.8e-6 and 3.6e-6).
 //
 // Products run on tcgen05 with the accumulator in tensor memory, in tiles of 128 x 128.  Matrices lie in the workspace as the
 // tiles that the instruction reads from shared memory: 128 rows of 64 columns in the 128-byte swizzle, hi and lo
@@ -60,7 +60,6 @@ constexpr int kStages = 3, kStage = 2 * kPair;        // both operands
 constexpr int kReaders = 16;                          // warps of results: four for each quarter of the columns
 constexpr int kThreads = 64 + 32 * kReaders;          // copies, products, results
 constexpr int kShared = kStages * kStage + 1024;      // (aligned to 1024 in the kernel)
-constexpr int kSegment = 1;                           // stages whose products are summed in tensor memory
 constexpr float kScale = 1024.0f;                     // of what is kept
 constexpr int kMost = 32768;                          // rows or columns
 constexpr int kItems = 128;                           // matrices of a launch
@@ -430,16 +429,17 @@ __device__ __forceinline__ void finish(const Call& p, int mode, int from, const 
   }
 }
 
-// The three products of a step, 16 columns of the contraction after the other
-__device__ __forceinline__ void products_of(uint32_t to, uint32_t a, uint32_t b, bool transposed, bool add) {
+// The three products of kCount sixteens of a stage's columns from `first`, to a sum of their own
+template <int kCount>
+__device__ __forceinline__ void products_of(uint32_t to, uint32_t a, uint32_t b, bool transposed, int first) {
   const uint32_t instruction = kInstruction | (transposed ? kTransposedB : 0);
   // (the lower terms first: what the accumulator cuts off is a share of what it holds)
 #pragma unroll
   for (int pair = 0; pair < 3; ++pair) {
 #pragma unroll
-    for (int s = 0; s < kDepth / 16; ++s) {
-      const uint32_t as = a + s * 32 + (pair == 0 ? kPlane : 0), bs = b + s * (transposed ? 2048 : 32) + (pair == 1 ? kPlane : 0);
-      product(to, descriptor(as, false), descriptor(bs, transposed), instruction, add || pair > 0 || s > 0);
+    for (int s = 0; s < kCount; ++s) {
+      const uint32_t as = a + (first + s) * 32 + (pair == 0 ? kPlane : 0), bs = b + (first + s) * (transposed ? 2048 : 32) + (pair == 1 ? kPlane : 0);
+      product(to, descriptor(as, false), descriptor(bs, transposed), instruction, pair > 0 || s > 0);
     }
   }
 }
@@ -548,20 +548,18 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
           const Tile tile(p, mode, t);
           const bool same = mode == kGram && tile.i == tile.j;
           for (int k = 0; k < tile.depth; ++k) {
-            if (k % kSegment == 0 && !mbar_wait(spent + half, half_parity) || !mbar_wait(full + stage, parity)) {
+            if (!mbar_wait(spent + half, half_parity) || !mbar_wait(full + stage, parity)) {
               good = false;
               break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t a = smem_u32(tiles + stage * kStage);
-            products_of(tmem + half * kTile, a, same ? a : a + kPair, wide, k % kSegment > 0);
+            products_of<kDepth / 16>(tmem + half * kTile, a, same ? a : a + kPair, wide, 0);
             commit(empty + stage);
+            commit(ready + half);
+            half ^= 1;
+            if (half == 0) half_parity ^= 1;
             if (++stage == kStages) stage = 0, parity ^= 1;
-            if ((k + 1) % kSegment == 0 || k + 1 == tile.depth) {
-              commit(ready + half);
-              half ^= 1;
-              if (half == 0) half_parity ^= 1;
-            }
           }
         }
         if (!good) {  // (what is issued ends before its memory goes)
@@ -578,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
         float acc[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) acc[e] = 0.0f;
-        for (int k = 0; k < tile.depth; k += kSegment) {
+        for (int k = 0; k < tile.depth; ++k) {
           good = __all_sync(0xffffffffu, mbar_wait(ready + half, half_parity));
           if (!good) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -626,6 +624,14 @@ __device__ __forceinline__ void put_shared(char* square, int row, int col, const
   *reinterpret_cast<Eight*>(to) = hi;
   *reinterpret_cast<Eight*>(to + kPlane) = lo;
 }
+
+// Sixteens of columns that a narrow matrix' products sum in tensor memory.  What the accumulator cuts off is of the sum's sign, and the
+// fewer rows there are, the less of it averages out.  With a stage's four 37 x 225 is 3.4e-6 off (float32 products 1.6e-6), 52 x 725 3.5e-6
+// (2.0e-6), 70 x 506 2.8e-6 (1.6e-6), 96 x 288 1.7e-6 (1.5e-6); with two 2.8e-6, 2.3e-6, 1.8e-6 and 1.1e-6, with one 2.0e-6, 1.7e-6, 1.3e-6
+// and 8e-7.  A small model's step (96 wide) takes 116 us with four, 124 with two, 146 with one.
+__device__ __forceinline__ int narrow_sum(const Item& it) { return it.n <= kDepth ? 1 : 2; }
+// Such sums of a contraction over `width` columns: those past the edge are zeros, and not worked on
+__device__ __forceinline__ int sums_of(int width, int each) { return (width + 16 * each - 1) / (16 * each); }
 
 template <int N>
 __global__ void __launch_bounds__(kThreads, 1) narrow_kernel(const __grid_constant__ Args<N> p) {
@@ -699,31 +705,32 @@ __global__ void __launch_bounds__(kThreads, 1) narrow_kernel(const __grid_consta
         const uint32_t square = smem_u32(squares);
         for (int t = blockIdx.x; t < p.wides && good; t += gridDim.x) {
           const Tile tile(p, kUpdate, t);
-          const int gram = (p.item[tile.index].m + kDepth - 1) / kDepth;
+          const Item& it = p.item[tile.index];
+          const int each = narrow_sum(it), stage_sums = kDepth / 16 / each;
           // A: X X^T, then the polynomial: A (b + c A), then X': the polynomial times X
           for (int part = 0; part < 3 && good; ++part) {
-            const int depth = part == 0 ? gram : tile.depth;
+            const int sums = sums_of(part == 0 ? it.m : it.n, each);
             if (part > 0) {
               good = mbar_wait(&made, made_parity);
               made_parity ^= 1;
             }
-            for (int k = 0; k < depth && good; ++k) {
-              if (k % kSegment == 0) good = mbar_wait(spent + half, half_parity);
-              if (part != 1) good = good && mbar_wait(full + stage, parity);
+            for (int c = 0; c < sums && good; ++c) {
+              const int k = c / stage_sums, first = c % stage_sums * each;
+              if (part != 1 && first == 0) good = mbar_wait(full + stage, parity);
+              good = good && mbar_wait(spent + half, half_parity);
               if (!good) break;
               asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
               const uint32_t own = smem_u32(ring + stage * kPair);
-              products_of(tmem + half * kTile, part == 0 ? own : square + k * kPair, part == 1 ? square + (2 + k) * kPair : own,
-                          part == 2, k % kSegment > 0);
-              if (part != 1) {
+              const uint32_t to = tmem + half * kTile, a = part == 0 ? own : square + k * kPair, b = part == 1 ? square + (2 + k) * kPair : own;
+              if (each == 1) products_of<1>(to, a, b, part == 2, first);
+              else products_of<2>(to, a, b, part == 2, first);
+              if (part != 1 && ((c + 1) % stage_sums == 0 || c + 1 == sums)) {
                 commit(empty + stage);
                 if (++stage == kNarrowStages) stage = 0, parity ^= 1;
               }
-              if ((k + 1) % kSegment == 0 || k + 1 == depth) {
-                commit(ready + half);
-                half ^= 1;
-                if (half == 0) half_parity ^= 1;
-              }
+              commit(ready + half);
+              half ^= 1;
+              if (half == 0) half_parity ^= 1;
             }
           }
         }
@@ -739,14 +746,13 @@ __global__ void __launch_bounds__(kThreads, 1) narrow_kernel(const __grid_consta
       for (int t = blockIdx.x; t < p.wides && good; t += gridDim.x) {
         const Tile tile(p, kUpdate, t);
         const Item& it = p.item[tile.index];
-        const int gram = (it.m + kDepth - 1) / kDepth;
 #pragma unroll 1
         for (int part = 0; part < 3 && good; ++part) {
-          const int depth = part == 0 ? gram : tile.depth;
+          const int sums = sums_of(part == 0 ? it.m : it.n, narrow_sum(it));
           float acc[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) acc[e] = 0.0f;
-          for (int k = 0; k < depth; k += kSegment) {
+          for (int c = 0; c < sums; ++c) {
             good = __all_sync(0xffffffffu, mbar_wait(ready + half, half_parity));
             if (!good) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
