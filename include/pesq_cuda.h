@@ -480,7 +480,8 @@ typedef struct pesq_layer_norm_desc {
   const float *weight, *bias; /* [heads, width]; bias NULL: zeros */
 } pesq_layer_norm_desc;
 
-/* y: [batch, steps, heads, width] dense.  All operands are aligned to their types. */
+/* y: [batch, steps, heads, width] dense.  All operands are aligned to their types; results
+ * share no memory with them. */
 int pesq_layer_norm_forward(const pesq_layer_norm_desc* desc, void* stream, void* y);
 /* Bytes of a backward's workspace. */
 int pesq_layer_norm_workspace(const pesq_layer_norm_desc* desc, size_t* bytes);
@@ -513,7 +514,7 @@ typedef struct pesq_linear_attention_desc {
 int pesq_linear_attention_sizes(const pesq_linear_attention_desc* desc, size_t* forward, size_t* kept, size_t* backward);
 /* y: [batch, steps, heads, value] dense; last: [batch, heads, key, value], the
  * state after the last step, or NULL; kept: for the backward call, or NULL.
- * Operands are aligned to their types; y to two elements where `value` is even, and
+ * Results share no memory with operands.  Operands are aligned to their types; y to two elements where `value` is even, and
  * so are the backward's dq and dk where `key` is, dv where `value` is. */
 int pesq_linear_attention_forward(const pesq_linear_attention_desc* desc, void* stream, void* y, float* last, void* kept,
                                   size_t kept_bytes, void* workspace, size_t workspace_bytes);

@@ -28,9 +28,10 @@
 // empty the accumulators, of which there are two, so that a tile's end overlaps the next one's products (each a quarter of
 // the columns: four warps with all of them took twice as long over a small model's tiles).  All products of
 // a call are one cooperative launch, whose CTAs wait for one another between the products of a step (15 launches of a
-// small model's step took 230 us of the host's time).  The bound is what a stage's products need brought in, 64 KB for 3 x 2.1 MFLOP:
-// 4096 x 4096 alone runs at 990 TFLOP/s of the three products, 10 TB/s out of the L2 cache; pairs of CTAs on 256 x 256, with half of that, at
-// 1030, but slower in all of a model's sizes (3.08 ms for 2.53).  All waits are
+// small model's step took 230 us of the host's time).  The bound is what a product's operands take: 128 x 128 x 16
+// reads 8 KB of shared memory in its 64 cycles, all that it gives, while 64 KB are copied in for a stage's 3 x 2.1 MFLOP beside.
+// 4096 x 4096 alone runs at 990 TFLOP/s of the three products, 10 TB/s out of the L2 cache; pairs of CTAs on 256 x 256, with half of those
+// copies, at 1030, but slower in all of a model's sizes (3.08 ms for 2.53).  All waits are
 // bounded; one that runs out sets an error word and the CTA returns.
 #include <cuda_runtime.h>
 

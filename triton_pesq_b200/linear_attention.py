@@ -9,8 +9,10 @@ Per row and head, in scan order::
 Sequences run in chunks of 64 steps on the tensor cores, and in parts that are
 joined where rows are few; a call of a few steps with ``state`` is the streaming form
 (csrc/linear_attention.cuh).  The state, the decays and every sum are float32
-whatever the streams' type, and a result is the same, to the last bit, every
-time.  The reference has no counterpart (its networks are its users').
+whatever the streams' type.  Products take what was computed as terms: all
+bits of it where the result is float32 beside bfloat16, 2^-18 of it left out where the
+result is rounded to bfloat16 itself, 2^-22 beside float16 and float32.  A result is the same,
+to the last bit, every time.  The reference has no counterpart (its networks are its users').
 """
 
 from __future__ import annotations
