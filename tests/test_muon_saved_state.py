@@ -33,3 +33,15 @@ def test_groups_come_back_with_what_schedulers_add():
     assert snapshot(new) == snapshot(opt) and new.param_groups[0]["initial_lr"] == 0.5
     with pytest.raises(ValueError):
         new.load_state_dict(MuonCuda(params).state_dict())
+
+
+def test_a_state_is_taken_as_often_as_it_is_given():
+    """By an optimiser that has loaded one before, and by copies of one, whose defaults the base class adds to."""
+
+    params = [torch.nn.Parameter(torch.ones(4, 4))]
+    opt, fresh = MuonCuda(params, lr=0.5), MuonCuda(params).state_dict()
+    for _ in range(2):
+        opt.load_state_dict(fresh)
+        twin = copy.deepcopy(opt)
+        twin.load_state_dict(fresh)
+    assert twin.param_groups[0]["lr"] == opt.param_groups[0]["lr"] == 1e-3

@@ -26,6 +26,8 @@ __all__ = ["orthogonalize", "muon_step", "MuonCuda", "COEFFICIENTS"]
 #: of the usual five steps, which bring singular values from 0.01 on to between 0.7 and 1.2
 COEFFICIENTS = (3.4445, -4.775, 2.0315)
 ADJUSTMENTS = ("original", "match_rms_adamw")
+#: of a parameter group
+HYPERPARAMETERS = frozenset(("lr", "momentum", "nesterov", "weight_decay", "coefficients", "eps", "steps", "adjust"))
 
 _ops = None
 
@@ -170,7 +172,7 @@ class MuonCuda(torch.optim.Optimizer):
         ``ValueError`` and changes nothing."""
 
         for g in state_dict["param_groups"]:
-            missing = sorted(set(self.defaults) - set(g))
+            missing = sorted(HYPERPARAMETERS - set(g))
             if missing:
                 raise ValueError(f"These are not the parameter groups of a MuonCuda: {missing} are missing.")
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
@@ -214,8 +216,7 @@ class MuonCuda(torch.optim.Optimizer):
                 masters = dtype != torch.float32
                 muon_step([s["master"] for s in states] if masters else params, [p.grad for p in params],
                           [s["momentum"] for s in states], copies=params if masters else None,
-                          **{k: group[k] for k in ("lr", "momentum", "nesterov", "weight_decay", "coefficients", "eps", "steps",
-                                                   "adjust")}, grad_scale=grad_scale)
+                          **{k: group[k] for k in HYPERPARAMETERS}, grad_scale=grad_scale)
         return loss
 
     def check_errors(self) -> int:
