@@ -36,7 +36,8 @@ cudaError_t launch_forward(const Args& p, const Geometry& g, Kind kind, cudaStre
 }
 
 // Whether the padding is worked on too: where the widths fill it, and of bfloat16, whose instructions are too few for its
-// tests to pay (a forward of 40 x 512 x 16 rows' steps of 12 x 20: 70 us with the padding, 74 without; float32 150 and 115)
+// tests to pay (a forward of 40 x 512 x 16 rows' steps of 12 x 20: 70 us with the padding, 74 without; float32 150 and 115.  Of backwards
+// padded to 128 x 128 it depends: 192 rows of 1000 steps of 72 x 72 take 599 and 522, of 100 x 100 612 and 719)
 template <class T>
 constexpr bool kAlwaysWhole = std::is_same<T, __nv_bfloat16>::value;
 
