@@ -103,3 +103,21 @@ def test_gradients_of_decays_by_their_norm(cuda_device, dtype, shape):
     off = float((got - want).norm() / want.norm())
     term = 2.0**-18 if dtype == BF16 else 3 * 2.0**-22 + 10**0.5 * 2.0**-23
     assert off <= 3**0.5 * term, off
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("shape", [(2, 150, 3, 32, 32), (2, 150, 3, 128, 128), (1, 1500, 2, 64, 48)])
+def test_gradients_behind_a_reset_see_nothing_of_the_state(cuda_device, dtype, shape):
+    """A state that is not a number, of rows that forget it at their first step: every gradient is what it is without."""
+
+    (q, k, v, decay, state), dy, dlast, kw = make(*shape, dtype, gated=True, seed=25)
+    reset = torch.zeros(shape[:2], dtype=torch.bool, device=cuda_device)
+    reset[:, 0] = True
+    outs = []
+    for s in (torch.full_like(state, float("nan")), torch.zeros_like(state)):
+        leaves = [t.to(cuda_device).requires_grad_(True) for t in (q, k, v, decay, s)]
+        out = linear_attention(*leaves, reset=reset, **kw)
+        outs.append([*(t.detach() for t in out), *torch.autograd.grad(out, leaves, (dy.to(cuda_device), dlast.to(cuda_device)))])
+    for a, e in zip(*outs):
+        assert torch.isfinite(e).all() and torch.equal(a, e)
+    assert not outs[0][-1].any()
